@@ -85,6 +85,17 @@ SIGNATURES = {
     "bbcu_fp32_DifferentiableLut6_BackwardStatsFromOutput": (_i, [_vp] * 4 + [_f] * 2 + [_i] * 4 + [_vp]),
     "bbcu_fp32_DifferentiableLut6_BackwardFromOutput": (_i, [_vp] * 11 + [_f] * 2 + [_i] * 5 + [_vp]),
     "bbcu_fp32_DifferentiableLut6_BackwardApply": (_i, [_vp] * 11 + [_f] * 3 + [_i] * 4 + [_ll, _i, _i, _vp]),
+    "bbcu_fp32_LayerNormalization_Forward": (_i, [_vp] * 6 + [_f] + [_i] * 4 + [_vp]),
+    "bbcu_bf16_LayerNormalization_Forward": (_i, [_vp] * 6 + [_f] + [_i] * 4 + [_vp]),
+    "bbcu_fp32_LayerNormalization_Backward": (_i, [_vp] * 8 + [_i] * 6 + [_vp]),
+    "bbcu_bf16_LayerNormalization_Backward": (_i, [_vp] * 8 + [_i] * 6 + [_vp]),
+    "bbcu_fp32_QuantizeInt8_Frames": (_i, [_vp] * 3 + [_i] * 4 + [_vp]),
+    "bbcu_bf16_QuantizeInt8_Frames": (_i, [_vp] * 3 + [_i] * 4 + [_vp]),
+    "bbcu_fp32_QuantizeInt8_Channels": (_i, [_vp] * 3 + [_i] * 4 + [_vp]),
+    "bbcu_int8_fp32_DenseAffine_Forward": (_i, [_vp] * 6 + [_i] * 6 + [_vp]),
+    "bbcu_int8_bf16_DenseAffine_Forward": (_i, [_vp] * 6 + [_i] * 6 + [_vp]),
+    "bbcu_fp32_LossDistillation": (_i, [_vp] * 8 + [_f] * 2 + [C.c_double] + [_i] * 7 + [_vp]),
+    "bbcu_bf16_LossDistillation": (_i, [_vp] * 8 + [_f] * 2 + [C.c_double] + [_i] * 7 + [_vp]),
 }
 
 

@@ -32,8 +32,9 @@ const DeviceInfo &device_info();
 // makes back-to-back calls on one stream safe; different streams get different blocks.  A stream has
 // kScratchSlots independent blocks, for callers whose scratch is alive at the same time (slot 0: batch-norm
 // sums, slot 1: per-node coefficient / pattern tables of the LUT operators, slot 2: the piece table of the bit Im2Col,
-// slot 3: fp32 rows packed to bits).
-constexpr int kScratchSlots = 5;
+// slot 3: fp32 rows packed to bits, slot 4: the counters below, slot 5: partial sums of the operators over the nodes of a frame).
+constexpr int kScratchSlots = 6;
+constexpr int kFrameOpSlot = 5;
 void *stream_scratch(cudaStream_t stream, size_t bytes, int slot = 0);
 
 // A number that is another one after every request for the stream's block (0: it has none).  A caller that leaves something in the block for

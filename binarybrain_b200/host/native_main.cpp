@@ -166,7 +166,11 @@ PyObject *scalar_f64(PyObject *, PyObject *const *o, Py_ssize_t n) { return empt
     X(bbcu_fp32_Reduce_Forward) X(bbcu_fp32_Reduce_Backward) X(bbcu_bit_fp32_RealToBinary_Forward) X(bbcu_bit_fp32_BinaryToReal_Forward)      \
     X(bbcu_fp32_BinaryToReal_Forward) X(bbcu_fp32_BinaryToReal_Backward) X(bbcu_fp32_Im2Col_Forward) X(bbcu_bit_Im2Col_Forward)               \
     X(bbcu_fp32_Im2Col_Backward) X(bbcu_fp32_Col2Im_Forward) X(bbcu_bit_Col2Im_Forward) X(bbcu_fp32_Col2Im_Backward)                          \
-    X(bbcu_fp32_MaxPooling_Forward) X(bbcu_bit_MaxPooling_Forward) X(bbcu_fp32_MaxPooling_Backward) X(bbcu_bit_fp32_MaxPooling_Backward)
+    X(bbcu_fp32_MaxPooling_Forward) X(bbcu_bit_MaxPooling_Forward) X(bbcu_fp32_MaxPooling_Backward) X(bbcu_bit_fp32_MaxPooling_Backward)     \
+    X(bbcu_fp32_LayerNormalization_Forward) X(bbcu_bf16_LayerNormalization_Forward) X(bbcu_fp32_LayerNormalization_Backward)                  \
+    X(bbcu_bf16_LayerNormalization_Backward) X(bbcu_fp32_QuantizeInt8_Frames) X(bbcu_bf16_QuantizeInt8_Frames)                                \
+    X(bbcu_fp32_QuantizeInt8_Channels) X(bbcu_int8_fp32_DenseAffine_Forward) X(bbcu_int8_bf16_DenseAffine_Forward)                            \
+    X(bbcu_fp32_LossDistillation) X(bbcu_bf16_LossDistillation)
 
 #define BB200_DEFINE(name)                                                          \
     PyObject *py_##name(PyObject *, PyObject *const *o, Py_ssize_t n)               \

@@ -47,6 +47,7 @@ extern "C" {
 #endif
 
 typedef void *bbcu_stream_t;
+typedef unsigned short bbcu_bf16_t;     /* the upper half of an fp32 number */
 
 #define BBCU_OK                 0
 #define BBCU_ERR_NULL_POINTER  (-1)
@@ -371,6 +372,66 @@ int bbcu_fp32_DifferentiableLut6_ForwardTraining_NoAlloc(const float *dev_x_buf,
                                                          float unbinarize_bias, int node_size, int frame_size, int frame_stride,
                                                          int lut_binarize, int binary_mode, bbcu_stream_t stream);
 int bbcu_fp32_DifferentiableLut6_ForwardTraining_NoAlloc_MaxNodes(void);
+
+/* ------------------------------------------------------------------ Additive: the dense teacher beside a LUT network.
+ * No counterparts in the reference.  Frame buffers are node-major as above, fp32 or bf16 (bbcu_bf16_*: two bytes an element, strides in elements);
+ * any stride and alignment of theirs is taken, rows on 16-byte boundaries are the fast ones, and outputs are written up to the last frame, never
+ * into a row's padding.  Outputs do not overlap inputs.  Sums and statistics are 32 bits or more; bf16 results are rounded once.  A batch without
+ * frames is no error.  Scratch as for the LUT operators above: the first call of a size on a stream allocates. */
+
+/* Layer norm over the nodes of a frame: y = (x - mean) * rstd * gamma + beta, mean and rstd = 1 / sqrt(variance + eps) [frame_size], which the
+ * backward takes.  dev_gamma / dev_beta [node_size], NULL: 1 / 0. */
+int bbcu_fp32_LayerNormalization_Forward(const float *dev_x_buf, float *dev_y_buf, const float *dev_gamma, const float *dev_beta, float *dev_mean_buf,
+                                         float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride, int y_frame_stride,
+                                         bbcu_stream_t stream);
+int bbcu_bf16_LayerNormalization_Forward(const bbcu_bf16_t *dev_x_buf, bbcu_bf16_t *dev_y_buf, const float *dev_gamma, const float *dev_beta,
+                                         float *dev_mean_buf, float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride,
+                                         int y_frame_stride, bbcu_stream_t stream);
+/* dx overwritten; dgamma and dbeta [node_size] (either may be NULL) overwritten, or with accumulate != 0 added to. */
+int bbcu_fp32_LayerNormalization_Backward(const float *dev_x_buf, const float *dev_dy_buf, float *dev_dx_buf, const float *dev_gamma,
+                                          const float *dev_mean_buf, const float *dev_rstd_buf, float *dev_dgamma, float *dev_dbeta, int accumulate,
+                                          int node_size, int frame_size, int x_frame_stride, int dy_frame_stride, int dx_frame_stride,
+                                          bbcu_stream_t stream);
+int bbcu_bf16_LayerNormalization_Backward(const bbcu_bf16_t *dev_x_buf, const bbcu_bf16_t *dev_dy_buf, bbcu_bf16_t *dev_dx_buf, const float *dev_gamma,
+                                          const float *dev_mean_buf, const float *dev_rstd_buf, float *dev_dgamma, float *dev_dbeta, int accumulate,
+                                          int node_size, int frame_size, int x_frame_stride, int dy_frame_stride, int dx_frame_stride,
+                                          bbcu_stream_t stream);
+
+/* Operands of the int8 product: every frame (or row of W) as a row of 8-bit integers along the nodes with a scale of its own, scale = max|x| / 127 and
+ * q = x / scale rounded to the nearest integer, ties to even, both in 32 bits.  A frame of zeros has scale 0; one that holds a NaN or an infinity
+ * has scale NaN and zeros, so that its product is NaN.  q_node_stride in bytes, a multiple of 16; bytes up to the next multiple of 16 nodes are cleared.
+ * dev_q_buf on a 16-byte boundary. */
+int bbcu_fp32_QuantizeInt8_Frames(const float *dev_x_buf, signed char *dev_q_buf, float *dev_scale_buf, int node_size, int frame_size, int x_frame_stride,
+                                  int q_node_stride, bbcu_stream_t stream);
+int bbcu_bf16_QuantizeInt8_Frames(const bbcu_bf16_t *dev_x_buf, signed char *dev_q_buf, float *dev_scale_buf, int node_size, int frame_size,
+                                  int x_frame_stride, int q_node_stride, bbcu_stream_t stream);
+int bbcu_fp32_QuantizeInt8_Channels(const float *dev_W, signed char *dev_q_buf, float *dev_scale_buf, int input_node_size, int output_node_size,
+                                    int w_node_stride, int q_node_stride, bbcu_stream_t stream);
+/* y[o][f] = w_scale[o] * q_scale[f] * sum_k W[o][k] * q[f][k] + bias[o] (dev_bias may be NULL), the sum exact: input_node_size up to 131071,
+ * BBCU_ERR_TOO_LARGE beyond.  W [output][input] and q [frame][input] are rows of 8-bit integers on 16-byte boundaries (node strides in bytes, multiples
+ * of 16, BBCU_ERR_BAD_STRIDE otherwise); what lies between input_node_size and the next multiple of 16 is not used. */
+int bbcu_int8_fp32_DenseAffine_Forward(const signed char *dev_q_buf, const float *dev_q_scale, const signed char *dev_W, const float *dev_w_scale,
+                                       const float *dev_bias, float *dev_y_buf, int input_node_size, int output_node_size, int frame_size,
+                                       int q_node_stride, int w_node_stride, int y_frame_stride, bbcu_stream_t stream);
+int bbcu_int8_bf16_DenseAffine_Forward(const signed char *dev_q_buf, const float *dev_q_scale, const signed char *dev_W, const float *dev_w_scale,
+                                       const float *dev_bias, bbcu_bf16_t *dev_y_buf, int input_node_size, int output_node_size, int frame_size,
+                                       int q_node_stride, int w_node_stride, int y_frame_stride, bbcu_stream_t stream);
+
+/* Distillation from a teacher's top logits.  dev_z_buf [class_size] rows: the student's logits; dev_t_buf and dev_index_buf [top_size] rows: logits of
+ * the teacher and the classes they belong to (a slot whose class is outside [0, class_size), or whose logit is -inf, is empty).  Per frame
+ *   p_k = exp(t_k / T - lse), lse over the frame's slots, or dev_t_lse[frame] = log sum exp(t / T) over all of the teacher's classes when it is given;
+ *   loss = T^2 sum_k p_k (log p_k - log softmax(z / T)[class_k]),   dz = its gradient;
+ * dev_loss_buf[frame] = weight * loss, *dev_loss = loss_reduction * their sum, dz = grad_reduction * weight * gradient (weight: dev_weight[frame],
+ * NULL: 1; both reductions 1 / frames for a mean).  A frame of weight 0 or without a slot gives zeros whatever it holds.  Classes that a frame names
+ * twice add up.  Results do not depend on the order in which anything runs. */
+int bbcu_fp32_LossDistillation(const float *dev_z_buf, float *dev_dz_buf, const float *dev_t_buf, const int *dev_index_buf, const float *dev_t_lse,
+                               const float *dev_weight, float *dev_loss_buf, float *dev_loss, float temperature, float grad_reduction,
+                               double loss_reduction, int class_size, int top_size, int frame_size, int z_frame_stride, int dz_frame_stride,
+                               int t_frame_stride, int index_frame_stride, bbcu_stream_t stream);
+int bbcu_bf16_LossDistillation(const bbcu_bf16_t *dev_z_buf, bbcu_bf16_t *dev_dz_buf, const bbcu_bf16_t *dev_t_buf, const int *dev_index_buf,
+                               const float *dev_t_lse, const float *dev_weight, float *dev_loss_buf, float *dev_loss, float temperature,
+                               float grad_reduction, double loss_reduction, int class_size, int top_size, int frame_size, int z_frame_stride,
+                               int dz_frame_stride, int t_frame_stride, int index_frame_stride, bbcu_stream_t stream);
 
 #ifdef __cplusplus
 }
