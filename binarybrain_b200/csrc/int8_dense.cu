@@ -5,12 +5,17 @@
 //               a frame of zeros has s = 0, one with a NaN or an infinity s = NaN, both q = 0.  The frames become rows, q[frame][node], 16-byte
 //               pieces along the nodes, which is how the product reads both of its operands.  The channel form does the same to the rows of W[out][in].
 //   product     y[o][f] = s_w[o] s_x[f] sum_k Wq[o][k] q[f][k] + bias[o],  the sum exact in 32-bit integers (at most 131071 inputs), y fp32 or bf16
+#include <cuda.h>
+
+#include "async_copy.cuh"
 #include "frame_columns.cuh"
+#include "tensor_core.cuh"
 
 namespace bb200 {
 
 constexpr int kQuantThreads = 256, kQuantRows = 128;      // rows of x that a CTA turns over at a time
 constexpr int kMostInputs = 131071;                       // times 128 x 128 is below 2^31
+constexpr int kRowFrames = 8;                             // up to this many frames the product reads rows of W, beyond it works on tiles
 
 __device__ __forceinline__ float quant_scale(uint32_t abs_bits)
 {
@@ -185,6 +190,239 @@ k_int8_dense_rows(const int8_t *__restrict__ q, const float *__restrict__ q_scal
         }
 }
 
+// ---- the product on the tensor cores: tiles of 128 output nodes x TN frames, D[o][f] = sum_k W[o][k] q[f][k] in TMEM (lane = output node, column =
+// frame), 128 bytes of k a stage, brought by TMA into 128-byte swizzled rows.  Warp 0 copies, warp 1 issues the matrix instructions, warps 2-5 scale and
+// store; the accumulator is double, so that the epilogue of a tile runs beside the products of the next.  Where there are fewer tiles than SMs, a
+// cluster of CTAs shares the k of one tile: the integer partial sums cross through distributed shared memory (in any order: they are exact), and every
+// CTA finishes its part of the columns.
+constexpr int kGemmThreads = 192, kTileO = 128, kTileK = 128;
+template <int TN> constexpr int kGemmStages = TN >= 256 ? 4 : TN >= 128 ? 6 : 8;
+template <int TN> constexpr int kStageBytes = (kTileO + TN) * kTileK;
+template <int TN> constexpr int kGemmSmem = kGemmStages<TN> * kStageBytes<TN> + 1024;
+constexpr int kTileGroup = 16;                           // tiles of output nodes that are walked together, so that their W and the q of some frames stay in L2
+
+struct GemmArgs {
+    const float *q_scale, *w_scale, *bias;
+    int K, O, F, splits, vec;
+    long long ys;
+    int *fault;
+};
+
+template <typename T, int TN>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+k_int8_dense_tiles(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q, T *y, const GemmArgs a)
+{
+    constexpr int kStages = kGemmStages<TN>, kAcc = 2, kColumns = kAcc * TN < 32 ? 32 : kAcc * TN;
+    static_assert(kColumns <= 512 && (kColumns & (kColumns - 1)) == 0, "TMEM");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[kStages], empty[kStages], acc_full[kAcc], acc_empty[kAcc], drained;
+    __shared__ uint32_t tmem_base;
+    __shared__ int gave_up;
+    __shared__ float s_scale[4][TN];                                      // of the frames of a tile, one copy an epilogue warp
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = a.splits > 1 ? cluster_rank() : 0;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 4); }
+        mbar_init(&drained, 1);
+        gave_up = 0;
+        mbar_init_fence();
+    }
+    if (warp == 1) tmem_alloc(&tmem_base, kColumns);
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = tmem_base;
+    grid_dependency();
+
+    const int tiles_o = (a.O + kTileO - 1) / kTileO, tiles_f = (a.F + TN - 1) / TN, tiles = tiles_o * tiles_f;
+    const int blocks_k = (a.K + kTileK - 1) / kTileK;
+    const int k0 = (int)((long long)blocks_k * rank / a.splits), k1 = (int)((long long)blocks_k * (rank + 1) / a.splits);
+    const int first = (int)blockIdx.x / a.splits, step = (int)gridDim.x / a.splits;
+    auto place = [&](int tile, int &o0, int &f0) {
+        const int group = tile / (kTileGroup * tiles_f), in = tile % (kTileGroup * tiles_f), rows = min(kTileGroup, tiles_o - group * kTileGroup);
+        o0 = (group * kTileGroup + in % rows) * kTileO;
+        f0 = in / rows * TN;
+    };
+
+    if (warp == 0 && lane == 0) {
+        int stage = 0, issued = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            int o0, f0;
+            place(tile, o0, f0);
+            for (int kb = k0; kb < k1 && ok; ++kb) {
+                ok = mbar_wait_one(&empty[stage], phase ^ 1, &gave_up);
+                if (!ok) break;
+                uint8_t *at = smem + stage * kStageBytes<TN>;
+                mbar_arrive_expect_tx(&full[stage], kStageBytes<TN>);
+                tma_load_2d(at, &map_w, kb * kTileK, o0, &full[stage]);
+                tma_load_2d(at + kTileO * kTileK, &map_q, kb * kTileK, f0, &full[stage]);
+                ++issued;
+                if (++stage == kStages) { stage = 0; phase ^= 1; }
+            }
+        }
+        // what is under way lands before the CTA leaves, also where a wait has run out
+        for (int b = issued > kStages ? issued - kStages : 0; b < issued; ++b) mbar_wait_some(&full[b % kStages], (uint32_t)(b / kStages) & 1u, kDrainSpins);
+    } else if (warp == 1 && lane == 0) {
+        constexpr uint32_t kInstr = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(kTileO >> 4) << 24);     // s32 += s8 x s8
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            ok = mbar_wait_one(&acc_empty[acc], acc_phase ^ 1, &gave_up);
+            if (!ok) break;
+            tcgen05_fence_after();
+            for (int kb = k0; kb < k1; ++kb) {
+                ok = mbar_wait_one(&full[stage], phase, &gave_up);
+                if (!ok) break;
+                tcgen05_fence_after();
+                const uint32_t at = smem_addr(smem + stage * kStageBytes<TN>);
+                const uint64_t da = smem_descriptor_128b(at), db = smem_descriptor_128b(at + kTileO * kTileK);
+#pragma unroll
+                for (int k = 0; k < kTileK / 32; ++k) mma_i8(tmem + acc * TN, da + 2 * k, db + 2 * k, kInstr, kb > k0 || k > 0);
+                tcgen05_commit(&empty[stage]);
+                if (++stage == kStages) { stage = 0; phase ^= 1; }
+            }
+            if (!ok) break;
+            tcgen05_commit(&acc_full[acc]);
+            if (++acc == kAcc) { acc = 0; acc_phase ^= 1; }
+        }
+        tcgen05_commit(&drained);                                         // no product is under way when the TMEM goes back
+        mbar_wait_some(&drained, 0, kDrainSpins);
+    } else if (warp >= 2) {
+        const int part = warp & 3, row = part * 32 + lane;                // the lanes of TMEM that this warp may read
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int tile = first; tile < tiles; tile += step) {
+            int o0, f0;
+            place(tile, o0, f0);
+            const int o = o0 + row;
+            __syncwarp();
+            for (int i = lane; i < TN; i += 32) s_scale[part][i] = f0 + i < a.F ? a.q_scale[f0 + i] : 0.0f;
+            const float ws = o < a.O ? a.w_scale[o] : 0.0f, b = o < a.O && a.bias ? a.bias[o] : 0.0f;
+            __syncwarp();
+            if (!mbar_wait_warp(&acc_full[acc], acc_phase, &gave_up)) break;
+            tcgen05_fence_after();
+            const uint32_t at = tmem + ((uint32_t)(part * 32) << 16) + acc * TN;
+            if (a.splits == 1) {
+#pragma unroll 1
+                for (int c = 0; c < TN; c += 32) {
+                    if (f0 + c >= a.F) break;
+                    int v[32];
+                    tmem_load_32(at + c, v);
+                    if (o < a.O) {
+                        float r[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) r[i] = fmaf((float)v[i], ws * s_scale[part][c + i], b);
+                        T *out = y + (long long)o * a.ys + f0 + c;
+                        if (a.vec && f0 + c + 32 <= a.F) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += kFramesPerVec<T>) {
+                                float w[kFramesPerVec<T>];
+#pragma unroll
+                                for (int j = 0; j < kFramesPerVec<T>; ++j) w[j] = r[i + j];
+                                *reinterpret_cast<uint4 *>(out + i) = pack<T>(w);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (f0 + c + i < a.F) out[i] = from_float<T>(r[i]);
+                        }
+                    }
+                }
+            } else {
+                // the stages are free: the tile's last product is done, and with it everything that read them
+                int *sums = reinterpret_cast<int *>(smem) + row * (TN + 4);
+#pragma unroll 1
+                for (int c = 0; c < TN; c += 32) {
+                    int v[32];
+                    tmem_load_32(at + c, v);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<int4 *>(sums + c + i) = make_int4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+            }
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[acc]);
+            if (++acc == kAcc) { acc = 0; acc_phase ^= 1; }
+        }
+    }
+    if (a.splits > 1) {
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (warp >= 2 && !gave_up) {
+            int o0, f0;
+            place(first, o0, f0);
+            const int row = (warp & 3) * 32 + lane, o = o0 + row, width = TN / a.splits, c0 = (int)rank * width;
+            if (o < a.O) {
+                const float ws = a.w_scale[o], b = a.bias ? a.bias[o] : 0.0f;
+                const uint32_t own = smem_addr(reinterpret_cast<int *>(smem) + row * (TN + 4));
+                for (int c = c0; c < c0 + width; c += 4) {
+                    int4 v = make_int4(0, 0, 0, 0);
+                    for (uint32_t r = 0; r < (uint32_t)a.splits; ++r) {
+                        const int4 p = peer_load_v4(own + c * 4, r);
+                        v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
+                    }
+                    const int sums[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (f0 + c + i < a.F) y[(long long)o * a.ys + f0 + c + i] = from_float<T>(fmaf((float)sums[i], ws * s_scale[warp & 3][c + i], b));
+                }
+            }
+        }
+        __syncwarp();
+        cluster_arrive();                                                 // nobody leaves while its sums may still be read
+        cluster_wait();
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    if (warp == 1) tmem_free(tmem, kColumns);
+    if (threadIdx.x == 0 && gave_up) atomicCAS(a.fault, 0, kFaultBarrierTimeout);
+}
+
+// rows of 8-bit integers as TMA sees them: boxes of 128 bytes x `box_rows` rows; what lies beyond the inputs or the rows reads as zero
+static int int8_rows_map(CUtensorMap *map, const int8_t *p, int K, int rows, long long stride, int box_rows)
+{
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            fn = nullptr;
+        }
+        return reinterpret_cast<Encode>(fn);
+    }();
+    BB200_REQUIRE(encode != nullptr, BBCU_ERR_NO_DEVICE);
+    const cuuint64_t size[2] = {(cuuint64_t)K, (cuuint64_t)rows}, pitch[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows}, unit[2] = {1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(p), size, pitch, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? BBCU_OK : (int)cudaErrorInvalidValue;
+}
+
+template <typename T, int TN>
+static int int8_dense_tiles(const int8_t *q, const int8_t *W, T *y, GemmArgs a, long long qs, long long ws, cudaStream_t st)
+{
+    CUtensorMap map_w, map_q;
+    if (const int e = int8_rows_map(&map_w, W, a.K, a.O, ws, kTileO)) return e;
+    if (const int e = int8_rows_map(&map_q, q, a.K, a.F, qs, TN)) return e;
+    const long long tiles = ((long long)a.O + kTileO - 1) / kTileO * (((long long)a.F + TN - 1) / TN);
+    BB200_REQUIRE(tiles < (1LL << 27), BBCU_ERR_TOO_LARGE);
+    auto kernel = k_int8_dense_tiles<T, TN>;
+    BB200_REQUIRE(allow_big_smem(kernel, kGemmSmem<TN>), (int)cudaErrorInvalidValue);
+    const long long sms = device_info().sm_count;
+    const unsigned grid = a.splits > 1 ? (unsigned)(tiles * a.splits) : (unsigned)(tiles < sms ? tiles : sms);
+    return launch_cluster(kernel, (unsigned)a.splits, grid, kGemmThreads, kGemmSmem<TN>, st, map_w, map_q, y, a);
+}
+
 template <typename T>
 static int quantize_frames(const T *x, int8_t *q, float *scale, int N, int F, int xs, int qs, bbcu_stream_t stream)
 {
@@ -222,12 +460,22 @@ static int int8_dense(const int8_t *q, const float *q_scale, const int8_t *W, co
                   reinterpret_cast<uintptr_t>(W) % 16 == 0 && ys >= F, BBCU_ERR_BAD_STRIDE);
     if (F == 0 || O == 0) return BBCU_OK;
     BB200_REQUIRE_PTR(q); BB200_REQUIRE_PTR(q_scale); BB200_REQUIRE_PTR(W); BB200_REQUIRE_PTR(w_scale); BB200_REQUIRE_PTR(y);
-    constexpr int kFrames = 8, kRows = 4;
-    const long long frame_ctas = ((long long)F + kFrames - 1) / kFrames, row_ctas = ((long long)O + 8 * kRows - 1) / (8 * kRows);
-    BB200_REQUIRE(frame_ctas <= 65535, BBCU_ERR_TOO_LARGE);
-    launch(k_int8_dense_rows<T, kFrames, kRows>, dim3((unsigned)row_ctas, (unsigned)frame_ctas), 256, 0, as_stream(stream), q, q_scale, W, w_scale, bias, y, K, O, F,
-           qs, ws, ys);
-    return launch_status();
+    cudaStream_t st = as_stream(stream);
+    if (F <= kRowFrames) {
+        constexpr int kRows = 4;
+        const long long row_ctas = ((long long)O + 8 * kRows - 1) / (8 * kRows);
+        launch(k_int8_dense_rows<T, kRowFrames, kRows>, (unsigned)row_ctas, 256, 0, st, q, q_scale, W, w_scale, bias, y, K, O, F, qs, ws, ys);
+        return launch_status();
+    }
+    int *fault = fault_word();
+    BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
+    GemmArgs a{q_scale, w_scale, bias, K, O, F, 1, frames_aligned<T>(y, ys), ys, fault};
+    const long long tiles_o = ((long long)O + kTileO - 1) / kTileO, sms = device_info().sm_count;
+    auto tiles = [&](int tn) { return tiles_o * ((F + tn - 1) / tn); };
+    const int tn = F <= 32 ? 32 : F <= 64 || tiles(128) < sms ? 64 : tiles(256) < sms ? 128 : 256;
+    while (a.splits < 8 && tiles(tn) * a.splits * 2 <= sms && (K + kTileK - 1) / kTileK >= a.splits * 4) a.splits *= 2;
+    return tn == 32 ? int8_dense_tiles<T, 32>(q, W, y, a, qs, ws, st) : tn == 64 ? int8_dense_tiles<T, 64>(q, W, y, a, qs, ws, st)
+         : tn == 128 ? int8_dense_tiles<T, 128>(q, W, y, a, qs, ws, st) : int8_dense_tiles<T, 256>(q, W, y, a, qs, ws, st);
 }
 
 }   // namespace bb200
