@@ -7,8 +7,11 @@
 // them; the column sums cross the warps through shared memory and the CTAs through distributed shared memory.
 #pragma once
 
+#include <algorithm>
+
 #include <cuda_bf16.h>
 
+#include "async_copy.cuh"
 #include "common.cuh"
 
 namespace bb200 {
@@ -79,6 +82,21 @@ template <typename T, bool ALIGNED> __device__ __forceinline__ void store_frames
     }
 }
 
+// a number of each of a thread's columns, 0 beyond the frames
+template <int VEC> __device__ __forceinline__ void load_columns(const float *__restrict__ from, int f, int F, float (&v)[VEC])
+{
+    if (f + VEC <= F && (reinterpret_cast<uintptr_t>(from) & 15) == 0) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) {
+            const float4 o = *reinterpret_cast<const float4 *>(from + f + j);
+            v[j] = o.x; v[j + 1] = o.y; v[j + 2] = o.z; v[j + 3] = o.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = f + j < F ? from[f + j] : 0.0f;
+    }
+}
+
 template <typename T> inline bool frames_aligned(const void *p, long long stride) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * (long long)sizeof(T) % 16 == 0; }
 
 // ---- clusters
@@ -86,17 +104,31 @@ __device__ __forceinline__ uint32_t cluster_rank()  { uint32_t r; asm volatile("
 __device__ __forceinline__ uint32_t cluster_size()  { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_arrive()    { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait()      { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t peer_addr(const void *own, uint32_t rank)
+{
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(own)), "r"(rank));
+    return at;
+}
 __device__ __forceinline__ float peer_load(const float *own, uint32_t rank)
 {
-    uint32_t a;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(own)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_addr(own, rank)) : "memory");
     return v;
+}
+__device__ __forceinline__ double2 peer_load_double2(const double2 *own, uint32_t rank)
+{
+    double2 v;
+    asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];" : "=d"(v.x), "=d"(v.y) : "r"(peer_addr(own, rank)) : "memory");
+    return v;
+}
+// a value for another CTA's shared memory, whose barrier counts the bytes when they have arrived
+__device__ __forceinline__ void peer_send(uint32_t to, float v, uint32_t bar)
+{
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(to), "f"(v), "r"(bar) : "memory");
 }
 
 // Launch with clusters of `cluster` CTAs (grid.x is a multiple of it); 16 needs the kernel's opt-in.
-bool allow_cluster_16_once(const void *kernel);
 template <typename... P, typename... A>
 inline int launch_cluster(void (*kernel)(P...), unsigned cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A &&...args)
 {
@@ -131,11 +163,52 @@ template <typename T, int LPR> struct Column {
 struct ColumnSum { __device__ static float join(float a, float b) { return a + b; }  static constexpr float none = 0.0f; };
 struct ColumnMax { __device__ static float join(float a, float b) { return fmaxf(a, b); }  static constexpr float none = -INFINITY; };
 
-// Joins v[Q][kVec] over all rows of the tile (CTA, then cluster); every thread gets the result of its own columns, in the same order of operations
-// everywhere.  `red`: warps * Q * kCols floats, `part`: Q * kCols floats, neither in use by an exchange that a neighbour may still be reading:
-// consecutive exchanges alternate between two of each.
-template <typename OP, int Q, typename T, int LPR>
-__device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], const Column<T, LPR> &c, float *red, float *part, uint32_t cluster)
+constexpr int kColumnThreads = 256, kMostCluster = 16;
+
+// Shared memory of one exchange of Q values a column; consecutive exchanges alternate between two of them, since a neighbour may still be reading.
+template <int Q, int COLS> struct Exchange {
+    float red[kColumnThreads / 32][Q * COLS];
+    float part[kMostCluster][Q * COLS];
+    __align__(16) float out[Q * COLS];
+    uint64_t bar;
+};
+
+// A cluster of CTAs and what its exchanges have come to.  CTAs send their parts into the shared memory of all others, whose barriers count the bytes:
+// unlike a barrier over the cluster, that does not wait for the stores of the tile before to be visible.
+struct Cluster {
+    uint32_t size, rank;
+    int *gave_up;                                        // in shared memory: a wait ran out, all later ones are passed over
+    __device__ Cluster(int *flag) : size(cluster_size()), rank(cluster_rank()), gave_up(flag) {}
+
+    // before the first exchange: the barriers are there, and all CTAs run
+    template <typename E> __device__ void meet(E *exchanges, int count)
+    {
+        if (size == 1) return;
+        if (threadIdx.x == 0) {
+            *gave_up = 0;
+            for (int i = 0; i < count; ++i) mbar_init(&exchanges[i].bar, 1);
+            mbar_init_fence();
+        }
+        cluster_arrive();
+        cluster_wait();
+    }
+    // nobody leaves while something may still be sent to it
+    __device__ void leave(int *fault)
+    {
+        if (size == 1) return;
+        __syncthreads();
+        if (threadIdx.x == 0 && *gave_up) atomicCAS(fault, 0, kFaultBarrierTimeout);
+        cluster_arrive();
+        cluster_wait();
+    }
+};
+
+// Joins v[Q][kVec] over all rows of the tile (CTA, then cluster) by a fixed order of operations; what finish(q, joined) makes of a value comes back in
+// v for the thread's own columns.  One thread a value joins the parts, since there are many threads and few columns.  `phase`: of the exchange's barrier,
+// 0 and 1 in turn.
+template <typename OP, int Q, typename T, int LPR, typename FINISH>
+__device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], const Column<T, LPR> &c, Exchange<Q, LPR * kFramesPerVec<T>> &e, const Cluster &cl,
+                                             uint32_t phase, FINISH finish)
 {
     constexpr int kVec = kFramesPerVec<T>, kCols = LPR * kVec;
 #pragma unroll
@@ -148,46 +221,60 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
 #pragma unroll
         for (int q = 0; q < Q; ++q)
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) red[(c.warp * Q + q) * kCols + c.col + j] = v[q][j];
+            for (int j = 0; j < kVec; ++j) e.red[c.warp][q * kCols + c.col + j] = v[q][j];
+    }
+    if (cl.size > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(&e.bar, cl.size * Q * kCols * (uint32_t)sizeof(float));
+    __syncthreads();
+    for (int i = threadIdx.x; i < Q * kCols; i += blockDim.x) {
+        float s = e.red[0][i];
+        for (int w = 1; w < c.warps; ++w) s = OP::join(s, e.red[w][i]);
+        if (cl.size == 1) {
+            e.out[i] = finish(i / kCols, s);
+        } else {
+            for (uint32_t r = 0; r < cl.size; ++r) peer_send(peer_addr(&e.part[cl.rank][i], r), s, peer_addr(&e.bar, r));
+        }
+    }
+    if (cl.size > 1) {
+        if (threadIdx.x / 32 * 32 < Q * kCols) {                          // warps that have something to join
+            bool ok = *(volatile int *)cl.gave_up == 0;
+            for (int i = 0; i < kWaitSpins && ok; ++i) {
+                if (mbar_try_wait(&e.bar, phase)) break;
+                if (i == kWaitSpins - 1) { *(volatile int *)cl.gave_up = 1; ok = false; }
+            }
+        }
+        for (int i = threadIdx.x; i < Q * kCols; i += blockDim.x) {
+            float s = e.part[0][i];
+            for (uint32_t r = 1; r < cl.size; ++r) s = OP::join(s, e.part[r][i]);
+            e.out[i] = finish(i / kCols, s);
+        }
     }
     __syncthreads();
-    if (cluster == 1) {
-#pragma unroll
-        for (int q = 0; q < Q; ++q)
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) v[q][j] = red[q * kCols + c.col + j];
-        for (int w = 1; w < c.warps; ++w)
-#pragma unroll
-            for (int q = 0; q < Q; ++q)
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) v[q][j] = OP::join(v[q][j], red[(w * Q + q) * kCols + c.col + j]);
-        return;
-    }
-    for (int i = threadIdx.x; i < Q * kCols; i += blockDim.x) {
-        float s = red[i];
-        for (int w = 1; w < c.warps; ++w) s = OP::join(s, red[w * Q * kCols + i]);
-        part[i] = s;
-    }
-    cluster_arrive();
-    cluster_wait();
 #pragma unroll
     for (int q = 0; q < Q; ++q)
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) v[q][j] = OP::none;
-    for (uint32_t r = 0; r < cluster; ++r)
-#pragma unroll
-        for (int q = 0; q < Q; ++q)
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) v[q][j] = OP::join(v[q][j], peer_load(part + q * kCols + c.col + j, r));
+        for (int j = 0; j < kVec; j += 4) {
+            const float4 o = *reinterpret_cast<const float4 *>(&e.out[q * kCols + c.col + j]);
+            v[q][j] = o.x; v[q][j + 1] = o.y; v[q][j + 2] = o.z; v[q][j + 3] = o.w;
+        }
 }
 
-// No CTA of a cluster leaves while another may still read its shared memory.
-__device__ __forceinline__ void cluster_leave(uint32_t cluster)
+// How a layer of N rows and F frames is cut: `lanes` lanes along a row, clusters of `cluster` CTAs (0: its columns are too long for one) of `warps` warps,
+// `rows` rows a thread, at most `most_rows`.
+struct ColumnPlan { int cluster, warps, rows, lanes; };
+template <typename T>
+inline ColumnPlan plan_columns(int N, int F, int lanes, int most_rows)
 {
-    if (cluster > 1) { cluster_arrive(); cluster_wait(); }
+    if (F <= 2 * kFramesPerVec<T>) lanes = 2;
+    const int per_warp = 32 / lanes, most_warps = kColumnThreads / 32;
+    const long long tiles = ((long long)F + lanes * kFramesPerVec<T> - 1) / (lanes * kFramesPerVec<T>), sms = device_info().sm_count;
+    int cluster = 1;
+    auto rows = [&] { return (N + cluster - 1) / cluster; };
+    // as many CTAs as it takes to hold a column, and more where there would be few
+    while (cluster < kMostCluster && rows() > most_warps * per_warp * most_rows) cluster *= 2;
+    if (rows() > most_warps * per_warp * most_rows) return {0, 0, 0, 0};
+    while (cluster < 8 && tiles * cluster * 2 <= sms && rows() > most_warps * per_warp) cluster *= 2;
+    const int warps = std::min(most_warps, (rows() + per_warp - 1) / per_warp);
+    return {cluster, warps, (rows() + per_warp * warps - 1) / (per_warp * warps), lanes};
 }
-
-// How a layer of N rows and F frames is cut: clusters of `cluster` CTAs of `warps` warps, `rows` rows a thread.
-struct ColumnPlan { int cluster, warps, rows; };
 
 }   // namespace bb200

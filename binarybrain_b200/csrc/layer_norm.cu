@@ -6,41 +6,46 @@
 //              dgamma_n = sum_f dy xh,  dbeta_n = sum_f dy
 //
 // Statistics and sums are 32 bits throughout; bf16 frames are widened when they are read and rounded once when they are written.
+#include <algorithm>
+
 #include "frame_columns.cuh"
 
 namespace bb200 {
 
-constexpr int kMostNodes = 1 << 24;                    // row numbers and their distances stay far from 2^31
+constexpr int kMostNodes = 1 << 20;                    // 32 rows a CTA are 32768 CTAs at most
 constexpr int kNormThreads = 256;                      // of the kernels that stream over chunks of rows
 
-// ---- sums of a chunk of rows: part[chunk][column] = (sum d, sum d^2), d = x minus the column's first value, which takes a large level out.  Eight
-// rows are added up in 32 bits and joined with the rest in 64, so that a long column costs no digits either.
+// ---- two passes: statistics of the frames, then what is made of them.  The second one finds what L2 (126 MB) still holds of the first.
+
+// A cluster has the columns of 128 bytes of a row; its CTAs take turns at the rows, add up d = x minus the column's first value (which takes a large
+// level out) and d^2, eight rows in 32 bits and those sums in 64, so that neither a level nor a long column costs digits, and join them in the first
+// CTA's shared memory.
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kNormThreads)
-k_layer_norm_stats(const T *x, double2 *part, int N, int F, long long xs, int chunk_rows, int columns)
+__global__ void __launch_bounds__(kNormThreads, 4)
+k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int N, int F, long long xs)
 {
     grid_dependency();
-    constexpr int kLpr = 8, kBatch = 8;
+    constexpr int kLpr = 8, kBatch = sizeof(T) == 4 ? 8 : 4;
     using Col = Column<T, kLpr>;
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
-    __shared__ double2 red[8][kCols];
+    __shared__ float2 red[8][kCols];
+    __shared__ double2 part[kCols];
     const Col c;
-    const int f = (int)blockIdx.x * kCols + c.col;
-    const int n0 = (int)blockIdx.y * chunk_rows, n1 = min(N, n0 + chunk_rows);
-    double s1[kVec] = {}, s2[kVec] = {};
-    float level[kVec];
+    const uint32_t cl = cluster_size(), rank = cluster_rank();
+    const int f0 = (int)(blockIdx.x / cl) * kCols, f = f0 + c.col, step = c.step * (int)cl;
+    float s1[kVec] = {}, s2[kVec] = {}, level[kVec];
     unpack<T>(load_frames<T, ALIGNED>(x, f, F), level);
-    for (int n = n0 + c.row; n < n1; n += c.step * kBatch) {
+    for (int n = (int)rank * c.step + c.row; n < N; n += step * kBatch) {
         uint4 raw[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int m = n + i * c.step;
-            if (m < n1) raw[i] = load_frames<T, ALIGNED>(x + (long long)m * xs, f, F);
+            const int m = n + i * step;
+            if (m < N) raw[i] = load_frames<T, ALIGNED>(x + (long long)m * xs, f, F);
         }
         float b1[kVec] = {}, b2[kVec] = {};
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            if (n + i * c.step < n1) {
+            if (n + i * step < N) {
                 float v[kVec];
                 unpack<T>(raw[i], v);
 #pragma unroll
@@ -52,7 +57,7 @@ k_layer_norm_stats(const T *x, double2 *part, int N, int F, long long xs, int ch
             }
         }
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) { s1[j] += (double)b1[j]; s2[j] += (double)b2[j]; }
+        for (int j = 0; j < kVec; ++j) { s1[j] += b1[j]; s2[j] += b2[j]; }
     }
 #pragma unroll
     for (int m = kLpr; m < 32; m <<= 1)
@@ -63,197 +68,383 @@ k_layer_norm_stats(const T *x, double2 *part, int N, int F, long long xs, int ch
         }
     if (c.lane < kLpr) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) red[c.warp][c.col + j] = make_double2(s1[j], s2[j]);
+        for (int j = 0; j < kVec; ++j) red[c.warp][c.col + j] = make_float2(s1[j], s2[j]);
     }
     __syncthreads();
     if (threadIdx.x < kCols) {
-        double2 t = red[0][threadIdx.x];
-        for (int w = 1; w < c.warps; ++w) { t.x += red[w][threadIdx.x].x; t.y += red[w][threadIdx.x].y; }
-        part[(long long)blockIdx.y * columns + (long long)blockIdx.x * kCols + threadIdx.x] = t;
+        double2 t = make_double2(0.0, 0.0);
+        for (int w = 0; w < c.warps; ++w) { t.x += (double)red[w][threadIdx.x].x; t.y += (double)red[w][threadIdx.x].y; }
+        part[threadIdx.x] = t;
     }
+    if (cl > 1) { cluster_arrive(); cluster_wait(); }
+    if (rank == 0 && threadIdx.x < kCols && f0 + (int)threadIdx.x < F) {
+        double2 t = part[threadIdx.x];
+        for (uint32_t r = 1; r < cl; ++r) {
+            const double2 p = peer_load_double2(&part[threadIdx.x], r);
+            t.x += p.x;
+            t.y += p.y;
+        }
+        t.x /= (double)N;
+        double var = t.y / (double)N - t.x * t.x;
+        if (var < 0.0) var = 0.0;                                         // (and a NaN stays one)
+        mean_out[f0 + threadIdx.x] = (float)((double)to_float(x[f0 + threadIdx.x]) + t.x);
+        rstd_out[f0 + threadIdx.x] = 1.0f / sqrtf((float)var + eps);
+    }
+    if (cl > 1) { cluster_arrive(); cluster_wait(); }                     // nobody leaves while its sums may still be read
 }
 
+// Along the rows: a warp takes 512 bytes of a row, a CTA 8 x kApplyRows rows, which share the frames' statistics.
+constexpr int kApplyRows = 8;
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kNormThreads)
-k_layer_norm_apply(const T *x, T *y, const double2 *__restrict__ part, const float *__restrict__ gamma, const float *__restrict__ beta, float *mean_out,
-                   float *rstd_out, float eps, int N, int F, long long xs, long long ys, int chunk_rows, int chunks, int columns)
+k_layer_norm_apply(const T *x, T *y, const float *__restrict__ gamma, const float *__restrict__ beta, const float *__restrict__ mean_in,
+                   const float *__restrict__ rstd_in, int N, int F, long long xs, long long ys)
 {
     grid_dependency();
-    constexpr int kLpr = 8, kBatch = 8;
-    using Col = Column<T, kLpr>;
-    constexpr int kVec = Col::kVec, kCols = Col::kCols;
-    __shared__ float s_mean[kCols], s_rstd[kCols];
-    const Col c;
-    const int f0 = (int)blockIdx.x * kCols, f = f0 + c.col;
-    if (threadIdx.x < kCols) {
-        double s1 = 0.0, s2 = 0.0;
-        for (int k = 0; k < chunks; ++k) {
-            const double2 p = part[(long long)k * columns + f0 + threadIdx.x];
-            s1 += p.x;
-            s2 += p.y;
-        }
-        const bool live = f0 + (int)threadIdx.x < F;
-        s1 /= (double)N;
-        double var = s2 / (double)N - s1 * s1;
-        if (var < 0.0) var = 0.0;                                        // (and a NaN stays one)
-        const float mean = (float)((live ? (double)to_float(x[f0 + threadIdx.x]) : 0.0) + s1), rstd = 1.0f / sqrtf((float)var + eps);
-        s_mean[threadIdx.x] = mean;
-        s_rstd[threadIdx.x] = rstd;
-        if (blockIdx.y == 0 && live) {
-            mean_out[f0 + threadIdx.x] = mean;
-            rstd_out[f0 + threadIdx.x] = rstd;
-        }
-    }
-    __syncthreads();
+    constexpr int kVec = kFramesPerVec<T>;
+    const int f = ((int)blockIdx.x * 32 + (int)(threadIdx.x & 31)) * kVec, n0 = ((int)blockIdx.y * 8 + (int)(threadIdx.x >> 5)) * kApplyRows;
+    if (f >= F) return;
+    uint4 raw[kApplyRows];
+#pragma unroll
+    for (int i = 0; i < kApplyRows; ++i)
+        if (n0 + i < N) raw[i] = load_frames<T, ALIGNED>(x + (long long)(n0 + i) * xs, f, F);
     float mean[kVec], rstd[kVec];
+    load_columns(mean_in, f, F, mean);
+    load_columns(rstd_in, f, F, rstd);
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) { mean[j] = s_mean[c.col + j]; rstd[j] = s_rstd[c.col + j]; }
-    const int n0 = (int)blockIdx.y * chunk_rows, n1 = min(N, n0 + chunk_rows);
-    for (int n = n0 + c.row; n < n1; n += c.step * kBatch) {
-        uint4 raw[kBatch];
+    for (int i = 0; i < kApplyRows; ++i) {
+        if (n0 + i < N) {
+            const float g = gamma ? gamma[n0 + i] : 1.0f, b = beta ? beta[n0 + i] : 0.0f;
+            float v[kVec];
+            unpack<T>(raw[i], v);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int m = n + i * c.step;
-            if (m < n1) raw[i] = load_frames<T, ALIGNED>(x + (long long)m * xs, f, F);
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int m = n + i * c.step;
-            if (m < n1) {
-                const float g = gamma ? gamma[m] : 1.0f, b = beta ? beta[m] : 0.0f;
-                float v[kVec];
-                unpack<T>(raw[i], v);
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) v[j] = fmaf((v[j] - mean[j]) * rstd[j], g, b);
-                store_frames<T, ALIGNED>(y + (long long)m * ys, f, F, v);
-            }
+            for (int j = 0; j < kVec; ++j) v[j] = fmaf((v[j] - mean[j]) * rstd[j], g, b);
+            store_frames<T, ALIGNED>(y + (long long)(n0 + i) * ys, f, F, v);
         }
     }
 }
 
-// ---- backward: the two sums over the nodes of a chunk
+// backward: sums[frame] = mean_n gamma dy, sums[padded + frame] = mean_n gamma dy xh
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, 4)
 k_layer_norm_grad_stats(const T *x, const T *dy, const float *__restrict__ gamma, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
-                        float2 *part, int N, int F, long long xs, long long dys, int chunk_rows, int columns)
+                        float *sums_out, int padded, int N, int F, long long xs, long long dys)
 {
     grid_dependency();
-    constexpr int kLpr = 8, kBatch = 4;
+    constexpr int kLpr = 8, kBatch = sizeof(T) == 4 ? 4 : 2;
     using Col = Column<T, kLpr>;
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
-    __shared__ float red[8 * 2 * kCols];
+    __shared__ float red[8][2 * kCols];
+    __shared__ float part[2 * kCols];
     const Col c;
-    const int f0 = (int)blockIdx.x * kCols, f = f0 + c.col;
-    const int n0 = (int)blockIdx.y * chunk_rows, n1 = min(N, n0 + chunk_rows);
-    float mean[kVec], rstd[kVec], s[2][kVec] = {};
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) { mean[j] = f + j < F ? mean_in[f + j] : 0.0f; rstd[j] = f + j < F ? rstd_in[f + j] : 0.0f; }
-    for (int n = n0 + c.row; n < n1; n += c.step * kBatch) {
+    const uint32_t cl = cluster_size(), rank = cluster_rank();
+    const int f0 = (int)(blockIdx.x / cl) * kCols, f = f0 + c.col, step = c.step * (int)cl;
+    float mean[kVec], s[2][kVec] = {};
+    load_columns(mean_in, f, F, mean);
+    for (int n = (int)rank * c.step + c.row; n < N; n += step * kBatch) {
         uint4 xr[kBatch], gr[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int m = n + i * c.step;
-            xr[i] = m < n1 ? load_frames<T, ALIGNED>(x + (long long)m * xs, f, F) : make_uint4(0, 0, 0, 0);
-            gr[i] = m < n1 ? load_frames<T, ALIGNED>(dy + (long long)m * dys, f, F) : make_uint4(0, 0, 0, 0);
+            const int m = n + i * step;
+            if (m < N) {
+                xr[i] = load_frames<T, ALIGNED>(x + (long long)m * xs, f, F);
+                gr[i] = load_frames<T, ALIGNED>(dy + (long long)m * dys, f, F);
+            }
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int m = n + i * c.step;
-            if (m < n1) {
+            const int m = n + i * step;
+            if (m < N) {
                 const float gm = gamma ? gamma[m] : 1.0f;
                 float xv[kVec], gv[kVec];
                 unpack<T>(xr[i], xv);
                 unpack<T>(gr[i], gv);
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) {
-                    const float g = gm * gv[j], xh = (xv[j] - mean[j]) * rstd[j];
+                    const float g = gm * gv[j];
                     s[0][j] += g;
-                    s[1][j] = fmaf(g, xh, s[1][j]);
+                    s[1][j] = fmaf(g, xv[j] - mean[j], s[1][j]);          // times rstd at the end
                 }
             }
         }
     }
-    join_columns<ColumnSum, 2, T, kLpr>(s, c, red, nullptr, 1);
-    if (c.warp == 0 && c.lane < kLpr) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) part[(long long)blockIdx.y * columns + f + j] = make_float2(s[0][j], s[1][j]);
+    for (int m = kLpr; m < 32; m <<= 1)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) s[q][j] += __shfl_xor_sync(0xffffffffu, s[q][j], m);
+    if (c.lane < kLpr) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) red[c.warp][q * kCols + c.col + j] = s[q][j];
     }
+    __syncthreads();
+    if (threadIdx.x < 2 * kCols) {
+        float t = red[0][threadIdx.x];
+        for (int w = 1; w < c.warps; ++w) t += red[w][threadIdx.x];
+        part[threadIdx.x] = t;
+    }
+    if (cl > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads();
+    if (rank == 0 && threadIdx.x < kCols && f0 + (int)threadIdx.x < F) {
+        float a = 0.0f, b = 0.0f;
+        for (uint32_t r = 0; r < cl; ++r) { a += peer_load(&part[threadIdx.x], r); b += peer_load(&part[kCols + threadIdx.x], r); }
+        sums_out[f0 + threadIdx.x] = a / (float)N;
+        sums_out[padded + f0 + threadIdx.x] = b * rstd_in[f0 + threadIdx.x] / (float)N;
+    }
+    if (cl > 1) { cluster_arrive(); cluster_wait(); }
 }
 
-// dx of R rows a thread over every gridDim.x-th column tile, with the sums over those frames kept in registers on the way:
+// Along the rows again: a CTA has 8 x R rows and every gridDim.x-th piece of 512 bytes of them, and adds up their sums over the frames on the way:
 // grad_part[blockIdx.x][node] = (sum dy xh, sum dy)
 template <typename T, int R, bool ALIGNED>
-__global__ void __launch_bounds__(kNormThreads)
-k_layer_norm_grad_apply(const T *x, const T *dy, T *dx, const float2 *__restrict__ part, const float *__restrict__ gamma, const float *__restrict__ mean_in,
-                        const float *__restrict__ rstd_in, float2 *grad_part, int N, int F, long long xs, long long dys, long long dxs, int chunks,
-                        int columns)
+__global__ void __launch_bounds__(kNormThreads, 2)
+k_layer_norm_grad_apply(const T *x, const T *dy, T *dx, const float *__restrict__ sums, int padded, const float *__restrict__ gamma, const float *__restrict__ mean_in,
+                        const float *__restrict__ rstd_in, float2 *grad_part, int N, int F, long long xs, long long dys, long long dxs)
 {
     grid_dependency();
-    constexpr int kLpr = 8;
-    using Col = Column<T, kLpr>;
-    constexpr int kVec = Col::kVec, kCols = Col::kCols;
-    __shared__ float s_c[2][kCols];
-    const Col c;
-    const long long first = (long long)blockIdx.y * c.step * R + c.row;
-    const float inv = 1.0f / (float)N;
-    float gm[R], ag[R], ab[R];
+    constexpr int kVec = kFramesPerVec<T>;
+    const int lane = threadIdx.x & 31, n0 = ((int)blockIdx.y * 8 + (int)(threadIdx.x >> 5)) * R;
+    float ag[R] = {}, ab[R] = {}, gm[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const long long n = first + i * c.step;
-        gm[i] = n < N ? (gamma ? gamma[n] : 1.0f) : 0.0f;
-        ag[i] = ab[i] = 0.0f;
-    }
-    for (int tile = blockIdx.x; tile < columns / kCols; tile += gridDim.x) {
-        const int f0 = tile * kCols, f = f0 + c.col;
+    for (int i = 0; i < R; ++i) gm[i] = gamma && n0 + i < N ? gamma[n0 + i] : 1.0f;
+    for (int f = ((int)blockIdx.x * 32 + lane) * kVec; f < F; f += (int)gridDim.x * 32 * kVec) {
         uint4 xr[R], gr[R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const long long n = first + i * c.step;
-            xr[i] = n < N ? load_frames<T, ALIGNED>(x + n * xs, f, F) : make_uint4(0, 0, 0, 0);
-            gr[i] = n < N ? load_frames<T, ALIGNED>(dy + n * dys, f, F) : make_uint4(0, 0, 0, 0);
-        }
-        __syncthreads();
-        if (threadIdx.x < kCols) {
-            float a = 0.0f, b = 0.0f;
-            for (int k = 0; k < chunks; ++k) {
-                const float2 p = part[(long long)k * columns + f0 + threadIdx.x];
-                a += p.x;
-                b += p.y;
+            if (n0 + i < N) {
+                xr[i] = load_frames<T, ALIGNED>(x + (long long)(n0 + i) * xs, f, F);
+                gr[i] = load_frames<T, ALIGNED>(dy + (long long)(n0 + i) * dys, f, F);
             }
-            s_c[0][threadIdx.x] = a * inv;
-            s_c[1][threadIdx.x] = b * inv;
         }
-        __syncthreads();
-        float mean[kVec], rstd[kVec];
+        float mean[kVec], rstd[kVec], k1[kVec], k2[kVec];                 // dx = (gamma rstd) dy + k1 + k2 xh
+        load_columns(mean_in, f, F, mean);
+        load_columns(rstd_in, f, F, rstd);
+        load_columns(sums, f, F, k1);
+        load_columns(sums + padded, f, F, k2);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) { mean[j] = f + j < F ? mean_in[f + j] : 0.0f; rstd[j] = f + j < F ? rstd_in[f + j] : 0.0f; }
+        for (int j = 0; j < kVec; ++j) { k1[j] *= -rstd[j]; k2[j] *= -rstd[j]; }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const long long n = first + i * c.step;
-            float xv[kVec], gv[kVec];
-            unpack<T>(xr[i], xv);
-            unpack<T>(gr[i], gv);
+            if (n0 + i < N) {
+                float xv[kVec], gv[kVec];
+                unpack<T>(xr[i], xv);
+                unpack<T>(gr[i], gv);
+                if (f + kVec > F) {                                       // what lies beyond the frames may be anything
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                const bool live = f + j < F;
-                const float g = live ? gv[j] : 0.0f, xh = live ? (xv[j] - mean[j]) * rstd[j] : 0.0f;
-                ag[i] = fmaf(g, xh, ag[i]);
-                ab[i] += g;
-                gv[j] = rstd[j] * (gm[i] * g - s_c[0][c.col + j] - xh * s_c[1][c.col + j]);
+                    for (int j = 0; j < kVec; ++j)
+                        if (f + j >= F) xv[j] = gv[j] = 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) {
+                    const float xh = (xv[j] - mean[j]) * rstd[j];
+                    ag[i] = fmaf(gv[j], xh, ag[i]);
+                    ab[i] += gv[j];
+                    gv[j] = fmaf(gv[j], gm[i] * rstd[j], fmaf(xh, k2[j], k1[j]));
+                }
+                store_frames<T, ALIGNED>(dx + (long long)(n0 + i) * dxs, f, F, gv);
             }
-            if (n < N) store_frames<T, ALIGNED>(dx + n * dxs, f, F, gv);
         }
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const long long n = first + i * c.step;
 #pragma unroll
-        for (int m = 1; m < kLpr; m <<= 1) {
+        for (int m = 16; m > 0; m >>= 1) {
             ag[i] += __shfl_xor_sync(0xffffffffu, ag[i], m);
             ab[i] += __shfl_xor_sync(0xffffffffu, ab[i], m);
         }
-        if (c.lane % kLpr == 0 && n < N) grad_part[(long long)blockIdx.x * N + n] = make_float2(ag[i], ab[i]);
+        if (lane == i && n0 + i < N) grad_part[(long long)blockIdx.x * N + n0 + i] = make_float2(ag[i], ab[i]);
     }
+}
+
+// ---- layers whose columns a cluster holds in shared memory: everything is read once.  The clusters walk over the column tiles; each thread brings its
+// own 16-byte pieces, reads them back for the statistics and for the output, and sends for those of the next tile.  The CTAs of an SM are in different
+// phases of this, so that the memory system does not wait for an exchange of sums.  Rows on 16-byte boundaries.
+template <typename T>
+__device__ __forceinline__ void fetch_rows(uint8_t *to, int piece, const T *from, long long distance, int rows)
+{
+    to += threadIdx.x * 16;
+#pragma unroll 4
+    for (int i = 0; i < rows; ++i, to += piece, from += distance) cp_async16(to, from, true);
+}
+
+template <typename T, int LPR>
+__global__ void __launch_bounds__(kColumnThreads, 4)
+k_layer_norm_once(const T *x, T *y, const float *__restrict__ gamma, const float *__restrict__ beta, float *mean_out, float *rstd_out, float eps, int N, int F,
+                  long long xs, long long ys, int rows, int tiles, int *fault)
+{
+    grid_dependency();
+    using Col = Column<T, LPR>;
+    constexpr int kVec = Col::kVec, kCols = Col::kCols;
+    extern __shared__ __align__(16) uint8_t buffer[];
+    __shared__ Exchange<1, kCols> sums[2];
+    __shared__ int gave_up;
+    const Col c;
+    Cluster cl(&gave_up);
+    const int clusters = (int)(gridDim.x / cl.size), cta_first = (int)cl.rank * c.step * rows, first = cta_first + c.row, piece = blockDim.x * 16;
+    const int mine = min(rows, (N - first + c.step - 1) / c.step);         // rows of this thread that exist (none: 0 or less)
+    float2 *const gain = reinterpret_cast<float2 *>(buffer + rows * piece);
+    const uint8_t *const at = buffer + threadIdx.x * 16;
+    const long long x_step = c.step * xs, y_step = c.step * ys;
+    const T *const x_first = x + first * xs;
+    int tile = (int)(blockIdx.x / cl.size), f = tile * kCols + c.col;
+    uint32_t phase = 0;
+    if (f < F) fetch_rows(buffer, piece, x_first + f, x_step, mine);
+    for (int i = threadIdx.x; i < c.step * rows; i += blockDim.x)
+        gain[i] = cta_first + i < N ? make_float2(gamma ? gamma[cta_first + i] : 1.0f, beta ? beta[cta_first + i] : 0.0f) : make_float2(0.0f, 0.0f);
+    cl.meet(sums, 2);
+    const float inv = 1.0f / (float)N;
+    for (; tile < tiles; tile += clusters, f += clusters * kCols, phase ^= 1) {
+        cp_async_commit();
+        cp_async_wait<0>();
+        float mean[1][kVec] = {}, rstd[1][kVec] = {};
+        {
+            const uint8_t *p = at;
+#pragma unroll 4
+            for (int i = 0; i < mine; ++i, p += piece) {
+                float v[kVec];
+                unpack<T>(*reinterpret_cast<const uint4 *>(p), v);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) mean[0][j] += v[j];
+            }
+        }
+        join_columns<ColumnSum, 1, T, LPR>(mean, c, sums[0], cl, phase, [&](int, float s) { return s * inv; });
+        {
+            const uint8_t *p = at;
+#pragma unroll 4
+            for (int i = 0; i < mine; ++i, p += piece) {
+                float v[kVec];
+                unpack<T>(*reinterpret_cast<const uint4 *>(p), v);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) { v[j] -= mean[0][j]; rstd[0][j] = fmaf(v[j], v[j], rstd[0][j]); }
+            }
+        }
+        join_columns<ColumnSum, 1, T, LPR>(rstd, c, sums[1], cl, phase, [&](int, float s) { return 1.0f / sqrtf(fmaf(s, inv, eps)); });
+        if (cl.rank == 0 && c.row == 0) {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+                if (f + j < F) { mean_out[f + j] = mean[0][j]; rstd_out[f + j] = rstd[0][j]; }
+        }
+        const uint8_t *p = at;
+        const float2 *g = gain + c.row;
+        T *out = y + first * ys;
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i, p += piece, g += c.step, out += y_step) {
+            const float2 gb = *g;
+            float v[kVec];
+            unpack<T>(*reinterpret_cast<const uint4 *>(p), v);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) v[j] = fmaf((v[j] - mean[0][j]) * rstd[0][j], gb.x, gb.y);
+            store_frames<T, true>(out, f, F, v);
+        }
+        if (f + clusters * kCols < F) fetch_rows(buffer, piece, x_first + f + clusters * kCols, x_step, mine);
+    }
+    cl.leave(fault);
+}
+
+// R rows a thread at most; the sums over the frames of a node stay in registers on the way: grad_part[cluster][node] = (sum dy xh, sum dy)
+template <typename T, int LPR, int R>
+__global__ void __launch_bounds__(kColumnThreads, sizeof(T) == 4 ? 4 : 3)
+k_layer_norm_grad_once(const T *x, const T *dy, T *dx, const float *__restrict__ gamma, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
+                       float2 *grad_part, int N, int F, long long xs, long long dys, long long dxs, int rows, int tiles, int *fault)
+{
+    grid_dependency();
+    using Col = Column<T, LPR>;
+    constexpr int kVec = Col::kVec, kCols = Col::kCols;
+    extern __shared__ __align__(16) uint8_t buffer[];
+    __shared__ Exchange<2, kCols> sums[2];
+    __shared__ int gave_up;
+    const Col c;
+    Cluster cl(&gave_up);
+    const int cluster = (int)(blockIdx.x / cl.size), clusters = (int)(gridDim.x / cl.size), first = (int)cl.rank * c.step * rows + c.row, piece = blockDim.x * 16;
+    const int mine = min(rows, (N - first + c.step - 1) / c.step), half = rows * piece;
+    float *const gain = reinterpret_cast<float *>(buffer + 2 * half);
+    const uint8_t *const at = buffer + threadIdx.x * 16;
+    const float inv = 1.0f / (float)N;
+    const long long x_step = c.step * xs, dy_step = c.step * dys, dx_step = c.step * dxs;
+    const T *const x_first = x + first * xs, *const dy_first = dy + first * dys;
+    int tile = cluster, f = tile * kCols + c.col;
+    if (f < F) {
+        fetch_rows(buffer, piece, x_first + f, x_step, mine);
+        fetch_rows(buffer + half, piece, dy_first + f, dy_step, mine);
+    }
+    for (int i = threadIdx.x; i < c.step * rows; i += blockDim.x) gain[i] = gamma && first - c.row + i < N ? gamma[first - c.row + i] : 1.0f;
+    float ag[R] = {}, ab[R] = {};
+    __syncthreads();
+    cl.meet(sums, 2);
+    uint32_t turn = 0;                                                    // the exchange is its lowest bit, the phase the next
+    for (; tile < tiles; tile += clusters, f += clusters * kCols, ++turn) {
+        cp_async_commit();
+        float mean[kVec], rstd[kVec], s[2][kVec] = {};
+        load_columns(mean_in, f, F, mean);
+        load_columns(rstd_in, f, F, rstd);
+        cp_async_wait<0>();
+        if (f < F && f + kVec > F) {                                      // what lies beyond the frames may be anything
+            for (int i = 0; i < mine; ++i)
+#pragma unroll
+                for (int j = 0; j < kVec; ++j)
+                    if (f + j >= F) {
+                        reinterpret_cast<T *>(buffer + threadIdx.x * 16 + i * piece)[j] = from_float<T>(0.0f);
+                        reinterpret_cast<T *>(buffer + threadIdx.x * 16 + half + i * piece)[j] = from_float<T>(0.0f);
+                    }
+        }
+        if (f < F) {
+            const uint8_t *p = at;
+            const float *g = gain + c.row;
+#pragma unroll
+            for (int i = 0; i < R; ++i, p += piece, g += c.step) {
+                if (i >= mine) break;
+                const float gm = *g;
+                float xv[kVec], gv[kVec];
+                unpack<T>(*reinterpret_cast<const uint4 *>(p), xv);
+                unpack<T>(*reinterpret_cast<const uint4 *>(p + half), gv);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) {
+                    const float d = xv[j] - mean[j], t = gm * gv[j];
+                    ag[i] = fmaf(gv[j], d * rstd[j], ag[i]);
+                    ab[i] += gv[j];
+                    s[0][j] += t;
+                    s[1][j] = fmaf(t, d, s[1][j]);
+                }
+            }
+        }
+        join_columns<ColumnSum, 2, T, LPR>(s, c, sums[turn & 1], cl, turn >> 1 & 1, [&](int, float v) { return v * inv; });
+        // dx = (gamma rstd) dy + k1 + k2 (x - mean)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) { s[0][j] *= -rstd[j]; s[1][j] *= -rstd[j] * rstd[j] * rstd[j]; }
+        if (f < F) {
+            const uint8_t *p = at;
+            const float *g = gain + c.row;
+            T *out = dx + first * dxs;
+#pragma unroll
+            for (int i = 0; i < R; ++i, p += piece, g += c.step, out += dx_step) {
+                if (i >= mine) break;
+                const float gm = *g;
+                float xv[kVec], gv[kVec];
+                unpack<T>(*reinterpret_cast<const uint4 *>(p), xv);
+                unpack<T>(*reinterpret_cast<const uint4 *>(p + half), gv);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) gv[j] = fmaf(gv[j], gm * rstd[j], fmaf(xv[j] - mean[j], s[1][j], s[0][j]));
+                store_frames<T, true>(out, f, F, gv);
+            }
+        }
+        if (f + clusters * kCols < F) {
+            fetch_rows(buffer, piece, x_first + f + clusters * kCols, x_step, mine);
+            fetch_rows(buffer + half, piece, dy_first + f + clusters * kCols, dy_step, mine);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int n = first + i * c.step;
+#pragma unroll
+        for (int m = 1; m < LPR; m <<= 1) {
+            ag[i] += __shfl_xor_sync(0xffffffffu, ag[i], m);
+            ab[i] += __shfl_xor_sync(0xffffffffu, ab[i], m);
+        }
+        if (i < mine && c.lane % LPR == 0) grad_part[(long long)cluster * N + n] = make_float2(ag[i], ab[i]);
+    }
+    cl.leave(fault);
 }
 
 // dgamma, dbeta (either may be absent) = or += the sums of the parts, 8 parts side by side and in a fixed order
@@ -291,15 +482,50 @@ __global__ void __launch_bounds__(256) k_layer_norm_no_frames(float *dgamma, flo
     if (n < N && dbeta) dbeta[n] = 0.0f;
 }
 
-// rows of a chunk so that about four CTAs an SM are there, a multiple of 64
-static int chunk_of(int N, long long tiles)
+// CTAs that share a column tile of the statistics: about eight CTAs an SM, and a round of rows for each
+static unsigned stats_cluster(int N, long long tiles)
 {
-    const long long want = 4LL * device_info().sm_count;
-    long long chunks = (want + tiles - 1) / tiles;
-    long long rows = ((N + chunks - 1) / chunks + 63) / 64 * 64;
-    if (rows < 64) rows = 64;
-    while ((N + rows - 1) / rows > 65535) rows *= 2;
-    return (int)rows;
+    unsigned cl = 1;
+    while (cl < (unsigned)kMostCluster && tiles * cl <= 4LL * device_info().sm_count && N > 32 * 8 * (int)cl) cl *= 2;
+    return cl;
+}
+
+constexpr int kNormRows = 16, kNormGradRows = 8;         // rows a thread where everything is read once, at most
+constexpr int kNormSmem = kColumnThreads * kNormRows * 16 + kColumnThreads / 2 * kNormRows * (int)sizeof(float2);    // of either direction
+
+template <typename T, int LPR>
+static int layer_norm_once(const T *x, T *y, const float *gamma, const float *beta, float *mean, float *rstd, float eps, int N, int F, long long xs,
+                           long long ys, const ColumnPlan &p, cudaStream_t st)
+{
+    constexpr int kCols = Column<T, LPR>::kCols;
+    int *fault = fault_word();
+    BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
+    auto kernel = k_layer_norm_once<T, LPR>;
+    const int threads = 32 * p.warps, smem = p.rows * threads * 16 + p.rows * p.warps * (32 / LPR) * (int)sizeof(float2), tiles = (F + kCols - 1) / kCols;
+    BB200_REQUIRE(allow_big_smem(kernel, kNormSmem), (int)cudaErrorInvalidValue);
+    const int clusters = std::min(tiles, resident_clusters(reinterpret_cast<const void *>(kernel), p.cluster, threads, smem));
+    return launch_cluster(kernel, (unsigned)p.cluster, (unsigned)(clusters * p.cluster), threads, smem, st, x, y, gamma, beta, mean, rstd, eps, N, F, xs, ys, p.rows,
+                          tiles, fault);
+}
+
+template <typename T, int LPR, int R>
+static int layer_norm_grad_once(const T *x, const T *dy, T *dx, const float *gamma, const float *mean, const float *rstd, float *dgamma, float *dbeta,
+                                int accumulate, int N, int F, long long xs, long long dys, long long dxs, const ColumnPlan &p, cudaStream_t st)
+{
+    constexpr int kCols = Column<T, LPR>::kCols;
+    int *fault = fault_word();
+    BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
+    auto kernel = k_layer_norm_grad_once<T, LPR, R>;
+    const int threads = 32 * p.warps, smem = 2 * p.rows * threads * 16 + p.rows * p.warps * (32 / LPR) * (int)sizeof(float), tiles = (F + kCols - 1) / kCols;
+    BB200_REQUIRE(allow_big_smem(kernel, kNormSmem), (int)cudaErrorInvalidValue);
+    const int clusters = std::min(tiles, resident_clusters(reinterpret_cast<const void *>(kernel), p.cluster, threads, smem));
+    float2 *part = static_cast<float2 *>(stream_scratch(st, (size_t)clusters * N * sizeof(float2), kFrameOpSlot));
+    BB200_REQUIRE(part != nullptr, BBCU_ERR_NO_MEMORY);
+    const int e = launch_cluster(kernel, (unsigned)p.cluster, (unsigned)(clusters * p.cluster), threads, smem, st, x, dy, dx, gamma, mean, rstd, part, N, F, xs, dys,
+                                 dxs, p.rows, tiles, fault);
+    if (e != BBCU_OK) return e;
+    if (dgamma || dbeta) launch(k_layer_norm_grad_weights, (unsigned)((N + 31) / 32), 256, 0, st, part, dgamma, dbeta, N, clusters, accumulate);
+    return launch_status();
 }
 
 template <typename T>
@@ -307,17 +533,17 @@ static int layer_norm_forward(const T *x, T *y, const float *gamma, const float 
                               long long ys, cudaStream_t st)
 {
     const bool aligned = frames_aligned<T>(x, xs) && frames_aligned<T>(y, ys);
-    constexpr int kCols = Column<T, 8>::kCols;
-    const long long tiles = ((long long)F + kCols - 1) / kCols;
-    BB200_REQUIRE(tiles * kCols < (1LL << 31), BBCU_ERR_TOO_LARGE);
-    const int columns = (int)(tiles * kCols), rows = chunk_of(N, tiles), chunks = (N + rows - 1) / rows;
-    double2 *part = static_cast<double2 *>(stream_scratch(st, (size_t)chunks * columns * sizeof(double2), kFrameOpSlot));
-    BB200_REQUIRE(part != nullptr, BBCU_ERR_NO_MEMORY);
-    const dim3 grid((unsigned)tiles, (unsigned)chunks);
-    launch(aligned ? k_layer_norm_stats<T, true> : k_layer_norm_stats<T, false>, grid, kNormThreads, 0, st, x, part, N, F, xs, rows, columns);
-    BB200_CUDA(cudaPeekAtLastError());
-    launch(aligned ? k_layer_norm_apply<T, true> : k_layer_norm_apply<T, false>, grid, kNormThreads, 0, st, x, y, part, gamma, beta, mean, rstd, eps, N, F,
-           xs, ys, rows, chunks, columns);
+    BB200_REQUIRE(F <= (1 << 30), BBCU_ERR_TOO_LARGE);
+    if (const ColumnPlan p = plan_columns<T>(N, F, sizeof(T) == 4 ? 8 : 4, kNormRows); aligned && p.cluster)
+        return (p.lanes == 2 ? layer_norm_once<T, 2> : layer_norm_once<T, sizeof(T) == 4 ? 8 : 4>)(x, y, gamma, beta, mean, rstd, eps, N, F, xs, ys, p, st);
+    constexpr int kCols = Column<T, 8>::kCols, kWide = 32 * kFramesPerVec<T>;
+    const long long tiles = ((long long)F + kCols - 1) / kCols, bands = ((long long)N + 8 * kApplyRows - 1) / (8 * kApplyRows);
+    BB200_REQUIRE(bands <= 65535, BBCU_ERR_TOO_LARGE);
+    const unsigned cl = stats_cluster(N, tiles);
+    if (const int e = launch_cluster(aligned ? k_layer_norm_stats<T, true> : k_layer_norm_stats<T, false>, cl, (unsigned)(tiles * cl), kNormThreads, 0, st, x, mean, rstd,
+                                     eps, N, F, xs)) return e;
+    launch(aligned ? k_layer_norm_apply<T, true> : k_layer_norm_apply<T, false>, dim3((unsigned)((F + kWide - 1) / kWide), (unsigned)bands), kNormThreads, 0, st, x, y, gamma,
+           beta, mean, rstd, N, F, xs, ys);
     return launch_status();
 }
 
@@ -326,23 +552,29 @@ static int layer_norm_backward(const T *x, const T *dy, T *dx, const float *gamm
                                int accumulate, int N, int F, long long xs, long long dys, long long dxs, cudaStream_t st)
 {
     const bool aligned = frames_aligned<T>(x, xs) && frames_aligned<T>(dy, dys) && frames_aligned<T>(dx, dxs);
-    constexpr int kCols = Column<T, 8>::kCols, kRows = 4, kPerCta = kNormThreads / 32 * 4 * kRows;
-    const long long tiles = ((long long)F + kCols - 1) / kCols;
-    BB200_REQUIRE(tiles * kCols < (1LL << 31), BBCU_ERR_TOO_LARGE);
-    const int columns = (int)(tiles * kCols), rows = chunk_of(N, tiles), chunks = (N + rows - 1) / rows;
-    const int row_ctas = (N + kPerCta - 1) / kPerCta;
-    BB200_REQUIRE(row_ctas <= 65535, BBCU_ERR_TOO_LARGE);
-    long long sweeps = (4LL * device_info().sm_count + row_ctas - 1) / row_ctas;
-    if (sweeps > tiles) sweeps = tiles;
-    const size_t part_bytes = (size_t)chunks * columns * sizeof(float2);
-    char *scratch = static_cast<char *>(stream_scratch(st, part_bytes + (size_t)sweeps * N * sizeof(float2), kFrameOpSlot));
+    BB200_REQUIRE(F <= (1 << 30), BBCU_ERR_TOO_LARGE);
+    const bool wide = N <= 8 * kColumnThreads / 8 * 4;                    // 128 bytes of a row and four rows a thread in clusters of up to 8, or 64 and eight
+    if (const ColumnPlan p = plan_columns<T>(N, F, wide ? 8 : 4, wide ? 4 : kNormGradRows); aligned && p.cluster) {
+#define BB200_ONCE(L) (p.rows <= 4 ? layer_norm_grad_once<T, L, 4> : layer_norm_grad_once<T, L, kNormGradRows>)
+        return (p.lanes == 2 ? BB200_ONCE(2) : p.lanes == 4 ? BB200_ONCE(4) : layer_norm_grad_once<T, 8, 4>)(x, dy, dx, gamma, mean, rstd, dgamma, dbeta, accumulate, N,
+                                                                                                        F, xs, dys, dxs, p, st);
+#undef BB200_ONCE
+    }
+    constexpr int kCols = Column<T, 8>::kCols, kWide = 32 * kFramesPerVec<T>, kRows = 4;
+    const long long tiles = ((long long)F + kCols - 1) / kCols, bands = ((long long)N + 8 * kRows - 1) / (8 * kRows), pieces = ((long long)F + kWide - 1) / kWide;
+    BB200_REQUIRE(bands <= 65535, BBCU_ERR_TOO_LARGE);
+    long long sweeps = std::min(pieces, std::max(1LL, (8LL * device_info().sm_count + bands - 1) / bands));
+    const int padded = (F + 3) / 4 * 4;
+    const size_t sums_bytes = (size_t)padded * sizeof(float2);
+    char *scratch = static_cast<char *>(stream_scratch(st, sums_bytes + (size_t)sweeps * N * sizeof(float2), kFrameOpSlot));
     BB200_REQUIRE(scratch != nullptr, BBCU_ERR_NO_MEMORY);
-    float2 *part = reinterpret_cast<float2 *>(scratch), *grad_part = reinterpret_cast<float2 *>(scratch + part_bytes);
-    launch(aligned ? k_layer_norm_grad_stats<T, true> : k_layer_norm_grad_stats<T, false>, dim3((unsigned)tiles, (unsigned)chunks), kNormThreads, 0, st, x, dy,
-           gamma, mean, rstd, part, N, F, xs, dys, rows, columns);
-    BB200_CUDA(cudaPeekAtLastError());
-    launch(aligned ? k_layer_norm_grad_apply<T, kRows, true> : k_layer_norm_grad_apply<T, kRows, false>, dim3((unsigned)sweeps, (unsigned)row_ctas), kNormThreads,
-           0, st, x, dy, dx, part, gamma, mean, rstd, grad_part, N, F, xs, dys, dxs, chunks, columns);
+    float *sums = reinterpret_cast<float *>(scratch);
+    float2 *grad_part = reinterpret_cast<float2 *>(scratch + sums_bytes);
+    const unsigned cl = stats_cluster(N, tiles);
+    if (const int e = launch_cluster(aligned ? k_layer_norm_grad_stats<T, true> : k_layer_norm_grad_stats<T, false>, cl, (unsigned)(tiles * cl), kNormThreads, 0, st, x, dy,
+                                     gamma, mean, rstd, sums, padded, N, F, xs, dys)) return e;
+    launch(aligned ? k_layer_norm_grad_apply<T, kRows, true> : k_layer_norm_grad_apply<T, kRows, false>, dim3((unsigned)sweeps, (unsigned)bands), kNormThreads, 0, st, x, dy,
+           dx, sums, padded, gamma, mean, rstd, grad_part, N, F, xs, dys, dxs);
     BB200_CUDA(cudaPeekAtLastError());
     if (dgamma || dbeta) launch(k_layer_norm_grad_weights, (unsigned)((N + 31) / 32), 256, 0, st, grad_part, dgamma, dbeta, N, (int)sweeps, accumulate);
     return launch_status();
@@ -373,11 +605,6 @@ static int layer_norm_backward_checked(const T *x, const T *dy, T *dx, const flo
     }
     BB200_REQUIRE_PTR(x); BB200_REQUIRE_PTR(dy); BB200_REQUIRE_PTR(dx); BB200_REQUIRE_PTR(mean); BB200_REQUIRE_PTR(rstd);
     return layer_norm_backward<T>(x, dy, dx, gamma, mean, rstd, dgamma, dbeta, accumulate, N, F, xs, dys, dxs, as_stream(stream));
-}
-
-bool allow_cluster_16_once(const void *kernel)
-{
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
 }
 
 }   // namespace bb200

@@ -14,6 +14,7 @@
 #include <atomic>
 #include <map>
 #include <mutex>
+#include <tuple>
 #include <unordered_map>
 #include <vector>
 
@@ -99,6 +100,54 @@ bool allow_big_smem_once(const void *kernel, int bytes)
     std::lock_guard<std::mutex> g(mu);
     done[key] = bytes;
     return true;
+}
+
+bool allow_cluster_16_once(const void *kernel)
+{
+    static std::mutex mu;
+    static std::map<std::pair<int, const void *>, bool> done;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> g(mu);
+    auto it = done.find({dev, kernel});
+    if (it == done.end()) {
+        const bool ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+        if (!ok) { cudaGetLastError(); return false; }
+        it = done.emplace(std::make_pair(dev, kernel), ok).first;
+    }
+    return it->second;
+}
+
+int resident_clusters(const void *kernel, int cluster, int threads, size_t smem)
+{
+    static std::mutex mu;
+    static std::map<std::tuple<int, const void *, int, int, size_t>, int> known;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const auto key = std::make_tuple(dev, kernel, cluster, threads, smem);
+    std::lock_guard<std::mutex> g(mu);
+    auto it = known.find(key);
+    if (it == known.end()) {
+        if (cluster > 8) allow_cluster_16_once(kernel);
+        int n = 0;
+        cudaError_t e;
+        if (cluster > 1) {
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = (unsigned)cluster;
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)cluster); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem;
+            cfg.attrs = &attr; cfg.numAttrs = 1;
+            e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+        } else {
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem);
+            n *= device_info().sm_count;
+        }
+        if (e != cudaSuccess) cudaGetLastError();
+        it = known.emplace(key, e == cudaSuccess && n > 0 ? n : 1).first;
+    }
+    return it->second;
 }
 
 int frame_tile(long long rows_touched, int bits_per_row_frame, int node_groups, int frame_size, int max_tile)
