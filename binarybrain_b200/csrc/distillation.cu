@@ -8,13 +8,37 @@
 //   loss = T^2 sum_k p_k (log p_k - log q_{i_k}),      dz_c = T (P q_c - sum_{k: i_k = c} p_k),  P = sum_k p_k
 //
 // both times the frame's weight; a slot with p_k = 0 adds nothing, whatever its class's log q is, and a class that is named twice gets both.  A frame
-// without a slot, or of weight 0, has loss 0 and gradient 0 whatever its logits are.  exp(z / T) is evaluated as exp2((z - max z) log2(e) / T).
+// without a slot, or of weight 0, has loss 0 and gradient 0 whatever its logits are.
+// exp(z / T) is evaluated as exp2((z - max z) log2(e) / T).
+#include <type_traits>
+
 #include "frame_columns.cuh"
 
 namespace bb200 {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kDistillThreads = 256;
+constexpr int kMostSlots = 512;                          // of the teacher, a column of them in shared memory
+constexpr int kDistillRows = 16, kDistillCluster = 4;    // rows a thread and CTAs a cluster where everything is read once, at most
+
+template <typename T> struct Distill {
+    const T *z, *t;
+    T *dz;
+    const int *index;
+    const float *t_lse, *weight;
+    float *loss_buf;
+    double *loss_part;                                   // [column tile]
+    float temperature, inv_t, scale, grad_reduction;     // scale = log2(e) / T
+    int C, K, F;
+    long long zs, dzs, ts, is;
+};
+
+// 2^x to 2^-22 of it, 0 below the normal numbers
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // maximum and sum of exponentials relative to it, of two sets joined; an empty set, and one of -inf alone, is (-inf, 0)
 struct SoftSum { float top, sum; };
@@ -22,243 +46,598 @@ __device__ __forceinline__ SoftSum join_soft(const SoftSum &a, const SoftSum &b,
 {
     const float top = fmaxf(a.top, b.top);
     if (top == -INFINITY) return {top, a.sum + b.sum};                    // (a NaN among them stays)
-    return {top, a.sum * exp2f((a.top - top) * scale) + b.sum * exp2f((b.top - top) * scale)};
+    return {top, a.sum * exp2_fast((a.top - top) * scale) + b.sum * exp2_fast((b.top - top) * scale)};
+}
+// what exponents are taken relative to: with no class left, anything finite
+__device__ __forceinline__ float reference(float top) { return top == -INFINITY ? 0.0f : top; }
+
+// How a frame's softmax becomes its gradient: dz = factor * min(exp2((z - top) scale), cap), minus `slope` times the teacher's probability where the
+// class is named.  A frame that takes no part has factor, cap and slope 0, and min() gives the cap for a NaN; elsewhere the cap is infinite, and a NaN
+// among the logits has made the factor one.
+struct FrameGrad { float top, factor, cap, slope; };
+__device__ __forceinline__ float soft_part(const FrameGrad &g, float z, float scale) { return g.factor * fminf(exp2_fast((z - g.top) * scale), g.cap); }
+
+// the larger of each pair of 16 bytes of logits, a NaN being the smaller
+template <typename T> __device__ __forceinline__ uint4 packed_max(const uint4 &a, const uint4 &b);
+template <> __device__ __forceinline__ uint4 packed_max<float>(const uint4 &a, const uint4 &b)
+{
+    return make_uint4(__float_as_uint(fmaxf(__uint_as_float(a.x), __uint_as_float(b.x))), __float_as_uint(fmaxf(__uint_as_float(a.y), __uint_as_float(b.y))),
+                      __float_as_uint(fmaxf(__uint_as_float(a.z), __uint_as_float(b.z))), __float_as_uint(fmaxf(__uint_as_float(a.w), __uint_as_float(b.w))));
+}
+template <> __device__ __forceinline__ uint4 packed_max<__nv_bfloat16>(const uint4 &a, const uint4 &b)
+{
+    uint4 r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r.x) : "r"(a.x), "r"(b.x));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r.y) : "r"(a.y), "r"(b.y));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r.z) : "r"(a.z), "r"(b.z));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r.w) : "r"(a.w), "r"(b.w));
+    return r;
 }
 
-// part[chunk][column] of the student's logits
-template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kDistillThreads)
-k_distill_stats(const T *z, SoftSum *part, float scale, int C, int F, long long zs, int chunk_rows, int columns)
+// ---- the teacher's side of COLS frames from f0 on, by a CTA of a multiple of COLS threads: thread t has column t % COLS and every (threads / COLS)-th
+// slot of it.  index[slot][column] (-1: empty) and p[slot][column] go to shared memory, and to each thread, for its column, P = sum p, E = sum p log p
+// and the weight (0: the frame takes no part).  A barrier stands behind the last write.
+struct TeacherColumn { float P, E, weight; };
+template <typename T, int COLS>
+__device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, int f0, int *index, float *p, float (&red)[2][kColumnThreads])
+{
+    const int col = threadIdx.x % COLS, group = threadIdx.x / COLS, groups = blockDim.x / COLS, f = f0 + col;
+    const float w = f < a.F ? (a.weight ? a.weight[f] : 1.0f) : 0.0f;
+    float top = -INFINITY, slots = 0.0f;
+    for (int k = group; k < a.K; k += groups) {
+        int i = -1;
+        float t = -INFINITY;
+        if (f < a.F) {
+            i = a.index[k * a.is + f];
+            t = to_float(a.t[k * a.ts + f]);
+            if (i < 0 || i >= a.C || t == -INFINITY) i = -1;
+        }
+        index[k * COLS + col] = i;
+        p[k * COLS + col] = t;
+        if (i >= 0) { top = fmaxf(top, t); slots += 1.0f; }
+    }
+    red[0][threadIdx.x] = top;
+    red[1][threadIdx.x] = slots;
+    __syncthreads();
+    top = -INFINITY;
+    slots = 0.0f;
+    for (int e = col; e < (int)blockDim.x; e += COLS) { top = fmaxf(top, red[0][e]); slots += red[1][e]; }
+    const bool live = slots > 0.0f && w != 0.0f;
+    float lse = 0.0f;
+    if (a.t_lse) {
+        if (live) lse = a.t_lse[f];
+        __syncthreads();
+    } else {
+        float sum = 0.0f;
+        for (int k = group; k < a.K; k += groups)
+            if (index[k * COLS + col] >= 0) sum += exp2_fast((p[k * COLS + col] - top) * a.scale);
+        __syncthreads();
+        red[0][threadIdx.x] = sum;
+        __syncthreads();
+        sum = 0.0f;
+        for (int e = col; e < (int)blockDim.x; e += COLS) sum += red[0][e];
+        lse = top * a.inv_t + logf(sum);
+        __syncthreads();
+    }
+    float P = 0.0f, E = 0.0f;
+    for (int k = group; k < a.K; k += groups) {
+        float q = 0.0f;
+        if (live && index[k * COLS + col] >= 0) {
+            const float log_p = p[k * COLS + col] * a.inv_t - lse;
+            q = exp2_fast(log_p * kLog2e);
+            if (q != 0.0f) E += q * log_p;
+            P += q;
+        }
+        p[k * COLS + col] = q;
+    }
+    red[0][threadIdx.x] = P;
+    red[1][threadIdx.x] = E;
+    __syncthreads();
+    TeacherColumn c = {0.0f, 0.0f, live ? w : 0.0f};
+    for (int e = col; e < (int)blockDim.x; e += COLS) { c.P += red[0][e]; c.E += red[1][e]; }
+    __syncthreads();
+    return c;
+}
+
+// The probabilities of all slots of the column that name the class of slot k, in the order of the slots; `first`: k is the first of them.
+template <int COLS> __device__ __forceinline__ float named_slots(const int *index, const float *p, int K, int k, int col, bool &first)
+{
+    const int i = index[k * COLS + col];
+    float sum = 0.0f;
+    first = true;
+    for (int e = 0; e < K; ++e)
+        if (index[e * COLS + col] == i) {
+            first = first && e >= k;
+            sum += p[e * COLS + col];
+        }
+    return sum;
+}
+
+// From a frame's joined parts (cross = sum p (z - top) / T over the named classes) its gradient's factors and its loss.
+template <typename T>
+__device__ __forceinline__ FrameGrad finish_frame(const Distill<T> &a, const TeacherColumn &c, const SoftSum &s, float cross, float &loss)
+{
+    loss = 0.0f;
+    if (c.weight == 0.0f) return {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool none = s.top == -INFINITY && s.sum == 0.0f;                // no class is left: cross is -inf, the loss infinite, q = 0
+    const float slope = a.grad_reduction * c.weight * a.temperature;
+    loss = c.weight * a.temperature * a.temperature * (c.E - cross + (none ? 0.0f : c.P * logf(s.sum)));
+    return {reference(s.top), none ? 0.0f : slope * c.P / s.sum, INFINITY, slope};
+}
+
+// loss_buf of the first warp's columns, and their sum
+template <typename T> __device__ __forceinline__ void write_losses(const Distill<T> &a, int tile, int f, bool has, float loss)
+{
+    if (has) a.loss_buf[f] = loss;
+    double sum = has ? (double)loss : 0.0;
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    if (threadIdx.x == 0) a.loss_part[tile] = sum;
+}
+
+// ---- everything read once, as far as a cluster holds the classes of a column tile in shared memory (see layer_norm.cu for the walk over the tiles).  Each
+// CTA reduces its classes to four numbers a frame, relative to its own largest logit m: m, sum exp((z - m) / T), and sum p (z - m) / T and sum p over
+// the slots that name one of its classes; one exchange joins them.
+template <typename T, int LPR>
+__global__ void __launch_bounds__(kColumnThreads, 3)
+k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
 {
     grid_dependency();
-    constexpr int kLpr = 8, kBatch = 8;
-    using Col = Column<T, kLpr>;
+    using Col = Column<T, LPR>;
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
-    __shared__ SoftSum s[8][kCols];
+    static_assert(kCols <= 32, "a warp finishes the columns");
+    extern __shared__ __align__(16) uint8_t buffer[];
+    __shared__ float red[2][kColumnThreads], red_soft[kColumnThreads / 32][kCols], s_top[kCols];
+    __shared__ float part[2][kDistillCluster][4][kCols];
+    __shared__ FrameGrad s_grad[kCols];
+    __shared__ uint64_t bar[2];
+    __shared__ int gave_up;
     const Col c;
-    const int f = (int)blockIdx.x * kCols + c.col;
-    const int n0 = (int)blockIdx.y * chunk_rows, n1 = min(C, n0 + chunk_rows);
-    SoftSum a[kVec];
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) a[j] = {-INFINITY, 0.0f};
-    for (int n = n0 + c.row; n < n1; n += c.step * kBatch) {
-        uint4 raw[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int m = n + i * c.step;
-            if (m < n1) raw[i] = load_frames<T, ALIGNED>(z + (long long)m * zs, f, F);
+    const uint32_t cl = cluster_size(), rank = cluster_rank();
+    const int clusters = (int)(gridDim.x / cl), cta_first = (int)rank * c.step * rows, first = cta_first + c.row, piece = blockDim.x * 16;
+    const int mine = min(rows, (a.C - first + c.step - 1) / c.step), cta_rows = min(c.step * rows, a.C - cta_first);
+    const uint8_t *const at = buffer + threadIdx.x * 16;
+    const int shift = 31 - __clz(c.step);                                 // the warps are a power of two
+    int *const index = reinterpret_cast<int *>(buffer + rows * piece);
+    float *const p = reinterpret_cast<float *>(index + a.K * kCols);
+    unsigned *const seen = reinterpret_cast<unsigned *>(p + a.K * kCols);   // a bit for each of the CTA's classes and columns: has a slot named it?
+    for (int i = threadIdx.x; i < (c.step * rows + 31) / 32 * kCols; i += blockDim.x) seen[i] = 0u;
+    const long long z_step = c.step * a.zs, dz_step = c.step * a.dzs;
+    const T *const z_first = a.z + first * a.zs;
+    // the logit of a class of this CTA in a column of the tile
+    auto logit = [&](int i, int col) {
+        const int local = i - cta_first, in = local & (c.step - 1);
+        return to_float(reinterpret_cast<const T *>(buffer + (local >> shift) * piece + (in * LPR + col / kVec) * 16)[col % kVec]);
+    };
+    auto fetch = [&](int f) {
+        if (f >= a.F) return;
+        uint8_t *to = buffer + threadIdx.x * 16;
+        const T *from = z_first + f;
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i, to += piece, from += z_step) cp_async16(to, from, true);
+    };
+    int tile = (int)(blockIdx.x / cl), f = tile * kCols + c.col;
+    fetch(f);
+    if (cl > 1) {
+        if (threadIdx.x == 0) {
+            gave_up = 0;
+            mbar_init(&bar[0], 1);
+            mbar_init(&bar[1], 1);
+            mbar_init_fence();
         }
-        float top[kVec];
+        cluster_arrive();
+        cluster_wait();
+    }
+    const int my_col = threadIdx.x % kCols, group = threadIdx.x / kCols, groups = blockDim.x / kCols;
+    for (uint32_t turn = 0; tile < tiles; tile += clusters, f += clusters * kCols, ++turn) {
+        cp_async_commit();
+        const TeacherColumn teacher = teacher_columns<T, kCols>(a, tile * kCols, index, p, red);
+        cp_async_wait<0>();
+        float v[kVec], m[kVec], sum[kVec] = {};
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) top[j] = a[j].top;
+        for (int j = 0; j < kVec; ++j) m[j] = -INFINITY;
+        {
+            const uint8_t *q = at;
+#pragma unroll 4
+            for (int i = 0; i < mine; ++i, q += piece) {
+                unpack<T>(*reinterpret_cast<const uint4 *>(q), v);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            if (n + i * c.step < n1) {
-                float v[kVec];
-                unpack<T>(raw[i], v);
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) top[j] = fmaxf(top[j], v[j]);
+                for (int j = 0; j < kVec; ++j) m[j] = fmaxf(m[j], v[j]);
             }
         }
+#pragma unroll
+        for (int d = LPR; d < 32; d <<= 1)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) m[j] = fmaxf(m[j], __shfl_xor_sync(0xffffffffu, m[j], d));
+        if (c.lane < LPR) {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) red_soft[c.warp][c.col + j] = m[j];
+        }
+        __syncthreads();                                                  // (the logits of the other threads are there, too)
+        if (threadIdx.x < kCols) {
+            float t = red_soft[0][threadIdx.x];
+            for (int w = 1; w < c.warps; ++w) t = fmaxf(t, red_soft[w][threadIdx.x]);
+            s_top[threadIdx.x] = t;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) m[j] = reference(s_top[c.col + j]);
+        {
+            const uint8_t *q = at;
+#pragma unroll 4
+            for (int i = 0; i < mine; ++i, q += piece) {
+                unpack<T>(*reinterpret_cast<const uint4 *>(q), v);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) sum[j] += exp2_fast((v[j] - m[j]) * a.scale);
+            }
+        }
+#pragma unroll
+        for (int d = LPR; d < 32; d <<= 1)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], d);
+        if (c.lane < LPR) {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) red_soft[c.warp][c.col + j] = sum[j];
+        }
+        const float own_top = reference(s_top[my_col]);
+        float cross = 0.0f, own_p = 0.0f;
+        int twice = 0;
+        for (int k = group; k < a.K; k += groups) {
+            const int i = index[k * kCols + my_col], local = i - cta_first;
+            const float q = p[k * kCols + my_col];
+            if (local >= 0 && local < cta_rows) {
+                const unsigned bit = 1u << (local & 31);
+                twice |= (int)(atomicOr(&seen[(local >> 5) * kCols + my_col], bit) & bit);
+                if (q != 0.0f) {
+                    cross += q * ((logit(i, my_col) - own_top) * a.inv_t);
+                    own_p += q;
+                }
+            }
+        }
+        red[0][threadIdx.x] = cross;
+        red[1][threadIdx.x] = own_p;
+        if (cl > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(&bar[turn & 1], cl * 4 * kCols * (uint32_t)sizeof(float));
+        twice = __syncthreads_or(twice);
+        if (threadIdx.x < kCols) {                                        // all of them in the first warp
+            float s = 0.0f;
+            cross = own_p = 0.0f;
+            for (int w = 0; w < c.warps; ++w) s += red_soft[w][threadIdx.x];
+            for (int e = threadIdx.x; e < (int)blockDim.x; e += kCols) { cross += red[0][e]; own_p += red[1][e]; }
+            SoftSum joined = {s_top[threadIdx.x], s};
+            if (cl > 1) {
+                float (*const to)[kCols] = part[turn & 1][rank];
+                for (uint32_t r = 0; r < cl; ++r) {
+                    const uint32_t b = peer_addr(&bar[turn & 1], r);
+                    peer_send(peer_addr(&to[0][threadIdx.x], r), joined.top, b);
+                    peer_send(peer_addr(&to[1][threadIdx.x], r), joined.sum, b);
+                    peer_send(peer_addr(&to[2][threadIdx.x], r), cross, b);
+                    peer_send(peer_addr(&to[3][threadIdx.x], r), own_p, b);
+                }
+                bool ok = *(volatile int *)&gave_up == 0;
+                for (int i = 0; i < kWaitSpins && ok; ++i) {
+                    if (mbar_try_wait(&bar[turn & 1], turn >> 1 & 1)) break;
+                    if (i == kWaitSpins - 1) { *(volatile int *)&gave_up = 1; ok = false; }
+                }
+                const float (*from)[4][kCols] = part[turn & 1];
+                joined = {from[0][0][threadIdx.x], from[0][1][threadIdx.x]};
+                for (uint32_t r = 1; r < cl; ++r) joined = join_soft(joined, {from[r][0][threadIdx.x], from[r][1][threadIdx.x]}, a.scale);
+                cross = 0.0f;
+                for (uint32_t r = 0; r < cl; ++r) {
+                    const float q = from[r][3][threadIdx.x];
+                    cross += from[r][2][threadIdx.x];
+                    if (q != 0.0f) cross += q * ((reference(from[r][0][threadIdx.x]) - reference(joined.top)) * a.inv_t);
+                }
+            }
+            float loss;
+            s_grad[threadIdx.x] = finish_frame(a, teacher, joined, cross, loss);
+            red[0][threadIdx.x] = loss;
+        }
+        __syncthreads();
+        if (rank == 0 && c.warp == 0)
+            write_losses(a, tile, tile * kCols + c.lane, c.lane < kCols && tile * kCols + c.lane < a.F, c.lane < kCols ? red[0][c.lane] : 0.0f);
+        if (f < a.F) {
+            FrameGrad g[kVec];
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) g[j] = s_grad[c.col + j];
+            const uint8_t *q = at;
+            T *out = a.dz + first * a.dzs;
+#pragma unroll 4
+            for (int i = 0; i < mine; ++i, q += piece, out += dz_step) {
+                unpack<T>(*reinterpret_cast<const uint4 *>(q), v);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) v[j] = soft_part(g[j], v[j], a.scale);
+                store_frames<T, true>(out, f, a.F, v);
+            }
+        }
+        __syncthreads();                                                  // the CTA's values of dz stand before those of the named classes are written again
+        if (tile * kCols + my_col < a.F) {
+            const FrameGrad g = s_grad[my_col];
+            for (int k = group; k < a.K; k += groups) {
+                const int i = index[k * kCols + my_col], local = i - cta_first;
+                if (local < 0 || local >= cta_rows) continue;
+                seen[(local >> 5) * kCols + my_col] = 0u;
+                bool leads = true;
+                float q = p[k * kCols + my_col];
+                if (twice) q = named_slots<kCols>(index, p, a.K, k, my_col, leads);
+                if (leads) a.dz[i * a.dzs + tile * kCols + my_col] = from_float<T>(soft_part(g, logit(i, my_col), a.scale) - g.slope * q);
+            }
+        }
+        __syncthreads();                                                  // nobody needs the logits and the slots any more
+        fetch(f + clusters * kCols);
+    }
+    if (cl > 1) {
+        if (threadIdx.x == 0 && gave_up) atomicCAS(fault, 0, kFaultBarrierTimeout);
+        __syncwarp();
+        cluster_arrive();                                                 // nobody leaves while something may still be sent to it
+        cluster_wait();
+    }
+}
+
+// ---- more classes than that: the softmax's sums, what follows from them for a frame, dz of all classes, dz of the named ones.
+// part[chunk of classes][column]
+template <typename T, int LPR, bool ALIGNED>
+__global__ void __launch_bounds__(kColumnThreads, 3)
+k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int columns)
+{
+    grid_dependency();
+    constexpr int kBatch = 8;
+    using Col = Column<T, LPR>;
+    constexpr int kVec = Col::kVec, kCols = Col::kCols;
+    __shared__ SoftSum red[kColumnThreads / 32][kCols];
+    const Col c;
+    const int f = (int)blockIdx.x * kCols + c.col, step = c.step, n0 = (int)blockIdx.y * chunk_rows, n1 = min(a.C, n0 + chunk_rows);
+    SoftSum s[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) s[j] = {-INFINITY, 0.0f};
+    // some rows at a time: their largest logits first, then the exponentials
+    auto add = [&](auto count, int n) {
+        constexpr int B = decltype(count)::value;
+        uint4 raw[B], most;
+#pragma unroll
+        for (int i = 0; i < B; ++i) raw[i] = load_frames<T, ALIGNED>(a.z + (long long)(n + i * step) * a.zs, f, a.F);
+        most = raw[0];
+#pragma unroll
+        for (int i = 1; i < B; ++i) most = packed_max<T>(most, raw[i]);
+        float top[kVec];
+        unpack<T>(most, top);
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
-            a[j].sum *= a[j].top == -INFINITY ? 1.0f : exp2f((a[j].top - top[j]) * scale);
-            a[j].top = top[j];
-        }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            if (n + i * c.step < n1) {
-                float v[kVec];
-                unpack<T>(raw[i], v);
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) a[j].sum += v[j] == -INFINITY ? 0.0f : exp2f((v[j] - top[j]) * scale);
+            top[j] = fmaxf(s[j].top, top[j]);
+            if (s[j].top != top[j]) {
+                if (s[j].top != -INFINITY) s[j].sum *= exp2_fast((s[j].top - top[j]) * a.scale);
+                s[j].top = top[j];
             }
+            top[j] = reference(top[j]);
         }
-    }
 #pragma unroll
-    for (int m = kLpr; m < 32; m <<= 1)
+        for (int i = 0; i < B; ++i) {
+            float v[kVec];
+            unpack<T>(raw[i], v);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) s[j].sum += exp2_fast((v[j] - top[j]) * a.scale);
+        }
+    };
+    int n = n0 + c.row;
+    for (; n + (kBatch - 1) * step < n1; n += kBatch * step) add(std::integral_constant<int, kBatch>(), n);
+    for (; n < n1; n += step) add(std::integral_constant<int, 1>(), n);
+#pragma unroll
+    for (int m = LPR; m < 32; m <<= 1)
 #pragma unroll
         for (int j = 0; j < kVec; ++j)
-            a[j] = join_soft(a[j], {__shfl_xor_sync(0xffffffffu, a[j].top, m), __shfl_xor_sync(0xffffffffu, a[j].sum, m)}, scale);
-    if (c.lane < kLpr) {
+            s[j] = join_soft(s[j], {__shfl_xor_sync(0xffffffffu, s[j].top, m), __shfl_xor_sync(0xffffffffu, s[j].sum, m)}, a.scale);
+    if (c.lane < LPR) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) s[c.warp][c.col + j] = a[j];
+        for (int j = 0; j < kVec; ++j) red[c.warp][c.col + j] = s[j];
     }
     __syncthreads();
     if (threadIdx.x < kCols) {
-        SoftSum t = s[0][threadIdx.x];
-        for (int w = 1; w < c.warps; ++w) t = join_soft(t, s[w][threadIdx.x], scale);
+        SoftSum t = red[0][threadIdx.x];
+        for (int w = 1; w < c.warps; ++w) t = join_soft(t, red[w][threadIdx.x], a.scale);
         part[(long long)blockIdx.y * columns + (long long)blockIdx.x * kCols + threadIdx.x] = t;
     }
 }
 
-// One thread a frame, its slots one after the other: coef[0] = max z, coef[1] = factor of exp2 in dz, loss_buf; and the slots' classes, -1 where the
-// slot is empty or its class has been named by an earlier one, with the probabilities of a class added up, in slot_index / slot_p [K][columns].
+// The numbers of FrameGrad as grad[4][columns], the frames' losses, and the slots as the last kernel takes them: the class, or -1 where the slot is empty
+// or names a class that an earlier one does, and the probabilities of a class added up.  A CTA has eight frames, 32 threads for each.
+constexpr int kFinishCols = 8;
 template <typename T>
-__global__ void __launch_bounds__(kDistillThreads)
-k_distill_teacher(const T *z, const T *__restrict__ t, const int *__restrict__ index, const float *__restrict__ t_lse, const float *__restrict__ weight,
-                  const SoftSum *__restrict__ part, float *coef, int *slot_index, float *slot_p, float *loss_buf, double *loss_part, float temperature,
-                  float grad_reduction, double loss_reduction, int C, int K, int F, long long zs, long long ts, long long is, int chunks, int columns)
+__global__ void __launch_bounds__(kColumnThreads)
+k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunks, float *grad, int *slot_index, float *slot_p, int columns)
 {
     grid_dependency();
-    __shared__ double red[kDistillThreads / 32];
-    const float inv_t = 1.0f / temperature, scale = kLog2e * inv_t;
-    const int f = (int)blockIdx.x * kDistillThreads + threadIdx.x;
-    double loss = 0.0;
-    if (f < F) {
-        SoftSum s = part[f];
-        for (int k = 1; k < chunks; ++k) s = join_soft(s, part[(long long)k * columns + f], scale);
-        const float w = weight ? weight[f] : 1.0f;
-        float top = -INFINITY;
-        int slots = 0;
-        for (int k = 0; k < K; ++k) {
-            const int i = index[k * is + f];
-            const float tk = to_float(t[k * ts + f]);
-            if (i >= 0 && i < C && tk != -INFINITY) { top = fmaxf(top, tk); ++slots; }
-        }
-        const bool live = slots > 0 && w != 0.0f;
-        float lse = 0.0f;
-        if (live) {
-            if (t_lse) {
-                lse = t_lse[f];
-            } else {
-                float sum = 0.0f;
-                for (int k = 0; k < K; ++k) {
-                    const int i = index[k * is + f];
-                    const float tk = to_float(t[k * ts + f]);
-                    if (i >= 0 && i < C && tk != -INFINITY) sum += exp2f((tk - top) * scale);
-                }
-                lse = top * inv_t + logf(sum);
-            }
-        }
-        const float log_sum = logf(s.sum);
-        float P = 0.0f, l = 0.0f;
-        for (int k = 0; k < K; ++k) {
-            const int i = index[k * is + f];
-            const float tk = to_float(t[k * ts + f]);
-            const bool has = live && i >= 0 && i < C && tk != -INFINITY;
-            float p = 0.0f;
-            if (has) {
-                const float log_p = tk * inv_t - lse;
-                p = exp2f(log_p * kLog2e);
-                const float zi = to_float(z[i * zs + f]);
-                const float log_q = zi == -INFINITY ? -INFINITY : (zi - s.top) * inv_t - log_sum;
-                if (p != 0.0f) l += p * (log_p - log_q);
-                P += p;
-            }
-            int owner = has ? i : -1;
-            for (int e = 0; e < k && owner >= 0; ++e)
-                if (slot_index[(long long)e * columns + f] == i) {
-                    slot_p[(long long)e * columns + f] += p;
-                    owner = -1;
-                }
-            slot_index[(long long)k * columns + f] = owner;
-            slot_p[(long long)k * columns + f] = p;
-        }
-        const float g = live ? grad_reduction * w * temperature : 0.0f;
-        coef[f] = s.top;
-        coef[columns + f] = live ? g * P / s.sum : 0.0f;
-        coef[2 * columns + f] = g;
-        l = live ? w * temperature * temperature * l : 0.0f;
-        loss_buf[f] = l;
-        loss = (double)l;
+    extern __shared__ __align__(16) uint8_t buffer[];
+    __shared__ float red[2][kColumnThreads], s_top[kFinishCols];
+    __shared__ SoftSum sums[kColumnThreads / kFinishCols][kFinishCols];
+    int *const index = reinterpret_cast<int *>(buffer);
+    float *const p = reinterpret_cast<float *>(index + a.K * kFinishCols);
+    const int col = threadIdx.x % kFinishCols, group = threadIdx.x / kFinishCols, f = (int)blockIdx.x * kFinishCols + col;
+    constexpr int kGroups = kColumnThreads / kFinishCols;
+    SoftSum s = {-INFINITY, 0.0f};
+    for (int k = group; k < chunks; k += kGroups) s = join_soft(s, part[(long long)k * columns + f], a.scale);
+    sums[group][col] = s;
+    const TeacherColumn teacher = teacher_columns<T, kFinishCols>(a, (int)blockIdx.x * kFinishCols, index, p, red);
+    if (group == 0) {
+        for (int k = 1; k < kGroups; ++k) s = join_soft(s, sums[k][col], a.scale);
+        s_top[col] = reference(s.top);
     }
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, m);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = loss;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < kDistillThreads / 32; ++k) loss += red[k];
-        loss_part[blockIdx.x] = loss * loss_reduction;
+    float cross = 0.0f;
+    for (int k = group; k < a.K; k += kGroups) {
+        const int i = index[k * kFinishCols + col];
+        float q = p[k * kFinishCols + col];
+        if (i >= 0 && q != 0.0f) cross += q * ((to_float(a.z[i * a.zs + f]) - s_top[col]) * a.inv_t);
+        bool leads = false;
+        if (i >= 0) q = named_slots<kFinishCols>(index, p, a.K, k, col, leads);
+        slot_index[(long long)k * columns + f] = leads ? i : -1;
+        slot_p[(long long)k * columns + f] = q;
+    }
+    red[0][threadIdx.x] = cross;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        float loss = 0.0f;
+        if (group == 0) {
+            cross = 0.0f;
+            for (int e = col; e < kColumnThreads; e += kFinishCols) cross += red[0][e];
+            const FrameGrad g = finish_frame(a, teacher, s, cross, loss);
+            grad[f] = g.top;
+            grad[columns + f] = g.factor;
+            grad[2LL * columns + f] = g.cap;
+            grad[3LL * columns + f] = g.slope;
+        }
+        write_losses(a, (int)blockIdx.x, f, group == 0 && f < a.F, loss);
     }
 }
 
+// Along the rows, as the layer norm's: what the softmax contributes to dz
+constexpr int kDistillBand = 8;
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kDistillThreads)
-k_distill_apply(const T *z, T *dz, const float *__restrict__ coef, const int *__restrict__ slot_index, const float *__restrict__ slot_p,
-                const double *__restrict__ loss_part, int loss_parts, float *loss, float scale, int C, int K, int F, long long zs, long long dzs, int chunk_rows,
-                int columns)
+__global__ void __launch_bounds__(kColumnThreads)
+k_distill_apply(const Distill<T> a, const float *__restrict__ grad, int columns)
 {
     grid_dependency();
-    constexpr int kLpr = 8, kBatch = 8;
-    using Col = Column<T, kLpr>;
-    constexpr int kVec = Col::kVec, kCols = Col::kCols;
-    const Col c;
-    const int f0 = (int)blockIdx.x * kCols, f = f0 + c.col;
-    const int n0 = (int)blockIdx.y * chunk_rows, n1 = min(C, n0 + chunk_rows);
-    float top[kVec], fac[kVec];
+    constexpr int kVec = kFramesPerVec<T>;
+    const int f = ((int)blockIdx.x * 32 + (int)(threadIdx.x & 31)) * kVec, n0 = ((int)blockIdx.y * 8 + (int)(threadIdx.x >> 5)) * kDistillBand;
+    if (f >= a.F) return;
+    uint4 raw[kDistillBand];
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) { top[j] = f + j < F ? coef[f + j] : 0.0f; fac[j] = f + j < F ? coef[columns + f + j] : 0.0f; }
-    for (int n = n0 + c.row; n < n1; n += c.step * kBatch) {
-        uint4 raw[kBatch];
+    for (int i = 0; i < kDistillBand; ++i)
+        if (n0 + i < a.C) raw[i] = load_frames<T, ALIGNED>(a.z + (long long)(n0 + i) * a.zs, f, a.F);
+    float top[kVec], factor[kVec], cap[kVec];                             // (grad is padded to whole vectors)
+    load_columns(grad, f, columns, top);
+    load_columns(grad + columns, f, columns, factor);
+    load_columns(grad + 2LL * columns, f, columns, cap);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int m = n + i * c.step;
-            if (m < n1) raw[i] = load_frames<T, ALIGNED>(z + (long long)m * zs, f, F);
-        }
+    for (int i = 0; i < kDistillBand; ++i) {
+        if (n0 + i < a.C) {
+            float v[kVec];
+            unpack<T>(raw[i], v);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int m = n + i * c.step;
-            if (m < n1) {
-                float v[kVec];
-                unpack<T>(raw[i], v);
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) v[j] = fac[j] == 0.0f || v[j] == -INFINITY ? 0.0f : fac[j] * exp2f((v[j] - top[j]) * scale);
-                store_frames<T, ALIGNED>(dz + (long long)m * dzs, f, F, v);
-            }
+            for (int j = 0; j < kVec; ++j) v[j] = soft_part({top[j], factor[j], cap[j], 0.0f}, v[j], a.scale);
+            store_frames<T, ALIGNED>(a.dz + (long long)(n0 + i) * a.dzs, f, a.F, v);
         }
     }
-    __syncthreads();                                                     // the block's own values of dz stand before the named classes are written again
-    for (int e = threadIdx.x; e < K * kCols; e += kDistillThreads) {
-        const int g = f0 + e % kCols;
-        const long long at = (long long)(e / kCols) * columns + g;
-        if (g >= F) continue;
-        const int i = slot_index[at];
-        if (i < n0 || i >= n1) continue;
-        const float v = to_float(z[i * zs + g]), fc = coef[columns + g];
-        const float q = fc == 0.0f || v == -INFINITY ? 0.0f : fc * exp2f((v - coef[g]) * scale);
-        dz[i * dzs + g] = from_float<T>(q - coef[2 * columns + g] * slot_p[at]);
-    }
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 32) {
-        double s = 0.0;
-        for (int k = threadIdx.x; k < loss_parts; k += 32) s += loss_part[k];
+}
+
+// the named classes, a frame and slot a thread
+template <typename T>
+__global__ void __launch_bounds__(kColumnThreads)
+k_distill_named(const Distill<T> a, const float *__restrict__ grad, const int *__restrict__ slot_index, const float *__restrict__ slot_p, int columns)
+{
+    grid_dependency();
+    const int f = (int)blockIdx.x * kColumnThreads + threadIdx.x, k = blockIdx.y;
+    if (f >= a.F) return;
+    const int i = slot_index[(long long)k * columns + f];
+    if (i < 0) return;
+    const FrameGrad g = {grad[f], grad[columns + f], grad[2LL * columns + f], grad[3LL * columns + f]};
+    a.dz[i * a.dzs + f] = from_float<T>(soft_part(g, to_float(a.z[i * a.zs + f]), a.scale) - g.slope * slot_p[(long long)k * columns + f]);
+}
+
+__global__ void __launch_bounds__(1024) k_distill_loss(const double *__restrict__ part, int parts, double loss_reduction, float *loss)
+{
+    grid_dependency();
+    __shared__ double red[32];
+    double s = 0.0;
+    for (int k = threadIdx.x; k < parts; k += 1024) s += part[k];
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        s = red[threadIdx.x];
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
-        if (threadIdx.x == 0) *loss = (float)s;
+        if (threadIdx.x == 0) *loss = (float)(s * loss_reduction);
     }
 }
 
-template <typename T>
-static int distillation(const T *z, T *dz, const T *t, const int *index, const float *t_lse, const float *weight, float *loss_buf, float *loss,
-                        float temperature, float grad_reduction, double loss_reduction, int C, int K, int F, long long zs, long long dzs, long long ts,
-                        long long is, cudaStream_t st)
+constexpr int kDistillSmem = 200 * 1024;                 // more than any call needs: 64 KB of logits, 128 KB of slots, 4 KB of bits
+
+template <typename T, int LPR>
+static int distillation_once(const Distill<T> &a, const ColumnPlan &p, int tiles, cudaStream_t st)
 {
-    const bool aligned = frames_aligned<T>(z, zs) && frames_aligned<T>(dz, dzs);
-    constexpr int kCols = Column<T, 8>::kCols;
-    const long long tiles = ((long long)F + kCols - 1) / kCols;
-    BB200_REQUIRE(tiles * kCols < (1LL << 31) && K <= (1 << 20) , BBCU_ERR_TOO_LARGE);
-    const int columns = (int)(tiles * kCols);
-    const long long want = 4LL * device_info().sm_count, per = (want + tiles - 1) / tiles;
-    int rows = (int)(((C + per - 1) / per + 63) / 64 * 64);
-    while ((C + rows - 1) / rows > 65535) rows *= 2;
-    const int chunks = (C + rows - 1) / rows;
-    const unsigned teacher_ctas = (unsigned)((F + kDistillThreads - 1) / kDistillThreads);
-    const size_t part_b = (size_t)chunks * columns * sizeof(SoftSum), coef_b = (size_t)columns * 3 * 4, slot_b = (size_t)K * columns * 4;
-    char *scratch = static_cast<char *>(stream_scratch(st, part_b + coef_b + 2 * slot_b + teacher_ctas * sizeof(double), kFrameOpSlot));
+    int *fault = fault_word();
+    BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
+    auto kernel = k_distill_once<T, LPR>;
+    constexpr int kCols = Column<T, LPR>::kCols;
+    const int threads = 32 * p.warps, smem = p.rows * threads * 16 + a.K * kCols * 8 + (p.warps * 32 / LPR * p.rows + 31) / 32 * kCols * 4;
+    BB200_REQUIRE(allow_big_smem(kernel, kDistillSmem), (int)cudaErrorInvalidValue);
+    const int clusters = std::min(tiles, resident_clusters(reinterpret_cast<const void *>(kernel), p.cluster, threads, smem));
+    return launch_cluster(kernel, (unsigned)p.cluster, (unsigned)(clusters * p.cluster), threads, smem, st, a, p.rows, tiles, fault);
+}
+
+// Chunks of rows that a streaming kernel is cut into beside its column tiles: of up to `most`, the number whose CTAs fill their last round on the
+// device best.
+static int best_chunks(long long tiles, long long resident, int most)
+{
+    int best = 1;
+    double filled = 0.0;
+    for (int n = 1; n <= most; ++n) {
+        const long long ctas = tiles * n, rounds = (ctas + resident - 1) / resident;
+        if (rounds > 4 && n > 1) break;
+        const double share = (double)ctas / (double)(rounds * resident);
+        if (share > filled + 0.02) { filled = share; best = n; }
+    }
+    return best;
+}
+
+template <typename T, int LPR>
+static int distillation_passes(Distill<T> &a, int &loss_parts, bool aligned, cudaStream_t st)
+{
+    constexpr int kCols = Column<T, LPR>::kCols, kWide = 32 * kFramesPerVec<T>;
+    const int tiles = (a.F + kCols - 1) / kCols, columns = tiles * kCols;
+    const long long bands = ((long long)a.C + 8 * kDistillBand - 1) / (8 * kDistillBand);
+    BB200_REQUIRE(bands <= 65535, BBCU_ERR_TOO_LARGE);
+    auto sums = aligned ? k_distill_sums<T, LPR, true> : k_distill_sums<T, LPR, false>;
+    const int chunks = best_chunks(tiles, resident_clusters(reinterpret_cast<const void *>(sums), 1, kColumnThreads, 0), std::min(64, std::max(1, a.C / 256)));
+    const int rows = (a.C + chunks - 1) / chunks;
+    loss_parts = columns / kFinishCols;
+    const size_t part_b = (size_t)chunks * columns * sizeof(SoftSum), loss_b = (size_t)loss_parts * sizeof(double), slots = (size_t)a.K * columns;
+    char *scratch = static_cast<char *>(stream_scratch(st, loss_b + part_b + ((size_t)4 * columns + 2 * slots) * 4, kFrameOpSlot));
     BB200_REQUIRE(scratch != nullptr, BBCU_ERR_NO_MEMORY);
-    SoftSum *part = reinterpret_cast<SoftSum *>(scratch);
-    double *loss_part = reinterpret_cast<double *>(scratch + part_b);
-    float *coef = reinterpret_cast<float *>(scratch + part_b + teacher_ctas * sizeof(double)), *slot_p = coef + 3 * (size_t)columns;
-    int *slot_index = reinterpret_cast<int *>(slot_p + (size_t)K * columns);
-    const float scale = kLog2e / temperature;
-    const dim3 grid((unsigned)tiles, (unsigned)chunks);
-    launch(aligned ? k_distill_stats<T, true> : k_distill_stats<T, false>, grid, kDistillThreads, 0, st, z, part, scale, C, F, zs, rows, columns);
+    a.loss_part = reinterpret_cast<double *>(scratch);
+    SoftSum *part = reinterpret_cast<SoftSum *>(scratch + loss_b);
+    float *grad = reinterpret_cast<float *>(scratch + loss_b + part_b), *slot_p = grad + (size_t)4 * columns;
+    int *slot_index = reinterpret_cast<int *>(slot_p + slots);
+    launch(sums, dim3((unsigned)tiles, (unsigned)chunks), kColumnThreads, 0, st, a, part, rows, columns);
     BB200_CUDA(cudaPeekAtLastError());
-    launch(k_distill_teacher<T>, teacher_ctas, kDistillThreads, 0, st, z, t, index, t_lse, weight, part, coef, slot_index, slot_p, loss_buf, loss_part, temperature,
-           grad_reduction, loss_reduction, C, K, F, zs, ts, is, chunks, columns);
+    launch(k_distill_finish<T>, (unsigned)loss_parts, kColumnThreads, (size_t)a.K * kFinishCols * 8, st, a, part, chunks, grad, slot_index, slot_p, columns);
     BB200_CUDA(cudaPeekAtLastError());
-    launch(aligned ? k_distill_apply<T, true> : k_distill_apply<T, false>, grid, kDistillThreads, 0, st, z, dz, coef, slot_index, slot_p, loss_part,
-           (int)teacher_ctas, loss, scale, C, K, F, zs, dzs, rows, columns);
+    launch(aligned ? k_distill_apply<T, true> : k_distill_apply<T, false>, dim3((unsigned)((a.F + kWide - 1) / kWide), (unsigned)bands), kColumnThreads, 0, st, a, grad,
+           columns);
+    BB200_CUDA(cudaPeekAtLastError());
+    if (a.K > 0)
+        launch(k_distill_named<T>, dim3((unsigned)((a.F + kColumnThreads - 1) / kColumnThreads), (unsigned)a.K), kColumnThreads, 0, st, a, grad, slot_index, slot_p, columns);
+    return launch_status();
+}
+
+template <typename T>
+static int distillation(Distill<T> a, float *loss, double loss_reduction, cudaStream_t st)
+{
+    constexpr int kLanes = 4;                                              // 64 bytes of a row: up to 1024 classes a CTA
+    const bool aligned = frames_aligned<T>(a.z, a.zs) && frames_aligned<T>(a.dz, a.dzs);
+    ColumnPlan p = plan_columns<T>(a.C, a.F, kLanes, kDistillRows, kDistillCluster);
+    if (!aligned || p.cluster > kDistillCluster) p.cluster = 0;
+    if (p.cluster) {
+        // a power of two of warps; where there are many tiles, few of them with more rows a thread, since all warps of a CTA take part in the teacher's side
+        // and its barriers (100 classes x 65536 frames: eight warps 51 us, two 28)
+        const int cols = p.lanes * kFramesPerVec<T>, per_warp = 32 / p.lanes, cta_rows = (a.C + p.cluster - 1) / p.cluster;
+        while (p.warps & (p.warps - 1)) ++p.warps;
+        if ((long long)(a.F / cols) * p.cluster >= 4LL * device_info().sm_count)
+            while (p.warps > 2 && cta_rows <= per_warp * (p.warps / 2) * kDistillRows / 2) p.warps /= 2;
+        p.rows = (cta_rows + per_warp * p.warps - 1) / (per_warp * p.warps);
+    }
+    int parts = 0, e;
+    if (p.cluster) {
+        const int cols = p.lanes * kFramesPerVec<T>;
+        parts = (a.F + cols - 1) / cols;
+        a.loss_part = static_cast<double *>(stream_scratch(st, (size_t)parts * sizeof(double), kFrameOpSlot));
+        BB200_REQUIRE(a.loss_part != nullptr, BBCU_ERR_NO_MEMORY);
+        e = p.lanes == 2 ? distillation_once<T, 2>(a, p, parts, st) : distillation_once<T, kLanes>(a, p, parts, st);
+    } else {
+        e = distillation_passes<T, sizeof(T) == 4 ? 8 : 4>(a, parts, aligned, st);
+    }
+    if (e != BBCU_OK) return e;
+    launch(k_distill_loss, 1, 1024, 0, st, a.loss_part, parts, loss_reduction, loss);
     return launch_status();
 }
 
@@ -267,8 +646,9 @@ static int distillation_checked(const T *z, T *dz, const T *t, const int *index,
                                 float temperature, float grad_reduction, double loss_reduction, int C, int K, int F, int zs, int dzs, int ts, int is,
                                 bbcu_stream_t stream)
 {
-    BB200_REQUIRE(C > 0 && K >= 0 && F >= 0 && temperature > 0.0f && temperature < INFINITY, BBCU_ERR_BAD_SIZE);
-    BB200_REQUIRE(C <= (1 << 24), BBCU_ERR_TOO_LARGE);
+    BB200_REQUIRE(C > 0 && K >= 0 && F >= 0 && temperature > 0.0f && temperature < INFINITY &&
+                  kLog2e / temperature < INFINITY, BBCU_ERR_BAD_SIZE);
+    BB200_REQUIRE(C <= (1 << 20) && K <= kMostSlots && F <= (1 << 30), BBCU_ERR_TOO_LARGE);
     BB200_REQUIRE(zs >= F && dzs >= F && (K == 0 || (ts >= F && is >= F)), BBCU_ERR_BAD_STRIDE);
     BB200_REQUIRE_PTR(loss);
     cudaStream_t st = as_stream(stream);
@@ -278,7 +658,8 @@ static int distillation_checked(const T *z, T *dz, const T *t, const int *index,
     }
     BB200_REQUIRE_PTR(z); BB200_REQUIRE_PTR(dz); BB200_REQUIRE_PTR(loss_buf);
     if (K > 0) { BB200_REQUIRE_PTR(t); BB200_REQUIRE_PTR(index); }
-    return distillation<T>(z, dz, t, index, t_lse, weight, loss_buf, loss, temperature, grad_reduction, loss_reduction, C, K, F, zs, dzs, ts, is, st);
+    return distillation<T>({z, t, dz, index, t_lse, weight, loss_buf, nullptr, temperature, 1.0f / temperature, kLog2e / temperature, grad_reduction, C, K, F, zs, dzs, ts, is},
+                           loss, loss_reduction, st);
 }
 
 }   // namespace bb200

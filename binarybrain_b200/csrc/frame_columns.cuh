@@ -262,7 +262,7 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
 // `rows` rows a thread, at most `most_rows`.
 struct ColumnPlan { int cluster, warps, rows, lanes; };
 template <typename T>
-inline ColumnPlan plan_columns(int N, int F, int lanes, int most_rows)
+inline ColumnPlan plan_columns(int N, int F, int lanes, int most_rows, int most_spread = 8)
 {
     if (F <= 2 * kFramesPerVec<T>) lanes = 2;
     const int per_warp = 32 / lanes, most_warps = kColumnThreads / 32;
@@ -272,7 +272,7 @@ inline ColumnPlan plan_columns(int N, int F, int lanes, int most_rows)
     // as many CTAs as it takes to hold a column, and more where there would be few
     while (cluster < kMostCluster && rows() > most_warps * per_warp * most_rows) cluster *= 2;
     if (rows() > most_warps * per_warp * most_rows) return {0, 0, 0, 0};
-    while (cluster < 8 && tiles * cluster * 2 <= sms && rows() > most_warps * per_warp) cluster *= 2;
+    while (cluster < most_spread && tiles * cluster * 2 <= sms && rows() > most_warps * per_warp) cluster *= 2;
     const int warps = std::min(most_warps, (rows() + per_warp - 1) / per_warp);
     return {cluster, warps, (rows() + per_warp * warps - 1) / (per_warp * warps), lanes};
 }

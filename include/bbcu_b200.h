@@ -377,7 +377,7 @@ int bbcu_fp32_DifferentiableLut6_ForwardTraining_NoAlloc_MaxNodes(void);
  * No counterparts in the reference.  Frame buffers are node-major as above, fp32 or bf16 (bbcu_bf16_*: two bytes an element, strides in elements);
  * any stride and alignment of theirs is taken, rows on 16-byte boundaries are the fast ones, and outputs are written up to the last frame, never
  * into a row's padding.  Outputs do not overlap inputs.  Sums and statistics are 32 bits or more; bf16 results are rounded once.  A batch without
- * frames is no error.  Scratch as for the LUT operators above: the first call of a size on a stream allocates. */
+ * frames is no error.  Layer norm and distillation take up to 2^20 nodes or classes and 2^30 frames, BBCU_ERR_TOO_LARGE beyond.  Scratch as for the LUT operators above: the first call of a size on a stream allocates. */
 
 /* Layer norm over the nodes of a frame: y = (x - mean) * rstd * gamma + beta, mean and rstd = 1 / sqrt(variance + eps) [frame_size], which the
  * backward takes.  dev_gamma / dev_beta [node_size], NULL: 1 / 0. */
@@ -422,7 +422,7 @@ int bbcu_int8_bf16_DenseAffine_Forward(const signed char *dev_q_buf, const float
  *   p_k = exp(t_k / T - lse), lse over the frame's slots, or dev_t_lse[frame] = log sum exp(t / T) over all of the teacher's classes when it is given;
  *   loss = T^2 sum_k p_k (log p_k - log softmax(z / T)[class_k]),   dz = its gradient;
  * dev_loss_buf[frame] = weight * loss, *dev_loss = loss_reduction * their sum, dz = grad_reduction * weight * gradient (weight: dev_weight[frame],
- * NULL: 1; both reductions 1 / frames for a mean).  A frame of weight 0 or without a slot gives zeros whatever it holds.  Classes that a frame names
+ * NULL: 1; both reductions 1 / frames for a mean).  top_size is up to 512, BBCU_ERR_TOO_LARGE beyond.  A frame of weight 0 or without a slot gives zeros whatever it holds.  Classes that a frame names
  * twice add up.  Results do not depend on the order in which anything runs. */
 int bbcu_fp32_LossDistillation(const float *dev_z_buf, float *dev_dz_buf, const float *dev_t_buf, const int *dev_index_buf, const float *dev_t_lse,
                                const float *dev_weight, float *dev_loss_buf, float *dev_loss, float temperature, float grad_reduction,
