@@ -13,9 +13,8 @@
 
 namespace bb200 {
 
-constexpr int kQuantThreads = 256, kQuantRows = 128;      // rows of x that a CTA turns over at a time
+constexpr int kQuantThreads = 256, kQuantRows = 128;      // rows of x that a CTA turns over
 constexpr int kMostInputs = 131071;                       // times 128 x 128 is below 2^31
-constexpr int kRowFrames = 8;                             // up to this many frames the product reads rows of W, beyond it works on tiles
 
 __device__ __forceinline__ float quant_scale(uint32_t abs_bits)
 {
@@ -28,96 +27,119 @@ __device__ __forceinline__ int quantize(float x, float scale)
     return max(-127, min(127, __float2int_rn(__fdiv_rn(x, scale))));
 }
 
-// part[chunk][column] = bits of the largest |x| (as integers they order like the numbers, with infinities and NaN on top)
+// Four numbers of a frame as a word of q.  x / scale comes through the reciprocal, off by less than 1e-4, and is rounded by adding 1.5 * 2^23, which
+// leaves the integer in the lowest byte; where that could have decided the rounding, and for scales without a normal reciprocal, the quotient is divided
+// out.  (The kernels are bound by their instructions, and the division costs more than all the rest.)
+struct Quantizer {
+    float scale, inv;
+    bool plain;
+    __device__ explicit Quantizer(float s) : scale(s), inv(1.0f / s), plain(s > 1e-36f && s < 1e36f) {}
+    __device__ uint32_t operator()(float x0, float x1, float x2, float x3) const
+    {
+        constexpr float kRound = 12582912.0f;
+        const float x[4] = {x0, x1, x2, x3};
+        float worst = 0.0f;
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float t = x[i] * inv, n = t + kRound;
+            worst = fmaxf(worst, fabsf(t - (n - kRound)));
+            r[i] = __float_as_uint(n);
+        }
+        if (worst > 0.4999f || !plain) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = (uint32_t)quantize(x[i], scale);
+        }
+        return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+    }
+};
+
+// the larger of the magnitudes of packed numbers, as integers: infinities and NaN are on top
+template <typename T> __device__ __forceinline__ uint32_t packed_abs_max(uint32_t a, uint32_t b)
+{
+    return sizeof(T) == 4 ? max(a, b & 0x7fffffffu) : __vmaxu2(a, b & 0x7fff7fffu);
+}
+
+// A cluster has the columns of 128 bytes of a row; its CTAs take turns at the rows and join the largest magnitudes in the first CTA's shared memory.
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(kQuantThreads)
-k_quantize_max(const T *x, uint32_t *part, int N, int F, long long xs, int chunk_rows, int columns)
+__global__ void __launch_bounds__(kQuantThreads, 4)
+k_quantize_scale(const T *x, float *scale_out, int N, int F, long long xs)
 {
     grid_dependency();
     constexpr int kLpr = 8, kBatch = 8;
     using Col = Column<T, kLpr>;
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
-    __shared__ uint32_t s[8][kCols];
+    __shared__ uint32_t red[8][kCols];
+    __shared__ float part[kCols];
     const Col c;
-    const int f = (int)blockIdx.x * kCols + c.col;
-    const int n0 = (int)blockIdx.y * chunk_rows, n1 = min(N, n0 + chunk_rows);
-    uint32_t top[kVec] = {};
-    for (int n = n0 + c.row; n < n1; n += c.step * kBatch) {
+    const uint32_t cl = cluster_size(), rank = cluster_rank();
+    const int f0 = (int)(blockIdx.x / cl) * kCols, f = f0 + c.col, step = c.step * (int)cl;
+    uint4 most = make_uint4(0, 0, 0, 0);
+    for (int n = (int)rank * c.step + c.row; n < N; n += step * kBatch) {
         uint4 raw[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int m = n + i * c.step;
-            raw[i] = m < n1 ? load_frames<T, ALIGNED>(x + (long long)m * xs, f, F) : make_uint4(0, 0, 0, 0);
+            const int m = n + i * step;
+            raw[i] = m < N ? load_frames<T, ALIGNED>(x + (long long)m * xs, f, F) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            float v[kVec];
-            unpack<T>(raw[i], v);
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) top[j] = max(top[j], __float_as_uint(fabsf(v[j])));
+            most.x = packed_abs_max<T>(most.x, raw[i].x); most.y = packed_abs_max<T>(most.y, raw[i].y);
+            most.z = packed_abs_max<T>(most.z, raw[i].z); most.w = packed_abs_max<T>(most.w, raw[i].w);
         }
     }
+    float v[kVec];
+    unpack<T>(most, v);
+    uint32_t top[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) top[j] = __float_as_uint(v[j]);
 #pragma unroll
     for (int m = kLpr; m < 32; m <<= 1)
 #pragma unroll
         for (int j = 0; j < kVec; ++j) top[j] = max(top[j], __shfl_xor_sync(0xffffffffu, top[j], m));
     if (c.lane < kLpr) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) s[c.warp][c.col + j] = top[j];
+        for (int j = 0; j < kVec; ++j) red[c.warp][c.col + j] = top[j];
     }
     __syncthreads();
+    uint32_t t = 0;
     if (threadIdx.x < kCols) {
-        uint32_t t = 0;
-        for (int w = 0; w < c.warps; ++w) t = max(t, s[w][threadIdx.x]);
-        part[(long long)blockIdx.y * columns + (long long)blockIdx.x * kCols + threadIdx.x] = t;
+        for (int w = 0; w < c.warps; ++w) t = max(t, red[w][threadIdx.x]);
+        part[threadIdx.x] = __uint_as_float(t);
     }
+    if (cl > 1) { cluster_arrive(); cluster_wait(); }
+    if (rank == 0 && threadIdx.x < kCols && f0 + (int)threadIdx.x < F) {
+        for (uint32_t r = 1; r < cl; ++r) t = max(t, __float_as_uint(peer_load(&part[threadIdx.x], r)));
+        scale_out[f0 + threadIdx.x] = quant_scale(t);
+    }
+    if (cl > 1) { cluster_arrive(); cluster_wait(); }                     // nobody leaves while its part may still be read
 }
 
-// 128 rows of x at a time: a thread reads four neighbouring rows of its columns, so that its four values of a frame are a word of q; the words cross
-// through shared memory and leave as 16 bytes of a frame's row.
+// 128 rows x 128 bytes of x: a thread reads four neighbouring rows of its columns, so that its four values of a frame are a word of q; the words cross
+// through shared memory, in 16-byte pieces whose order differs from column to column so that no banks collide, and leave as 128 bytes of a frame's row.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kQuantThreads)
-k_quantize_apply(const T *x, int8_t *q, const uint32_t *__restrict__ part, float *scale_out, int N, int F, long long xs, long long qs, int chunk_rows,
-                 int chunks, int columns)
+k_quantize_apply(const T *x, int8_t *q, const float *__restrict__ scale_in, int N, int F, long long xs, long long qs)
 {
     grid_dependency();
-    constexpr int kLpr = 8;
+    constexpr int kLpr = 8, kPieces = kQuantRows / 16;
     using Col = Column<T, kLpr>;
-    constexpr int kVec = Col::kVec, kCols = Col::kCols, kWords = kQuantRows / 4;
-    __shared__ float s_scale[kCols];
-    __shared__ __align__(16) uint32_t tile[kCols][kWords + 4];
+    constexpr int kVec = Col::kVec, kCols = Col::kCols;
+    __shared__ __align__(16) uint32_t tile[kCols][kQuantRows / 4];
     const Col c;
-    const int f0 = (int)blockIdx.x * kCols, f = f0 + c.col;
-    if (threadIdx.x < kCols) {
-        uint32_t t = 0;
-        for (int k = 0; k < chunks; ++k) t = max(t, part[(long long)k * columns + f0 + threadIdx.x]);
-        const float s = quant_scale(t);
-        s_scale[threadIdx.x] = s;
-        if (blockIdx.y == 0 && f0 + (int)threadIdx.x < F) scale_out[f0 + threadIdx.x] = s;
-    }
+    const int f0 = (int)blockIdx.x * kCols, f = f0 + c.col, n0 = (int)blockIdx.y * kQuantRows, n = n0 + 4 * c.row;
+    float v[4][kVec], scale[kVec];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack<T>(n + i < N ? load_frames<T, ALIGNED>(x + (long long)(n + i) * xs, f, F) : make_uint4(0, 0, 0, 0), v[i]);
+    load_columns(scale_in, f, F, scale);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+        tile[c.col + j][(c.row / 4 ^ c.lane % kLpr) * 4 + c.row % 4] = Quantizer(scale[j])(v[0][j], v[1][j], v[2][j], v[3][j]);
     __syncthreads();
-    float scale[kVec];
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) scale[j] = s_scale[c.col + j];
-    const int n0 = (int)blockIdx.y * chunk_rows, n1 = min(N, n0 + chunk_rows);
-    for (int base = n0; base < n1; base += kQuantRows) {
-        uint32_t word[kVec] = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = base + 4 * c.row + i;
-            float v[kVec];
-            unpack<T>(n < n1 ? load_frames<T, ALIGNED>(x + (long long)n * xs, f, F) : make_uint4(0, 0, 0, 0), v);
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) word[j] |= (uint32_t)(quantize(v[j], scale[j]) & 0xff) << (8 * i);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) tile[c.col + j][c.row] = word[j];
-        __syncthreads();
-        for (int e = threadIdx.x; e < kCols * (kQuantRows / 16); e += kQuantThreads) {
-            const int col = e / (kQuantRows / 16), piece = e % (kQuantRows / 16), n = base + 16 * piece;
-            if (f0 + col < F && n < n1) *reinterpret_cast<uint4 *>(q + (long long)(f0 + col) * qs + n) = *reinterpret_cast<const uint4 *>(&tile[col][4 * piece]);
-        }
+    for (int e = threadIdx.x; e < kCols * kPieces; e += kQuantThreads) {
+        const int col = e / kPieces, piece = e % kPieces, m = n0 + 16 * piece;
+        if (f0 + col < F && m < N)
+            *reinterpret_cast<uint4 *>(q + (long long)(f0 + col) * qs + m) = *reinterpret_cast<const uint4 *>(&tile[col][(piece ^ col / kVec) * 4]);
     }
 }
 
@@ -141,6 +163,77 @@ k_quantize_channels(const float *__restrict__ W, int8_t *q, float *scale_out, in
     for (int n = threadIdx.x; n < padded; n += 256) q[(long long)blockIdx.x * qs + n] = n < N ? (int8_t)quantize(row[n], scale) : (int8_t)0;
 }
 
+// Small calls in one launch: a cluster holds the columns of 64 bytes of a row in shared memory (see layer_norm.cu for the walk over the tiles), and a thread
+// then takes 16 rows of a column, which are 16 bytes of q.
+struct BitsMax { __device__ static float join(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); } };
+constexpr int kQuantOnceRows = 16;
+constexpr long long kQuantSmall = 1 << 18;
+
+template <typename T, int LPR>
+__global__ void __launch_bounds__(kColumnThreads, 3)
+k_quantize_once(const T *x, int8_t *q, float *scale_out, int N, int F, long long xs, long long qs, int rows, int tiles, int *fault)
+{
+    grid_dependency();
+    using Col = Column<T, LPR>;
+    constexpr int kVec = Col::kVec, kCols = Col::kCols;
+    extern __shared__ __align__(16) uint8_t buffer[];
+    __shared__ Exchange<1, kCols> tops[2];
+    __shared__ int gave_up;
+    const Col c;
+    Cluster cl(&gave_up);
+    const int clusters = (int)(gridDim.x / cl.size), cta_first = (int)cl.rank * c.step * rows, first = cta_first + c.row, piece = blockDim.x * 16;
+    const int mine = min(rows, (N - first + c.step - 1) / c.step), cta_rows = min(c.step * rows, N - cta_first);
+    const uint8_t *const at = buffer + threadIdx.x * 16;
+    const long long x_step = c.step * xs;
+    int tile = (int)(blockIdx.x / cl.size), f = tile * kCols + c.col;
+    auto fetch = [&](int f) {
+        if (f >= F) return;
+        uint8_t *to = buffer + threadIdx.x * 16;
+        const T *from = x + first * xs + f;
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i, to += piece, from += x_step) cp_async16(to, from, true);
+    };
+    fetch(f);
+    cl.meet(tops, 2);
+    uint32_t turn = 0;                                                    // the exchange is its lowest bit, the phase the next
+    for (; tile < tiles; tile += clusters, f += clusters * kCols, ++turn) {
+        cp_async_commit();
+        cp_async_wait<0>();
+        float top[1][kVec] = {};
+        {
+            const uint8_t *p = at;
+#pragma unroll 4
+            for (int i = 0; i < mine; ++i, p += piece) {
+                float v[kVec];
+                unpack<T>(*reinterpret_cast<const uint4 *>(p), v);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) top[0][j] = BitsMax::join(top[0][j], fabsf(v[j]));
+            }
+        }
+        Exchange<1, kCols> &e = tops[turn & 1];
+        join_columns<BitsMax, 1, T, LPR>(top, c, e, cl, turn >> 1 & 1, [](int, float t) { return quant_scale(__float_as_uint(t)); });
+        const int f0 = tile * kCols;
+        if (cl.rank == 0 && threadIdx.x < kCols && f0 + (int)threadIdx.x < F) scale_out[f0 + threadIdx.x] = e.out[threadIdx.x];
+        for (int i = threadIdx.x; i < (cta_rows + 15) / 16 * kCols; i += blockDim.x) {
+            const int col = i % kCols, n = i / kCols * 16;
+            if (f0 + col >= F) continue;
+            const Quantizer quantize(e.out[col]);
+            // (the distance between a thread's rows is a multiple of 16, so that the 16 are of one round)
+            const uint8_t *const from = buffer + n / c.step * piece + (n % c.step * LPR + col / kVec) * 16 + col % kVec * sizeof(T);
+            float v[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[r] = n + r < cta_rows ? to_float(*reinterpret_cast<const T *>(from + r * LPR * 16)) : 0.0f;
+            uint32_t word[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) word[w] = quantize(v[4 * w], v[4 * w + 1], v[4 * w + 2], v[4 * w + 3]);
+            *reinterpret_cast<uint4 *>(q + (long long)(f0 + col) * qs + cta_first + n) = make_uint4(word[0], word[1], word[2], word[3]);
+        }
+        __syncthreads();                                                  // nobody needs the tile any more
+        fetch(f + clusters * kCols);
+    }
+    cl.leave(fault);
+}
+
 // The 16 bytes at k of a frame's row, with what lies beyond the inputs cleared: the padding of W may then hold anything.
 __device__ __forceinline__ int4 load_q(const int8_t *row, int k, int K)
 {
@@ -156,38 +249,54 @@ __device__ __forceinline__ int4 load_q(const int8_t *row, int k, int K)
     return v;
 }
 
-// NF frames and ROWS output nodes a warp, 512 bytes of every row a step
-template <typename T, int NF, int ROWS>
+// A single frame: what counts is to have W on its way.  A warp has a row of W, or one of `splits` parts of its inputs where there are few rows, and asks
+// for 2048 bytes of it before it multiplies; q comes out of L1.  (Two rows a warp for two to eight frames: 9.9 to 22.7 us for 4096 x 4096, the tiles below 9.3.)
+template <typename T>
 __global__ void __launch_bounds__(256)
-k_int8_dense_rows(const int8_t *__restrict__ q, const float *__restrict__ q_scale, const int8_t *__restrict__ W, const float *__restrict__ w_scale,
-                  const float *__restrict__ bias, T *y, int K, int O, int F, long long qs, long long ws, long long ys)
+k_int8_dense_row(const int8_t *__restrict__ q, const float *__restrict__ q_scale, const int8_t *__restrict__ W, const float *__restrict__ w_scale,
+                 const float *__restrict__ bias, T *y, int K, int O, long long ws, long long ys, int splits)
 {
     grid_dependency();
-    const int lane = threadIdx.x & 31;
-    const int o0 = ((int)blockIdx.x * 8 + (int)(threadIdx.x >> 5)) * ROWS;
-    const int f0 = (int)blockIdx.y * NF;
-    if (o0 >= O) return;
-    int acc[ROWS][NF] = {};
-    for (int k = lane * 16; k < K; k += 512) {
-        int4 w[ROWS];
+    constexpr int kAhead = 4;
+    __shared__ int red[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % splits, o = (int)blockIdx.x * (8 / splits) + warp / splits;
+    const int steps = (K + 511) / 512, s0 = (int)((long long)steps * part / splits), s1 = (int)((long long)steps * (part + 1) / splits);
+    const int8_t *const row = W + (long long)min(o, O - 1) * ws;
+    int sum = 0;
+    for (int s = s0; s < s1; s += kAhead) {
+        int4 w[kAhead];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) w[r] = *reinterpret_cast<const int4 *>(W + (long long)min(o0 + r, O - 1) * ws + k);
+        for (int a = 0; a < kAhead; ++a) {
+            const int k = (s + a) * 512 + lane * 16;
+            w[a] = s + a < s1 && k < K ? *reinterpret_cast<const int4 *>(row + k) : make_int4(0, 0, 0, 0);
+        }
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            const int4 v = load_q(q + (long long)min(f0 + f, F - 1) * qs, k, K);
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r)
-                acc[r][f] = __dp4a(w[r].w, v.w, __dp4a(w[r].z, v.z, __dp4a(w[r].y, v.y, __dp4a(w[r].x, v.x, acc[r][f]))));
+        for (int a = 0; a < kAhead; ++a) {
+            const int k = (s + a) * 512 + lane * 16;
+            if (s + a < s1 && k < K) {
+                const int4 v = load_q(q, k, K);
+                sum = __dp4a(w[a].w, v.w, __dp4a(w[a].z, v.z, __dp4a(w[a].y, v.y, __dp4a(w[a].x, v.x, sum))));
+            }
         }
     }
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-            const int s = __reduce_add_sync(0xffffffffu, acc[r][f]);
-            if (lane == (r * NF + f) % 32 && o0 + r < O && f0 + f < F)
-                y[(long long)(o0 + r) * ys + f0 + f] = from_float<T>(fmaf((float)s, w_scale[o0 + r] * q_scale[f0 + f], bias ? bias[o0 + r] : 0.0f));
-        }
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (splits > 1) {
+        if (lane == 0) red[warp] = sum;
+        __syncthreads();
+        if (part == 0)
+            for (int i = 1; i < splits; ++i) sum += red[warp + i];
+    }
+    if (part == 0 && lane == 0 && o < O) y[(long long)o * ys] = from_float<T>(fmaf((float)sum, w_scale[o] * q_scale[0], bias ? bias[o] : 0.0f));
+}
+
+template <typename T>
+static int int8_dense_row(const int8_t *q, const float *q_scale, const int8_t *W, const float *w_scale, const float *bias, T *y, int K, int O, int ws, int ys,
+                          cudaStream_t st)
+{
+    int splits = 1;
+    while (splits < 8 && (long long)O * splits < 16LL * device_info().sm_count && (K + 511) / 512 >= 2 * splits) splits *= 2;
+    launch(k_int8_dense_row<T>, (unsigned)(((long long)O * splits + 7) / 8), 256, 0, st, q, q_scale, W, w_scale, bias, y, K, O, ws, ys, splits);
+    return launch_status();
 }
 
 // ---- the product on the tensor cores: tiles of 128 output nodes x TN frames, D[o][f] = sum_k W[o][k] q[f][k] in TMEM (lane = output node, column =
@@ -427,25 +536,34 @@ template <typename T>
 static int quantize_frames(const T *x, int8_t *q, float *scale, int N, int F, int xs, int qs, bbcu_stream_t stream)
 {
     BB200_REQUIRE(N > 0 && F >= 0, BBCU_ERR_BAD_SIZE);
-    BB200_REQUIRE(N <= (1 << 24), BBCU_ERR_TOO_LARGE);
+    BB200_REQUIRE(N <= (1 << 22), BBCU_ERR_TOO_LARGE);
     BB200_REQUIRE(xs >= F && qs >= (N + 15) / 16 * 16 && qs % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0, BBCU_ERR_BAD_STRIDE);
     if (F == 0) return BBCU_OK;
     BB200_REQUIRE_PTR(x); BB200_REQUIRE_PTR(q); BB200_REQUIRE_PTR(scale);
     cudaStream_t st = as_stream(stream);
     const bool aligned = frames_aligned<T>(x, xs);
+    BB200_REQUIRE(F <= (1 << 30), BBCU_ERR_TOO_LARGE);
+    if (ColumnPlan p = plan_columns<T>(N, F, 4, kQuantOnceRows); aligned && p.cluster && (long long)N * F <= kQuantSmall) {
+        const int per_warp = 32 / p.lanes;
+        if (p.warps * per_warp % 16) ++p.warps;                           // a round of rows is whole 16-byte pieces of q
+        p.rows = ((N + p.cluster - 1) / p.cluster + per_warp * p.warps - 1) / (per_warp * p.warps);
+        int *fault = fault_word();
+        BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
+        const int cols = p.lanes * kFramesPerVec<T>, once_tiles = (F + cols - 1) / cols, threads = 32 * p.warps, smem = p.rows * threads * 16;
+        auto kernel = p.lanes == 2 ? k_quantize_once<T, 2> : k_quantize_once<T, 4>;
+        BB200_REQUIRE(allow_big_smem(kernel, kQuantOnceRows * kColumnThreads * 16), (int)cudaErrorInvalidValue);
+        const int clusters = std::min(once_tiles, resident_clusters(reinterpret_cast<const void *>(kernel), p.cluster, threads, smem));
+        return launch_cluster(kernel, (unsigned)p.cluster, (unsigned)(clusters * p.cluster), threads, smem, st, x, q, scale, N, F, (long long)xs, (long long)qs, p.rows,
+                              once_tiles, fault);
+    }
     constexpr int kCols = Column<T, 8>::kCols;
-    const long long tiles = ((long long)F + kCols - 1) / kCols;
-    BB200_REQUIRE(tiles * kCols < (1LL << 31), BBCU_ERR_TOO_LARGE);
-    const long long want = 4LL * device_info().sm_count, per = (want + tiles - 1) / tiles;
-    int rows = (int)(((N + per - 1) / per + kQuantRows - 1) / kQuantRows * kQuantRows);
-    while ((N + rows - 1) / rows > 65535) rows *= 2;
-    const int columns = (int)(tiles * kCols), chunks = (N + rows - 1) / rows;
-    uint32_t *part = static_cast<uint32_t *>(stream_scratch(st, (size_t)chunks * columns * sizeof(uint32_t), kFrameOpSlot));
-    BB200_REQUIRE(part != nullptr, BBCU_ERR_NO_MEMORY);
-    const dim3 grid((unsigned)tiles, (unsigned)chunks);
-    launch(aligned ? k_quantize_max<T, true> : k_quantize_max<T, false>, grid, kQuantThreads, 0, st, x, part, N, F, xs, rows, columns);
-    BB200_CUDA(cudaPeekAtLastError());
-    launch(aligned ? k_quantize_apply<T, true> : k_quantize_apply<T, false>, grid, kQuantThreads, 0, st, x, q, part, scale, N, F, xs, qs, rows, chunks, columns);
+    const long long tiles = ((long long)F + kCols - 1) / kCols, bands = ((long long)N + kQuantRows - 1) / kQuantRows;
+    BB200_REQUIRE(bands <= 65535, BBCU_ERR_TOO_LARGE);
+    unsigned cl = 1;
+    while (cl < (unsigned)kMostCluster && tiles * cl <= 4LL * device_info().sm_count && N > 32 * 8 * (int)cl) cl *= 2;
+    if (const int e = launch_cluster(aligned ? k_quantize_scale<T, true> : k_quantize_scale<T, false>, cl, (unsigned)(tiles * cl), kQuantThreads, 0, st, x, scale, N, F,
+                                     (long long)xs)) return e;
+    launch(aligned ? k_quantize_apply<T, true> : k_quantize_apply<T, false>, dim3((unsigned)tiles, (unsigned)bands), kQuantThreads, 0, st, x, q, scale, N, F, xs, qs);
     return launch_status();
 }
 
@@ -461,12 +579,7 @@ static int int8_dense(const int8_t *q, const float *q_scale, const int8_t *W, co
     if (F == 0 || O == 0) return BBCU_OK;
     BB200_REQUIRE_PTR(q); BB200_REQUIRE_PTR(q_scale); BB200_REQUIRE_PTR(W); BB200_REQUIRE_PTR(w_scale); BB200_REQUIRE_PTR(y);
     cudaStream_t st = as_stream(stream);
-    if (F <= kRowFrames) {
-        constexpr int kRows = 4;
-        const long long row_ctas = ((long long)O + 8 * kRows - 1) / (8 * kRows);
-        launch(k_int8_dense_rows<T, kRowFrames, kRows>, (unsigned)row_ctas, 256, 0, st, q, q_scale, W, w_scale, bias, y, K, O, F, qs, ws, ys);
-        return launch_status();
-    }
+    if (F == 1) return int8_dense_row<T>(q, q_scale, W, w_scale, bias, y, K, O, ws, ys, st);
     int *fault = fault_word();
     BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
     GemmArgs a{q_scale, w_scale, bias, K, O, F, 1, frames_aligned<T>(y, ys), ys, fault};

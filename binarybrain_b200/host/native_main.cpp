@@ -12,6 +12,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdint>
 #include <exception>
@@ -299,12 +300,239 @@ PyObject *train_backward(PyObject *, PyObject *const *o, Py_ssize_t n)
     }
 }
 
+// ---- operators over the nodes of a frame: checks, new tensors and the call in one, as for the training step above (a call on one frame is some 5 us of
+// device time; the checks and allocations in Python took 8)
+
+bool refuse(const char *name, const char *what) { PyErr_Format(PyExc_ValueError, "%s: %s", name, what); return false; }
+
+// the size as the operators take it
+bool fits(int64_t n, int &v)
+{
+    if (n < 0 || n > INT_MAX) { PyErr_SetString(PyExc_OverflowError, "a size does not fit the operator"); return false; }
+    v = (int)n;
+    return true;
+}
+
+// A buffer of at least `frames` columns that are next to each other, rows any distance apart; `rows` < 0: any number.
+struct Frames {
+    PyObject *given = nullptr;
+    at::Tensor made;
+    const at::Tensor *t = nullptr;
+    int stride = 0;
+
+    bool check(PyObject *o, const char *name, int64_t frames, int64_t rows)
+    {
+        if (!THPVariable_Check(o)) { PyErr_Format(PyExc_TypeError, "%s: expected a tensor", name); return false; }
+        given = o;
+        t = &THPVariable_Unpack(o);
+        if (!t->is_cuda()) return refuse(name, "expected a CUDA tensor (the bbcu_* operators have no CPU path)");
+        if (t->dim() != 2 || t->size(1) < frames || (t->size(1) > 1 && t->stride(1) != 1) || (t->size(0) > 1 && t->stride(0) < frames))
+            return refuse(name, "expected [nodes, frame_stride] of at least the frames asked for, the frames of a node next to each other");
+        if (rows >= 0 && t->size(0) != rows) { PyErr_Format(PyExc_ValueError, "%s: expected %lld rows, got %lld", name, (long long)rows, (long long)t->size(0)); return false; }
+        return fits(t->size(0) > 1 ? t->stride(0) : t->size(1), stride);
+    }
+    // fp32 or bf16, or of the same type as `like`
+    bool take(PyObject *o, const char *name, int64_t frames, const at::Tensor *like, int64_t rows)
+    {
+        if (!check(o, name, frames, rows)) return false;
+        if (t->scalar_type() != at::kFloat && t->scalar_type() != at::kBFloat16) return refuse(name, "expected dtype float32 or bfloat16");
+        if (like && t->scalar_type() != like->scalar_type()) return refuse(name, "expected the dtype of the other frames");
+        return true;
+    }
+    // an output: the given buffer, or for None a new one whose rows are padded to 32 bytes
+    bool output(PyObject *o, const char *name, int64_t frames, at::ScalarType type, const at::Tensor &like, int64_t rows)
+    {
+        if (o != Py_None) {
+            if (!take(o, name, frames, nullptr, rows)) return false;
+            return t->scalar_type() == type || refuse(name, "expected the dtype of the other frames");
+        }
+        const int64_t unit = type == at::kFloat ? 8 : 16;
+        made = at::empty({rows, (frames + unit - 1) / unit * unit}, at::TensorOptions().dtype(type).device(like.device()));
+        t = &made;
+        return fits(made.size(1), stride);
+    }
+    bool fp32() const { return t->scalar_type() == at::kFloat; }
+    template <class P> P in() const { return static_cast<P>(t->const_data_ptr()); }
+    template <class P> P out() const { return static_cast<P>(t->mutable_data_ptr()); }
+    PyObject *result() const { return given ? Py_NewRef(given) : THPVariable_Wrap(made); }
+};
+
+// fp32 numbers of nodes or frames: given, or for None absent (input) or new (output)
+struct Numbers {
+    PyObject *given = nullptr;
+    at::Tensor made;
+    float *data = nullptr;
+
+    bool check(PyObject *o, const char *name, int64_t size, bool written)
+    {
+        if (!THPVariable_Check(o)) { PyErr_Format(PyExc_TypeError, "%s: expected a tensor", name); return false; }
+        const at::Tensor &t = THPVariable_Unpack(o);
+        if (!t.is_cuda()) return refuse(name, "expected a CUDA tensor (the bbcu_* operators have no CPU path)");
+        if (t.scalar_type() != at::kFloat || t.numel() < size || !t.is_contiguous()) {
+            PyErr_Format(PyExc_ValueError, "%s: expected a contiguous float32 tensor of %lld values", name, (long long)size);
+            return false;
+        }
+        data = written ? static_cast<float *>(t.mutable_data_ptr()) : const_cast<float *>(static_cast<const float *>(t.const_data_ptr()));
+        given = o;
+        return true;
+    }
+    bool input(PyObject *o, const char *name, int64_t size) { return o == Py_None || check(o, name, size, false); }
+    bool output(PyObject *o, const char *name, int64_t size, const at::Tensor &like)
+    {
+        if (o != Py_None) return check(o, name, size, true);
+        made = at::empty({size}, at::TensorOptions().dtype(at::kFloat).device(like.device()));
+        data = static_cast<float *>(made.mutable_data_ptr());
+        return true;
+    }
+    PyObject *result() const { return given ? Py_NewRef(given) : THPVariable_Wrap(made); }
+};
+
+// rows of 8-bit integers
+const at::Tensor *int8_rows(PyObject *o, const char *name)
+{
+    if (!THPVariable_Check(o)) { PyErr_Format(PyExc_TypeError, "%s: expected a tensor", name); return nullptr; }
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (!t.is_cuda() || t.scalar_type() != at::kChar || t.dim() != 2 || !t.is_contiguous()) { refuse(name, "expected a contiguous int8 CUDA tensor [rows, inputs]"); return nullptr; }
+    return &t;
+}
+
+PyObject *tuple_of(PyObject *a, PyObject *b, PyObject *c = nullptr)
+{
+    PyObject *r = a && b ? (c ? PyTuple_Pack(3, a, b, c) : PyTuple_Pack(2, a, b)) : nullptr;
+    Py_XDECREF(a); Py_XDECREF(b); Py_XDECREF(c);
+    return r;
+}
+
+bbcu_stream_t current_stream() { return reinterpret_cast<bbcu_stream_t>(c10::cuda::getCurrentCUDAStream().stream()); }
+
+// the operator of the frames' type, looked up once; a status, or INT_MIN with a Python error set
+#define BB200_CALL_OF_TYPE(fp32, name32, name16, T32, T16, ...)                                            \
+    [&] {                                                                                                  \
+        static decltype(&name32) fn32 = nullptr;                                                           \
+        static decltype(&name16) fn16 = nullptr;                                                           \
+        if (fp32 ? !bound(fn32, #name32) : !bound(fn16, #name16)) return INT_MIN;                          \
+        int status = 0;                                                                                    \
+        Py_BEGIN_ALLOW_THREADS                                                                             \
+        if (fp32) { using T = T32; status = fn32(__VA_ARGS__); } else { using T = T16; status = fn16(__VA_ARGS__); } \
+        Py_END_ALLOW_THREADS                                                                               \
+        if (status != 0) { raise_status(fp32 ? #name32 : #name16, status); return INT_MIN; }               \
+        return 0;                                                                                          \
+    }()
+
+#define BB200_GUARDED(name, args)                                                                           \
+    PyObject *name(PyObject *, PyObject *const *o, Py_ssize_t n)                                            \
+    {                                                                                                       \
+        if (n != args) { PyErr_SetString(PyExc_TypeError, #name " takes " #args " arguments"); return nullptr; } \
+        try {                                                                                               \
+            return name##_body(o);                                                                          \
+        } catch (const std::exception &e) {                                                                 \
+            PyErr_SetString(PyExc_RuntimeError, e.what());                                                  \
+            return nullptr;                                                                                 \
+        }                                                                                                   \
+    }
+
+// layer_norm_forward(x, frames, gamma, beta, eps, y, mean, rstd) -> (y, mean, rstd)
+PyObject *layer_norm_forward_body(PyObject *const *o)
+{
+    int frames, nodes;
+    float eps;
+    Frames x, y;
+    Numbers gamma, beta, mean, rstd;
+    if (!parse(o[1], frames) || !parse(o[4], eps) || !x.take(o[0], "x", frames, nullptr, -1) || !fits(x.t->size(0), nodes) || !gamma.input(o[2], "gamma", nodes) ||
+        !beta.input(o[3], "beta", nodes) || !y.output(o[5], "y", frames, x.t->scalar_type(), *x.t, nodes) || !mean.output(o[6], "mean", frames, *x.t) ||
+        !rstd.output(o[7], "rstd", frames, *x.t)) return nullptr;
+    if (BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_LayerNormalization_Forward, bbcu_bf16_LayerNormalization_Forward, float, bbcu_bf16_t, x.in<const T *>(), y.out<T *>(),
+                           gamma.data, beta.data, mean.data, rstd.data, eps, nodes, frames, x.stride, y.stride, current_stream())) return nullptr;
+    return tuple_of(y.result(), mean.result(), rstd.result());
+}
+BB200_GUARDED(layer_norm_forward, 8)
+
+// layer_norm_backward(x, dy, mean, rstd, frames, gamma, dx, dgamma, dbeta) -> (dx, dgamma, dbeta)
+PyObject *layer_norm_backward_body(PyObject *const *o)
+{
+    int frames, nodes;
+    Frames x, dy, dx;
+    Numbers gamma, mean, rstd, dgamma, dbeta;
+    if (!parse(o[4], frames) || !x.take(o[0], "x", frames, nullptr, -1) || !fits(x.t->size(0), nodes) || !dy.take(o[1], "dy", frames, x.t, nodes) ||
+        !gamma.input(o[5], "gamma", nodes) || !mean.check(o[2], "mean", frames, false) || !rstd.check(o[3], "rstd", frames, false)) return nullptr;
+    if ((o[7] == Py_None) != (o[8] == Py_None)) { refuse("dgamma and dbeta", "both or neither"); return nullptr; }
+    const int accumulate = o[7] != Py_None;
+    if (!dgamma.output(o[7], "dgamma", nodes, *x.t) || !dbeta.output(o[8], "dbeta", nodes, *x.t) ||
+        !dx.output(o[6], "dx", frames, x.t->scalar_type(), *x.t, nodes)) return nullptr;
+    if (BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_LayerNormalization_Backward, bbcu_bf16_LayerNormalization_Backward, float, bbcu_bf16_t, x.in<const T *>(), dy.in<const T *>(),
+                           dx.out<T *>(), gamma.data, mean.data, rstd.data, dgamma.data, dbeta.data, accumulate, nodes, frames, x.stride, dy.stride, dx.stride,
+                           current_stream())) return nullptr;
+    return tuple_of(dx.result(), dgamma.result(), dbeta.result());
+}
+BB200_GUARDED(layer_norm_backward, 9)
+
+// quantize_int8(x, frames) -> (q, scale)
+PyObject *quantize_int8_body(PyObject *const *o)
+{
+    int frames, nodes;
+    Frames x;
+    Numbers scale;
+    if (!parse(o[1], frames) || !x.take(o[0], "x", frames, nullptr, -1) || !fits(x.t->size(0), nodes) || !scale.output(Py_None, "scale", frames, *x.t)) return nullptr;
+    const int row = (int)std::min<int64_t>(((int64_t)nodes + 15) / 16 * 16, INT_MAX / 16 * 16);
+    at::Tensor q = at::empty({frames, row}, at::TensorOptions().dtype(at::kChar).device(x.t->device()));
+    if (BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_QuantizeInt8_Frames, bbcu_bf16_QuantizeInt8_Frames, float, bbcu_bf16_t, x.in<const T *>(),
+                           static_cast<signed char *>(q.mutable_data_ptr()), scale.data, nodes, frames, x.stride, row, current_stream())) return nullptr;
+    return tuple_of(THPVariable_Wrap(q), scale.result());
+}
+BB200_GUARDED(quantize_int8, 2)
+
+// int8_dense_forward(q, scale, W, w_scale, n_in, bias, y, bf16) -> y; n_in None: the length of q's rows; bf16: the type of a new y
+PyObject *int8_dense_forward_body(PyObject *const *o)
+{
+    int frames, nodes, n_in, q_stride, w_stride, bf16;
+    Frames y;
+    Numbers scale, w_scale, bias;
+    const at::Tensor *q = int8_rows(o[0], "q"), *W = q ? int8_rows(o[2], "W") : nullptr;
+    if (!W || !fits(q->size(0), frames) || !fits(W->size(0), nodes) || !fits(q->size(1), q_stride) || !fits(W->size(1), w_stride) || !parse_flag(o[7], bf16) ||
+        !scale.check(o[1], "scale", frames, false) || !w_scale.check(o[3], "w_scale", nodes, false) || !bias.input(o[5], "bias", nodes)) return nullptr;
+    n_in = q_stride;
+    if (o[4] != Py_None && !parse(o[4], n_in)) return nullptr;
+    if (o[6] != Py_None ? !y.take(o[6], "y", frames, nullptr, nodes) : !y.output(Py_None, "y", frames, bf16 ? at::kBFloat16 : at::kFloat, *q, nodes)) return nullptr;
+    if (BB200_CALL_OF_TYPE(y.fp32(), bbcu_int8_fp32_DenseAffine_Forward, bbcu_int8_bf16_DenseAffine_Forward, float, bbcu_bf16_t,
+                           static_cast<const signed char *>(q->const_data_ptr()), scale.data, static_cast<const signed char *>(W->const_data_ptr()), w_scale.data,
+                           bias.data, y.out<T *>(), n_in, nodes, frames, q_stride, w_stride, y.stride, current_stream())) return nullptr;
+    return y.result();
+}
+BB200_GUARDED(int8_dense_forward, 8)
+
+// distillation_loss(z, t, index, frames, temperature, t_lse, weight, batch_size, dz, loss_buf) -> (dz, loss, loss_buf)
+PyObject *distillation_loss_body(PyObject *const *o)
+{
+    int frames, classes, top;
+    float temperature;
+    double batch;
+    Frames z, t, index, dz;
+    Numbers t_lse, weight, loss_buf;
+    if (!parse(o[3], frames) || !parse(o[4], temperature) || !z.take(o[0], "z", frames, nullptr, -1) || !fits(z.t->size(0), classes) ||
+        !t.take(o[1], "t", frames, z.t, -1) || !fits(t.t->size(0), top) || !index.check(o[2], "index", frames, top)) return nullptr;
+    if (index.t->scalar_type() != at::kInt) { refuse("index", "expected dtype int32"); return nullptr; }
+    if (!t_lse.input(o[5], "t_lse", frames) || !weight.input(o[6], "weight", frames) || !dz.output(o[8], "dz", frames, z.t->scalar_type(), *z.t, classes) ||
+        !loss_buf.output(o[9], "loss_buf", frames, *z.t)) return nullptr;
+    batch = frames;
+    if (o[7] != Py_None && !parse(o[7], batch)) return nullptr;
+    const double reduction = 1.0 / (batch > 1.0 ? batch : 1.0);
+    at::Tensor loss = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(z.t->device()));
+    float *const loss_data = static_cast<float *>(loss.mutable_data_ptr());
+    if (BB200_CALL_OF_TYPE(z.fp32(), bbcu_fp32_LossDistillation, bbcu_bf16_LossDistillation, float, bbcu_bf16_t, z.in<const T *>(), dz.out<T *>(), t.in<const T *>(),
+                           index.in<const int *>(), t_lse.data, weight.data, loss_buf.data, loss_data, temperature, (float)reduction, reduction, classes, top, frames,
+                           z.stride, dz.stride, t.stride, index.stride, current_stream())) return nullptr;
+    return tuple_of(dz.result(), THPVariable_Wrap(loss), loss_buf.result());
+}
+BB200_GUARDED(distillation_loss, 10)
+
 #define BB200_METHOD(name, function) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(function)), METH_FASTCALL, nullptr},
 #define BB200_OPERATOR_METHOD(name) BB200_METHOD(#name, py_##name)
 PyMethodDef g_methods[] = {
     BB200_OPERATORS(BB200_OPERATOR_METHOD)
     BB200_METHOD("empty_f32", empty_f32) BB200_METHOD("empty_i32", empty_i32) BB200_METHOD("vector_f32", vector_f32) BB200_METHOD("scalar_f64", scalar_f64)
     BB200_METHOD("train_forward", train_forward) BB200_METHOD("train_backward", train_backward)
+    BB200_METHOD("layer_norm_forward", layer_norm_forward) BB200_METHOD("layer_norm_backward", layer_norm_backward) BB200_METHOD("quantize_int8", quantize_int8)
+    BB200_METHOD("int8_dense_forward", int8_dense_forward) BB200_METHOD("distillation_loss", distillation_loss)
     {nullptr, nullptr, 0, nullptr}};
 #undef BB200_METHOD
 

@@ -397,72 +397,20 @@ def int8_stride(nodes):
     return (nodes + 15) // 16 * 16
 
 
-def _frames(t, name, frames, like=None, rows=None):
-    """An fp32 or bf16 frame buffer of at least `frames` frames: [rows, stride], frames contiguous; rows may be any distance apart."""
-    if not t.is_cuda:
-        raise ValueError(f"{name}: expected a CUDA tensor (the bbcu_* operators have no CPU path)")
-    if t.dtype not in (torch.float32, torch.bfloat16) or (like is not None and t.dtype != like.dtype):
-        raise ValueError(f"{name}: expected dtype {'float32 or bfloat16' if like is None else like.dtype}, got {t.dtype}")
-    if t.dim() != 2 or t.shape[1] < frames or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < frames):
-        raise ValueError(f"{name}: expected [nodes, frame_stride] of at least {frames} frames, the frames of a node next to each other")
-    if rows is not None and t.shape[0] != rows:
-        raise ValueError(f"{name}: expected {rows} rows, got {t.shape[0]}")
-    return t
-
-
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-
-
-def _vector(t, name, size, dtype=torch.float32):
-    if t is not None and (not t.is_cuda or t.dtype != dtype or t.numel() < size or not t.is_contiguous()):
-        raise ValueError(f"{name}: expected a contiguous {dtype} CUDA tensor of {size} values")
-    return t
-
-
-def _for_type(fp32, bf16, t):
-    return fp32 if t.dtype == torch.float32 else bf16
-
-
 def layer_norm_forward(x, frames, gamma=None, beta=None, eps=1e-5, y=None, mean=None, rstd=None):
     """Layer norm over the nodes of every frame: returns (y, mean, rstd), y = (x - mean) * rstd * gamma + beta, the statistics [frames] fp32."""
-    _frames(x, "x", frames)
-    nodes = x.shape[0]
-    _vector(gamma, "gamma", nodes); _vector(beta, "beta", nodes)
-    y = torch.empty((nodes, frame_stride(frames, x.dtype)), dtype=x.dtype, device=x.device) if y is None else _frames(y, "y", frames, x, nodes)
-    mean = _n.vector_f32(x, frames) if mean is None else _vector(mean, "mean", frames)
-    rstd = _n.vector_f32(x, frames) if rstd is None else _vector(rstd, "rstd", frames)
-    _for_type(_n.bbcu_fp32_LayerNormalization_Forward, _n.bbcu_bf16_LayerNormalization_Forward, x)(
-        x, y, gamma, beta, mean, rstd, eps, nodes, frames, _row_stride(x), _row_stride(y))
-    return y, mean, rstd
+    return _n.layer_norm_forward(x, frames, gamma, beta, eps, y, mean, rstd)
 
 
 def layer_norm_backward(x, dy, mean, rstd, frames, gamma=None, dx=None, dgamma=None, dbeta=None):
     """Returns (dx, dgamma, dbeta).  dx is overwritten; dgamma and dbeta are accumulated into where they are given (both or neither)."""
-    _frames(x, "x", frames)
-    nodes = x.shape[0]
-    _frames(dy, "dy", frames, x, nodes)
-    _vector(gamma, "gamma", nodes); _vector(mean, "mean", frames); _vector(rstd, "rstd", frames)
-    if (dgamma is None) != (dbeta is None):
-        raise ValueError("dgamma and dbeta: both or neither")
-    accumulate = dgamma is not None
-    dgamma = _vector(dgamma, "dgamma", nodes) if accumulate else _n.vector_f32(x, nodes)
-    dbeta = _vector(dbeta, "dbeta", nodes) if accumulate else _n.vector_f32(x, nodes)
-    dx = torch.empty((nodes, frame_stride(frames, x.dtype)), dtype=x.dtype, device=x.device) if dx is None else _frames(dx, "dx", frames, x, nodes)
-    _for_type(_n.bbcu_fp32_LayerNormalization_Backward, _n.bbcu_bf16_LayerNormalization_Backward, x)(
-        x, dy, dx, gamma, mean, rstd, dgamma, dbeta, int(accumulate), nodes, frames, _row_stride(x), _row_stride(dy), _row_stride(dx))
-    return dx, dgamma, dbeta
+    return _n.layer_norm_backward(x, dy, mean, rstd, frames, gamma, dx, dgamma, dbeta)
 
 
 def quantize_int8(x, frames):
     """Frames of an fp32 or bf16 buffer [nodes, frame_stride] as rows of 8-bit integers: returns (q [frames, int8_stride(nodes)], scale [frames]),
     x ~ q * scale with scale = max|x| / 127 of the frame."""
-    _frames(x, "x", frames)
-    nodes = x.shape[0]
-    q = torch.empty((frames, int8_stride(nodes)), dtype=torch.int8, device=x.device)
-    scale = _n.vector_f32(x, frames)
-    _for_type(_n.bbcu_fp32_QuantizeInt8_Frames, _n.bbcu_bf16_QuantizeInt8_Frames, x)(x, q, scale, nodes, frames, _row_stride(x), q.shape[1])
-    return q, scale
+    return _n.quantize_int8(x, frames)
 
 
 def quantize_int8_channels(W):
@@ -477,16 +425,9 @@ def quantize_int8_channels(W):
 def int8_dense_forward(q, scale, W, w_scale, n_in=None, bias=None, y=None, dtype=torch.float32):
     """y[o][f] = w_scale[o] * scale[f] * sum_k W[o][k] * q[f][k] + bias[o] as a frame buffer of `dtype` (fp32 or bf16).  q [frames, >= n_in] and
     W [out, >= n_in] are rows as the quantisers make them; n_in: inputs, where rows are longer than that (default: the length of q's rows)."""
-    for t, name in ((q, "q"), (W, "W")):
-        if not t.is_cuda or t.dtype != torch.int8 or t.dim() != 2 or not t.is_contiguous():
-            raise ValueError(f"{name}: expected a contiguous int8 CUDA tensor [rows, inputs]")
-    frames, nodes = q.shape[0], W.shape[0]
-    n_in = q.shape[1] if n_in is None else n_in
-    _vector(scale, "scale", frames); _vector(w_scale, "w_scale", nodes); _vector(bias, "bias", nodes)
-    y = torch.empty((nodes, frame_stride(frames, dtype)), dtype=dtype, device=q.device) if y is None else _frames(y, "y", frames, None, nodes)
-    _for_type(_n.bbcu_int8_fp32_DenseAffine_Forward, _n.bbcu_int8_bf16_DenseAffine_Forward, y)(
-        q, scale, W, w_scale, bias, y, n_in, nodes, frames, q.shape[1], W.shape[1], _row_stride(y))
-    return y
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"dtype: expected float32 or bfloat16, got {dtype}")
+    return _n.int8_dense_forward(q, scale, W, w_scale, n_in, bias, y, dtype == torch.bfloat16)
 
 
 def distillation_loss(z, t, index, frames, temperature=1.0, t_lse=None, weight=None, batch_size=None, dz=None, loss_buf=None):
@@ -494,21 +435,7 @@ def distillation_loss(z, t, index, frames, temperature=1.0, t_lse=None, weight=N
     classes index [top, frame_stride] (int32; outside [0, classes): an empty slot) are known, at `temperature` and times its square.  The teacher's
     probabilities are those among its slots or, with t_lse [frames] = log sum exp(t / temperature) over all of its classes, the true ones.  Returns
     (dz, loss, loss_buf): the gradient of loss, the mean over batch_size frames (default: these), and weight * loss of every frame."""
-    _frames(z, "z", frames)
-    classes, top = z.shape[0], t.shape[0]
-    _frames(t, "t", frames, z)
-    if not index.is_cuda or index.dtype != torch.int32 or index.dim() != 2 or index.shape[0] != top or index.shape[1] < frames or \
-            (index.shape[1] > 1 and index.stride(1) != 1) or (top > 1 and index.stride(0) < frames):
-        raise ValueError(f"index: expected an int32 CUDA tensor [{top}, at least {frames}], the frames of a slot next to each other")
-    _vector(t_lse, "t_lse", frames); _vector(weight, "weight", frames)
-    dz = torch.empty((classes, frame_stride(frames, z.dtype)), dtype=z.dtype, device=z.device) if dz is None else _frames(dz, "dz", frames, z, classes)
-    loss_buf = _n.vector_f32(z, frames) if loss_buf is None else _vector(loss_buf, "loss_buf", frames)
-    loss = torch.empty((), dtype=torch.float32, device=z.device)
-    reduction = 1.0 / max(1, frames if batch_size is None else batch_size)
-    _for_type(_n.bbcu_fp32_LossDistillation, _n.bbcu_bf16_LossDistillation, z)(
-        z, dz, t, index, t_lse, weight, loss_buf, loss, temperature, reduction, reduction, classes, top, frames, _row_stride(z), _row_stride(dz), _row_stride(t),
-        _row_stride(index))
-    return dz, loss, loss_buf
+    return _n.distillation_loss(z, t, index, frames, temperature, t_lse, weight, batch_size, dz, loss_buf)
 
 
 # ------------------------------------------------------------------------------------------ frame-sharded halves
