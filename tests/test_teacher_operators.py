@@ -607,3 +607,39 @@ def test_refusals_of_the_tensor_calls_on_the_device():
     for call in (lambda: ops.distillation_loss(x, x[:2], idx, 8, temperature=0.0), lambda: ops.layer_norm_forward(x, 8, eps=-1.0), lambda: ops.int8_dense_forward(q, v, q, v, n_in=17)):
         with pytest.raises(abi.BbcuError):
             call()
+
+
+@pytest.mark.gpu
+def test_a_lut_network_learns_from_an_int8_teacher():
+    """The example: all operators together.  A loss of 100 steps on is well below the first one, the mean divergence from the teacher of a student that knows
+    nothing; and every step leaves the numbers that the next one needs finite."""
+    import importlib.util
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location("distill_int8_teacher", os.path.join(root, "examples", "distill_int8_teacher.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses = example.train(steps=101, frames=333)
+    assert all(math.isfinite(v) for v in losses) and losses[-1] < 0.7 * losses[0]
+
+
+@pytest.mark.gpu
+def test_the_teachers_layers_are_their_operators():
+    from binarybrain_b200 import ops
+    from binarybrain_b200.teacher import Int8Dense, LayerNormalization, top_logits
+    x, dy = (buffer(normal(s, 90, 21), torch.float32) for s in (0, 1))
+    norm = LayerNormalization(90, gamma=1.5, beta=0.25)
+    y = norm.forward(x, 21)
+    want, mean, rstd = ops.layer_norm_forward(x, 21, gamma=norm.gamma, beta=norm.beta)
+    assert torch.equal(y[:, :21], want[:, :21])
+    for turn in (1, 2):                                                  # the gradients of the weights add up
+        if turn == 2:
+            norm.forward(x, 21)
+        dx = norm.backward(dy)
+        dx_w, dgamma, dbeta = ops.layer_norm_backward(x, dy, mean, rstd, 21, gamma=norm.gamma)
+        assert torch.equal(dx[:, :21], dx_w[:, :21]) and torch.equal(norm.dgamma, turn * dgamma) and torch.equal(norm.dbeta, turn * dbeta)
+    W = normal(2, 30, 90).float().cuda()
+    z = Int8Dense(W).forward(y, 21)
+    assert torch.equal(z[:, :21], ops.int8_dense_forward(*ops.quantize_int8(y, 21), *ops.quantize_int8_channels(W), n_in=90)[:, :21])
+    t, index = top_logits(z, 21, 4)
+    assert torch.equal(t[:, :21], torch.gather(z, 0, index[:, :21].long())) and (t[:-1, :21] >= t[1:, :21]).all()
