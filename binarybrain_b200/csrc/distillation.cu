@@ -76,10 +76,19 @@ template <> __device__ __forceinline__ uint4 packed_max<__nv_bfloat16>(const uin
 
 // ---- the teacher's side of COLS frames from f0 on, by a CTA of a multiple of COLS threads: thread t has column t % COLS and every (threads / COLS)-th
 // slot of it.  index[slot][column] (-1: empty) and p[slot][column] go to shared memory, and to each thread, for its column, P = sum p, E = sum p log p
-// and the weight (0: the frame takes no part).  A barrier stands behind the last write.
+// and the weight (0: the frame takes no part).  A barrier stands behind the last write of the two; red[0] and red[1] may still be read.
 struct TeacherColumn { float P, E, weight; };
+
+// a value of each column joined over the lanes of a warp that have it
+template <int COLS, typename JOIN> __device__ __forceinline__ float column_of_warp(float v, JOIN join)
+{
+#pragma unroll
+    for (int m = COLS; m < 32; m <<= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, m));
+    return v;
+}
+
 template <typename T, int COLS>
-__device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, int f0, int *index, float *p, float (&red)[2][kColumnThreads])
+__device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, int f0, int *index, float *p, float (&red)[3][kColumnThreads / 32 * COLS])
 {
     const int col = threadIdx.x % COLS, group = threadIdx.x / COLS, groups = blockDim.x / COLS, f = f0 + col;
     const float w = f < a.F ? (a.weight ? a.weight[f] : 1.0f) : 0.0f;
@@ -96,28 +105,32 @@ __device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, in
         p[k * COLS + col] = t;
         if (i >= 0) { top = fmaxf(top, t); slots += 1.0f; }
     }
-    red[0][threadIdx.x] = top;
-    red[1][threadIdx.x] = slots;
+    const int warps = blockDim.x / 32, own = threadIdx.x / 32 * COLS + threadIdx.x % 32;
+    top = column_of_warp<COLS>(top, [](float a, float b) { return fmaxf(a, b); });
+    slots = column_of_warp<COLS>(slots, [](float a, float b) { return a + b; });
+    if (threadIdx.x % 32 < COLS) {
+        red[0][own] = top;
+        red[1][own] = slots;
+    }
     __syncthreads();
-    top = -INFINITY;
-    slots = 0.0f;
-    for (int e = col; e < (int)blockDim.x; e += COLS) { top = fmaxf(top, red[0][e]); slots += red[1][e]; }
+    top = red[0][col];
+    slots = red[1][col];
+    for (int e = 1; e < warps; ++e) { top = fmaxf(top, red[0][e * COLS + col]); slots += red[1][e * COLS + col]; }
     const bool live = slots > 0.0f && w != 0.0f;
     float lse = 0.0f;
     if (a.t_lse) {
         if (live) lse = a.t_lse[f];
-        __syncthreads();
+        __syncthreads();                                                  // (the two sums are read before the next two take their place)
     } else {
         float sum = 0.0f;
         for (int k = group; k < a.K; k += groups)
             if (index[k * COLS + col] >= 0) sum += exp2_fast((p[k * COLS + col] - top) * a.scale);
+        sum = column_of_warp<COLS>(sum, [](float a, float b) { return a + b; });
+        if (threadIdx.x % 32 < COLS) red[2][own] = sum;
         __syncthreads();
-        red[0][threadIdx.x] = sum;
-        __syncthreads();
-        sum = 0.0f;
-        for (int e = col; e < (int)blockDim.x; e += COLS) sum += red[0][e];
+        sum = red[2][col];
+        for (int e = 1; e < warps; ++e) sum += red[2][e * COLS + col];
         lse = top * a.inv_t + logf(sum);
-        __syncthreads();
     }
     float P = 0.0f, E = 0.0f;
     for (int k = group; k < a.K; k += groups) {
@@ -130,12 +143,15 @@ __device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, in
         }
         p[k * COLS + col] = q;
     }
-    red[0][threadIdx.x] = P;
-    red[1][threadIdx.x] = E;
+    P = column_of_warp<COLS>(P, [](float a, float b) { return a + b; });
+    E = column_of_warp<COLS>(E, [](float a, float b) { return a + b; });
+    if (threadIdx.x % 32 < COLS) {
+        red[0][own] = P;
+        red[1][own] = E;
+    }
     __syncthreads();
-    TeacherColumn c = {0.0f, 0.0f, live ? w : 0.0f};
-    for (int e = col; e < (int)blockDim.x; e += COLS) { c.P += red[0][e]; c.E += red[1][e]; }
-    __syncthreads();
+    TeacherColumn c = {red[0][col], red[1][col], live ? w : 0.0f};
+    for (int e = 1; e < warps; ++e) { c.P += red[0][e * COLS + col]; c.E += red[1][e * COLS + col]; }
     return c;
 }
 
@@ -187,8 +203,7 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
     static_assert(kCols <= 32, "a warp finishes the columns");
     extern __shared__ __align__(16) uint8_t buffer[];
-    __shared__ float red[2][kColumnThreads], red_soft[kColumnThreads / 32][kCols], s_top[kCols];
-    __shared__ float part[2][kDistillCluster][4][kCols];
+    __shared__ float red[3][kColumnThreads / 32 * kCols], red_soft[kColumnThreads / 32][kCols], s_top[kCols];
     __shared__ FrameGrad s_grad[kCols];
     __shared__ uint64_t bar[2];
     __shared__ int gave_up;
@@ -201,7 +216,9 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
     int *const index = reinterpret_cast<int *>(buffer + rows * piece);
     float *const p = reinterpret_cast<float *>(index + a.K * kCols);
     unsigned *const seen = reinterpret_cast<unsigned *>(p + a.K * kCols);   // a bit for each of the CTA's classes and columns: has a slot named it?
-    for (int i = threadIdx.x; i < (c.step * rows + 31) / 32 * kCols; i += blockDim.x) seen[i] = 0u;
+    const int seen_words = (c.step * rows + 31) / 32 * kCols;
+    float (*const part)[4][kCols] = reinterpret_cast<float (*)[4][kCols]>(seen + seen_words);      // [two exchanges of the cluster's CTAs]
+    for (int i = threadIdx.x; i < seen_words; i += blockDim.x) seen[i] = 0u;
     const long long z_step = c.step * a.zs, dz_step = c.step * a.dzs;
     const T *const z_first = a.z + first * a.zs;
     // the logit of a class of this CTA in a column of the tile
@@ -294,18 +311,25 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
                 }
             }
         }
-        red[0][threadIdx.x] = cross;
-        red[1][threadIdx.x] = own_p;
+        cross = column_of_warp<kCols>(cross, [](float a, float b) { return a + b; });
+        own_p = column_of_warp<kCols>(own_p, [](float a, float b) { return a + b; });
+        if (c.lane < kCols) {
+            red[0][c.warp * kCols + c.lane] = cross;
+            red[1][c.warp * kCols + c.lane] = own_p;
+        }
         if (cl > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(&bar[turn & 1], cl * 4 * kCols * (uint32_t)sizeof(float));
         twice = __syncthreads_or(twice);
         if (threadIdx.x < kCols) {                                        // all of them in the first warp
             float s = 0.0f;
             cross = own_p = 0.0f;
-            for (int w = 0; w < c.warps; ++w) s += red_soft[w][threadIdx.x];
-            for (int e = threadIdx.x; e < (int)blockDim.x; e += kCols) { cross += red[0][e]; own_p += red[1][e]; }
+            for (int w = 0; w < c.warps; ++w) {
+                s += red_soft[w][threadIdx.x];
+                cross += red[0][w * kCols + threadIdx.x];
+                own_p += red[1][w * kCols + threadIdx.x];
+            }
             SoftSum joined = {s_top[threadIdx.x], s};
             if (cl > 1) {
-                float (*const to)[kCols] = part[turn & 1][rank];
+                float (*const from)[4][kCols] = part + (turn & 1) * cl, (*const to)[kCols] = from[rank];
                 for (uint32_t r = 0; r < cl; ++r) {
                     const uint32_t b = peer_addr(&bar[turn & 1], r);
                     peer_send(peer_addr(&to[0][threadIdx.x], r), joined.top, b);
@@ -318,7 +342,6 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
                     if (mbar_try_wait(&bar[turn & 1], turn >> 1 & 1)) break;
                     if (i == kWaitSpins - 1) { *(volatile int *)&gave_up = 1; ok = false; }
                 }
-                const float (*from)[4][kCols] = part[turn & 1];
                 joined = {from[0][0][threadIdx.x], from[0][1][threadIdx.x]};
                 for (uint32_t r = 1; r < cl; ++r) joined = join_soft(joined, {from[r][0][threadIdx.x], from[r][1][threadIdx.x]}, a.scale);
                 cross = 0.0f;
@@ -373,19 +396,54 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
     }
 }
 
-// ---- more classes than that: the softmax's sums, what follows from them for a frame, dz of all classes, dz of the named ones.
-// part[chunk of classes][column]
+// ---- more classes than that: the teacher's side beside the softmax's sums, what follows from both for a frame, dz of all classes, dz of the named ones.
+// The teacher's CTAs have eight frames, 32 threads for each, and leave P, E and weight as teacher[3][columns] and the slots as the last kernel takes them:
+// the class, or -1 where the slot is empty or names a class that an earlier one does, and the probabilities of a class added up.
+constexpr int kFinishCols = 8, kFinishGroups = kColumnThreads / kFinishCols;
+template <typename T>
+__device__ __forceinline__ void teacher_slots(const Distill<T> &a, int cta, float *teacher, int *slot_index, float *slot_p, int columns)
+{
+    extern __shared__ __align__(16) uint8_t buffer[];
+    __shared__ float red[3][kColumnThreads / 32 * kFinishCols];
+    int *const index = reinterpret_cast<int *>(buffer);
+    float *const p = reinterpret_cast<float *>(index + a.K * kFinishCols);
+    const int col = threadIdx.x % kFinishCols, group = threadIdx.x / kFinishCols, f = cta * kFinishCols + col;
+    const TeacherColumn c = teacher_columns<T, kFinishCols>(a, cta * kFinishCols, index, p, red);
+    for (int k = group; k < a.K; k += kFinishGroups) {
+        const int i = index[k * kFinishCols + col];
+        bool leads = false;
+        float q = 0.0f;
+        if (i >= 0) q = named_slots<kFinishCols>(index, p, a.K, k, col, leads);
+        slot_index[(long long)k * columns + f] = leads ? i : -1;
+        slot_p[(long long)k * columns + f] = q;
+    }
+    if (group == 0) {
+        teacher[f] = c.P;
+        teacher[columns + f] = c.E;
+        teacher[2LL * columns + f] = c.weight;
+    }
+}
+
+// part[chunk of classes][column], by the CTAs behind the teacher's.  A thread's sum is relative to a logit not much below its largest one: it changes
+// only where one is 2^64 times as much, so that the rows cost little more than their exponentials.
 template <typename T, int LPR, bool ALIGNED>
 __global__ void __launch_bounds__(kColumnThreads, 3)
-k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int columns)
+k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, float *teacher, int *slot_index, float *slot_p, int teacher_ctas)
 {
     grid_dependency();
     constexpr int kBatch = 8;
     using Col = Column<T, LPR>;
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
     __shared__ SoftSum red[kColumnThreads / 32][kCols];
+    const int columns = tiles * kCols;
+    if ((int)blockIdx.x < teacher_ctas) {
+        teacher_slots(a, (int)blockIdx.x, teacher, slot_index, slot_p, columns);
+        return;
+    }
     const Col c;
-    const int f = (int)blockIdx.x * kCols + c.col, step = c.step, n0 = (int)blockIdx.y * chunk_rows, n1 = min(a.C, n0 + chunk_rows);
+    const int cta = (int)blockIdx.x - teacher_ctas, tile = cta % tiles, chunk = cta / tiles;
+    const int f = tile * kCols + c.col, step = c.step, n0 = chunk * chunk_rows, n1 = min(a.C, n0 + chunk_rows);
+    const float most_above = 64.0f / a.scale;
     SoftSum s[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) s[j] = {-INFINITY, 0.0f};
@@ -400,15 +458,20 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int columns)
         for (int i = 1; i < B; ++i) most = packed_max<T>(most, raw[i]);
         float top[kVec];
         unpack<T>(most, top);
+        bool above = false;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-            top[j] = fmaxf(s[j].top, top[j]);
-            if (s[j].top != top[j]) {
-                if (s[j].top != -INFINITY) s[j].sum *= exp2_fast((s[j].top - top[j]) * a.scale);
-                s[j].top = top[j];
+        for (int j = 0; j < kVec; ++j) above |= top[j] > s[j].top + most_above;
+        if (above) {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                if (top[j] > s[j].top) {
+                    if (s[j].top != -INFINITY) s[j].sum *= exp2_fast((s[j].top - top[j]) * a.scale);
+                    s[j].top = top[j];
+                }
             }
-            top[j] = reference(top[j]);
         }
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) top[j] = reference(s[j].top);
 #pragma unroll
         for (int i = 0; i < B; ++i) {
             float v[kVec];
@@ -433,52 +496,47 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int columns)
     if (threadIdx.x < kCols) {
         SoftSum t = red[0][threadIdx.x];
         for (int w = 1; w < c.warps; ++w) t = join_soft(t, red[w][threadIdx.x], a.scale);
-        part[(long long)blockIdx.y * columns + (long long)blockIdx.x * kCols + threadIdx.x] = t;
+        part[(long long)chunk * columns + tile * kCols + threadIdx.x] = t;
     }
 }
 
-// The numbers of FrameGrad as grad[4][columns], the frames' losses, and the slots as the last kernel takes them: the class, or -1 where the slot is empty
-// or names a class that an earlier one does, and the probabilities of a class added up.  A CTA has eight frames, 32 threads for each.
-constexpr int kFinishCols = 8;
+// The numbers of FrameGrad as grad[4][columns], and the frames' losses
 template <typename T>
 __global__ void __launch_bounds__(kColumnThreads)
-k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunks, float *grad, int *slot_index, float *slot_p, int columns)
+k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunks, const float *__restrict__ teacher, const int *__restrict__ slot_index,
+                 const float *__restrict__ slot_p, float *grad, int columns)
 {
     grid_dependency();
-    extern __shared__ __align__(16) uint8_t buffer[];
-    __shared__ float red[2][kColumnThreads], s_top[kFinishCols];
-    __shared__ SoftSum sums[kColumnThreads / kFinishCols][kFinishCols];
-    int *const index = reinterpret_cast<int *>(buffer);
-    float *const p = reinterpret_cast<float *>(index + a.K * kFinishCols);
-    const int col = threadIdx.x % kFinishCols, group = threadIdx.x / kFinishCols, f = (int)blockIdx.x * kFinishCols + col;
-    constexpr int kGroups = kColumnThreads / kFinishCols;
+    __shared__ SoftSum sums[kColumnThreads / 32][kFinishCols];
+    __shared__ float red[kColumnThreads / 32][kFinishCols], s_top[kFinishCols];
+    const int col = threadIdx.x % kFinishCols, group = threadIdx.x / kFinishCols, warp = threadIdx.x / 32, f = (int)blockIdx.x * kFinishCols + col;
     SoftSum s = {-INFINITY, 0.0f};
-    for (int k = group; k < chunks; k += kGroups) s = join_soft(s, part[(long long)k * columns + f], a.scale);
-    sums[group][col] = s;
-    const TeacherColumn teacher = teacher_columns<T, kFinishCols>(a, (int)blockIdx.x * kFinishCols, index, p, red);
-    if (group == 0) {
-        for (int k = 1; k < kGroups; ++k) s = join_soft(s, sums[k][col], a.scale);
+    for (int k = group; k < chunks; k += kFinishGroups) s = join_soft(s, part[(long long)k * columns + f], a.scale);
+#pragma unroll
+    for (int m = kFinishCols; m < 32; m <<= 1) s = join_soft(s, {__shfl_xor_sync(0xffffffffu, s.top, m), __shfl_xor_sync(0xffffffffu, s.sum, m)}, a.scale);
+    if (threadIdx.x % 32 < kFinishCols) sums[warp][col] = s;
+    __syncthreads();
+    if (threadIdx.x < kFinishCols) {
+        for (int w = 1; w < kColumnThreads / 32; ++w) s = join_soft(s, sums[w][col], a.scale);
         s_top[col] = reference(s.top);
     }
     __syncthreads();
+    const float top = s_top[col];
     float cross = 0.0f;
-    for (int k = group; k < a.K; k += kGroups) {
-        const int i = index[k * kFinishCols + col];
-        float q = p[k * kFinishCols + col];
-        if (i >= 0 && q != 0.0f) cross += q * ((to_float(a.z[i * a.zs + f]) - s_top[col]) * a.inv_t);
-        bool leads = false;
-        if (i >= 0) q = named_slots<kFinishCols>(index, p, a.K, k, col, leads);
-        slot_index[(long long)k * columns + f] = leads ? i : -1;
-        slot_p[(long long)k * columns + f] = q;
+    for (int k = group; k < a.K; k += kFinishGroups) {
+        const int i = slot_index[(long long)k * columns + f];
+        const float q = slot_p[(long long)k * columns + f];
+        if (i >= 0 && q != 0.0f) cross += q * ((to_float(a.z[i * a.zs + f]) - top) * a.inv_t);
     }
-    red[0][threadIdx.x] = cross;
+    cross = column_of_warp<kFinishCols>(cross, [](float x, float y) { return x + y; });
+    if (threadIdx.x % 32 < kFinishCols) red[warp][col] = cross;
     __syncthreads();
     if (threadIdx.x < 32) {
         float loss = 0.0f;
         if (group == 0) {
             cross = 0.0f;
-            for (int e = col; e < kColumnThreads; e += kFinishCols) cross += red[0][e];
-            const FrameGrad g = finish_frame(a, teacher, s, cross, loss);
+            for (int w = 0; w < kColumnThreads / 32; ++w) cross += red[w][col];
+            const FrameGrad g = finish_frame(a, TeacherColumn{teacher[f], teacher[columns + f], teacher[2LL * columns + f]}, s, cross, loss);
             grad[f] = g.top;
             grad[columns + f] = g.factor;
             grad[2LL * columns + f] = g.cap;
@@ -559,7 +617,8 @@ static int distillation_once(const Distill<T> &a, const ColumnPlan &p, int tiles
     BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
     auto kernel = k_distill_once<T, LPR>;
     constexpr int kCols = Column<T, LPR>::kCols;
-    const int threads = 32 * p.warps, smem = p.rows * threads * 16 + a.K * kCols * 8 + (p.warps * 32 / LPR * p.rows + 31) / 32 * kCols * 4;
+    const int threads = 32 * p.warps, smem = p.rows * threads * 16 + a.K * kCols * 8 + (p.warps * 32 / LPR * p.rows + 31) / 32 * kCols * 4 +
+              (p.cluster > 1 ? 2 * p.cluster * 4 * kCols * 4 : 0);
     BB200_REQUIRE(allow_big_smem(kernel, kDistillSmem), (int)cudaErrorInvalidValue);
     const int clusters = std::min(tiles, resident_clusters(reinterpret_cast<const void *>(kernel), p.cluster, threads, smem));
     return launch_cluster(kernel, (unsigned)p.cluster, (unsigned)(clusters * p.cluster), threads, smem, st, a, p.rows, tiles, fault);
@@ -592,15 +651,17 @@ static int distillation_passes(Distill<T> &a, int &loss_parts, bool aligned, cud
     const int rows = (a.C + chunks - 1) / chunks;
     loss_parts = columns / kFinishCols;
     const size_t part_b = (size_t)chunks * columns * sizeof(SoftSum), loss_b = (size_t)loss_parts * sizeof(double), slots = (size_t)a.K * columns;
-    char *scratch = static_cast<char *>(stream_scratch(st, loss_b + part_b + ((size_t)4 * columns + 2 * slots) * 4, kFrameOpSlot));
+    char *scratch = static_cast<char *>(stream_scratch(st, loss_b + part_b + ((size_t)7 * columns + 2 * slots) * 4, kFrameOpSlot));
     BB200_REQUIRE(scratch != nullptr, BBCU_ERR_NO_MEMORY);
     a.loss_part = reinterpret_cast<double *>(scratch);
     SoftSum *part = reinterpret_cast<SoftSum *>(scratch + loss_b);
-    float *grad = reinterpret_cast<float *>(scratch + loss_b + part_b), *slot_p = grad + (size_t)4 * columns;
+    float *grad = reinterpret_cast<float *>(scratch + loss_b + part_b), *teacher = grad + (size_t)4 * columns, *slot_p = teacher + (size_t)3 * columns;
     int *slot_index = reinterpret_cast<int *>(slot_p + slots);
-    launch(sums, dim3((unsigned)tiles, (unsigned)chunks), kColumnThreads, 0, st, a, part, rows, columns);
+    const size_t teacher_smem = (size_t)a.K * kFinishCols * 8;
+    BB200_REQUIRE((long long)tiles * chunks + loss_parts < (1LL << 31), BBCU_ERR_TOO_LARGE);
+    launch(sums, (unsigned)(tiles * chunks + loss_parts), kColumnThreads, teacher_smem, st, a, part, rows, tiles, teacher, slot_index, slot_p, loss_parts);
     BB200_CUDA(cudaPeekAtLastError());
-    launch(k_distill_finish<T>, (unsigned)loss_parts, kColumnThreads, (size_t)a.K * kFinishCols * 8, st, a, part, chunks, grad, slot_index, slot_p, columns);
+    launch(k_distill_finish<T>, (unsigned)loss_parts, kColumnThreads, 0, st, a, part, chunks, teacher, slot_index, slot_p, grad, columns);
     BB200_CUDA(cudaPeekAtLastError());
     launch(aligned ? k_distill_apply<T, true> : k_distill_apply<T, false>, dim3((unsigned)((a.F + kWide - 1) / kWide), (unsigned)bands), kColumnThreads, 0, st, a, grad,
            columns);

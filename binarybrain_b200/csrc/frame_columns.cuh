@@ -166,12 +166,15 @@ struct ColumnMax { __device__ static float join(float a, float b) { return fmaxf
 constexpr int kColumnThreads = 256, kMostCluster = 16;
 
 // Shared memory of one exchange of Q values a column; consecutive exchanges alternate between two of them, since a neighbour may still be reading.
+// The parts of the cluster's CTAs, exchange_bytes(cluster) of them, lie in dynamic shared memory: their number is the launch's, and what they take decides
+// how many CTAs an SM holds.
 template <int Q, int COLS> struct Exchange {
     float red[kColumnThreads / 32][Q * COLS];
-    float part[kMostCluster][Q * COLS];
     __align__(16) float out[Q * COLS];
+    float (*part)[Q * COLS];
     uint64_t bar;
 };
+template <int Q, int COLS> constexpr int exchange_bytes(int cluster) { return cluster > 1 ? 2 * cluster * Q * COLS * (int)sizeof(float) : 0; }
 
 // A cluster of CTAs and what its exchanges have come to.  CTAs send their parts into the shared memory of all others, whose barriers count the bytes:
 // unlike a barrier over the cluster, that does not wait for the stores of the tile before to be visible.
@@ -180,13 +183,16 @@ struct Cluster {
     int *gave_up;                                        // in shared memory: a wait ran out, all later ones are passed over
     __device__ Cluster(int *flag) : size(cluster_size()), rank(cluster_rank()), gave_up(flag) {}
 
-    // before the first exchange: the barriers are there, and all CTAs run
-    template <typename E> __device__ void meet(E *exchanges, int count)
+    // before the first exchange: the barriers are there, and all CTAs run.  `parts`: exchange_bytes() of shared memory.
+    template <int Q, int COLS> __device__ void meet(Exchange<Q, COLS> (&exchanges)[2], void *parts)
     {
         if (size == 1) return;
         if (threadIdx.x == 0) {
             *gave_up = 0;
-            for (int i = 0; i < count; ++i) mbar_init(&exchanges[i].bar, 1);
+            for (int i = 0; i < 2; ++i) {
+                exchanges[i].part = reinterpret_cast<float (*)[Q * COLS]>(parts) + i * size;
+                mbar_init(&exchanges[i].bar, 1);
+            }
             mbar_init_fence();
         }
         cluster_arrive();

@@ -194,7 +194,7 @@ k_quantize_once(const T *x, int8_t *q, float *scale_out, int N, int F, long long
         for (int i = 0; i < mine; ++i, to += piece, from += x_step) cp_async16(to, from, true);
     };
     fetch(f);
-    cl.meet(tops, 2);
+    cl.meet(tops, buffer + rows * piece);
     uint32_t turn = 0;                                                    // the exchange is its lowest bit, the phase the next
     for (; tile < tiles; tile += clusters, f += clusters * kCols, ++turn) {
         cp_async_commit();
@@ -250,14 +250,14 @@ __device__ __forceinline__ int4 load_q(const int8_t *row, int k, int K)
 }
 
 // A single frame: what counts is to have W on its way.  A warp has a row of W, or one of `splits` parts of its inputs where there are few rows, and asks
-// for 2048 bytes of it before it multiplies; q comes out of L1.  (Two rows a warp for two to eight frames: 9.9 to 22.7 us for 4096 x 4096, the tiles below 9.3.)
+// for 4096 bytes of it before it multiplies; q comes out of L1.  (Two rows a warp for two to eight frames: 9.9 to 22.7 us for 4096 x 4096, the tiles below 9.3.)
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_int8_dense_row(const int8_t *__restrict__ q, const float *__restrict__ q_scale, const int8_t *__restrict__ W, const float *__restrict__ w_scale,
                  const float *__restrict__ bias, T *y, int K, int O, long long ws, long long ys, int splits)
 {
     grid_dependency();
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     __shared__ int red[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % splits, o = (int)blockIdx.x * (8 / splits) + warp / splits;
     const int steps = (K + 511) / 512, s0 = (int)((long long)steps * part / splits), s1 = (int)((long long)steps * (part + 1) / splits);
@@ -308,6 +308,7 @@ constexpr int kGemmThreads = 192, kTileO = 128, kTileK = 128;
 template <int TN> constexpr int kGemmStages = TN >= 256 ? 4 : TN >= 128 ? 6 : 8;
 template <int TN> constexpr int kStageBytes = (kTileO + TN) * kTileK;
 template <int TN> constexpr int kGemmSmem = kGemmStages<TN> * kStageBytes<TN> + 1024;
+constexpr int kMostSplits = 8;
 constexpr int kTileGroup = 16;                           // tiles of output nodes that are walked together, so that their W and the q of some frames stay in L2
 
 struct GemmArgs {
@@ -338,6 +339,8 @@ k_int8_dense_tiles(const __grid_constant__ CUtensorMap map_w, const __grid_const
         mbar_init(&drained, 1);
         gave_up = 0;
         mbar_init_fence();
+        tma_prefetch(&map_w);
+        tma_prefetch(&map_q);
     }
     if (warp == 1) tmem_alloc(&tmem_base, kColumns);
     tcgen05_fence_before();
@@ -471,12 +474,15 @@ k_int8_dense_tiles(const __grid_constant__ CUtensorMap map_w, const __grid_const
             if (o < a.O) {
                 const float ws = a.w_scale[o], b = a.bias ? a.bias[o] : 0.0f;
                 const uint32_t own = smem_addr(reinterpret_cast<int *>(smem) + row * (TN + 4));
+#pragma unroll 2
                 for (int c = c0; c < c0 + width; c += 4) {
-                    int4 v = make_int4(0, 0, 0, 0);
-                    for (uint32_t r = 0; r < (uint32_t)a.splits; ++r) {
-                        const int4 p = peer_load_v4(own + c * 4, r);
-                        v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
-                    }
+                    int4 v = make_int4(0, 0, 0, 0), p[kMostSplits];
+#pragma unroll
+                    for (int r = 0; r < kMostSplits; ++r)                   // all of them under way at a time
+                        if (r < a.splits) p[r] = peer_load_v4(own + c * 4, (uint32_t)r);
+#pragma unroll
+                    for (int r = 0; r < kMostSplits; ++r)
+                        if (r < a.splits) { v.x += p[r].x; v.y += p[r].y; v.z += p[r].z; v.w += p[r].w; }
                     const int sums[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -549,9 +555,10 @@ static int quantize_frames(const T *x, int8_t *q, float *scale, int N, int F, in
         p.rows = ((N + p.cluster - 1) / p.cluster + per_warp * p.warps - 1) / (per_warp * p.warps);
         int *fault = fault_word();
         BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
-        const int cols = p.lanes * kFramesPerVec<T>, once_tiles = (F + cols - 1) / cols, threads = 32 * p.warps, smem = p.rows * threads * 16;
+        const int cols = p.lanes * kFramesPerVec<T>, once_tiles = (F + cols - 1) / cols, threads = 32 * p.warps;
+        const int smem = p.rows * threads * 16 + (p.lanes == 2 ? exchange_bytes<1, Column<T, 2>::kCols>(p.cluster) : exchange_bytes<1, Column<T, 4>::kCols>(p.cluster));
         auto kernel = p.lanes == 2 ? k_quantize_once<T, 2> : k_quantize_once<T, 4>;
-        BB200_REQUIRE(allow_big_smem(kernel, kQuantOnceRows * kColumnThreads * 16), (int)cudaErrorInvalidValue);
+        BB200_REQUIRE(allow_big_smem(kernel, kQuantOnceRows * kColumnThreads * 16 + exchange_bytes<1, Column<T, 4>::kCols>(kMostCluster)), (int)cudaErrorInvalidValue);
         const int clusters = std::min(once_tiles, resident_clusters(reinterpret_cast<const void *>(kernel), p.cluster, threads, smem));
         return launch_cluster(kernel, (unsigned)p.cluster, (unsigned)(clusters * p.cluster), threads, smem, st, x, q, scale, N, F, (long long)xs, (long long)qs, p.rows,
                               once_tiles, fault);
@@ -586,7 +593,7 @@ static int int8_dense(const int8_t *q, const float *q_scale, const int8_t *W, co
     const long long tiles_o = ((long long)O + kTileO - 1) / kTileO, sms = device_info().sm_count;
     auto tiles = [&](int tn) { return tiles_o * ((F + tn - 1) / tn); };
     const int tn = F <= 32 ? 32 : F <= 64 || tiles(128) < sms ? 64 : tiles(256) < sms ? 128 : 256;
-    while (a.splits < 8 && tiles(tn) * a.splits * 2 <= sms && (K + kTileK - 1) / kTileK >= a.splits * 4) a.splits *= 2;
+    while (a.splits < kMostSplits && tiles(tn) * a.splits * 2 <= sms && (K + kTileK - 1) / kTileK >= a.splits * 4) a.splits *= 2;
     return tn == 32 ? int8_dense_tiles<T, 32>(q, W, y, a, qs, ws, st) : tn == 64 ? int8_dense_tiles<T, 64>(q, W, y, a, qs, ws, st)
          : tn == 128 ? int8_dense_tiles<T, 128>(q, W, y, a, qs, ws, st) : int8_dense_tiles<T, 256>(q, W, y, a, qs, ws, st);
 }

@@ -293,7 +293,7 @@ k_layer_norm_once(const T *x, T *y, const float *__restrict__ gamma, const float
     if (f < F) fetch_rows(buffer, piece, x_first + f, x_step, mine);
     for (int i = threadIdx.x; i < c.step * rows; i += blockDim.x)
         gain[i] = cta_first + i < N ? make_float2(gamma ? gamma[cta_first + i] : 1.0f, beta ? beta[cta_first + i] : 0.0f) : make_float2(0.0f, 0.0f);
-    cl.meet(sums, 2);
+    cl.meet(sums, gain + c.step * rows);
     const float inv = 1.0f / (float)N;
     for (; tile < tiles; tile += clusters, f += clusters * kCols, phase ^= 1) {
         cp_async_commit();
@@ -372,7 +372,7 @@ k_layer_norm_grad_once(const T *x, const T *dy, T *dx, const float *__restrict__
     for (int i = threadIdx.x; i < c.step * rows; i += blockDim.x) gain[i] = gamma && first - c.row + i < N ? gamma[first - c.row + i] : 1.0f;
     float ag[R] = {}, ab[R] = {};
     __syncthreads();
-    cl.meet(sums, 2);
+    cl.meet(sums, gain + (c.step * rows + 3) / 4 * 4);
     uint32_t turn = 0;                                                    // the exchange is its lowest bit, the phase the next
     for (; tile < tiles; tile += clusters, f += clusters * kCols, ++turn) {
         cp_async_commit();
@@ -491,7 +491,7 @@ static unsigned stats_cluster(int N, long long tiles)
 }
 
 constexpr int kNormRows = 16, kNormGradRows = 8;         // rows a thread where everything is read once, at most
-constexpr int kNormSmem = kColumnThreads * kNormRows * 16 + kColumnThreads / 2 * kNormRows * (int)sizeof(float2);    // of either direction
+constexpr int kNormSmem = 120 * 1024;                    // more than either direction's tile, weights and parts take
 
 template <typename T, int LPR>
 static int layer_norm_once(const T *x, T *y, const float *gamma, const float *beta, float *mean, float *rstd, float eps, int N, int F, long long xs,
@@ -501,7 +501,8 @@ static int layer_norm_once(const T *x, T *y, const float *gamma, const float *be
     int *fault = fault_word();
     BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
     auto kernel = k_layer_norm_once<T, LPR>;
-    const int threads = 32 * p.warps, smem = p.rows * threads * 16 + p.rows * p.warps * (32 / LPR) * (int)sizeof(float2), tiles = (F + kCols - 1) / kCols;
+    const int threads = 32 * p.warps, smem = p.rows * threads * 16 + p.rows * p.warps * (32 / LPR) * (int)sizeof(float2) + exchange_bytes<1, kCols>(p.cluster),
+              tiles = (F + kCols - 1) / kCols;
     BB200_REQUIRE(allow_big_smem(kernel, kNormSmem), (int)cudaErrorInvalidValue);
     const int clusters = std::min(tiles, resident_clusters(reinterpret_cast<const void *>(kernel), p.cluster, threads, smem));
     return launch_cluster(kernel, (unsigned)p.cluster, (unsigned)(clusters * p.cluster), threads, smem, st, x, y, gamma, beta, mean, rstd, eps, N, F, xs, ys, p.rows,
@@ -516,7 +517,8 @@ static int layer_norm_grad_once(const T *x, const T *dy, T *dx, const float *gam
     int *fault = fault_word();
     BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
     auto kernel = k_layer_norm_grad_once<T, LPR, R>;
-    const int threads = 32 * p.warps, smem = 2 * p.rows * threads * 16 + p.rows * p.warps * (32 / LPR) * (int)sizeof(float), tiles = (F + kCols - 1) / kCols;
+    const int threads = 32 * p.warps, smem = 2 * p.rows * threads * 16 + (p.rows * p.warps * (32 / LPR) + 3) / 4 * 4 * (int)sizeof(float) +
+              exchange_bytes<2, kCols>(p.cluster), tiles = (F + kCols - 1) / kCols;
     BB200_REQUIRE(allow_big_smem(kernel, kNormSmem), (int)cudaErrorInvalidValue);
     const int clusters = std::min(tiles, resident_clusters(reinterpret_cast<const void *>(kernel), p.cluster, threads, smem));
     float2 *part = static_cast<float2 *>(stream_scratch(st, (size_t)clusters * N * sizeof(float2), kFrameOpSlot));
