@@ -677,7 +677,7 @@ static int distillation(Distill<T> a, float *loss, double loss_reduction, cudaSt
     constexpr int kLanes = 4;                                              // 64 bytes of a row: up to 1024 classes a CTA
     const bool aligned = frames_aligned<T>(a.z, a.zs) && frames_aligned<T>(a.dz, a.dzs);
     ColumnPlan p = plan_columns<T>(a.C, a.F, kLanes, kDistillRows, kDistillCluster);
-    if (!aligned || p.cluster > kDistillCluster) p.cluster = 0;
+    if (!aligned) p.cluster = 0;
     if (p.cluster) {
         // a power of two of warps; where there are many tiles, few of them with more rows a thread, since all warps of a CTA take part in the teacher's side
         // and its barriers (100 classes x 65536 frames: eight warps 51 us, two 28)

@@ -264,11 +264,11 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
         }
 }
 
-// How a layer of N rows and F frames is cut: `lanes` lanes along a row, clusters of `cluster` CTAs (0: its columns are too long for one) of `warps` warps,
-// `rows` rows a thread, at most `most_rows`.
+// How a layer of N rows and F frames is cut: `lanes` lanes along a row, clusters of `cluster` CTAs, `most` at most (0: its columns are too long for one),
+// of `warps` warps, `rows` rows a thread, at most `most_rows`.
 struct ColumnPlan { int cluster, warps, rows, lanes; };
 template <typename T>
-inline ColumnPlan plan_columns(int N, int F, int lanes, int most_rows, int most_spread = 8)
+inline ColumnPlan plan_columns(int N, int F, int lanes, int most_rows, int most)
 {
     if (F <= 2 * kFramesPerVec<T>) lanes = 2;
     const int per_warp = 32 / lanes, most_warps = kColumnThreads / 32;
@@ -276,9 +276,9 @@ inline ColumnPlan plan_columns(int N, int F, int lanes, int most_rows, int most_
     int cluster = 1;
     auto rows = [&] { return (N + cluster - 1) / cluster; };
     // as many CTAs as it takes to hold a column, and more where there would be few
-    while (cluster < kMostCluster && rows() > most_warps * per_warp * most_rows) cluster *= 2;
+    while (cluster < most && rows() > most_warps * per_warp * most_rows) cluster *= 2;
     if (rows() > most_warps * per_warp * most_rows) return {0, 0, 0, 0};
-    while (cluster < most_spread && tiles * cluster * 2 <= sms && rows() > most_warps * per_warp) cluster *= 2;
+    while (cluster < most && tiles * cluster * 2 <= sms && rows() > most_warps * per_warp) cluster *= 2;
     const int warps = std::min(most_warps, (rows() + per_warp - 1) / per_warp);
     return {cluster, warps, (rows() + per_warp * warps - 1) / (per_warp * warps), lanes};
 }

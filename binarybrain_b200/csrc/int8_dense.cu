@@ -13,7 +13,7 @@
 
 namespace bb200 {
 
-constexpr int kQuantThreads = 256, kQuantRows = 128;      // rows of x that a CTA turns over
+constexpr int kQuantThreads = 256, kQuantRows = 256;      // rows of x that a CTA turns over
 constexpr int kMostInputs = 131071;                       // times 128 x 128 is below 2^31
 
 __device__ __forceinline__ float quant_scale(uint32_t abs_bits)
@@ -115,8 +115,8 @@ k_quantize_scale(const T *x, float *scale_out, int N, int F, long long xs)
     if (cl > 1) { cluster_arrive(); cluster_wait(); }                     // nobody leaves while its part may still be read
 }
 
-// 128 rows x 128 bytes of x: a thread reads four neighbouring rows of its columns, so that its four values of a frame are a word of q; the words cross
-// through shared memory, in 16-byte pieces whose order differs from column to column so that no banks collide, and leave as 128 bytes of a frame's row.
+// 256 rows x 128 bytes of x: a thread reads twice four neighbouring rows of its columns, so that four values of a frame are a word of q; the words cross
+// through shared memory, in 16-byte pieces whose order differs from column to column so that no banks collide, and leave as lines of the frames' rows.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kQuantThreads)
 k_quantize_apply(const T *x, int8_t *q, const float *__restrict__ scale_in, int N, int F, long long xs, long long qs)
@@ -128,13 +128,25 @@ k_quantize_apply(const T *x, int8_t *q, const float *__restrict__ scale_in, int 
     __shared__ __align__(16) uint32_t tile[kCols][kQuantRows / 4];
     const Col c;
     const int f0 = (int)blockIdx.x * kCols, f = f0 + c.col, n0 = (int)blockIdx.y * kQuantRows, n = n0 + 4 * c.row;
-    float v[4][kVec], scale[kVec];
+    uint4 raw[2][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) unpack<T>(n + i < N ? load_frames<T, ALIGNED>(x + (long long)(n + i) * xs, f, F) : make_uint4(0, 0, 0, 0), v[i]);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int m = n + 128 * h + i;
+            raw[h][i] = m < N ? load_frames<T, ALIGNED>(x + (long long)m * xs, f, F) : make_uint4(0, 0, 0, 0);
+        }
+    float scale[kVec];
     load_columns(scale_in, f, F, scale);
 #pragma unroll
-    for (int j = 0; j < kVec; ++j)
-        tile[c.col + j][(c.row / 4 ^ c.lane % kLpr) * 4 + c.row % 4] = Quantizer(scale[j])(v[0][j], v[1][j], v[2][j], v[3][j]);
+    for (int h = 0; h < 2; ++h) {
+        float v[4][kVec];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) unpack<T>(raw[h][i], v[i]);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+            tile[c.col + j][h * 32 + (c.row / 4 ^ c.lane % kLpr) * 4 + c.row % 4] = Quantizer(scale[j])(v[0][j], v[1][j], v[2][j], v[3][j]);
+    }
     __syncthreads();
     for (int e = threadIdx.x; e < kCols * kPieces; e += kQuantThreads) {
         const int col = e / kPieces, piece = e % kPieces, m = n0 + 16 * piece;
@@ -167,7 +179,7 @@ k_quantize_channels(const float *__restrict__ W, int8_t *q, float *scale_out, in
 // then takes 16 rows of a column, which are 16 bytes of q.
 struct BitsMax { __device__ static float join(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); } };
 constexpr int kQuantOnceRows = 16;
-constexpr long long kQuantSmall = 1 << 18;
+constexpr long long kQuantSmall = 1 << 18;                 // values (1020 x 200: 5.1 us, in two launches 8.4; 5000 x 70: 15.1 and 8.4)
 
 template <typename T, int LPR>
 __global__ void __launch_bounds__(kColumnThreads, 3)
@@ -305,7 +317,7 @@ static int int8_dense_row(const int8_t *q, const float *q_scale, const int8_t *W
 // cluster of CTAs shares the k of one tile: the integer partial sums cross through distributed shared memory (in any order: they are exact), and every
 // CTA finishes its part of the columns.
 constexpr int kGemmThreads = 192, kTileO = 128, kTileK = 128;
-template <int TN> constexpr int kGemmStages = TN >= 256 ? 4 : TN >= 128 ? 6 : 8;
+template <int TN> constexpr int kGemmStages = TN >= 128 ? 6 : 8;
 template <int TN> constexpr int kStageBytes = (kTileO + TN) * kTileK;
 template <int TN> constexpr int kGemmSmem = kGemmStages<TN> * kStageBytes<TN> + 1024;
 constexpr int kMostSplits = 8;
@@ -317,6 +329,47 @@ struct GemmArgs {
     long long ys;
     int *fault;
 };
+
+// Columns of TMEM (`at`: a warp's 32 lanes, from column `c` on) to y, as many as make 128 bytes of a row: a lane has an output node, from o0 on, the columns
+// are the frames f on, `scale` theirs.  The values cross through 4 KB of the warp's shared memory, in 16-byte pieces whose order differs from row to row
+// so that no banks collide, and leave as whole lines of four rows a store.  (A store of 16 bytes by each lane for its own row touches 32 lines at a time:
+// 8192 x 8192 x 1024 91 us, with the products done in 42.)
+template <typename T, int TN> constexpr int kStoreColumns = TN < 128 / (int)sizeof(T) ? TN : 128 / (int)sizeof(T);      // (of a tile of TN frames)
+template <typename T, int COLS>
+__device__ __forceinline__ void store_columns(const GemmArgs &a, T *y, uint32_t at, int c, int o0, int f, float ws, float b, const float *scale, uint4 (*stage)[8])
+{
+    constexpr int kVec = kFramesPerVec<T>, kPieces = COLS / kVec;
+    const int lane = threadIdx.x & 31;
+    const bool whole = a.vec && f + COLS <= a.F;
+#pragma unroll
+    for (int h = 0; h < COLS; h += 32) {
+        if (f + h >= a.F) break;
+        int v[32];
+        tmem_load_32(at + c + h, v);
+#pragma unroll
+        for (int i = 0; i < 32; i += kVec) {
+            float r[kVec];
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) r[j] = fmaf((float)v[i + j], ws * scale[h + i + j], b);
+            if (whole) {
+                stage[lane][(h + i) / kVec ^ (lane & (kPieces - 1))] = pack<T>(r);
+            } else if (o0 + lane < a.O) {
+#pragma unroll
+                for (int j = 0; j < kVec; ++j)
+                    if (f + h + i + j < a.F) y[(long long)(o0 + lane) * a.ys + f + h + i + j] = from_float<T>(r[j]);
+            }
+        }
+    }
+    if (whole) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int row = (i * 32 + lane) / kPieces, piece = lane % kPieces;
+            if (o0 + row < a.O) *reinterpret_cast<uint4 *>(y + (long long)(o0 + row) * a.ys + f + piece * kVec) = stage[row][piece ^ (row & (kPieces - 1))];
+        }
+        __syncwarp();
+    }
+}
 
 template <typename T, int TN>
 __global__ void __launch_bounds__(kGemmThreads, 1)
@@ -330,6 +383,7 @@ k_int8_dense_tiles(const __grid_constant__ CUtensorMap map_w, const __grid_const
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
     __shared__ float s_scale[4][TN];                                      // of the frames of a tile, one copy an epilogue warp
+    __shared__ uint4 stage_out[4][32][8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = a.splits > 1 ? cluster_rank() : 0;
 
@@ -422,29 +476,9 @@ k_int8_dense_tiles(const __grid_constant__ CUtensorMap map_w, const __grid_const
             const uint32_t at = tmem + ((uint32_t)(part * 32) << 16) + acc * TN;
             if (a.splits == 1) {
 #pragma unroll 1
-                for (int c = 0; c < TN; c += 32) {
+                for (int c = 0; c < TN; c += kStoreColumns<T, TN>) {
                     if (f0 + c >= a.F) break;
-                    int v[32];
-                    tmem_load_32(at + c, v);
-                    if (o < a.O) {
-                        float r[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) r[i] = fmaf((float)v[i], ws * s_scale[part][c + i], b);
-                        T *out = y + (long long)o * a.ys + f0 + c;
-                        if (a.vec && f0 + c + 32 <= a.F) {
-#pragma unroll
-                            for (int i = 0; i < 32; i += kFramesPerVec<T>) {
-                                float w[kFramesPerVec<T>];
-#pragma unroll
-                                for (int j = 0; j < kFramesPerVec<T>; ++j) w[j] = r[i + j];
-                                *reinterpret_cast<uint4 *>(out + i) = pack<T>(w);
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (f0 + c + i < a.F) out[i] = from_float<T>(r[i]);
-                        }
-                    }
+                    store_columns<T, kStoreColumns<T, TN>>(a, y, at, c, o0 + part * 32, f0 + c, ws, b, &s_scale[part][c], stage_out[part]);
                 }
             } else {
                 // the stages are free: the tile's last product is done, and with it everything that read them
@@ -501,6 +535,137 @@ k_int8_dense_tiles(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (threadIdx.x == 0 && gave_up) atomicCAS(a.fault, 0, kFaultBarrierTimeout);
 }
 
+// Large products: two CTAs on one tile of 256 output nodes x 256 frames.  Each brings 128 rows of either operand, the tensor cores of both work on all of
+// them, and each CTA gets the sums of its 128 output nodes.  That halves what a CTA has to bring and read of q: alone, with 128 x 256, shared memory
+// bounds the products (8192^3: 374 us, 79 % of the tensor cores' cycles).  The first CTA issues the products and has the barriers of what has arrived and
+// of free accumulators; of consumed stages and finished sums each has its own.
+constexpr int kPairN = 256, kPairStages = 6, kPairStageBytes = 2 * kTileO * kTileK, kPairSmem = kPairStages * kPairStageBytes + 1024, kPairGroup = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+k_int8_dense_pairs(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q, T *y, const GemmArgs a)
+{
+    constexpr int kAcc = 2, kColumns = kAcc * kPairN;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[kPairStages], empty[kPairStages], acc_full[kAcc], acc_empty[kAcc], drained;
+    __shared__ uint32_t tmem_base;
+    __shared__ int gave_up;
+    __shared__ float s_scale[4][kPairN];
+    __shared__ uint4 stage_out[4][32][8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8); }
+        mbar_init(&drained, 1);
+        gave_up = 0;
+        mbar_init_fence();
+        tma_prefetch(&map_w);
+        tma_prefetch(&map_q);
+    }
+    __syncwarp();
+    if (warp == 1) tmem_alloc_pair(&tmem_base, kColumns);
+    tcgen05_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    tcgen05_fence_after();
+    const uint32_t tmem = tmem_base;
+    grid_dependency();
+
+    const int tiles_o = (a.O + 2 * kTileO - 1) / (2 * kTileO), tiles_f = (a.F + kPairN - 1) / kPairN, tiles = tiles_o * tiles_f;
+    const int blocks_k = (a.K + kTileK - 1) / kTileK, first = (int)blockIdx.x / 2, step = (int)gridDim.x / 2;
+    auto place = [&](int tile, int &o0, int &f0) {
+        const int group = tile / (kPairGroup * tiles_f), in = tile % (kPairGroup * tiles_f), rows = min(kPairGroup, tiles_o - group * kPairGroup);
+        o0 = (group * kPairGroup + in % rows) * 2 * kTileO + (int)rank * kTileO;
+        f0 = in / rows * kPairN;
+    };
+
+    if (warp == 0 && lane == 0) {
+        int stage = 0, issued = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            int o0, f0;
+            place(tile, o0, f0);
+            for (int kb = 0; kb < blocks_k; ++kb) {
+                ok = mbar_wait_one(&empty[stage], phase ^ 1, &gave_up);
+                if (!ok) break;
+                uint8_t *at = smem + stage * kPairStageBytes;
+                if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * kPairStageBytes);
+                const uint32_t bar = peer_addr(&full[stage], 0);
+                tma_load_2d_pair(at, &map_w, kb * kTileK, o0, bar);
+                tma_load_2d_pair(at + kTileO * kTileK, &map_q, kb * kTileK, f0 + (int)rank * (kPairN / 2), bar);
+                ++issued;
+                if (++stage == kPairStages) { stage = 0; phase ^= 1; }
+            }
+        }
+        // what is under way, for either CTA, lands before they leave, also where a wait has run out
+        if (rank == 0)
+            for (int b = issued > kPairStages ? issued - kPairStages : 0; b < issued; ++b)
+                mbar_wait_some(&full[b % kPairStages], (uint32_t)(b / kPairStages) & 1u, kDrainSpins);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        constexpr uint32_t kInstr = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kPairN >> 3) << 17) | ((uint32_t)(2 * kTileO >> 4) << 24);
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            ok = mbar_wait_one(&acc_empty[acc], acc_phase ^ 1, &gave_up);
+            if (!ok) break;
+            tcgen05_fence_after();
+            for (int kb = 0; kb < blocks_k; ++kb) {
+                ok = mbar_wait_one(&full[stage], phase, &gave_up);
+                if (!ok) break;
+                tcgen05_fence_after();
+                const uint32_t at = smem_addr(smem + stage * kPairStageBytes);
+                const uint64_t da = smem_descriptor_128b(at), db = smem_descriptor_128b(at + kTileO * kTileK);
+#pragma unroll
+                for (int k = 0; k < kTileK / 32; ++k) mma_i8_pair(tmem + acc * kPairN, da + 2 * k, db + 2 * k, kInstr, kb > 0 || k > 0);
+                tcgen05_commit_pair(&empty[stage]);
+                if (++stage == kPairStages) { stage = 0; phase ^= 1; }
+            }
+            if (!ok) break;
+            tcgen05_commit_pair(&acc_full[acc]);
+            if (++acc == kAcc) { acc = 0; acc_phase ^= 1; }
+        }
+        tcgen05_commit_pair_own(&drained);                                // no product is under way when the TMEM goes back
+        mbar_wait_some(&drained, 0, kDrainSpins);
+    } else if (warp >= 2) {
+        const int part = warp & 3, row = part * 32 + lane;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int tile = first; tile < tiles; tile += step) {
+            int o0, f0;
+            place(tile, o0, f0);
+            const int o = o0 + row;
+            __syncwarp();
+            for (int i = lane; i < kPairN; i += 32) s_scale[part][i] = f0 + i < a.F ? a.q_scale[f0 + i] : 0.0f;
+            const float ws = o < a.O ? a.w_scale[o] : 0.0f, b = o < a.O && a.bias ? a.bias[o] : 0.0f;
+            __syncwarp();
+            if (!mbar_wait_warp(&acc_full[acc], acc_phase, &gave_up)) break;
+            tcgen05_fence_after();
+            const uint32_t at = tmem + ((uint32_t)(part * 32) << 16) + acc * kPairN;
+#pragma unroll 1
+            for (int c = 0; c < kPairN; c += kStoreColumns<T, kPairN>) {
+                if (f0 + c >= a.F) break;
+                store_columns<T, kStoreColumns<T, kPairN>>(a, y, at, c, o0 + part * 32, f0 + c, ws, b, &s_scale[part][c], stage_out[part]);
+            }
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(peer_addr(&acc_empty[acc], 0));
+            if (++acc == kAcc) { acc = 0; acc_phase ^= 1; }
+        }
+    }
+    __syncwarp();
+    tcgen05_fence_before();
+    cluster_arrive();
+    cluster_wait();
+    tcgen05_fence_after();
+    if (warp == 1) tmem_free_pair(tmem, kColumns);
+    if (threadIdx.x == 0 && gave_up) atomicCAS(a.fault, 0, kFaultBarrierTimeout);
+}
+
 // rows of 8-bit integers as TMA sees them: boxes of 128 bytes x `box_rows` rows; what lies beyond the inputs or the rows reads as zero
 static int int8_rows_map(CUtensorMap *map, const int8_t *p, int K, int rows, long long stride, int box_rows)
 {
@@ -538,6 +703,41 @@ static int int8_dense_tiles(const int8_t *q, const int8_t *W, T *y, GemmArgs a, 
     return launch_cluster(kernel, (unsigned)a.splits, grid, kGemmThreads, kGemmSmem<TN>, st, map_w, map_q, y, a);
 }
 
+// Frames a tile (kPairN: by a pair of CTAs) and CTAs that share the inputs of one, by the clocks of an SM: rounds of tiles times blocks of 128 inputs times
+// what a block costs, 2 (128 + frames) where shared memory takes in and gives out both operands at 128 bytes a clock, 512 for a pair, which the tensor
+// cores bound; and about 12 for each column that is stored at the end, 2500 where sums cross a cluster.  (us, this choice and the best of others: 2048^3
+// 14 by pairs and 15 by 128 columns; 4096 x 4096 x 16 9.5 by four CTAs, 25 by one.)
+struct TileChoice { int columns, splits; };
+static TileChoice choose_tiles(int K, int O, int F)
+{
+    const long long sms = device_info().sm_count, blocks = (K + kTileK - 1) / kTileK, tiles_o = ((long long)O + kTileO - 1) / kTileO;
+    const long long pair_tiles = ((long long)O + 2 * kTileO - 1) / (2 * kTileO) * (((long long)F + kPairN - 1) / kPairN);
+    TileChoice best = {kPairN, 1};
+    long long least = (pair_tiles + sms / 2 - 1) / (sms / 2) * blocks * 512 + 12 * kPairN;
+    for (int columns = 32; columns <= 128; columns *= 2) {
+        const long long tiles = tiles_o * ((F + columns - 1) / columns);
+        for (int splits = 1; splits <= kMostSplits; splits *= 2) {
+            if (splits > 1 && (tiles * splits > sms || blocks < 2 * splits)) break;
+            const long long cost = (tiles * splits + sms - 1) / sms * ((blocks + splits - 1) / splits) * 2 * (kTileO + columns) + 12 * columns + (splits > 1 ? 2500 : 0);
+            if (cost < least) { least = cost; best = {columns, splits}; }
+        }
+    }
+    return best;
+}
+
+template <typename T>
+static int int8_dense_pairs(const int8_t *q, const int8_t *W, T *y, const GemmArgs &a, long long qs, long long ws, cudaStream_t st)
+{
+    CUtensorMap map_w, map_q;
+    if (const int e = int8_rows_map(&map_w, W, a.K, a.O, ws, kTileO)) return e;
+    if (const int e = int8_rows_map(&map_q, q, a.K, a.F, qs, kPairN / 2)) return e;
+    const long long tiles = ((long long)a.O + 2 * kTileO - 1) / (2 * kTileO) * (((long long)a.F + kPairN - 1) / kPairN), pairs = device_info().sm_count / 2;
+    BB200_REQUIRE(tiles < (1LL << 30), BBCU_ERR_TOO_LARGE);
+    auto kernel = k_int8_dense_pairs<T>;
+    BB200_REQUIRE(allow_big_smem(kernel, kPairSmem), (int)cudaErrorInvalidValue);
+    return launch_cluster(kernel, 2u, (unsigned)(2 * (tiles < pairs ? tiles : pairs)), kGemmThreads, kPairSmem, st, map_w, map_q, y, a);
+}
+
 template <typename T>
 static int quantize_frames(const T *x, int8_t *q, float *scale, int N, int F, int xs, int qs, bbcu_stream_t stream)
 {
@@ -549,7 +749,7 @@ static int quantize_frames(const T *x, int8_t *q, float *scale, int N, int F, in
     cudaStream_t st = as_stream(stream);
     const bool aligned = frames_aligned<T>(x, xs);
     BB200_REQUIRE(F <= (1 << 30), BBCU_ERR_TOO_LARGE);
-    if (ColumnPlan p = plan_columns<T>(N, F, 4, kQuantOnceRows); aligned && p.cluster && (long long)N * F <= kQuantSmall) {
+    if (ColumnPlan p = plan_columns<T>(N, F, 4, kQuantOnceRows, 8); aligned && p.cluster && (long long)N * F <= kQuantSmall) {
         const int per_warp = 32 / p.lanes;
         if (p.warps * per_warp % 16) ++p.warps;                           // a round of rows is whole 16-byte pieces of q
         p.rows = ((N + p.cluster - 1) / p.cluster + per_warp * p.warps - 1) / (per_warp * p.warps);
@@ -558,7 +758,7 @@ static int quantize_frames(const T *x, int8_t *q, float *scale, int N, int F, in
         const int cols = p.lanes * kFramesPerVec<T>, once_tiles = (F + cols - 1) / cols, threads = 32 * p.warps;
         const int smem = p.rows * threads * 16 + (p.lanes == 2 ? exchange_bytes<1, Column<T, 2>::kCols>(p.cluster) : exchange_bytes<1, Column<T, 4>::kCols>(p.cluster));
         auto kernel = p.lanes == 2 ? k_quantize_once<T, 2> : k_quantize_once<T, 4>;
-        BB200_REQUIRE(allow_big_smem(kernel, kQuantOnceRows * kColumnThreads * 16 + exchange_bytes<1, Column<T, 4>::kCols>(kMostCluster)), (int)cudaErrorInvalidValue);
+        BB200_REQUIRE(allow_big_smem(kernel, kQuantOnceRows * kColumnThreads * 16 + exchange_bytes<1, Column<T, 4>::kCols>(8)), (int)cudaErrorInvalidValue);
         const int clusters = std::min(once_tiles, resident_clusters(reinterpret_cast<const void *>(kernel), p.cluster, threads, smem));
         return launch_cluster(kernel, (unsigned)p.cluster, (unsigned)(clusters * p.cluster), threads, smem, st, x, q, scale, N, F, (long long)xs, (long long)qs, p.rows,
                               once_tiles, fault);
@@ -590,12 +790,12 @@ static int int8_dense(const int8_t *q, const float *q_scale, const int8_t *W, co
     int *fault = fault_word();
     BB200_REQUIRE(fault != nullptr, BBCU_ERR_NO_DEVICE);
     GemmArgs a{q_scale, w_scale, bias, K, O, F, 1, frames_aligned<T>(y, ys), ys, fault};
-    const long long tiles_o = ((long long)O + kTileO - 1) / kTileO, sms = device_info().sm_count;
-    auto tiles = [&](int tn) { return tiles_o * ((F + tn - 1) / tn); };
-    const int tn = F <= 32 ? 32 : F <= 64 || tiles(128) < sms ? 64 : tiles(256) < sms ? 128 : 256;
-    while (a.splits < kMostSplits && tiles(tn) * a.splits * 2 <= sms && (K + kTileK - 1) / kTileK >= a.splits * 4) a.splits *= 2;
+    const TileChoice t = choose_tiles(K, O, F);
+    if (t.columns == kPairN) return int8_dense_pairs<T>(q, W, y, a, qs, ws, st);
+    a.splits = t.splits;
+    const int tn = t.columns;
     return tn == 32 ? int8_dense_tiles<T, 32>(q, W, y, a, qs, ws, st) : tn == 64 ? int8_dense_tiles<T, 64>(q, W, y, a, qs, ws, st)
-         : tn == 128 ? int8_dense_tiles<T, 128>(q, W, y, a, qs, ws, st) : int8_dense_tiles<T, 256>(q, W, y, a, qs, ws, st);
+                    : int8_dense_tiles<T, 128>(q, W, y, a, qs, ws, st);
 }
 
 }   // namespace bb200

@@ -536,7 +536,9 @@ static int layer_norm_forward(const T *x, T *y, const float *gamma, const float 
 {
     const bool aligned = frames_aligned<T>(x, xs) && frames_aligned<T>(y, ys);
     BB200_REQUIRE(F <= (1 << 30), BBCU_ERR_TOO_LARGE);
-    if (const ColumnPlan p = plan_columns<T>(N, F, sizeof(T) == 4 ? 8 : 4, kNormRows); aligned && p.cluster)
+    // Larger clusters than these lose to the two passes, larger ones of the backward than 8, too (us a pass, once / two passes: 4096 x 8192 fp32 63 / 71,
+    // 8192 x 16384 251 / 253, bf16 158 / 140; backward 4096 x 16384 bf16 130 / 139, fp32 202 / 231, 8192 x 8192 fp32 225 / 223).
+    if (const ColumnPlan p = plan_columns<T>(N, F, sizeof(T) == 4 ? 8 : 4, kNormRows, sizeof(T) == 4 ? 8 : 4); aligned && p.cluster)
         return (p.lanes == 2 ? layer_norm_once<T, 2> : layer_norm_once<T, sizeof(T) == 4 ? 8 : 4>)(x, y, gamma, beta, mean, rstd, eps, N, F, xs, ys, p, st);
     constexpr int kCols = Column<T, 8>::kCols, kWide = 32 * kFramesPerVec<T>;
     const long long tiles = ((long long)F + kCols - 1) / kCols, bands = ((long long)N + 8 * kApplyRows - 1) / (8 * kApplyRows);
@@ -556,7 +558,7 @@ static int layer_norm_backward(const T *x, const T *dy, T *dx, const float *gamm
     const bool aligned = frames_aligned<T>(x, xs) && frames_aligned<T>(dy, dys) && frames_aligned<T>(dx, dxs);
     BB200_REQUIRE(F <= (1 << 30), BBCU_ERR_TOO_LARGE);
     const bool wide = N <= 8 * kColumnThreads / 8 * 4;                    // 128 bytes of a row and four rows a thread in clusters of up to 8, or 64 and eight
-    if (const ColumnPlan p = plan_columns<T>(N, F, wide ? 8 : 4, wide ? 4 : kNormGradRows); aligned && p.cluster) {
+    if (const ColumnPlan p = plan_columns<T>(N, F, wide ? 8 : 4, wide ? 4 : kNormGradRows, 8); aligned && p.cluster) {
 #define BB200_ONCE(L) (p.rows <= 4 ? layer_norm_grad_once<T, L, 4> : layer_norm_grad_once<T, L, kNormGradRows>)
         return (p.lanes == 2 ? BB200_ONCE(2) : p.lanes == 4 ? BB200_ONCE(4) : layer_norm_grad_once<T, 8, 4>)(x, dy, dx, gamma, mean, rstd, dgamma, dbeta, accumulate, N,
                                                                                                         F, xs, dys, dxs, p, st);

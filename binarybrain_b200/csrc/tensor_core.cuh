@@ -48,6 +48,18 @@ __device__ __forceinline__ void tma_load_2d(void *smem_dst, const CUtensorMap *m
                  ::"r"(smem_addr(smem_dst)), "l"(map), "r"(x), "r"(row), "r"(smem_addr(bar)) : "memory");
 }
 
+// the same by one CTA of a pair, whose bytes count at a barrier of either (a cluster address)
+__device__ __forceinline__ void tma_load_2d_pair(void *smem_dst, const CUtensorMap *map, int x, int row, uint32_t cluster_bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_addr(smem_dst)), "l"(map), "r"(x), "r"(row), "r"(cluster_bar) : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
 __device__ __forceinline__ void tmem_alloc(uint32_t *smem_out, int columns)
 {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(smem_out)), "r"(columns) : "memory");
@@ -59,6 +71,18 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, int columns)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
+// for a pair of CTAs, by a warp of each
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t *smem_out, int columns)
+{
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(smem_out)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_free_pair(uint32_t tmem, int columns)
+{
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+}
+
 __device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_fence_after()  { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -66,6 +90,16 @@ __device__ __forceinline__ void tcgen05_fence_after()  { asm volatile("tcgen05.f
 __device__ __forceinline__ void tcgen05_commit(uint64_t *bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// the same for a pair's products: at this place in both CTAs, or in this one alone
+__device__ __forceinline__ void tcgen05_commit_pair(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tcgen05_commit_pair_own(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
 // Rows of 128 bytes (k) in groups of eight, 128-byte swizzled, 1024 bytes a group: start address, group distance, version 1, swizzle mode 2.  32 bytes
@@ -78,6 +112,13 @@ __device__ __forceinline__ uint64_t smem_descriptor_128b(uint32_t addr)
 __device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t a, uint64_t b, uint32_t instr, bool accumulate)
 {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)accumulate) : "memory");
+}
+
+// both CTAs of a pair, each with half of the rows of either operand at the same place of its shared memory
+__device__ __forceinline__ void mma_i8_pair(uint32_t tmem, uint64_t a, uint64_t b, uint32_t instr, bool accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(tmem), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)accumulate) : "memory");
 }
 

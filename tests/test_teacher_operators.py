@@ -234,7 +234,7 @@ def int8_case(n_in, n_out, frames, seed=0, rough=True):
 
 INT8_SIZES = [(1, 1, 1), (16, 8, 1), (33, 5, 2), (64, 16, 3), (1000, 10, 1), (4096, 257, 1), (1020, 1000, 4), (129, 130, 5), (512, 77, 8), (300, 129, 9), (1024, 128, 16),
               (777, 300, 17), (128, 128, 32), (100, 33, 33), (1020, 1000, 200), (2048, 64, 64), (255, 513, 100), (4099, 130, 65), (64, 1024, 129), (500, 1, 300), (16384, 40, 24),
-              (131071, 3, 2), (131071, 20, 40), (640, 700, 513), (272, 2000, 777), (1, 300, 300), (2000, 129, 1025)]
+              (131071, 3, 2), (131071, 20, 40), (640, 700, 513), (272, 2000, 777), (1, 300, 300), (2000, 129, 1025), (130, 5000, 3000), (1000, 4999, 2113), (33, 9001, 1500)]
 
 
 @pytest.mark.gpu
