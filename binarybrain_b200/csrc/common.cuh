@@ -117,9 +117,6 @@ int *fault_word();
 bool allow_big_smem_once(const void *kernel, int bytes);
 template <typename K> inline bool allow_big_smem(K *kernel, int bytes) { return allow_big_smem_once(reinterpret_cast<const void *>(kernel), bytes); }
 
-// Opt-in to clusters of 16, once per kernel and device.  False when it is refused.
-bool allow_cluster_16_once(const void *kernel);
-
 // Clusters of this size (1: CTAs) that the device holds at a time, asked for once per kernel and shape; at least 1.
 int resident_clusters(const void *kernel, int cluster, int threads, size_t smem);
 

@@ -9,7 +9,8 @@
 //
 // both times the frame's weight; a slot with p_k = 0 adds nothing, whatever its class's log q is, and a class that is named twice gets both.  A frame
 // without a slot, or of weight 0, has loss 0 and gradient 0 whatever its logits are.
-// exp(z / T) is evaluated as exp2((z - max z) log2(e) / T).
+// exp(z / T) is evaluated as exp2((z - max z) log2(e) / T), and by expf() in the sums of up to kFewClasses classes: there a small loss comes out of large
+// terms, times T^2, and the teacher's sums, which are expf()'s, have the same errors.
 #include <type_traits>
 
 #include "frame_columns.cuh"
@@ -17,6 +18,7 @@
 namespace bb200 {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kFewClasses = 256;                         // (10 classes, T = 4: the mean loss is off by 5e-7 of it with exp2, by 2e-7 with expf)
 constexpr int kMostSlots = 512;                          // of the teacher, a column of them in shared memory
 constexpr int kDistillRows = 16, kDistillCluster = 4;    // rows a thread and CTAs a cluster where everything is read once, at most
 
@@ -75,7 +77,7 @@ template <> __device__ __forceinline__ uint4 packed_max<__nv_bfloat16>(const uin
 }
 
 // ---- the teacher's side of COLS frames from f0 on, by a CTA of a multiple of COLS threads: thread t has column t % COLS and every (threads / COLS)-th
-// slot of it.  index[slot][column] (-1: empty) and p[slot][column] go to shared memory, and to each thread, for its column, P = sum p, E = sum p log p
+// slot of it.  index[slot][column] (-1: empty) and log_p[slot][column] (-inf: p = 0) go to shared memory, and to each thread, for its column, P = sum p, E = sum p log p
 // and the weight (0: the frame takes no part).  A barrier stands behind the last write of the two; red[0] and red[1] may still be read.
 struct TeacherColumn { float P, E, weight; };
 
@@ -88,7 +90,7 @@ template <int COLS, typename JOIN> __device__ __forceinline__ float column_of_wa
 }
 
 template <typename T, int COLS>
-__device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, int f0, int *index, float *p, float (&red)[3][kColumnThreads / 32 * COLS])
+__device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, int f0, int *index, float *log_p, float (&red)[3][kColumnThreads / 32 * COLS])
 {
     const int col = threadIdx.x % COLS, group = threadIdx.x / COLS, groups = blockDim.x / COLS, f = f0 + col;
     const float w = f < a.F ? (a.weight ? a.weight[f] : 1.0f) : 0.0f;
@@ -102,7 +104,7 @@ __device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, in
             if (i < 0 || i >= a.C || t == -INFINITY) i = -1;
         }
         index[k * COLS + col] = i;
-        p[k * COLS + col] = t;
+        log_p[k * COLS + col] = t;
         if (i >= 0) { top = fmaxf(top, t); slots += 1.0f; }
     }
     const int warps = blockDim.x / 32, own = threadIdx.x / 32 * COLS + threadIdx.x % 32;
@@ -124,7 +126,7 @@ __device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, in
     } else {
         float sum = 0.0f;
         for (int k = group; k < a.K; k += groups)
-            if (index[k * COLS + col] >= 0) sum += exp2_fast((p[k * COLS + col] - top) * a.scale);
+            if (index[k * COLS + col] >= 0) sum += expf((log_p[k * COLS + col] - top) * a.inv_t);
         sum = column_of_warp<COLS>(sum, [](float a, float b) { return a + b; });
         if (threadIdx.x % 32 < COLS) red[2][own] = sum;
         __syncthreads();
@@ -134,14 +136,14 @@ __device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, in
     }
     float P = 0.0f, E = 0.0f;
     for (int k = group; k < a.K; k += groups) {
-        float q = 0.0f;
+        float lp = -INFINITY;
         if (live && index[k * COLS + col] >= 0) {
-            const float log_p = p[k * COLS + col] * a.inv_t - lse;
-            q = exp2_fast(log_p * kLog2e);
-            if (q != 0.0f) E += q * log_p;
-            P += q;
+            lp = log_p[k * COLS + col] * a.inv_t - lse;
+            const float p = expf(lp);
+            if (p != 0.0f) E += p * lp;
+            P += p;
         }
-        p[k * COLS + col] = q;
+        log_p[k * COLS + col] = lp;
     }
     P = column_of_warp<COLS>(P, [](float a, float b) { return a + b; });
     E = column_of_warp<COLS>(E, [](float a, float b) { return a + b; });
@@ -156,7 +158,7 @@ __device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, in
 }
 
 // The probabilities of all slots of the column that name the class of slot k, in the order of the slots; `first`: k is the first of them.
-template <int COLS> __device__ __forceinline__ float named_slots(const int *index, const float *p, int K, int k, int col, bool &first)
+template <int COLS> __device__ __forceinline__ float named_slots(const int *index, const float *log_p, int K, int k, int col, bool &first)
 {
     const int i = index[k * COLS + col];
     float sum = 0.0f;
@@ -164,20 +166,20 @@ template <int COLS> __device__ __forceinline__ float named_slots(const int *inde
     for (int e = 0; e < K; ++e)
         if (index[e * COLS + col] == i) {
             first = first && e >= k;
-            sum += p[e * COLS + col];
+            sum += expf(log_p[e * COLS + col]);
         }
     return sum;
 }
 
-// From a frame's joined parts (cross = sum p (z - top) / T over the named classes) its gradient's factors and its loss.
+// From a frame's joined parts (spread = sum p (log p - (z - top) / T) over the slots) its gradient's factors and its loss.
 template <typename T>
-__device__ __forceinline__ FrameGrad finish_frame(const Distill<T> &a, const TeacherColumn &c, const SoftSum &s, float cross, float &loss)
+__device__ __forceinline__ FrameGrad finish_frame(const Distill<T> &a, const TeacherColumn &c, const SoftSum &s, float spread, float &loss)
 {
     loss = 0.0f;
     if (c.weight == 0.0f) return {0.0f, 0.0f, 0.0f, 0.0f};
-    const bool none = s.top == -INFINITY && s.sum == 0.0f;                // no class is left: cross is -inf, the loss infinite, q = 0
+    const bool none = s.top == -INFINITY && s.sum == 0.0f;                // no class is left: the spread is infinite, as the loss is, and q = 0
     const float slope = a.grad_reduction * c.weight * a.temperature;
-    loss = c.weight * a.temperature * a.temperature * (c.E - cross + (none ? 0.0f : c.P * logf(s.sum)));
+    loss = c.weight * a.temperature * a.temperature * (spread + (none ? 0.0f : c.P * logf(s.sum)));
     return {reference(s.top), none ? 0.0f : slope * c.P / s.sum, INFINITY, slope};
 }
 
@@ -192,7 +194,7 @@ template <typename T> __device__ __forceinline__ void write_losses(const Distill
 }
 
 // ---- everything read once, as far as a cluster holds the classes of a column tile in shared memory (see layer_norm.cu for the walk over the tiles).  Each
-// CTA reduces its classes to four numbers a frame, relative to its own largest logit m: m, sum exp((z - m) / T), and sum p (z - m) / T and sum p over
+// CTA reduces its classes to four numbers a frame, relative to its own largest logit m: m, sum exp((z - m) / T), and sum p (log p - (z - m) / T) and sum p over
 // the slots that name one of its classes; one exchange joins them.
 template <typename T, int LPR>
 __global__ void __launch_bounds__(kColumnThreads, 3)
@@ -214,8 +216,8 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
     const uint8_t *const at = buffer + threadIdx.x * 16;
     const int shift = 31 - __clz(c.step);                                 // the warps are a power of two
     int *const index = reinterpret_cast<int *>(buffer + rows * piece);
-    float *const p = reinterpret_cast<float *>(index + a.K * kCols);
-    unsigned *const seen = reinterpret_cast<unsigned *>(p + a.K * kCols);   // a bit for each of the CTA's classes and columns: has a slot named it?
+    float *const log_p = reinterpret_cast<float *>(index + a.K * kCols);
+    unsigned *const seen = reinterpret_cast<unsigned *>(log_p + a.K * kCols);   // a bit for each of the CTA's classes and columns: has a slot named it?
     const int seen_words = (c.step * rows + 31) / 32 * kCols;
     float (*const part)[4][kCols] = reinterpret_cast<float (*)[4][kCols]>(seen + seen_words);      // [two exchanges of the cluster's CTAs]
     for (int i = threadIdx.x; i < seen_words; i += blockDim.x) seen[i] = 0u;
@@ -246,9 +248,10 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
         cluster_wait();
     }
     const int my_col = threadIdx.x % kCols, group = threadIdx.x / kCols, groups = blockDim.x / kCols;
+    const bool few = a.C <= kFewClasses;
     for (uint32_t turn = 0; tile < tiles; tile += clusters, f += clusters * kCols, ++turn) {
         cp_async_commit();
-        const TeacherColumn teacher = teacher_columns<T, kCols>(a, tile * kCols, index, p, red);
+        const TeacherColumn teacher = teacher_columns<T, kCols>(a, tile * kCols, index, log_p, red);
         cp_async_wait<0>();
         float v[kVec], m[kVec], sum[kVec] = {};
 #pragma unroll
@@ -285,7 +288,7 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
             for (int i = 0; i < mine; ++i, q += piece) {
                 unpack<T>(*reinterpret_cast<const uint4 *>(q), v);
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) sum[j] += exp2_fast((v[j] - m[j]) * a.scale);
+                for (int j = 0; j < kVec; ++j) sum[j] += few ? expf((v[j] - m[j]) * a.inv_t) : exp2_fast((v[j] - m[j]) * a.scale);
             }
         }
 #pragma unroll
@@ -297,34 +300,34 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
             for (int j = 0; j < kVec; ++j) red_soft[c.warp][c.col + j] = sum[j];
         }
         const float own_top = reference(s_top[my_col]);
-        float cross = 0.0f, own_p = 0.0f;
+        float spread = 0.0f, own_p = 0.0f;
         int twice = 0;
         for (int k = group; k < a.K; k += groups) {
             const int i = index[k * kCols + my_col], local = i - cta_first;
-            const float q = p[k * kCols + my_col];
+            const float lp = log_p[k * kCols + my_col], p = expf(lp);
             if (local >= 0 && local < cta_rows) {
                 const unsigned bit = 1u << (local & 31);
                 twice |= (int)(atomicOr(&seen[(local >> 5) * kCols + my_col], bit) & bit);
-                if (q != 0.0f) {
-                    cross += q * ((logit(i, my_col) - own_top) * a.inv_t);
-                    own_p += q;
+                if (p != 0.0f) {
+                    spread += p * (lp - (logit(i, my_col) - own_top) * a.inv_t);
+                    own_p += p;
                 }
             }
         }
-        cross = column_of_warp<kCols>(cross, [](float a, float b) { return a + b; });
+        spread = column_of_warp<kCols>(spread, [](float a, float b) { return a + b; });
         own_p = column_of_warp<kCols>(own_p, [](float a, float b) { return a + b; });
         if (c.lane < kCols) {
-            red[0][c.warp * kCols + c.lane] = cross;
+            red[0][c.warp * kCols + c.lane] = spread;
             red[1][c.warp * kCols + c.lane] = own_p;
         }
         if (cl > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(&bar[turn & 1], cl * 4 * kCols * (uint32_t)sizeof(float));
         twice = __syncthreads_or(twice);
         if (threadIdx.x < kCols) {                                        // all of them in the first warp
             float s = 0.0f;
-            cross = own_p = 0.0f;
+            spread = own_p = 0.0f;
             for (int w = 0; w < c.warps; ++w) {
                 s += red_soft[w][threadIdx.x];
-                cross += red[0][w * kCols + threadIdx.x];
+                spread += red[0][w * kCols + threadIdx.x];
                 own_p += red[1][w * kCols + threadIdx.x];
             }
             SoftSum joined = {s_top[threadIdx.x], s};
@@ -334,7 +337,7 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
                     const uint32_t b = peer_addr(&bar[turn & 1], r);
                     peer_send(peer_addr(&to[0][threadIdx.x], r), joined.top, b);
                     peer_send(peer_addr(&to[1][threadIdx.x], r), joined.sum, b);
-                    peer_send(peer_addr(&to[2][threadIdx.x], r), cross, b);
+                    peer_send(peer_addr(&to[2][threadIdx.x], r), spread, b);
                     peer_send(peer_addr(&to[3][threadIdx.x], r), own_p, b);
                 }
                 bool ok = *(volatile int *)&gave_up == 0;
@@ -344,15 +347,15 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
                 }
                 joined = {from[0][0][threadIdx.x], from[0][1][threadIdx.x]};
                 for (uint32_t r = 1; r < cl; ++r) joined = join_soft(joined, {from[r][0][threadIdx.x], from[r][1][threadIdx.x]}, a.scale);
-                cross = 0.0f;
+                spread = 0.0f;
                 for (uint32_t r = 0; r < cl; ++r) {
-                    const float q = from[r][3][threadIdx.x];
-                    cross += from[r][2][threadIdx.x];
-                    if (q != 0.0f) cross += q * ((reference(from[r][0][threadIdx.x]) - reference(joined.top)) * a.inv_t);
+                    const float p = from[r][3][threadIdx.x];
+                    spread += from[r][2][threadIdx.x];
+                    if (p != 0.0f) spread -= p * ((reference(from[r][0][threadIdx.x]) - reference(joined.top)) * a.inv_t);
                 }
             }
             float loss;
-            s_grad[threadIdx.x] = finish_frame(a, teacher, joined, cross, loss);
+            s_grad[threadIdx.x] = finish_frame(a, teacher, joined, spread, loss);
             red[0][threadIdx.x] = loss;
         }
         __syncthreads();
@@ -380,8 +383,7 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
                 if (local < 0 || local >= cta_rows) continue;
                 seen[(local >> 5) * kCols + my_col] = 0u;
                 bool leads = true;
-                float q = p[k * kCols + my_col];
-                if (twice) q = named_slots<kCols>(index, p, a.K, k, my_col, leads);
+                const float q = twice ? named_slots<kCols>(index, log_p, a.K, k, my_col, leads) : expf(log_p[k * kCols + my_col]);
                 if (leads) a.dz[i * a.dzs + tile * kCols + my_col] = from_float<T>(soft_part(g, logit(i, my_col), a.scale) - g.slope * q);
             }
         }
@@ -406,14 +408,14 @@ __device__ __forceinline__ void teacher_slots(const Distill<T> &a, int cta, floa
     extern __shared__ __align__(16) uint8_t buffer[];
     __shared__ float red[3][kColumnThreads / 32 * kFinishCols];
     int *const index = reinterpret_cast<int *>(buffer);
-    float *const p = reinterpret_cast<float *>(index + a.K * kFinishCols);
+    float *const log_p = reinterpret_cast<float *>(index + a.K * kFinishCols);
     const int col = threadIdx.x % kFinishCols, group = threadIdx.x / kFinishCols, f = cta * kFinishCols + col;
-    const TeacherColumn c = teacher_columns<T, kFinishCols>(a, cta * kFinishCols, index, p, red);
+    const TeacherColumn c = teacher_columns<T, kFinishCols>(a, cta * kFinishCols, index, log_p, red);
     for (int k = group; k < a.K; k += kFinishGroups) {
         const int i = index[k * kFinishCols + col];
         bool leads = false;
         float q = 0.0f;
-        if (i >= 0) q = named_slots<kFinishCols>(index, p, a.K, k, col, leads);
+        if (i >= 0) q = named_slots<kFinishCols>(index, log_p, a.K, k, col, leads);
         slot_index[(long long)k * columns + f] = leads ? i : -1;
         slot_p[(long long)k * columns + f] = q;
     }
@@ -536,7 +538,8 @@ k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunk
         if (group == 0) {
             cross = 0.0f;
             for (int w = 0; w < kColumnThreads / 32; ++w) cross += red[w][col];
-            const FrameGrad g = finish_frame(a, TeacherColumn{teacher[f], teacher[columns + f], teacher[2LL * columns + f]}, s, cross, loss);
+            const TeacherColumn t = {teacher[f], teacher[columns + f], teacher[2LL * columns + f]};
+            const FrameGrad g = finish_frame(a, t, s, t.E - cross, loss);
             grad[f] = g.top;
             grad[columns + f] = g.factor;
             grad[2LL * columns + f] = g.cap;

@@ -3,7 +3,7 @@
 //
 // Common layout of a CTA: LPR lanes of a warp stand side by side along the frames (8 lanes: 128 bytes, 2 lanes: 32 bytes of a row), the 32 / LPR
 // groups of a warp and the warps of the CTA one row below the other; a thread's further rows follow at a distance of all of them.  A cluster of
-// 1 to 16 CTAs shares the rows of one column tile, so that a tile is read once and held in registers between the statistics and what is made of
+// 1 to 8 CTAs shares the rows of one column tile, so that a tile is read once and held in registers between the statistics and what is made of
 // them; the column sums cross the warps through shared memory and the CTAs through distributed shared memory.
 #pragma once
 
@@ -128,11 +128,10 @@ __device__ __forceinline__ void peer_send(uint32_t to, float v, uint32_t bar)
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(to), "f"(v), "r"(bar) : "memory");
 }
 
-// Launch with clusters of `cluster` CTAs (grid.x is a multiple of it); 16 needs the kernel's opt-in.
+// Launch with clusters of `cluster` CTAs (grid.x is a multiple of it).
 template <typename... P, typename... A>
 inline int launch_cluster(void (*kernel)(P...), unsigned cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A &&...args)
 {
-    if (cluster > 8 && !allow_cluster_16_once(reinterpret_cast<const void *>(kernel))) return (int)cudaErrorInvalidClusterSize;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -163,7 +162,7 @@ template <typename T, int LPR> struct Column {
 struct ColumnSum { __device__ static float join(float a, float b) { return a + b; }  static constexpr float none = 0.0f; };
 struct ColumnMax { __device__ static float join(float a, float b) { return fmaxf(a, b); }  static constexpr float none = -INFINITY; };
 
-constexpr int kColumnThreads = 256, kMostCluster = 16;
+constexpr int kColumnThreads = 256;
 
 // Shared memory of one exchange of Q values a column; consecutive exchanges alternate between two of them, since a neighbour may still be reading.
 // The parts of the cluster's CTAs, exchange_bytes(cluster) of them, lie in dynamic shared memory: their number is the launch's, and what they take decides
@@ -262,6 +261,15 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
             const float4 o = *reinterpret_cast<const float4 *>(&e.out[q * kCols + c.col + j]);
             v[q][j] = o.x; v[q][j + 1] = o.y; v[q][j + 2] = o.z; v[q][j + 3] = o.w;
         }
+}
+
+// CTAs that share a column tile (128 bytes of a row) of a kernel that streams over N rows: as many as an SM holds four of, and eight rounds of rows for each.
+// (One more doubling, to a second round of CTAs, or clusters of 16, lost: layer norm of 16384 x 4096 bf16 72 us, 87 by clusters of 16; 3000 x 5001 33 and 37.)
+inline unsigned streaming_cluster(int N, long long tiles)
+{
+    unsigned cl = 1;
+    while (cl < 8 && tiles * cl <= 2LL * device_info().sm_count && N > 32 * 8 * (int)cl) cl *= 2;
+    return cl;
 }
 
 // How a layer of N rows and F frames is cut: `lanes` lanes along a row, clusters of `cluster` CTAs, `most` at most (0: its columns are too long for one),

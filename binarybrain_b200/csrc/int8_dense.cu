@@ -766,8 +766,7 @@ static int quantize_frames(const T *x, int8_t *q, float *scale, int N, int F, in
     constexpr int kCols = Column<T, 8>::kCols;
     const long long tiles = ((long long)F + kCols - 1) / kCols, bands = ((long long)N + kQuantRows - 1) / kQuantRows;
     BB200_REQUIRE(bands <= 65535, BBCU_ERR_TOO_LARGE);
-    unsigned cl = 1;
-    while (cl < (unsigned)kMostCluster && tiles * cl <= 4LL * device_info().sm_count && N > 32 * 8 * (int)cl) cl *= 2;
+    const unsigned cl = streaming_cluster(N, tiles);
     if (const int e = launch_cluster(aligned ? k_quantize_scale<T, true> : k_quantize_scale<T, false>, cl, (unsigned)(tiles * cl), kQuantThreads, 0, st, x, scale, N, F,
                                      (long long)xs)) return e;
     launch(aligned ? k_quantize_apply<T, true> : k_quantize_apply<T, false>, dim3((unsigned)tiles, (unsigned)bands), kQuantThreads, 0, st, x, q, scale, N, F, xs, qs);

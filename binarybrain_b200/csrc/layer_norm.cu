@@ -482,14 +482,6 @@ __global__ void __launch_bounds__(256) k_layer_norm_no_frames(float *dgamma, flo
     if (n < N && dbeta) dbeta[n] = 0.0f;
 }
 
-// CTAs that share a column tile of the statistics: about eight CTAs an SM, and a round of rows for each
-static unsigned stats_cluster(int N, long long tiles)
-{
-    unsigned cl = 1;
-    while (cl < (unsigned)kMostCluster && tiles * cl <= 4LL * device_info().sm_count && N > 32 * 8 * (int)cl) cl *= 2;
-    return cl;
-}
-
 constexpr int kNormRows = 16, kNormGradRows = 8;         // rows a thread where everything is read once, at most
 constexpr int kNormSmem = 120 * 1024;                    // more than either direction's tile, weights and parts take
 
@@ -543,7 +535,7 @@ static int layer_norm_forward(const T *x, T *y, const float *gamma, const float 
     constexpr int kCols = Column<T, 8>::kCols, kWide = 32 * kFramesPerVec<T>;
     const long long tiles = ((long long)F + kCols - 1) / kCols, bands = ((long long)N + 8 * kApplyRows - 1) / (8 * kApplyRows);
     BB200_REQUIRE(bands <= 65535, BBCU_ERR_TOO_LARGE);
-    const unsigned cl = stats_cluster(N, tiles);
+    const unsigned cl = streaming_cluster(N, tiles);
     if (const int e = launch_cluster(aligned ? k_layer_norm_stats<T, true> : k_layer_norm_stats<T, false>, cl, (unsigned)(tiles * cl), kNormThreads, 0, st, x, mean, rstd,
                                      eps, N, F, xs)) return e;
     launch(aligned ? k_layer_norm_apply<T, true> : k_layer_norm_apply<T, false>, dim3((unsigned)((F + kWide - 1) / kWide), (unsigned)bands), kNormThreads, 0, st, x, y, gamma,
@@ -574,7 +566,7 @@ static int layer_norm_backward(const T *x, const T *dy, T *dx, const float *gamm
     BB200_REQUIRE(scratch != nullptr, BBCU_ERR_NO_MEMORY);
     float *sums = reinterpret_cast<float *>(scratch);
     float2 *grad_part = reinterpret_cast<float2 *>(scratch + sums_bytes);
-    const unsigned cl = stats_cluster(N, tiles);
+    const unsigned cl = streaming_cluster(N, tiles);
     if (const int e = launch_cluster(aligned ? k_layer_norm_grad_stats<T, true> : k_layer_norm_grad_stats<T, false>, cl, (unsigned)(tiles * cl), kNormThreads, 0, st, x, dy,
                                      gamma, mean, rstd, sums, padded, N, F, xs, dys)) return e;
     launch(aligned ? k_layer_norm_grad_apply<T, kRows, true> : k_layer_norm_grad_apply<T, kRows, false>, dim3((unsigned)sweeps, (unsigned)bands), kNormThreads, 0, st, x, dy,

@@ -102,22 +102,6 @@ bool allow_big_smem_once(const void *kernel, int bytes)
     return true;
 }
 
-bool allow_cluster_16_once(const void *kernel)
-{
-    static std::mutex mu;
-    static std::map<std::pair<int, const void *>, bool> done;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    std::lock_guard<std::mutex> g(mu);
-    auto it = done.find({dev, kernel});
-    if (it == done.end()) {
-        const bool ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
-        if (!ok) { cudaGetLastError(); return false; }
-        it = done.emplace(std::make_pair(dev, kernel), ok).first;
-    }
-    return it->second;
-}
-
 int resident_clusters(const void *kernel, int cluster, int threads, size_t smem)
 {
     static std::mutex mu;
@@ -128,7 +112,6 @@ int resident_clusters(const void *kernel, int cluster, int threads, size_t smem)
     std::lock_guard<std::mutex> g(mu);
     auto it = known.find(key);
     if (it == known.end()) {
-        if (cluster > 8) allow_cluster_16_once(kernel);
         int n = 0;
         cudaError_t e;
         if (cluster > 1) {
