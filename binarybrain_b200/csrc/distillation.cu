@@ -77,9 +77,9 @@ template <> __device__ __forceinline__ uint4 packed_max<__nv_bfloat16>(const uin
 }
 
 // ---- the teacher's side of COLS frames from f0 on, by a CTA of a multiple of COLS threads: thread t has column t % COLS and every (threads / COLS)-th
-// slot of it.  index[slot][column] (-1: empty) and log_p[slot][column] (-inf: p = 0) go to shared memory, and to each thread, for its column, P = sum p, E = sum p log p
-// and the weight (0: the frame takes no part).  A barrier stands behind the last write of the two; red[0] and red[1] may still be read.
-struct TeacherColumn { float P, E, weight; };
+// slot of it.  index[slot][column] (-1: empty) and log_p[slot][column] (-inf: p = 0) go to shared memory, and to each thread, for its column, P = sum p and the
+// weight (0: the frame takes no part).  A barrier stands behind the last write of the two; red[0] may still be read.
+struct TeacherColumn { float P, weight; };
 
 // a value of each column joined over the lanes of a warp that have it
 template <int COLS, typename JOIN> __device__ __forceinline__ float column_of_warp(float v, JOIN join)
@@ -115,9 +115,8 @@ __device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, in
         red[1][own] = slots;
     }
     __syncthreads();
-    top = red[0][col];
-    slots = red[1][col];
-    for (int e = 1; e < warps; ++e) { top = fmaxf(top, red[0][e * COLS + col]); slots += red[1][e * COLS + col]; }
+    top = join_parts<ColumnMax>(&red[0][col], COLS, warps);
+    slots = join_parts<ColumnSum>(&red[1][col], COLS, warps);
     const bool live = slots > 0.0f && w != 0.0f;
     float lse = 0.0f;
     if (a.t_lse) {
@@ -130,31 +129,22 @@ __device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, in
         sum = column_of_warp<COLS>(sum, [](float a, float b) { return a + b; });
         if (threadIdx.x % 32 < COLS) red[2][own] = sum;
         __syncthreads();
-        sum = red[2][col];
-        for (int e = 1; e < warps; ++e) sum += red[2][e * COLS + col];
+        sum = join_parts<ColumnSum>(&red[2][col], COLS, warps);
         lse = top * a.inv_t + logf(sum);
     }
-    float P = 0.0f, E = 0.0f;
+    float P = 0.0f;
     for (int k = group; k < a.K; k += groups) {
         float lp = -INFINITY;
         if (live && index[k * COLS + col] >= 0) {
             lp = log_p[k * COLS + col] * a.inv_t - lse;
-            const float p = expf(lp);
-            if (p != 0.0f) E += p * lp;
-            P += p;
+            P += expf(lp);
         }
         log_p[k * COLS + col] = lp;
     }
     P = column_of_warp<COLS>(P, [](float a, float b) { return a + b; });
-    E = column_of_warp<COLS>(E, [](float a, float b) { return a + b; });
-    if (threadIdx.x % 32 < COLS) {
-        red[0][own] = P;
-        red[1][own] = E;
-    }
+    if (threadIdx.x % 32 < COLS) red[0][own] = P;
     __syncthreads();
-    TeacherColumn c = {red[0][col], red[1][col], live ? w : 0.0f};
-    for (int e = 1; e < warps; ++e) { c.P += red[0][e * COLS + col]; c.E += red[1][e * COLS + col]; }
-    return c;
+    return {join_parts<ColumnSum>(&red[0][col], COLS, warps), live ? w : 0.0f};
 }
 
 // The probabilities of all slots of the column that name the class of slot k, in the order of the slots; `first`: k is the first of them.
@@ -171,16 +161,12 @@ template <int COLS> __device__ __forceinline__ float named_slots(const int *inde
     return sum;
 }
 
-// From a frame's joined parts (spread = sum p (log p - (z - top) / T) over the slots) its gradient's factors and its loss.
-template <typename T>
-__device__ __forceinline__ FrameGrad finish_frame(const Distill<T> &a, const TeacherColumn &c, const SoftSum &s, float spread, float &loss)
+// From a frame's joined sums its gradient's factors.  No class left: q = 0.
+template <typename T> __device__ __forceinline__ FrameGrad finish_frame(const Distill<T> &a, float P, float weight, const SoftSum &s)
 {
-    loss = 0.0f;
-    if (c.weight == 0.0f) return {0.0f, 0.0f, 0.0f, 0.0f};
-    const bool none = s.top == -INFINITY && s.sum == 0.0f;                // no class is left: the spread is infinite, as the loss is, and q = 0
-    const float slope = a.grad_reduction * c.weight * a.temperature;
-    loss = c.weight * a.temperature * a.temperature * (spread + (none ? 0.0f : c.P * logf(s.sum)));
-    return {reference(s.top), none ? 0.0f : slope * c.P / s.sum, INFINITY, slope};
+    if (weight == 0.0f) return {0.0f, 0.0f, 0.0f, 0.0f};
+    const float slope = a.grad_reduction * weight * a.temperature;
+    return {reference(s.top), s.top == -INFINITY && s.sum == 0.0f ? 0.0f : slope * P / s.sum, INFINITY, slope};
 }
 
 // loss_buf of the first warp's columns, and their sum
@@ -205,7 +191,7 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
     static_assert(kCols <= 32, "a warp finishes the columns");
     extern __shared__ __align__(16) uint8_t buffer[];
-    __shared__ float red[3][kColumnThreads / 32 * kCols], red_soft[kColumnThreads / 32][kCols], s_top[kCols];
+    __shared__ float red[3][kColumnThreads / 32 * kCols], red_soft[kColumnThreads / 32][kCols], s_top[kCols], s_log_sum[kCols];
     __shared__ FrameGrad s_grad[kCols];
     __shared__ uint64_t bar[2];
     __shared__ int gave_up;
@@ -275,9 +261,7 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
         }
         __syncthreads();                                                  // (the logits of the other threads are there, too)
         if (threadIdx.x < kCols) {
-            float t = red_soft[0][threadIdx.x];
-            for (int w = 1; w < c.warps; ++w) t = fmaxf(t, red_soft[w][threadIdx.x]);
-            s_top[threadIdx.x] = t;
+            s_top[threadIdx.x] = join_parts<ColumnMax>(&red_soft[0][threadIdx.x], kCols, c.warps);
         }
         __syncthreads();
 #pragma unroll
@@ -304,34 +288,33 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
         int twice = 0;
         for (int k = group; k < a.K; k += groups) {
             const int i = index[k * kCols + my_col], local = i - cta_first;
-            const float lp = log_p[k * kCols + my_col], p = expf(lp);
             if (local >= 0 && local < cta_rows) {
                 const unsigned bit = 1u << (local & 31);
                 twice |= (int)(atomicOr(&seen[(local >> 5) * kCols + my_col], bit) & bit);
-                if (p != 0.0f) {
-                    spread += p * (lp - (logit(i, my_col) - own_top) * a.inv_t);
-                    own_p += p;
+                if (cl > 1) {
+                    const float lp = log_p[k * kCols + my_col], p = expf(lp);
+                    if (p != 0.0f) {
+                        spread += p * (lp - (logit(i, my_col) - own_top) * a.inv_t);
+                        own_p += p;
+                    }
                 }
             }
         }
-        spread = column_of_warp<kCols>(spread, [](float a, float b) { return a + b; });
-        own_p = column_of_warp<kCols>(own_p, [](float a, float b) { return a + b; });
-        if (c.lane < kCols) {
-            red[0][c.warp * kCols + c.lane] = spread;
-            red[1][c.warp * kCols + c.lane] = own_p;
+        if (cl > 1) {
+            spread = column_of_warp<kCols>(spread, [](float a, float b) { return a + b; });
+            own_p = column_of_warp<kCols>(own_p, [](float a, float b) { return a + b; });
+            if (c.lane < kCols) {
+                red[0][c.warp * kCols + c.lane] = spread;
+                red[1][c.warp * kCols + c.lane] = own_p;
+            }
+            if (threadIdx.x == 0) mbar_arrive_expect_tx(&bar[turn & 1], cl * 4 * kCols * (uint32_t)sizeof(float));
         }
-        if (cl > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(&bar[turn & 1], cl * 4 * kCols * (uint32_t)sizeof(float));
         twice = __syncthreads_or(twice);
         if (threadIdx.x < kCols) {                                        // all of them in the first warp
-            float s = 0.0f;
-            spread = own_p = 0.0f;
-            for (int w = 0; w < c.warps; ++w) {
-                s += red_soft[w][threadIdx.x];
-                spread += red[0][w * kCols + threadIdx.x];
-                own_p += red[1][w * kCols + threadIdx.x];
-            }
-            SoftSum joined = {s_top[threadIdx.x], s};
+            SoftSum joined = {s_top[threadIdx.x], join_parts<ColumnSum>(&red_soft[0][threadIdx.x], kCols, c.warps)};
             if (cl > 1) {
+                spread = join_parts<ColumnSum>(&red[0][threadIdx.x], kCols, c.warps);
+                own_p = join_parts<ColumnSum>(&red[1][threadIdx.x], kCols, c.warps);
                 float (*const from)[4][kCols] = part + (turn & 1) * cl, (*const to)[kCols] = from[rank];
                 for (uint32_t r = 0; r < cl; ++r) {
                     const uint32_t b = peer_addr(&bar[turn & 1], r);
@@ -354,12 +337,13 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
                     if (p != 0.0f) spread -= p * ((reference(from[r][0][threadIdx.x]) - reference(joined.top)) * a.inv_t);
                 }
             }
-            float loss;
-            s_grad[threadIdx.x] = finish_frame(a, teacher, joined, spread, loss);
-            red[0][threadIdx.x] = loss;
+            s_grad[threadIdx.x] = finish_frame(a, teacher.P, teacher.weight, joined);
+            const float log_sum = joined.sum == 0.0f ? 0.0f : logf(joined.sum);     // (no class left: the spread is infinite, as the loss is)
+            s_log_sum[threadIdx.x] = log_sum;
+            red[0][threadIdx.x] = teacher.weight == 0.0f ? 0.0f : teacher.weight * a.temperature * a.temperature * (spread + teacher.P * log_sum);
         }
         __syncthreads();
-        if (rank == 0 && c.warp == 0)
+        if (cl > 1 && rank == 0 && c.warp == 0)
             write_losses(a, tile, tile * kCols + c.lane, c.lane < kCols && tile * kCols + c.lane < a.F, c.lane < kCols ? red[0][c.lane] : 0.0f);
         if (f < a.F) {
             FrameGrad g[kVec];
@@ -376,19 +360,32 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
             }
         }
         __syncthreads();                                                  // the CTA's values of dz stand before those of the named classes are written again
+        float divergence = 0.0f;                                          // of a CTA by itself: term by term, which keeps the digits of a small one
         if (tile * kCols + my_col < a.F) {
             const FrameGrad g = s_grad[my_col];
+            const float log_sum = s_log_sum[my_col];
             for (int k = group; k < a.K; k += groups) {
                 const int i = index[k * kCols + my_col], local = i - cta_first;
                 if (local < 0 || local >= cta_rows) continue;
                 seen[(local >> 5) * kCols + my_col] = 0u;
                 bool leads = true;
-                const float q = twice ? named_slots<kCols>(index, log_p, a.K, k, my_col, leads) : expf(log_p[k * kCols + my_col]);
+                const float lp = log_p[k * kCols + my_col], p = expf(lp);
+                if (cl == 1 && p != 0.0f) divergence += p * (lp - ((logit(i, my_col) - g.top) * a.inv_t - log_sum));
+                const float q = twice ? named_slots<kCols>(index, log_p, a.K, k, my_col, leads) : p;
                 if (leads) a.dz[i * a.dzs + tile * kCols + my_col] = from_float<T>(soft_part(g, logit(i, my_col), a.scale) - g.slope * q);
             }
         }
+        if (cl == 1) {
+            divergence = column_of_warp<kCols>(divergence, [](float a, float b) { return a + b; });
+            if (c.lane < kCols) red[2][c.warp * kCols + c.lane] = divergence;
+        }
         __syncthreads();                                                  // nobody needs the logits and the slots any more
         fetch(f + clusters * kCols);
+        if (cl == 1 && c.warp == 0) {                                     // (red[2] is written again behind a barrier of this warp)
+            const bool has = c.lane < kCols && tile * kCols + c.lane < a.F;
+            write_losses(a, tile, tile * kCols + c.lane, has,
+                         has && teacher.weight != 0.0f ? teacher.weight * a.temperature * a.temperature * join_parts<ColumnSum>(&red[2][c.lane], kCols, c.warps) : 0.0f);
+        }
     }
     if (cl > 1) {
         if (threadIdx.x == 0 && gave_up) atomicCAS(fault, 0, kFaultBarrierTimeout);
@@ -399,11 +396,12 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
 }
 
 // ---- more classes than that: the teacher's side beside the softmax's sums, what follows from both for a frame, dz of all classes, dz of the named ones.
-// The teacher's CTAs have eight frames, 32 threads for each, and leave P, E and weight as teacher[3][columns] and the slots as the last kernel takes them:
-// the class, or -1 where the slot is empty or names a class that an earlier one does, and the probabilities of a class added up.
+// The teacher's CTAs have eight frames, 32 threads for each, and leave P and weight as teacher[2][columns], and of every slot its class i (~1 - i where an
+// earlier slot names it, too, and -1 where the slot is empty), log p, and the probabilities of its class added up.
+struct Slots { int *index; float *log_p, *p; };
 constexpr int kFinishCols = 8, kFinishGroups = kColumnThreads / kFinishCols;
 template <typename T>
-__device__ __forceinline__ void teacher_slots(const Distill<T> &a, int cta, float *teacher, int *slot_index, float *slot_p, int columns)
+__device__ __forceinline__ void teacher_slots(const Distill<T> &a, int cta, float *teacher, const Slots &slots, int columns)
 {
     extern __shared__ __align__(16) uint8_t buffer[];
     __shared__ float red[3][kColumnThreads / 32 * kFinishCols];
@@ -416,13 +414,14 @@ __device__ __forceinline__ void teacher_slots(const Distill<T> &a, int cta, floa
         bool leads = false;
         float q = 0.0f;
         if (i >= 0) q = named_slots<kFinishCols>(index, log_p, a.K, k, col, leads);
-        slot_index[(long long)k * columns + f] = leads ? i : -1;
-        slot_p[(long long)k * columns + f] = q;
+        const long long at = (long long)k * columns + f;
+        slots.index[at] = i < 0 || leads ? i : ~1 - i;
+        slots.log_p[at] = log_p[k * kFinishCols + col];
+        slots.p[at] = q;
     }
     if (group == 0) {
         teacher[f] = c.P;
-        teacher[columns + f] = c.E;
-        teacher[2LL * columns + f] = c.weight;
+        teacher[columns + f] = c.weight;
     }
 }
 
@@ -430,7 +429,7 @@ __device__ __forceinline__ void teacher_slots(const Distill<T> &a, int cta, floa
 // only where one is 2^64 times as much, so that the rows cost little more than their exponentials.
 template <typename T, int LPR, bool ALIGNED>
 __global__ void __launch_bounds__(kColumnThreads, 3)
-k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, float *teacher, int *slot_index, float *slot_p, int teacher_ctas)
+k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, float *teacher, const Slots slots, int teacher_ctas)
 {
     grid_dependency();
     constexpr int kBatch = 8;
@@ -439,7 +438,7 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, flo
     __shared__ SoftSum red[kColumnThreads / 32][kCols];
     const int columns = tiles * kCols;
     if ((int)blockIdx.x < teacher_ctas) {
-        teacher_slots(a, (int)blockIdx.x, teacher, slot_index, slot_p, columns);
+        teacher_slots(a, (int)blockIdx.x, teacher, slots, columns);
         return;
     }
     const Col c;
@@ -505,12 +504,11 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, flo
 // The numbers of FrameGrad as grad[4][columns], and the frames' losses
 template <typename T>
 __global__ void __launch_bounds__(kColumnThreads)
-k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunks, const float *__restrict__ teacher, const int *__restrict__ slot_index,
-                 const float *__restrict__ slot_p, float *grad, int columns)
+k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunks, const float *__restrict__ teacher, const Slots slots, float *grad, int columns)
 {
     grid_dependency();
     __shared__ SoftSum sums[kColumnThreads / 32][kFinishCols];
-    __shared__ float red[kColumnThreads / 32][kFinishCols], s_top[kFinishCols];
+    __shared__ float red[kColumnThreads / 32][kFinishCols], s_top[kFinishCols], s_log_sum[kFinishCols];
     const int col = threadIdx.x % kFinishCols, group = threadIdx.x / kFinishCols, warp = threadIdx.x / 32, f = (int)blockIdx.x * kFinishCols + col;
     SoftSum s = {-INFINITY, 0.0f};
     for (int k = group; k < chunks; k += kFinishGroups) s = join_soft(s, part[(long long)k * columns + f], a.scale);
@@ -521,25 +519,26 @@ k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunk
     if (threadIdx.x < kFinishCols) {
         for (int w = 1; w < kColumnThreads / 32; ++w) s = join_soft(s, sums[w][col], a.scale);
         s_top[col] = reference(s.top);
+        s_log_sum[col] = s.sum == 0.0f ? 0.0f : logf(s.sum);
     }
     __syncthreads();
-    const float top = s_top[col];
-    float cross = 0.0f;
+    const float top = s_top[col], log_sum = s_log_sum[col];
+    float divergence = 0.0f;
     for (int k = group; k < a.K; k += kFinishGroups) {
-        const int i = slot_index[(long long)k * columns + f];
-        const float q = slot_p[(long long)k * columns + f];
-        if (i >= 0 && q != 0.0f) cross += q * ((to_float(a.z[i * a.zs + f]) - top) * a.inv_t);
+        const long long at = (long long)k * columns + f;
+        const int code = slots.index[at], i = code < -1 ? ~1 - code : code;
+        const float lp = slots.log_p[at], p = expf(lp);
+        if (i >= 0 && p != 0.0f) divergence += p * (lp - ((to_float(a.z[i * a.zs + f]) - top) * a.inv_t - log_sum));
     }
-    cross = column_of_warp<kFinishCols>(cross, [](float x, float y) { return x + y; });
-    if (threadIdx.x % 32 < kFinishCols) red[warp][col] = cross;
+    divergence = column_of_warp<kFinishCols>(divergence, [](float x, float y) { return x + y; });
+    if (threadIdx.x % 32 < kFinishCols) red[warp][col] = divergence;
     __syncthreads();
     if (threadIdx.x < 32) {
         float loss = 0.0f;
         if (group == 0) {
-            cross = 0.0f;
-            for (int w = 0; w < kColumnThreads / 32; ++w) cross += red[w][col];
-            const TeacherColumn t = {teacher[f], teacher[columns + f], teacher[2LL * columns + f]};
-            const FrameGrad g = finish_frame(a, t, s, t.E - cross, loss);
+            const float weight = teacher[columns + f];
+            const FrameGrad g = finish_frame(a, teacher[f], weight, s);
+            if (weight != 0.0f) loss = weight * a.temperature * a.temperature * join_parts<ColumnSum>(&red[0][col], kFinishCols, kColumnThreads / 32);
             grad[f] = g.top;
             grad[columns + f] = g.factor;
             grad[2LL * columns + f] = g.cap;
@@ -582,15 +581,15 @@ k_distill_apply(const Distill<T> a, const float *__restrict__ grad, int columns)
 // the named classes, a frame and slot a thread
 template <typename T>
 __global__ void __launch_bounds__(kColumnThreads)
-k_distill_named(const Distill<T> a, const float *__restrict__ grad, const int *__restrict__ slot_index, const float *__restrict__ slot_p, int columns)
+k_distill_named(const Distill<T> a, const float *__restrict__ grad, const Slots slots, int columns)
 {
     grid_dependency();
     const int f = (int)blockIdx.x * kColumnThreads + threadIdx.x, k = blockIdx.y;
     if (f >= a.F) return;
-    const int i = slot_index[(long long)k * columns + f];
+    const int i = slots.index[(long long)k * columns + f];
     if (i < 0) return;
     const FrameGrad g = {grad[f], grad[columns + f], grad[2LL * columns + f], grad[3LL * columns + f]};
-    a.dz[i * a.dzs + f] = from_float<T>(soft_part(g, to_float(a.z[i * a.zs + f]), a.scale) - g.slope * slot_p[(long long)k * columns + f]);
+    a.dz[i * a.dzs + f] = from_float<T>(soft_part(g, to_float(a.z[i * a.zs + f]), a.scale) - g.slope * slots.p[(long long)k * columns + f]);
 }
 
 __global__ void __launch_bounds__(1024) k_distill_loss(const double *__restrict__ part, int parts, double loss_reduction, float *loss)
@@ -654,23 +653,23 @@ static int distillation_passes(Distill<T> &a, int &loss_parts, bool aligned, cud
     const int rows = (a.C + chunks - 1) / chunks;
     loss_parts = columns / kFinishCols;
     const size_t part_b = (size_t)chunks * columns * sizeof(SoftSum), loss_b = (size_t)loss_parts * sizeof(double), slots = (size_t)a.K * columns;
-    char *scratch = static_cast<char *>(stream_scratch(st, loss_b + part_b + ((size_t)7 * columns + 2 * slots) * 4, kFrameOpSlot));
+    char *scratch = static_cast<char *>(stream_scratch(st, loss_b + part_b + ((size_t)6 * columns + 3 * slots) * 4, kFrameOpSlot));
     BB200_REQUIRE(scratch != nullptr, BBCU_ERR_NO_MEMORY);
     a.loss_part = reinterpret_cast<double *>(scratch);
     SoftSum *part = reinterpret_cast<SoftSum *>(scratch + loss_b);
-    float *grad = reinterpret_cast<float *>(scratch + loss_b + part_b), *teacher = grad + (size_t)4 * columns, *slot_p = teacher + (size_t)3 * columns;
-    int *slot_index = reinterpret_cast<int *>(slot_p + slots);
+    float *grad = reinterpret_cast<float *>(scratch + loss_b + part_b), *teacher = grad + (size_t)4 * columns, *slot_p = teacher + (size_t)2 * columns;
+    const Slots kept = {reinterpret_cast<int *>(slot_p + 2 * slots), slot_p + slots, slot_p};
     const size_t teacher_smem = (size_t)a.K * kFinishCols * 8;
     BB200_REQUIRE((long long)tiles * chunks + loss_parts < (1LL << 31), BBCU_ERR_TOO_LARGE);
-    launch(sums, (unsigned)(tiles * chunks + loss_parts), kColumnThreads, teacher_smem, st, a, part, rows, tiles, teacher, slot_index, slot_p, loss_parts);
+    launch(sums, (unsigned)(tiles * chunks + loss_parts), kColumnThreads, teacher_smem, st, a, part, rows, tiles, teacher, kept, loss_parts);
     BB200_CUDA(cudaPeekAtLastError());
-    launch(k_distill_finish<T>, (unsigned)loss_parts, kColumnThreads, 0, st, a, part, chunks, teacher, slot_index, slot_p, grad, columns);
+    launch(k_distill_finish<T>, (unsigned)loss_parts, kColumnThreads, 0, st, a, part, chunks, teacher, kept, grad, columns);
     BB200_CUDA(cudaPeekAtLastError());
     launch(aligned ? k_distill_apply<T, true> : k_distill_apply<T, false>, dim3((unsigned)((a.F + kWide - 1) / kWide), (unsigned)bands), kColumnThreads, 0, st, a, grad,
            columns);
     BB200_CUDA(cudaPeekAtLastError());
     if (a.K > 0)
-        launch(k_distill_named<T>, dim3((unsigned)((a.F + kColumnThreads - 1) / kColumnThreads), (unsigned)a.K), kColumnThreads, 0, st, a, grad, slot_index, slot_p, columns);
+        launch(k_distill_named<T>, dim3((unsigned)((a.F + kColumnThreads - 1) / kColumnThreads), (unsigned)a.K), kColumnThreads, 0, st, a, grad, kept, columns);
     return launch_status();
 }
 

@@ -208,6 +208,19 @@ struct Cluster {
     }
 };
 
+// Up to eight values `distance` apart, in their order; all of them on their way before the first is joined.
+template <typename OP> __device__ __forceinline__ float join_parts(const float *from, int distance, int count)
+{
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < count ? from[i * distance] : 0.0f;
+    float s = v[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i)
+        if (i < count) s = OP::join(s, v[i]);
+    return s;
+}
+
 // Joins v[Q][kVec] over all rows of the tile (CTA, then cluster) by a fixed order of operations; what finish(q, joined) makes of a value comes back in
 // v for the thread's own columns.  One thread a value joins the parts, since there are many threads and few columns.  `phase`: of the exchange's barrier,
 // 0 and 1 in turn.
@@ -231,8 +244,7 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
     if (cl.size > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(&e.bar, cl.size * Q * kCols * (uint32_t)sizeof(float));
     __syncthreads();
     for (int i = threadIdx.x; i < Q * kCols; i += blockDim.x) {
-        float s = e.red[0][i];
-        for (int w = 1; w < c.warps; ++w) s = OP::join(s, e.red[w][i]);
+        const float s = join_parts<OP>(&e.red[0][i], Q * kCols, c.warps);
         if (cl.size == 1) {
             e.out[i] = finish(i / kCols, s);
         } else {
@@ -248,9 +260,7 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
             }
         }
         for (int i = threadIdx.x; i < Q * kCols; i += blockDim.x) {
-            float s = e.part[0][i];
-            for (uint32_t r = 1; r < cl.size; ++r) s = OP::join(s, e.part[r][i]);
-            e.out[i] = finish(i / kCols, s);
+            e.out[i] = finish(i / kCols, join_parts<OP>(&e.part[0][i], Q * kCols, (int)cl.size));
         }
     }
     __syncthreads();
