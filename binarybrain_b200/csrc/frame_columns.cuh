@@ -273,13 +273,19 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
         }
 }
 
-// CTAs that share a column tile (128 bytes of a row) of a kernel that streams over N rows: as many as an SM holds four of, and eight rounds of rows for each.
-// (One more doubling, to a second round of CTAs, or clusters of 16, lost: layer norm of 16384 x 4096 bf16 72 us, 87 by clusters of 16; 3000 x 5001 33 and 37.)
-inline unsigned streaming_cluster(int N, long long tiles)
+// How a kernel that streams over N rows is cut: `lanes` lanes along a row, 8 or, where those would leave most SMs without a cluster, 2; clusters that share
+// a column tile, of as many CTAs as an SM holds four of and eight rounds of rows for each.  (Backward of 65536 x 64: 81 us by 8 lanes, 38 by 2; of 65536 x 1024,
+// 256 CTAs by 8 lanes, 219 and 270.  One more doubling of the cluster, to a second round of CTAs, or clusters
+// of 16, lost: layer norm of 16384 x 4096 bf16 72 us, 87 by clusters of 16; 3000 x 5001 33 and 37.)
+struct StreamingPlan { int lanes; unsigned cluster, ctas; };
+template <typename T> inline StreamingPlan plan_streaming(int N, int F)
 {
+    const long long sms = device_info().sm_count;
+    auto tiles = [&](int lanes) { return ((long long)F + lanes * kFramesPerVec<T> - 1) / (lanes * kFramesPerVec<T>); };
+    const int lanes = tiles(8) * 8 < sms ? 2 : 8;
     unsigned cl = 1;
-    while (cl < 8 && tiles * cl <= 2LL * device_info().sm_count && N > 32 * 8 * (int)cl) cl *= 2;
-    return cl;
+    while (cl < 8 && tiles(lanes) * cl <= 2 * sms && N > 256 / lanes * 8 * (int)cl) cl *= 2;
+    return {lanes, cl, (unsigned)(tiles(lanes) * cl)};
 }
 
 // How a layer of N rows and F frames is cut: `lanes` lanes along a row, clusters of `cluster` CTAs, `most` at most (0: its columns are too long for one),

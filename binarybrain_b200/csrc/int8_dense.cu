@@ -60,14 +60,14 @@ template <typename T> __device__ __forceinline__ uint32_t packed_abs_max(uint32_
     return sizeof(T) == 4 ? max(a, b & 0x7fffffffu) : __vmaxu2(a, b & 0x7fff7fffu);
 }
 
-// A cluster has the columns of 128 bytes of a row; its CTAs take turns at the rows and join the largest magnitudes in the first CTA's shared memory.
-template <typename T, bool ALIGNED>
+// A cluster has the columns of 128 (few frames: 32) bytes of a row; its CTAs take turns at the rows and join the largest magnitudes in the first CTA's shared memory.
+template <typename T, int LPR, bool ALIGNED>
 __global__ void __launch_bounds__(kQuantThreads, 4)
 k_quantize_scale(const T *x, float *scale_out, int N, int F, long long xs)
 {
     grid_dependency();
-    constexpr int kLpr = 8, kBatch = 8;
-    using Col = Column<T, kLpr>;
+    constexpr int kBatch = 8;
+    using Col = Column<T, LPR>;
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
     __shared__ uint32_t red[8][kCols];
     __shared__ float part[kCols];
@@ -94,10 +94,10 @@ k_quantize_scale(const T *x, float *scale_out, int N, int F, long long xs)
 #pragma unroll
     for (int j = 0; j < kVec; ++j) top[j] = __float_as_uint(v[j]);
 #pragma unroll
-    for (int m = kLpr; m < 32; m <<= 1)
+    for (int m = LPR; m < 32; m <<= 1)
 #pragma unroll
         for (int j = 0; j < kVec; ++j) top[j] = max(top[j], __shfl_xor_sync(0xffffffffu, top[j], m));
-    if (c.lane < kLpr) {
+    if (c.lane < LPR) {
 #pragma unroll
         for (int j = 0; j < kVec; ++j) red[c.warp][c.col + j] = top[j];
     }
@@ -766,9 +766,10 @@ static int quantize_frames(const T *x, int8_t *q, float *scale, int N, int F, in
     constexpr int kCols = Column<T, 8>::kCols;
     const long long tiles = ((long long)F + kCols - 1) / kCols, bands = ((long long)N + kQuantRows - 1) / kQuantRows;
     BB200_REQUIRE(bands <= 65535, BBCU_ERR_TOO_LARGE);
-    const unsigned cl = streaming_cluster(N, tiles);
-    if (const int e = launch_cluster(aligned ? k_quantize_scale<T, true> : k_quantize_scale<T, false>, cl, (unsigned)(tiles * cl), kQuantThreads, 0, st, x, scale, N, F,
-                                     (long long)xs)) return e;
+    const StreamingPlan s = plan_streaming<T>(N, F);
+    auto scales = s.lanes == 2 ? (aligned ? k_quantize_scale<T, 2, true> : k_quantize_scale<T, 2, false>)
+                               : (aligned ? k_quantize_scale<T, 8, true> : k_quantize_scale<T, 8, false>);
+    if (const int e = launch_cluster(scales, s.cluster, s.ctas, kQuantThreads, 0, st, x, scale, N, F, (long long)xs)) return e;
     launch(aligned ? k_quantize_apply<T, true> : k_quantize_apply<T, false>, dim3((unsigned)tiles, (unsigned)bands), kQuantThreads, 0, st, x, q, scale, N, F, xs, qs);
     return launch_status();
 }

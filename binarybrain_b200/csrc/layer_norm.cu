@@ -24,16 +24,16 @@ constexpr int kNormThreads = 256;                      // of the kernels that st
 // ---- two passes: statistics of the frames, then what is made of them.  The second one finds what L2 (126 MB) still holds of the first.
 // (8192 x 16384 fp32: statistics 88 us, y 154; backward of 65536 x 1024 230 us with the sums of the weights, 134 of them and less for the second pass.)
 
-// A cluster has the columns of 128 bytes of a row; its CTAs take turns at the rows, add up d = x minus the column's first value (which takes a large
+// A cluster has the columns of 128 (few frames: 32) bytes of a row; its CTAs take turns at the rows, add up d = x minus the column's first value (which takes a large
 // level out) and d^2, eight rows in 32 bits and those sums in 64, so that neither a level nor a long column costs digits, and join them in the first
 // CTA's shared memory.
-template <typename T, bool ALIGNED>
+template <typename T, int LPR, bool ALIGNED>
 __global__ void __launch_bounds__(kNormThreads, 4)
 k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int N, int F, long long xs)
 {
     grid_dependency();
-    constexpr int kLpr = 8, kBatch = sizeof(T) == 4 ? 8 : 4;
-    using Col = Column<T, kLpr>;
+    constexpr int kBatch = sizeof(T) == 4 ? 8 : 4;
+    using Col = Column<T, LPR>;
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
     __shared__ float2 red[8][kCols];
     __shared__ double2 part[kCols];
@@ -67,13 +67,13 @@ k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int 
         for (int j = 0; j < kVec; ++j) { s1[j] += b1[j]; s2[j] += b2[j]; }
     }
 #pragma unroll
-    for (int m = kLpr; m < 32; m <<= 1)
+    for (int m = LPR; m < 32; m <<= 1)
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
             s1[j] += __shfl_xor_sync(0xffffffffu, s1[j], m);
             s2[j] += __shfl_xor_sync(0xffffffffu, s2[j], m);
         }
-    if (c.lane < kLpr) {
+    if (c.lane < LPR) {
 #pragma unroll
         for (int j = 0; j < kVec; ++j) red[c.warp][c.col + j] = make_float2(s1[j], s2[j]);
     }
@@ -132,14 +132,14 @@ k_layer_norm_apply(const T *x, T *y, const float *__restrict__ gamma, const floa
 }
 
 // backward: sums[frame] = mean_n gamma dy, sums[padded + frame] = mean_n gamma dy xh
-template <typename T, bool ALIGNED>
+template <typename T, int LPR, bool ALIGNED>
 __global__ void __launch_bounds__(kNormThreads, 4)
 k_layer_norm_grad_stats(const T *x, const T *dy, const float *__restrict__ gamma, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
                         float *sums_out, int padded, int N, int F, long long xs, long long dys)
 {
     grid_dependency();
-    constexpr int kLpr = 8, kBatch = sizeof(T) == 4 ? 4 : 2;
-    using Col = Column<T, kLpr>;
+    constexpr int kBatch = sizeof(T) == 4 ? 4 : 2;
+    using Col = Column<T, LPR>;
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
     __shared__ float red[8][2 * kCols];
     __shared__ float part[2 * kCols];
@@ -176,12 +176,12 @@ k_layer_norm_grad_stats(const T *x, const T *dy, const float *__restrict__ gamma
         }
     }
 #pragma unroll
-    for (int m = kLpr; m < 32; m <<= 1)
+    for (int m = LPR; m < 32; m <<= 1)
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int j = 0; j < kVec; ++j) s[q][j] += __shfl_xor_sync(0xffffffffu, s[q][j], m);
-    if (c.lane < kLpr) {
+    if (c.lane < LPR) {
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -539,12 +539,13 @@ static int layer_norm_forward(const T *x, T *y, const float *gamma, const float 
     // 8192 x 16384 251 / 253, bf16 158 / 140; backward 4096 x 16384 bf16 130 / 139, fp32 202 / 231, 8192 x 8192 fp32 225 / 223).
     if (const ColumnPlan p = plan_columns<T>(N, F, sizeof(T) == 4 ? 8 : 4, kNormRows, sizeof(T) == 4 ? 8 : 4); aligned && p.cluster)
         return (p.lanes == 2 ? layer_norm_once<T, 2> : layer_norm_once<T, sizeof(T) == 4 ? 8 : 4>)(x, y, gamma, beta, mean, rstd, eps, N, F, xs, ys, p, st);
-    constexpr int kCols = Column<T, 8>::kCols, kWide = 32 * kFramesPerVec<T>;
-    const long long tiles = ((long long)F + kCols - 1) / kCols, bands = ((long long)N + 8 * kApplyRows - 1) / (8 * kApplyRows);
+    constexpr int kWide = 32 * kFramesPerVec<T>;
+    const long long bands = ((long long)N + 8 * kApplyRows - 1) / (8 * kApplyRows);
     BB200_REQUIRE(bands <= 65535, BBCU_ERR_TOO_LARGE);
-    const unsigned cl = streaming_cluster(N, tiles);
-    if (const int e = launch_cluster(aligned ? k_layer_norm_stats<T, true> : k_layer_norm_stats<T, false>, cl, (unsigned)(tiles * cl), kNormThreads, 0, st, x, mean, rstd,
-                                     eps, N, F, xs)) return e;
+    const StreamingPlan s = plan_streaming<T>(N, F);
+    auto stats = s.lanes == 2 ? (aligned ? k_layer_norm_stats<T, 2, true> : k_layer_norm_stats<T, 2, false>)
+                              : (aligned ? k_layer_norm_stats<T, 8, true> : k_layer_norm_stats<T, 8, false>);
+    if (const int e = launch_cluster(stats, s.cluster, s.ctas, kNormThreads, 0, st, x, mean, rstd, eps, N, F, xs)) return e;
     launch(aligned ? k_layer_norm_apply<T, true> : k_layer_norm_apply<T, false>, dim3((unsigned)((F + kWide - 1) / kWide), (unsigned)bands), kNormThreads, 0, st, x, y, gamma,
            beta, mean, rstd, N, F, xs, ys);
     return launch_status();
@@ -563,8 +564,8 @@ static int layer_norm_backward(const T *x, const T *dy, T *dx, const float *gamm
                                                                                                         F, xs, dys, dxs, p, st);
 #undef BB200_ONCE
     }
-    constexpr int kCols = Column<T, 8>::kCols, kWide = 32 * kFramesPerVec<T>, kRows = 4;
-    const long long tiles = ((long long)F + kCols - 1) / kCols, bands = ((long long)N + 8 * kRows - 1) / (8 * kRows), pieces = ((long long)F + kWide - 1) / kWide;
+    constexpr int kWide = 32 * kFramesPerVec<T>, kRows = 4;
+    const long long bands = ((long long)N + 8 * kRows - 1) / (8 * kRows), pieces = ((long long)F + kWide - 1) / kWide;
     BB200_REQUIRE(bands <= 65535, BBCU_ERR_TOO_LARGE);
     long long sweeps = std::min(pieces, std::max(1LL, (8LL * device_info().sm_count + bands - 1) / bands));
     const int padded = (F + 3) / 4 * 4;
@@ -573,9 +574,10 @@ static int layer_norm_backward(const T *x, const T *dy, T *dx, const float *gamm
     BB200_REQUIRE(scratch != nullptr, BBCU_ERR_NO_MEMORY);
     float *sums = reinterpret_cast<float *>(scratch);
     float2 *grad_part = reinterpret_cast<float2 *>(scratch + sums_bytes);
-    const unsigned cl = streaming_cluster(N, tiles);
-    if (const int e = launch_cluster(aligned ? k_layer_norm_grad_stats<T, true> : k_layer_norm_grad_stats<T, false>, cl, (unsigned)(tiles * cl), kNormThreads, 0, st, x, dy,
-                                     gamma, mean, rstd, sums, padded, N, F, xs, dys)) return e;
+    const StreamingPlan s = plan_streaming<T>(N, F);
+    auto stats = s.lanes == 2 ? (aligned ? k_layer_norm_grad_stats<T, 2, true> : k_layer_norm_grad_stats<T, 2, false>)
+                              : (aligned ? k_layer_norm_grad_stats<T, 8, true> : k_layer_norm_grad_stats<T, 8, false>);
+    if (const int e = launch_cluster(stats, s.cluster, s.ctas, kNormThreads, 0, st, x, dy, gamma, mean, rstd, sums, padded, N, F, xs, dys)) return e;
     launch(aligned ? k_layer_norm_grad_apply<T, kRows, true> : k_layer_norm_grad_apply<T, kRows, false>, dim3((unsigned)sweeps, (unsigned)bands), kNormThreads, 0, st, x, dy,
            dx, sums, padded, gamma, mean, rstd, grad_part, N, F, xs, dys, dxs);
     BB200_CUDA(cudaPeekAtLastError());
