@@ -400,7 +400,7 @@ int bbcu_bf16_LayerNormalization_Backward(const bbcu_bf16_t *dev_x_buf, const bb
 /* Operands of the int8 product: every frame (or row of W) as a row of 8-bit integers along the nodes with a scale of its own, scale = max|x| / 127 and
  * q = x / scale rounded to the nearest integer, ties to even, both in 32 bits.  A frame of zeros has scale 0; one that holds a NaN or an infinity
  * has scale NaN and zeros, so that its product is NaN.  q_node_stride in bytes, a multiple of 16; bytes up to the next multiple of 16 nodes are cleared.
- * dev_q_buf on a 16-byte boundary. */
+ * dev_q_buf on a 16-byte boundary.  Up to 2^22 nodes and 2^30 frames, BBCU_ERR_TOO_LARGE beyond. */
 int bbcu_fp32_QuantizeInt8_Frames(const float *dev_x_buf, signed char *dev_q_buf, float *dev_scale_buf, int node_size, int frame_size, int x_frame_stride,
                                   int q_node_stride, bbcu_stream_t stream);
 int bbcu_bf16_QuantizeInt8_Frames(const bbcu_bf16_t *dev_x_buf, signed char *dev_q_buf, float *dev_scale_buf, int node_size, int frame_size,
