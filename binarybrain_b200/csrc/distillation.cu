@@ -400,20 +400,47 @@ k_distill_once(const Distill<T> a, int rows, int tiles, int *fault)
 // earlier slot names it, too, and -1 where the slot is empty), log p, and the probabilities of its class added up.
 struct Slots { int *index; float *log_p, *p; };
 constexpr int kFinishCols = 8, kFinishGroups = kColumnThreads / kFinishCols;
+
+// Does a frame name a class twice?  Its slots mark a bit each of 2^slot_hash_bits(K), some 32 to 64 for a slot, and one that finds its bit marked looks
+// through all of them; only a frame where that finds a class twice adds up all of its slots by K searches.  (500 slots of 6000 classes x 3000 frames
+// bf16, with the searches for every frame: 343 us a call.)
+__host__ __device__ inline int slot_hash_bits(int K)
+{
+    int bits = 5;
+    while (bits < 14 && (1 << bits) < 32 * K) ++bits;
+    return bits;
+}
 template <typename T>
 __device__ __forceinline__ void teacher_slots(const Distill<T> &a, int cta, float *teacher, const Slots &slots, int columns)
 {
     extern __shared__ __align__(16) uint8_t buffer[];
     __shared__ float red[3][kColumnThreads / 32 * kFinishCols];
+    __shared__ int twice[kFinishCols];
     int *const index = reinterpret_cast<int *>(buffer);
     float *const log_p = reinterpret_cast<float *>(index + a.K * kFinishCols);
     const int col = threadIdx.x % kFinishCols, group = threadIdx.x / kFinishCols, f = cta * kFinishCols + col;
+    unsigned *const hit = reinterpret_cast<unsigned *>(log_p + a.K * kFinishCols);
+    const int hit_bits = slot_hash_bits(a.K);
+    for (int i = threadIdx.x; i < (kFinishCols << hit_bits) / 32; i += kColumnThreads) hit[i] = 0u;
+    if (threadIdx.x < kFinishCols) twice[threadIdx.x] = 0;
     const TeacherColumn c = teacher_columns<T, kFinishCols>(a, cta * kFinishCols, index, log_p, red);
     for (int k = group; k < a.K; k += kFinishGroups) {
         const int i = index[k * kFinishCols + col];
-        bool leads = false;
+        if (i < 0) continue;
+        const unsigned h = (unsigned)i * 2654435769u >> (32 - hit_bits), bit = 1u << (h & 31);
+        if (atomicOr(&hit[(h >> 5) * kFinishCols + col], bit) & bit) {
+            int named = 0;
+            for (int e = 0; e < a.K; ++e) named += index[e * kFinishCols + col] == i;
+            if (named > 1) twice[col] = 1;
+        }
+    }
+    __syncthreads();
+    const bool search = twice[col] != 0;
+    for (int k = group; k < a.K; k += kFinishGroups) {
+        const int i = index[k * kFinishCols + col];
+        bool leads = true;
         float q = 0.0f;
-        if (i >= 0) q = named_slots<kFinishCols>(index, log_p, a.K, k, col, leads);
+        if (i >= 0) q = search ? named_slots<kFinishCols>(index, log_p, a.K, k, col, leads) : expf(log_p[k * kFinishCols + col]);
         const long long at = (long long)k * columns + f;
         slots.index[at] = i < 0 || leads ? i : ~1 - i;
         slots.log_p[at] = log_p[k * kFinishCols + col];
@@ -426,13 +453,15 @@ __device__ __forceinline__ void teacher_slots(const Distill<T> &a, int cta, floa
 }
 
 // part[chunk of classes][column], by the CTAs behind the teacher's.  A thread's sum is relative to a logit not much below its largest one: it changes
-// only where one is 2^64 times as much, so that the rows cost little more than their exponentials.
+// only where one is 2^64 times as much, so that the rows cost little more than their exponentials.  Rows on 16-byte boundaries come through a ring in
+// shared memory, in which each thread has the rows that it will read itself: two batches are on their way while the exponentials of a third are taken.
+constexpr int kSumBatch = 4, kSumRing = 3, kSumSmem = kSumBatch * kSumRing * kColumnThreads * 16;
 template <typename T, int LPR, bool ALIGNED>
-__global__ void __launch_bounds__(kColumnThreads, 3)
+__global__ void __launch_bounds__(kColumnThreads, 4)
 k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, float *teacher, const Slots slots, int teacher_ctas)
 {
     grid_dependency();
-    constexpr int kBatch = 8;
+    extern __shared__ __align__(16) uint8_t buffer[];
     using Col = Column<T, LPR>;
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
     __shared__ SoftSum red[kColumnThreads / 32][kCols];
@@ -448,15 +477,42 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, flo
     SoftSum s[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) s[j] = {-INFINITY, 0.0f};
-    // some rows at a time: their largest logits first, then the exponentials
-    auto add = [&](auto count, int n) {
-        constexpr int B = decltype(count)::value;
-        uint4 raw[B], most;
+    constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;      // logits of -inf add nothing
+    const T *from = a.z + (long long)(n0 + c.row) * a.zs + f;
+    const long long z_step = step * a.zs;
+    uint8_t *const mine = buffer + threadIdx.x * 16;
+    const bool has = f < a.F;
+    auto fetch = [&](int slot, int n) {
 #pragma unroll
-        for (int i = 0; i < B; ++i) raw[i] = load_frames<T, ALIGNED>(a.z + (long long)(n + i * step) * a.zs, f, a.F);
+        for (int i = 0; i < kSumBatch; ++i, from += z_step)
+            if (has && n + i * step < n1) cp_async16(mine + (slot * kSumBatch + i) * (kColumnThreads * 16), from, true);
+        cp_async_commit();
+    };
+    int n = n0 + c.row, ahead = n, slot = 0, to = 0;
+    if constexpr (ALIGNED) {
+        for (; to < kSumRing - 1; ++to, ahead += kSumBatch * step) fetch(to, ahead);
+    }
+    for (; n < n1; n += kSumBatch * step) {
+        uint4 raw[kSumBatch], most;
+        if constexpr (ALIGNED) {
+            fetch(to, ahead);
+            ahead += kSumBatch * step;
+            to = to == kSumRing - 1 ? 0 : to + 1;
+            cp_async_wait<kSumRing - 1>();
+        }
+#pragma unroll
+        for (int i = 0; i < kSumBatch; ++i) {
+            raw[i] = make_uint4(kNone, kNone, kNone, kNone);
+            if (has && n + i * step < n1) {
+                if constexpr (ALIGNED) raw[i] = *reinterpret_cast<const uint4 *>(mine + (slot * kSumBatch + i) * (kColumnThreads * 16));
+                else raw[i] = load_frames<T, false>(a.z + (long long)(n + i * step) * a.zs, f, a.F);
+            }
+        }
+        slot = slot == kSumRing - 1 ? 0 : slot + 1;
+        // their largest logits first, then the exponentials
         most = raw[0];
 #pragma unroll
-        for (int i = 1; i < B; ++i) most = packed_max<T>(most, raw[i]);
+        for (int i = 1; i < kSumBatch; ++i) most = packed_max<T>(most, raw[i]);
         float top[kVec];
         unpack<T>(most, top);
         bool above = false;
@@ -474,16 +530,13 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, flo
 #pragma unroll
         for (int j = 0; j < kVec; ++j) top[j] = reference(s[j].top);
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
+        for (int i = 0; i < kSumBatch; ++i) {
             float v[kVec];
             unpack<T>(raw[i], v);
 #pragma unroll
             for (int j = 0; j < kVec; ++j) s[j].sum += exp2_fast((v[j] - top[j]) * a.scale);
         }
-    };
-    int n = n0 + c.row;
-    for (; n + (kBatch - 1) * step < n1; n += kBatch * step) add(std::integral_constant<int, kBatch>(), n);
-    for (; n < n1; n += step) add(std::integral_constant<int, 1>(), n);
+    }
 #pragma unroll
     for (int m = LPR; m < 32; m <<= 1)
 #pragma unroll
@@ -501,7 +554,8 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, flo
     }
 }
 
-// The numbers of FrameGrad as grad[4][columns], and the frames' losses
+// The numbers of FrameGrad but the slope as grad[3][columns], the frames' losses, and in the place of the named classes' probabilities their dz.  A thread's
+// first slots, and the logits that they name, are on their way before the sums are joined.
 template <typename T>
 __global__ void __launch_bounds__(kColumnThreads)
 k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunks, const float *__restrict__ teacher, const Slots slots, float *grad, int columns)
@@ -509,7 +563,27 @@ k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunk
     grid_dependency();
     __shared__ SoftSum sums[kColumnThreads / 32][kFinishCols];
     __shared__ float red[kColumnThreads / 32][kFinishCols], s_top[kFinishCols], s_log_sum[kFinishCols];
+    __shared__ FrameGrad s_grad[kFinishCols];
     const int col = threadIdx.x % kFinishCols, group = threadIdx.x / kFinishCols, warp = threadIdx.x / 32, f = (int)blockIdx.x * kFinishCols + col;
+    constexpr int kAhead = 2;
+    int code[kAhead];
+    float lp[kAhead], p_all[kAhead], z[kAhead];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+            const int k = k0 + e * kFinishGroups;
+            const long long at = (long long)k * columns + f;
+            code[e] = k < a.K ? slots.index[at] : -1;
+            lp[e] = k < a.K ? slots.log_p[at] : -INFINITY;
+            p_all[e] = k < a.K ? slots.p[at] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+            const int i = code[e] < -1 ? ~1 - code[e] : code[e];
+            z[e] = i >= 0 ? to_float(a.z[i * a.zs + f]) : 0.0f;
+        }
+    };
+    load(group);
     SoftSum s = {-INFINITY, 0.0f};
     for (int k = group; k < chunks; k += kFinishGroups) s = join_soft(s, part[(long long)k * columns + f], a.scale);
 #pragma unroll
@@ -520,15 +594,20 @@ k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunk
         for (int w = 1; w < kColumnThreads / 32; ++w) s = join_soft(s, sums[w][col], a.scale);
         s_top[col] = reference(s.top);
         s_log_sum[col] = s.sum == 0.0f ? 0.0f : logf(s.sum);
+        s_grad[col] = finish_frame(a, teacher[f], teacher[columns + f], s);
     }
     __syncthreads();
     const float top = s_top[col], log_sum = s_log_sum[col];
+    const FrameGrad g = s_grad[col];
     float divergence = 0.0f;
-    for (int k = group; k < a.K; k += kFinishGroups) {
-        const long long at = (long long)k * columns + f;
-        const int code = slots.index[at], i = code < -1 ? ~1 - code : code;
-        const float lp = slots.log_p[at], p = expf(lp);
-        if (i >= 0 && p != 0.0f) divergence += p * (lp - ((to_float(a.z[i * a.zs + f]) - top) * a.inv_t - log_sum));
+    for (int k = group; k < a.K; k += kAhead * kFinishGroups) {
+        if (k > group) load(k);
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+            const float p = expf(lp[e]);                                  // (0 of an empty slot, and beyond the last one)
+            if (p != 0.0f) divergence += p * (lp[e] - ((z[e] - top) * a.inv_t - log_sum));
+            if (code[e] >= 0) slots.p[(long long)(k + e * kFinishGroups) * columns + f] = soft_part(g, z[e], a.scale) - g.slope * p_all[e];
+        }
     }
     divergence = column_of_warp<kFinishCols>(divergence, [](float x, float y) { return x + y; });
     if (threadIdx.x % 32 < kFinishCols) red[warp][col] = divergence;
@@ -537,12 +616,10 @@ k_distill_finish(const Distill<T> a, const SoftSum *__restrict__ part, int chunk
         float loss = 0.0f;
         if (group == 0) {
             const float weight = teacher[columns + f];
-            const FrameGrad g = finish_frame(a, teacher[f], weight, s);
             if (weight != 0.0f) loss = weight * a.temperature * a.temperature * join_parts<ColumnSum>(&red[0][col], kFinishCols, kColumnThreads / 32);
             grad[f] = g.top;
             grad[columns + f] = g.factor;
             grad[2LL * columns + f] = g.cap;
-            grad[3LL * columns + f] = g.slope;
         }
         write_losses(a, (int)blockIdx.x, f, group == 0 && f < a.F, loss);
     }
@@ -581,15 +658,14 @@ k_distill_apply(const Distill<T> a, const float *__restrict__ grad, int columns)
 // the named classes, a frame and slot a thread
 template <typename T>
 __global__ void __launch_bounds__(kColumnThreads)
-k_distill_named(const Distill<T> a, const float *__restrict__ grad, const Slots slots, int columns)
+k_distill_named(const Distill<T> a, const Slots slots, int columns)
 {
     grid_dependency();
     const int f = (int)blockIdx.x * kColumnThreads + threadIdx.x, k = blockIdx.y;
     if (f >= a.F) return;
     const int i = slots.index[(long long)k * columns + f];
-    if (i < 0) return;
-    const FrameGrad g = {grad[f], grad[columns + f], grad[2LL * columns + f], grad[3LL * columns + f]};
-    a.dz[i * a.dzs + f] = from_float<T>(soft_part(g, to_float(a.z[i * a.zs + f]), a.scale) - g.slope * slots.p[(long long)k * columns + f]);
+    const float dz = slots.p[(long long)k * columns + f];
+    if (i >= 0) a.dz[i * a.dzs + f] = from_float<T>(dz);
 }
 
 __global__ void __launch_bounds__(1024) k_distill_loss(const double *__restrict__ part, int parts, double loss_reduction, float *loss)
@@ -649,19 +725,20 @@ static int distillation_passes(Distill<T> &a, int &loss_parts, bool aligned, cud
     const long long bands = ((long long)a.C + 8 * kDistillBand - 1) / (8 * kDistillBand);
     BB200_REQUIRE(bands <= 65535, BBCU_ERR_TOO_LARGE);
     auto sums = aligned ? k_distill_sums<T, LPR, true> : k_distill_sums<T, LPR, false>;
-    const int chunks = best_chunks(tiles, resident_clusters(reinterpret_cast<const void *>(sums), 1, kColumnThreads, 0), std::min(64, std::max(1, a.C / 256)));
+    const size_t sum_smem = std::max(aligned ? (size_t)kSumSmem : (size_t)0, (size_t)a.K * kFinishCols * 8 + ((size_t)kFinishCols << slot_hash_bits(a.K)) / 8);
+    BB200_REQUIRE(allow_big_smem(sums, (int)sum_smem), (int)cudaErrorInvalidValue);
+    const int chunks = best_chunks(tiles, resident_clusters(reinterpret_cast<const void *>(sums), 1, kColumnThreads, sum_smem), std::min(64, std::max(1, a.C / 256)));
     const int rows = (a.C + chunks - 1) / chunks;
     loss_parts = columns / kFinishCols;
     const size_t part_b = (size_t)chunks * columns * sizeof(SoftSum), loss_b = (size_t)loss_parts * sizeof(double), slots = (size_t)a.K * columns;
-    char *scratch = static_cast<char *>(stream_scratch(st, loss_b + part_b + ((size_t)6 * columns + 3 * slots) * 4, kFrameOpSlot));
+    char *scratch = static_cast<char *>(stream_scratch(st, loss_b + part_b + ((size_t)5 * columns + 3 * slots) * 4, kFrameOpSlot));
     BB200_REQUIRE(scratch != nullptr, BBCU_ERR_NO_MEMORY);
     a.loss_part = reinterpret_cast<double *>(scratch);
     SoftSum *part = reinterpret_cast<SoftSum *>(scratch + loss_b);
-    float *grad = reinterpret_cast<float *>(scratch + loss_b + part_b), *teacher = grad + (size_t)4 * columns, *slot_p = teacher + (size_t)2 * columns;
+    float *grad = reinterpret_cast<float *>(scratch + loss_b + part_b), *teacher = grad + (size_t)3 * columns, *slot_p = teacher + (size_t)2 * columns;
     const Slots kept = {reinterpret_cast<int *>(slot_p + 2 * slots), slot_p + slots, slot_p};
-    const size_t teacher_smem = (size_t)a.K * kFinishCols * 8;
     BB200_REQUIRE((long long)tiles * chunks + loss_parts < (1LL << 31), BBCU_ERR_TOO_LARGE);
-    launch(sums, (unsigned)(tiles * chunks + loss_parts), kColumnThreads, teacher_smem, st, a, part, rows, tiles, teacher, kept, loss_parts);
+    launch(sums, (unsigned)(tiles * chunks + loss_parts), kColumnThreads, sum_smem, st, a, part, rows, tiles, teacher, kept, loss_parts);
     BB200_CUDA(cudaPeekAtLastError());
     launch(k_distill_finish<T>, (unsigned)loss_parts, kColumnThreads, 0, st, a, part, chunks, teacher, kept, grad, columns);
     BB200_CUDA(cudaPeekAtLastError());
@@ -669,7 +746,7 @@ static int distillation_passes(Distill<T> &a, int &loss_parts, bool aligned, cud
            columns);
     BB200_CUDA(cudaPeekAtLastError());
     if (a.K > 0)
-        launch(k_distill_named<T>, dim3((unsigned)((a.F + kColumnThreads - 1) / kColumnThreads), (unsigned)a.K), kColumnThreads, 0, st, a, grad, kept, columns);
+        launch(k_distill_named<T>, dim3((unsigned)((a.F + kColumnThreads - 1) / kColumnThreads), (unsigned)a.K), kColumnThreads, 0, st, a, kept, columns);
     return launch_status();
 }
 
