@@ -452,7 +452,7 @@ __device__ __forceinline__ void teacher_slots(const Distill<T> &a, int cta, floa
     }
 }
 
-// part[chunk of classes][column], by the CTAs behind the teacher's.  A thread's sum is relative to a logit not much below its largest one: it changes
+// part[chunk of classes][column], by the CTAs before the teacher's.  A thread's sum is relative to a logit not much below its largest one: it changes
 // only where one is 2^64 times as much, so that the rows cost little more than their exponentials.  Rows on 16-byte boundaries come through a ring in
 // shared memory, in which each thread has the rows that it will read itself: two batches are on their way while the exponentials of a third are taken.
 constexpr int kSumBatch = 4, kSumRing = 3, kSumSmem = kSumBatch * kSumRing * kColumnThreads * 16;
@@ -466,12 +466,13 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, flo
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
     __shared__ SoftSum red[kColumnThreads / 32][kCols];
     const int columns = tiles * kCols;
-    if ((int)blockIdx.x < teacher_ctas) {
-        teacher_slots(a, (int)blockIdx.x, teacher, slots, columns);
+    const int cta = (int)blockIdx.x, first_teacher = (int)gridDim.x - teacher_ctas;
+    if (cta >= first_teacher) {
+        teacher_slots(a, cta - first_teacher, teacher, slots, columns);
         return;
     }
     const Col c;
-    const int cta = (int)blockIdx.x - teacher_ctas, tile = cta % tiles, chunk = cta / tiles;
+    const int tile = cta % tiles, chunk = cta / tiles;
     const int f = tile * kCols + c.col, step = c.step, n0 = chunk * chunk_rows, n1 = min(a.C, n0 + chunk_rows);
     const float most_above = 64.0f / a.scale;
     SoftSum s[kVec];
@@ -727,7 +728,8 @@ static int distillation_passes(Distill<T> &a, int &loss_parts, bool aligned, cud
     auto sums = aligned ? k_distill_sums<T, LPR, true> : k_distill_sums<T, LPR, false>;
     const size_t sum_smem = std::max(aligned ? (size_t)kSumSmem : (size_t)0, (size_t)a.K * kFinishCols * 8 + ((size_t)kFinishCols << slot_hash_bits(a.K)) / 8);
     BB200_REQUIRE(allow_big_smem(sums, (int)sum_smem), (int)cudaErrorInvalidValue);
-    const int chunks = best_chunks(tiles, resident_clusters(reinterpret_cast<const void *>(sums), 1, kColumnThreads, sum_smem), std::min(64, std::max(1, a.C / 256)));
+    // (chunks of 1024 rows at least, or 256 where there are few tiles: 8192 classes x 8192 frames bf16, 64 slots, 107 us by two chunks, 120 by nine)
+    const int chunks = best_chunks(tiles, resident_clusters(reinterpret_cast<const void *>(sums), 1, kColumnThreads, sum_smem), std::min(64, std::max(1, a.C / (tiles >= device_info().sm_count / 2 ? 1024 : 256))));
     const int rows = (a.C + chunks - 1) / chunks;
     loss_parts = columns / kFinishCols;
     const size_t part_b = (size_t)chunks * columns * sizeof(SoftSum), loss_b = (size_t)loss_parts * sizeof(double), slots = (size_t)a.K * columns;
