@@ -634,16 +634,17 @@ k_distill_apply(const Distill<T> a, const float *__restrict__ grad, int columns)
 {
     grid_dependency();
     constexpr int kVec = kFramesPerVec<T>;
-    const int f = ((int)blockIdx.x * 32 + (int)(threadIdx.x & 31)) * kVec, n0 = ((int)blockIdx.y * 8 + (int)(threadIdx.x >> 5)) * kDistillBand;
-    if (f >= a.F) return;
+    const Line<T, ALIGNED> line((int)blockIdx.x * 32 * kVec, (int)(threadIdx.x & 31), a.F);
+    const int n0 = ((int)blockIdx.y * 8 + (int)(threadIdx.x >> 5)) * kDistillBand;
+    if (line.empty()) return;
     uint4 raw[kDistillBand];
 #pragma unroll
     for (int i = 0; i < kDistillBand; ++i)
-        if (n0 + i < a.C) raw[i] = load_frames<T, ALIGNED>(a.z + (long long)(n0 + i) * a.zs, f, a.F);
-    float top[kVec], factor[kVec], cap[kVec];                             // (grad is padded to whole vectors)
-    load_columns(grad, f, columns, top);
-    load_columns(grad + columns, f, columns, factor);
-    load_columns(grad + 2LL * columns, f, columns, cap);
+        if (n0 + i < a.C) raw[i] = line.load(a.z + (long long)(n0 + i) * a.zs);
+    float top[kVec], factor[kVec], cap[kVec];
+    line.load_columns(grad, top);
+    line.load_columns(grad + columns, factor);
+    line.load_columns(grad + 2LL * columns, cap);
 #pragma unroll
     for (int i = 0; i < kDistillBand; ++i) {
         if (n0 + i < a.C) {
@@ -651,7 +652,7 @@ k_distill_apply(const Distill<T> a, const float *__restrict__ grad, int columns)
             unpack<T>(raw[i], v);
 #pragma unroll
             for (int j = 0; j < kVec; ++j) v[j] = soft_part({top[j], factor[j], cap[j], 0.0f}, v[j], a.scale);
-            store_frames<T, ALIGNED>(a.dz + (long long)(n0 + i) * a.dzs, f, a.F, v);
+            line.store(a.dz + (long long)(n0 + i) * a.dzs, v);
         }
     }
 }
