@@ -452,8 +452,10 @@ __device__ __forceinline__ void teacher_slots(const Distill<T> &a, int cta, floa
     }
 }
 
+template <typename T> constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;       // logits of -inf, which add nothing
+
 // part[chunk of classes][column], by the CTAs before the teacher's.  A thread's sum is relative to a logit not much below its largest one: it changes
-// only where one is 2^64 times as much, so that the rows cost little more than their exponentials.  Rows on 16-byte boundaries come through a ring in
+// only where one is 2^32 to 2^64 times as much, so that the rows cost little more than their exponentials.  Rows on 16-byte boundaries come through a ring in
 // shared memory, in which each thread has the rows that it will read itself: two batches are on their way while the exponentials of a third are taken.
 constexpr int kSumBatch = 4, kSumRing = 3, kSumSmem = kSumBatch * kSumRing * kColumnThreads * 16;
 template <typename T, int LPR, bool ALIGNED>
@@ -474,11 +476,11 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, flo
     const Col c;
     const int tile = cta % tiles, chunk = cta / tiles;
     const int f = tile * kCols + c.col, step = c.step, n0 = chunk * chunk_rows, n1 = min(a.C, n0 + chunk_rows);
-    const float most_above = 64.0f / a.scale;
-    SoftSum s[kVec];
+    const float most_above = 32.0f / a.scale;                             // (as a limit in T up to twice that: 2^64)
+    float ref[kVec], sum[kVec];                                           // a sum of 0: nothing above -inf yet
+    uint4 limit = make_uint4(kNone<T>, kNone<T>, kNone<T>, kNone<T>);     // what a logit has to exceed to become the reference, in T
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) s[j] = {-INFINITY, 0.0f};
-    constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;      // logits of -inf add nothing
+    for (int j = 0; j < kVec; ++j) ref[j] = sum[j] = 0.0f;
     const T *from = a.z + (long long)(n0 + c.row) * a.zs + f;
     const long long z_step = step * a.zs;
     uint8_t *const mine = buffer + threadIdx.x * 16;
@@ -501,12 +503,17 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, flo
             to = to == kSumRing - 1 ? 0 : to + 1;
             cp_async_wait<kSumRing - 1>();
         }
+        if (ALIGNED && has && n + (kSumBatch - 1) * step < n1) {
 #pragma unroll
-        for (int i = 0; i < kSumBatch; ++i) {
-            raw[i] = make_uint4(kNone, kNone, kNone, kNone);
-            if (has && n + i * step < n1) {
-                if constexpr (ALIGNED) raw[i] = *reinterpret_cast<const uint4 *>(mine + (slot * kSumBatch + i) * (kColumnThreads * 16));
-                else raw[i] = load_frames<T, false>(a.z + (long long)(n + i * step) * a.zs, f, a.F);
+            for (int i = 0; i < kSumBatch; ++i) raw[i] = *reinterpret_cast<const uint4 *>(mine + (slot * kSumBatch + i) * (kColumnThreads * 16));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kSumBatch; ++i) {
+                raw[i] = make_uint4(kNone<T>, kNone<T>, kNone<T>, kNone<T>);
+                if (has && n + i * step < n1) {
+                    if constexpr (ALIGNED) raw[i] = *reinterpret_cast<const uint4 *>(mine + (slot * kSumBatch + i) * (kColumnThreads * 16));
+                    else raw[i] = load_frames<T, false>(a.z + (long long)(n + i * step) * a.zs, f, a.F);
+                }
             }
         }
         slot = slot == kSumRing - 1 ? 0 : slot + 1;
@@ -514,30 +521,32 @@ k_distill_sums(const Distill<T> a, SoftSum *part, int chunk_rows, int tiles, flo
         most = raw[0];
 #pragma unroll
         for (int i = 1; i < kSumBatch; ++i) most = packed_max<T>(most, raw[i]);
-        float top[kVec];
-        unpack<T>(most, top);
-        bool above = false;
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) above |= top[j] > s[j].top + most_above;
-        if (above) {
+        const uint4 reach = packed_max<T>(most, limit);
+        if (reach.x != limit.x || reach.y != limit.y || reach.z != limit.z || reach.w != limit.w) {
+            float top[kVec], l[kVec];
+            unpack<T>(most, top);
 #pragma unroll
             for (int j = 0; j < kVec; ++j) {
-                if (top[j] > s[j].top) {
-                    if (s[j].top != -INFINITY) s[j].sum *= exp2_fast((s[j].top - top[j]) * a.scale);
-                    s[j].top = top[j];
+                const bool first = sum[j] == 0.0f;
+                if (first ? top[j] > -INFINITY : top[j] > ref[j]) {
+                    if (!first) sum[j] *= exp2_fast((ref[j] - top[j]) * a.scale);
+                    ref[j] = top[j];
                 }
+                l[j] = first && !(top[j] > -INFINITY) ? -INFINITY : ref[j] + most_above;
             }
+            limit = pack<T>(l);
         }
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) top[j] = reference(s[j].top);
 #pragma unroll
         for (int i = 0; i < kSumBatch; ++i) {
             float v[kVec];
             unpack<T>(raw[i], v);
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) s[j].sum += exp2_fast((v[j] - top[j]) * a.scale);
+            for (int j = 0; j < kVec; ++j) sum[j] += exp2_fast((v[j] - ref[j]) * a.scale);
         }
     }
+    SoftSum s[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) s[j] = {sum[j] == 0.0f ? -INFINITY : ref[j], sum[j]};
 #pragma unroll
     for (int m = LPR; m < 32; m <<= 1)
 #pragma unroll
