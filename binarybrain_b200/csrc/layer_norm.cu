@@ -24,9 +24,17 @@ constexpr int kNormThreads = 256;                      // of the kernels that st
 // ---- two passes: statistics of the frames, then what is made of them.  The second one finds what L2 (126 MB) still holds of the first.
 // (8192 x 16384 fp32: statistics 88 us, y 154; backward of 65536 x 1024 230 us with the sums of the weights, 134 of them and less for the second pass.)
 
-// A cluster has the columns of 128 (few frames: 32) bytes of a row; its CTAs take turns at the rows, add up d = x minus the column's first value (which takes a large
-// level out) and d^2, in 32 bits for each thread's rows and in 64 across the threads, so that neither a level nor a long column costs digits (64 bits in
-// the threads, too: 8192 x 16384 bf16 76 us instead of 60), and join them in the first CTA's shared memory.
+// rows first, first + step, ... below N
+__device__ __forceinline__ int n_rows(int N, int first, int step) { return first < N ? (N - first + step - 1) / step : 0; }
+
+// A cluster has the columns of 128 (few frames: 32) bytes of a row; its CTAs take turns at the rows.  Each thread adds up d = x - level and d^2 of its rows in 32
+// bits, with a level of its own: the middle one of its first three values, moved to the mean of all its rows so far after 1, 2, 4, 8, 16, 32, 48 ... batches, when d^2 goes
+// to a sum of its own.  A move subtracts (sum d)^2 / count, which after the first one is at most half of what the rows since the last one have added to sum d^2: neither a level of the
+// frame nor single nodes far from all others, wherever they are, cost digits (one level for all threads, the frame's first value, left rstd of 65536 nodes off
+// by 7e-4 where that value was 1000 standard deviations away).  Threads of a warp move to a level in common, and warps and CTAs join relative to the first value
+// in 64 bits.  A frame of one value has d = 0 at every step: its mean is that value and its variance 0.
+// (64 bits in the threads, too: 8192 x 16384 bf16 76 us instead of 60.)
+constexpr int kFoldBatches = 16;
 template <typename T, int LPR, bool ALIGNED>
 __global__ void __launch_bounds__(kNormThreads, 4)
 k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int N, int F, long long xs)
@@ -35,21 +43,41 @@ k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int 
     constexpr int kBatch = sizeof(T) == 4 ? 8 : 4;
     using Col = Column<T, LPR>;
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
-    __shared__ float2 red[8][kCols];
+    __shared__ float red[8][3][kCols];                                    // level, mean from there, sum of squares about the mean
+    __shared__ int red_rows[8];
     __shared__ double2 part[kCols];
     const Col c;
     const uint32_t cl = cluster_size(), rank = cluster_rank();
-    const int f0 = (int)(blockIdx.x / cl) * kCols, f = f0 + c.col, step = c.step * (int)cl;
-    float s1[kVec] = {}, s2[kVec] = {}, level[kVec];
-    unpack<T>(load_frames<T, ALIGNED>(x, f, F), level);
-    for (int n = (int)rank * c.step + c.row; n < N; n += step * kBatch) {
+    const int f0 = (int)(blockIdx.x / cl) * kCols, f = f0 + c.col, step = c.step * (int)cl, first = (int)rank * c.step + c.row;
+    float s1[kVec] = {}, s2[kVec] = {}, folded[kVec] = {}, level[kVec] = {};
+    for (int n = first, k = 0; n < N; n += step * kBatch, ++k) {
+        if (k > 0 && ((k & (k - 1)) == 0 || k % kFoldBatches == 0)) {
+            const float count = (float)(k * kBatch), inv = 1.0f / count;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                const float to = fmaf(s1[j], inv, level[j]), d = to - level[j], moved = count * d;
+                folded[j] += fmaf(d, moved - 2.0f * s1[j], s2[j]);
+                s1[j] -= moved;
+                s2[j] = 0.0f;
+                level[j] = to;
+            }
+        }
         uint4 raw[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             const int m = n + i * step;
             if (m < N) raw[i] = load_frames<T, ALIGNED>(x + (long long)m * xs, f, F);
         }
-        float b1[kVec] = {}, b2[kVec] = {};
+        if (k == 0) {
+            unpack<T>(raw[0], level);
+            if (n + 2 * step < N) {
+                float u[kVec], v[kVec];
+                unpack<T>(raw[1], u);
+                unpack<T>(raw[2], v);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) level[j] = fmaxf(fminf(level[j], u[j]), fminf(fmaxf(level[j], u[j]), v[j]));
+            }
+        }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             if (n + i * step < N) {
@@ -58,33 +86,55 @@ k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int 
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) {
                     const float d = v[j] - level[j];
-                    b1[j] += d;
-                    b2[j] = fmaf(d, d, b2[j]);
+                    s1[j] += d;
+                    s2[j] = fmaf(d, d, s2[j]);
                 }
             }
         }
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) { s1[j] += b1[j]; s2[j] += b2[j]; }
     }
+    // a warp's lanes of a column take the mean of their means for a level
+    const int rows = n_rows(N, first, step), warp_rows = __reduce_add_sync(0xffffffffu, rows) / LPR;
+    const float count = (float)rows, inv = rows ? 1.0f / count : 0.0f, inv_warp = warp_rows ? 1.0f / (float)warp_rows : 0.0f;
 #pragma unroll
-    for (int m = LPR; m < 32; m <<= 1)
+    for (int j = 0; j < kVec; ++j) {
+        const float mean = fmaf(s1[j], inv, level[j]), start = __shfl_sync(0xffffffffu, mean, c.lane % LPR);
+        float to = (mean - start) * (count * inv_warp);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
+        for (int m = LPR; m < 32; m <<= 1) to += __shfl_xor_sync(0xffffffffu, to, m);
+        to += start;
+        const float d = to - level[j], moved = count * d;
+        s2[j] = rows ? fmaf(d, moved - 2.0f * s1[j], folded[j] + s2[j]) : 0.0f;
+        s1[j] = rows ? s1[j] - moved : 0.0f;
+        level[j] = to;
+#pragma unroll
+        for (int m = LPR; m < 32; m <<= 1) {
             s1[j] += __shfl_xor_sync(0xffffffffu, s1[j], m);
             s2[j] += __shfl_xor_sync(0xffffffffu, s2[j], m);
         }
+    }
     if (c.lane < LPR) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) red[c.warp][c.col + j] = make_float2(s1[j], s2[j]);
+        for (int j = 0; j < kVec; ++j) {
+            const float off = s1[j] * inv_warp;
+            red[c.warp][0][c.col + j] = level[j];
+            red[c.warp][1][c.col + j] = off;
+            red[c.warp][2][c.col + j] = fmaf(-s1[j], off, s2[j]);
+        }
+        if (c.lane == 0) red_rows[c.warp] = warp_rows;
     }
     __syncthreads();
+    const bool has = threadIdx.x < kCols && f0 + (int)threadIdx.x < F;
+    const double start = has ? (double)to_float(x[f0 + threadIdx.x]) : 0.0;
     if (threadIdx.x < kCols) {
         double2 t = make_double2(0.0, 0.0);
-        for (int w = 0; w < c.warps; ++w) { t.x += (double)red[w][threadIdx.x].x; t.y += (double)red[w][threadIdx.x].y; }
+        for (int w = 0; w < c.warps; ++w) {
+            const double n = (double)red_rows[w], d = (double)red[w][0][threadIdx.x] - start + (double)red[w][1][threadIdx.x];
+            if (n > 0.0) { t.x += n * d; t.y += (double)red[w][2][threadIdx.x] + n * d * d; }
+        }
         part[threadIdx.x] = t;
     }
     if (cl > 1) { cluster_arrive(); cluster_wait(); }
-    if (rank == 0 && threadIdx.x < kCols && f0 + (int)threadIdx.x < F) {
+    if (rank == 0 && has) {
         double2 t = part[threadIdx.x];
         for (uint32_t r = 1; r < cl; ++r) {
             const double2 p = peer_load_double2(&part[threadIdx.x], r);
@@ -94,7 +144,7 @@ k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int 
         t.x /= (double)N;
         double var = t.y / (double)N - t.x * t.x;
         if (var < 0.0) var = 0.0;                                         // (and a NaN stays one)
-        mean_out[f0 + threadIdx.x] = (float)((double)to_float(x[f0 + threadIdx.x]) + t.x);
+        mean_out[f0 + threadIdx.x] = (float)(start + t.x);
         rstd_out[f0 + threadIdx.x] = 1.0f / sqrtf((float)var + eps);
     }
     if (cl > 1) { cluster_arrive(); cluster_wait(); }                     // nobody leaves while its sums may still be read

@@ -1,0 +1,69 @@
+"""The teacher's operators where their arithmetic is strained: nodes far from all others, levels, spreads near the ends of 32 bits, frames of one value.  As
+in test_teacher_operators.py, U is half a unit in the last place of 1.0 and the factors in front of it count roundings."""
+import numpy as np
+import pytest
+import torch
+
+from test_teacher_operators import BF, IDS, TYPES, U, buffer, normal
+
+
+def far_nodes(nodes, frames, dtype):
+    """Frames of N(0, 1) in which single nodes, the first ones among them, lie far from all others; a frame of each kind in turn."""
+    x = normal(nodes, nodes, frames)
+    for f in range(frames):
+        kind = f % 8
+        if kind < 3:
+            x[0, f] = (100.0, 1000.0, 30000.0)[kind]
+        elif kind == 3:
+            x[-1, f] = 30000.0
+        elif kind == 4:
+            x[nodes // 2, f] = -1000.0
+        elif kind == 5:
+            x[:16, f] = 1000.0
+        elif kind == 6:
+            x[::97, f] = 1e4
+        else:
+            x[:, f] += torch.arange(nodes) * 0.1
+    return x.to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("nodes,frames,layout", [(300, 19, "odd"), (300, 19, "rows"), (4096, 24, "rows"), (5000, 40, "rows"), (5000, 9600, "rows"), (8192, 70, "odd"), (16384, 200, "rows"),
+                                                 (65536, 9, "rows"), (65536, 9, "odd"), (1 << 20, 8, "rows")])
+def test_layer_norm_of_frames_with_far_nodes(nodes, frames, layout, dtype):
+    from binarybrain_b200 import ops
+    x = far_nodes(nodes, min(frames, 200), dtype)
+    x = x[:, torch.arange(frames) % x.shape[1]]
+    y, mean, rstd = ops.layer_norm_forward(buffer(x, dtype, layout), frames, eps=1e-5)
+    x = x.cuda().double()
+    mean_w = x.mean(0)
+    rstd_w = 1 / torch.sqrt((x - mean_w).square().mean(0) + 1e-5)
+    # A value may be in 16 partial sums of about its own size.  A thread adds up to 128 squares one after the other, then 8 such sums, and they are joined in
+    # 16 steps; half of that is left of it in a square root.  The mean's error counts by its square.
+    off = 16 * U * x.abs().mean(0)
+    rel = 80 * U + 2 * (off * rstd_w) ** 2
+    assert ((mean.double() - mean_w).abs() - off - U * mean_w.abs()).max() <= 0
+    assert ((rstd.double() - rstd_w).abs() / rstd_w - rel).max() <= 0
+    want = (x - mean_w) * rstd_w
+    tol = off * rstd_w + want.abs() * (rel + 2 * off * rstd_w) + 4 * U * want.abs()
+    if dtype == torch.bfloat16:
+        tol = tol + BF * (want.abs() + tol)
+    assert ((y[:, :frames].double() - want).abs() - tol).max() <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nodes,layout", [(300, "odd"), (9001, "rows"), (9001, "odd")])
+def test_layer_norm_of_broken_frames_beside_others(nodes, layout):
+    """A NaN or an infinity stays in its own frame, wherever it is, also where the rows are read twice."""
+    from binarybrain_b200 import ops
+    frames = 24
+    x = normal(1, nodes, frames).float()
+    for f, (n, v) in enumerate(((0, "nan"), (nodes - 1, "nan"), (0, "inf"), (7, "-inf"), (nodes - 1, "inf"), (nodes // 2, "-inf"))):
+        x[n, 2 * f] = float(v)
+    y, mean, rstd = ops.layer_norm_forward(buffer(x, torch.float32, layout), frames)
+    assert torch.isnan(y[:, 0:12:2]).all() and torch.isnan(rstd[0:12:2]).all()
+    keep = [1, 3, 5, 7, 9, *range(11, frames)]
+    want = x[:, keep].double()
+    want = (want - want.mean(0)) / torch.sqrt(want.var(0, unbiased=False) + 1e-5)
+    assert (y[:, keep].double().cpu() - want).abs().max() <= 64 * U * want.abs().max()
