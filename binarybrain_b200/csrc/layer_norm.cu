@@ -461,18 +461,18 @@ k_layer_norm_grad_once(const T *x, const T *dy, T *dx, const float *__restrict__
                 unpack<T>(*reinterpret_cast<const uint4 *>(p + half), gv);
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) {
-                    const float d = xv[j] - mean[j], t = gm * gv[j];
-                    ag[i] = fmaf(gv[j], d * rstd[j], ag[i]);
+                    const float xh = (xv[j] - mean[j]) * rstd[j], t = gm * gv[j];
+                    ag[i] = fmaf(gv[j], xh, ag[i]);
                     ab[i] += gv[j];
                     s[0][j] += t;
-                    s[1][j] = fmaf(t, d, s[1][j]);
+                    s[1][j] = fmaf(t, xh, s[1][j]);
                 }
             }
         }
         join_columns<ColumnSum, 2, T, LPR>(s, c, sums[turn & 1], cl, turn >> 1 & 1, [&](int, float v) { return v * inv; });
-        // dx = (gamma rstd) dy + k1 + k2 (x - mean)
+        // dx = rstd (gamma dy - c1 - (c2 rstd) (x - mean)): no power of rstd, which is 1e18 for spreads of 1e-18 and the reverse
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) { s[0][j] *= -rstd[j]; s[1][j] *= -rstd[j] * rstd[j] * rstd[j]; }
+        for (int j = 0; j < kVec; ++j) s[1][j] *= rstd[j];
         if (f < F) {
             const uint8_t *p = at;
             const float *g = gain + c.row;
@@ -485,7 +485,7 @@ k_layer_norm_grad_once(const T *x, const T *dy, T *dx, const float *__restrict__
                 unpack<T>(*reinterpret_cast<const uint4 *>(p), xv);
                 unpack<T>(*reinterpret_cast<const uint4 *>(p + half), gv);
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) gv[j] = fmaf(gv[j], gm * rstd[j], fmaf(xv[j] - mean[j], s[1][j], s[0][j]));
+                for (int j = 0; j < kVec; ++j) gv[j] = rstd[j] * fmaf(gv[j], gm, -fmaf(xv[j] - mean[j], s[1][j], s[0][j]));
                 store_frames<T, true>(out, f, F, gv);
             }
         }

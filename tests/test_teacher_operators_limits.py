@@ -67,3 +67,30 @@ def test_layer_norm_of_broken_frames_beside_others(nodes, layout):
     want = x[:, keep].double()
     want = (want - want.mean(0)) / torch.sqrt(want.var(0, unbiased=False) + 1e-5)
     assert (y[:, keep].double().cpu() - want).abs().max() <= 64 * U * want.abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("nodes,frames,layout", [(7, 5, "rows"), (300, 19, "rows"), (1000, 31, "rows"), (3000, 40, "rows"), (4096, 24, "rows"), (300, 19, "odd"), (9001, 16, "rows")])
+def test_layer_norm_of_small_and_of_large_spreads(nodes, frames, layout, dtype):
+    """Spreads at which rstd^3, and rstd^2 of the widest, is outside of 32 bits: the same digits as at 1, forward without eps and backward."""
+    from binarybrain_b200 import ops
+    from test_teacher_operators import norm_backward_64, norm_case, norm_forward_64
+    for scale in (2.0 ** -58, 2.0 ** -45, 2.0 ** 45, 2.0 ** 55):
+        x, gamma, beta = norm_case(nodes, frames, dtype, 0.5)
+        x = (x.double() * scale).to(dtype)
+        want, mean_w, rstd_w, tol, off, rel = norm_forward_64(x, gamma, beta, 0.0)
+        y, mean, rstd = ops.layer_norm_forward(buffer(x, dtype, layout), frames, gamma=gamma.cuda(), beta=beta.cuda(), eps=0.0)
+        if dtype == torch.bfloat16:
+            tol = tol + BF * (want.abs() + tol)
+        assert ((y[:, :frames].double().cpu() - want).abs() - tol).max() <= 0
+        assert ((mean.cpu().double() - mean_w).abs() - off - U * mean_w.abs()).max() <= 0
+        assert ((rstd.cpu().double() - rstd_w).abs() / rstd_w - rel).max() <= 0
+        dy = normal(9, nodes, frames).to(dtype)
+        mean, rstd = mean_w.float(), rstd_w.float()
+        (dx_w, dgamma_w, dbeta_w), tol = norm_backward_64(x, dy, mean, rstd, gamma)
+        dx, dgamma, dbeta = ops.layer_norm_backward(buffer(x, dtype, layout), buffer(dy, dtype, layout), mean.cuda(), rstd.cuda(), frames, gamma=gamma.cuda())
+        limit = tol[0] + (BF * (dx_w.abs() + tol[0]) if dtype == torch.bfloat16 else 0)
+        assert ((dx[:, :frames].double().cpu() - dx_w).abs() - limit).max() <= 0
+        assert ((dgamma.cpu().double() - dgamma_w).abs() - tol[1]).max() <= 0
+        assert ((dbeta.cpu().double() - dbeta_w).abs() - tol[2]).max() <= 0
