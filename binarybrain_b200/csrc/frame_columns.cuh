@@ -3,7 +3,7 @@
 //
 // Common layout of a CTA: LPR lanes of a warp stand side by side along the frames (8 lanes: 128 bytes, 2 lanes: 32 bytes of a row), the 32 / LPR
 // groups of a warp and the warps of the CTA one row below the other; a thread's further rows follow at a distance of all of them.  A cluster of
-// 1 to 8 CTAs shares the rows of one column tile, so that a tile is read once and held in registers between the statistics and what is made of
+// 1 to 8 CTAs shares the rows of one column tile, so that a tile is read once and held in shared memory between the statistics and what is made of
 // them; the column sums cross the warps through shared memory and the CTAs through distributed shared memory.
 #pragma once
 
@@ -258,20 +258,14 @@ template <typename OP> __device__ __forceinline__ float join_parts(const float *
     return s;
 }
 
-// Joins v[Q][kVec] over all rows of the tile (CTA, then cluster) by a fixed order of operations; what finish(q, joined) makes of a value comes back in
-// v for the thread's own columns.  One thread a value joins the parts, since there are many threads and few columns.  `phase`: of the exchange's barrier,
-// 0 and 1 in turn.
-template <typename OP, int Q, typename T, int LPR, typename FINISH>
-__device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], const Column<T, LPR> &c, Exchange<Q, LPR * kFramesPerVec<T>> &e, const Cluster &cl,
-                                             uint32_t phase, FINISH finish)
+// The way of v[Q][kVec] from the warps' lowest LPR lanes, which have their warp's columns, to what finish(q, joined) makes of a value over all rows of the tile,
+// which comes back in v for the thread's own columns.  join_warps(from, distance, count) joins the parts of a CTA's warps, join_ctas those of a cluster's CTAs; one
+// thread a value does so, since there are many threads and few columns.  `phase`: of the exchange's barrier, 0 and 1 in turn.
+template <int Q, typename T, int LPR, typename WARPS, typename CTAS, typename FINISH>
+__device__ __forceinline__ void exchange_columns(float (&v)[Q][kFramesPerVec<T>], const Column<T, LPR> &c, Exchange<Q, LPR * kFramesPerVec<T>> &e, const Cluster &cl,
+                                                 uint32_t phase, WARPS join_warps, CTAS join_ctas, FINISH finish)
 {
     constexpr int kVec = kFramesPerVec<T>, kCols = LPR * kVec;
-#pragma unroll
-    for (int m = LPR; m < 32; m <<= 1)
-#pragma unroll
-        for (int q = 0; q < Q; ++q)
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) v[q][j] = OP::join(v[q][j], __shfl_xor_sync(0xffffffffu, v[q][j], m));
     if (c.lane < LPR) {
 #pragma unroll
         for (int q = 0; q < Q; ++q)
@@ -281,7 +275,7 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
     if (cl.size > 1 && threadIdx.x == 0) mbar_arrive_expect_tx(&e.bar, cl.size * Q * kCols * (uint32_t)sizeof(float));
     __syncthreads();
     for (int i = threadIdx.x; i < Q * kCols; i += blockDim.x) {
-        const float s = join_parts<OP>(&e.red[0][i], Q * kCols, c.warps);
+        const float s = join_warps(&e.red[0][i], Q * kCols, c.warps);
         if (cl.size == 1) {
             e.out[i] = finish(i / kCols, s);
         } else {
@@ -296,9 +290,7 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
                 if (i == kWaitSpins - 1) { *(volatile int *)cl.gave_up = 1; ok = false; }
             }
         }
-        for (int i = threadIdx.x; i < Q * kCols; i += blockDim.x) {
-            e.out[i] = finish(i / kCols, join_parts<OP>(&e.part[0][i], Q * kCols, (int)cl.size));
-        }
+        for (int i = threadIdx.x; i < Q * kCols; i += blockDim.x) e.out[i] = finish(i / kCols, join_ctas(&e.part[0][i], Q * kCols, (int)cl.size));
     }
     __syncthreads();
 #pragma unroll
@@ -308,6 +300,20 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
             const float4 o = *reinterpret_cast<const float4 *>(&e.out[q * kCols + c.col + j]);
             v[q][j] = o.x; v[q][j + 1] = o.y; v[q][j + 2] = o.z; v[q][j + 3] = o.w;
         }
+}
+
+// Joins v[Q][kVec] of all threads over all rows of the tile by a fixed order of operations.
+template <typename OP, int Q, typename T, int LPR, typename FINISH>
+__device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], const Column<T, LPR> &c, Exchange<Q, LPR * kFramesPerVec<T>> &e, const Cluster &cl,
+                                             uint32_t phase, FINISH finish)
+{
+#pragma unroll
+    for (int m = LPR; m < 32; m <<= 1)
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int j = 0; j < kFramesPerVec<T>; ++j) v[q][j] = OP::join(v[q][j], __shfl_xor_sync(0xffffffffu, v[q][j], m));
+    exchange_columns<Q, T, LPR>(v, c, e, cl, phase, join_parts<OP>, join_parts<OP>, finish);
 }
 
 // How a kernel that streams over N rows is cut: `lanes` lanes along a row, 8 or, where those would leave most SMs without a cluster, 2; clusters that share

@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "frame_columns.cuh"
+#include "packed_pairs.cuh"
 
 namespace bb200 {
 
@@ -23,6 +24,8 @@ constexpr int kNormThreads = 256;                      // of the kernels that st
 
 // ---- two passes: statistics of the frames, then what is made of them.  The second one finds what L2 (126 MB) still holds of the first.
 // (8192 x 16384 fp32: statistics 88 us, y 154; backward of 65536 x 1024 230 us with the sums of the weights, 134 of them and less for the second pass.)
+
+__device__ __forceinline__ float middle(float a, float b, float c) { return fmaxf(fminf(a, b), fminf(fmaxf(a, b), c)); }
 
 // rows first, first + step, ... below N
 __device__ __forceinline__ int n_rows(int N, int first, int step) { return first < N ? (N - first + step - 1) / step : 0; }
@@ -75,7 +78,7 @@ k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int 
                 unpack<T>(raw[1], u);
                 unpack<T>(raw[2], v);
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) level[j] = fmaxf(fminf(level[j], u[j]), fminf(fmaxf(level[j], u[j]), v[j]));
+                for (int j = 0; j < kVec; ++j) level[j] = middle(level[j], u[j], v[j]);
             }
         }
 #pragma unroll
@@ -329,6 +332,51 @@ __device__ __forceinline__ void fetch_rows(uint8_t *to, int piece, const T *from
     for (int i = 0; i < rows; ++i, to += piece, from += distance) cp_async16(to, from, true);
 }
 
+// Means of rows joined to their mean with weights that are the shares of the rows, each part as its distance from the first one: means that are equal stay
+// what they are, so that a frame of one value has that value for a mean and nothing but zeros about it.
+template <typename T, int LPR> struct MeanWeights {
+    float mine, lane;                                                     // 1 / rows of the thread; their share of the warp's
+    float (&shared)[2][8];                                                // the shares of the CTA's warps and of the cluster's CTAs
+
+    // rows: of this thread, cta_rows: of a CTA at most; a barrier stands between this and the first use
+    __device__ __forceinline__ MeanWeights(const Column<T, LPR> &c, const Cluster &cl, float (&shared)[2][8], int rows, int cta_rows, int N) : shared(shared)
+    {
+        const int count = max(rows, 0), warp = __reduce_add_sync(0xffffffffu, count) / LPR;
+        auto of_cta = [&](uint32_t r) { return (float)min(max(N - (int)r * cta_rows, 0), cta_rows); };
+        mine = count ? __fdividef(1.0f, (float)count) : 0.0f;
+        lane = count ? __fdividef((float)count, (float)warp) : 0.0f;
+        if (c.lane == 0) shared[0][c.warp] = warp ? __fdividef((float)warp, of_cta(cl.rank)) : 0.0f;
+        if (threadIdx.x < cl.size) shared[1][threadIdx.x] = __fdividef(of_cta(threadIdx.x), (float)N);
+    }
+    template <int WHAT> __device__ __forceinline__ float join_parts(const float *from, int distance, int count) const      // up to eight, all of them on their way first
+    {
+        const float4 lower = *reinterpret_cast<const float4 *>(shared[WHAT]), upper = *reinterpret_cast<const float4 *>(shared[WHAT] + 4);
+        const float w[8] = {lower.x, lower.y, lower.z, lower.w, upper.x, upper.y, upper.z, upper.w};
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < count ? from[i * distance] : 0.0f;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 1; i < 8; ++i)
+            if (i < count) s = fmaf(v[i] - v[0], w[i], s);
+        return v[0] + s;
+    }
+    // v: of this thread's rows, then of all rows of the tile
+    __device__ __forceinline__ void join(float (&v)[1][kFramesPerVec<T>], const Column<T, LPR> &c, Exchange<1, LPR * kFramesPerVec<T>> &e, const Cluster &cl, uint32_t phase) const
+    {
+#pragma unroll
+        for (int j = 0; j < kFramesPerVec<T>; ++j) {
+            const float start = __shfl_sync(0xffffffffu, v[0][j], c.lane % LPR);
+            float off = (v[0][j] - start) * lane;
+#pragma unroll
+            for (int m = LPR; m < 32; m <<= 1) off += __shfl_xor_sync(0xffffffffu, off, m);
+            v[0][j] = start + off;
+        }
+        exchange_columns<1, T, LPR>(v, c, e, cl, phase, [&](const float *from, int distance, int count) { return join_parts<0>(from, distance, count); },
+                                    [&](const float *from, int distance, int count) { return join_parts<1>(from, distance, count); }, [](int, float m) { return m; });
+    }
+};
+
 template <typename T, int LPR>
 __global__ void __launch_bounds__(kColumnThreads, 4)
 k_layer_norm_once(const T *x, T *y, const float *__restrict__ gamma, const float *__restrict__ beta, float *mean_out, float *rstd_out, float eps, int N, int F,
@@ -339,6 +387,7 @@ k_layer_norm_once(const T *x, T *y, const float *__restrict__ gamma, const float
     constexpr int kVec = Col::kVec, kCols = Col::kCols;
     extern __shared__ __align__(16) uint8_t buffer[];
     __shared__ Exchange<1, kCols> sums[2];
+    __shared__ __align__(16) float shares[2][8];
     __shared__ int gave_up;
     const Col c;
     Cluster cl(&gave_up);
@@ -351,25 +400,38 @@ k_layer_norm_once(const T *x, T *y, const float *__restrict__ gamma, const float
     int tile = (int)(blockIdx.x / cl.size), f = tile * kCols + c.col;
     uint32_t phase = 0;
     if (f < F) fetch_rows(buffer, piece, x_first + f, x_step, mine);
-    for (int i = threadIdx.x; i < c.step * rows; i += blockDim.x)
-        gain[i] = cta_first + i < N ? make_float2(gamma ? gamma[cta_first + i] : 1.0f, beta ? beta[cta_first + i] : 0.0f) : make_float2(0.0f, 0.0f);
+    auto gain_at = [&](int i) { return cta_first + i < N ? make_float2(gamma ? gamma[cta_first + i] : 1.0f, beta ? beta[cta_first + i] : 0.0f) : make_float2(0.0f, 0.0f); };
+    const float2 first_gain = gain_at(threadIdx.x);                       // on its way beside the shares of the rows
+    const MeanWeights<T, LPR> weights(c, cl, shares, mine, c.step * rows, N);
+    if ((int)threadIdx.x < c.step * rows) gain[threadIdx.x] = first_gain;
+    for (int i = threadIdx.x + blockDim.x; i < c.step * rows; i += blockDim.x) gain[i] = gain_at(i);
     cl.meet(sums, gain + c.step * rows);
     const float inv = 1.0f / (float)N;
     for (; tile < tiles; tile += clusters, f += clusters * kCols, phase ^= 1) {
         cp_async_commit();
         cp_async_wait<0>();
         float mean[1][kVec] = {}, rstd[1][kVec] = {};
-        {
+        if (mine > 0) {                                                   // about one of the first two values, the smaller one: far nodes stay out of it
+            float level[kVec], v[kVec];
+            unpack<T>(*reinterpret_cast<const uint4 *>(at), level);
+            unpack<T>(*reinterpret_cast<const uint4 *>(at + (mine > 1 ? piece : 0)), v);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) level[j] = fabsf(v[j]) < fabsf(level[j]) ? v[j] : level[j];
+            f32x2 sum[kVec / 2], from[kVec / 2];
+#pragma unroll
+            for (int j = 0; j < kVec / 2; ++j) { sum[j] = pack2(0.0f, 0.0f); from[j] = pack2(level[2 * j], level[2 * j + 1]); }
             const uint8_t *p = at;
-#pragma unroll 4
+#pragma unroll 2
             for (int i = 0; i < mine; ++i, p += piece) {
                 float v[kVec];
                 unpack<T>(*reinterpret_cast<const uint4 *>(p), v);
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) mean[0][j] += v[j];
+                for (int j = 0; j < kVec / 2; ++j) sum[j] = add2(sum[j], sub2(pack2(v[2 * j], v[2 * j + 1]), from[j]));
             }
+#pragma unroll
+            for (int j = 0; j < kVec / 2; ++j) unpack2(fma2(sum[j], pack2(weights.mine, weights.mine), from[j]), mean[0][2 * j], mean[0][2 * j + 1]);
         }
-        join_columns<ColumnSum, 1, T, LPR>(mean, c, sums[0], cl, phase, [&](int, float s) { return s * inv; });
+        weights.join(mean, c, sums[0], cl, phase);
         {
             const uint8_t *p = at;
 #pragma unroll 4

@@ -94,3 +94,20 @@ def test_layer_norm_of_small_and_of_large_spreads(nodes, frames, layout, dtype):
         assert ((dx[:, :frames].double().cpu() - dx_w).abs() - limit).max() <= 0
         assert ((dgamma.cpu().double() - dgamma_w).abs() - tol[1]).max() <= 0
         assert ((dbeta.cpu().double() - dbeta_w).abs() - tol[2]).max() <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("layout", ["rows", "odd"])
+@pytest.mark.parametrize("nodes", [1, 2, 3, 5, 15, 30, 60, 61, 100, 255, 300, 333, 500, 777, 1001, 1500, 2047, 2999, 3333, 4000, 4096, 4097, 5001, 9001, 20011, 70001])
+def test_layer_norm_of_frames_of_one_value(nodes, layout, dtype):
+    """No deviation, at any level and size: mean = the value, rstd = 1 / sqrt(eps), y = beta, each in every bit."""
+    from binarybrain_b200 import ops
+    levels = torch.tensor([2.5, 0.1, 1000.1, -7.7, 1e-30, -3e38, 12345.678, 0.0, 1 / 3, 6e4, -1e-3]).to(dtype)
+    x = levels.expand(nodes, -1).clone()
+    beta = normal(1, nodes).float().to(dtype).float()
+    for eps in (1e-5, 1e-12):
+        y, mean, rstd = ops.layer_norm_forward(buffer(x, dtype, layout), len(levels), beta=beta.cuda(), eps=eps)
+        assert torch.equal(mean.cpu(), levels.float())
+        assert (rstd.cpu().numpy() == np.float32(1) / np.sqrt(np.float32(eps))).all()
+        assert torch.equal(y[:, :len(levels)].float().cpu(), beta[:, None].expand(-1, len(levels)))
