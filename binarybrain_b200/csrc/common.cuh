@@ -32,9 +32,8 @@ const DeviceInfo &device_info();
 // makes back-to-back calls on one stream safe; different streams get different blocks.  A stream has
 // kScratchSlots independent blocks, for callers whose scratch is alive at the same time (slot 0: batch-norm
 // sums, slot 1: per-node coefficient / pattern tables of the LUT operators, slot 2: the piece table of the bit Im2Col,
-// slot 3: fp32 rows packed to bits, slot 4: the counters below, slot 5: partial sums of the operators over the nodes of a frame).
-constexpr int kScratchSlots = 6;
-constexpr int kFrameOpSlot = 5;
+// slot 3: fp32 rows packed to bits, slot 4: the counters below).
+constexpr int kScratchSlots = 5;
 void *stream_scratch(cudaStream_t stream, size_t bytes, int slot = 0);
 
 // A number that is another one after every request for the stream's block (0: it has none).  A caller that leaves something in the block for
@@ -45,6 +44,22 @@ unsigned long long stream_scratch_ticket(cudaStream_t stream, int slot);
 // for the per-thread default stream, whose one handle stands for a stream of every thread, and for a stream that is being captured: the
 // graph may be launched on any stream, beside kernels of this one, and the zeroing would only be a node of the graph.
 unsigned *stream_counters(cudaStream_t stream);
+
+// Scratch of an operator that is a chain of kernels (those over the nodes of a frame), a block of the stream that the operator has to itself from get() until
+// this object goes: another host thread that calls on the same stream waits for its turn, so that the kernels of two chains do not alternate on one block.
+// The per-thread default stream has a block a thread.  A call that is captured gets a block of the capture's own, which belongs to the graph and what is
+// instantiated from it, and comes back to the heap when the last of them is destroyed: neither calls outside, nor a replay on another stream, touch it.
+class HeldScratch {
+public:
+    HeldScratch() = default;
+    ~HeldScratch();
+    HeldScratch(const HeldScratch &) = delete;
+    HeldScratch &operator=(const HeldScratch &) = delete;
+    void *get(cudaStream_t stream, size_t bytes);        // once; nullptr: no memory
+
+private:
+    struct HeldBlock *block_ = nullptr;
+};
 
 // Pass 1 of the DifferentiableLut6 training forward (raw LUT values into y, fp64 sums per node); with may_allocate = false
 // it takes nothing from the heap or the stream scratch.

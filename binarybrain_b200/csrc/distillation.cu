@@ -729,7 +729,7 @@ static int best_chunks(long long tiles, long long resident, int most)
 }
 
 template <typename T, int LPR>
-static int distillation_passes(Distill<T> &a, int &loss_parts, bool aligned, cudaStream_t st)
+static int distillation_passes(Distill<T> &a, int &loss_parts, bool aligned, HeldScratch &held, cudaStream_t st)
 {
     constexpr int kCols = Column<T, LPR>::kCols, kWide = 32 * kFramesPerVec<T>;
     const int tiles = (a.F + kCols - 1) / kCols, columns = tiles * kCols;
@@ -743,7 +743,7 @@ static int distillation_passes(Distill<T> &a, int &loss_parts, bool aligned, cud
     const int rows = (a.C + chunks - 1) / chunks;
     loss_parts = columns / kFinishCols;
     const size_t part_b = (size_t)chunks * columns * sizeof(SoftSum), loss_b = (size_t)loss_parts * sizeof(double), slots = (size_t)a.K * columns;
-    char *scratch = static_cast<char *>(stream_scratch(st, loss_b + part_b + ((size_t)5 * columns + 3 * slots) * 4, kFrameOpSlot));
+    char *scratch = static_cast<char *>(held.get(st, loss_b + part_b + ((size_t)5 * columns + 3 * slots) * 4));
     BB200_REQUIRE(scratch != nullptr, BBCU_ERR_NO_MEMORY);
     a.loss_part = reinterpret_cast<double *>(scratch);
     SoftSum *part = reinterpret_cast<SoftSum *>(scratch + loss_b);
@@ -778,15 +778,16 @@ static int distillation(Distill<T> a, float *loss, double loss_reduction, cudaSt
             while (p.warps > 2 && cta_rows <= per_warp * (p.warps / 2) * kDistillRows / 2) p.warps /= 2;
         p.rows = (cta_rows + per_warp * p.warps - 1) / (per_warp * p.warps);
     }
+    HeldScratch held;                                                     // until the loss is on its way
     int parts = 0, e;
     if (p.cluster) {
         const int cols = p.lanes * kFramesPerVec<T>;
         parts = (a.F + cols - 1) / cols;
-        a.loss_part = static_cast<double *>(stream_scratch(st, (size_t)parts * sizeof(double), kFrameOpSlot));
+        a.loss_part = static_cast<double *>(held.get(st, (size_t)parts * sizeof(double)));
         BB200_REQUIRE(a.loss_part != nullptr, BBCU_ERR_NO_MEMORY);
         e = p.lanes == 2 ? distillation_once<T, 2>(a, p, parts, st) : distillation_once<T, kLanes>(a, p, parts, st);
     } else {
-        e = distillation_passes<T, sizeof(T) == 4 ? 8 : 4>(a, parts, aligned, st);
+        e = distillation_passes<T, sizeof(T) == 4 ? 8 : 4>(a, parts, aligned, held, st);
     }
     if (e != BBCU_OK) return e;
     launch(k_distill_loss, 1, 1024, 0, st, a.loss_part, parts, loss_reduction, loss);

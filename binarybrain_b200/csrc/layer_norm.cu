@@ -635,7 +635,8 @@ static int layer_norm_grad_once(const T *x, const T *dy, T *dx, const float *gam
               exchange_bytes<2, kCols>(p.cluster), tiles = (F + kCols - 1) / kCols;
     BB200_REQUIRE(allow_big_smem(kernel, kNormSmem), (int)cudaErrorInvalidValue);
     const int clusters = std::min(tiles, resident_clusters(reinterpret_cast<const void *>(kernel), p.cluster, threads, smem));
-    float2 *part = static_cast<float2 *>(stream_scratch(st, (size_t)clusters * N * sizeof(float2), kFrameOpSlot));
+    HeldScratch held;
+    float2 *part = static_cast<float2 *>(held.get(st, (size_t)clusters * N * sizeof(float2)));
     BB200_REQUIRE(part != nullptr, BBCU_ERR_NO_MEMORY);
     const int e = launch_cluster(kernel, (unsigned)p.cluster, (unsigned)(clusters * p.cluster), threads, smem, st, x, dy, dx, gamma, mean, rstd, part, N, F, xs, dys,
                                  dxs, p.rows, tiles, fault);
@@ -685,7 +686,8 @@ static int layer_norm_backward(const T *x, const T *dy, T *dx, const float *gamm
     long long sweeps = std::min(pieces, std::max(1LL, (8LL * device_info().sm_count + bands - 1) / bands));
     const int padded = (F + 3) / 4 * 4;
     const size_t sums_bytes = (size_t)padded * sizeof(float2);
-    char *scratch = static_cast<char *>(stream_scratch(st, sums_bytes + (size_t)sweeps * N * sizeof(float2), kFrameOpSlot));
+    HeldScratch held;
+    char *scratch = static_cast<char *>(held.get(st, sums_bytes + (size_t)sweeps * N * sizeof(float2)));
     BB200_REQUIRE(scratch != nullptr, BBCU_ERR_NO_MEMORY);
     float *sums = reinterpret_cast<float *>(scratch);
     float2 *grad_part = reinterpret_cast<float2 *>(scratch + sums_bytes);

@@ -13,6 +13,7 @@
 //     keeps the 256-byte alignment cudaMalloc gives.
 #include <atomic>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <tuple>
 #include <unordered_map>
@@ -23,7 +24,15 @@
 
 namespace bb200 {
 
+struct HeldBlock {
+    std::mutex busy;                                  // an operator has the block
+    void *ptr = nullptr;
+    size_t bytes = 0;
+};
+
 namespace {
+
+using HeldKey = std::tuple<cudaStream_t, unsigned long long, unsigned long long>;      // stream, its number where one handle stands for several, capture or 0
 
 struct Pool {
     std::mutex mu;
@@ -33,6 +42,7 @@ struct Pool {
     struct Scratch { void *ptr; size_t bytes; unsigned long long ticket; };
     std::map<std::pair<cudaStream_t, int>, Scratch> scratch;                       // (stream, slot) -> block
     unsigned long long tickets = 0;                                                // requests for scratch blocks so far
+    std::map<HeldKey, std::unique_ptr<HeldBlock>> held;                            // those without a capture stay for good
 };
 
 std::mutex g_pools_mu;
@@ -230,6 +240,108 @@ unsigned *stream_counters(cudaStream_t stream)
     return static_cast<unsigned *>(stream_scratch(stream, 256, kCounterSlot));
 }
 
+// Blocks whose graph is gone.  CUDA says so on a thread of its own that may not call CUDA or wait for who does, so that they are noted here, and taken
+// back by the next request.
+struct Retired { Pool *pool; HeldKey key; void *ptr; };
+static std::mutex g_retired_mu;
+static std::vector<Retired *> &g_retired = *new std::vector<Retired *>;
+static std::atomic<bool> g_any_retired{false};
+
+static void CUDART_CB retire(void *block)
+{
+    try {
+        std::lock_guard<std::mutex> g(g_retired_mu);
+        g_retired.push_back(static_cast<Retired *>(block));
+        g_any_retired.store(true, std::memory_order_release);
+    } catch (...) {                                                       // no host memory: the block stays where it is
+    }
+}
+
+static void take_back_retired()
+{
+    if (!g_any_retired.load(std::memory_order_acquire)) return;
+    std::vector<Retired *> list;
+    {
+        std::lock_guard<std::mutex> g(g_retired_mu);
+        list.swap(g_retired);
+        g_any_retired.store(false, std::memory_order_release);
+    }
+    for (Retired *r : list) {
+        std::lock_guard<std::mutex> g(r->pool->mu);
+        auto held = r->pool->held.find(r->key);
+        if (held != r->pool->held.end() && held->second->ptr == r->ptr) r->pool->held.erase(held);
+        auto it = r->pool->live.find(r->ptr);
+        if (it != r->pool->live.end()) {
+            r->pool->live_bytes -= it->second;
+            r->pool->cached_bytes += it->second;
+            r->pool->cached.emplace(it->second, r->ptr);
+            r->pool->live.erase(it);
+        }
+        delete r;
+    }
+}
+
+HeldScratch::~HeldScratch()
+{
+    if (block_) block_->busy.unlock();
+}
+
+void *HeldScratch::get(cudaStream_t stream, size_t bytes)
+{
+    try {
+        take_back_retired();
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        unsigned long long capture = 0, number = 0;
+        cudaGraph_t graph = nullptr;
+        if (cudaStreamGetCaptureInfo_v2(stream, &status, &capture, &graph) != cudaSuccess) { cudaGetLastError(); status = cudaStreamCaptureStatusNone; }
+        if (status != cudaStreamCaptureStatusActive) capture = 0;
+        if (stream == cudaStreamPerThread && cudaStreamGetId(stream, &number) != cudaSuccess) { cudaGetLastError(); return nullptr; }
+        const HeldKey key(stream, number, capture);
+        Pool &p = pool_of_current_device();
+        HeldBlock *block;
+        {
+            std::lock_guard<std::mutex> g(p.mu);
+            std::unique_ptr<HeldBlock> &entry = p.held[key];
+            if (!entry) entry.reset(new HeldBlock);
+            block = entry.get();
+        }
+        block->busy.lock();
+        block_ = block;
+        if (block->ptr && block->bytes >= bytes) return block->ptr;
+        std::unique_ptr<Retired> owned(capture ? new Retired{&p, key, nullptr} : nullptr);
+        // a capture forbids allocations unless the thread says that it knows of none that the graph depends on
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if (capture && cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) { cudaGetLastError(); return nullptr; }
+        void *fresh = bbcu_LocalHeap_Malloc(bytes ? bytes : 256);
+        if (capture && cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) cudaGetLastError();
+        if (!fresh) return nullptr;
+        if (capture) {
+            cudaUserObject_t object = nullptr;
+            owned->ptr = fresh;
+            if (cudaUserObjectCreate(&object, owned.get(), retire, 1, cudaUserObjectNoDestructorSync) != cudaSuccess) {
+                cudaGetLastError();
+                bbcu_LocalHeap_Free(fresh);
+                return nullptr;
+            }
+            owned.release();                                              // retire() has it now
+            if (cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+                cudaGetLastError();
+                cudaUserObjectRelease(object, 1);
+                return nullptr;
+            }
+        } else if (block->ptr) {
+            // (an outgrown block that work may still be enqueued on is better lost than given away)
+            if (cudaStreamSynchronize(stream) == cudaSuccess) bbcu_LocalHeap_Free(block->ptr);
+            else cudaGetLastError();
+        }
+        block->ptr = fresh;
+        block->bytes = bytes;
+        return fresh;
+    } catch (...) {                                                       // no host memory
+        return nullptr;
+    }
+}
+
 }   // namespace bb200
 
 using namespace bb200;
@@ -399,10 +511,20 @@ extern "C" void bbcu_LocalHeap_GarbageCollect(void)
 {
     Pool &p = pool_of_current_device();
     std::vector<void *> scratch;
+    std::vector<HeldBlock *> held;
+    take_back_retired();
     {
         std::lock_guard<std::mutex> g(p.mu);
         for (auto &kv : p.scratch) scratch.push_back(kv.second.ptr);
         p.scratch.clear();
+        for (auto &kv : p.held)
+            if (std::get<2>(kv.first) == 0) held.push_back(kv.second.get());
+    }
+    for (HeldBlock *b : held) {                                           // (what a graph has stays the graph's)
+        std::lock_guard<std::mutex> g(b->busy);
+        if (b->ptr) scratch.push_back(b->ptr);
+        b->ptr = nullptr;
+        b->bytes = 0;
     }
     if (!scratch.empty()) cudaDeviceSynchronize();
     for (void *s : scratch) bbcu_LocalHeap_Free(s);

@@ -377,7 +377,10 @@ int bbcu_fp32_DifferentiableLut6_ForwardTraining_NoAlloc_MaxNodes(void);
  * No counterparts in the reference.  Frame buffers are node-major as above, fp32 or bf16 (bbcu_bf16_*: two bytes an element, strides in elements);
  * any stride and alignment of theirs is taken, rows on 16-byte boundaries are the fast ones, and outputs are written up to the last frame, never
  * into a row's padding.  Outputs do not overlap inputs.  Sums and statistics are 32 bits or more; bf16 results are rounded once.  A batch without
- * frames is no error.  Layer norm and distillation take up to 2^20 nodes or classes and 2^30 frames, BBCU_ERR_TOO_LARGE beyond.  Scratch as for the LUT operators above: the first call of a size on a stream allocates. */
+ * frames is no error.  Layer norm and distillation take up to 2^20 nodes or classes and 2^30 frames, BBCU_ERR_TOO_LARGE beyond.
+ * Scratch: a block per stream, or per thread for the per-thread default stream; the first call of a size allocates, bbcu_LocalHeap_GarbageCollect
+ * releases.  Host threads may call on one stream at the same time.  Calls that are captured need no call before them: their block is the graph's own,
+ * lives as long as the graph and what is instantiated from it, and is shared by the captured calls of one stream. */
 
 /* Layer norm over the nodes of a frame: y = (x - mean) * rstd * gamma + beta, mean and rstd = 1 / sqrt(variance + eps) [frame_size], which the
  * backward takes.  dev_gamma / dev_beta [node_size], NULL: 1 / 0. */
