@@ -111,3 +111,25 @@ def test_layer_norm_of_frames_of_one_value(nodes, layout, dtype):
         assert torch.equal(mean.cpu(), levels.float())
         assert (rstd.cpu().numpy() == np.float32(1) / np.sqrt(np.float32(eps))).all()
         assert torch.equal(y[:, :len(levels)].float().cpu(), beta[:, None].expand(-1, len(levels)))
+
+
+@pytest.mark.gpu
+def test_many_slots():
+    """As many slots as a call takes, read once and by passes."""
+    from test_teacher_operators import check_distill, distill_case
+    for classes, frames in ((600, 9), (1500, 5), (9000, 6)):
+        for dtype in (torch.float32, torch.bfloat16):
+            z, t, index, weight, _ = distill_case(classes, 512, frames, dtype)
+            index[1::7, 2] = index[0, 2]
+            check_distill(z, t, index, frames, dtype, 2.0, weight=weight)
+
+
+@pytest.mark.gpu
+def test_layer_norm_backward_without_frames():
+    from binarybrain_b200 import ops
+    x, v = torch.ones((300, 8), device="cuda"), torch.zeros(0, device="cuda")
+    dx, dgamma, dbeta = ops.layer_norm_backward(x, x, v, v, 0)
+    assert not dgamma.any() and not dbeta.any()
+    dgamma, dbeta = torch.full((300,), 2.0, device="cuda"), torch.full((300,), 3.0, device="cuda")
+    ops.layer_norm_backward(x, x, v, v, 0, dgamma=dgamma, dbeta=dbeta)
+    assert (dgamma == 2.0).all() and (dbeta == 3.0).all()
