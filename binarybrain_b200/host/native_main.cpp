@@ -313,19 +313,50 @@ bool fits(int64_t n, int &v)
     return true;
 }
 
+// The device of a call's tensors: that of the first one, and the current one, since that is whose stream and scratch the operators take.
+struct Place {
+    int index = -1;
+
+    bool take(const at::Tensor &t, const char *name)
+    {
+        if (!t.is_cuda()) return refuse(name, "expected a CUDA tensor (the bbcu_* operators have no CPU path)");
+        const int at = t.device().index();
+        if (index < 0) index = at;
+        if (at == index) return true;
+        PyErr_Format(PyExc_ValueError, "%s: expected a tensor on cuda:%d, as the others of the call, got cuda:%d", name, index, at);
+        return false;
+    }
+    // before anything is allocated or launched
+    bool here() const
+    {
+        const int current = c10::cuda::current_device();
+        if (current == index) return true;
+        PyErr_Format(PyExc_ValueError, "the tensors are on cuda:%d, the current device is cuda:%d", index, current);
+        return false;
+    }
+    bool stream(bbcu_stream_t &s) const
+    {
+        if (!here()) return false;
+        s = reinterpret_cast<bbcu_stream_t>(c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)index).stream());
+        return true;
+    }
+};
+
 // A buffer of at least `frames` columns that are next to each other, rows any distance apart; `rows` < 0: any number.
 struct Frames {
+    Place &place;
     PyObject *given = nullptr;
     at::Tensor made;
     const at::Tensor *t = nullptr;
     int stride = 0;
 
+    explicit Frames(Place &place) : place(place) {}
     bool check(PyObject *o, const char *name, int64_t frames, int64_t rows)
     {
         if (!THPVariable_Check(o)) { PyErr_Format(PyExc_TypeError, "%s: expected a tensor", name); return false; }
         given = o;
         t = &THPVariable_Unpack(o);
-        if (!t->is_cuda()) return refuse(name, "expected a CUDA tensor (the bbcu_* operators have no CPU path)");
+        if (!place.take(*t, name)) return false;
         if (t->dim() != 2 || t->size(1) < frames || (t->size(1) > 1 && t->stride(1) != 1) || (t->size(0) > 1 && t->stride(0) < frames))
             return refuse(name, "expected [nodes, frame_stride] of at least the frames asked for, the frames of a node next to each other");
         if (rows >= 0 && t->size(0) != rows) { PyErr_Format(PyExc_ValueError, "%s: expected %lld rows, got %lld", name, (long long)rows, (long long)t->size(0)); return false; }
@@ -346,6 +377,7 @@ struct Frames {
             if (!take(o, name, frames, nullptr, rows)) return false;
             return t->scalar_type() == type || refuse(name, "expected the dtype of the other frames");
         }
+        if (!place.here()) return false;
         const int64_t unit = type == at::kFloat ? 8 : 16;
         made = at::empty({rows, (frames + unit - 1) / unit * unit}, at::TensorOptions().dtype(type).device(like.device()));
         t = &made;
@@ -359,15 +391,17 @@ struct Frames {
 
 // fp32 numbers of nodes or frames: given, or for None absent (input) or new (output)
 struct Numbers {
+    Place &place;
     PyObject *given = nullptr;
     at::Tensor made;
     float *data = nullptr;
 
+    explicit Numbers(Place &place) : place(place) {}
     bool check(PyObject *o, const char *name, int64_t size, bool written)
     {
         if (!THPVariable_Check(o)) { PyErr_Format(PyExc_TypeError, "%s: expected a tensor", name); return false; }
         const at::Tensor &t = THPVariable_Unpack(o);
-        if (!t.is_cuda()) return refuse(name, "expected a CUDA tensor (the bbcu_* operators have no CPU path)");
+        if (!place.take(t, name)) return false;
         if (t.scalar_type() != at::kFloat || t.numel() < size || !t.is_contiguous()) {
             PyErr_Format(PyExc_ValueError, "%s: expected a contiguous float32 tensor of %lld values", name, (long long)size);
             return false;
@@ -380,6 +414,7 @@ struct Numbers {
     bool output(PyObject *o, const char *name, int64_t size, const at::Tensor &like)
     {
         if (o != Py_None) return check(o, name, size, true);
+        if (!place.here()) return false;
         made = at::empty({size}, at::TensorOptions().dtype(at::kFloat).device(like.device()));
         data = static_cast<float *>(made.mutable_data_ptr());
         return true;
@@ -388,11 +423,12 @@ struct Numbers {
 };
 
 // rows of 8-bit integers
-const at::Tensor *int8_rows(PyObject *o, const char *name)
+const at::Tensor *int8_rows(PyObject *o, const char *name, Place &place)
 {
     if (!THPVariable_Check(o)) { PyErr_Format(PyExc_TypeError, "%s: expected a tensor", name); return nullptr; }
     const at::Tensor &t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.scalar_type() != at::kChar || t.dim() != 2 || !t.is_contiguous()) { refuse(name, "expected a contiguous int8 CUDA tensor [rows, inputs]"); return nullptr; }
+    if (!place.take(t, name)) return nullptr;
+    if (t.scalar_type() != at::kChar || t.dim() != 2 || !t.is_contiguous()) { refuse(name, "expected a contiguous int8 CUDA tensor [rows, inputs]"); return nullptr; }
     return &t;
 }
 
@@ -402,8 +438,6 @@ PyObject *tuple_of(PyObject *a, PyObject *b, PyObject *c = nullptr)
     Py_XDECREF(a); Py_XDECREF(b); Py_XDECREF(c);
     return r;
 }
-
-bbcu_stream_t current_stream() { return reinterpret_cast<bbcu_stream_t>(c10::cuda::getCurrentCUDAStream().stream()); }
 
 // the operator of the frames' type, looked up once; a status, or INT_MIN with a Python error set
 #define BB200_CALL_OF_TYPE(fp32, name32, name16, T32, T16, ...)                                            \
@@ -436,13 +470,15 @@ PyObject *layer_norm_forward_body(PyObject *const *o)
 {
     int frames, nodes;
     float eps;
-    Frames x, y;
-    Numbers gamma, beta, mean, rstd;
+    Place place;
+    bbcu_stream_t stream;
+    Frames x(place), y(place);
+    Numbers gamma(place), beta(place), mean(place), rstd(place);
     if (!parse(o[1], frames) || !parse(o[4], eps) || !x.take(o[0], "x", frames, nullptr, -1) || !fits(x.t->size(0), nodes) || !gamma.input(o[2], "gamma", nodes) ||
         !beta.input(o[3], "beta", nodes) || !y.output(o[5], "y", frames, x.t->scalar_type(), *x.t, nodes) || !mean.output(o[6], "mean", frames, *x.t) ||
         !rstd.output(o[7], "rstd", frames, *x.t)) return nullptr;
-    if (BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_LayerNormalization_Forward, bbcu_bf16_LayerNormalization_Forward, float, bbcu_bf16_t, x.in<const T *>(), y.out<T *>(),
-                           gamma.data, beta.data, mean.data, rstd.data, eps, nodes, frames, x.stride, y.stride, current_stream())) return nullptr;
+    if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_LayerNormalization_Forward, bbcu_bf16_LayerNormalization_Forward, float, bbcu_bf16_t, x.in<const T *>(), y.out<T *>(),
+                           gamma.data, beta.data, mean.data, rstd.data, eps, nodes, frames, x.stride, y.stride, stream)) return nullptr;
     return tuple_of(y.result(), mean.result(), rstd.result());
 }
 BB200_GUARDED(layer_norm_forward, 8)
@@ -451,17 +487,19 @@ BB200_GUARDED(layer_norm_forward, 8)
 PyObject *layer_norm_backward_body(PyObject *const *o)
 {
     int frames, nodes;
-    Frames x, dy, dx;
-    Numbers gamma, mean, rstd, dgamma, dbeta;
+    Place place;
+    bbcu_stream_t stream;
+    Frames x(place), dy(place), dx(place);
+    Numbers gamma(place), mean(place), rstd(place), dgamma(place), dbeta(place);
     if (!parse(o[4], frames) || !x.take(o[0], "x", frames, nullptr, -1) || !fits(x.t->size(0), nodes) || !dy.take(o[1], "dy", frames, x.t, nodes) ||
         !gamma.input(o[5], "gamma", nodes) || !mean.check(o[2], "mean", frames, false) || !rstd.check(o[3], "rstd", frames, false)) return nullptr;
     if ((o[7] == Py_None) != (o[8] == Py_None)) { refuse("dgamma and dbeta", "both or neither"); return nullptr; }
     const int accumulate = o[7] != Py_None;
     if (!dgamma.output(o[7], "dgamma", nodes, *x.t) || !dbeta.output(o[8], "dbeta", nodes, *x.t) ||
         !dx.output(o[6], "dx", frames, x.t->scalar_type(), *x.t, nodes)) return nullptr;
-    if (BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_LayerNormalization_Backward, bbcu_bf16_LayerNormalization_Backward, float, bbcu_bf16_t, x.in<const T *>(), dy.in<const T *>(),
+    if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_LayerNormalization_Backward, bbcu_bf16_LayerNormalization_Backward, float, bbcu_bf16_t, x.in<const T *>(), dy.in<const T *>(),
                            dx.out<T *>(), gamma.data, mean.data, rstd.data, dgamma.data, dbeta.data, accumulate, nodes, frames, x.stride, dy.stride, dx.stride,
-                           current_stream())) return nullptr;
+                           stream)) return nullptr;
     return tuple_of(dx.result(), dgamma.result(), dbeta.result());
 }
 BB200_GUARDED(layer_norm_backward, 9)
@@ -470,13 +508,15 @@ BB200_GUARDED(layer_norm_backward, 9)
 PyObject *quantize_int8_body(PyObject *const *o)
 {
     int frames, nodes;
-    Frames x;
-    Numbers scale;
+    Place place;
+    bbcu_stream_t stream;
+    Frames x(place);
+    Numbers scale(place);
     if (!parse(o[1], frames) || !x.take(o[0], "x", frames, nullptr, -1) || !fits(x.t->size(0), nodes) || !scale.output(Py_None, "scale", frames, *x.t)) return nullptr;
     const int row = (int)std::min<int64_t>(((int64_t)nodes + 15) / 16 * 16, INT_MAX / 16 * 16);
     at::Tensor q = at::empty({frames, row}, at::TensorOptions().dtype(at::kChar).device(x.t->device()));
-    if (BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_QuantizeInt8_Frames, bbcu_bf16_QuantizeInt8_Frames, float, bbcu_bf16_t, x.in<const T *>(),
-                           static_cast<signed char *>(q.mutable_data_ptr()), scale.data, nodes, frames, x.stride, row, current_stream())) return nullptr;
+    if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_QuantizeInt8_Frames, bbcu_bf16_QuantizeInt8_Frames, float, bbcu_bf16_t, x.in<const T *>(),
+                           static_cast<signed char *>(q.mutable_data_ptr()), scale.data, nodes, frames, x.stride, row, stream)) return nullptr;
     return tuple_of(THPVariable_Wrap(q), scale.result());
 }
 BB200_GUARDED(quantize_int8, 2)
@@ -485,17 +525,19 @@ BB200_GUARDED(quantize_int8, 2)
 PyObject *int8_dense_forward_body(PyObject *const *o)
 {
     int frames, nodes, n_in, q_stride, w_stride, bf16;
-    Frames y;
-    Numbers scale, w_scale, bias;
-    const at::Tensor *q = int8_rows(o[0], "q"), *W = q ? int8_rows(o[2], "W") : nullptr;
+    Place place;
+    bbcu_stream_t stream;
+    Frames y(place);
+    Numbers scale(place), w_scale(place), bias(place);
+    const at::Tensor *q = int8_rows(o[0], "q", place), *W = q ? int8_rows(o[2], "W", place) : nullptr;
     if (!W || !fits(q->size(0), frames) || !fits(W->size(0), nodes) || !fits(q->size(1), q_stride) || !fits(W->size(1), w_stride) || !parse_flag(o[7], bf16) ||
         !scale.check(o[1], "scale", frames, false) || !w_scale.check(o[3], "w_scale", nodes, false) || !bias.input(o[5], "bias", nodes)) return nullptr;
     n_in = q_stride;
     if (o[4] != Py_None && !parse(o[4], n_in)) return nullptr;
     if (o[6] != Py_None ? !y.take(o[6], "y", frames, nullptr, nodes) : !y.output(Py_None, "y", frames, bf16 ? at::kBFloat16 : at::kFloat, *q, nodes)) return nullptr;
-    if (BB200_CALL_OF_TYPE(y.fp32(), bbcu_int8_fp32_DenseAffine_Forward, bbcu_int8_bf16_DenseAffine_Forward, float, bbcu_bf16_t,
+    if (!place.stream(stream) || BB200_CALL_OF_TYPE(y.fp32(), bbcu_int8_fp32_DenseAffine_Forward, bbcu_int8_bf16_DenseAffine_Forward, float, bbcu_bf16_t,
                            static_cast<const signed char *>(q->const_data_ptr()), scale.data, static_cast<const signed char *>(W->const_data_ptr()), w_scale.data,
-                           bias.data, y.out<T *>(), n_in, nodes, frames, q_stride, w_stride, y.stride, current_stream())) return nullptr;
+                           bias.data, y.out<T *>(), n_in, nodes, frames, q_stride, w_stride, y.stride, stream)) return nullptr;
     return y.result();
 }
 BB200_GUARDED(int8_dense_forward, 8)
@@ -506,8 +548,10 @@ PyObject *distillation_loss_body(PyObject *const *o)
     int frames, classes, top;
     float temperature;
     double batch;
-    Frames z, t, index, dz;
-    Numbers t_lse, weight, loss_buf;
+    Place place;
+    bbcu_stream_t stream;
+    Frames z(place), t(place), index(place), dz(place);
+    Numbers t_lse(place), weight(place), loss_buf(place);
     if (!parse(o[3], frames) || !parse(o[4], temperature) || !z.take(o[0], "z", frames, nullptr, -1) || !fits(z.t->size(0), classes) ||
         !t.take(o[1], "t", frames, z.t, -1) || !fits(t.t->size(0), top) || !index.check(o[2], "index", frames, top)) return nullptr;
     if (index.t->scalar_type() != at::kInt) { refuse("index", "expected dtype int32"); return nullptr; }
@@ -518,9 +562,9 @@ PyObject *distillation_loss_body(PyObject *const *o)
     const double reduction = 1.0 / (batch > 1.0 ? batch : 1.0);
     at::Tensor loss = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(z.t->device()));
     float *const loss_data = static_cast<float *>(loss.mutable_data_ptr());
-    if (BB200_CALL_OF_TYPE(z.fp32(), bbcu_fp32_LossDistillation, bbcu_bf16_LossDistillation, float, bbcu_bf16_t, z.in<const T *>(), dz.out<T *>(), t.in<const T *>(),
+    if (!place.stream(stream) || BB200_CALL_OF_TYPE(z.fp32(), bbcu_fp32_LossDistillation, bbcu_bf16_LossDistillation, float, bbcu_bf16_t, z.in<const T *>(), dz.out<T *>(), t.in<const T *>(),
                            index.in<const int *>(), t_lse.data, weight.data, loss_buf.data, loss_data, temperature, (float)reduction, reduction, classes, top, frames,
-                           z.stride, dz.stride, t.stride, index.stride, current_stream())) return nullptr;
+                           z.stride, dz.stride, t.stride, index.stride, stream)) return nullptr;
     return tuple_of(dz.result(), THPVariable_Wrap(loss), loss_buf.result());
 }
 BB200_GUARDED(distillation_loss, 10)

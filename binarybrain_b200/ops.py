@@ -416,6 +416,8 @@ def quantize_int8(x, frames):
 def quantize_int8_channels(W):
     """Rows of W [out, in] fp32 as 8-bit integers: returns (q [out, int8_stride(in)], scale [out]).  Done once, when a network is loaded."""
     _chk(W, torch.float32, "W")
+    if W.device.index != torch.cuda.current_device():
+        raise ValueError(f"W: the tensor is on {W.device}, the current device is cuda:{torch.cuda.current_device()}")
     q = torch.empty((W.shape[0], int8_stride(W.shape[1])), dtype=torch.int8, device=W.device)
     scale = _n.vector_f32(W, W.shape[0])
     _n.bbcu_fp32_QuantizeInt8_Channels(W, q, scale, W.shape[1], W.shape[0], W.shape[1], q.shape[1])

@@ -133,3 +133,42 @@ def test_layer_norm_backward_without_frames():
     dgamma, dbeta = torch.full((300,), 2.0, device="cuda"), torch.full((300,), 3.0, device="cuda")
     ops.layer_norm_backward(x, x, v, v, 0, dgamma=dgamma, dbeta=dbeta)
     assert (dgamma == 2.0).all() and (dbeta == 3.0).all()
+
+
+class Elsewhere(torch.Tensor):
+    """A tensor of no memory that says it is on a CUDA device, for checks that end before any memory is asked for."""
+
+    @staticmethod
+    def __new__(cls, size, dtype, device):
+        return torch.Tensor._make_wrapper_subclass(cls, size, dtype=dtype, device=device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError
+
+
+def on_device(index):
+    """x [4, 8], v [8], rows of 8-bit integers and indices"""
+    device = torch.device("cuda", index)
+    return (Elsewhere((4, 8), torch.float32, device), Elsewhere((8,), torch.float32, device), Elsewhere((8, 16), torch.int8, device), Elsewhere((4, 8), torch.int32, device))
+
+
+def test_tensors_of_two_devices_are_refused():
+    pytest.importorskip("binarybrain_b200._native")
+    from binarybrain_b200 import ops
+    (x, v, q, i), (x1, v1, q1, i1) = on_device(0), on_device(1)
+    for call in (lambda: ops.layer_norm_forward(x, 8, gamma=v1), lambda: ops.layer_norm_forward(x, 8, beta=v1), lambda: ops.layer_norm_backward(x, x1, v, v, 8),
+                 lambda: ops.layer_norm_backward(x, x, v, v, 8, gamma=v1), lambda: ops.layer_norm_backward(x, x, v1, v, 8), lambda: ops.int8_dense_forward(q, v, q1, v),
+                 lambda: ops.int8_dense_forward(q, v1, q, v), lambda: ops.distillation_loss(x, x1, i, 8), lambda: ops.distillation_loss(x, x, i1, 8),
+                 lambda: ops.distillation_loss(x, x, i, 8, weight=v1), lambda: ops.distillation_loss(x1, x1, i1, 8, t_lse=v)):
+        with pytest.raises(ValueError, match="cuda:[01], as the others of the call"):
+            call()
+
+
+@pytest.mark.gpu
+def test_tensors_of_another_than_the_current_device_are_refused():
+    from binarybrain_b200 import ops
+    x, v, q, i = on_device(torch.cuda.current_device() + 1)
+    for call in (lambda: ops.layer_norm_forward(x, 8), lambda: ops.quantize_int8(x, 8), lambda: ops.distillation_loss(x, x, i, 8), lambda: ops.quantize_int8_channels(x)):
+        with pytest.raises(ValueError, match="the current device is cuda:"):
+            call()
