@@ -779,7 +779,7 @@ static int int8_dense(const int8_t *q, const float *q_scale, const int8_t *W, co
                       int ws, int ys, bbcu_stream_t stream)
 {
     BB200_REQUIRE(K > 0 && O >= 0 && F >= 0, BBCU_ERR_BAD_SIZE);
-    BB200_REQUIRE(K <= kMostInputs, BBCU_ERR_TOO_LARGE);
+    BB200_REQUIRE(K <= kMostInputs && O <= (1 << 30) && F <= (1 << 30), BBCU_ERR_TOO_LARGE);       // (counts are rounded up to whole tiles in 32 bits)
     const int least = (K + 15) / 16 * 16;
     BB200_REQUIRE(qs >= least && ws >= least && qs % 16 == 0 && ws % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(W) % 16 == 0 && ys >= F, BBCU_ERR_BAD_STRIDE);

@@ -411,7 +411,7 @@ int bbcu_bf16_QuantizeInt8_Frames(const bbcu_bf16_t *dev_x_buf, signed char *dev
 int bbcu_fp32_QuantizeInt8_Channels(const float *dev_W, signed char *dev_q_buf, float *dev_scale_buf, int input_node_size, int output_node_size,
                                     int w_node_stride, int q_node_stride, bbcu_stream_t stream);
 /* y[o][f] = w_scale[o] * q_scale[f] * sum_k W[o][k] * q[f][k] + bias[o] (dev_bias may be NULL), the sum exact: input_node_size up to 131071,
- * BBCU_ERR_TOO_LARGE beyond.  W [output][input] and q [frame][input] are rows of 8-bit integers on 16-byte boundaries (node strides in bytes, multiples
+ * output_node_size and frame_size up to 2^30, BBCU_ERR_TOO_LARGE beyond.  W [output][input] and q [frame][input] are rows of 8-bit integers on 16-byte boundaries (node strides in bytes, multiples
  * of 16, BBCU_ERR_BAD_STRIDE otherwise); what lies between input_node_size and the next multiple of 16 is not used. */
 int bbcu_int8_fp32_DenseAffine_Forward(const signed char *dev_q_buf, const float *dev_q_scale, const signed char *dev_W, const float *dev_w_scale,
                                        const float *dev_bias, float *dev_y_buf, int input_node_size, int output_node_size, int frame_size,

@@ -172,3 +172,15 @@ def test_tensors_of_another_than_the_current_device_are_refused():
     for call in (lambda: ops.layer_norm_forward(x, 8), lambda: ops.quantize_int8(x, 8), lambda: ops.distillation_loss(x, x, i, 8), lambda: ops.quantize_int8_channels(x)):
         with pytest.raises(ValueError, match="the current device is cuda:"):
             call()
+
+
+def test_the_int8_product_refuses_more_than_it_counts():
+    """Output nodes and frames within a tile of 2^31 would be no tiles at all; nothing is run or asked for (the pointers are made up)."""
+    native = pytest.importorskip("binarybrain_b200._native")
+    from binarybrain_b200 import abi
+    at, most = 1 << 20, 1 << 30
+    for kind in ("fp32", "bf16"):
+        for nodes, frames in ((4, most + 1), (4, 2 ** 31 - 1), (most + 1, 8), (2 ** 31 - 1, 1), (2 ** 31 - 100, 2)):
+            with pytest.raises(abi.BbcuError) as e:
+                getattr(native, f"bbcu_int8_{kind}_DenseAffine_Forward")(at, at, at, at, None, at, 16, nodes, frames, 16, 16, frames, 0)
+            assert e.value.status == -6, (nodes, frames)
