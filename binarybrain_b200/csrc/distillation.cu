@@ -118,7 +118,8 @@ __device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, in
     top = join_parts<ColumnMax>(&red[0][col], COLS, warps);
     slots = join_parts<ColumnSum>(&red[1][col], COLS, warps);
     const bool live = slots > 0.0f && w != 0.0f;
-    float lse = 0.0f;
+    // log p = (t - base) / T - lse: with the slots' own sum the level of the logits leaves before anything is rounded
+    float lse = 0.0f, base = 0.0f;
     if (a.t_lse) {
         if (live) lse = a.t_lse[f];
         __syncthreads();                                                  // (the two sums are read before the next two take their place)
@@ -130,13 +131,14 @@ __device__ __forceinline__ TeacherColumn teacher_columns(const Distill<T> &a, in
         if (threadIdx.x % 32 < COLS) red[2][own] = sum;
         __syncthreads();
         sum = join_parts<ColumnSum>(&red[2][col], COLS, warps);
-        lse = top * a.inv_t + logf(sum);
+        lse = logf(sum);
+        base = top;
     }
     float P = 0.0f;
     for (int k = group; k < a.K; k += groups) {
         float lp = -INFINITY;
         if (live && index[k * COLS + col] >= 0) {
-            lp = log_p[k * COLS + col] * a.inv_t - lse;
+            lp = (log_p[k * COLS + col] - base) * a.inv_t - lse;
             P += expf(lp);
         }
         log_p[k * COLS + col] = lp;

@@ -184,3 +184,21 @@ def test_the_int8_product_refuses_more_than_it_counts():
             with pytest.raises(abi.BbcuError) as e:
                 getattr(native, f"bbcu_int8_{kind}_DenseAffine_Forward")(at, at, at, at, None, at, 16, nodes, frames, 16, 16, frames, 0)
             assert e.value.status == -6, (nodes, frames)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,level", [(torch.float32, 2.0 ** 13), (torch.float32, -2.0 ** 16), (torch.bfloat16, 2.0 ** 7)], ids=["fp32+", "fp32-", "bf16"])
+@pytest.mark.parametrize("classes,top,frames", [(10, 10, 40), (3000, 32, 33), (9000, 64, 20)])
+def test_the_level_of_a_teachers_logits_does_not_count(classes, top, frames, dtype, level):
+    """Without a sum over all of its classes a teacher's probabilities are those of its slots: the same in every bit whatever is added to all of a frame's
+    logits, as long as the logits take it exactly."""
+    from binarybrain_b200 import ops
+    step = 1.0 if dtype == torch.bfloat16 else 2.0 ** -6
+    t = torch.from_numpy(np.random.default_rng(classes).integers(0, int(8 / step), (top, frames)) * step)
+    index = torch.argsort(normal(1, classes, frames), 0)[:top].to(torch.int32).cuda()
+    z = buffer(normal(2, classes, frames), dtype)
+    assert torch.equal((t + level).to(dtype).double() - level, t)
+    for temperature in (1.0, 3.0):
+        want = ops.distillation_loss(z, buffer(t, dtype), index, frames, temperature=temperature)
+        got = ops.distillation_loss(z, buffer(t + level, dtype), index, frames, temperature=temperature)
+        assert torch.equal(got[0][:, :frames], want[0][:, :frames]) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
