@@ -261,6 +261,9 @@ __device__ __forceinline__ int4 load_q(const int8_t *row, int k, int K)
     return v;
 }
 
+// An output from its sum.  The scales one after the other: their product may be outside of 32 bits where the output is not.
+__device__ __forceinline__ float scaled(int sum, float w_scale, float q_scale, float bias) { return fmaf((float)sum * w_scale, q_scale, bias); }
+
 // A single frame: what counts is to have W on its way.  A warp has a row of W, or one of `splits` parts of its inputs where there are few rows, and asks
 // for 4096 bytes of it before it multiplies; q comes out of L1.  (Two rows a warp for two to eight frames: 9.9 to 22.7 us for 4096 x 4096, the tiles below 9.3.)
 template <typename T>
@@ -298,7 +301,7 @@ k_int8_dense_row(const int8_t *__restrict__ q, const float *__restrict__ q_scale
         if (part == 0)
             for (int i = 1; i < splits; ++i) sum += red[warp + i];
     }
-    if (part == 0 && lane == 0 && o < O) y[(long long)o * ys] = from_float<T>(fmaf((float)sum, w_scale[o] * q_scale[0], bias ? bias[o] : 0.0f));
+    if (part == 0 && lane == 0 && o < O) y[(long long)o * ys] = from_float<T>(scaled(sum, w_scale[o], q_scale[0], bias ? bias[o] : 0.0f));
 }
 
 template <typename T>
@@ -350,7 +353,7 @@ __device__ __forceinline__ void store_columns(const GemmArgs &a, T *y, uint32_t 
         for (int i = 0; i < 32; i += kVec) {
             float r[kVec];
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) r[j] = fmaf((float)v[i + j], ws * scale[h + i + j], b);
+            for (int j = 0; j < kVec; ++j) r[j] = scaled(v[i + j], ws, scale[h + i + j], b);
             if (whole) {
                 stage[lane][(h + i) / kVec ^ (lane & (kPieces - 1))] = pack<T>(r);
             } else if (o0 + lane < a.O) {
@@ -520,7 +523,7 @@ k_int8_dense_tiles(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     const int sums[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (f0 + c + i < a.F) y[(long long)o * a.ys + f0 + c + i] = from_float<T>(fmaf((float)sums[i], ws * s_scale[warp & 3][c + i], b));
+                        if (f0 + c + i < a.F) y[(long long)o * a.ys + f0 + c + i] = from_float<T>(scaled(sums[i], ws, s_scale[warp & 3][c + i], b));
                 }
             }
         }

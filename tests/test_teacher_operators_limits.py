@@ -202,3 +202,25 @@ def test_the_level_of_a_teachers_logits_does_not_count(classes, top, frames, dty
         want = ops.distillation_loss(z, buffer(t, dtype), index, frames, temperature=temperature)
         got = ops.distillation_loss(z, buffer(t + level, dtype), index, frames, temperature=temperature)
         assert torch.equal(got[0][:, :frames], want[0][:, :frames]) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("n_in,n_out,frames", [(1000, 300, 1), (1000, 130, 5), (16384, 40, 24), (1024, 700, 333), (1024, 2048, 2048)])
+def test_int8_product_of_scales_whose_product_is_no_number_of_32_bits(n_in, n_out, frames, dtype):
+    from binarybrain_b200 import ops
+    from test_teacher_operators import int8_case
+    q, scale, W, w_scale, bias = int8_case(n_in, n_out, frames)
+    W[0] = 0                                                                         # sums of 0 stay 0 where the scales' product is beyond the largest number
+    acc = W[:, :n_in].cuda().double() @ q[:, :n_in].cuda().double().T                # exact: below 2**31
+    for by_w, by_q in ((-85, -45), (-45, -85), (70, 45)):
+        ws, s = (w_scale * 2.0 ** by_w).cuda(), (scale * 2.0 ** by_q).cuda()
+        b = (bias.double() * 2.0 ** max(-126, by_w + by_q + 20)).float().cuda() if by_w + by_q < 0 else bias.cuda()
+        y = ops.int8_dense_forward(q.cuda(), s, W.cuda(), ws, n_in=n_in, bias=b, dtype=dtype)[:, :frames].double()
+        product = acc * ws.double()[:, None] * s.double()
+        want = product + b.double()[:, None]
+        tol = 3 * U * product.abs() + 2 * U * want.abs() + 2.0 ** -149
+        if dtype == torch.bfloat16:
+            tol = tol + BF * (want.abs() + tol) + 2.0 ** -134                        # (half of the smallest subnormal)
+        inside = want.abs() < 2.0 ** 127
+        assert ((y - want).abs() - tol)[inside].max() <= 0 and torch.equal(y[0], b[0].to(dtype).double().expand(frames))
