@@ -319,7 +319,7 @@ __device__ __forceinline__ void join_columns(float (&v)[Q][kFramesPerVec<T>], co
 // How a kernel that streams over N rows is cut: `lanes` lanes along a row, 8 or, where those would leave most SMs without a cluster, 2; clusters that share
 // a column tile, of as many CTAs as an SM holds four of and eight rounds of rows for each.  (Backward of 65536 x 64: 81 us by 8 lanes, 38 by 2; of 65536 x 1024,
 // 256 CTAs by 8 lanes, 219 and 270.  One more doubling of the cluster, to a second round of CTAs, or clusters
-// of 16, lost: layer norm of 16384 x 4096 bf16 72 us, 87 by clusters of 16; 3000 x 5001 33 and 37.)
+// of 16, lost: layer norm of 16384 x 4096 bf16 72 us, 87 by clusters of 16 (its statistics have taken 2 us more since); 3000 x 5001 33 and 37.)
 struct StreamingPlan { int lanes; unsigned cluster, ctas; };
 template <typename T> inline StreamingPlan plan_streaming(int N, int F)
 {

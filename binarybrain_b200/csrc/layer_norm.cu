@@ -5,7 +5,8 @@
 //   backward   xh = (x - m) r,  c1 = mean_n gamma_n dy,  c2 = mean_n gamma_n dy xh,  dx = r (gamma_n dy - c1 - xh c2),
 //              dgamma_n = sum_f dy xh,  dbeta_n = sum_f dy
 //
-// Statistics and sums are 32 bits throughout; bf16 frames are widened when they are read and rounded once when they are written.
+// Statistics and sums are 32 bits or more throughout; bf16 frames are widened when they are read and rounded once when they are written.  A frame of one value
+// has that value for a mean and a variance of 0 in both forms below, and single nodes far from all others cost neither of them digits.
 //
 // The work is some ten operations a value, so memory bounds it: 8 bytes a value of fp32 forward, 12 backward, at the 6.5 TB/s of a copy.  A frame's values lie
 // a row apart, but 64 or 128 bytes of every row are enough: copies in columns of such pieces run at 5.5 to 6.4 TB/s.  What costs is that a frame is needed
@@ -23,7 +24,7 @@ constexpr int kMostNodes = 1 << 20;                    // 32 rows a CTA are 3276
 constexpr int kNormThreads = 256;                      // of the kernels that stream over chunks of rows
 
 // ---- two passes: statistics of the frames, then what is made of them.  The second one finds what L2 (126 MB) still holds of the first.
-// (8192 x 16384 fp32: statistics 88 us, y 154; backward of 65536 x 1024 230 us with the sums of the weights, 134 of them and less for the second pass.)
+// (8192 x 16384 fp32: statistics 95 us, y 153; backward of 65536 x 1024: sums 103, dx and the weights' parts 119, their sums 4.)
 
 __device__ __forceinline__ float middle(float a, float b, float c) { return fmaxf(fminf(a, b), fminf(fmaxf(a, b), c)); }
 
@@ -36,7 +37,7 @@ __device__ __forceinline__ int n_rows(int N, int first, int step) { return first
 // frame nor single nodes far from all others, wherever they are, cost digits (one level for all threads, the frame's first value, left rstd of 65536 nodes off
 // by 7e-4 where that value was 1000 standard deviations away).  Threads of a warp move to a level in common, and warps and CTAs join relative to the first value
 // in 64 bits.  A frame of one value has d = 0 at every step: its mean is that value and its variance 0.
-// (64 bits in the threads, too: 8192 x 16384 bf16 76 us instead of 60.)
+// (64 bits in the threads, too: 8192 x 16384 bf16 76 us instead of 62.  One level for all threads, an operation a value and the moves less: 60.)
 constexpr int kFoldBatches = 16;
 template <typename T, int LPR, bool ALIGNED>
 __global__ void __launch_bounds__(kNormThreads, 4)
@@ -332,6 +333,8 @@ __device__ __forceinline__ void fetch_rows(uint8_t *to, int piece, const T *from
     for (int i = 0; i < rows; ++i, to += piece, from += distance) cp_async16(to, from, true);
 }
 
+// (A sum over all rows times 1 / N, one operation a value less, is off by a rounding for equal values: y by 0.02 at a level of 1000.  The operations in pairs
+// pay for it: 4096 x 8192 fp32 61.5 us with that sum, 58 now; a single frame of 1024, in a graph, 4.85 and 5.05.)
 // Means of rows joined to their mean with weights that are the shares of the rows, each part as its distance from the first one: means that are equal stay
 // what they are, so that a frame of one value has that value for a mean and nothing but zeros about it.
 template <typename T, int LPR> struct MeanWeights {
@@ -651,8 +654,8 @@ static int layer_norm_forward(const T *x, T *y, const float *gamma, const float 
 {
     const bool aligned = frames_aligned<T>(x, xs) && frames_aligned<T>(y, ys);
     BB200_REQUIRE(F <= (1 << 30), BBCU_ERR_TOO_LARGE);
-    // Larger clusters than these lose to the two passes, larger ones of the backward than 8, too (us a pass, once / two passes: 4096 x 8192 fp32 63 / 71,
-    // 8192 x 16384 251 / 253, bf16 158 / 140; backward 4096 x 16384 bf16 130 / 139, fp32 202 / 231, 8192 x 8192 fp32 225 / 223).
+    // us a pass, once / two passes: 4096 x 8192 fp32 58 / 68, 3000 x 5001 31 / 34; backward 4096 x 16384 bf16 123 / 137, fp32 189 / 224.  Larger clusters than
+    // these lose to the two passes, larger ones of the backward than 8, too (8192 x 16384 fp32 251 / 253, bf16 158 / 140; backward 8192 x 8192 fp32 225 / 223).
     if (const ColumnPlan p = plan_columns<T>(N, F, sizeof(T) == 4 ? 8 : 4, kNormRows, sizeof(T) == 4 ? 8 : 4); aligned && p.cluster)
         return (p.lanes == 2 ? layer_norm_once<T, 2> : layer_norm_once<T, sizeof(T) == 4 ? 8 : 4>)(x, y, gamma, beta, mean, rstd, eps, N, F, xs, ys, p, st);
     constexpr int kWide = 32 * kFramesPerVec<T>;
