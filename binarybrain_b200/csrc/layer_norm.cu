@@ -36,7 +36,8 @@ __device__ __forceinline__ int n_rows(int N, int first, int step) { return first
 // to a sum of its own.  A move subtracts (sum d)^2 / count, which after the first one is at most half of what the rows since the last one have added to sum d^2: neither a level of the
 // frame nor single nodes far from all others, wherever they are, cost digits (one level for all threads, the frame's first value, left rstd of 65536 nodes off
 // by 7e-4 where that value was 1000 standard deviations away).  Threads of a warp move to a level in common, and warps and CTAs join relative to the first value
-// in 64 bits.  A frame of one value has d = 0 at every step: its mean is that value and its variance 0.
+// in 64 bits.  A frame of one value has d = 0 at every step: its mean is that value and its variance 0.  Where d^2 is beyond the
+// largest number (a node at the type's lowest one, say) the level stays, so that the mean is a number, the variance infinite and rstd 0.
 // (64 bits in the threads, too: 8192 x 16384 bf16 76 us instead of 62.  One level for all threads, an operation a value and the moves less: 60.)
 constexpr int kFoldBatches = 16;
 template <typename T, int LPR, bool ALIGNED>
@@ -60,10 +61,12 @@ k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int 
 #pragma unroll
             for (int j = 0; j < kVec; ++j) {
                 const float to = fmaf(s1[j], inv, level[j]), d = to - level[j], moved = count * d;
-                folded[j] += fmaf(d, moved - 2.0f * s1[j], s2[j]);
-                s1[j] -= moved;
-                s2[j] = 0.0f;
-                level[j] = to;
+                if (folded[j] + s2[j] < INFINITY) {
+                    folded[j] += fmaf(d, moved - 2.0f * s1[j], s2[j]);
+                    s1[j] -= moved;
+                    s2[j] = 0.0f;
+                    level[j] = to;
+                }
             }
         }
         uint4 raw[kBatch];
@@ -107,7 +110,8 @@ k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int 
         for (int m = LPR; m < 32; m <<= 1) to += __shfl_xor_sync(0xffffffffu, to, m);
         to += start;
         const float d = to - level[j], moved = count * d;
-        s2[j] = rows ? fmaf(d, moved - 2.0f * s1[j], folded[j] + s2[j]) : 0.0f;
+        const float squares = folded[j] + s2[j];
+        s2[j] = !rows ? 0.0f : squares < INFINITY ? fmaf(d, moved - 2.0f * s1[j], squares) : squares;
         s1[j] = rows ? s1[j] - moved : 0.0f;
         level[j] = to;
 #pragma unroll
@@ -122,7 +126,7 @@ k_layer_norm_stats(const T *x, float *mean_out, float *rstd_out, float eps, int 
             const float off = s1[j] * inv_warp;
             red[c.warp][0][c.col + j] = level[j];
             red[c.warp][1][c.col + j] = off;
-            red[c.warp][2][c.col + j] = fmaf(-s1[j], off, s2[j]);
+            red[c.warp][2][c.col + j] = s2[j] < INFINITY ? fmaf(-s1[j], off, s2[j]) : s2[j];
         }
         if (c.lane == 0) red_rows[c.warp] = warp_rows;
     }

@@ -224,3 +224,25 @@ def test_int8_product_of_scales_whose_product_is_no_number_of_32_bits(n_in, n_ou
             tol = tol + BF * (want.abs() + tol) + 2.0 ** -134                        # (half of the smallest subnormal)
         inside = want.abs() < 2.0 ** 127
         assert ((y - want).abs() - tol)[inside].max() <= 0 and torch.equal(y[0], b[0].to(dtype).double().expand(frames))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("nodes,layout", [(40, "rows"), (300, "rows"), (300, "odd"), (3000, "rows"), (9001, "rows"), (9001, "odd"), (70001, "rows")])
+def test_layer_norm_of_squares_beyond_the_largest_number(nodes, layout, dtype):
+    """Deviations of finite values whose squares are infinite: rstd is 0, the mean a number, y = beta."""
+    from binarybrain_b200 import ops
+    frames, lowest = 12, float(torch.finfo(dtype).min)
+    x = normal(nodes, nodes, frames)
+    x[0, 0] = x[-1, 1] = x[nodes // 2, 2] = x[nodes // 3, 3] = lowest
+    x[0, 4] = x[-1, 5] = -lowest
+    x[7, 6] = 1e30
+    x[:, 7] *= 1e25
+    x[::2, 8] *= 1e22
+    x = x.to(dtype)
+    beta = normal(1, nodes).float().to(dtype).float()
+    y, mean, rstd = ops.layer_norm_forward(buffer(x, dtype, layout), frames, beta=beta.cuda())
+    assert not rstd[:9].any() and (rstd[9:] > 0.5).all()
+    want = x.double().mean(0)
+    assert ((mean.cpu().double() - want).abs() - 16 * U * x.double().abs().mean(0) - U * want.abs()).max() <= 0
+    assert torch.equal(y[:, :9].float().cpu(), beta[:, None].expand(-1, 9))
