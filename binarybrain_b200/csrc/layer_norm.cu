@@ -257,7 +257,9 @@ k_layer_norm_grad_stats(const T *x, const T *dy, const float *__restrict__ gamma
         float a = 0.0f, b = 0.0f;
         for (uint32_t r = 0; r < cl; ++r) { a += peer_load(&part[threadIdx.x], r); b += peer_load(&part[kCols + threadIdx.x], r); }
         sums_out[f0 + threadIdx.x] = a / (float)N;
-        sums_out[padded + f0 + threadIdx.x] = b * rstd_in[f0 + threadIdx.x] / (float)N;
+        // (where rstd is 0 every xh is, though x - mean may have been too much for a sum)
+        const float rstd = rstd_in[f0 + threadIdx.x];
+        sums_out[padded + f0 + threadIdx.x] = rstd == 0.0f ? 0.0f : b * rstd / (float)N;
     }
     if (cl > 1) { cluster_arrive(); cluster_wait(); }
 }

@@ -230,7 +230,7 @@ def test_int8_product_of_scales_whose_product_is_no_number_of_32_bits(n_in, n_ou
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("nodes,layout", [(40, "rows"), (300, "rows"), (300, "odd"), (3000, "rows"), (9001, "rows"), (9001, "odd"), (70001, "rows")])
 def test_layer_norm_of_squares_beyond_the_largest_number(nodes, layout, dtype):
-    """Deviations of finite values whose squares are infinite: rstd is 0, the mean a number, y = beta."""
+    """Deviations of finite values whose squares are infinite: rstd is 0, the mean a number, y = beta, and the gradient 0."""
     from binarybrain_b200 import ops
     frames, lowest = 12, float(torch.finfo(dtype).min)
     x = normal(nodes, nodes, frames)
@@ -246,3 +246,5 @@ def test_layer_norm_of_squares_beyond_the_largest_number(nodes, layout, dtype):
     want = x.double().mean(0)
     assert ((mean.cpu().double() - want).abs() - 16 * U * x.double().abs().mean(0) - U * want.abs()).max() <= 0
     assert torch.equal(y[:, :9].float().cpu(), beta[:, None].expand(-1, 9))
+    dx, dgamma, dbeta = ops.layer_norm_backward(buffer(x, dtype, layout), buffer(normal(2, nodes, frames), dtype, layout), mean, rstd, frames)
+    assert not dx[:, :9].any() and torch.isfinite(dx[:, 9:frames]).all() and torch.isfinite(dgamma).all()
