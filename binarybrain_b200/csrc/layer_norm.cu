@@ -31,13 +31,14 @@ __device__ __forceinline__ float middle(float a, float b, float c) { return fmax
 // rows first, first + step, ... below N
 __device__ __forceinline__ int n_rows(int N, int first, int step) { return first < N ? (N - first + step - 1) / step : 0; }
 
-// A cluster has the columns of 128 (few frames: 32) bytes of a row; its CTAs take turns at the rows.  Each thread adds up d = x - level and d^2 of its rows in 32
-// bits, with a level of its own: the middle one of its first three values, moved to the mean of all its rows so far after 1, 2, 4, 8, 16, 32, 48 ... batches, when d^2 goes
-// to a sum of its own.  A move subtracts (sum d)^2 / count, which after the first one is at most half of what the rows since the last one have added to sum d^2: neither a level of the
-// frame nor single nodes far from all others, wherever they are, cost digits (one level for all threads, the frame's first value, left rstd of 65536 nodes off
-// by 7e-4 where that value was 1000 standard deviations away).  Threads of a warp move to a level in common, and warps and CTAs join relative to the first value
-// in 64 bits.  A frame of one value has d = 0 at every step: its mean is that value and its variance 0.  Where d^2 is beyond the
-// largest number (a node at the type's lowest one, say) the level stays, so that the mean is a number, the variance infinite and rstd 0.
+// A cluster has the columns of 128 (few frames: 32) bytes of a row; its CTAs take turns at the rows.  Each thread adds up d = x - level and d^2 of its rows
+// in 32 bits, with a level of its own: the middle one of its first three values, moved to the mean of all its rows so far after 1, 2, 4, 8, 16, 32, 48 ...
+// batches, when d^2 goes to a sum of its own.  A move subtracts (sum d)^2 / count, which after the first one is at most half of what the rows since the last
+// one have added to sum d^2: neither a level of the frame nor single nodes far from all others, wherever they are, cost digits (one level for all threads,
+// the frame's first value, left rstd of 65536 nodes off by 7e-4 where that value was 1000 standard deviations away).  Threads of a warp move to a level in
+// common, and warps and CTAs join relative to the first value in 64 bits.  A frame of one value has d = 0 at every step: its mean is that value and its
+// variance 0.  Where d^2 is beyond the largest number (a node at the type's lowest one, say) the level stays, so that the mean is a number, the variance
+// infinite and rstd 0.
 // (64 bits in the threads, too: 8192 x 16384 bf16 76 us instead of 62.  One level for all threads, an operation a value and the moves less: 60.)
 constexpr int kFoldBatches = 16;
 template <typename T, int LPR, bool ALIGNED>
