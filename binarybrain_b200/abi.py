@@ -96,6 +96,20 @@ SIGNATURES = {
     "bbcu_int8_bf16_DenseAffine_Forward": (_i, [_vp] * 6 + [_i] * 6 + [_vp]),
     "bbcu_fp32_LossDistillation": (_i, [_vp] * 8 + [_f] * 2 + [C.c_double] + [_i] * 7 + [_vp]),
     "bbcu_bf16_LossDistillation": (_i, [_vp] * 8 + [_f] * 2 + [C.c_double] + [_i] * 7 + [_vp]),
+    "bbcu_bf16_DenseAffine_Forward": (_i, [_vp] * 6 + [_i] * 9 + [_vp]),
+    "bbcu_bf16_fp32_DenseAffine_Forward": (_i, [_vp] * 6 + [_i] * 9 + [_vp]),
+    "bbcu_bf16_GatedDense_Forward": (_i, [_vp] * 5 + [_i] * 8 + [_vp]),
+    "bbcu_bf16_DenseAffine_BackwardInput": (_i, [_vp] * 4 + [_i] * 9 + [_vp]),
+    "bbcu_bf16_DenseAffine_BackwardWeights": (_i, [_vp] * 4 + [_i] * 7 + [_vp]),
+    "bbcu_fp32_RmsNormalization_Forward": (_i, [_vp] * 6 + [_f] + [_i] * 6 + [_vp]),
+    "bbcu_bf16_RmsNormalization_Forward": (_i, [_vp] * 6 + [_f] + [_i] * 6 + [_vp]),
+    "bbcu_fp32_RmsNormalization_QuantizeInt8": (_i, [_vp] * 7 + [_f] + [_i] * 6 + [_vp]),
+    "bbcu_bf16_RmsNormalization_QuantizeInt8": (_i, [_vp] * 7 + [_f] + [_i] * 6 + [_vp]),
+    "bbcu_fp32_RmsNormalization_Backward": (_i, [_vp] * 7 + [_i] * 7 + [_vp]),
+    "bbcu_bf16_RmsNormalization_Backward": (_i, [_vp] * 7 + [_i] * 7 + [_vp]),
+    "bbcu_fp32_GradientNorm": (_i, [_i] + [_vp] * 4),
+    "bbcu_fp32_GradientClip": (_i, [_i] + [_vp] * 2 + [_f] + [_vp] * 2),
+    "bbcu_fp32_OptimizerAdamClipped": (_i, [_i] + [_vp] * 5 + [_f] * 4 + [_vp, _i, _vp]),
 }
 
 

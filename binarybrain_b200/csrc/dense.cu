@@ -1,0 +1,821 @@
+// Dense layers in bf16 on the tensor cores, with what follows a product done before its sums leave the chip, and their gradients.  (The reference's dense
+// layers are fp32 through cuBLAS, include/bb/DenseAffine.h; it has no gated block.)
+//
+//   forward          z[o][f] = sum_k W[o][k] x[k][f] + b[o],   y = act(z) + r
+//   gated            g = (W x)[h],  u = (W x)[H + h]  (+ bias),   y[h][f] = act(g) u           both products on one read of x
+//   input gradient   dx[i][f] = sum_o W[o][i] dy[o][f],  times act'(z[i][f]) where the input was an activation of z,  or, where it was a gated block's
+//                    output, the gradients of both of its products: dg = dx u act'(g), du = dx act(g)
+//   weight gradient  dW[o][i] += sum_f dy[o][f] x[i][f],  db[o] += sum_f dy[o][f]
+//
+// x, W, dy and the kept z are bf16; the sums are 32 bits, bias, activation, residual and gate are applied to them in 32 bits, and each output is rounded once.
+// Frame buffers are read as they lie, frames next to each other: where the product sums over nodes, its operand is "across" (rows of shared memory along
+// the frames), which the tensor cores take from TMA's 128-byte swizzled boxes as well as rows along k; the gradients read W and x the other way round, and nothing is transposed.
+#include <cuda.h>
+
+#include "async_copy.cuh"
+#include "frame_columns.cuh"
+#include "tensor_core.cuh"
+
+namespace bb200 {
+
+enum DenseKind { kForward, kGated, kInputGrad, kWeightGrad };
+
+constexpr int kDenseThreads = 320, kDenseWarps = 8;      // warp 0 copies, warp 1 issues the products, eight warps take the sums out of TMEM
+constexpr int kTileM = 128, kTileK = 64;                 // output rows of a CTA; k of a stage (128 bytes)
+constexpr int kMostSplits = 8;
+constexpr int kTileGroup = 8;                            // tiles of output rows that are walked together, so that their operands stay in L2
+
+struct DenseArgs {
+    const float *bias;
+    const void *extra;                                   // residual (forward), z (input gradient)
+    void *out, *z_out;
+    int act, gated, accumulate, vec;                     // vec: the rows of extra, out and z_out start on 16-byte boundaries
+    int M, N, K, half;                                   // half: rows of a gated block's output, the distance between its two products
+    int splits;
+    long long extra_stride, out_stride, z_stride;
+    int *fault;
+};
+
+// ---- activations, in 32 bits.  gelu is z times the normal distribution's integral, through erfc, which keeps its digits where that is small; the logistic
+// function's divisor is between 1 and 2.
+__device__ __forceinline__ float logistic(float z)
+{
+    const float e = expf(-fabsf(z)), inv = __fdividef(1.0f, 1.0f + e);
+    return z < 0.0f ? e * inv : inv;
+}
+
+__device__ __forceinline__ float activate(float z, int act)
+{
+    switch (act) {
+    case BBCU_ACTIVATION_RELU: return fmaxf(z, 0.0f) + (z != z ? z : 0.0f);
+    case BBCU_ACTIVATION_GELU: return 0.5f * z * erfcf(z * -0.70710678f);
+    case BBCU_ACTIVATION_SILU: return z * logistic(z);
+    default: return z;
+    }
+}
+
+__device__ __forceinline__ float activation_slope(float z, int act)
+{
+    switch (act) {
+    case BBCU_ACTIVATION_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
+    case BBCU_ACTIVATION_GELU: return fmaf(z * 0.39894228f, expf(-0.5f * z * z), 0.5f * erfcf(z * -0.70710678f));
+    case BBCU_ACTIVATION_SILU: return logistic(z) * fmaf(z, logistic(-z), 1.0f);
+    default: return 1.0f;
+    }
+}
+
+// ---- what is made of eight (or, at the end of a row or at odd addresses, one) neighbouring sums of a row
+template <typename T> __device__ __forceinline__ void load_8(const T *p, float (&v)[8])
+{
+    if constexpr (sizeof(T) == 4) {
+        float a[4], b[4];
+        unpack<float>(*reinterpret_cast<const uint4 *>(p), a);
+        unpack<float>(*reinterpret_cast<const uint4 *>(p + 4), b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+    } else {
+        unpack<T>(*reinterpret_cast<const uint4 *>(p), v);
+    }
+}
+template <typename T> __device__ __forceinline__ void store_8(T *p, const float (&v)[8])
+{
+    if constexpr (sizeof(T) == 4) {
+        const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
+        *reinterpret_cast<uint4 *>(p) = pack<float>(a);
+        *reinterpret_cast<uint4 *>(p + 4) = pack<float>(b);
+    } else {
+        *reinterpret_cast<uint4 *>(p) = pack<T>(v);
+    }
+}
+template <typename T, int V> __device__ __forceinline__ void load_some(const T *p, float (&v)[V])
+{
+    if constexpr (V == 8) load_8<T>(p, v);
+    else v[0] = to_float(*p);
+}
+template <typename T, int V> __device__ __forceinline__ void store_some(T *p, const float (&v)[V])
+{
+    if constexpr (V == 8) store_8<T>(p, v);
+    else *p = from_float<T>(v[0]);
+}
+
+// v: sums of row m, columns n on; w: those of a gated block's second product
+template <int KIND, typename T, int V> __device__ __forceinline__ void finish(const DenseArgs &a, int m, int n, float (&v)[V], float (&w)[V])
+{
+    using B = __nv_bfloat16;
+    T *const out = static_cast<T *>(a.out) + (long long)m * a.out_stride + n;
+    if constexpr (KIND == kForward) {
+        float r[V];
+        if (a.extra) load_some<T, V>(static_cast<const T *>(a.extra) + (long long)m * a.extra_stride + n, r);
+        const float b = a.bias ? a.bias[m] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += b;
+        if (a.z_out) store_some<B, V>(static_cast<B *>(a.z_out) + (long long)m * a.z_stride + n, v);
+        if (a.act != BBCU_ACTIVATION_NONE) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = activate(v[j], a.act);
+        }
+        if (a.extra) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] += r[j];
+        }
+        store_some<T, V>(out, v);
+    } else if constexpr (KIND == kGated) {
+        const float b = a.bias ? a.bias[m] : 0.0f, c = a.bias ? a.bias[a.half + m] : 0.0f;
+        float y[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) { v[j] += b; w[j] += c; y[j] = activate(v[j], a.act) * w[j]; }
+        store_some<T, V>(out, y);
+        if (a.z_out) {
+            store_some<B, V>(static_cast<B *>(a.z_out) + (long long)m * a.z_stride + n, v);
+            store_some<B, V>(static_cast<B *>(a.z_out) + (long long)(a.half + m) * a.z_stride + n, w);
+        }
+    } else if constexpr (KIND == kInputGrad) {
+        const B *const z = static_cast<const B *>(a.extra) + (long long)m * a.extra_stride + n;
+        if (a.gated) {
+            float g[V], u[V], d[V];
+            load_some<B, V>(z, g);
+            load_some<B, V>(z + (long long)a.half * a.extra_stride, u);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                d[j] = v[j] * activate(g[j], a.act);
+                v[j] *= u[j] * activation_slope(g[j], a.act);
+            }
+            store_some<T, V>(out, v);
+            store_some<T, V>(out + (long long)a.half * a.out_stride, d);
+        } else {
+            if (a.extra) {
+                float g[V];
+                load_some<B, V>(z, g);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] *= activation_slope(g[j], a.act);
+            }
+            store_some<T, V>(out, v);
+        }
+    } else {
+        if (a.accumulate) {
+            float r[V];
+            load_some<T, V>(out, r);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] += r[j];
+        }
+        store_some<T, V>(out, v);
+    }
+}
+
+// as many of eight columns as there are
+template <int KIND, typename T> __device__ __forceinline__ void finish_8(const DenseArgs &a, int m, int n, float (&v)[8], float (&w)[8])
+{
+    if (a.vec && n + 8 <= a.N) {
+        finish<KIND, T, 8>(a, m, n, v, w);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (n + j < a.N) {
+                float p[1] = {v[j]}, q[1] = {w[j]};
+                finish<KIND, T, 1>(a, m, n + j, p, q);
+            }
+    }
+}
+
+// ---- a single frame: what counts is to have W on its way.  A warp has a row of W (a gated block: a row of both products), or one of `splits` parts of its
+// inputs where there are few rows, and asks for 4096 bytes of it before it multiplies; the frame comes out of shared memory, where a CTA has gathered it.
+constexpr int kRowThreads = 1024, kRowInputs = 16384;    // inputs that a CTA holds at a time
+template <int KIND, typename T>
+__global__ void __launch_bounds__(kRowThreads, 1)
+k_dense_row(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__restrict__ W, long long xs, long long ws, const DenseArgs a)
+{
+    grid_dependency();
+    constexpr int kAhead = 8;
+    constexpr int kParts = KIND == kGated ? 2 : 1;
+    __shared__ __align__(16) __nv_bfloat16 frame[kRowInputs];
+    __shared__ float red[kRowThreads / 32][2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % a.splits, per_cta = kRowThreads / 32 / a.splits;
+    const int rows = (a.M + (int)gridDim.x * per_cta - 1) / ((int)gridDim.x * per_cta);       // that a warp takes one after the other
+    float total[kParts] = {};
+    for (int r = 0; r < rows; ++r) {
+        const int m = (r * (int)gridDim.x + (int)blockIdx.x) * per_cta + warp / a.splits;
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) total[p] = 0.0f;
+        for (int k0 = 0; k0 < a.K; k0 += kRowInputs) {
+            const int inputs = min(kRowInputs, a.K - k0), steps = (inputs + 255) / 256;
+            const int s0 = steps * part / a.splits, s1 = steps * (part + 1) / a.splits;
+            uint4 w[kParts][kAhead / kParts];
+            constexpr int kBatch = kAhead / kParts;
+            auto fetch = [&](int s) {
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    const __nv_bfloat16 *const row = W + (long long)(min(m, a.M - 1) + p * a.half) * ws + k0;
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        const int k = (s + i) * 256 + lane * 8;
+                        w[p][i] = s + i < s1 && k < inputs ? __ldg(reinterpret_cast<const uint4 *>(row + k)) : make_uint4(0, 0, 0, 0);
+                    }
+                }
+            };
+            fetch(s0);
+            if (r == 0 || a.K > kRowInputs) {
+                __syncthreads();
+                for (int k = threadIdx.x; k < (inputs + 7) / 8 * 8; k += kRowThreads)
+                    frame[k] = k < inputs ? x[(long long)(k0 + k) * xs] : __nv_bfloat16(0.0f);
+                __syncthreads();
+            }
+            for (int s = s0; s < s1; s += kBatch) {
+                if (s > s0) fetch(s);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int k = (s + i) * 256 + lane * 8;
+                    if (s + i < s1 && k < inputs) {
+                        float v[8];
+                        load_8<__nv_bfloat16>(frame + k, v);
+#pragma unroll
+                        for (int p = 0; p < kParts; ++p) {
+                            float u[8];
+                            unpack<__nv_bfloat16>(w[p][i], u);
+                            if (k + 8 > inputs) {                         // the padding of W may hold anything
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) u[j] = k + j < inputs ? u[j] : 0.0f;
+                            }
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) total[p] = fmaf(u[j], v[j], total[p]);
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; ++p)
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) total[p] += __shfl_xor_sync(0xffffffffu, total[p], d);
+        if (a.splits > 1) {
+            __syncthreads();
+            if (lane == 0)
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) red[warp][p] = total[p];
+            __syncthreads();
+            if (part == 0)
+                for (int i = 1; i < a.splits; ++i)
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p) total[p] += red[warp + i][p];
+        }
+        if (part == 0 && lane == 0 && m < a.M) {
+            float v[1] = {total[0]}, w[1] = {total[kParts - 1]};
+            finish<KIND, T, 1>(a, m, 0, v, w);
+        }
+    }
+}
+
+// ---- tiles of 128 output rows x TN columns in TMEM (lane = row), by one CTA; or, PAIR, of 256 rows by a pair of CTAs (cta_group::2), each of which brings its
+// 128 rows of A and half of the columns of B and gets the sums of its rows.  64 of k a stage.  The accumulator is double: the sums of a tile leave beside the
+// products of the next.  Where there are fewer tiles than SMs, a cluster of CTAs shares the k of one: their sums cross through distributed shared memory and
+// are added in the order of the CTAs.
+//
+// fp32 outputs: the tensor cores cut the digits that do not fit their running sum, which over thousands of steps drifts (see kChunk); those sums are taken out
+// after every chunk of k and added up in registers.
+template <int KIND, typename T, int TN, bool PAIR> struct DenseShape {
+    static constexpr bool kAAcross = KIND == kInputGrad, kBAcross = KIND != kWeightGrad, kPromote = sizeof(T) == 4;
+    static constexpr int kParts = KIND == kGated ? 2 : 1, kOwnN = PAIR ? TN / 2 : TN, kBRows = kBAcross && kOwnN < 64 ? 64 : kOwnN;
+    static constexpr int kABytes = kTileM * kTileK * 2, kStageBytes = kParts * kABytes + kBRows * kTileK * 2;
+    static constexpr int kOutBytes = KIND == kGated ? 2048 : 4096;        // of a warp: 32 rows x 32 columns, bf16 or fp32
+    static constexpr int kRoom = 225 * 1024 - kDenseWarps * kOutBytes, kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
+    static constexpr int kSmem = kStages * kStageBytes + kDenseWarps * kOutBytes + 1024;
+    static constexpr int kAccColumns = kParts * TN, kColumns = 2 * kAccColumns < 32 ? 32 : 2 * kAccColumns;
+    static constexpr int kWarpColumns = TN / 2 < 32 ? 32 : TN / 2;        // a warp's share of a tile's columns
+};
+constexpr int kChunk = 8;                                // stages of k between two additions in registers
+
+template <int KIND, typename T, int TN, bool PAIR>
+__global__ void __launch_bounds__(kDenseThreads, 1)
+k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const DenseArgs a)
+{
+    using S = DenseShape<KIND, T, TN, PAIR>;
+    constexpr int kStages = S::kStages, kAcc = 2, kParts = S::kParts;
+    static_assert(S::kColumns <= 512 && (S::kColumns & (S::kColumns - 1)) == 0, "TMEM");
+    static_assert(kStages >= 4 && kParts * kTileM * (TN + 4) * 4 <= kStages * S::kStageBytes, "shared memory");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full[kStages], empty[kStages], acc_full[kAcc], acc_empty[kAcc], drained;
+    __shared__ uint32_t tmem_base;
+    __shared__ int gave_up;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR || a.splits > 1 ? cluster_rank() : 0;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], PAIR ? 2 * kDenseWarps : kDenseWarps); }
+        mbar_init(&drained, 1);
+        gave_up = 0;
+        mbar_init_fence();
+        tma_prefetch(&map_a);
+        tma_prefetch(&map_b);
+    }
+    __syncwarp();
+    if (warp == 1) {
+        if constexpr (PAIR) tmem_alloc_pair(&tmem_base, S::kColumns);
+        else tmem_alloc(&tmem_base, S::kColumns);
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if constexpr (PAIR) { cluster_arrive(); cluster_wait(); }
+    tcgen05_fence_after();
+    const uint32_t tmem = tmem_base;
+    grid_dependency();
+
+    constexpr int kRows = PAIR ? 2 * kTileM : kTileM;
+    const int tiles_m = (a.M + kRows - 1) / kRows, tiles_n = (a.N + TN - 1) / TN, tiles = tiles_m * tiles_n;
+    const int blocks_k = (a.K + kTileK - 1) / kTileK, splits = PAIR ? 1 : a.splits;
+    const int k0 = PAIR ? 0 : (int)((long long)blocks_k * rank / splits), k1 = PAIR ? blocks_k : (int)((long long)blocks_k * (rank + 1) / splits);
+    const int first = (int)blockIdx.x / (PAIR ? 2 : splits), step = (int)gridDim.x / (PAIR ? 2 : splits);
+    auto place = [&](int tile, int &m0, int &n0) {
+        const int group = tile / (kTileGroup * tiles_n), in = tile % (kTileGroup * tiles_n), rows = min(kTileGroup, tiles_m - group * kTileGroup);
+        m0 = (group * kTileGroup + in % rows) * kRows + (PAIR ? (int)rank * kTileM : 0);
+        n0 = in / rows * TN;
+    };
+
+    if (warp == 0 && lane == 0) {
+        int stage = 0, issued = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            int m0, n0;
+            place(tile, m0, n0);
+            if (PAIR) n0 += (int)rank * S::kOwnN;
+            for (int kb = k0; kb < k1; ++kb) {
+                ok = mbar_wait_one(&empty[stage], phase ^ 1, &gave_up);
+                if (!ok) break;
+                uint8_t *const at = smem + stage * S::kStageBytes;
+                if (!PAIR || rank == 0) mbar_arrive_expect_tx(&full[stage], (PAIR ? 2 : 1) * S::kStageBytes);
+                const uint32_t bar = PAIR ? peer_addr(&full[stage], 0) : 0;
+                auto load = [&](uint8_t *to, const CUtensorMap *map, int x, int row) {
+                    if constexpr (PAIR) tma_load_2d_pair(to, map, x, row, bar);
+                    else tma_load_2d(to, map, x, row, &full[stage]);
+                };
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    if constexpr (S::kAAcross) {
+                        load(at, &map_a, m0, kb * kTileK);
+                        load(at + S::kABytes / 2, &map_a, m0 + 64, kb * kTileK);
+                    } else {
+                        load(at + p * S::kABytes, &map_a, kb * kTileK, m0 + p * a.half);
+                    }
+                }
+                if constexpr (S::kBAcross) {
+#pragma unroll
+                    for (int j = 0; j < S::kBRows; j += 64) load(at + kParts * S::kABytes + j * kTileK * 2, &map_b, n0 + j, kb * kTileK);
+                } else {
+                    load(at + S::kABytes, &map_b, kb * kTileK, n0);
+                }
+                ++issued;
+                if (++stage == kStages) { stage = 0; phase ^= 1; }
+            }
+        }
+        // what is under way, for either CTA of a pair, lands before they leave, also where a wait has run out
+        if (!PAIR || rank == 0)
+            for (int b = issued > kStages ? issued - kStages : 0; b < issued; ++b)
+                mbar_wait_some(&full[b % kStages], (uint32_t)(b / kStages) & 1u, kDrainSpins);
+    } else if (warp == 1 && lane == 0 && (!PAIR || rank == 0)) {
+        constexpr uint32_t kInstr = mma_bf16_instruction(kRows, TN, S::kAAcross, S::kBAcross);
+        constexpr uint32_t kHalfBox = 64 * kTileK * 2;                    // 64 rows along m or n of a stage
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+            for (int c = k0; c < k1 && ok;) {
+                const int end = S::kPromote ? min(c + kChunk, k1) : k1, begin = c;
+                ok = mbar_wait_one(&acc_empty[acc], acc_phase ^ 1, &gave_up);
+                if (!ok) break;
+                tcgen05_fence_after();
+                for (; c < end; ++c) {
+                    ok = mbar_wait_one(&full[stage], phase, &gave_up);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const uint32_t at = smem_addr(smem + stage * S::kStageBytes), bt = at + kParts * S::kABytes;
+                    const uint64_t db = S::kBAcross ? smem_descriptor_128b_across(bt, kHalfBox) : smem_descriptor_128b(bt);
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p) {
+                        const uint64_t da = S::kAAcross ? smem_descriptor_128b_across(at, kHalfBox) : smem_descriptor_128b(at + p * S::kABytes);
+#pragma unroll
+                        for (int k = 0; k < kTileK / 16; ++k)
+                            mma_bf16<PAIR>(tmem + acc * S::kAccColumns + p * TN, da + k * (S::kAAcross ? 128 : 2), db + k * (S::kBAcross ? 128 : 2), kInstr, c > begin || k > 0);
+                    }
+                    if constexpr (PAIR) tcgen05_commit_pair(&empty[stage]);
+                    else tcgen05_commit(&empty[stage]);
+                    if (++stage == kStages) { stage = 0; phase ^= 1; }
+                }
+                if (!ok) break;
+                if constexpr (PAIR) tcgen05_commit_pair(&acc_full[acc]);
+                else tcgen05_commit(&acc_full[acc]);
+                if (++acc == kAcc) { acc = 0; acc_phase ^= 1; }
+            }
+        }
+        // no product is under way when the TMEM goes back
+        if constexpr (PAIR) tcgen05_commit_pair_own(&drained);
+        else tcgen05_commit(&drained);
+        mbar_wait_some(&drained, 0, kDrainSpins);
+    } else if (warp >= 2) {
+        const int part = warp & 3, c0 = (warp - 2) / 4 * S::kWarpColumns;  // the lanes of TMEM that this warp may read, its first column
+        uint4 *const stage_out = reinterpret_cast<uint4 *>(smem + kStages * S::kStageBytes + (warp - 2) * S::kOutBytes);
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        const uint32_t arrive = PAIR ? peer_addr(&acc_empty[0], 0) : smem_addr(&acc_empty[0]);
+        auto give_back = [&] {
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_cluster(arrive + acc * 8);
+                else mbar_arrive(&acc_empty[acc]);
+            }
+            if (++acc == kAcc) { acc = 0; acc_phase ^= 1; }
+        };
+        for (int tile = first; tile < tiles; tile += step) {
+            int m0, n0;
+            place(tile, m0, n0);
+            const int m = m0 + part * 32;
+            float sums[S::kPromote ? S::kWarpColumns : 1];
+            bool ok = true;
+            if constexpr (S::kPromote) {
+#pragma unroll
+                for (int i = 0; i < S::kWarpColumns; ++i) sums[i] = 0.0f;
+                for (int c = k0; c < k1; c += kChunk) {
+                    ok = mbar_wait_warp(&acc_full[acc], acc_phase, &gave_up);
+                    if (!ok) break;
+                    tcgen05_fence_after();
+                    const uint32_t at = tmem + ((uint32_t)(part * 32) << 16) + acc * S::kAccColumns + c0;
+                    if (c0 < TN) {
+#pragma unroll
+                        for (int i = 0; i < S::kWarpColumns; i += 32) {
+                            int v[32];
+                            tmem_load_32(at + i, v);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) sums[i + j] += __int_as_float(v[j]);
+                        }
+                    }
+                    give_back();
+                }
+            } else {
+                ok = mbar_wait_warp(&acc_full[acc], acc_phase, &gave_up);
+                tcgen05_fence_after();
+            }
+            if (!ok) break;
+            const uint32_t at = tmem + ((uint32_t)(part * 32) << 16) + acc * S::kAccColumns + c0;
+            if (splits > 1) {
+                // the stages are free: the tile's last product is done, and with it everything that read them
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    float *const to = reinterpret_cast<float *>(smem) + ((p * kTileM) + part * 32 + lane) * (TN + 4) + c0;
+                    if (c0 < TN) {
+#pragma unroll
+                        for (int i = 0; i < S::kWarpColumns; i += 32) {
+                            int v[32];
+                            if constexpr (S::kPromote) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] = __float_as_int(sums[i + j]);
+                            } else {
+                                tmem_load_32(at + p * TN + i, v);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) *reinterpret_cast<int4 *>(to + i + j) = make_int4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                        }
+                    }
+                }
+            } else if (c0 < TN) {
+#pragma unroll
+                for (int i = 0; i < S::kWarpColumns; i += 32) {
+                    const int n = n0 + c0 + i;
+                    if (n >= a.N) continue;
+                    if constexpr (KIND == kGated) {
+                        // everything is made in the lane of the row; the results cross shared memory in bf16, one of h, g and u after the other
+                        int v[32], w[32];
+                        tmem_load_32(at + i, v);
+                        tmem_load_32(at + TN + i, w);
+                        const int row = min(m + lane, a.M - 1);
+                        const float b = a.bias ? a.bias[row] : 0.0f, c = a.bias ? a.bias[a.half + row] : 0.0f;
+                        for (int what = 0; what < (a.z_out ? 3 : 1); ++what) {
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                float r[8];
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    const float g = __int_as_float(v[8 * q + j]) + b, u = __int_as_float(w[8 * q + j]) + c;
+                                    r[j] = what == 0 ? activate(g, a.act) * u : what == 1 ? g : u;
+                                }
+                                stage_out[lane * 4 + (q ^ (lane >> 1 & 3))] = pack<__nv_bfloat16>(r);
+                            }
+                            __syncwarp();
+                            __nv_bfloat16 *const base = what == 0 ? static_cast<__nv_bfloat16 *>(a.out) + (long long)m * a.out_stride
+                                                                  : static_cast<__nv_bfloat16 *>(a.z_out) + (long long)(m + (what == 2 ? a.half : 0)) * a.z_stride;
+                            const long long stride = what == 0 ? a.out_stride : a.z_stride;
+                            if (a.vec) {
+#pragma unroll
+                                for (int it = 0; it < 4; ++it) {
+                                    const int r = it * 8 + lane / 4, q = lane % 4;
+                                    const uint4 piece = stage_out[r * 4 + (q ^ (r >> 1 & 3))];
+                                    __nv_bfloat16 *const to = base + r * stride + n + 8 * q;
+                                    if (m + r >= a.M) continue;
+                                    if (n + 8 * q + 8 <= a.N) {
+                                        *reinterpret_cast<uint4 *>(to) = piece;
+                                    } else {
+                                        const __nv_bfloat16 *const one = reinterpret_cast<const __nv_bfloat16 *>(&piece);
+#pragma unroll
+                                        for (int j = 0; j < 8; ++j)
+                                            if (n + 8 * q + j < a.N) to[j] = one[j];
+                                    }
+                                }
+                            } else if (n + lane < a.N) {
+#pragma unroll 8
+                                for (int r = 0; r < min(32, a.M - m); ++r)
+                                    base[r * stride + n + lane] = reinterpret_cast<const __nv_bfloat16 *>(&stage_out[r * 4 + (lane / 8 ^ (r >> 1 & 3))])[lane % 8];
+                            }
+                            __syncwarp();
+                        }
+                    } else {
+                        // the sums cross 4 KB of shared memory, in 16-byte pieces whose order differs from row to row so that no banks collide: eight
+                        // columns a lane of four lanes side by side, or, where rows are not on 16-byte boundaries, a lane for each of the 32 columns
+                        int v[32];
+                        if constexpr (S::kPromote) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = __float_as_int(sums[i + j]);
+                        } else {
+                            tmem_load_32(at + i, v);
+                        }
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) stage_out[lane * 8 + (q ^ (lane & 7))] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                        __syncwarp();
+                        if (a.vec) {
+#pragma unroll
+                            for (int it = 0; it < 4; ++it) {
+                                const int r = it * 8 + lane / 4, q = lane % 4;
+                                float lo[4], hi[4], none[8];
+                                unpack<float>(stage_out[r * 8 + (2 * q ^ (r & 7))], lo);
+                                unpack<float>(stage_out[r * 8 + (2 * q + 1 ^ (r & 7))], hi);
+                                float s[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                                if (m + r < a.M && n + 8 * q < a.N) finish_8<KIND, T>(a, m + r, n + 8 * q, s, none);
+                            }
+                        } else if (n + lane < a.N) {
+#pragma unroll 4
+                            for (int r = 0; r < min(32, a.M - m); ++r) {
+                                float s[1] = {reinterpret_cast<const float *>(&stage_out[r * 8 + (lane / 4 ^ (r & 7))])[lane % 4]}, none[1];
+                                finish<KIND, T, 1>(a, m + r, n + lane, s, none);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+            if constexpr (!S::kPromote) give_back();
+        }
+    }
+    if (!PAIR && splits > 1) {
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (warp >= 2 && !gave_up) {
+            // a cluster has one tile; each of its CTAs finishes some of the rows
+            int m0, n0;
+            place(first, m0, n0);
+            const int rows = kTileM / splits, r0 = (int)rank * rows;
+            for (int e = threadIdx.x - 64; e < rows * (TN / 8); e += kDenseThreads - 64) {
+                const int r = r0 + e / (TN / 8), c = e % (TN / 8) * 8;
+                if (m0 + r >= a.M || n0 + c >= a.N) continue;
+                float s[2][8];
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    const uint32_t own = smem_addr(reinterpret_cast<float *>(smem) + (p * kTileM + r) * (TN + 4) + c);
+                    int4 lo[kMostSplits], hi[kMostSplits];
+#pragma unroll
+                    for (int q = 0; q < kMostSplits; ++q)                   // all of them under way at a time
+                        if (q < splits) { lo[q] = peer_load_v4(own, (uint32_t)q); hi[q] = peer_load_v4(own + 16, (uint32_t)q); }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) s[p][j] = 0.0f;
+#pragma unroll
+                    for (int q = 0; q < kMostSplits; ++q)
+                        if (q < splits) {
+                            s[p][0] += __int_as_float(lo[q].x); s[p][1] += __int_as_float(lo[q].y); s[p][2] += __int_as_float(lo[q].z); s[p][3] += __int_as_float(lo[q].w);
+                            s[p][4] += __int_as_float(hi[q].x); s[p][5] += __int_as_float(hi[q].y); s[p][6] += __int_as_float(hi[q].z); s[p][7] += __int_as_float(hi[q].w);
+                        }
+                }
+                finish_8<KIND, T>(a, m0 + r, n0 + c, s[0], s[kParts - 1]);
+            }
+        }
+        __syncwarp();
+        cluster_arrive();                                                 // nobody leaves while its sums may still be read
+        cluster_wait();
+    }
+    __syncwarp();
+    tcgen05_fence_before();
+    if constexpr (PAIR) { cluster_arrive(); cluster_wait(); } else __syncthreads();
+    tcgen05_fence_after();
+    if (warp == 1) {
+        if constexpr (PAIR) tmem_free_pair(tmem, S::kColumns);
+        else tmem_free(tmem, S::kColumns);
+    }
+    if (threadIdx.x == 0 && gave_up) atomicCAS(a.fault, 0, kFaultBarrierTimeout);
+}
+
+// db = or += the sums of the rows of dy: a CTA a row, 16 bytes a thread and round
+__global__ void __launch_bounds__(256)
+k_dense_bias_grad(const __nv_bfloat16 *__restrict__ dy, float *db, int F, long long stride, int accumulate)
+{
+    grid_dependency();
+    __shared__ float red[8];
+    const __nv_bfloat16 *const row = dy + (long long)blockIdx.x * stride;
+    float sum = 0.0f;
+    for (int f = threadIdx.x * 8; f < F; f += 256 * 8) {
+        float v[8];
+        load_8<__nv_bfloat16>(row + f, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += f + j < F ? v[j] : 0.0f;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 8; ++w) sum += red[w];
+        db[blockIdx.x] = accumulate ? db[blockIdx.x] + sum : sum;
+    }
+}
+
+// dW = db = 0 of a batch without frames
+__global__ void __launch_bounds__(256) k_dense_no_frames(float *dW, float *db, int I, long long stride)
+{
+    grid_dependency();
+    for (int i = threadIdx.x; i < I; i += 256)
+        if (dW) dW[(long long)blockIdx.x * stride + i] = 0.0f;
+    if (threadIdx.x == 0 && db) db[blockIdx.x] = 0.0f;
+}
+
+// ---- host side
+struct Operand { const __nv_bfloat16 *p; long long size, rows, stride; };     // rows of `size` elements
+
+template <int KIND, typename T, int TN, bool PAIR>
+static int dense_tiles(const Operand &A, const Operand &B, const DenseArgs &a, cudaStream_t st)
+{
+    using S = DenseShape<KIND, T, TN, PAIR>;
+    const TensorMapEncode encode = tensor_map_encode();
+    BB200_REQUIRE(encode != nullptr, BBCU_ERR_NO_DEVICE);
+    CUtensorMap map_a, map_b;
+    auto map = [&](CUtensorMap *m, const Operand &o, int box_rows) {
+        return tensor_map_rows(encode, m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, o.p, o.size, o.rows, o.stride * 2, box_rows) == CUDA_SUCCESS;
+    };
+    BB200_REQUIRE(map(&map_a, A, S::kAAcross ? kTileK : kTileM) && map(&map_b, B, S::kBAcross ? kTileK : S::kBRows), (int)cudaErrorInvalidValue);
+    constexpr int kRows = PAIR ? 2 * kTileM : kTileM;
+    const long long tiles = ((long long)a.M + kRows - 1) / kRows * (((long long)a.N + TN - 1) / TN), sms = device_info().sm_count;
+    BB200_REQUIRE(tiles < (1LL << 27), BBCU_ERR_TOO_LARGE);
+    auto kernel = k_dense_tiles<KIND, T, TN, PAIR>;
+    BB200_REQUIRE(allow_big_smem(kernel, S::kSmem), (int)cudaErrorInvalidValue);
+    const unsigned cluster = PAIR ? 2u : (unsigned)a.splits;
+    const long long slots = PAIR ? sms / 2 : sms;
+    const unsigned grid = cluster * (unsigned)(!PAIR && a.splits > 1 ? tiles : tiles < slots ? tiles : slots);
+    return launch_cluster(kernel, cluster, grid, kDenseThreads, S::kSmem, st, map_a, map_b, a);
+}
+
+// Columns a tile (0: by a pair of CTAs) and CTAs that share the k of one, by the clocks of an SM: rounds of tiles times stages of k times what a stage
+// costs -- 256 a product of 128 x 128 where the tensor cores bound, more where bringing the operands does -- and what it takes to store a tile.
+struct DenseTiles { int columns, splits; };
+static DenseTiles choose_dense_tiles(int M, int N, int K, int parts)
+{
+    const long long sms = device_info().sm_count, blocks = (K + kTileK - 1) / kTileK, tiles_m = ((long long)M + kTileM - 1) / kTileM;
+    const int pair_n = parts == 2 ? 128 : 256;
+    const long long pair_tiles = ((long long)M + 2 * kTileM - 1) / (2 * kTileM) * (((long long)N + pair_n - 1) / pair_n);
+    DenseTiles best = {0, 1};
+    long long least = (pair_tiles + sms / 2 - 1) / (sms / 2) * blocks * 512 + 3000;
+    for (int columns = 32; columns <= 128; columns *= 2) {
+        const long long tiles = tiles_m * (((long long)N + columns - 1) / columns);
+        for (int splits = 1; splits <= kMostSplits; splits *= 2) {
+            if (splits > 1 && (tiles * splits > sms || blocks < 2 * splits)) break;
+            const long long cost = (tiles * splits + sms - 1) / sms * ((blocks + splits - 1) / splits) * 2 * (kTileM * parts + columns) + 12 * columns * parts +
+                                   (splits > 1 ? 2500 : 0);
+            if (cost < least) { least = cost; best = {columns, splits}; }
+        }
+    }
+    return best;
+}
+
+template <int KIND, typename T> static int dense_product(const Operand &A, const Operand &B, DenseArgs &a, cudaStream_t st)
+{
+    a.fault = fault_word();
+    BB200_REQUIRE(a.fault != nullptr, BBCU_ERR_NO_DEVICE);
+    const DenseTiles t = choose_dense_tiles(a.M, a.N, a.K, KIND == kGated ? 2 : 1);
+    a.splits = t.splits;
+    switch (t.columns) {
+    case 32: return dense_tiles<KIND, T, 32, false>(A, B, a, st);
+    case 64: return dense_tiles<KIND, T, 64, false>(A, B, a, st);
+    case 128: return dense_tiles<KIND, T, 128, false>(A, B, a, st);
+    default: return dense_tiles<KIND, T, KIND == kGated ? 128 : 256, true>(A, B, a, st);
+    }
+}
+
+template <int KIND, typename T> static int dense_row(const __nv_bfloat16 *x, const __nv_bfloat16 *W, long long xs, long long ws, DenseArgs &a, cudaStream_t st)
+{
+    const int sms = device_info().sm_count, per_cta = kRowThreads / 32, steps = (std::min(a.K, kRowInputs) + 255) / 256;
+    a.splits = 1;
+    while (a.splits < 8 && (long long)a.M * a.splits < 16LL * sms && steps >= 2 * a.splits) a.splits *= 2;
+    const long long ctas = ((long long)a.M * a.splits + per_cta - 1) / per_cta;
+    launch(k_dense_row<KIND, T>, (unsigned)std::min<long long>(ctas, sms), kRowThreads, 0, st, x, W, xs, ws, a);
+    return launch_status();
+}
+
+constexpr int kMostExtent = 1 << 27;
+
+static bool rows_on_16(const void *p, long long stride) { return frames_aligned<__nv_bfloat16>(p, stride); }
+
+template <typename T>
+static int dense_forward(bool gated, const bbcu_bf16_t *x_, const bbcu_bf16_t *W_, const float *bias, const T *residual, T *y, bbcu_bf16_t *z, int activation, int K, int O,
+                         int F, int ws, int xs, int rs, int ys, int zs, bbcu_stream_t stream)
+{
+    const auto *x = reinterpret_cast<const __nv_bfloat16 *>(x_), *W = reinterpret_cast<const __nv_bfloat16 *>(W_);
+    BB200_REQUIRE(K > 0 && O >= 0 && F >= 0 && activation >= BBCU_ACTIVATION_NONE && activation <= BBCU_ACTIVATION_SILU, BBCU_ERR_BAD_SIZE);
+    BB200_REQUIRE(K <= kMostExtent && O <= kMostExtent && F <= kMostExtent, BBCU_ERR_TOO_LARGE);
+    BB200_REQUIRE(ws >= K && xs >= F && ys >= F && (!residual || rs >= F) && (!z || zs >= F) && rows_on_16(W, ws) && rows_on_16(x, xs), BBCU_ERR_BAD_STRIDE);
+    if (F == 0 || O == 0) return BBCU_OK;
+    BB200_REQUIRE_PTR(x); BB200_REQUIRE_PTR(W); BB200_REQUIRE_PTR(y);
+    DenseArgs a{};
+    a.bias = bias; a.extra = residual; a.out = y; a.z_out = z; a.act = activation;
+    a.M = O; a.N = F; a.K = K; a.half = O; a.splits = 1;
+    a.extra_stride = rs; a.out_stride = ys; a.z_stride = zs;
+    a.vec = frames_aligned<T>(y, ys) && (!residual || frames_aligned<T>(residual, rs)) && (!z || rows_on_16(z, zs));
+    cudaStream_t st = as_stream(stream);
+    const Operand A = {W, K, gated ? 2LL * O : O, ws}, B = {x, F, K, xs};
+    if constexpr (sizeof(T) == 2) {
+        if (gated) return F == 1 ? dense_row<kGated, T>(x, W, xs, ws, a, st) : dense_product<kGated, T>(A, B, a, st);
+    }
+    return F == 1 ? dense_row<kForward, T>(x, W, xs, ws, a, st) : dense_product<kForward, T>(A, B, a, st);
+}
+
+}   // namespace bb200
+
+using namespace bb200;
+
+extern "C" int bbcu_bf16_DenseAffine_Forward(const bbcu_bf16_t *x, const bbcu_bf16_t *W, const float *bias, const bbcu_bf16_t *residual, bbcu_bf16_t *y, bbcu_bf16_t *z,
+                                             int activation, int input_node_size, int output_node_size, int frame_size, int w_node_stride, int x_frame_stride,
+                                             int residual_frame_stride, int y_frame_stride, int z_frame_stride, bbcu_stream_t stream)
+{
+    return dense_forward<__nv_bfloat16>(false, x, W, bias, reinterpret_cast<const __nv_bfloat16 *>(residual), reinterpret_cast<__nv_bfloat16 *>(y), z, activation,
+                                        input_node_size, output_node_size, frame_size, w_node_stride, x_frame_stride, residual_frame_stride, y_frame_stride,
+                                        z_frame_stride, stream);
+}
+
+extern "C" int bbcu_bf16_fp32_DenseAffine_Forward(const bbcu_bf16_t *x, const bbcu_bf16_t *W, const float *bias, const float *residual, float *y, bbcu_bf16_t *z,
+                                                  int activation, int input_node_size, int output_node_size, int frame_size, int w_node_stride, int x_frame_stride,
+                                                  int residual_frame_stride, int y_frame_stride, int z_frame_stride, bbcu_stream_t stream)
+{
+    return dense_forward<float>(false, x, W, bias, residual, y, z, activation, input_node_size, output_node_size, frame_size, w_node_stride, x_frame_stride,
+                                residual_frame_stride, y_frame_stride, z_frame_stride, stream);
+}
+
+extern "C" int bbcu_bf16_GatedDense_Forward(const bbcu_bf16_t *x, const bbcu_bf16_t *W, const float *bias, bbcu_bf16_t *y, bbcu_bf16_t *z, int activation, int input_node_size,
+                                            int output_node_size, int frame_size, int w_node_stride, int x_frame_stride, int y_frame_stride, int z_frame_stride,
+                                            bbcu_stream_t stream)
+{
+    return dense_forward<__nv_bfloat16>(true, x, W, bias, nullptr, reinterpret_cast<__nv_bfloat16 *>(y), z, activation, input_node_size, output_node_size, frame_size,
+                                        w_node_stride, x_frame_stride, 0, y_frame_stride, z_frame_stride, stream);
+}
+
+extern "C" int bbcu_bf16_DenseAffine_BackwardInput(const bbcu_bf16_t *dy_, const bbcu_bf16_t *W_, const bbcu_bf16_t *z, bbcu_bf16_t *dx, int activation, int gated,
+                                                   int input_node_size, int output_node_size, int frame_size, int w_node_stride, int dy_frame_stride,
+                                                   int z_frame_stride, int dx_frame_stride, bbcu_stream_t stream)
+{
+    const auto *dy = reinterpret_cast<const __nv_bfloat16 *>(dy_), *W = reinterpret_cast<const __nv_bfloat16 *>(W_);
+    const int I = input_node_size, O = output_node_size, F = frame_size;
+    BB200_REQUIRE(I >= 0 && O > 0 && F >= 0 && activation >= BBCU_ACTIVATION_NONE && activation <= BBCU_ACTIVATION_SILU, BBCU_ERR_BAD_SIZE);
+    BB200_REQUIRE(I <= kMostExtent && O <= kMostExtent && F <= kMostExtent, BBCU_ERR_TOO_LARGE);
+    BB200_REQUIRE(w_node_stride >= I && dy_frame_stride >= F && dx_frame_stride >= F && (!z || z_frame_stride >= F) && rows_on_16(W, w_node_stride) &&
+                  rows_on_16(dy, dy_frame_stride), BBCU_ERR_BAD_STRIDE);
+    if (F == 0 || I == 0) return BBCU_OK;
+    BB200_REQUIRE_PTR(dy); BB200_REQUIRE_PTR(W); BB200_REQUIRE_PTR(dx);
+    if (gated) BB200_REQUIRE_PTR(z);
+    DenseArgs a{};
+    a.extra = z; a.out = dx; a.act = activation; a.gated = gated != 0;
+    a.M = I; a.N = F; a.K = O; a.half = I; a.splits = 1;
+    a.extra_stride = z_frame_stride; a.out_stride = dx_frame_stride;
+    a.vec = rows_on_16(dx, dx_frame_stride) && (!z || rows_on_16(z, z_frame_stride));
+    return dense_product<kInputGrad, __nv_bfloat16>({W, I, O, w_node_stride}, {dy, F, O, dy_frame_stride}, a, as_stream(stream));
+}
+
+extern "C" int bbcu_bf16_DenseAffine_BackwardWeights(const bbcu_bf16_t *x_, const bbcu_bf16_t *dy_, float *dW, float *dbias, int accumulate, int input_node_size,
+                                                     int output_node_size, int frame_size, int x_frame_stride, int dy_frame_stride, int dw_node_stride,
+                                                     bbcu_stream_t stream)
+{
+    const auto *x = reinterpret_cast<const __nv_bfloat16 *>(x_), *dy = reinterpret_cast<const __nv_bfloat16 *>(dy_);
+    const int I = input_node_size, O = output_node_size, F = frame_size;
+    BB200_REQUIRE(I > 0 && O >= 0 && F >= 0, BBCU_ERR_BAD_SIZE);
+    BB200_REQUIRE(I <= kMostExtent && O <= kMostExtent && F <= kMostExtent, BBCU_ERR_TOO_LARGE);
+    BB200_REQUIRE(x_frame_stride >= F && dy_frame_stride >= F && (!dW || dw_node_stride >= I) && rows_on_16(x, x_frame_stride) && rows_on_16(dy, dy_frame_stride),
+                  BBCU_ERR_BAD_STRIDE);
+    if (O == 0 || (!dW && !dbias)) return BBCU_OK;
+    cudaStream_t st = as_stream(stream);
+    if (F == 0) {
+        if (!accumulate) launch(k_dense_no_frames, (unsigned)O, 256, 0, st, dW, dbias, I, (long long)dw_node_stride);
+        return launch_status();
+    }
+    BB200_REQUIRE_PTR(dy);
+    if (dbias) launch(k_dense_bias_grad, (unsigned)O, 256, 0, st, dy, dbias, F, (long long)dy_frame_stride, accumulate);
+    if (!dW) return launch_status();
+    BB200_REQUIRE_PTR(x);
+    DenseArgs a{};
+    a.out = dW; a.accumulate = accumulate; a.act = BBCU_ACTIVATION_NONE;
+    a.M = O; a.N = I; a.K = F; a.splits = 1;
+    a.out_stride = dw_node_stride;
+    a.vec = frames_aligned<float>(dW, dw_node_stride);
+    return dense_product<kWeightGrad, float>({dy, F, O, dy_frame_stride}, {x, F, I, x_frame_stride}, a, st);
+}

@@ -9,56 +9,13 @@
 
 #include "async_copy.cuh"
 #include "frame_columns.cuh"
+#include "quantize.cuh"
 #include "tensor_core.cuh"
 
 namespace bb200 {
 
 constexpr int kQuantThreads = 256, kQuantRows = 256;      // rows of x that a CTA turns over
 constexpr int kMostInputs = 131071;                       // times 128 x 128 is below 2^31
-
-__device__ __forceinline__ float quant_scale(uint32_t abs_bits)
-{
-    return abs_bits >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __fdiv_rn(__uint_as_float(abs_bits), 127.0f);
-}
-
-__device__ __forceinline__ int quantize(float x, float scale)
-{
-    if (!(scale > 0.0f)) return 0;                        // zeros, or not finite
-    return max(-127, min(127, __float2int_rn(__fdiv_rn(x, scale))));
-}
-
-// Four numbers of a frame as a word of q.  x / scale comes through the reciprocal, off by less than 1e-4, and is rounded by adding 1.5 * 2^23, which
-// leaves the integer in the lowest byte; where that could have decided the rounding, and for scales without a normal reciprocal, the quotient is divided
-// out.  (The kernels are bound by their instructions, and the division costs more than all the rest.)
-struct Quantizer {
-    float scale, inv;
-    bool plain;
-    __device__ explicit Quantizer(float s) : scale(s), inv(1.0f / s), plain(s > 1e-36f && s < 1e36f) {}
-    __device__ uint32_t operator()(float x0, float x1, float x2, float x3) const
-    {
-        constexpr float kRound = 12582912.0f;
-        const float x[4] = {x0, x1, x2, x3};
-        float worst = 0.0f;
-        uint32_t r[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float t = x[i] * inv, n = t + kRound;
-            worst = fmaxf(worst, fabsf(t - (n - kRound)));
-            r[i] = __float_as_uint(n);
-        }
-        if (worst > 0.4999f || !plain) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = (uint32_t)quantize(x[i], scale);
-        }
-        return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
-    }
-};
-
-// the larger of the magnitudes of packed numbers, as integers: infinities and NaN are on top
-template <typename T> __device__ __forceinline__ uint32_t packed_abs_max(uint32_t a, uint32_t b)
-{
-    return sizeof(T) == 4 ? max(a, b & 0x7fffffffu) : __vmaxu2(a, b & 0x7fff7fffu);
-}
 
 // A cluster has the columns of 128 (few frames: 32) bytes of a row; its CTAs take turns at the rows and join the largest magnitudes in the first CTA's shared memory.
 template <typename T, int LPR, bool ALIGNED>
@@ -672,22 +629,9 @@ k_int8_dense_pairs(const __grid_constant__ CUtensorMap map_w, const __grid_const
 // rows of 8-bit integers as TMA sees them: boxes of 128 bytes x `box_rows` rows; what lies beyond the inputs or the rows reads as zero
 static int int8_rows_map(CUtensorMap *map, const int8_t *p, int K, int rows, long long stride, int box_rows)
 {
-    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static const Encode encode = [] {
-        void *fn = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            fn = nullptr;
-        }
-        return reinterpret_cast<Encode>(fn);
-    }();
+    const TensorMapEncode encode = tensor_map_encode();
     BB200_REQUIRE(encode != nullptr, BBCU_ERR_NO_DEVICE);
-    const cuuint64_t size[2] = {(cuuint64_t)K, (cuuint64_t)rows}, pitch[1] = {(cuuint64_t)stride};
-    const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows}, unit[2] = {1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(p), size, pitch, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = tensor_map_rows(encode, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p, K, rows, stride, box_rows);
     return r == CUDA_SUCCESS ? BBCU_OK : (int)cudaErrorInvalidValue;
 }
 

@@ -8,6 +8,7 @@
 //
 // All four operators are HBM-bound streams over [node][frame] rows: one CTA per (node, 8192-frame chunk),
 // 128-bit accesses when the rows are 16-byte aligned.
+#include "adam.cuh"
 #include "common.cuh"
 
 namespace bb200 {
@@ -205,11 +206,7 @@ k_adam(const int *__restrict__ size_table, float *const *params, float *const *g
     const int t = blockIdx.y;
     const int n = size_table[t];
     float *p = params[t], *m = m_tab[t], *v = v_tab[t], *g = grads[t];
-    auto one = [&](float &pi, float gi, float &mi, float &vi) {
-        mi += (1.0f - beta1) * (gi - mi);
-        vi += (1.0f - beta2) * (gi * gi - vi);
-        pi -= lr_t * mi / (sqrtf(vi) + 1.0e-7f);
-    };
+    auto one = [&](float &pi, float gi, float &mi, float &vi) { adam_step(pi, gi, mi, vi, lr_t, beta1, beta2); };
     const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(g)) & 15) == 0;
     const int quads = vec ? n / 4 : 0, threads = gridDim.x * blockDim.x, id = blockIdx.x * blockDim.x + threadIdx.x;
     for (int i = id; i < quads; i += threads) {

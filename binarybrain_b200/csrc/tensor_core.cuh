@@ -1,5 +1,5 @@
-// The fifth-generation tensor cores as inline PTX for sm_100a: tiled TMA loads, shared-memory descriptors, 8-bit integer products into TMEM, and the
-// bounded waits around them.
+// The fifth-generation tensor cores as inline PTX for sm_100a: tiled TMA loads, shared-memory descriptors, products of 8-bit integers and of bf16 into TMEM,
+// and the bounded waits around them.
 //
 // Rules kept here: a tiled copy starts on a 16-byte boundary of a row; one thread issues all products and commits of a CTA; every wait has a limit, and
 // the first one that runs out sets the CTA's flag, which all others look at, so that no role waits for another that has left.
@@ -109,6 +109,29 @@ __device__ __forceinline__ uint64_t smem_descriptor_128b(uint32_t addr)
     return (uint64_t)((addr & 0x3ffffu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// The same rows along m or n, 64 of them (128 bytes) a row of k, eight rows of k a group of 1024 bytes: 64 further ones lie `next` bytes on.  16 rows of k
+// further on are 128 units of the address field.
+__device__ __forceinline__ uint64_t smem_descriptor_128b_across(uint32_t addr, uint32_t next)
+{
+    return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// what a product of bf16 with sums of 32 bits is told about its operands; across: their rows lie along m or n instead of k
+__host__ __device__ constexpr uint32_t mma_bf16_instruction(int m, int n, bool a_across, bool b_across)
+{
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_across << 15) | ((uint32_t)b_across << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+template <bool PAIR> __device__ __forceinline__ void mma_bf16(uint32_t tmem, uint64_t a, uint64_t b, uint32_t instr, bool accumulate)
+{
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(tmem), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(tmem), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)accumulate) : "memory");
+}
+
 __device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t a, uint64_t b, uint32_t instr, bool accumulate)
 {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
@@ -140,6 +163,34 @@ __device__ __forceinline__ int4 peer_load_v4(uint32_t own_smem, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(own_smem), "r"(rank));
     asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
+}
+
+// cuTensorMapEncodeTiled of the driver, looked up once; null where there is none
+using TensorMapEncode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                     const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline TensorMapEncode tensor_map_encode()
+{
+    static const TensorMapEncode encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            fn = nullptr;
+        }
+        return reinterpret_cast<TensorMapEncode>(fn);
+    }();
+    return encode;
+}
+
+// Rows of `size` elements as TMA sees them: 128-byte swizzled boxes of 128 bytes x `box_rows` rows; what lies beyond the elements or the rows reads as zero.
+// The rows start on 16-byte boundaries.
+inline CUresult tensor_map_rows(TensorMapEncode encode, CUtensorMap *map, CUtensorMapDataType type, int element, const void *p, long long size, long long rows,
+                                long long stride_bytes, int box_rows)
+{
+    const cuuint64_t extent[2] = {(cuuint64_t)size, (cuuint64_t)rows}, pitch[1] = {(cuuint64_t)stride_bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / element), (cuuint32_t)box_rows}, unit[2] = {1, 1};
+    return encode(map, type, 2, const_cast<void *>(p), extent, pitch, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 }   // namespace bb200

@@ -130,7 +130,7 @@ template <class... A> struct Operator<int(A...)> {
     }
 };
 
-// A new uninitialised tensor on the device of `like`: empty_f32 / empty_i32(like, rows, cols), vector_f32(like, n), scalar_f64(like)
+// A new uninitialised tensor on the device of `like`: empty_f32 / empty_i32(like, rows, cols), vector_f32(like, n), scalar_f64 / scalar_f32(like)
 template <int DIM> PyObject *empty(at::ScalarType type, PyObject *const *o, Py_ssize_t n)
 {
     constexpr Py_ssize_t want = DIM + 1;
@@ -151,6 +151,7 @@ PyObject *empty_f32(PyObject *, PyObject *const *o, Py_ssize_t n)  { return empt
 PyObject *empty_i32(PyObject *, PyObject *const *o, Py_ssize_t n)  { return empty<2>(at::kInt, o, n); }
 PyObject *vector_f32(PyObject *, PyObject *const *o, Py_ssize_t n) { return empty<1>(at::kFloat, o, n); }
 PyObject *scalar_f64(PyObject *, PyObject *const *o, Py_ssize_t n) { return empty<0>(at::kDouble, o, n); }
+PyObject *scalar_f32(PyObject *, PyObject *const *o, Py_ssize_t n) { return empty<0>(at::kFloat, o, n); }
 
 #define BB200_OPERATORS(X)                                                                                                                    \
     X(bbcu_fp32_StochasticLut6_Forward) X(bbcu_bit_fp32_StochasticLut6_Forward) X(bbcu_bit_bit_fp32_StochasticLut6_Forward)                   \
@@ -171,7 +172,11 @@ PyObject *scalar_f64(PyObject *, PyObject *const *o, Py_ssize_t n) { return empt
     X(bbcu_fp32_LayerNormalization_Forward) X(bbcu_bf16_LayerNormalization_Forward) X(bbcu_fp32_LayerNormalization_Backward)                  \
     X(bbcu_bf16_LayerNormalization_Backward) X(bbcu_fp32_QuantizeInt8_Frames) X(bbcu_bf16_QuantizeInt8_Frames)                                \
     X(bbcu_fp32_QuantizeInt8_Channels) X(bbcu_int8_fp32_DenseAffine_Forward) X(bbcu_int8_bf16_DenseAffine_Forward)                            \
-    X(bbcu_fp32_LossDistillation) X(bbcu_bf16_LossDistillation)
+    X(bbcu_fp32_LossDistillation) X(bbcu_bf16_LossDistillation) X(bbcu_bf16_DenseAffine_Forward) X(bbcu_bf16_fp32_DenseAffine_Forward)          \
+    X(bbcu_bf16_GatedDense_Forward) X(bbcu_bf16_DenseAffine_BackwardInput) X(bbcu_bf16_DenseAffine_BackwardWeights)                            \
+    X(bbcu_fp32_RmsNormalization_Forward) X(bbcu_bf16_RmsNormalization_Forward) X(bbcu_fp32_RmsNormalization_QuantizeInt8)                    \
+    X(bbcu_bf16_RmsNormalization_QuantizeInt8) X(bbcu_fp32_RmsNormalization_Backward) X(bbcu_bf16_RmsNormalization_Backward)                  \
+    X(bbcu_fp32_GradientNorm) X(bbcu_fp32_GradientClip) X(bbcu_fp32_OptimizerAdamClipped)
 
 #define BB200_DEFINE(name)                                                          \
     PyObject *py_##name(PyObject *, PyObject *const *o, Py_ssize_t n)               \
@@ -569,6 +574,199 @@ PyObject *distillation_loss_body(PyObject *const *o)
 }
 BB200_GUARDED(distillation_loss, 10)
 
+// rms_norm_forward(x, frames, gamma, eps, residual, y, s, rstd) -> (y, s, rstd); without a residual s is x
+PyObject *rms_norm_forward_body(PyObject *const *o)
+{
+    int frames, nodes;
+    float eps;
+    Place place;
+    bbcu_stream_t stream;
+    Frames x(place), residual(place), s(place), y(place);
+    Numbers gamma(place), rstd(place);
+    if (!parse(o[1], frames) || !parse(o[3], eps) || !x.take(o[0], "x", frames, nullptr, -1) || !fits(x.t->size(0), nodes) || !gamma.input(o[2], "gamma", nodes) ||
+        (o[4] != Py_None && (!residual.take(o[4], "residual", frames, x.t, nodes) || !s.output(o[6], "s", frames, x.t->scalar_type(), *x.t, nodes))) ||
+        !y.output(o[5], "y", frames, x.t->scalar_type(), *x.t, nodes) || !rstd.output(o[7], "rstd", frames, *x.t)) return nullptr;
+    if (o[4] == Py_None && o[6] != Py_None) { refuse("s", "given without a residual"); return nullptr; }
+    if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_RmsNormalization_Forward, bbcu_bf16_RmsNormalization_Forward, float, bbcu_bf16_t, x.in<const T *>(),
+                           residual.t ? residual.in<const T *>() : nullptr, s.t ? s.out<T *>() : nullptr, y.out<T *>(), gamma.data, rstd.data, eps, nodes, frames, x.stride,
+                           residual.stride, s.stride, y.stride, stream)) return nullptr;
+    return tuple_of(y.result(), s.t ? s.result() : x.result(), rstd.result());
+}
+BB200_GUARDED(rms_norm_forward, 8)
+
+// rms_norm_int8(x, frames, gamma, eps, residual, s) -> (q, scale, s)
+PyObject *rms_norm_int8_body(PyObject *const *o)
+{
+    int frames, nodes;
+    float eps;
+    Place place;
+    bbcu_stream_t stream;
+    Frames x(place), residual(place), s(place);
+    Numbers gamma(place), scale(place);
+    if (!parse(o[1], frames) || !parse(o[3], eps) || !x.take(o[0], "x", frames, nullptr, -1) || !fits(x.t->size(0), nodes) || !gamma.input(o[2], "gamma", nodes) ||
+        (o[4] != Py_None && (!residual.take(o[4], "residual", frames, x.t, nodes) || !s.output(o[5], "s", frames, x.t->scalar_type(), *x.t, nodes))) ||
+        !scale.output(Py_None, "scale", frames, *x.t)) return nullptr;
+    if (o[4] == Py_None && o[5] != Py_None) { refuse("s", "given without a residual"); return nullptr; }
+    const int row = (int)std::min<int64_t>(((int64_t)nodes + 15) / 16 * 16, INT_MAX / 16 * 16);
+    at::Tensor q = at::empty({frames, row}, at::TensorOptions().dtype(at::kChar).device(x.t->device()));
+    if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_RmsNormalization_QuantizeInt8, bbcu_bf16_RmsNormalization_QuantizeInt8, float, bbcu_bf16_t,
+                           x.in<const T *>(), residual.t ? residual.in<const T *>() : nullptr, s.t ? s.out<T *>() : nullptr, static_cast<signed char *>(q.mutable_data_ptr()),
+                           scale.data, gamma.data, nullptr, eps, nodes, frames, x.stride, residual.stride, s.stride, row, stream)) return nullptr;
+    return tuple_of(THPVariable_Wrap(q), scale.result(), s.t ? s.result() : x.result());
+}
+BB200_GUARDED(rms_norm_int8, 6)
+
+// rms_norm_backward(s, dy, rstd, frames, gamma, dresidual, ds, dgamma) -> (ds, dgamma); a given dgamma is added to
+PyObject *rms_norm_backward_body(PyObject *const *o)
+{
+    int frames, nodes;
+    Place place;
+    bbcu_stream_t stream;
+    Frames s(place), dy(place), dresidual(place), ds(place);
+    Numbers gamma(place), rstd(place), dgamma(place);
+    if (!parse(o[3], frames) || !s.take(o[0], "s", frames, nullptr, -1) || !fits(s.t->size(0), nodes) || !dy.take(o[1], "dy", frames, s.t, nodes) ||
+        !gamma.input(o[4], "gamma", nodes) || !rstd.check(o[2], "rstd", frames, false) || (o[5] != Py_None && !dresidual.take(o[5], "dresidual", frames, s.t, nodes)) ||
+        !dgamma.output(o[7], "dgamma", nodes, *s.t) || !ds.output(o[6], "ds", frames, s.t->scalar_type(), *s.t, nodes)) return nullptr;
+    const int accumulate = o[7] != Py_None;
+    if (!place.stream(stream) || BB200_CALL_OF_TYPE(s.fp32(), bbcu_fp32_RmsNormalization_Backward, bbcu_bf16_RmsNormalization_Backward, float, bbcu_bf16_t, s.in<const T *>(),
+                           dy.in<const T *>(), dresidual.t ? dresidual.in<const T *>() : nullptr, ds.out<T *>(), gamma.data, rstd.data, dgamma.data, accumulate, nodes,
+                           frames, s.stride, dy.stride, dresidual.stride, ds.stride, stream)) return nullptr;
+    return tuple_of(ds.result(), dgamma.result());
+}
+BB200_GUARDED(rms_norm_backward, 8)
+
+// ---- dense products in bf16: weights and frames on 16-byte boundaries, as TMA reads them
+
+bool on_16(const at::Tensor &t, int64_t stride) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 && stride * t.element_size() % 16 == 0; }
+
+// rows of bf16 weights
+const at::Tensor *bf16_weights(PyObject *o, Place &place, int &stride)
+{
+    if (!THPVariable_Check(o)) { PyErr_SetString(PyExc_TypeError, "W: expected a tensor"); return nullptr; }
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (!place.take(t, "W")) return nullptr;
+    if (t.scalar_type() != at::kBFloat16 || t.dim() != 2 || (t.size(1) > 1 && t.stride(1) != 1)) { refuse("W", "expected bfloat16 [outputs, inputs], the inputs of a row next to each other"); return nullptr; }
+    const int64_t row = t.size(0) > 1 ? t.stride(0) : (t.size(1) + 7) / 8 * 8;
+    if (row < t.size(1) || !on_16(t, row)) { refuse("W", "expected rows that start on 16-byte boundaries (a row stride that is a multiple of 8)"); return nullptr; }
+    return fits(row, stride) ? &t : nullptr;
+}
+
+bool bf16_operand(Frames &f, PyObject *o, const char *name, int64_t frames, int64_t rows)
+{
+    if (!f.check(o, name, frames, rows)) return false;
+    if (f.t->scalar_type() != at::kBFloat16) return refuse(name, "expected dtype bfloat16");
+    if (f.t->size(0) <= 1 && f.stride % 8 != 0) f.stride = (int)std::min<int64_t>(((int64_t)f.stride + 7) / 8 * 8, INT_MAX / 8 * 8);      // a single row has no stride
+    return on_16(*f.t, f.stride) || refuse(name, "expected rows that start on 16-byte boundaries (a stride that is a multiple of 8)");
+}
+
+// what is kept of a product for its gradient: nothing (false or None), a new buffer (true), or the given one
+bool kept(Frames &z, PyObject *o, int64_t frames, const at::Tensor &like, int64_t rows)
+{
+    if (o == Py_None || o == Py_False) return true;
+    return z.output(o == Py_True ? Py_None : o, "z", frames, at::kBFloat16, like, rows);
+}
+
+// dense_forward(x, W, frames, bias, activation, residual, y, bf16, z) -> y, or (y, z)
+PyObject *dense_forward_body(PyObject *const *o)
+{
+    int frames, nodes, inputs, w_stride, act, bf16;
+    Place place;
+    bbcu_stream_t stream;
+    Frames x(place), residual(place), y(place), z(place);
+    Numbers bias(place);
+    const at::Tensor *W = parse(o[2], frames) && parse(o[4], act) && parse_flag(o[7], bf16) ? bf16_weights(o[1], place, w_stride) : nullptr;
+    if (!W || !fits(W->size(0), nodes) || !fits(W->size(1), inputs) || !bf16_operand(x, o[0], "x", frames, inputs) || !bias.input(o[3], "bias", nodes) ||
+        (o[6] != Py_None ? !y.take(o[6], "y", frames, nullptr, nodes) : !y.output(Py_None, "y", frames, bf16 ? at::kBFloat16 : at::kFloat, *x.t, nodes)) ||
+        (o[5] != Py_None && !residual.take(o[5], "residual", frames, y.t, nodes)) || !kept(z, o[8], frames, *x.t, nodes)) return nullptr;
+    const auto *in = static_cast<const bbcu_bf16_t *>(x.t->const_data_ptr()), *w = static_cast<const bbcu_bf16_t *>(W->const_data_ptr());
+    auto *zp = z.t ? z.out<bbcu_bf16_t *>() : nullptr;
+    if (!place.stream(stream) || BB200_CALL_OF_TYPE(y.fp32(), bbcu_bf16_fp32_DenseAffine_Forward, bbcu_bf16_DenseAffine_Forward, float, bbcu_bf16_t, in, w, bias.data,
+                           residual.t ? residual.in<const T *>() : nullptr, y.out<T *>(), zp, act, inputs, nodes, frames, w_stride, x.stride, residual.stride, y.stride,
+                           z.stride, stream)) return nullptr;
+    return z.t ? tuple_of(y.result(), z.result()) : y.result();
+}
+BB200_GUARDED(dense_forward, 9)
+
+// a call of one operator; a status, or INT_MIN with a Python error set
+#define BB200_CALL(name, ...)                                              \
+    [&] {                                                                  \
+        static decltype(&name) fn = nullptr;                               \
+        if (!bound(fn, #name)) return INT_MIN;                             \
+        int status = 0;                                                    \
+        Py_BEGIN_ALLOW_THREADS                                             \
+        status = fn(__VA_ARGS__);                                          \
+        Py_END_ALLOW_THREADS                                               \
+        if (status != 0) { raise_status(#name, status); return INT_MIN; }  \
+        return 0;                                                          \
+    }()
+
+// gated_dense_forward(x, W, frames, bias, activation, y, z) -> y, or (y, z)
+PyObject *gated_dense_forward_body(PyObject *const *o)
+{
+    int frames, rows, inputs, w_stride, act;
+    Place place;
+    bbcu_stream_t stream;
+    Frames x(place), y(place), z(place);
+    Numbers bias(place);
+    const at::Tensor *W = parse(o[2], frames) && parse(o[4], act) ? bf16_weights(o[1], place, w_stride) : nullptr;
+    if (!W || !fits(W->size(0), rows) || !fits(W->size(1), inputs)) return nullptr;
+    if (rows % 2) { refuse("W", "expected an even number of rows, the gate's and those that it multiplies"); return nullptr; }
+    if (!bf16_operand(x, o[0], "x", frames, inputs) || !bias.input(o[3], "bias", rows) || !y.output(o[5], "y", frames, at::kBFloat16, *x.t, rows / 2) ||
+        !kept(z, o[6], frames, *x.t, rows)) return nullptr;
+    if (!place.stream(stream) || BB200_CALL(bbcu_bf16_GatedDense_Forward, x.in<const bbcu_bf16_t *>(), static_cast<const bbcu_bf16_t *>(W->const_data_ptr()), bias.data,
+                           y.out<bbcu_bf16_t *>(), z.t ? z.out<bbcu_bf16_t *>() : nullptr, act, inputs, rows / 2, frames, w_stride, x.stride, y.stride, z.stride,
+                           stream)) return nullptr;
+    return z.t ? tuple_of(y.result(), z.result()) : y.result();
+}
+BB200_GUARDED(gated_dense_forward, 7)
+
+// dense_backward_input(dy, W, frames, z, activation, gated, dx) -> dx
+PyObject *dense_backward_input_body(PyObject *const *o)
+{
+    int frames, nodes, inputs, w_stride, act, gated;
+    Place place;
+    bbcu_stream_t stream;
+    Frames dy(place), z(place), dx(place);
+    const at::Tensor *W = parse(o[2], frames) && parse(o[4], act) && parse_flag(o[5], gated) ? bf16_weights(o[1], place, w_stride) : nullptr;
+    if (!W || !fits(W->size(0), nodes) || !fits(W->size(1), inputs) || !bf16_operand(dy, o[0], "dy", frames, nodes)) return nullptr;
+    if (gated && o[3] == Py_None) { refuse("z", "a gated block's gradient needs what its forward pass kept"); return nullptr; }
+    const int64_t rows = gated ? 2 * (int64_t)inputs : inputs;
+    if ((o[3] != Py_None && !z.take(o[3], "z", frames, dy.t, rows)) || !dx.output(o[6], "dx", frames, at::kBFloat16, *dy.t, rows)) return nullptr;
+    if (!place.stream(stream) || BB200_CALL(bbcu_bf16_DenseAffine_BackwardInput, dy.in<const bbcu_bf16_t *>(), static_cast<const bbcu_bf16_t *>(W->const_data_ptr()),
+                           z.t ? z.in<const bbcu_bf16_t *>() : nullptr, dx.out<bbcu_bf16_t *>(), act, gated, inputs, nodes, frames, w_stride, dy.stride, z.stride,
+                           dx.stride, stream)) return nullptr;
+    return dx.result();
+}
+BB200_GUARDED(dense_backward_input, 7)
+
+// dense_backward_weights(x, dy, frames, dW, dbias) -> (dW, dbias); given ones are added to; dW alone: no dbias
+PyObject *dense_backward_weights_body(PyObject *const *o)
+{
+    int frames, nodes, inputs;
+    Place place;
+    bbcu_stream_t stream;
+    Frames x(place), dy(place);
+    Numbers dW(place), dbias(place);
+    if (!parse(o[2], frames) || !bf16_operand(x, o[0], "x", frames, -1) || !bf16_operand(dy, o[1], "dy", frames, -1) || !fits(x.t->size(0), inputs) ||
+        !fits(dy.t->size(0), nodes)) return nullptr;
+    const int accumulate = o[3] != Py_None;
+    if (!accumulate && o[4] != Py_None) { refuse("dbias", "given without dW"); return nullptr; }
+    if (accumulate) {
+        if (!dW.check(o[3], "dW", (int64_t)nodes * inputs, true) || (o[4] != Py_None && !dbias.check(o[4], "dbias", nodes, true))) return nullptr;
+        const at::Tensor &t = THPVariable_Unpack(o[3]);
+        if (t.dim() != 2 || t.size(0) != nodes || t.size(1) != inputs) { refuse("dW", "expected [outputs, inputs]"); return nullptr; }
+    } else {
+        if (!place.here()) return nullptr;
+        dW.made = at::empty({nodes, inputs}, at::TensorOptions().dtype(at::kFloat).device(x.t->device()));
+        dW.data = static_cast<float *>(dW.made.mutable_data_ptr());
+        if (!dbias.output(Py_None, "dbias", nodes, *x.t)) return nullptr;
+    }
+    if (!place.stream(stream) || BB200_CALL(bbcu_bf16_DenseAffine_BackwardWeights, x.in<const bbcu_bf16_t *>(), dy.in<const bbcu_bf16_t *>(), dW.data, dbias.data, accumulate,
+                           inputs, nodes, frames, x.stride, dy.stride, inputs, stream)) return nullptr;
+    return tuple_of(dW.result(), dbias.data || !accumulate ? dbias.result() : Py_NewRef(Py_None));
+}
+BB200_GUARDED(dense_backward_weights, 5)
+
 #define BB200_METHOD(name, function) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(function)), METH_FASTCALL, nullptr},
 #define BB200_OPERATOR_METHOD(name) BB200_METHOD(#name, py_##name)
 PyMethodDef g_methods[] = {
@@ -577,6 +775,9 @@ PyMethodDef g_methods[] = {
     BB200_METHOD("train_forward", train_forward) BB200_METHOD("train_backward", train_backward)
     BB200_METHOD("layer_norm_forward", layer_norm_forward) BB200_METHOD("layer_norm_backward", layer_norm_backward) BB200_METHOD("quantize_int8", quantize_int8)
     BB200_METHOD("int8_dense_forward", int8_dense_forward) BB200_METHOD("distillation_loss", distillation_loss)
+    BB200_METHOD("dense_forward", dense_forward) BB200_METHOD("gated_dense_forward", gated_dense_forward) BB200_METHOD("dense_backward_input", dense_backward_input)
+    BB200_METHOD("dense_backward_weights", dense_backward_weights) BB200_METHOD("rms_norm_forward", rms_norm_forward) BB200_METHOD("rms_norm_int8", rms_norm_int8)
+    BB200_METHOD("rms_norm_backward", rms_norm_backward) BB200_METHOD("scalar_f32", scalar_f32)
     {nullptr, nullptr, 0, nullptr}};
 #undef BB200_METHOD
 

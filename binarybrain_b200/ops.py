@@ -45,6 +45,19 @@ def _chk(t, dtype, name):
     return t
 
 
+def _current_device(t):
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _one_device(tensors):
+    devices = {t.device for t in tensors}
+    if len(devices) > 1:
+        raise ValueError(f"expected tensors of one device, got {', '.join(sorted(map(str, devices)))}")
+    if any(t.numel() > 0x7fffffff for t in tensors):
+        raise OverflowError("a size does not fit the operator")
+
+
 def fp32_stride(frames):
     """Row stride in floats: rows padded to 32 bytes (include/bb/FrameBuffer.h:414-417)."""
     return (frames + 7) // 8 * 8
@@ -356,10 +369,18 @@ def maxpool_backward(sel, dy, frames, c, h, w, fh, fw, bit_input=False):
 
 
 class Adam:
-    """bb::OptimizerAdam over a list of (param, grad) CUDA tensors (include/bb/OptimizerAdam.h:142-184)."""
+    """bb::OptimizerAdam over a list of (param, grad) CUDA tensors (include/bb/OptimizerAdam.h:142-184).  max_norm: the step is made with gradients clipped to
+    that global norm, and step() and update() return the norm before clipping, a scalar on the device."""
 
-    def __init__(self, params, grads, lr=0.001, beta1=0.9, beta2=0.999):
-        self.params, self.grads = list(params), list(grads)
+    def __init__(self, params, grads, lr=0.001, beta1=0.9, beta2=0.999, max_norm=None):
+        self.params, self.grads, self.max_norm = list(params), list(grads), max_norm
+        if max_norm is not None:
+            if not max_norm >= 0:
+                raise ValueError(f"max_norm: expected a number that is not negative, got {max_norm}")
+            for p, g in zip(self.params, self.grads, strict=True):
+                if _chk(p, torch.float32, "params").shape != _chk(g, torch.float32, "grads").shape:
+                    raise ValueError(f"grads: expected the shape of the parameter, {tuple(p.shape)}, got {tuple(g.shape)}")
+            _one_device(self.params + self.grads)
         self.m = [torch.zeros_like(p) for p in self.params]
         self.v = [torch.zeros_like(p) for p in self.params]
         dev = self.params[0].device
@@ -369,21 +390,56 @@ class Adam:
         self.lr, self.beta1, self.beta2 = lr, beta1, beta2
         self.b1, self.b2 = beta1, beta2
 
-    def _step(self, operator):
+    def _step(self, operator, clear=0):
         lr_t = self.lr * (1.0 - self.b2) ** 0.5 / (1.0 - self.b1)
-        operator(len(self.params), self._sizes, *self._tabs, lr_t, self.beta1, self.beta2)
+        norm = None
+        if self.max_norm is None:
+            operator(len(self.params), self._sizes, *self._tabs, lr_t, self.beta1, self.beta2)
+        else:
+            _current_device(self._sizes)
+            norm = _n.scalar_f32(self._sizes)
+            _n.bbcu_fp32_OptimizerAdamClipped(len(self.params), self._sizes, *self._tabs, lr_t, self.beta1, self.beta2, self.max_norm, norm, clear)
         self.b1 *= self.beta1
         self.b2 *= self.beta2
+        return norm
 
     def step(self):
-        self._step(_n.bbcu_fp32_OptimizerAdam)
+        return self._step(_n.bbcu_fp32_OptimizerAdam)
 
     def zero_grad(self):
         for g in self.grads:
             g.zero_()
 
     def update(self):          # Optimizer::Update = Step + ZeroGrad (include/bb/Optimizer.h:29-33), one pass over the tables
-        self._step(_n.bbcu_fp32_OptimizerAdamUpdate)
+        return self._step(_n.bbcu_fp32_OptimizerAdamUpdate, clear=1)
+
+
+class GradientNorm:
+    """The global norm of a list of fp32 CUDA tensors, sqrt of the sum of all squares (added up in 64 bits), and clipping by it.  The tensors are the ones
+    given here, whatever they hold when it is called."""
+
+    def __init__(self, grads):
+        self.grads = [_chk(g, torch.float32, "grads") for g in grads]
+        if not self.grads:
+            raise ValueError("grads: expected at least one tensor")
+        _one_device(self.grads)
+        dev = self.grads[0].device
+        self._sizes = torch.tensor([g.numel() for g in self.grads], dtype=torch.int32, device=dev)
+        self._table = torch.tensor([g.data_ptr() for g in self.grads], dtype=torch.int64, device=dev)
+
+    def norm(self):
+        """The norm, a scalar on the device."""
+        _current_device(self._sizes)
+        norm = _n.scalar_f32(self._sizes)
+        _n.bbcu_fp32_GradientNorm(len(self.grads), self._sizes, self._table, norm)
+        return norm
+
+    def clip_(self, max_norm):
+        """Multiplies all of them by max_norm / norm where the norm is above max_norm (a norm that is NaN clips nothing); returns the norm before."""
+        _current_device(self._sizes)
+        norm = _n.scalar_f32(self._sizes)
+        _n.bbcu_fp32_GradientClip(len(self.grads), self._sizes, self._table, max_norm, norm)
+        return norm
 
 
 # ------------------------------------------------------------------------------------------ the dense teacher beside a LUT network
@@ -438,6 +494,66 @@ def distillation_loss(z, t, index, frames, temperature=1.0, t_lse=None, weight=N
     probabilities are those among its slots or, with t_lse [frames] = log sum exp(t / temperature) over all of its classes, the true ones.  Returns
     (dz, loss, loss_buf): the gradient of loss, the mean over batch_size frames (default: these), and weight * loss of every frame."""
     return _n.distillation_loss(z, t, index, frames, temperature, t_lse, weight, batch_size, dz, loss_buf)
+
+
+# ------------------------------------------------------------------------------------------ training and serving that teacher in bf16
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _activation(name):
+    try:
+        return ACTIVATIONS["none" if name is None else name]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation: expected one of {', '.join(ACTIVATIONS)}, got {name!r}") from None
+
+
+def rms_norm_forward(x, frames, gamma=None, eps=1e-5, residual=None, y=None, s=None, rstd=None):
+    """Root-mean-square norm over the nodes of every frame of s = x + residual, which is kept in x's type (without a residual s is x): returns (y, s, rstd),
+    y = s * rstd * gamma, rstd [frames] fp32.  A given s may be x or residual itself."""
+    return _n.rms_norm_forward(x, frames, gamma, eps, residual, y, s, rstd)
+
+
+def rms_norm_int8(x, frames, gamma=None, eps=1e-5, residual=None, s=None):
+    """The same with y as rows of 8-bit integers, as int8_dense_forward reads them: returns (q [frames, int8_stride(nodes)], scale [frames], s)."""
+    return _n.rms_norm_int8(x, frames, gamma, eps, residual, s)
+
+
+def rms_norm_backward(s, dy, rstd, frames, gamma=None, dresidual=None, ds=None, dgamma=None):
+    """Returns (ds, dgamma): ds the gradient of s through y, plus dresidual, the one that arrives by the other path.  A given dgamma is added to."""
+    return _n.rms_norm_backward(s, dy, rstd, frames, gamma, dresidual, ds, dgamma)
+
+
+def dense_weights(W):
+    """W [out, in] as the dense products read it: bf16, in rows that start on 16-byte boundaries.  Done once, when a network is loaded, or after a step."""
+    buf = torch.zeros((W.shape[0], (W.shape[1] + 7) // 8 * 8), dtype=torch.bfloat16, device=W.device)
+    buf[:, :W.shape[1]] = W
+    return buf[:, :W.shape[1]]
+
+
+def dense_forward(x, W, frames, bias=None, activation=None, residual=None, y=None, dtype=torch.bfloat16, keep=False):
+    """y = activation(W x + bias) + residual as a frame buffer of `dtype` (bf16 or fp32).  x [in, frame_stride] and W [out, in] bf16 in rows on 16-byte
+    boundaries, bias [out] fp32, residual in y's type, activation none, relu, gelu or silu.  keep: True, or a bf16 buffer for it: z = W x + bias, which the
+    gradient of an activation needs, is returned as well."""
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"dtype: expected float32 or bfloat16, got {dtype}")
+    return _n.dense_forward(x, W, frames, bias, _activation(activation), residual, y, dtype == torch.bfloat16, keep)
+
+
+def gated_dense_forward(x, W, frames, bias=None, activation="silu", y=None, keep=False):
+    """The gated block y = activation(g) * u, g and u the upper and the lower half of W x + bias (W [2 * out, in], bias [2 * out]), bf16.  keep: True, or a buffer
+    [2 * out, frame_stride] for it: z, g above u, which the block's gradient needs, is returned as well."""
+    return _n.gated_dense_forward(x, W, frames, bias, _activation(activation), y, keep)
+
+
+def dense_backward_input(dy, W, frames, z=None, activation=None, gated=False, dx=None):
+    """dx = W^T dy, bf16.  Where the layer's input was activation(z): with z given, the gradient of z.  Where it was a gated block's output: with that block's z
+    and gated=True, the gradient of that z, [2 * in, frame_stride]."""
+    return _n.dense_backward_input(dy, W, frames, z, _activation(activation), bool(gated), dx)
+
+
+def dense_backward_weights(x, dy, frames, dW=None, dbias=None):
+    """Returns (dW, dbias), fp32: dW [out, in] = dy x^T, dbias [out] = the sums of dy's rows.  Given ones are added to; with dW alone given there is no dbias."""
+    return _n.dense_backward_weights(x, dy, frames, dW, dbias)
 
 
 # ------------------------------------------------------------------------------------------ frame-sharded halves

@@ -1,4 +1,4 @@
-"""Layers of the dense teacher beside a LUT network, and the normalised head of a student that learns from it.
+"""Layers of the dense teacher beside a LUT network, to train it and to serve it, and the normalised head of a student that learns from it.
 
 No counterpart in the reference.  Like the other layers here they have ``forward(x, frames, total_frames)`` on CUDA frame buffers [nodes, stride], fp32
 or bf16; the arithmetic is that of the bbcu_* operators (``ops``), there is no CPU path behind it.
@@ -39,8 +39,127 @@ class Int8Dense:
         self.bias = bias
 
     def forward(self, x, frames, total_frames=None, y=None):
-        q, scale = ops.quantize_int8(x, frames)
+        return self.forward_int8(*ops.quantize_int8(x, frames), y=y)
+
+    def forward_int8(self, q, scale, y=None):
+        """On frames that come as 8-bit integers already."""
         return ops.int8_dense_forward(q, scale, self.W, self.w_scale, n_in=self.n_in, bias=self.bias, y=y, dtype=self.dtype)
+
+
+class RmsNormalization:
+    """Root-mean-square norm over the nodes of a frame with a learned scale a node, and the residual's addition before it.  forward() returns (y, s): s = x +
+    residual is what the next residual goes on from; backward() takes the gradients of both."""
+
+    def __init__(self, nodes, eps=1e-5, gamma=1.0, device="cuda"):
+        self.n_out, self.eps = nodes, eps
+        self.gamma = torch.full((nodes,), float(gamma), device=device)
+        self.dgamma = torch.zeros_like(self.gamma)
+        self._saved = None
+
+    def parameters(self):
+        return [(self.gamma, self.dgamma)]
+
+    def forward(self, x, frames, total_frames=None, residual=None, y=None):
+        y, s, rstd = ops.rms_norm_forward(x, frames, gamma=self.gamma, eps=self.eps, residual=residual, y=y)
+        self._saved = s, rstd, frames
+        return y, s
+
+    def forward_int8(self, x, frames, residual=None):
+        """For serving: returns (q, scale, s), q and scale as Int8Dense.forward_int8 takes them."""
+        return ops.rms_norm_int8(x, frames, gamma=self.gamma, eps=self.eps, residual=residual)
+
+    def backward(self, dy, ds=None, out=None):
+        s, rstd, frames = self._saved
+        self._saved = None
+        return ops.rms_norm_backward(s, dy, rstd, frames, gamma=self.gamma, dresidual=ds, ds=out, dgamma=self.dgamma)[0]
+
+
+class DenseAffine:
+    """A dense layer in bf16: activation(W x + bias) + residual.  The weights that are trained are fp32; refresh() lays them out in bf16 as the product reads
+    them, after they have changed.  backward() returns the gradient of x and adds to dW and dbias; the residual's gradient is dy itself."""
+
+    def __init__(self, W, bias=None, activation=None, dtype=torch.bfloat16):
+        self.n_in, self.n_out, self.activation, self.dtype = W.shape[1], W.shape[0], activation, dtype
+        self.W, self.bias = W.float().contiguous(), bias
+        self.dW, self.dbias = torch.zeros_like(self.W), None if bias is None else torch.zeros_like(bias)
+        self.W16 = ops.dense_weights(self.W)
+        self._saved = None
+
+    def parameters(self):
+        return [(self.W, self.dW)] + ([] if self.bias is None else [(self.bias, self.dbias)])
+
+    def refresh(self):
+        self.W16.copy_(self.W)
+
+    def forward(self, x, frames, total_frames=None, residual=None, y=None, train=True):
+        keep = train and self.activation not in (None, "none")
+        y = ops.dense_forward(x, self.W16, frames, bias=self.bias, activation=self.activation, residual=residual, y=y, dtype=self.dtype, keep=keep)
+        y, z = y if keep else (y, None)
+        self._saved = (x, z, frames) if train else None
+        return y
+
+    def backward(self, dy, dx=None, below=None):
+        """dy: the gradient of y, or, for a layer with an activation, of z: what the layer above returns when this one is its `below`.  below: the layer whose
+        output x is; where that has an activation or is gated, the gradient of its z is returned."""
+        x, _, frames = self._saved
+        ops.dense_backward_weights(x, dy, frames, dW=self.dW, dbias=self.dbias)
+        z, activation, gated = below.kept() if below is not None else (None, None, False)
+        dx = ops.dense_backward_input(dy, self.W16, frames, z=z, activation=activation, gated=gated, dx=dx)
+        self._saved = None
+        return dx
+
+    def kept(self):
+        return self._saved[1], self.activation, False
+
+
+class GatedDense(DenseAffine):
+    """The gated block: activation(g) * u, g and u the upper and the lower half of W x + bias.  backward() takes the gradient of both, as the layer above
+    returns it when this one is its `below`."""
+
+    def __init__(self, W, bias=None, activation="silu"):
+        super().__init__(W, bias, activation)
+        self.n_out //= 2
+
+    def forward(self, x, frames, total_frames=None, y=None, train=True):
+        y = ops.gated_dense_forward(x, self.W16, frames, bias=self.bias, activation=self.activation, y=y, keep=train)
+        y, z = y if train else (y, None)
+        self._saved = (x, z, frames) if train else None
+        return y
+
+    def kept(self):
+        return self._saved[1], self.activation, True
+
+
+class FeedForward:
+    """Norm, gated block and dense layer of a residual stream: forward(x, frames, residual) returns (y, s), s = x + residual and y what is to be added to it by
+    the next norm; backward(dy, ds) returns the gradient of s, which is that of x and of the residual."""
+
+    def __init__(self, nodes, hidden, generator=None, activation="silu", device="cuda"):
+        def weights(rows, inputs):
+            return torch.randn((rows, inputs), device=device, generator=generator) / inputs ** 0.5
+        self.norm = RmsNormalization(nodes, device=device)
+        self.gated = GatedDense(weights(2 * hidden, nodes), activation=activation)
+        self.dense = DenseAffine(weights(nodes, hidden))
+
+    def parameters(self):
+        return self.norm.parameters() + self.gated.parameters() + self.dense.parameters()
+
+    def refresh(self):
+        self.gated.refresh()
+        self.dense.refresh()
+
+    def forward(self, x, frames, residual=None, train=True):
+        n, s = self.norm.forward(x, frames, residual=residual)
+        return self.dense.forward(self.gated.forward(n, frames, train=train), frames, train=train), s
+
+    def backward(self, dy, ds=None):
+        return self.norm.backward(self.gated.backward(self.dense.backward(dy, below=self.gated)), ds)
+
+
+def clipped_adam(layers, max_norm, **kw):
+    """Adam over all parameters of `layers`, clipped by the global norm of their gradients; call refresh() of the layers after its update()."""
+    pairs = [pair for layer in layers for pair in layer.parameters()]
+    return ops.Adam([p for p, _ in pairs], [g for _, g in pairs], max_norm=max_norm, **kw)
 
 
 def top_logits(logits, frames, top, stride=None):

@@ -436,6 +436,74 @@ int bbcu_bf16_LossDistillation(const bbcu_bf16_t *dev_z_buf, bbcu_bf16_t *dev_dz
                                float grad_reduction, double loss_reduction, int class_size, int top_size, int frame_size, int z_frame_stride,
                                int dz_frame_stride, int t_frame_stride, int index_frame_stride, bbcu_stream_t stream);
 
+/* ------------------------------------------------------------------ Additive: training and serving that teacher in bf16.
+ * No counterparts in the reference.  The rules of the section above hold; each output is rounded once, from 32 bits.  The products' operands are read by
+ * TMA: rows of W, x and dy start on 16-byte boundaries (strides in elements, multiples of 8; BBCU_ERR_BAD_STRIDE otherwise), what lies in their padding is
+ * not used.  The other buffers may have any stride and alignment.  Extents up to 2^27, BBCU_ERR_TOO_LARGE beyond. */
+#define BBCU_ACTIVATION_NONE 0
+#define BBCU_ACTIVATION_RELU 1
+#define BBCU_ACTIVATION_GELU 2          /* z * (1 + erf(z / sqrt 2)) / 2 */
+#define BBCU_ACTIVATION_SILU 3          /* z / (1 + exp(-z)) */
+
+/* z = W x + bias (dev_bias [output_node_size] may be NULL), y = activation(z) + residual (dev_residual_buf may be NULL); z is kept where dev_z_buf is given,
+ * as the gradient of an activation needs it.  W [output][input]. */
+int bbcu_bf16_DenseAffine_Forward(const bbcu_bf16_t *dev_x_buf, const bbcu_bf16_t *dev_W, const float *dev_bias, const bbcu_bf16_t *dev_residual_buf,
+                                  bbcu_bf16_t *dev_y_buf, bbcu_bf16_t *dev_z_buf, int activation, int input_node_size, int output_node_size, int frame_size,
+                                  int w_node_stride, int x_frame_stride, int residual_frame_stride, int y_frame_stride, int z_frame_stride, bbcu_stream_t stream);
+/* the same with residual and y in fp32 */
+int bbcu_bf16_fp32_DenseAffine_Forward(const bbcu_bf16_t *dev_x_buf, const bbcu_bf16_t *dev_W, const float *dev_bias, const float *dev_residual_buf, float *dev_y_buf,
+                                       bbcu_bf16_t *dev_z_buf, int activation, int input_node_size, int output_node_size, int frame_size, int w_node_stride,
+                                       int x_frame_stride, int residual_frame_stride, int y_frame_stride, int z_frame_stride, bbcu_stream_t stream);
+/* The gated block: g = (W x)[n], u = (W x)[output_node_size + n], W [2 * output][input] (dev_bias [2 * output] may be NULL): y = activation(g) * u.  z [2 * output]
+ * rows, g above u, is kept where dev_z_buf is given. */
+int bbcu_bf16_GatedDense_Forward(const bbcu_bf16_t *dev_x_buf, const bbcu_bf16_t *dev_W, const float *dev_bias, bbcu_bf16_t *dev_y_buf, bbcu_bf16_t *dev_z_buf,
+                                 int activation, int input_node_size, int output_node_size, int frame_size, int w_node_stride, int x_frame_stride,
+                                 int y_frame_stride, int z_frame_stride, bbcu_stream_t stream);
+/* dx = W^T dy.  With dev_z_buf [input_node_size] rows, of which the layer's input was the activation: times activation'(z), the gradient of z.  With gated != 0,
+ * dev_z_buf [2 * input] rows of a gated block whose output was the layer's input: dx [2 * input] rows are the gradients of that block's z. */
+int bbcu_bf16_DenseAffine_BackwardInput(const bbcu_bf16_t *dev_dy_buf, const bbcu_bf16_t *dev_W, const bbcu_bf16_t *dev_z_buf, bbcu_bf16_t *dev_dx_buf, int activation,
+                                        int gated, int input_node_size, int output_node_size, int frame_size, int w_node_stride, int dy_frame_stride,
+                                        int z_frame_stride, int dx_frame_stride, bbcu_stream_t stream);
+/* dW [output][dw_node_stride] = dy x^T and dbias [output] = the sums of dy's rows (either may be NULL), with accumulate != 0 added to what is there. */
+int bbcu_bf16_DenseAffine_BackwardWeights(const bbcu_bf16_t *dev_x_buf, const bbcu_bf16_t *dev_dy_buf, float *dev_dW, float *dev_dbias, int accumulate,
+                                          int input_node_size, int output_node_size, int frame_size, int x_frame_stride, int dy_frame_stride, int dw_node_stride,
+                                          bbcu_stream_t stream);
+
+/* Root-mean-square norm over the nodes of a frame with the residual's addition: s = x + residual, kept in the frames' type in dev_s_buf (dev_residual_buf NULL:
+ * s = x, and dev_s_buf is not used); rstd [frame_size] = 1 / sqrt(mean s^2 + eps); y = s * rstd * gamma.  dev_gamma [node_size], NULL: 1.  dev_s_buf may be
+ * dev_x_buf or dev_residual_buf itself.  Any stride and alignment; up to 2^20 nodes and 2^27 frames, BBCU_ERR_TOO_LARGE beyond. */
+int bbcu_fp32_RmsNormalization_Forward(const float *dev_x_buf, const float *dev_residual_buf, float *dev_s_buf, float *dev_y_buf, const float *dev_gamma,
+                                       float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride, int residual_frame_stride,
+                                       int s_frame_stride, int y_frame_stride, bbcu_stream_t stream);
+int bbcu_bf16_RmsNormalization_Forward(const bbcu_bf16_t *dev_x_buf, const bbcu_bf16_t *dev_residual_buf, bbcu_bf16_t *dev_s_buf, bbcu_bf16_t *dev_y_buf,
+                                       const float *dev_gamma, float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride,
+                                       int residual_frame_stride, int s_frame_stride, int y_frame_stride, bbcu_stream_t stream);
+/* The same with y as the int8 product's rows (see QuantizeInt8_Frames): t = s * gamma in 32 bits, u = max|t| / 127, q = t / u rounded to the nearest integer,
+ * ties to even, scale = u * rstd.  dev_rstd_buf may be NULL. */
+int bbcu_fp32_RmsNormalization_QuantizeInt8(const float *dev_x_buf, const float *dev_residual_buf, float *dev_s_buf, signed char *dev_q_buf, float *dev_scale_buf,
+                                            const float *dev_gamma, float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride,
+                                            int residual_frame_stride, int s_frame_stride, int q_node_stride, bbcu_stream_t stream);
+int bbcu_bf16_RmsNormalization_QuantizeInt8(const bbcu_bf16_t *dev_x_buf, const bbcu_bf16_t *dev_residual_buf, bbcu_bf16_t *dev_s_buf, signed char *dev_q_buf,
+                                            float *dev_scale_buf, const float *dev_gamma, float *dev_rstd_buf, float eps, int node_size, int frame_size,
+                                            int x_frame_stride, int residual_frame_stride, int s_frame_stride, int q_node_stride, bbcu_stream_t stream);
+/* ds = the gradient of s through y, plus dev_dresidual_buf (may be NULL), the one that arrives by the other path; dgamma [node_size] (may be NULL)
+ * overwritten, or with accumulate != 0 added to. */
+int bbcu_fp32_RmsNormalization_Backward(const float *dev_s_buf, const float *dev_dy_buf, const float *dev_dresidual_buf, float *dev_ds_buf, const float *dev_gamma,
+                                        const float *dev_rstd_buf, float *dev_dgamma, int accumulate, int node_size, int frame_size, int s_frame_stride,
+                                        int dy_frame_stride, int dresidual_frame_stride, int ds_frame_stride, bbcu_stream_t stream);
+int bbcu_bf16_RmsNormalization_Backward(const bbcu_bf16_t *dev_s_buf, const bbcu_bf16_t *dev_dy_buf, const bbcu_bf16_t *dev_dresidual_buf, bbcu_bf16_t *dev_ds_buf,
+                                        const float *dev_gamma, const float *dev_rstd_buf, float *dev_dgamma, int accumulate, int node_size, int frame_size,
+                                        int s_frame_stride, int dy_frame_stride, int dresidual_frame_stride, int ds_frame_stride, bbcu_stream_t stream);
+
+/* The global norm of `size` gradients, tables as for the optimizer above: *dev_norm = sqrt(sum of all squares), which are added up in 64 bits. */
+int bbcu_fp32_GradientNorm(int size, const int *dev_size_table, float *const *dev_grads_buf_table, float *dev_norm, bbcu_stream_t stream);
+/* The same, and where the norm is above max_norm (>= 0) all gradients are multiplied by max_norm / norm.  A norm that is NaN clips nothing. */
+int bbcu_fp32_GradientClip(int size, const int *dev_size_table, float *const *dev_grads_buf_table, float max_norm, float *dev_norm, bbcu_stream_t stream);
+/* The optimizer's step on gradients that are clipped on the way: they stay as they are, or with clear_grads != 0 are cleared.  *dev_norm: before clipping. */
+int bbcu_fp32_OptimizerAdamClipped(int size, const int *dev_size_table, float *const *dev_params_buf_table, float *const *dev_grads_buf_table,
+                                   float *const *dev_m_buf_table, float *const *dev_v_buf_table, float lr_t, float beta1, float beta2, float max_norm,
+                                   float *dev_norm, int clear_grads, bbcu_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
