@@ -10,6 +10,8 @@
 // x, W, dy and the kept z are bf16; the sums are 32 bits, bias, activation, residual and gate are applied to them in 32 bits, and each output is rounded once.
 // Frame buffers are read as they lie, frames next to each other: where the product sums over nodes, its operand is "across" (rows of shared memory along
 // the frames), which the tensor cores take from TMA's 128-byte swizzled boxes as well as rows along k; the gradients read W and x the other way round, and nothing is transposed.
+#include <type_traits>
+
 #include <cuda.h>
 
 #include "async_copy.cuh"
@@ -20,7 +22,6 @@ namespace bb200 {
 
 enum DenseKind { kForward, kGated, kInputGrad, kWeightGrad };
 
-constexpr int kDenseThreads = 320, kDenseWarps = 8;      // warp 0 copies, warp 1 issues the products, eight warps take the sums out of TMEM
 constexpr int kTileM = 128, kTileK = 64;                 // output rows of a CTA; k of a stage (128 bytes)
 constexpr int kMostSplits = 8;
 constexpr int kTileGroup = 8;                            // tiles of output rows that are walked together, so that their operands stay in L2
@@ -36,31 +37,54 @@ struct DenseArgs {
     int *fault;
 };
 
-// ---- activations, in 32 bits.  gelu is z times the normal distribution's integral, through erfc, which keeps its digits where that is small; the logistic
-// function's divisor is between 1 and 2.
-__device__ __forceinline__ float logistic(float z)
+// ---- activations, in 32 bits: value and slope, of which the compiler keeps what is used.  FAST, for outputs of 16 bits: exp(x) by the special function unit,
+// whose argument is rounded, so that it is off by |x| + 2 half-units in the last place of 32 bits; 88 at most.
+struct Curve { float value, slope; };
+
+template <bool FAST> __device__ __forceinline__ float exp_of(float x) { return FAST ? __expf(x) : expf(x); }
+
+template <bool FAST> __device__ __forceinline__ Curve silu(float z)
 {
-    const float e = expf(-fabsf(z)), inv = __fdividef(1.0f, 1.0f + e);
-    return z < 0.0f ? e * inv : inv;
+    // (the divisor is between 1 and 2)
+    const float e = exp_of<FAST>(-fabsf(z)), inv = __fdividef(1.0f, 1.0f + e), rest = e * inv, p = z < 0.0f ? rest : inv;
+    return {z * p, fmaf(z, rest * inv, p)};
 }
 
-__device__ __forceinline__ float activate(float z, int act)
+// gelu = z Phi(z), slope = Phi(z) + z phi(z).  Phi(-|z|) exp(z^2 / 2) is t times a polynomial in t = 1 / (1 + 0.35 |z|), fitted to 0.5 erfcx(|z| / sqrt 2) / t over
+// |z| <= 14 by weighted least squares to 3.2e-8 of its value, so that the digits stay where Phi is small; gelu is off by 11 half-units in the last place for |z| < 3,
+// and by those of the exponent's rounding beyond.  (erfcf takes three times the operations, which were half of the time of a product of 1024 inputs.)
+template <bool FAST> __device__ __forceinline__ Curve gelu(float z)
 {
-    switch (act) {
-    case BBCU_ACTIVATION_RELU: return fmaxf(z, 0.0f) + (z != z ? z : 0.0f);
-    case BBCU_ACTIVATION_GELU: return 0.5f * z * erfcf(z * -0.70710678f);
-    case BBCU_ACTIVATION_SILU: return z * logistic(z);
-    default: return z;
-    }
+    const float a = fabsf(z), t = __fdividef(1.0f, fmaf(0.35f, a, 1.0f)), e = FAST ? __expf(-0.5f * z * z) : exp2f(-0.72134752f * z * z);
+    float p = -0.029145934f;
+    p = fmaf(p, t, 0.14397171f);
+    p = fmaf(p, t, -0.25571427f);
+    p = fmaf(p, t, 0.15917419f);
+    p = fmaf(p, t, -0.02310985f);
+    p = fmaf(p, t, 0.10550801f);
+    p = fmaf(p, t, 0.119832866f);
+    p = fmaf(p, t, 0.13986187f);
+    p = fmaf(p, t, 0.1396214f);
+    const float q = t * p * e, phi = z < 0.0f ? q : 1.0f - q;
+    return {z * phi, fmaf(z * 0.39894228f, e, phi)};
 }
 
-__device__ __forceinline__ float activation_slope(float z, int act)
+template <int ACT, bool FAST> __device__ __forceinline__ Curve curve(float z)
+{
+    if constexpr (ACT == BBCU_ACTIVATION_RELU) return {z < 0.0f ? 0.0f : z, z > 0.0f ? 1.0f : z != z ? z : 0.0f};
+    if constexpr (ACT == BBCU_ACTIVATION_GELU) return gelu<FAST>(z);
+    if constexpr (ACT == BBCU_ACTIVATION_SILU) return silu<FAST>(z);
+    return {z, 1.0f};
+}
+
+// f(std::integral_constant<int, act>): the activation is one for all of a call
+template <typename F> __device__ __forceinline__ void with_activation(int act, F f)
 {
     switch (act) {
-    case BBCU_ACTIVATION_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
-    case BBCU_ACTIVATION_GELU: return fmaf(z * 0.39894228f, expf(-0.5f * z * z), 0.5f * erfcf(z * -0.70710678f));
-    case BBCU_ACTIVATION_SILU: return logistic(z) * fmaf(z, logistic(-z), 1.0f);
-    default: return 1.0f;
+    case BBCU_ACTIVATION_RELU: f(std::integral_constant<int, BBCU_ACTIVATION_RELU>()); break;
+    case BBCU_ACTIVATION_GELU: f(std::integral_constant<int, BBCU_ACTIVATION_GELU>()); break;
+    case BBCU_ACTIVATION_SILU: f(std::integral_constant<int, BBCU_ACTIVATION_SILU>()); break;
+    default: f(std::integral_constant<int, BBCU_ACTIVATION_NONE>()); break;
     }
 }
 
@@ -110,10 +134,10 @@ template <int KIND, typename T, int V> __device__ __forceinline__ void finish(co
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] += b;
         if (a.z_out) store_some<B, V>(static_cast<B *>(a.z_out) + (long long)m * a.z_stride + n, v);
-        if (a.act != BBCU_ACTIVATION_NONE) {
+        with_activation(a.act, [&](auto act) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = activate(v[j], a.act);
-        }
+            for (int j = 0; j < V; ++j) v[j] = curve<decltype(act)::value, sizeof(T) == 2>(v[j]).value;
+        });
         if (a.extra) {
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] += r[j];
@@ -123,7 +147,11 @@ template <int KIND, typename T, int V> __device__ __forceinline__ void finish(co
         const float b = a.bias ? a.bias[m] : 0.0f, c = a.bias ? a.bias[a.half + m] : 0.0f;
         float y[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) { v[j] += b; w[j] += c; y[j] = activate(v[j], a.act) * w[j]; }
+        for (int j = 0; j < V; ++j) { v[j] += b; w[j] += c; }
+        with_activation(a.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) y[j] = curve<decltype(act)::value, sizeof(T) == 2>(v[j]).value * w[j];
+        });
         store_some<T, V>(out, y);
         if (a.z_out) {
             store_some<B, V>(static_cast<B *>(a.z_out) + (long long)m * a.z_stride + n, v);
@@ -135,19 +163,24 @@ template <int KIND, typename T, int V> __device__ __forceinline__ void finish(co
             float g[V], u[V], d[V];
             load_some<B, V>(z, g);
             load_some<B, V>(z + (long long)a.half * a.extra_stride, u);
+            with_activation(a.act, [&](auto act) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                d[j] = v[j] * activate(g[j], a.act);
-                v[j] *= u[j] * activation_slope(g[j], a.act);
-            }
+                for (int j = 0; j < V; ++j) {
+                    const Curve k = curve<decltype(act)::value, sizeof(T) == 2>(g[j]);
+                    d[j] = v[j] * k.value;
+                    v[j] *= u[j] * k.slope;
+                }
+            });
             store_some<T, V>(out, v);
             store_some<T, V>(out + (long long)a.half * a.out_stride, d);
         } else {
             if (a.extra) {
                 float g[V];
                 load_some<B, V>(z, g);
+                with_activation(a.act, [&](auto act) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] *= activation_slope(g[j], a.act);
+                    for (int j = 0; j < V; ++j) v[j] *= curve<decltype(act)::value, sizeof(T) == 2>(g[j]).slope;
+                });
             }
             store_some<T, V>(out, v);
         }
@@ -269,26 +302,143 @@ k_dense_row(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__restrict
 // products of the next.  Where there are fewer tiles than SMs, a cluster of CTAs shares the k of one: their sums cross through distributed shared memory and
 // are added in the order of the CTAs.
 //
-// fp32 outputs: the tensor cores cut the digits that do not fit their running sum, which over thousands of steps drifts (see kChunk); those sums are taken out
-// after every chunk of k and added up in registers.
+// fp32 outputs: the tensor cores cut the digits that do not fit their running sum, which over thousands of steps drifts towards zero; those sums are taken out
+// after every kChunk stages and added up in registers.  (Error of the 2-norm of dW, 4096 x 4096 x 8192, and of y: 4.8e-7 at 8 stages, 7.2e-7 at 12, 1.0e-6 at 16, 2.1e-6 at
+// 32; plain fp32 1e-6.  Taking them out stands in the products' way in TMEM: dW 246, 239, 236 us at 8, 12, 16.)
 template <int KIND, typename T, int TN, bool PAIR> struct DenseShape {
     static constexpr bool kAAcross = KIND == kInputGrad, kBAcross = KIND != kWeightGrad, kPromote = sizeof(T) == 4;
     static constexpr int kParts = KIND == kGated ? 2 : 1, kOwnN = PAIR ? TN / 2 : TN, kBRows = kBAcross && kOwnN < 64 ? 64 : kOwnN;
     static constexpr int kABytes = kTileM * kTileK * 2, kStageBytes = kParts * kABytes + kBRows * kTileK * 2;
-    static constexpr int kOutBytes = KIND == kGated ? 2048 : 4096;        // of a warp: 32 rows x 32 columns, bf16 or fp32
-    static constexpr int kRoom = 225 * 1024 - kDenseWarps * kOutBytes, kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
-    static constexpr int kSmem = kStages * kStageBytes + kDenseWarps * kOutBytes + 1024;
+    static constexpr int kWarps = 16, kThreads = 64 + 32 * kWarps;        // warp 0 copies, warp 1 issues the products, the others take the sums out of TMEM
+    static constexpr int kPiece = kPromote || KIND == kGated ? 16 : 32;   // columns that a warp takes at a time
+    static constexpr int kOutBytes = 32 * kPiece * (int)sizeof(T);
+    static constexpr int kRoom = 225 * 1024 - kWarps * kOutBytes, kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
+    static constexpr int kSmem = kStages * kStageBytes + kWarps * kOutBytes + 1024;
     static constexpr int kAccColumns = kParts * TN, kColumns = 2 * kAccColumns < 32 ? 32 : 2 * kAccColumns;
-    static constexpr int kWarpColumns = TN / 2 < 32 ? 32 : TN / 2;        // a warp's share of a tile's columns
+    static constexpr int kWarpColumns = TN * 4 / kWarps < kPiece ? kPiece : TN * 4 / kWarps;  // a warp's share of a tile's columns
 };
-constexpr int kChunk = 8;                                // stages of k between two additions in registers
+constexpr int kChunk = 12;                               // stages of k between two additions in registers
+
+// A warp's 32 rows, a row a lane, of P pieces of eight columns (fp32: of four) to memory (`base`: the first row at the first column, `rows` and `left` columns of it
+// exist): they cross shared memory, where the order of a row's pieces differs from row to row so that no banks collide, and leave as P * 16 bytes of a row; at odd
+// addresses a column a lane.
+template <int P> __device__ __forceinline__ int staged_piece(int row, int q) { return row * P + (q ^ (P == 8 ? row & 7 : P == 4 ? row >> 1 & 3 : row >> 2 & 1)); }
+template <int P> __device__ __forceinline__ void store_rows(uint4 *stage, const uint4 (&v)[P], __nv_bfloat16 *base, long long stride, int rows, int left, bool vec)
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int q = 0; q < P; ++q) stage[staged_piece<P>(lane, q)] = v[q];
+    __syncwarp();
+    if (vec) {
+        const int q = lane % P;
+#pragma unroll
+        for (int it = 0; it < P; ++it) {
+            const int r = it * (32 / P) + lane / P;
+            const uint4 piece = stage[staged_piece<P>(r, q)];
+            __nv_bfloat16 *const to = base + r * stride + 8 * q;
+            if (r >= rows) continue;
+            if (8 * q + 8 <= left) {
+                *reinterpret_cast<uint4 *>(to) = piece;
+            } else {
+                const __nv_bfloat16 *const one = reinterpret_cast<const __nv_bfloat16 *>(&piece);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (8 * q + j < left) to[j] = one[j];
+            }
+        }
+    } else if (lane < left && lane < 8 * P) {
+#pragma unroll 8
+        for (int r = 0; r < min(32, rows); ++r) base[r * stride + lane] = reinterpret_cast<const __nv_bfloat16 *>(&stage[staged_piece<P>(r, lane / 8)])[lane % 8];
+    }
+    __syncwarp();
+}
+
+// The way back: 32 rows of P pieces of eight columns of an input of the epilogue are asked for as they lie, P * 16 bytes of a row by P lanes side by side, and
+// change places through the same shared memory when they are needed, so that each lane has its row.  (A lane asking for its own row brings every sector twice:
+// product of 2000 x 5500 x 3001 with a gate's gradient 105 us, 3.4 times its input's bytes out of L2.)
+template <int P> __device__ __forceinline__ void load_rows(uint4 (&e)[P], const __nv_bfloat16 *base, long long stride, int rows, int left, bool vec)
+{
+    const int lane = threadIdx.x & 31, q = lane % P;
+#pragma unroll
+    for (int it = 0; it < P; ++it) {
+        const int r = it * (32 / P) + lane / P;
+        const __nv_bfloat16 *const p = base + r * stride + 8 * q;
+        e[it] = make_uint4(0, 0, 0, 0);
+        if (r >= rows || 8 * q >= left) continue;
+        if (vec) {
+            e[it] = *reinterpret_cast<const uint4 *>(p);
+        } else {
+            __nv_bfloat16 *const one = reinterpret_cast<__nv_bfloat16 *>(&e[it]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (8 * q + j < left) one[j] = p[j];
+        }
+    }
+}
+template <int P> __device__ __forceinline__ void spread_rows(uint4 *stage, uint4 (&e)[P])
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int it = 0; it < P; ++it) stage[staged_piece<P>(it * (32 / P) + lane / P, lane % P)] = e[it];
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < P; ++q) e[q] = stage[staged_piece<P>(lane, q)];
+    __syncwarp();
+}
+
+// fp32, with `extra` (null: nothing) added on the way, or added to what is there (one addition an element, so that its order does not matter)
+template <int C> __device__ __forceinline__ void store_rows(uint4 *stage, const float (&v)[C], float *base, long long stride, const float *extra, long long extra_stride,
+                                                            bool accumulate, int rows, int left, bool vec)
+{
+    constexpr int P = C / 4;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+        const float p[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        stage[staged_piece<P>(lane, q)] = pack<float>(p);
+    }
+    __syncwarp();
+    if (vec) {
+        const int q = lane % P;
+#pragma unroll
+        for (int it = 0; it < P; ++it) {
+            const int r = it * (32 / P) + lane / P;
+            float p[4];
+            unpack<float>(stage[staged_piece<P>(r, q)], p);
+            float *const to = base + r * stride + 4 * q;
+            if (r >= rows || 4 * q >= left) continue;
+            if (4 * q + 4 <= left) {
+                if (extra) {
+                    float e[4];
+                    unpack<float>(*reinterpret_cast<const uint4 *>(extra + r * extra_stride + 4 * q), e);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[j] += e[j];
+                }
+                if (accumulate) red_add_v4(to, p[0], p[1], p[2], p[3]);
+                else *reinterpret_cast<uint4 *>(to) = pack<float>(p);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (4 * q + j < left) to[j] = accumulate ? to[j] + p[j] : extra ? p[j] + extra[r * extra_stride + 4 * q + j] : p[j];
+            }
+        }
+    } else if (lane < left && lane < C) {
+#pragma unroll 4
+        for (int r = 0; r < min(32, rows); ++r) {
+            const float p = reinterpret_cast<const float *>(&stage[staged_piece<P>(r, lane / 4)])[lane % 4];
+            float *const to = base + r * stride + lane;
+            *to = accumulate ? *to + p : extra ? p + extra[r * extra_stride + lane] : p;
+        }
+    }
+    __syncwarp();
+}
 
 template <int KIND, typename T, int TN, bool PAIR>
-__global__ void __launch_bounds__(kDenseThreads, 1)
+__global__ void __launch_bounds__(DenseShape<KIND, T, TN, PAIR>::kThreads, 1)
 k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const DenseArgs a)
 {
     using S = DenseShape<KIND, T, TN, PAIR>;
-    constexpr int kStages = S::kStages, kAcc = 2, kParts = S::kParts;
+    constexpr int kStages = S::kStages, kAcc = 2, kParts = S::kParts, kPiece = S::kPiece;
     static_assert(S::kColumns <= 512 && (S::kColumns & (S::kColumns - 1)) == 0, "TMEM");
     static_assert(kStages >= 4 && kParts * kTileM * (TN + 4) * 4 <= kStages * S::kStageBytes, "shared memory");
     extern __shared__ uint8_t smem_raw[];
@@ -301,7 +451,7 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], PAIR ? 2 * kDenseWarps : kDenseWarps); }
+        for (int s = 0; s < kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], PAIR ? 2 * S::kWarps : S::kWarps); }
         mbar_init(&drained, 1);
         gave_up = 0;
         mbar_init_fence();
@@ -429,7 +579,24 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         for (int tile = first; tile < tiles; tile += step) {
             int m0, n0;
             place(tile, m0, n0);
-            const int m = m0 + part * 32;
+            // what a lane has is a row; the epilogue's inputs of its first columns are on their way before the sums are there
+            const int m = m0 + part * 32, row = min(m + lane, a.M - 1);
+            float bias[2] = {0.0f, 0.0f};
+            if (KIND <= kGated && a.bias) {
+                bias[0] = a.bias[row];
+                if (KIND == kGated) bias[1] = a.bias[a.half + row];
+            }
+            constexpr bool kExtra = sizeof(T) == 2 && (KIND == kForward || KIND == kInputGrad);
+            uint4 extra[2][kPiece / 8];
+            const bool has_extra = kExtra && a.extra && splits == 1 && c0 < TN;
+            auto fetch_extra = [&](int i) {
+                const int n = n0 + c0 + i;
+                if (!has_extra || i >= S::kWarpColumns || n >= a.N) return;
+                const __nv_bfloat16 *const p = static_cast<const __nv_bfloat16 *>(a.extra) + m * a.extra_stride + n;
+                load_rows(extra[0], p, a.extra_stride, a.M - m, a.N - n, a.vec);
+                if (KIND == kInputGrad && a.gated) load_rows(extra[1], p + a.half * a.extra_stride, a.extra_stride, a.M - m, a.N - n, a.vec);
+            };
+            fetch_extra(0);
             float sums[S::kPromote ? S::kWarpColumns : 1];
             bool ok = true;
             if constexpr (S::kPromote) {
@@ -442,11 +609,11 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     const uint32_t at = tmem + ((uint32_t)(part * 32) << 16) + acc * S::kAccColumns + c0;
                     if (c0 < TN) {
 #pragma unroll
-                        for (int i = 0; i < S::kWarpColumns; i += 32) {
-                            int v[32];
-                            tmem_load_32(at + i, v);
+                        for (int i = 0; i < S::kWarpColumns; i += kPiece) {
+                            int v[kPiece];
+                            tmem_load(at + i, v);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) sums[i + j] += __int_as_float(v[j]);
+                            for (int j = 0; j < kPiece; ++j) sums[i + j] += __int_as_float(v[j]);
                         }
                     }
                     give_back();
@@ -464,104 +631,130 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     float *const to = reinterpret_cast<float *>(smem) + ((p * kTileM) + part * 32 + lane) * (TN + 4) + c0;
                     if (c0 < TN) {
 #pragma unroll
-                        for (int i = 0; i < S::kWarpColumns; i += 32) {
-                            int v[32];
+                        for (int i = 0; i < S::kWarpColumns; i += kPiece) {
+                            int v[kPiece];
                             if constexpr (S::kPromote) {
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) v[j] = __float_as_int(sums[i + j]);
+                                for (int j = 0; j < kPiece; ++j) v[j] = __float_as_int(sums[i + j]);
                             } else {
-                                tmem_load_32(at + p * TN + i, v);
+                                tmem_load(at + p * TN + i, v);
                             }
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4) *reinterpret_cast<int4 *>(to + i + j) = make_int4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                            for (int j = 0; j < kPiece; j += 4) *reinterpret_cast<int4 *>(to + i + j) = make_int4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                         }
                     }
                 }
-            } else if (c0 < TN) {
+                if constexpr (!S::kPromote) give_back();
+                continue;
+            }
+            bool returned = S::kPromote;
+            // (rolled where no registers are indexed: unrolled four times the epilogue's instructions do not stay in their cache)
+#pragma unroll (S::kPromote ? S::kWarpColumns / kPiece : 1)
+            for (int i = 0; i < S::kWarpColumns; i += kPiece) {
+                const int n = n0 + c0 + i, left = a.N - n, rows = a.M - m;
+                if (c0 >= TN || left <= 0) break;
+                int v[kPiece], w[KIND == kGated ? kPiece : 1];
+                if constexpr (S::kPromote) {
 #pragma unroll
-                for (int i = 0; i < S::kWarpColumns; i += 32) {
-                    const int n = n0 + c0 + i;
-                    if (n >= a.N) continue;
-                    if constexpr (KIND == kGated) {
-                        // everything is made in the lane of the row; the results cross shared memory in bf16, one of h, g and u after the other
-                        int v[32], w[32];
-                        tmem_load_32(at + i, v);
-                        tmem_load_32(at + TN + i, w);
-                        const int row = min(m + lane, a.M - 1);
-                        const float b = a.bias ? a.bias[row] : 0.0f, c = a.bias ? a.bias[a.half + row] : 0.0f;
-                        for (int what = 0; what < (a.z_out ? 3 : 1); ++what) {
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                float r[8];
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    const float g = __int_as_float(v[8 * q + j]) + b, u = __int_as_float(w[8 * q + j]) + c;
-                                    r[j] = what == 0 ? activate(g, a.act) * u : what == 1 ? g : u;
-                                }
-                                stage_out[lane * 4 + (q ^ (lane >> 1 & 3))] = pack<__nv_bfloat16>(r);
-                            }
-                            __syncwarp();
-                            __nv_bfloat16 *const base = what == 0 ? static_cast<__nv_bfloat16 *>(a.out) + (long long)m * a.out_stride
-                                                                  : static_cast<__nv_bfloat16 *>(a.z_out) + (long long)(m + (what == 2 ? a.half : 0)) * a.z_stride;
-                            const long long stride = what == 0 ? a.out_stride : a.z_stride;
-                            if (a.vec) {
-#pragma unroll
-                                for (int it = 0; it < 4; ++it) {
-                                    const int r = it * 8 + lane / 4, q = lane % 4;
-                                    const uint4 piece = stage_out[r * 4 + (q ^ (r >> 1 & 3))];
-                                    __nv_bfloat16 *const to = base + r * stride + n + 8 * q;
-                                    if (m + r >= a.M) continue;
-                                    if (n + 8 * q + 8 <= a.N) {
-                                        *reinterpret_cast<uint4 *>(to) = piece;
-                                    } else {
-                                        const __nv_bfloat16 *const one = reinterpret_cast<const __nv_bfloat16 *>(&piece);
-#pragma unroll
-                                        for (int j = 0; j < 8; ++j)
-                                            if (n + 8 * q + j < a.N) to[j] = one[j];
-                                    }
-                                }
-                            } else if (n + lane < a.N) {
-#pragma unroll 8
-                                for (int r = 0; r < min(32, a.M - m); ++r)
-                                    base[r * stride + n + lane] = reinterpret_cast<const __nv_bfloat16 *>(&stage_out[r * 4 + (lane / 8 ^ (r >> 1 & 3))])[lane % 8];
-                            }
-                            __syncwarp();
-                        }
-                    } else {
-                        // the sums cross 4 KB of shared memory, in 16-byte pieces whose order differs from row to row so that no banks collide: eight
-                        // columns a lane of four lanes side by side, or, where rows are not on 16-byte boundaries, a lane for each of the 32 columns
-                        int v[32];
-                        if constexpr (S::kPromote) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = __float_as_int(sums[i + j]);
-                        } else {
-                            tmem_load_32(at + i, v);
-                        }
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) stage_out[lane * 8 + (q ^ (lane & 7))] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                        __syncwarp();
-                        if (a.vec) {
-#pragma unroll
-                            for (int it = 0; it < 4; ++it) {
-                                const int r = it * 8 + lane / 4, q = lane % 4;
-                                float lo[4], hi[4], none[8];
-                                unpack<float>(stage_out[r * 8 + (2 * q ^ (r & 7))], lo);
-                                unpack<float>(stage_out[r * 8 + (2 * q + 1 ^ (r & 7))], hi);
-                                float s[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                                if (m + r < a.M && n + 8 * q < a.N) finish_8<KIND, T>(a, m + r, n + 8 * q, s, none);
-                            }
-                        } else if (n + lane < a.N) {
-#pragma unroll 4
-                            for (int r = 0; r < min(32, a.M - m); ++r) {
-                                float s[1] = {reinterpret_cast<const float *>(&stage_out[r * 8 + (lane / 4 ^ (r & 7))])[lane % 4]}, none[1];
-                                finish<KIND, T, 1>(a, m + r, n + lane, s, none);
-                            }
-                        }
-                        __syncwarp();
+                    for (int j = 0; j < kPiece; ++j) v[j] = __float_as_int(sums[i + j]);
+                } else {
+                    tmem_load(at + i, v);
+                    if constexpr (KIND == kGated) tmem_load(at + TN + i, w);
+                    if (i + kPiece >= S::kWarpColumns || left <= kPiece) {        // the last of its columns: the next tile's products may have them
+                        give_back();
+                        returned = true;
                     }
+                }
+                uint4 out[kPiece / 8];
+                // a number of each of the columns, made eight at a time: f(column) -> float
+                auto made = [&](auto f) {
+#pragma unroll
+                    for (int q = 0; q < kPiece / 8; ++q) {
+                        float r[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) r[j] = f(8 * q + j);
+                        out[q] = pack<__nv_bfloat16>(r);
+                    }
+                };
+                auto extra_of = [&](int which, int j) {
+                    const uint32_t word = reinterpret_cast<const uint32_t *>(extra[which])[j / 2];
+                    return __uint_as_float(j % 2 ? word & 0xffff0000u : word << 16);
+                };
+                __nv_bfloat16 *const z_base = KIND <= kGated && a.z_out ? static_cast<__nv_bfloat16 *>(a.z_out) + m * a.z_stride + n : nullptr;
+                T *const base = static_cast<T *>(a.out) + m * a.out_stride + n;
+                if constexpr (KIND == kForward) {
+                    if (a.bias) {
+#pragma unroll
+                        for (int j = 0; j < kPiece; ++j) v[j] = __float_as_int(__int_as_float(v[j]) + bias[0]);
+                    }
+                    if (z_base) {
+                        made([&](int j) { return __int_as_float(v[j]); });
+                        store_rows(stage_out, out, z_base, a.z_stride, rows, left, a.vec);
+                    }
+                    with_activation(a.act, [&](auto act) {
+#pragma unroll
+                        for (int j = 0; j < kPiece; ++j) v[j] = __float_as_int(curve<decltype(act)::value, sizeof(T) == 2>(__int_as_float(v[j])).value);
+                    });
+                }
+                if constexpr (sizeof(T) == 4) {
+                    float r[kPiece];
+#pragma unroll
+                    for (int j = 0; j < kPiece; ++j) r[j] = __int_as_float(v[j]);
+                    store_rows(stage_out, r, base, a.out_stride, a.extra ? static_cast<const float *>(a.extra) + m * a.extra_stride + n : nullptr, a.extra_stride,
+                                  a.accumulate, rows, left, a.vec);
+                } else if constexpr (KIND == kForward) {
+                    if (a.extra) spread_rows(stage_out, extra[0]);
+                    if (a.extra) made([&](int j) { return __int_as_float(v[j]) + extra_of(0, j); });
+                    else made([&](int j) { return __int_as_float(v[j]); });
+                    fetch_extra(i + kPiece);
+                    store_rows(stage_out, out, base, a.out_stride, rows, left, a.vec);
+                } else if constexpr (KIND == kGated) {
+                    if (a.bias) {
+#pragma unroll
+                        for (int j = 0; j < kPiece; ++j) {
+                            v[j] = __float_as_int(__int_as_float(v[j]) + bias[0]);
+                            w[j] = __float_as_int(__int_as_float(w[j]) + bias[1]);
+                        }
+                    }
+                    with_activation(a.act, [&](auto act) { made([&](int j) { return curve<decltype(act)::value, sizeof(T) == 2>(__int_as_float(v[j])).value * __int_as_float(w[j]); }); });
+                    store_rows(stage_out, out, base, a.out_stride, rows, left, a.vec);
+                    if (z_base) {
+                        made([&](int j) { return __int_as_float(v[j]); });
+                        store_rows(stage_out, out, z_base, a.z_stride, rows, left, a.vec);
+                        made([&](int j) { return __int_as_float(w[j]); });
+                        store_rows(stage_out, out, z_base + a.half * a.z_stride, a.z_stride, rows, left, a.vec);
+                    }
+                } else if (a.gated) {
+                    spread_rows(stage_out, extra[0]);
+                    spread_rows(stage_out, extra[1]);
+                    uint4 up[kPiece / 8];
+                    with_activation(a.act, [&](auto act) {
+#pragma unroll
+                        for (int q = 0; q < kPiece / 8; ++q) {
+                            float d[8], e[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const Curve k = curve<decltype(act)::value, sizeof(T) == 2>(extra_of(0, 8 * q + j));
+                                const float s = __int_as_float(v[8 * q + j]);
+                                d[j] = s * (extra_of(1, 8 * q + j) * k.slope);
+                                e[j] = s * k.value;
+                            }
+                            out[q] = pack<__nv_bfloat16>(d);
+                            up[q] = pack<__nv_bfloat16>(e);
+                        }
+                    });
+                    fetch_extra(i + kPiece);
+                    store_rows(stage_out, out, base, a.out_stride, rows, left, a.vec);
+                    store_rows(stage_out, up, base + a.half * a.out_stride, a.out_stride, rows, left, a.vec);
+                } else {
+                    if (a.extra) spread_rows(stage_out, extra[0]);
+                    if (a.extra) with_activation(a.act, [&](auto act) { made([&](int j) { return __int_as_float(v[j]) * curve<decltype(act)::value, sizeof(T) == 2>(extra_of(0, j)).slope; }); });
+                    else made([&](int j) { return __int_as_float(v[j]); });
+                    fetch_extra(i + kPiece);
+                    store_rows(stage_out, out, base, a.out_stride, rows, left, a.vec);
                 }
             }
-            if constexpr (!S::kPromote) give_back();
+            if (!returned) give_back();
         }
     }
     if (!PAIR && splits > 1) {
@@ -573,7 +766,7 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             int m0, n0;
             place(first, m0, n0);
             const int rows = kTileM / splits, r0 = (int)rank * rows;
-            for (int e = threadIdx.x - 64; e < rows * (TN / 8); e += kDenseThreads - 64) {
+            for (int e = threadIdx.x - 64; e < rows * (TN / 8); e += S::kThreads - 64) {
                 const int r = r0 + e / (TN / 8), c = e % (TN / 8) * 8;
                 if (m0 + r >= a.M || n0 + c >= a.N) continue;
                 float s[2][8];
@@ -666,7 +859,7 @@ static int dense_tiles(const Operand &A, const Operand &B, const DenseArgs &a, c
     const unsigned cluster = PAIR ? 2u : (unsigned)a.splits;
     const long long slots = PAIR ? sms / 2 : sms;
     const unsigned grid = cluster * (unsigned)(!PAIR && a.splits > 1 ? tiles : tiles < slots ? tiles : slots);
-    return launch_cluster(kernel, cluster, grid, kDenseThreads, S::kSmem, st, map_a, map_b, a);
+    return launch_cluster(kernel, cluster, grid, S::kThreads, S::kSmem, st, map_a, map_b, a);
 }
 
 // Columns a tile (0: by a pair of CTAs) and CTAs that share the k of one, by the clocks of an SM: rounds of tiles times stages of k times what a stage
