@@ -9,9 +9,9 @@
 // Sums are 32 bits; bf16 frames are widened when they are read and rounded once when they are written.  What is normalised is the sum as it is kept, so that
 // the backward pass, which is given that, sees the numbers that the statistics are of.
 //
-// Memory bounds it (16 bytes a value of fp32 forward with a residual, 16 backward).  A frame is needed whole before its first output: a cluster of CTAs has
-// the columns of 32 to 128 bytes of a row and goes over the rows twice.  Up to kHeldRows rows a thread stay in registers in between; the others are read
-// again, out of L2, which holds them since they were written, or read, some microseconds before.
+// Memory bounds it (16 bytes a value of fp32 forward with a residual, 16 backward).  A frame is needed whole before its first output.  Small calls take one launch: a
+// cluster of CTAs has the columns of 32 or 128 bytes of a row and goes over the rows twice, or once where they stay in registers.  Large ones go along the rows
+// in two passes, which move a quarter more (a residual's sum is written by the first and read by the second), at 5.9 to 6.9 TB/s.
 #include <algorithm>
 
 #include "frame_columns.cuh"
@@ -20,7 +20,7 @@
 namespace bb200 {
 
 constexpr int kMostRmsNodes = 1 << 20;
-constexpr int kHeldRows = 8;
+constexpr int kHeldRows = 4;
 
 template <typename T> struct RmsForward {
     const T *x, *r;
@@ -33,20 +33,85 @@ template <typename T> struct RmsForward {
     int *fault;
 };
 
-// a vector of s = x + r as it is kept
+// a vector of s = x + r as it is kept.  (bf16: rounded once by the packed addition, which is what the sum of 32 bits rounded again gives: it is inexact only
+// where the smaller term is below half of the last place.)
 template <typename T> __device__ __forceinline__ uint4 add_frames(const uint4 &x, const uint4 &r)
 {
-    float a[kFramesPerVec<T>], b[kFramesPerVec<T>];
-    unpack<T>(x, a);
-    unpack<T>(r, b);
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t p[4] = {x.x, x.y, x.z, x.w}, q[4] = {r.x, r.y, r.z, r.w};
+        uint32_t s[4];
 #pragma unroll
-    for (int j = 0; j < kFramesPerVec<T>; ++j) a[j] += b[j];
-    return pack<T>(a);
+        for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 v = __hadd2(reinterpret_cast<const __nv_bfloat162 &>(p[j]), reinterpret_cast<const __nv_bfloat162 &>(q[j]));
+            s[j] = reinterpret_cast<const uint32_t &>(v);
+        }
+        return make_uint4(s[0], s[1], s[2], s[3]);
+    } else {
+        float a[4], b[4];
+        unpack<T>(x, a);
+        unpack<T>(r, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] += b[j];
+        return pack<T>(a);
+    }
 }
+
+// The end of a row: four, two and one of eight numbers.  (Apart, since it is rare and would slow the rest; one by one it took twice the time of a call whose tiles
+// are few, 16384 x 100 bf16.)
+__device__ __noinline__ void store_end(__nv_bfloat16 *at, uint4 v, int left)
+{
+    if (left & 4) *reinterpret_cast<uint2 *>(at) = make_uint2(v.x, v.y);
+    if (left & 2) *reinterpret_cast<uint32_t *>(at + (left & 4)) = left & 4 ? v.z : v.x;
+    if (left & 1) {
+        const uint32_t word = left < 2 ? v.x : left < 4 ? v.y : left < 6 ? v.z : v.w;
+        at[left & 6] = __ushort_as_bfloat16((unsigned short)word);
+    }
+}
+
+template <typename T, bool ALIGNED> __device__ __forceinline__ void store_vector(T *row, int f, int F, const uint4 &v)
+{
+    if (ALIGNED && f + kFramesPerVec<T> <= F) {
+        *reinterpret_cast<uint4 *>(row + f) = v;
+    } else if constexpr (ALIGNED && sizeof(T) == 2) {
+        if (f < F) store_end(row + f, v, F - f);
+    } else {
+        const T *const one = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int j = 0; j < kFramesPerVec<T>; ++j)
+            if (f + j < F) row[f + j] = one[j];
+    }
+}
+
+// The same and a load for what is read or written once: it leaves L2 first, so that what is read again stays.  (3000 x 5001 fp32 with a residual in two passes 51.4
+// and 44.7 us, 1024 x 16384 bf16 in one 26.8 and 22.9.)
+template <typename T, bool ONCE, bool ALIGNED> __device__ __forceinline__ uint4 load_frames_once(const T *row, int f, int F)
+{
+    if constexpr (ONCE) return f < F ? __ldcs(reinterpret_cast<const uint4 *>(row + f)) : make_uint4(0, 0, 0, 0);
+    return load_frames<T, ALIGNED>(row, f, F);
+}
+template <typename T, bool ALIGNED> __device__ __forceinline__ void store_frames_once(T *row, int f, int F, const float (&v)[kFramesPerVec<T>])
+{
+    if (ALIGNED && f + kFramesPerVec<T> <= F) __stcs(reinterpret_cast<uint4 *>(row + f), pack<T>(v));
+    else store_vector<T, ALIGNED>(row, f, F, pack<T>(v));
+}
+template <typename T, bool ALIGNED> __device__ __forceinline__ uint4 load_once(const Line<T, ALIGNED> &line, const T *row)
+{
+    if constexpr (ALIGNED) return load_frames_once<T, true, true>(row, line.first, line.F);
+    return line.load(row);
+}
+template <typename T, bool ALIGNED> __device__ __forceinline__ void store_once(const Line<T, ALIGNED> &line, T *row, const float (&v)[kFramesPerVec<T>])
+{
+    if constexpr (ALIGNED) store_frames_once<T, true>(row, line.first, line.F, v);
+    else line.store(row, v);
+}
+
+// the larger one, and NaN where either is
+__device__ __forceinline__ float max_or_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+struct MaxOrNan { __device__ static float join(float a, float b) { return max_or_nan(a, b); } };
 
 // A thread takes kRows neighbouring rows a round (8 bits: four, which are a word of q), the rounds of a cluster's CTAs in turn.
 template <typename T, int LPR, bool ALIGNED, bool INT8, bool HELD>
-__global__ void __launch_bounds__(kColumnThreads, 4)
+__global__ void __launch_bounds__(kColumnThreads, HELD ? 2 : 4)
 k_rms_forward(const RmsForward<T> a)
 {
     grid_dependency();
@@ -67,16 +132,14 @@ k_rms_forward(const RmsForward<T> a)
         const int n = (round * (int)cl.size + (int)cl.rank) * round_rows + c.row * kRows;
         uint4 raw[kRows], more[kRows];
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) raw[i] = n + i < a.N ? load_frames<T, ALIGNED>(a.x + (long long)(n + i) * a.xs, f, a.F) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kRows; ++i) raw[i] = n + i < a.N ? load_frames_once<T, ALIGNED && HELD, ALIGNED>(a.x + (long long)(n + i) * a.xs, f, a.F) : make_uint4(0, 0, 0, 0);
         if (a.r) {
 #pragma unroll
-            for (int i = 0; i < kRows; ++i) more[i] = n + i < a.N ? load_frames<T, ALIGNED>(a.r + (long long)(n + i) * a.rs, f, a.F) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < kRows; ++i) more[i] = n + i < a.N ? load_frames_once<T, ALIGNED, ALIGNED>(a.r + (long long)(n + i) * a.rs, f, a.F) : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < kRows; ++i) {
                 raw[i] = add_frames<T>(raw[i], more[i]);
-                float w[kVec];
-                unpack<T>(raw[i], w);
-                if (n + i < a.N) store_frames<T, ALIGNED>(a.s + (long long)(n + i) * a.ss, f, a.F, w);
+                if (n + i < a.N) store_vector<T, ALIGNED>(a.s + (long long)(n + i) * a.ss, f, a.F, raw[i]);
             }
         }
 #pragma unroll
@@ -87,7 +150,7 @@ k_rms_forward(const RmsForward<T> a)
 #pragma unroll
             for (int j = 0; j < kVec; ++j) {
                 v[0][j] = fmaf(w[j], w[j], v[0][j]);
-                if constexpr (INT8) v[1][j] = __uint_as_float(max(__float_as_uint(v[1][j]), __float_as_uint(fabsf(w[j] * g))));
+                if constexpr (INT8) v[1][j] = max_or_nan(v[1][j], fabsf(w[j] * g));
             }
             if constexpr (HELD) {
 #pragma unroll
@@ -102,15 +165,14 @@ k_rms_forward(const RmsForward<T> a)
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
             v[0][j] += __shfl_xor_sync(0xffffffffu, v[0][j], m);
-            if constexpr (INT8) v[1][j] = __uint_as_float(max(__float_as_uint(v[1][j]), __float_as_uint(__shfl_xor_sync(0xffffffffu, v[1][j], m))));
+            if constexpr (INT8) v[1][j] = max_or_nan(v[1][j], __shfl_xor_sync(0xffffffffu, v[1][j], m));
         }
-    struct BitsMax { __device__ static float join(float p, float q) { return __uint_as_float(max(__float_as_uint(p), __float_as_uint(q))); } };
     const float inv = 1.0f / (float)a.N;
     Exchange<kQ, kCols> &e = sums[0];
     exchange_columns<kQ, T, LPR>(v, c, e, cl, 0,
-        [&](const float *from, int distance, int count) { return from - &e.red[0][0] < kCols ? join_parts<ColumnSum>(from, distance, count) : join_parts<BitsMax>(from, distance, count); },
-        [&](const float *from, int distance, int count) { return from - &e.part[0][0] < kCols ? join_parts<ColumnSum>(from, distance, count) : join_parts<BitsMax>(from, distance, count); },
-        [&](int q, float t) { return q == 0 ? 1.0f / sqrtf(fmaf(t, inv, a.eps)) : quant_scale(__float_as_uint(t)); });
+        [&](const float *from, int distance, int count) { return from - &e.red[0][0] < kCols ? join_parts<ColumnSum>(from, distance, count) : join_parts<MaxOrNan>(from, distance, count); },
+        [&](const float *from, int distance, int count) { return from - &e.part[0][0] < kCols ? join_parts<ColumnSum>(from, distance, count) : join_parts<MaxOrNan>(from, distance, count); },
+        [&](int q, float t) { return q == 0 ? 1.0f / sqrtf(fmaf(t, inv, a.eps)) : quant_scale(__float_as_uint(t) & 0x7fffffffu); });
     if (cl.rank == 0 && threadIdx.x < kCols && f0 + (int)threadIdx.x < a.F) {
         if constexpr (INT8) a.scale[f0 + threadIdx.x] = e.out[threadIdx.x] * e.out[kCols + threadIdx.x];
         if (a.rstd) a.rstd[f0 + threadIdx.x] = e.out[threadIdx.x];
@@ -137,7 +199,7 @@ k_rms_forward(const RmsForward<T> a)
 #pragma unroll
             for (int j = 0; j < kVec; ++j) w[i][j] = INT8 ? w[i][j] * g : (w[i][j] * v[0][j]) * g;
             if constexpr (!INT8) {
-                if (n + i < a.N) store_frames<T, ALIGNED>(a.y + (long long)(n + i) * a.ys, f, a.F, w[i]);
+                if (n + i < a.N) store_frames_once<T, ALIGNED>(a.y + (long long)(n + i) * a.ys, f, a.F, w[i]);
             }
         }
         if constexpr (INT8) {
@@ -162,14 +224,14 @@ template <typename T> struct RmsBackward {
     const T *s, *dy, *dr;
     T *ds;
     const float *gamma, *rstd;
-    float *gamma_part;                                   // [tile][node]
+    float *gamma_part;                                   // [tile or sweep][node]
     int N, F, rounds;
     long long ss, dys, drs, dss;
     int *fault;
 };
 
 template <typename T, int LPR, bool ALIGNED, bool HELD>
-__global__ void __launch_bounds__(kColumnThreads, 3)
+__global__ void __launch_bounds__(kColumnThreads, HELD ? 2 : 3)
 k_rms_backward(const RmsBackward<T> a)
 {
     grid_dependency();
@@ -215,28 +277,45 @@ k_rms_backward(const RmsBackward<T> a)
             for (int i = 0; i < kRows; ++i) r_raw[i] = n + i < a.N ? load_frames<T, ALIGNED>(a.dr + (long long)(n + i) * a.drs, f, a.F) : make_uint4(0, 0, 0, 0);
         }
         if constexpr (!HELD) load(n);
+        float along[kRows];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             const float g = a.gamma && n + i < a.N ? a.gamma[n + i] : 1.0f;
-            float s[kVec], d[kVec], along = 0.0f;
+            float s[kVec], d[kVec], r[kVec] = {};
             unpack<T>(s_raw[i], s);
             unpack<T>(g_raw[i], d);
+            if (a.dr) unpack<T>(r_raw[i], r);
+            if (f + kVec > a.F) {                                         // what lies beyond the frames may be anything
+#pragma unroll
+                for (int j = 0; j < kVec; ++j)
+                    if (f + j >= a.F) s[j] = d[j] = 0.0f;
+            }
+            along[i] = 0.0f;
 #pragma unroll
             for (int j = 0; j < kVec; ++j) {
                 const float xh = s[j] * rstd[j];
-                if (f + j < a.F) along = fmaf(d[j], xh, along);            // what lies beyond the frames may be anything
-                d[j] = rstd[j] * fmaf(-xh, v[0][j], g * d[j]);
+                along[i] = fmaf(d[j], xh, along[i]);
+                d[j] = fmaf(rstd[j], fmaf(-xh, v[0][j], g * d[j]), r[j]);
             }
-            if (a.dr) {
-                float r[kVec];
-                unpack<T>(r_raw[i], r);
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) d[j] += r[j];
-            }
-            if (n + i < a.N) store_frames<T, ALIGNED>(a.ds + (long long)(n + i) * a.dss, f, a.F, d);
-#pragma unroll
-            for (int m = 1; m < LPR; m <<= 1) along += __shfl_xor_sync(0xffffffffu, along, m);
-            if (a.gamma_part && c.lane % LPR == 0 && n + i < a.N) a.gamma_part[(long long)tile * a.N + n + i] = along;
+            if (n + i < a.N) store_vector<T, ALIGNED>(a.ds + (long long)(n + i) * a.dss, f, a.F, pack<T>(d));
+        }
+        if (!a.gamma_part) continue;
+        // four rows over the lanes of a row: half of the rows change places for half of the lanes at each step
+        static_assert(kRows == 4 && (LPR == 2 || LPR == 8));
+        const bool odd = c.lane & 1;
+        float p = odd ? along[2] : along[0], q = odd ? along[3] : along[1];
+        p += __shfl_xor_sync(0xffffffffu, odd ? along[0] : along[2], 1);
+        q += __shfl_xor_sync(0xffffffffu, odd ? along[1] : along[3], 1);
+        float *const part = a.gamma_part + (long long)tile * a.N + n + (odd ? 2 : 0);
+        if constexpr (LPR == 2) {
+            if (n + (odd ? 2 : 0) < a.N) part[0] = p;
+            if (n + (odd ? 3 : 1) < a.N) part[1] = q;
+        } else {
+            const bool second = c.lane & 2;
+            float one = second ? q : p;
+            one += __shfl_xor_sync(0xffffffffu, second ? p : q, 2);
+            one += __shfl_xor_sync(0xffffffffu, one, 4);
+            if (!(c.lane & 4) && n + (odd ? 2 : 0) + (second ? 1 : 0) < a.N) part[second ? 1 : 0] = one;
         }
     }
     cl.leave(a.fault);
@@ -251,6 +330,7 @@ k_rms_gamma(const float *__restrict__ part, float *dgamma, int N, int parts, int
     const int n = (int)blockIdx.x * 32 + (threadIdx.x & 31);
     float t = 0.0f;
     if (n < N)
+#pragma unroll 4
         for (int k = threadIdx.x >> 5; k < parts; k += 8) t += part[(long long)k * N + n];
     s[threadIdx.x >> 5][threadIdx.x & 31] = t;
     __syncthreads();
@@ -267,6 +347,317 @@ __global__ void __launch_bounds__(256) k_rms_no_frames(float *dgamma, int N)
     if (n < N) dgamma[n] = 0.0f;
 }
 
+// ---- large layers in two passes along the rows: a CTA has 512 bytes of the rows of a band, a warp every eighth of them, and the bands are as many as the device
+// holds at a time.  The first pass adds up the columns of its band (part[band][frame], for 8 bits the largest numbers as well), the second one makes the output,
+// and goes through the rows of its band from the end, where L2 still holds what the first one left there.  (Held by clusters in shared memory and read once,
+// in columns of 64 and 128 bytes, these layers ran at 4.6 to 5.0 TB/s, with or without the exchange of sums; along the rows a copy runs at 6.5.)
+constexpr int kBandWarps = 8, kBandBatch = 4;
+
+// sums of the warps' columns, in the order of the warps; the first warp of the CTA has them
+template <typename T, bool ALIGNED, int Q, typename JOIN>
+__device__ __forceinline__ void store_band(float (&v)[Q][kFramesPerVec<T>], float *part, int bands, int band, int padded, const Line<T, ALIGNED> &line, JOIN join)
+{
+    constexpr int kVec = kFramesPerVec<T>;
+    __shared__ float red[kBandWarps][Q][kVec][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) red[warp][q][j][lane] = v[q][j];
+    __syncthreads();
+    // a warp joins some of the values
+    for (int e = warp; e < Q * kVec; e += kBandWarps) {
+        const int q = e / kVec, j = e % kVec;
+        float s = red[0][q][j][lane];
+        for (int w = 1; w < kBandWarps; ++w) s = join(q, s, red[w][q][j][lane]);
+        if (line.frame(j) < line.F) part[((long long)q * bands + band) * padded + line.frame(j)] = s;
+    }
+}
+
+template <typename T, bool ALIGNED, bool RESIDUAL, bool INT8>
+__global__ void __launch_bounds__(32 * kBandWarps, 4)
+k_rms_sums(const RmsForward<T> a, float *part, int rows, int padded)
+{
+    grid_dependency();
+    constexpr int kVec = kFramesPerVec<T>, kQ = INT8 ? 2 : 1;
+    const Line<T, ALIGNED> line((int)blockIdx.x * 32 * kVec, (int)(threadIdx.x & 31), a.F);
+    const int first = (int)blockIdx.y * rows, end = min(first + rows, a.N);
+    float v[kQ][kVec] = {};
+    for (int n = first + (int)(threadIdx.x >> 5); n < end; n += kBandWarps * kBandBatch) {
+        uint4 raw[kBandBatch], more[kBandBatch];
+#pragma unroll
+        for (int i = 0; i < kBandBatch; ++i)
+            if (n + i * kBandWarps < end) raw[i] = RESIDUAL && !INT8 ? load_once(line, a.x + (n + i * kBandWarps) * a.xs) : line.load(a.x + (n + i * kBandWarps) * a.xs);
+        if (RESIDUAL) {
+#pragma unroll
+            for (int i = 0; i < kBandBatch; ++i)
+                if (n + i * kBandWarps < end) more[i] = INT8 ? line.load(a.r + (n + i * kBandWarps) * a.rs) : load_once(line, a.r + (n + i * kBandWarps) * a.rs);
+        }
+#pragma unroll
+        for (int i = 0; i < kBandBatch; ++i) {
+            const int m = n + i * kBandWarps;
+            if (m >= end) break;
+            float w[kVec];
+            if (RESIDUAL) {
+                raw[i] = add_frames<T>(raw[i], more[i]);
+                unpack<T>(raw[i], w);
+                line.store(a.s + m * a.ss, w);
+            } else {
+                unpack<T>(raw[i], w);
+            }
+            const float g = INT8 && a.gamma ? a.gamma[m] : 1.0f;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                v[0][j] = fmaf(w[j], w[j], v[0][j]);
+                if constexpr (INT8) v[1][j] = max_or_nan(v[1][j], fabsf(w[j] * g));
+            }
+        }
+    }
+    store_band<T, ALIGNED, kQ>(v, part, (int)gridDim.y, (int)blockIdx.y, padded, line, [](int q, float p, float o) { return q == 0 ? p + o : max_or_nan(p, o); });
+}
+
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kBandWarps, 4)
+k_rms_apply(const RmsForward<T> a, const float *__restrict__ part, int rows, int padded)
+{
+    grid_dependency();
+    constexpr int kVec = kFramesPerVec<T>;
+    __shared__ float red[kBandWarps][kVec][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Line<T, ALIGNED> line((int)blockIdx.x * 32 * kVec, lane, a.F);
+    const int first = (int)blockIdx.y * rows, end = min(first + rows, a.N);
+    const T *const in = a.r ? a.s : a.x;
+    const long long stride = a.r ? a.ss : a.xs;
+    int n = end - 1 - warp;
+    uint4 raw[kBandBatch];
+    auto load = [&] {
+#pragma unroll
+        for (int i = 0; i < kBandBatch; ++i)
+            if (n - i * kBandWarps >= first && !line.empty()) raw[i] = line.load(in + (n - i * kBandWarps) * stride);
+    };
+    load();                                                               // on their way beside the parts of the sums, of which each warp adds up some
+    float rstd[kVec] = {};
+#pragma unroll 4
+    for (int b = warp; b < (int)gridDim.y; b += kBandWarps) {
+        float p[kVec];
+        line.load_columns(part + (long long)b * padded, p);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) rstd[j] += p[j];
+    }
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) red[warp][j][lane] = rstd[j];
+    __syncthreads();
+    if (line.empty()) return;
+    const float inv = 1.0f / (float)a.N;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+        float s = red[0][j][lane];
+#pragma unroll
+        for (int w = 1; w < kBandWarps; ++w) s += red[w][j][lane];
+        rstd[j] = 1.0f / sqrtf(fmaf(s, inv, a.eps));
+        if (blockIdx.y == 0 && warp == 0 && line.frame(j) < a.F) a.rstd[line.frame(j)] = rstd[j];
+    }
+    while (n >= first) {
+#pragma unroll
+        for (int i = 0; i < kBandBatch; ++i) {
+            const int m = n - i * kBandWarps;
+            if (m < first) break;
+            const float g = a.gamma ? a.gamma[m] : 1.0f;
+            float w[kVec];
+            unpack<T>(raw[i], w);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) w[j] = (w[j] * rstd[j]) * g;
+            store_once(line, a.y + m * a.ys, w);
+        }
+        n -= kBandWarps * kBandBatch;
+        load();
+    }
+}
+
+// unit[frame] for k_rms_quantize, scale and rstd, from the parts of the bands
+__global__ void __launch_bounds__(256)
+k_rms_scales(const float *__restrict__ part, int bands, int padded, float *unit_out, float *scale_out, float *rstd_out, float eps, int N, int F)
+{
+    grid_dependency();
+    const int f = (int)blockIdx.x * 256 + threadIdx.x;
+    if (f >= F) return;
+    float sum = 0.0f, top = 0.0f;
+#pragma unroll 8
+    for (int b = 0; b < bands; ++b) {
+        sum += part[(long long)b * padded + f];
+        top = max_or_nan(top, part[(long long)(bands + b) * padded + f]);
+    }
+    const float rstd = 1.0f / sqrtf(fmaf(sum, 1.0f / (float)N, eps)), unit = quant_scale(__float_as_uint(top) & 0x7fffffffu);
+    unit_out[f] = unit;
+    scale_out[f] = unit * rstd;
+    if (rstd_out) rstd_out[f] = rstd;
+}
+
+// 256 rows x 128 bytes of s turned over into rows of q, as by k_quantize_apply of the quantisers, from the last rows on
+constexpr int kRmsQuantRows = 256;
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256)
+k_rms_quantize(const T *s, int8_t *q, const float *__restrict__ gamma, const float *__restrict__ unit_in, int N, int F, long long ss, long long qs)
+{
+    grid_dependency();
+    constexpr int kLpr = 8, kPieces = kRmsQuantRows / 16;
+    using Col = Column<T, kLpr>;
+    constexpr int kVec = Col::kVec, kCols = Col::kCols;
+    __shared__ __align__(16) uint32_t tile[kCols][kRmsQuantRows / 4];
+    const Col c;
+    const int f0 = (int)blockIdx.x * kCols, f = f0 + c.col, n0 = (int)(gridDim.y - 1 - blockIdx.y) * kRmsQuantRows, n = n0 + 4 * c.row;
+    uint4 raw[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int m = n + 128 * h + i;
+            raw[h][i] = m < N ? load_frames<T, ALIGNED>(s + m * ss, f, F) : make_uint4(0, 0, 0, 0);
+        }
+    float unit[kVec];
+    load_columns(unit_in, f, F, unit);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float v[4][kVec];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            unpack<T>(raw[h][i], v[i]);
+            const float g = gamma && n + 128 * h + i < N ? gamma[n + 128 * h + i] : 1.0f;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) v[i][j] *= g;
+        }
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+            tile[c.col + j][h * 32 + (c.row / 4 ^ c.lane % kLpr) * 4 + c.row % 4] = Quantizer(unit[j])(v[0][j], v[1][j], v[2][j], v[3][j]);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < kCols * kPieces; e += 256) {
+        const int col = e / kPieces, piece = e % kPieces, m = n0 + 16 * piece;
+        if (f0 + col < F && m < N)
+            *reinterpret_cast<uint4 *>(q + (long long)(f0 + col) * qs + m) = *reinterpret_cast<const uint4 *>(&tile[col][(piece ^ col / kVec) * 4]);
+    }
+}
+
+// backward: part[band][frame] = the band's sum of gamma dy xh
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kBandWarps, 4)
+k_rms_grad_sums(const RmsBackward<T> a, float *part, int rows, int padded)
+{
+    grid_dependency();
+    constexpr int kVec = kFramesPerVec<T>;
+    const Line<T, ALIGNED> line((int)blockIdx.x * 32 * kVec, (int)(threadIdx.x & 31), a.F);
+    const int first = (int)blockIdx.y * rows, end = min(first + rows, a.N);
+    float v[1][kVec] = {}, rstd[kVec];
+    line.load_columns(a.rstd, rstd);
+    for (int n = first + (int)(threadIdx.x >> 5); n < end; n += kBandWarps * kBandBatch) {
+        uint4 s_raw[kBandBatch], d_raw[kBandBatch];
+#pragma unroll
+        for (int i = 0; i < kBandBatch; ++i)
+            if (n + i * kBandWarps < end) {
+                s_raw[i] = line.load(a.s + (n + i * kBandWarps) * a.ss);
+                d_raw[i] = line.load(a.dy + (n + i * kBandWarps) * a.dys);
+            }
+#pragma unroll
+        for (int i = 0; i < kBandBatch; ++i) {
+            const int m = n + i * kBandWarps;
+            if (m >= end) break;
+            const float g = a.gamma ? a.gamma[m] : 1.0f;
+            float s[kVec], d[kVec];
+            unpack<T>(s_raw[i], s);
+            unpack<T>(d_raw[i], d);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) v[0][j] = fmaf(g * d[j], s[j] * rstd[j], v[0][j]);
+        }
+    }
+    store_band<T, ALIGNED, 1>(v, part, (int)gridDim.y, (int)blockIdx.y, padded, line, [](int, float p, float o) { return p + o; });
+}
+
+// mean[frame] = the mean over all rows, from the parts of the bands
+__global__ void __launch_bounds__(256) k_rms_grad_means(const float *__restrict__ part, int bands, int padded, float *mean, int N, int F)
+{
+    grid_dependency();
+    const int f = (int)blockIdx.x * 256 + threadIdx.x;
+    if (f >= F) return;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int b = 0; b < bands; ++b) sum += part[(long long)b * padded + f];
+    mean[f] = sum / (float)N;
+}
+
+// A CTA has 8 x kGradRows rows and every gridDim.x-th piece of 512 bytes of them, and adds up their sums over the frames on the way: gamma_part[blockIdx.x][node].
+// The rows are those of the bands' ends first.
+constexpr int kGradRows = 4;
+template <typename T, bool ALIGNED, bool RESIDUAL>
+__global__ void __launch_bounds__(32 * kBandWarps, 2)
+k_rms_grad_apply(const RmsBackward<T> a, const float *__restrict__ mean_in, int rows, int bands)
+{
+    grid_dependency();
+    constexpr int kVec = kFramesPerVec<T>, R = kGradRows;
+    const int lane = threadIdx.x & 31, band = (int)blockIdx.y % bands, back = (int)blockIdx.y / bands;
+    const int end = min((band + 1) * rows, a.N), top = end - (back * kBandWarps + (int)(threadIdx.x >> 5)) * R, n0 = max(top - R, band * rows);
+    const int mine = top - n0;                                            // rows of the warp, below 1: none
+    float along[R] = {}, gm[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) gm[i] = a.gamma && i < mine ? a.gamma[n0 + i] : 1.0f;
+    if (mine > 0)
+        for (int f0 = (int)blockIdx.x * 32 * kVec; f0 < a.F; f0 += (int)gridDim.x * 32 * kVec) {
+            const Line<T, ALIGNED> line(f0, lane, a.F);
+            if (line.empty()) break;
+            uint4 s_raw[R], d_raw[R], r_raw[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (i < mine) {
+                    s_raw[i] = line.load(a.s + (n0 + i) * a.ss);
+                    d_raw[i] = line.load(a.dy + (n0 + i) * a.dys);
+                    if (RESIDUAL) r_raw[i] = load_once(line, a.dr + (n0 + i) * a.drs);
+                }
+            float rstd[kVec], mean[kVec];
+            line.load_columns(a.rstd, rstd);
+            line.load_columns(mean_in, mean);
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (i < mine) {
+                    float s[kVec], d[kVec], r[kVec] = {};
+                    unpack<T>(s_raw[i], s);
+                    unpack<T>(d_raw[i], d);
+                    if (RESIDUAL) unpack<T>(r_raw[i], r);
+                    if (line.frame(kVec - 1) >= a.F) {                    // what lies beyond the frames may be anything
+#pragma unroll
+                        for (int j = 0; j < kVec; ++j)
+                            if (line.frame(j) >= a.F) s[j] = d[j] = 0.0f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) {
+                        const float xh = s[j] * rstd[j];
+                        along[i] = fmaf(d[j], xh, along[i]);
+                        d[j] = fmaf(rstd[j], fmaf(-xh, mean[j], gm[i] * d[j]), r[j]);
+                    }
+                    store_once(line, a.ds + (n0 + i) * a.dss, d);
+                }
+        }
+    if (!a.gamma_part) return;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) along[i] += __shfl_xor_sync(0xffffffffu, along[i], m);
+        if (lane == i && i < mine) a.gamma_part[(long long)blockIdx.x * a.N + n0 + i] = along[i];
+    }
+}
+
+// Pieces of 512 bytes along the frames, bands that make one round of CTAs, four an SM, with whole batches of rows
+constexpr long long kRmsInL2 = 104 << 20, kRmsFew = 1 << 21;              // bytes, values
+// Backward: us, one launch and two passes: 4096 x 1024 fp32 15.0 / 19.0, 1024 x 4096 20.6 / 16.7, 5000 x 1000 bf16 33 / 20.6, 16384 x 100 fp32 15.1 / 30.8.
+constexpr long long kRmsGradSmall = 1 << 22;             // values
+struct BandPlan { int pieces, bands, rows, padded; };
+template <typename T> static BandPlan plan_bands(int N, int F)
+{
+    constexpr int kWide = 32 * kFramesPerVec<T>, kUnit = kBandWarps * kBandBatch;
+    const int pieces = (F + kWide - 1) / kWide, slots = 4 * device_info().sm_count;
+    const int bands = std::max(1, std::min({slots / pieces, (N + kUnit - 1) / kUnit, 65535}));
+    const int rows = ((N + bands - 1) / bands + kUnit - 1) / kUnit * kUnit;
+    return {pieces, (N + rows - 1) / rows, rows, (F + 3) / 4 * 4};
+}
+
 // Lanes along a row (8, or 2 where frames are few), CTAs of a cluster, and rounds of four rows a thread.
 struct RmsPlan { int lanes, cluster, rounds; unsigned ctas; };
 template <typename T> static RmsPlan plan_rms(int N, int F)
@@ -281,11 +672,36 @@ template <typename T> static RmsPlan plan_rms(int N, int F)
 
 template <typename T, bool INT8> static int rms_forward(RmsForward<T> &a, bool aligned, cudaStream_t st)
 {
+    // The cluster's second reading finds L2 as the first one left it where everything fits there, and costs a latency a round where columns are few and long.  (us, one
+    // launch and two passes: 1024 x 16384 bf16 with a residual 21.1 / 26.4, fp32 55.9 / 49.7; 4096 x 1024 fp32 12.3 / 13.6; 5000 x 1000 bf16 20.4 / 16.4; 16384 x 100 fp32
+    // 13.5 / 27.2.)
     const RmsPlan p = plan_rms<T>(a.N, a.F);
+    const bool held = p.rounds <= kHeldRows / 4;
+    const long long values = (long long)a.N * a.F, bytes = values * (long long)sizeof(T) * (a.r ? 3 : 1);
+    if (!held && (bytes > kRmsInL2 || (p.rounds > 4 && values > kRmsFew))) {
+        const BandPlan b = plan_bands<T>(a.N, a.F);
+        HeldScratch held;
+        float *part = static_cast<float *>(held.get(st, ((size_t)b.bands * (INT8 ? 2 : 1) + 1) * b.padded * sizeof(float)));
+        BB200_REQUIRE(part != nullptr, BBCU_ERR_NO_MEMORY);
+        const dim3 grid((unsigned)b.pieces, (unsigned)b.bands);
+        auto sums = aligned ? (a.r ? k_rms_sums<T, true, true, INT8> : k_rms_sums<T, true, false, INT8>) : (a.r ? k_rms_sums<T, false, true, INT8> : k_rms_sums<T, false, false, INT8>);
+        launch(sums, grid, 32 * kBandWarps, 0, st, a, part, b.rows, b.padded);
+        BB200_CUDA(cudaPeekAtLastError());
+        if constexpr (INT8) {
+            float *const unit = part + 2LL * b.bands * b.padded;
+            constexpr int kCols = Column<T, 8>::kCols;
+            const int bands = (a.N + kRmsQuantRows - 1) / kRmsQuantRows;
+            launch(k_rms_scales, (unsigned)((a.F + 255) / 256), 256, 0, st, part, b.bands, b.padded, unit, a.scale, a.rstd, a.eps, a.N, a.F);
+            launch(aligned ? k_rms_quantize<T, true> : k_rms_quantize<T, false>, dim3((unsigned)((a.F + kCols - 1) / kCols), (unsigned)bands), 256, 0, st, a.r ? a.s : a.x, a.q, a.gamma,
+                   unit, a.N, a.F, a.r ? a.ss : a.xs, a.qs);
+        } else {
+            launch(aligned ? k_rms_apply<T, true> : k_rms_apply<T, false>, grid, 32 * kBandWarps, 0, st, a, part, b.rows, b.padded);
+        }
+        return launch_status();
+    }
     a.rounds = p.rounds;
     a.fault = fault_word();
     BB200_REQUIRE(a.fault != nullptr, BBCU_ERR_NO_DEVICE);
-    const bool held = p.rounds <= kHeldRows / 4;
 #define BB200_RMS(L) (aligned ? (held ? k_rms_forward<T, L, true, INT8, true> : k_rms_forward<T, L, true, INT8, false>)  \
                               : (held ? k_rms_forward<T, L, false, INT8, true> : k_rms_forward<T, L, false, INT8, false>))
     auto kernel = p.lanes == 2 ? BB200_RMS(2) : BB200_RMS(8);
@@ -329,10 +745,29 @@ static int rms_backward_checked(const T *s, const T *dy, const T *dr, T *ds, con
     RmsBackward<T> a{s, dy, dr, ds, gamma, rstd, nullptr, N, F, 0, ss, dys, drs, dss, fault_word()};
     BB200_REQUIRE(a.fault != nullptr, BBCU_ERR_NO_DEVICE);
     const bool aligned = frames_aligned<T>(s, ss) && frames_aligned<T>(dy, dys) && frames_aligned<T>(ds, dss) && (!dr || frames_aligned<T>(dr, drs));
+    HeldScratch held_scratch;
+    if ((long long)N * F > kRmsGradSmall) {
+        const BandPlan b = plan_bands<T>(N, F);
+        const int backs = (b.rows + kBandWarps * kGradRows - 1) / (kBandWarps * kGradRows);
+        const long long groups = (long long)b.bands * backs;
+        BB200_REQUIRE(groups <= 65535, BBCU_ERR_TOO_LARGE);
+        const int sweeps = (int)std::min<long long>(b.pieces, std::max(1LL, (8LL * device_info().sm_count + groups - 1) / groups));
+        const size_t sums = ((size_t)b.bands + 1) * b.padded;
+        float *part = static_cast<float *>(held_scratch.get(st, (sums + (dgamma ? (size_t)sweeps * N : 0)) * sizeof(float)));
+        BB200_REQUIRE(part != nullptr, BBCU_ERR_NO_MEMORY);
+        float *const mean = part + (size_t)b.bands * b.padded;
+        if (dgamma) a.gamma_part = part + sums;
+        launch(aligned ? k_rms_grad_sums<T, true> : k_rms_grad_sums<T, false>, dim3((unsigned)b.pieces, (unsigned)b.bands), 32 * kBandWarps, 0, st, a, part, b.rows, b.padded);
+        BB200_CUDA(cudaPeekAtLastError());
+        launch(k_rms_grad_means, (unsigned)((F + 255) / 256), 256, 0, st, part, b.bands, b.padded, mean, N, F);
+        auto apply = aligned ? (dr ? k_rms_grad_apply<T, true, true> : k_rms_grad_apply<T, true, false>) : (dr ? k_rms_grad_apply<T, false, true> : k_rms_grad_apply<T, false, false>);
+        launch(apply, dim3((unsigned)sweeps, (unsigned)groups), 32 * kBandWarps, 0, st, a, mean, b.rows, b.bands);
+        if (dgamma) launch(k_rms_gamma, (unsigned)((N + 31) / 32), 256, 0, st, a.gamma_part, dgamma, N, sweeps, accumulate);
+        return launch_status();
+    }
     const RmsPlan p = plan_rms<T>(N, F);
     a.rounds = p.rounds;
     const int tiles = (int)(p.ctas / p.cluster);
-    HeldScratch held_scratch;
     if (dgamma) {
         a.gamma_part = static_cast<float *>(held_scratch.get(st, (size_t)tiles * N * sizeof(float)));
         BB200_REQUIRE(a.gamma_part != nullptr, BBCU_ERR_NO_MEMORY);
