@@ -23,6 +23,7 @@ namespace bb200 {
 enum DenseKind { kForward, kGated, kInputGrad, kWeightGrad };
 
 constexpr int kTileM = 128, kTileK = 64;                 // output rows of a CTA; k of a stage (128 bytes)
+constexpr int kChunk = 12;                               // stages of k between two additions in registers, where sums are taken out on the way (see the tiles below)
 constexpr int kMostSplits = 8;
 constexpr int kTileGroup = 8;                            // tiles of output rows that are walked together, so that their operands stay in L2
 
@@ -210,90 +211,116 @@ template <int KIND, typename T> __device__ __forceinline__ void finish_8(const D
     }
 }
 
-// ---- a single frame: what counts is to have W on its way.  A warp has a row of W (a gated block: a row of both products), or one of `splits` parts of its
-// inputs where there are few rows, and asks for 4096 bytes of it before it multiplies; the frame comes out of shared memory, where a CTA has gathered it.
-constexpr int kRowThreads = 1024, kRowInputs = 16384;    // inputs that a CTA holds at a time
+// ---- up to eight frames: what counts is to have W on its way, once.  A CTA has its share of the rows, whatever their number; a warp takes up to 16 rows and a part of the
+// inputs, and each lane has its pieces of W, 16 bytes of two rows a block of 32 inputs, asked for two batches ahead, in registers, from where they go into products of
+// 16 rows x 8 frames (the k of a product may be any, as long as W and the frames have the same: a lane's 16 bytes are two pairs of pairs).  The frames come
+// out of shared memory, where the CTA has turned them over; the parts' sums meet there, in the order of the warps.
+// (Multiplied out by each lane, a single frame took 27 instructions for 16 bytes of W: 4096 -> 2 x 8192 31 us.)
+constexpr int kFewThreads = 512, kFewFrames = 8, kFewInputs = 32768;           // inputs x frames that a CTA holds at a time
+constexpr int few_chunk(int frames) { return kFewInputs / (frames > 4 ? 8 : frames > 2 ? 4 : frames); }
 template <int KIND, typename T>
-__global__ void __launch_bounds__(kRowThreads, 1)
-k_dense_row(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__restrict__ W, long long xs, long long ws, const DenseArgs a)
+__global__ void __launch_bounds__(kFewThreads, 1)
+k_dense_few(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__restrict__ W, long long xs, long long ws, const DenseArgs a, int groups, int chunk)
 {
     grid_dependency();
-    constexpr int kAhead = 8;
-    constexpr int kParts = KIND == kGated ? 2 : 1;
-    __shared__ __align__(16) __nv_bfloat16 frame[kRowInputs];
-    __shared__ float red[kRowThreads / 32][2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % a.splits, per_cta = kRowThreads / 32 / a.splits;
-    const int rows = (a.M + (int)gridDim.x * per_cta - 1) / ((int)gridDim.x * per_cta);       // that a warp takes one after the other
-    float total[kParts] = {};
-    for (int r = 0; r < rows; ++r) {
-        const int m = (r * (int)gridDim.x + (int)blockIdx.x) * per_cta + warp / a.splits;
+    constexpr int kParts = KIND == kGated ? 2 : 1, kBatch = 4 / kParts, kWarps = kFewThreads / 32, kBlock = 32;
+    extern __shared__ __align__(16) uint8_t smem_few[];
+    __nv_bfloat16 *const frames = reinterpret_cast<__nv_bfloat16 *>(smem_few);     // [frame][chunk + 8]
+    __shared__ float sums[kWarps][kParts][16][kFewFrames];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, pitch = chunk + 8;
+    const int first = (int)((long long)a.M * blockIdx.x / gridDim.x), last = (int)((long long)a.M * (blockIdx.x + 1) / gridDim.x);
+    const int group = warp % groups, part = warp / groups, parts = kWarps / groups;
+    for (int m0 = first; m0 < last; m0 += groups * 16) {
+        const int rows = min(groups * 16, last - m0), per_group = (rows + groups - 1) / groups;
+        const int r0 = group * per_group + g, here = min(per_group, rows - group * per_group);      // rows of the group that exist
+        float acc[kParts][4] = {}, total[kParts][4] = {};
+        for (int k0 = 0; k0 < a.K; k0 += chunk) {
+            const int inputs = min(chunk, a.K - k0), blocks = (inputs + kBlock - 1) / kBlock, begin = blocks * part / parts, end = blocks * (part + 1) / parts;
+            const __nv_bfloat16 *const base = W + (long long)(m0 + r0) * ws + k0 + 8 * t;
+            uint4 w[kBatch][kParts][2], next[kBatch][kParts][2];
+            auto fetch = [&](int b, uint4 (&w)[kBatch][kParts][2]) {
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) total[p] = 0.0f;
-        for (int k0 = 0; k0 < a.K; k0 += kRowInputs) {
-            const int inputs = min(kRowInputs, a.K - k0), steps = (inputs + 255) / 256;
-            const int s0 = steps * part / a.splits, s1 = steps * (part + 1) / a.splits;
-            uint4 w[kParts][kAhead / kParts];
-            constexpr int kBatch = kAhead / kParts;
-            auto fetch = [&](int s) {
+                for (int i = 0; i < kBatch; ++i)
 #pragma unroll
-                for (int p = 0; p < kParts; ++p) {
-                    const __nv_bfloat16 *const row = W + (long long)(min(m, a.M - 1) + p * a.half) * ws + k0;
+                    for (int p = 0; p < kParts; ++p)
 #pragma unroll
-                    for (int i = 0; i < kBatch; ++i) {
-                        const int k = (s + i) * 256 + lane * 8;
-                        w[p][i] = s + i < s1 && k < inputs ? __ldg(reinterpret_cast<const uint4 *>(row + k)) : make_uint4(0, 0, 0, 0);
-                    }
-                }
+                        for (int h = 0; h < 2; ++h) {
+                            const int k = (b + i) * kBlock;
+                            w[i][p][h] = b + i < end && k + 8 * t < inputs && g + 8 * h < here
+                                             ? __ldg(reinterpret_cast<const uint4 *>(base + (long long)(8 * h + p * a.half) * ws + k)) : make_uint4(0, 0, 0, 0);
+                        }
             };
-            fetch(s0);
-            if (r == 0 || a.K > kRowInputs) {
+            fetch(begin, w);
+            if (m0 == first || a.K > chunk) {
                 __syncthreads();
-                for (int k = threadIdx.x; k < (inputs + 7) / 8 * 8; k += kRowThreads)
-                    frame[k] = k < inputs ? x[(long long)(k0 + k) * xs] : __nv_bfloat16(0.0f);
+#pragma unroll 4
+                for (int k = threadIdx.x; k < blocks * kBlock; k += kFewThreads) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (k < inputs) v = *reinterpret_cast<const uint4 *>(x + (long long)(k0 + k) * xs);
+                    const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int f = 0; f < kFewFrames; ++f)
+                        if (f < a.N) reinterpret_cast<uint16_t *>(frames)[f * pitch + k] = (uint16_t)(word[f / 2] >> (16 * (f % 2)));
+                }
                 __syncthreads();
             }
-            for (int s = s0; s < s1; s += kBatch) {
-                if (s > s0) fetch(s);
+            for (int b = begin, done = 0; b < end; b += kBatch) {
+                fetch(b + kBatch, next);
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {
-                    const int k = (s + i) * 256 + lane * 8;
-                    if (s + i < s1 && k < inputs) {
-                        float v[8];
-                        load_8<__nv_bfloat16>(frame + k, v);
+                    if (b + i >= end) break;
+                    const int k = (b + i) * kBlock + 8 * t;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (g < a.N) v = *reinterpret_cast<const uint4 *>(frames + g * pitch + k);
+                    if (k + 8 > inputs) {                                 // the padding of W may hold anything
+                        const int left = inputs - k;
 #pragma unroll
-                        for (int p = 0; p < kParts; ++p) {
-                            float u[8];
-                            unpack<__nv_bfloat16>(w[p][i], u);
-                            if (k + 8 > inputs) {                         // the padding of W may hold anything
+                        for (int p = 0; p < kParts; ++p)
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) u[j] = k + j < inputs ? u[j] : 0.0f;
+                            for (int h = 0; h < 2; ++h) {
+                                uint32_t *const word = reinterpret_cast<uint32_t *>(&w[i][p][h]);
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) word[q] = left >= 2 * q + 2 ? word[q] : left == 2 * q + 1 ? word[q] & 0xffffu : 0u;
                             }
+                    }
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) total[p] = fmaf(u[j], v[j], total[p]);
-                        }
+                    for (int p = 0; p < kParts; ++p) {
+                        mma_rows_bf16(acc[p], w[i][p][0].x, w[i][p][1].x, w[i][p][0].y, w[i][p][1].y, v.x, v.y);
+                        mma_rows_bf16(acc[p], w[i][p][0].z, w[i][p][1].z, w[i][p][0].w, w[i][p][1].w, v.z, v.w);
                     }
                 }
+                done += kBatch;
+                if (sizeof(T) == 4 && done >= kChunk * kTileK / kBlock) {  // the tensor cores cut what does not fit their running sum, see kChunk
+                    done = 0;
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { total[p][j] += acc[p][j]; acc[p][j] = 0.0f; }
+                }
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) w[i][p][h] = next[i][p][h];
             }
         }
 #pragma unroll
         for (int p = 0; p < kParts; ++p)
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) total[p] += __shfl_xor_sync(0xffffffffu, total[p], d);
-        if (a.splits > 1) {
-            __syncthreads();
-            if (lane == 0)
+            for (int j = 0; j < 4; ++j) sums[warp][p][g + (j >= 2 ? 8 : 0)][2 * t + j % 2] = total[p][j] + acc[p][j];
+        __syncthreads();
+        if ((int)threadIdx.x < rows) {
+            const int from = threadIdx.x / per_group, row = threadIdx.x % per_group;
+            float v[2][8] = {};
+            for (int i = 0; i < parts; ++i)
 #pragma unroll
-                for (int p = 0; p < kParts; ++p) red[warp][p] = total[p];
-            __syncthreads();
-            if (part == 0)
-                for (int i = 1; i < a.splits; ++i)
+                for (int p = 0; p < kParts; ++p)
 #pragma unroll
-                    for (int p = 0; p < kParts; ++p) total[p] += red[warp + i][p];
+                    for (int f = 0; f < kFewFrames; ++f) v[p][f] += sums[i * groups + from][p][row][f];
+            finish_8<KIND, T>(a, m0 + threadIdx.x, 0, v[0], v[kParts - 1]);
         }
-        if (part == 0 && lane == 0 && m < a.M) {
-            float v[1] = {total[0]}, w[1] = {total[kParts - 1]};
-            finish<KIND, T, 1>(a, m, 0, v, w);
-        }
+        __syncthreads();
     }
 }
 
@@ -317,7 +344,6 @@ template <int KIND, typename T, int TN, bool PAIR> struct DenseShape {
     static constexpr int kAccColumns = kParts * TN, kColumns = 2 * kAccColumns < 32 ? 32 : 2 * kAccColumns;
     static constexpr int kWarpColumns = TN * 4 / kWarps < kPiece ? kPiece : TN * 4 / kWarps;  // a warp's share of a tile's columns
 };
-constexpr int kChunk = 12;                               // stages of k between two additions in registers
 
 // A warp's 32 rows, a row a lane, of P pieces of eight columns (fp32: of four) to memory (`base`: the first row at the first column, `rows` and `left` columns of it
 // exist): they cross shared memory, where the order of a row's pieces differs from row to row so that no banks collide, and leave as P * 16 bytes of a row; at odd
@@ -898,13 +924,15 @@ template <int KIND, typename T> static int dense_product(const Operand &A, const
     }
 }
 
-template <int KIND, typename T> static int dense_row(const __nv_bfloat16 *x, const __nv_bfloat16 *W, long long xs, long long ws, DenseArgs &a, cudaStream_t st)
+template <int KIND, typename T> static int dense_few(const __nv_bfloat16 *x, const __nv_bfloat16 *W, long long xs, long long ws, DenseArgs &a, cudaStream_t st)
 {
-    const int sms = device_info().sm_count, per_cta = kRowThreads / 32, steps = (std::min(a.K, kRowInputs) + 255) / 256;
-    a.splits = 1;
-    while (a.splits < 8 && (long long)a.M * a.splits < 16LL * sms && steps >= 2 * a.splits) a.splits *= 2;
-    const long long ctas = ((long long)a.M * a.splits + per_cta - 1) / per_cta;
-    launch(k_dense_row<KIND, T>, (unsigned)std::min<long long>(ctas, sms), kRowThreads, 0, st, x, W, xs, ws, a);
+    const int ctas = std::min(a.M, device_info().sm_count), rows = (a.M + ctas - 1) / ctas;
+    int groups = 1;
+    while (groups < kFewThreads / 32 && rows > 16 * groups) groups *= 2;
+    const int chunk = std::min(few_chunk(a.N), (a.K + 31) / 32 * 32), smem = (a.N * (chunk + 8) + 8) * 2;
+    auto kernel = k_dense_few<KIND, T>;
+    BB200_REQUIRE(allow_big_smem(kernel, (kFewInputs + 9 * 8) * 2), (int)cudaErrorInvalidValue);
+    launch(kernel, (unsigned)ctas, kFewThreads, (size_t)smem, st, x, W, xs, ws, a, groups, chunk);
     return launch_status();
 }
 
@@ -930,9 +958,9 @@ static int dense_forward(bool gated, const bbcu_bf16_t *x_, const bbcu_bf16_t *W
     cudaStream_t st = as_stream(stream);
     const Operand A = {W, K, gated ? 2LL * O : O, ws}, B = {x, F, K, xs};
     if constexpr (sizeof(T) == 2) {
-        if (gated) return F == 1 ? dense_row<kGated, T>(x, W, xs, ws, a, st) : dense_product<kGated, T>(A, B, a, st);
+        if (gated) return F <= kFewFrames ? dense_few<kGated, T>(x, W, xs, ws, a, st) : dense_product<kGated, T>(A, B, a, st);
     }
-    return F == 1 ? dense_row<kForward, T>(x, W, xs, ws, a, st) : dense_product<kForward, T>(A, B, a, st);
+    return F <= kFewFrames ? dense_few<kForward, T>(x, W, xs, ws, a, st) : dense_product<kForward, T>(A, B, a, st);
 }
 
 }   // namespace bb200

@@ -132,6 +132,14 @@ template <bool PAIR> __device__ __forceinline__ void mma_bf16(uint32_t tmem, uin
                      ::"r"(tmem), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)accumulate) : "memory");
 }
 
+// A warp's own product in registers, 16 rows x 16 of k times 16 of k x 8 columns: for operands that come once and are not worth the way through shared memory.
+// Lane 4 g + t has the pairs t and t + 4 of k of rows g and g + 8 (a) and of column g (b), and columns 2 t and 2 t + 1 of those rows of the sums.
+__device__ __forceinline__ void mma_rows_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t a, uint64_t b, uint32_t instr, bool accumulate)
 {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
