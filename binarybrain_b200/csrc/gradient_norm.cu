@@ -5,14 +5,15 @@
 //
 // Squares are added up in 64 bits, so that neither large nor small gradients leave the range of the sum, in an order that the sizes alone decide.
 //
-// Memory bounds it: a gradient is read for the norm and again for what follows it.  The second kernel goes through the tensors and their elements from the
-// end, where L2 still holds what the first one has read last, and marks everything else as read and written once.
+// Memory bounds it: a gradient is read for the norm and again for what follows it.  The second kernel goes through the pieces of the tensors from the end, each by
+// the CTA that had it before, since L2 still holds what has been read last, and marks everything else as read and written once.  (Clipped Adam of 6 x 65536 x 64: 126 us,
+// from the end by other CTAs 129; the plain step 112, the norm alone 15.)
 #include "adam.cuh"
 #include "common.cuh"
 
 namespace bb200 {
 
-constexpr int kNormThreads = 512, kNormCtasPerSm = 2, kNormBatch = 4;
+constexpr int kNormThreads = 512, kNormCtasPerSm = 2;
 
 __device__ __forceinline__ double block_total(double v, double *smem)      // in every thread
 {
@@ -26,27 +27,74 @@ __device__ __forceinline__ double block_total(double v, double *smem)      // in
     return v;
 }
 
-// part[CTA] = the sum of the squares of its pieces of all tensors
+// The tensors in pieces of kPieceSize elements (kSmallPiece where those would leave most CTAs without one), numbered through for 512 tensors at a time; the CTAs take
+// turns at them, from the first or, BACK, from the last one.  f(tensor, first element, count) is called by the whole CTA.  (Tensor by tensor, each over all
+// threads, 200 tensors of 1000 took 250 us, now 8.  Pieces of 4096: 6 x 65536 x 64 130 us, of 8192 126; four small tensors 7.8 and 9.5.)
+constexpr int kPieceSize = 8192, kSmallPiece = 2048;
+template <bool BACK, typename F> __device__ __forceinline__ void for_pieces(int size, const int *__restrict__ size_table, F f)
+{
+    __shared__ int start[kNormThreads + 1], warp_sum[kNormThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tables = (size + kNormThreads - 1) / kNormThreads;
+    for (int k = 0; k < tables; ++k) {
+        const int t0 = (BACK ? tables - 1 - k : k) * kNormThreads, count = min(kNormThreads, size - t0);
+        const long long size_here = (int)threadIdx.x < count ? size_table[t0 + threadIdx.x] : 0;
+        auto number = [&](int piece) {
+            int n = (int)((size_here + piece - 1) / piece);
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int before = __shfl_up_sync(0xffffffffu, n, d);
+                if (lane >= d) n += before;
+            }
+            __syncthreads();                                              // the numbers before are done with
+            if (lane == 31) warp_sum[warp] = n;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) n += warp_sum[w];
+            start[threadIdx.x + 1] = n;
+            if (threadIdx.x == 0) start[0] = 0;
+            __syncthreads();
+        };
+        int piece = kPieceSize;
+        number(piece);
+        if (start[count] * 4 <= (int)gridDim.x) number(piece = kSmallPiece);
+        const int total = start[count], step = (int)gridDim.x;
+        int t = 0;
+        for (int c = BACK ? (total - 1 - (int)blockIdx.x) / step * step + (int)blockIdx.x : (int)blockIdx.x; c >= (int)blockIdx.x && c < total; c += BACK ? -step : step) {
+            if (c < start[t] || c >= start[t + 1]) {                      // the last tensor that starts at or before the piece and is not empty
+                int lo = 0, hi = count - 1;
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) / 2;
+                    if (start[mid] <= c) lo = mid; else hi = mid - 1;
+                }
+                t = lo;
+            }
+            const int first = (c - start[t]) * piece;
+            f(t0 + t, first, min(piece, size_table[t0 + t] - first));
+        }
+    }
+}
+
+// part[CTA] = the sum of the squares of its pieces
 __global__ void __launch_bounds__(kNormThreads, kNormCtasPerSm)
 k_gradient_squares(int size, const int *__restrict__ size_table, float *const *__restrict__ grads, double *part)
 {
     grid_dependency();
     __shared__ double red[kNormThreads / 32];
-    const int threads = gridDim.x * kNormThreads, id = blockIdx.x * kNormThreads + threadIdx.x;
     double sum = 0.0;
     auto add = [&](float g) { sum = fma((double)g, (double)g, sum); };
-    for (int t = 0; t < size; ++t) {
-        const float *g = grads[t];
-        const int n = size_table[t], quads = (reinterpret_cast<uintptr_t>(g) & 15) == 0 ? n / 4 : 0;
-        for (long long i = id; i < quads; i += (long long)kNormBatch * threads) {
-            float4 q[kNormBatch];
+    for_pieces<false>(size, size_table, [&](int t, int first, int count) {
+        const float *g = grads[t] + first;
+        const int quads = (reinterpret_cast<uintptr_t>(g) & 15) == 0 ? count / 4 : 0;
+        float4 q[kPieceSize / 4 / kNormThreads];
 #pragma unroll
-            for (int b = 0; b < kNormBatch; ++b) q[b] = i + (long long)b * threads < quads ? reinterpret_cast<const float4 *>(g)[i + (long long)b * threads] : make_float4(0, 0, 0, 0);
-#pragma unroll
-            for (int b = 0; b < kNormBatch; ++b) { add(q[b].x); add(q[b].y); add(q[b].z); add(q[b].w); }
+        for (int i = 0; i < kPieceSize / 4 / kNormThreads; ++i) {
+            const int k = threadIdx.x + i * kNormThreads;
+            q[i] = k < quads ? reinterpret_cast<const float4 *>(g)[k] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        for (long long i = 4LL * quads + id; i < n; i += threads) add(g[i]);
-    }
+#pragma unroll
+        for (int i = 0; i < kPieceSize / 4 / kNormThreads; ++i) { add(q[i].x); add(q[i].y); add(q[i].z); add(q[i].w); }
+#pragma unroll 4
+        for (int i = 4 * quads + threadIdx.x; i < count; i += kNormThreads) add(g[i]);
+    });
     sum = block_total(sum, red);
     if (threadIdx.x == 0) part[blockIdx.x] = sum;
 }
@@ -77,18 +125,17 @@ k_gradient_clip(int size, const int *__restrict__ size_table, float *const *__re
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const float factor = clip_factor(norm, max_norm);
     if (factor == 1.0f) return;                                           // nothing changes
-    const int threads = gridDim.x * kNormThreads, id = blockIdx.x * kNormThreads + threadIdx.x;
-    for (int t = size - 1; t >= 0; --t) {
-        float *g = grads[t];
-        const int n = size_table[t], quads = (reinterpret_cast<uintptr_t>(g) & 15) == 0 ? n / 4 : 0;
-        for (long long k = id; k < quads; k += threads) {
-            float4 *at = reinterpret_cast<float4 *>(g) + (quads - 1 - k);
-            float4 q = *at;
+    for_pieces<true>(size, size_table, [&](int t, int first, int count) {
+        float *g = grads[t] + first;
+        const int quads = (reinterpret_cast<uintptr_t>(g) & 15) == 0 ? count / 4 : 0;
+#pragma unroll 2
+        for (int i = threadIdx.x; i < quads; i += kNormThreads) {
+            float4 q = reinterpret_cast<float4 *>(g)[i];
             q.x *= factor; q.y *= factor; q.z *= factor; q.w *= factor;
-            __stcs(at, q);
+            __stcs(reinterpret_cast<float4 *>(g) + i, q);
         }
-        for (long long i = 4LL * quads + id; i < n; i += threads) g[i] *= factor;
-    }
+        for (int i = 4 * quads + threadIdx.x; i < count; i += kNormThreads) g[i] *= factor;
+    });
 }
 
 template <bool CLEAR>
@@ -100,14 +147,12 @@ k_adam_clipped(int size, const int *__restrict__ size_table, float *const *__res
     const double norm = norm_of(part, parts);
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const float factor = clip_factor(norm, max_norm);
-    const int threads = gridDim.x * kNormThreads, id = blockIdx.x * kNormThreads + threadIdx.x;
-    for (int t = size - 1; t >= 0; --t) {
-        float *p = params[t], *m = m_tab[t], *v = v_tab[t], *g = grads[t];
-        const int n = size_table[t];
+    for_pieces<true>(size, size_table, [&](int t, int first, int count) {
+        float *p = params[t] + first, *m = m_tab[t] + first, *v = v_tab[t] + first, *g = grads[t] + first;
         const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(g)) & 15) == 0;
-        const int quads = vec ? n / 4 : 0;
-        for (long long k = id; k < quads; k += threads) {
-            const long long i = quads - 1 - k;
+        const int quads = vec ? count / 4 : 0;
+#pragma unroll 2
+        for (int i = threadIdx.x; i < quads; i += kNormThreads) {
             float4 gq = reinterpret_cast<float4 *>(g)[i], pq = __ldcs(reinterpret_cast<float4 *>(p) + i), mq = __ldcs(reinterpret_cast<float4 *>(m) + i),
                    vq = __ldcs(reinterpret_cast<float4 *>(v) + i);
             adam_step(pq.x, gq.x * factor, mq.x, vq.x, lr_t, beta1, beta2);
@@ -119,7 +164,7 @@ k_adam_clipped(int size, const int *__restrict__ size_table, float *const *__res
             __stcs(reinterpret_cast<float4 *>(v) + i, vq);
             if (CLEAR) __stcs(reinterpret_cast<float4 *>(g) + i, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
         }
-        for (long long i = 4LL * quads + id; i < n; i += threads) {
+        for (int i = 4 * quads + threadIdx.x; i < count; i += kNormThreads) {
             float pi = p[i], mi = m[i], vi = v[i];
             adam_step(pi, g[i] * factor, mi, vi, lr_t, beta1, beta2);
             p[i] = pi;
@@ -127,7 +172,7 @@ k_adam_clipped(int size, const int *__restrict__ size_table, float *const *__res
             v[i] = vi;
             if (CLEAR) g[i] = 0.0f;
         }
-    }
+    });
 }
 
 // the squares of all gradients as `parts` partial sums; null with a status set where there is no scratch
