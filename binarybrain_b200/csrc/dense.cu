@@ -888,22 +888,26 @@ static int dense_tiles(const Operand &A, const Operand &B, const DenseArgs &a, c
     return launch_cluster(kernel, cluster, grid, S::kThreads, S::kSmem, st, map_a, map_b, a);
 }
 
-// Columns a tile (0: by a pair of CTAs) and CTAs that share the k of one, by the clocks of an SM: rounds of tiles times stages of k times what a stage
-// costs -- 256 a product of 128 x 128 where the tensor cores bound, more where bringing the operands does -- and what it takes to store a tile.
+// Columns a tile (0: by a pair of CTAs) and CTAs that share the k of one, by what they take in nanoseconds, measured with one tile an SM: a stage of k 325 whatever the
+// columns (a CTA's 24 to 32 KB come at about 50 bytes a clock; both products of a gated block 505), by a pair 410 (540); to start and to store 3700 and some for
+// each column, by a pair 7000; to join sums in a cluster 1500 and more for columns and CTAs.  A cluster has one tile, so that there are no more of them than
+// the device holds (clusters of eight: fewer than its SMs would make; 1024 x 1024 x 64 7.5 us by four CTAs, 12.9 where 16 clusters of eight took two rounds).
+// Of 36 shapes from 420 x 70 x 512 to 4096 x 4096 x 1000 the choice is within 3 % of the best one, two within 9 %.
 struct DenseTiles { int columns, splits; };
-static DenseTiles choose_dense_tiles(int M, int N, int K, int parts)
+static DenseTiles choose_dense_tiles(int M, int N, int K, int parts, const int (&clusters)[4])
 {
     const long long sms = device_info().sm_count, blocks = (K + kTileK - 1) / kTileK, tiles_m = ((long long)M + kTileM - 1) / kTileM;
     const int pair_n = parts == 2 ? 128 : 256;
     const long long pair_tiles = ((long long)M + 2 * kTileM - 1) / (2 * kTileM) * (((long long)N + pair_n - 1) / pair_n);
     DenseTiles best = {0, 1};
-    long long least = (pair_tiles + sms / 2 - 1) / (sms / 2) * blocks * 512 + 3000;
+    long long least = (pair_tiles + sms / 2 - 1) / (sms / 2) * blocks * (parts == 2 ? 540 : 410) + 7000;
     for (int columns = 32; columns <= 128; columns *= 2) {
         const long long tiles = tiles_m * (((long long)N + columns - 1) / columns);
-        for (int splits = 1; splits <= kMostSplits; splits *= 2) {
-            if (splits > 1 && (tiles * splits > sms || blocks < 2 * splits)) break;
-            const long long cost = (tiles * splits + sms - 1) / sms * ((blocks + splits - 1) / splits) * 2 * (kTileM * parts + columns) + 12 * columns * parts +
-                                   (splits > 1 ? 2500 : 0);
+        for (int splits = 1, i = 0; splits <= kMostSplits; splits *= 2, ++i) {
+            if (splits > 1 && (tiles > clusters[i] || blocks < 2 * splits)) break;
+            const long long rounds = splits > 1 ? 1 : (tiles + sms - 1) / sms;
+            const long long cost = rounds * ((blocks + splits - 1) / splits) * (parts == 2 ? 505 : 325) + 3700 + columns * (parts == 2 ? 14 : 6) + (rounds - 1) * 8 * columns * parts +
+                                   (splits > 1 ? 1500 + (splits > 2 ? 26 : 14) * columns * parts : 0);
             if (cost < least) { least = cost; best = {columns, splits}; }
         }
     }
@@ -914,7 +918,12 @@ template <int KIND, typename T> static int dense_product(const Operand &A, const
 {
     a.fault = fault_word();
     BB200_REQUIRE(a.fault != nullptr, BBCU_ERR_NO_DEVICE);
-    const DenseTiles t = choose_dense_tiles(a.M, a.N, a.K, KIND == kGated ? 2 : 1);
+    int clusters[4];
+    using S = DenseShape<KIND, T, 64, false>;
+    auto kernel = k_dense_tiles<KIND, T, 64, false>;
+    BB200_REQUIRE(allow_big_smem(kernel, S::kSmem), (int)cudaErrorInvalidValue);
+    for (int i = 0; i < 4; ++i) clusters[i] = resident_clusters(reinterpret_cast<const void *>(kernel), 1 << i, S::kThreads, S::kSmem);
+    const DenseTiles t = choose_dense_tiles(a.M, a.N, a.K, KIND == kGated ? 2 : 1, clusters);
     a.splits = t.splits;
     switch (t.columns) {
     case 32: return dense_tiles<KIND, T, 32, false>(A, B, a, st);
