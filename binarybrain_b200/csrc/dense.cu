@@ -329,18 +329,25 @@ k_dense_few(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__restrict
 // products of the next.  Where there are fewer tiles than SMs, a cluster of CTAs shares the k of one: their sums cross through distributed shared memory and
 // are added in the order of the CTAs.
 //
+// Both products of a gated block: a CTA brings both operands' rows and has two accumulators, so that a lane has both sums of its row; a pair would bring 40 KB a stage
+// that way, and 50 bytes a clock are what an SM gets.  A pair's tile is 128 rows x 256 columns of the output instead, 64 rows of either product in the 128
+// lanes of a CTA, and the warps of the lower lanes get the second product's sums from those of the upper ones through shared memory.
+//
 // fp32 outputs: the tensor cores cut the digits that do not fit their running sum, which over thousands of steps drifts towards zero; those sums are taken out
 // after every kChunk stages and added up in registers.  (Error of the 2-norm of dW, 4096 x 4096 x 8192, and of y: 4.8e-7 at 8 stages, 7.2e-7 at 12, 1.0e-6 at 16, 2.1e-6 at
 // 32; plain fp32 1e-6.  Taking them out stands in the products' way in TMEM: dW 246, 239, 236 us at 8, 12, 16.)
 template <int KIND, typename T, int TN, bool PAIR> struct DenseShape {
     static constexpr bool kAAcross = KIND == kInputGrad, kBAcross = KIND != kWeightGrad, kPromote = sizeof(T) == 4;
-    static constexpr int kParts = KIND == kGated ? 2 : 1, kOwnN = PAIR ? TN / 2 : TN, kBRows = kBAcross && kOwnN < 64 ? 64 : kOwnN;
+    static constexpr bool kStacked = KIND == kGated && PAIR;
+    static constexpr int kRows = PAIR && !kStacked ? 2 * kTileM : kTileM, kOwnRows = kStacked ? kTileM / 2 : kTileM;      // output rows of a tile, of a CTA
+    static constexpr int kParts = KIND == kGated && !PAIR ? 2 : 1, kOwnN = PAIR ? TN / 2 : TN, kBRows = kBAcross && kOwnN < 64 ? 64 : kOwnN;
     static constexpr int kABytes = kTileM * kTileK * 2, kStageBytes = kParts * kABytes + kBRows * kTileK * 2;
     static constexpr int kWarps = 16, kThreads = 64 + 32 * kWarps;        // warp 0 copies, warp 1 issues the products, the others take the sums out of TMEM
     static constexpr int kPiece = kPromote || KIND == kGated ? 16 : 32;   // columns that a warp takes at a time
     static constexpr int kOutBytes = 32 * kPiece * (int)sizeof(T);
-    static constexpr int kRoom = 225 * 1024 - kWarps * kOutBytes, kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
-    static constexpr int kSmem = kStages * kStageBytes + kWarps * kOutBytes + 1024;
+    static constexpr int kCross = kStacked ? kWarps / 2 : 0, kCrossBytes = 2 * 32 * kPiece * 4;        // pairs of warps that exchange sums, two buffers each
+    static constexpr int kRoom = 225 * 1024 - kWarps * kOutBytes - kCross * kCrossBytes, kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
+    static constexpr int kSmem = kStages * kStageBytes + kWarps * kOutBytes + kCross * kCrossBytes + 1024;
     static constexpr int kAccColumns = kParts * TN, kColumns = 2 * kAccColumns < 32 ? 32 : 2 * kAccColumns;
     static constexpr int kWarpColumns = TN * 4 / kWarps < kPiece ? kPiece : TN * 4 / kWarps;  // a warp's share of a tile's columns
 };
@@ -469,7 +476,7 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     static_assert(kStages >= 4 && kParts * kTileM * (TN + 4) * 4 <= kStages * S::kStageBytes, "shared memory");
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full[kStages], empty[kStages], acc_full[kAcc], acc_empty[kAcc], drained;
+    __shared__ uint64_t full[kStages], empty[kStages], acc_full[kAcc], acc_empty[kAcc], drained, cross_full[S::kStacked ? S::kCross : 1][2], cross_empty[S::kStacked ? S::kCross : 1][2];
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -479,6 +486,8 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int s = 0; s < kAcc; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], PAIR ? 2 * S::kWarps : S::kWarps); }
         mbar_init(&drained, 1);
+        if (S::kStacked)
+            for (int i = 0; i < 2 * S::kCross; ++i) { mbar_init(&cross_full[i / 2][i % 2], 1); mbar_init(&cross_empty[i / 2][i % 2], 1); }
         gave_up = 0;
         mbar_init_fence();
         tma_prefetch(&map_a);
@@ -496,14 +505,14 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     const uint32_t tmem = tmem_base;
     grid_dependency();
 
-    constexpr int kRows = PAIR ? 2 * kTileM : kTileM;
+    constexpr int kRows = S::kRows;
     const int tiles_m = (a.M + kRows - 1) / kRows, tiles_n = (a.N + TN - 1) / TN, tiles = tiles_m * tiles_n;
     const int blocks_k = (a.K + kTileK - 1) / kTileK, splits = PAIR ? 1 : a.splits;
     const int k0 = PAIR ? 0 : (int)((long long)blocks_k * rank / splits), k1 = PAIR ? blocks_k : (int)((long long)blocks_k * (rank + 1) / splits);
     const int first = (int)blockIdx.x / (PAIR ? 2 : splits), step = (int)gridDim.x / (PAIR ? 2 : splits);
     auto place = [&](int tile, int &m0, int &n0) {
         const int group = tile / (kTileGroup * tiles_n), in = tile % (kTileGroup * tiles_n), rows = min(kTileGroup, tiles_m - group * kTileGroup);
-        m0 = (group * kTileGroup + in % rows) * kRows + (PAIR ? (int)rank * kTileM : 0);
+        m0 = (group * kTileGroup + in % rows) * kRows + (PAIR ? (int)rank * S::kOwnRows : 0);
         n0 = in / rows * TN;
     };
 
@@ -527,7 +536,10 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                 };
 #pragma unroll
                 for (int p = 0; p < kParts; ++p) {
-                    if constexpr (S::kAAcross) {
+                    if constexpr (S::kStacked) {
+                        load(at, &map_a, kb * kTileK, m0);
+                        load(at + S::kABytes / 2, &map_a, kb * kTileK, m0 + a.half);
+                    } else if constexpr (S::kAAcross) {
                         load(at, &map_a, m0, kb * kTileK);
                         load(at + S::kABytes / 2, &map_a, m0 + 64, kb * kTileK);
                     } else {
@@ -549,7 +561,7 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             for (int b = issued > kStages ? issued - kStages : 0; b < issued; ++b)
                 mbar_wait_some(&full[b % kStages], (uint32_t)(b / kStages) & 1u, kDrainSpins);
     } else if (warp == 1 && lane == 0 && (!PAIR || rank == 0)) {
-        constexpr uint32_t kInstr = mma_bf16_instruction(kRows, TN, S::kAAcross, S::kBAcross);
+        constexpr uint32_t kInstr = mma_bf16_instruction(PAIR ? 2 * kTileM : kTileM, TN, S::kAAcross, S::kBAcross);
         constexpr uint32_t kHalfBox = 64 * kTileK * 2;                    // 64 rows along m or n of a stage
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
@@ -590,7 +602,9 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     } else if (warp >= 2) {
         const int part = warp & 3, c0 = (warp - 2) / 4 * S::kWarpColumns;  // the lanes of TMEM that this warp may read, its first column
         uint4 *const stage_out = reinterpret_cast<uint4 *>(smem + kStages * S::kStageBytes + (warp - 2) * S::kOutBytes);
-        int acc = 0;
+        uint8_t *const cross = smem + kStages * S::kStageBytes + S::kWarps * S::kOutBytes;
+        const int cross_pair = (warp - 2) / 4 * 2 + (part & 1), lower = part < 2;
+        int acc = 0, turn = 0;
         uint32_t acc_phase = 0;
         const uint32_t arrive = PAIR ? peer_addr(&acc_empty[0], 0) : smem_addr(&acc_empty[0]);
         auto give_back = [&] {
@@ -606,11 +620,11 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             int m0, n0;
             place(tile, m0, n0);
             // what a lane has is a row; the epilogue's inputs of its first columns are on their way before the sums are there
-            const int m = m0 + part * 32, row = min(m + lane, a.M - 1);
+            const int m = m0 + (S::kStacked ? part & 1 : part) * 32, row = min(m + lane, a.M - 1);
             float bias[2] = {0.0f, 0.0f};
             if (KIND <= kGated && a.bias) {
-                bias[0] = a.bias[row];
-                if (KIND == kGated) bias[1] = a.bias[a.half + row];
+                bias[0] = a.bias[S::kStacked && !lower ? a.half + row : row];
+                if (KIND == kGated && !S::kStacked) bias[1] = a.bias[a.half + row];
             }
             constexpr bool kExtra = sizeof(T) == 2 && (KIND == kForward || KIND == kInputGrad);
             uint4 extra[2][kPiece / 8];
@@ -685,7 +699,7 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     for (int j = 0; j < kPiece; ++j) v[j] = __float_as_int(sums[i + j]);
                 } else {
                     tmem_load(at + i, v);
-                    if constexpr (KIND == kGated) tmem_load(at + TN + i, w);
+                    if constexpr (KIND == kGated && !S::kStacked) tmem_load(at + TN + i, w);
                     if (i + kPiece >= S::kWarpColumns || left <= kPiece) {        // the last of its columns: the next tile's products may have them
                         give_back();
                         returned = true;
@@ -734,6 +748,44 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     else made([&](int j) { return __int_as_float(v[j]); });
                     fetch_extra(i + kPiece);
                     store_rows(stage_out, out, base, a.out_stride, rows, left, a.vec);
+                } else if constexpr (S::kStacked) {
+                    if (a.bias) {
+#pragma unroll
+                        for (int j = 0; j < kPiece; ++j) v[j] = __float_as_int(__int_as_float(v[j]) + bias[0]);
+                    }
+                    const int b = turn & 1;
+                    const uint32_t phase = turn >> 1 & 1;
+                    uint4 *const at_cross = reinterpret_cast<uint4 *>(cross + (cross_pair * 2 + b) * 32 * kPiece * 4);
+                    ++turn;
+                    if (!lower) {
+                        ok = mbar_wait_warp(&cross_empty[cross_pair][b], phase ^ 1, &gave_up);
+                        if (!ok) break;
+#pragma unroll
+                        for (int q = 0; q < kPiece / 4; ++q)
+                            at_cross[staged_piece<kPiece / 4>(lane, q)] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&cross_full[cross_pair][b]);
+                        if (z_base) {
+                            made([&](int j) { return __int_as_float(v[j]); });
+                            store_rows(stage_out, out, z_base + a.half * a.z_stride, a.z_stride, rows, left, a.vec);
+                        }
+                    } else {
+                        ok = mbar_wait_warp(&cross_full[cross_pair][b], phase, &gave_up);
+                        if (!ok) break;
+#pragma unroll
+                        for (int q = 0; q < kPiece / 4; ++q) {
+                            const uint4 p = at_cross[staged_piece<kPiece / 4>(lane, q)];
+                            w[4 * q] = (int)p.x; w[4 * q + 1] = (int)p.y; w[4 * q + 2] = (int)p.z; w[4 * q + 3] = (int)p.w;
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&cross_empty[cross_pair][b]);
+                        with_activation(a.act, [&](auto act) { made([&](int j) { return curve<decltype(act)::value, sizeof(T) == 2>(__int_as_float(v[j])).value * __int_as_float(w[j]); }); });
+                        store_rows(stage_out, out, base, a.out_stride, rows, left, a.vec);
+                        if (z_base) {
+                            made([&](int j) { return __int_as_float(v[j]); });
+                            store_rows(stage_out, out, z_base, a.z_stride, rows, left, a.vec);
+                        }
+                    }
                 } else if constexpr (KIND == kGated) {
                     if (a.bias) {
 #pragma unroll
@@ -780,6 +832,7 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     store_rows(stage_out, out, base, a.out_stride, rows, left, a.vec);
                 }
             }
+            if (!ok) break;
             if (!returned) give_back();
         }
     }
@@ -838,11 +891,17 @@ k_dense_bias_grad(const __nv_bfloat16 *__restrict__ dy, float *db, int F, long l
     __shared__ float red[8];
     const __nv_bfloat16 *const row = dy + (long long)blockIdx.x * stride;
     float sum = 0.0f;
-    for (int f = threadIdx.x * 8; f < F; f += 256 * 8) {
-        float v[8];
-        load_8<__nv_bfloat16>(row + f, v);
+    for (int f = threadIdx.x * 8; f < F; f += 4 * 256 * 8) {
+        uint4 raw[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += f + j < F ? v[j] : 0.0f;
+        for (int i = 0; i < 4; ++i) raw[i] = f + i * 2048 < F ? *reinterpret_cast<const uint4 *>(row + f + i * 2048) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v[8];
+            unpack<__nv_bfloat16>(raw[i], v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += f + i * 2048 + j < F ? v[j] : 0.0f;
+        }
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -876,9 +935,8 @@ static int dense_tiles(const Operand &A, const Operand &B, const DenseArgs &a, c
     auto map = [&](CUtensorMap *m, const Operand &o, int box_rows) {
         return tensor_map_rows(encode, m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, o.p, o.size, o.rows, o.stride * 2, box_rows) == CUDA_SUCCESS;
     };
-    BB200_REQUIRE(map(&map_a, A, S::kAAcross ? kTileK : kTileM) && map(&map_b, B, S::kBAcross ? kTileK : S::kBRows), (int)cudaErrorInvalidValue);
-    constexpr int kRows = PAIR ? 2 * kTileM : kTileM;
-    const long long tiles = ((long long)a.M + kRows - 1) / kRows * (((long long)a.N + TN - 1) / TN), sms = device_info().sm_count;
+    BB200_REQUIRE(map(&map_a, A, S::kAAcross ? kTileK : S::kOwnRows) && map(&map_b, B, S::kBAcross ? kTileK : S::kBRows), (int)cudaErrorInvalidValue);
+    const long long tiles = ((long long)a.M + S::kRows - 1) / S::kRows * (((long long)a.N + TN - 1) / TN), sms = device_info().sm_count;
     BB200_REQUIRE(tiles < (1LL << 27), BBCU_ERR_TOO_LARGE);
     auto kernel = k_dense_tiles<KIND, T, TN, PAIR>;
     BB200_REQUIRE(allow_big_smem(kernel, S::kSmem), (int)cudaErrorInvalidValue);
@@ -889,7 +947,7 @@ static int dense_tiles(const Operand &A, const Operand &B, const DenseArgs &a, c
 }
 
 // Columns a tile (0: by a pair of CTAs) and CTAs that share the k of one, by what they take in nanoseconds, measured with one tile an SM: a stage of k 325 whatever the
-// columns (a CTA's 24 to 32 KB come at about 50 bytes a clock; both products of a gated block 505), by a pair 410 (540); to start and to store 3700 and some for
+// columns (a CTA's 24 to 32 KB come at about 50 bytes a clock; both products of a gated block 505), by a pair 410; to start and to store 3700 and some for
 // each column, by a pair 7000; to join sums in a cluster 1500 and more for columns and CTAs.  A cluster has one tile, so that there are no more of them than
 // the device holds (clusters of eight: fewer than its SMs would make; 1024 x 1024 x 64 7.5 us by four CTAs, 12.9 where 16 clusters of eight took two rounds).
 // Of 36 shapes from 420 x 70 x 512 to 4096 x 4096 x 1000 the choice is within 3 % of the best one, two within 9 %.
@@ -897,10 +955,9 @@ struct DenseTiles { int columns, splits; };
 static DenseTiles choose_dense_tiles(int M, int N, int K, int parts, const int (&clusters)[4])
 {
     const long long sms = device_info().sm_count, blocks = (K + kTileK - 1) / kTileK, tiles_m = ((long long)M + kTileM - 1) / kTileM;
-    const int pair_n = parts == 2 ? 128 : 256;
-    const long long pair_tiles = ((long long)M + 2 * kTileM - 1) / (2 * kTileM) * (((long long)N + pair_n - 1) / pair_n);
+    const long long pair_rows = parts == 2 ? kTileM : 2 * kTileM, pair_tiles = (M + pair_rows - 1) / pair_rows * (((long long)N + 255) / 256);
     DenseTiles best = {0, 1};
-    long long least = (pair_tiles + sms / 2 - 1) / (sms / 2) * blocks * (parts == 2 ? 540 : 410) + 7000;
+    long long least = (pair_tiles + sms / 2 - 1) / (sms / 2) * blocks * 410 + 7000;
     for (int columns = 32; columns <= 128; columns *= 2) {
         const long long tiles = tiles_m * (((long long)N + columns - 1) / columns);
         for (int splits = 1, i = 0; splits <= kMostSplits; splits *= 2, ++i) {
@@ -929,7 +986,7 @@ template <int KIND, typename T> static int dense_product(const Operand &A, const
     case 32: return dense_tiles<KIND, T, 32, false>(A, B, a, st);
     case 64: return dense_tiles<KIND, T, 64, false>(A, B, a, st);
     case 128: return dense_tiles<KIND, T, 128, false>(A, B, a, st);
-    default: return dense_tiles<KIND, T, KIND == kGated ? 128 : 256, true>(A, B, a, st);
+    default: return dense_tiles<KIND, T, 256, true>(A, B, a, st);
     }
 }
 
