@@ -87,6 +87,18 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// 32 bytes of global memory, a whole sector, aligned to that
+__device__ __forceinline__ void load_32_bytes(const void *p, uint4 &a, uint4 &b)
+{
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(__cvta_generic_to_global(p)) : "memory");
+}
+__device__ __forceinline__ void store_32_bytes(void *p, const uint4 &a, const uint4 &b)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(__cvta_generic_to_global(p)), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+}
+
 // Vector reductions into global memory (resolved in L2): 16 / 8 bytes per lane, address aligned to the vector size.
 __device__ __forceinline__ void red_add_v4(float *addr, float a, float b, float c, float d)
 {

@@ -10,6 +10,7 @@
 // x, W, dy and the kept z are bf16; the sums are 32 bits, bias, activation, residual and gate are applied to them in 32 bits, and each output is rounded once.
 // Frame buffers are read as they lie, frames next to each other: where the product sums over nodes, its operand is "across" (rows of shared memory along
 // the frames), which the tensor cores take from TMA's 128-byte swizzled boxes as well as rows along k; the gradients read W and x the other way round, and nothing is transposed.
+#include <algorithm>
 #include <type_traits>
 
 #include <cuda.h>
@@ -31,7 +32,7 @@ struct DenseArgs {
     const float *bias;
     const void *extra;                                   // residual (forward), z (input gradient)
     void *out, *z_out;
-    int act, gated, accumulate, vec;                     // vec: the rows of extra, out and z_out start on 16-byte boundaries
+    int act, gated, accumulate, vec;                     // vec: the rows of extra, out and z_out start on 16-byte boundaries; 2: on 32-byte ones
     int M, N, K, half;                                   // half: rows of a gated block's output, the distance between its two products
     int splits;
     long long extra_stride, out_stride, z_stride;
@@ -343,7 +344,7 @@ template <int KIND, typename T, int TN, bool PAIR> struct DenseShape {
     static constexpr int kParts = KIND == kGated && !PAIR ? 2 : 1, kOwnN = PAIR ? TN / 2 : TN, kBRows = kBAcross && kOwnN < 64 ? 64 : kOwnN;
     static constexpr int kABytes = kTileM * kTileK * 2, kStageBytes = kParts * kABytes + kBRows * kTileK * 2;
     static constexpr int kWarps = 16, kThreads = 64 + 32 * kWarps;        // warp 0 copies, warp 1 issues the products, the others take the sums out of TMEM
-    static constexpr int kPiece = kPromote || KIND == kGated ? 16 : 32;   // columns that a warp takes at a time
+    static constexpr int kPiece = 16;                                     // columns that a warp takes at a time: a sector of bf16 (32: registers, gelu's gradient 91 -> 84 us)
     static constexpr int kOutBytes = 32 * kPiece * (int)sizeof(T);
     static constexpr int kCross = kStacked ? kWarps / 2 : 0, kCrossBytes = 2 * 32 * kPiece * 4;        // pairs of warps that exchange sums, two buffers each
     static constexpr int kRoom = 225 * 1024 - kWarps * kOutBytes - kCross * kCrossBytes, kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
@@ -356,9 +357,27 @@ template <int KIND, typename T, int TN, bool PAIR> struct DenseShape {
 // exist): they cross shared memory, where the order of a row's pieces differs from row to row so that no banks collide, and leave as P * 16 bytes of a row; at odd
 // addresses a column a lane.
 template <int P> __device__ __forceinline__ int staged_piece(int row, int q) { return row * P + (q ^ (P == 8 ? row & 7 : P == 4 ? row >> 1 & 3 : row >> 2 & 1)); }
-template <int P> __device__ __forceinline__ void store_rows(uint4 *stage, const uint4 (&v)[P], __nv_bfloat16 *base, long long stride, int rows, int left, bool vec)
+template <int P> __device__ __forceinline__ void store_rows(uint4 *stage, const uint4 (&v)[P], __nv_bfloat16 *base, long long stride, int rows, int left, int vec)
 {
     const int lane = threadIdx.x & 31;
+    if (vec == 2) {
+        // whole sectors of the lane's own row: nothing crosses shared memory, whose bandwidth the products live on
+        if (lane >= rows) return;
+        __nv_bfloat16 *const to = base + lane * stride;
+#pragma unroll
+        for (int q = 0; q < P; q += 2) {
+            if (8 * q + 16 <= left) {
+                store_32_bytes(to + 8 * q, v[q], v[q + 1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const uint32_t word = reinterpret_cast<const uint32_t *>(&v[q + j / 8])[j % 8 / 2];
+                    if (8 * q + j < left) to[8 * q + j] = __ushort_as_bfloat16((unsigned short)(j % 2 ? word >> 16 : word));
+                }
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int q = 0; q < P; ++q) stage[staged_piece<P>(lane, q)] = v[q];
     __syncwarp();
@@ -386,12 +405,20 @@ template <int P> __device__ __forceinline__ void store_rows(uint4 *stage, const 
     __syncwarp();
 }
 
-// The way back: 32 rows of P pieces of eight columns of an input of the epilogue are asked for as they lie, P * 16 bytes of a row by P lanes side by side, and
-// change places through the same shared memory when they are needed, so that each lane has its row.  (A lane asking for its own row brings every sector twice:
-// product of 2000 x 5500 x 3001 with a gate's gradient 105 us, 3.4 times its input's bytes out of L2.)
-template <int P> __device__ __forceinline__ void load_rows(uint4 (&e)[P], const __nv_bfloat16 *base, long long stride, int rows, int left, bool vec)
+// The way back: 32 rows of P pieces of eight columns of an input of the epilogue.  Rows on 32-byte boundaries come as whole sectors of the lane's own row.  Others are
+// asked for as they lie, P * 16 bytes of a row by P lanes side by side, and change places through the same shared memory when they are needed.  (A lane asking for
+// 16 bytes of its own row brings every sector twice.)
+template <int P> __device__ __forceinline__ void load_rows(uint4 (&e)[P], const __nv_bfloat16 *base, long long stride, int rows, int left, int vec)
 {
     const int lane = threadIdx.x & 31, q = lane % P;
+    if (vec == 2) {
+#pragma unroll
+        for (int i = 0; i < P; i += 2) {
+            e[i] = e[i + 1] = make_uint4(0, 0, 0, 0);
+            if (lane < rows && 8 * i < left) load_32_bytes(base + lane * stride + 8 * i, e[i], e[i + 1]);
+        }
+        return;
+    }
 #pragma unroll
     for (int it = 0; it < P; ++it) {
         const int r = it * (32 / P) + lane / P;
@@ -408,9 +435,10 @@ template <int P> __device__ __forceinline__ void load_rows(uint4 (&e)[P], const 
         }
     }
 }
-template <int P> __device__ __forceinline__ void spread_rows(uint4 *stage, uint4 (&e)[P])
+template <int P> __device__ __forceinline__ void spread_rows(uint4 *stage, uint4 (&e)[P], int vec)
 {
     const int lane = threadIdx.x & 31;
+    if (vec == 2) return;
 #pragma unroll
     for (int it = 0; it < P; ++it) stage[staged_piece<P>(it * (32 / P) + lane / P, lane % P)] = e[it];
     __syncwarp();
@@ -743,7 +771,7 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     store_rows(stage_out, r, base, a.out_stride, a.extra ? static_cast<const float *>(a.extra) + m * a.extra_stride + n : nullptr, a.extra_stride,
                                   a.accumulate, rows, left, a.vec);
                 } else if constexpr (KIND == kForward) {
-                    if (a.extra) spread_rows(stage_out, extra[0]);
+                    if (a.extra) spread_rows(stage_out, extra[0], a.vec);
                     if (a.extra) made([&](int j) { return __int_as_float(v[j]) + extra_of(0, j); });
                     else made([&](int j) { return __int_as_float(v[j]); });
                     fetch_extra(i + kPiece);
@@ -803,8 +831,8 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                         store_rows(stage_out, out, z_base + a.half * a.z_stride, a.z_stride, rows, left, a.vec);
                     }
                 } else if (a.gated) {
-                    spread_rows(stage_out, extra[0]);
-                    spread_rows(stage_out, extra[1]);
+                    spread_rows(stage_out, extra[0], a.vec);
+                    spread_rows(stage_out, extra[1], a.vec);
                     uint4 up[kPiece / 8];
                     with_activation(a.act, [&](auto act) {
 #pragma unroll
@@ -825,7 +853,7 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     store_rows(stage_out, out, base, a.out_stride, rows, left, a.vec);
                     store_rows(stage_out, up, base + a.half * a.out_stride, a.out_stride, rows, left, a.vec);
                 } else {
-                    if (a.extra) spread_rows(stage_out, extra[0]);
+                    if (a.extra) spread_rows(stage_out, extra[0], a.vec);
                     if (a.extra) with_activation(a.act, [&](auto act) { made([&](int j) { return __int_as_float(v[j]) * curve<decltype(act)::value, sizeof(T) == 2>(extra_of(0, j)).slope; }); });
                     else made([&](int j) { return __int_as_float(v[j]); });
                     fetch_extra(i + kPiece);
@@ -1004,6 +1032,13 @@ template <int KIND, typename T> static int dense_few(const __nv_bfloat16 *x, con
 
 constexpr int kMostExtent = 1 << 27;
 
+// 2: rows on 32-byte boundaries, 1: on 16-byte ones
+template <typename T> static int alignment(const T *p, long long stride)
+{
+    const unsigned long long both = reinterpret_cast<uintptr_t>(p) | (unsigned long long)(stride * (long long)sizeof(T));
+    return both % 32 == 0 ? 2 : both % 16 == 0 ? 1 : 0;
+}
+
 static bool rows_on_16(const void *p, long long stride) { return frames_aligned<__nv_bfloat16>(p, stride); }
 
 template <typename T>
@@ -1020,7 +1055,7 @@ static int dense_forward(bool gated, const bbcu_bf16_t *x_, const bbcu_bf16_t *W
     a.bias = bias; a.extra = residual; a.out = y; a.z_out = z; a.act = activation;
     a.M = O; a.N = F; a.K = K; a.half = O; a.splits = 1;
     a.extra_stride = rs; a.out_stride = ys; a.z_stride = zs;
-    a.vec = frames_aligned<T>(y, ys) && (!residual || frames_aligned<T>(residual, rs)) && (!z || rows_on_16(z, zs));
+    a.vec = std::min({alignment(y, ys), residual ? alignment(residual, rs) : 2, z ? alignment(reinterpret_cast<const __nv_bfloat16 *>(z), zs) : 2});
     cudaStream_t st = as_stream(stream);
     const Operand A = {W, K, gated ? 2LL * O : O, ws}, B = {x, F, K, xs};
     if constexpr (sizeof(T) == 2) {
@@ -1075,7 +1110,7 @@ extern "C" int bbcu_bf16_DenseAffine_BackwardInput(const bbcu_bf16_t *dy_, const
     a.extra = z; a.out = dx; a.act = activation; a.gated = gated != 0;
     a.M = I; a.N = F; a.K = O; a.half = I; a.splits = 1;
     a.extra_stride = z_frame_stride; a.out_stride = dx_frame_stride;
-    a.vec = rows_on_16(dx, dx_frame_stride) && (!z || rows_on_16(z, z_frame_stride));
+    a.vec = std::min(alignment(reinterpret_cast<const __nv_bfloat16 *>(dx), dx_frame_stride), z ? alignment(reinterpret_cast<const __nv_bfloat16 *>(z), z_frame_stride) : 2);
     return dense_product<kInputGrad, __nv_bfloat16>({W, I, O, w_node_stride}, {dy, F, O, dy_frame_stride}, a, as_stream(stream));
 }
 
