@@ -58,6 +58,13 @@ def _one_device(tensors):
         raise OverflowError("a size does not fit the operator")
 
 
+def _apart(tensors, name):
+    """Each element is written once: a tensor may not be given twice, nor two that share memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in tensors if t.numel())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError(f"{name}: expected tensors that share no memory")
+
+
 def fp32_stride(frames):
     """Row stride in floats: rows padded to 32 bytes (include/bb/FrameBuffer.h:414-417)."""
     return (frames + 7) // 8 * 8
@@ -381,6 +388,7 @@ class Adam:
                 if _chk(p, torch.float32, "params").shape != _chk(g, torch.float32, "grads").shape:
                     raise ValueError(f"grads: expected the shape of the parameter, {tuple(p.shape)}, got {tuple(g.shape)}")
             _one_device(self.params + self.grads)
+            _apart(self.params + self.grads, "params and grads")
         self.m = [torch.zeros_like(p) for p in self.params]
         self.v = [torch.zeros_like(p) for p in self.params]
         dev = self.params[0].device
@@ -423,6 +431,7 @@ class GradientNorm:
         if not self.grads:
             raise ValueError("grads: expected at least one tensor")
         _one_device(self.grads)
+        _apart(self.grads, "grads")
         dev = self.grads[0].device
         self._sizes = torch.tensor([g.numel() for g in self.grads], dtype=torch.int32, device=dev)
         self._table = torch.tensor([g.data_ptr() for g in self.grads], dtype=torch.int64, device=dev)

@@ -703,9 +703,129 @@ def test_refusals_of_the_tensor_calls_on_the_device():
                  lambda: ops.rms_norm_int8(x.int(), 8), lambda: ops.rms_norm_backward(x, xf, v, 8), lambda: ops.rms_norm_backward(x, x, v[:4], 8),
                  lambda: ops.rms_norm_backward(x, x, v, 8, dresidual=x[:4]), lambda: ops.rms_norm_backward(x, x, v, 8, dgamma=v[:4]),
                  lambda: ops.GradientNorm([x]), lambda: ops.GradientNorm([xf.T]), lambda: ops.Adam([xf], [xf[:4]], max_norm=1.0), lambda: ops.Adam([xf], [x], max_norm=1.0),
-                 lambda: ops.Adam([xf, xf], [xf], max_norm=1.0)):
+                 lambda: ops.Adam([xf, xf], [xf], max_norm=1.0), lambda: ops.Adam([xf], [xf], max_norm=1.0), lambda: ops.GradientNorm([v, v]),
+                 lambda: ops.GradientNorm([v[:9], v[8:]]), lambda: ops.Adam([v[:8], v[8:]], [xf[0, :8], xf[0, 7:15]], max_norm=1.0)):
         with pytest.raises(ValueError):
             call()
     for call in (lambda: ops.rms_norm_forward(x, 8, eps=-1.0), lambda: ops.GradientNorm([xf]).clip_(-1.0)):
         with pytest.raises(abi.BbcuError):
             call()
+
+
+# ------------------------------------------------------------------------------------------------------------------------ scratch, large buffers
+@pytest.mark.gpu
+def test_host_threads_on_one_stream_with_scratch():
+    """Chains of kernels with scratch between them from four host threads on one stream, forty times each: the bits of the same calls by themselves."""
+    import threading
+    from binarybrain_b200 import ops
+    runs = []
+    for k, (N, F, dtype) in enumerate([(300, 40, torch.float32), (2500, 1800, BF16), (4096, 1500, torch.float32), (9001, 100, BF16)]):
+        s, dr, gamma = rms_case(N, F, dtype, seed=200 + k)
+        dy, rstd = normal(210 + k, N, F).to(dtype), rms_64(s, 1e-5)[0].float().cuda()
+        s, dr, dy, gamma, clip = buffer(s, dtype), buffer(dr, dtype), buffer(dy, dtype), gamma.cuda(), ops.GradientNorm(tensors([N, 7 * F, 3], 220 + k))
+
+        def run(s=s, dr=dr, dy=dy, gamma=gamma, rstd=rstd, clip=clip, F=F):
+            ds, dgamma = ops.rms_norm_backward(s, dy, rstd, F, gamma=gamma, dresidual=dr)
+            y, _, r = ops.rms_norm_forward(s, F, gamma=gamma, residual=dr)
+            q, scale, _ = ops.rms_norm_int8(s, F, gamma=gamma, residual=dr)
+            return ds[:, :F], dgamma, y[:, :F], r, q, scale, clip.norm()
+        runs.append(run)
+    want = [[t.clone() for t in run()] for run in runs]
+    torch.cuda.synchronize()
+    stream, failed, start = torch.cuda.current_stream(), [], threading.Barrier(len(runs))
+
+    def work(k):
+        try:
+            with torch.cuda.stream(stream):
+                start.wait(60)
+                got = [runs[k]() for _ in range(40)]
+            stream.synchronize()
+            failed.extend((k, i) for i, g in enumerate(got) if not all(torch.equal(a, b) for a, b in zip(g, want[k])))
+        except Exception as e:  # noqa: BLE001 (a thread's exception is the test's)
+            failed.append((k, repr(e)))
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(runs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
+@pytest.mark.gpu
+def test_a_graph_keeps_its_scratch_beside_larger_calls():
+    from binarybrain_b200 import ops
+    s, dr, gamma = rms_case(2500, 1800, BF16, seed=230)
+    dy, rstd = buffer(normal(231, 2500, 1800), BF16), rms_64(s, 1e-5)[0].float().cuda()
+    s, dr, gamma, clip = buffer(s, BF16), buffer(dr, BF16), gamma.cuda(), ops.GradientNorm(tensors([5000, 3], 232))
+    run = lambda: [*ops.rms_norm_backward(s, dy, rstd, 1800, gamma=gamma, dresidual=dr), *ops.rms_norm_forward(s, 1800, gamma=gamma, residual=dr), clip.norm()]  # noqa: E731
+    want = [t.clone() for t in run()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    big = [buffer(normal(240 + i, 9001, 900), BF16) for i in range(3)]
+    for _ in range(5):
+        graph.replay()
+        ops.rms_norm_backward(big[0], big[1], rstd[:900].contiguous(), 900, dresidual=big[2])
+        ops.rms_norm_int8(big[0], 900, residual=big[1])
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        n = min(1800, a.shape[-1]) if a.dim() == 2 else None
+        assert torch.equal(a[:, :n], b[:, :n]) if n else torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_buffers_of_more_than_2_31_elements():
+    """The last rows and columns, whose offsets do not fit 32 bits, against the same in 64 bits.  (Some 20 GB at a time.)"""
+    from binarybrain_b200 import ops
+    F = 60000
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def frames(rows):
+        t = torch.empty((rows, F), dtype=BF16, device="cuda")
+        for at in range(0, rows, 4096):
+            t[at:at + 4096] = torch.randn((min(4096, rows - at), F), device="cuda", generator=g)
+        return t
+    R, C = slice(-70, None), slice(-300, None)                            # the corner that is looked at
+    bound = 2.0 ** -7                                                     # two roundings to bf16 and the sums of 64 products, of values of order 1 (relative and absolute)
+
+    def near(got, want):
+        assert float(((got.double() - want).abs() - bound * (1 + want.abs())).max()) <= 0
+    K, O = 64, 40000
+    x, W, r = frames(K), weights(torch.randn(O, K, generator=torch.Generator().manual_seed(4)) / 8), frames(O)
+    y, z = ops.dense_forward(x, W, F, activation="gelu", residual=r, keep=True)
+    zw = W[R].double() @ x[:, C].double()
+    near(z[R, C], zw)
+    near(y[R, C], act64(zw, "gelu")[0] + r[R, C].double())
+    dx = ops.dense_backward_input(r, W, F)
+    near(dx[:, C] / 64, (W.double().t() @ r[:, C].double()) / 64)
+    dW, db = ops.dense_backward_weights(x, r, F)
+    close(dW[R], r[R].double() @ x.double().t(), 200 * U * (r[R].double().abs() @ x.double().abs().t()).cpu())
+    close(db[R], r[R].double().sum(1), 300 * U * r[R].double().abs().sum(1).cpu())
+    del y, z, dx
+    kept, rstd = ops.rms_norm_forward(r, F, residual=r)[1:]
+    s = 2 * r[:, C].double()
+    rw = 1 / torch.sqrt((s * s).mean(0) + 1e-5)
+    close(rstd[C], rw, (O / 512 + 24) * U * rw.cpu())
+    assert torch.equal(kept[R, C], 2 * r[R, C])
+    ds, _ = ops.rms_norm_backward(kept, r, rstd, F)
+    xh, dy = kept[:, C].double() * rstd[C].double(), r[:, C].double()
+    near(ds[R, C], (rstd[C].double() * (dy - xh * (dy * xh).mean(0)))[R])
+    del ds
+    q, scale, _ = ops.rms_norm_int8(kept, F)
+    unit = (kept[:, C].float().abs().amax(0) / torch.full((300,), 127.0, device="cuda"))
+    assert torch.equal(q[C, R], torch.round(kept[R, C].float() / unit).clamp(-127, 127).to(torch.int8).t())
+    del q, kept, r
+    H = 20000
+    W = weights(torch.randn(2 * H, K, generator=torch.Generator().manual_seed(5)) / 8)
+    h, z = ops.gated_dense_forward(x, W, F, keep=True)
+    g64, u64 = W[H - 70:H].double() @ x[:, C].double(), W[R].double() @ x[:, C].double()
+    near(z[H - 70:H, C], g64)
+    near(z[R, C], u64)
+    near(h[R, C] / 4, act64(g64, "silu")[0] * u64 / 4)
+    dy, Wd = frames(K), weights(torch.randn(K, H, generator=torch.Generator().manual_seed(6)) / 8)
+    dz = ops.dense_backward_input(dy, Wd, F, z=z, activation="silu", gated=True)
+    d = Wd[:, R].double().t() @ dy[:, C].double()
+    zg, zu = z[H - 70:H, C].double(), z[R, C].double()
+    value, slope, _, _ = act64(zg, "silu")
+    near(dz[H - 70:H, C] / 8, d * slope * zu / 8)
+    near(dz[R, C] / 8, d * value / 8)
