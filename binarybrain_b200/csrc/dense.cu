@@ -911,34 +911,42 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     if (threadIdx.x == 0 && gave_up) atomicCAS(a.fault, 0, kFaultBarrierTimeout);
 }
 
-// db = or += the sums of the rows of dy: a CTA a row, 16 bytes a thread and round
-__global__ void __launch_bounds__(256)
-k_dense_bias_grad(const __nv_bfloat16 *__restrict__ dy, float *db, int F, long long stride, int accumulate)
+// db = or += the sums of the rows of dy: a warp or a CTA of 8 a row, 16 bytes a lane, four of them under way
+template <int W> __global__ void __launch_bounds__(256)
+k_dense_bias_grad(const __nv_bfloat16 *__restrict__ dy, float *db, int O, int F, long long stride, int accumulate)
 {
     grid_dependency();
-    __shared__ float red[8];
-    const __nv_bfloat16 *const row = dy + (long long)blockIdx.x * stride;
-    float sum = 0.0f;
-    for (int f = threadIdx.x * 8; f < F; f += 4 * 256 * 8) {
-        uint4 raw[4];
+    static_assert(W == 1 || W == 8, "a row is a warp's or a CTA's");
+    const int lane = threadIdx.x & 31, warp = (int)threadIdx.x >> 5, part = warp % W, o = ((int)blockIdx.x * 8 + warp) / W;
+    const __nv_bfloat16 *const row = dy + (long long)o * stride;
+    float sum[8] = {};
+    const unsigned whole = (unsigned)F & ~7u;
+    constexpr unsigned step = W * 256;
+    if (o < O)
+        for (unsigned at = part * 256 + lane * 8; at < whole; at += 4 * step) {
+            uint4 raw[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) raw[i] = f + i * 2048 < F ? *reinterpret_cast<const uint4 *>(row + f + i * 2048) : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 4; ++i) raw[i] = at + i * step < whole ? *reinterpret_cast<const uint4 *>(row + at + i * step) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v[8];
-            unpack<__nv_bfloat16>(raw[i], v);
+            for (int i = 0; i < 4; ++i) {
+                float v[8];
+                unpack<__nv_bfloat16>(raw[i], v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum += f + i * 2048 + j < F ? v[j] : 0.0f;
+                for (int j = 0; j < 8; ++j) sum[j] += v[j];
+            }
         }
-    }
+    if (o < O && part == 0 && lane < F - (int)whole) sum[0] += to_float(row[whole + lane]);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 8; ++w) sum += red[w];
-        db[blockIdx.x] = accumulate ? db[blockIdx.x] + sum : sum;
+    for (int j = 1; j < 8; ++j) sum[0] += sum[j];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], d);
+    if constexpr (W > 1) {
+        __shared__ float s_sum[W];
+        if (lane == 0) s_sum[warp] = sum[0];
+        __syncthreads();
+        for (int i = 1; i < W; ++i) sum[0] += s_sum[i];
     }
+    if (o < O && part == 0 && lane == 0) db[o] = accumulate ? db[o] + sum[0] : sum[0];
 }
 
 // dW = db = 0 of a batch without frames
@@ -1131,7 +1139,13 @@ extern "C" int bbcu_bf16_DenseAffine_BackwardWeights(const bbcu_bf16_t *x_, cons
         return launch_status();
     }
     BB200_REQUIRE_PTR(dy);
-    if (dbias) launch(k_dense_bias_grad, (unsigned)O, 256, 0, st, dy, dbias, F, (long long)dy_frame_stride, accumulate);
+    if (dbias) {
+        // A warp a row where that gives every SM two CTAs, or where a row has no more than a warp's four loads; else a CTA a row.  By the warp and
+        // by the CTA: 4096 rows x 1000 frames 2 and 7 us, 4096 x 8192 9 and 10, 1024 x 8192 4 and 3, 64 x 65536 24 and 4.
+        if (O >= 16 * device_info().sm_count || F <= 1024)
+            launch(k_dense_bias_grad<1>, (unsigned)((O + 7) / 8), 256, 0, st, dy, dbias, O, F, (long long)dy_frame_stride, accumulate);
+        else launch(k_dense_bias_grad<8>, (unsigned)O, 256, 0, st, dy, dbias, O, F, (long long)dy_frame_stride, accumulate);
+    }
     if (!dW) return launch_status();
     BB200_REQUIRE_PTR(x);
     DenseArgs a{};
