@@ -474,20 +474,37 @@ k_rms_apply(const RmsForward<T> a, const float *__restrict__ part, int rows, int
     }
 }
 
-// unit[frame] for k_rms_quantize, scale and rstd, from the parts of the bands
+// The parts of the bands joined over a frame: eight threads take some of them each, and one adds up what they have in a fixed order.
+template <int Q, typename JOIN> __device__ __forceinline__ bool join_bands(const float *__restrict__ part, int bands, int padded, int F, int &f, float (&v)[Q], JOIN join)
+{
+    __shared__ float s[8][Q][32];
+    const int lane = threadIdx.x & 31, some = threadIdx.x >> 5;
+    f = (int)blockIdx.x * 32 + lane;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        v[q] = 0.0f;
+#pragma unroll 4
+        for (int b = some; b < bands; b += 8)
+            if (f < F) v[q] = join(q, v[q], part[((long long)q * bands + b) * padded + f]);
+        s[some][q][lane] = v[q];
+    }
+    __syncthreads();
+    if (some || f >= F) return false;
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        for (int i = 1; i < 8; ++i) v[q] = join(q, v[q], s[i][q][lane]);
+    return true;
+}
+
+// unit[frame] for k_rms_quantize, scale and rstd
 __global__ void __launch_bounds__(256)
 k_rms_scales(const float *__restrict__ part, int bands, int padded, float *unit_out, float *scale_out, float *rstd_out, float eps, int N, int F)
 {
     grid_dependency();
-    const int f = (int)blockIdx.x * 256 + threadIdx.x;
-    if (f >= F) return;
-    float sum = 0.0f, top = 0.0f;
-#pragma unroll 8
-    for (int b = 0; b < bands; ++b) {
-        sum += part[(long long)b * padded + f];
-        top = max_or_nan(top, part[(long long)(bands + b) * padded + f]);
-    }
-    const float rstd = 1.0f / sqrtf(fmaf(sum, 1.0f / (float)N, eps)), unit = quant_scale(__float_as_uint(top) & 0x7fffffffu);
+    int f;
+    float v[2];
+    if (!join_bands<2>(part, bands, padded, F, f, v, [](int q, float a, float b) { return q == 0 ? a + b : max_or_nan(a, b); })) return;
+    const float rstd = 1.0f / sqrtf(fmaf(v[0], 1.0f / (float)N, eps)), unit = quant_scale(__float_as_uint(v[1]) & 0x7fffffffu);
     unit_out[f] = unit;
     scale_out[f] = unit * rstd;
     if (rstd_out) rstd_out[f] = rstd;
@@ -572,16 +589,13 @@ k_rms_grad_sums(const RmsBackward<T> a, float *part, int rows, int padded)
     store_band<T, ALIGNED, 1>(v, part, (int)gridDim.y, (int)blockIdx.y, padded, line, [](int, float p, float o) { return p + o; });
 }
 
-// mean[frame] = the mean over all rows, from the parts of the bands
+// mean[frame] = the mean over all rows
 __global__ void __launch_bounds__(256) k_rms_grad_means(const float *__restrict__ part, int bands, int padded, float *mean, int N, int F)
 {
     grid_dependency();
-    const int f = (int)blockIdx.x * 256 + threadIdx.x;
-    if (f >= F) return;
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int b = 0; b < bands; ++b) sum += part[(long long)b * padded + f];
-    mean[f] = sum / (float)N;
+    int f;
+    float v[1];
+    if (join_bands<1>(part, bands, padded, F, f, v, [](int, float a, float b) { return a + b; })) mean[f] = v[0] / (float)N;
 }
 
 // A CTA has 8 x kGradRows rows and every gridDim.x-th piece of 512 bytes of them, and adds up their sums over the frames on the way: gamma_part[blockIdx.x][node].
@@ -691,7 +705,7 @@ template <typename T, bool INT8> static int rms_forward(RmsForward<T> &a, bool a
             float *const unit = part + 2LL * b.bands * b.padded;
             constexpr int kCols = Column<T, 8>::kCols;
             const int bands = (a.N + kRmsQuantRows - 1) / kRmsQuantRows;
-            launch(k_rms_scales, (unsigned)((a.F + 255) / 256), 256, 0, st, part, b.bands, b.padded, unit, a.scale, a.rstd, a.eps, a.N, a.F);
+            launch(k_rms_scales, (unsigned)((a.F + 31) / 32), 256, 0, st, part, b.bands, b.padded, unit, a.scale, a.rstd, a.eps, a.N, a.F);
             launch(aligned ? k_rms_quantize<T, true> : k_rms_quantize<T, false>, dim3((unsigned)((a.F + kCols - 1) / kCols), (unsigned)bands), 256, 0, st, a.r ? a.s : a.x, a.q, a.gamma,
                    unit, a.N, a.F, a.r ? a.ss : a.xs, a.qs);
         } else {
@@ -759,7 +773,7 @@ static int rms_backward_checked(const T *s, const T *dy, const T *dr, T *ds, con
         if (dgamma) a.gamma_part = part + sums;
         launch(aligned ? k_rms_grad_sums<T, true> : k_rms_grad_sums<T, false>, dim3((unsigned)b.pieces, (unsigned)b.bands), 32 * kBandWarps, 0, st, a, part, b.rows, b.padded);
         BB200_CUDA(cudaPeekAtLastError());
-        launch(k_rms_grad_means, (unsigned)((F + 255) / 256), 256, 0, st, part, b.bands, b.padded, mean, N, F);
+        launch(k_rms_grad_means, (unsigned)((F + 31) / 32), 256, 0, st, part, b.bands, b.padded, mean, N, F);
         auto apply = aligned ? (dr ? k_rms_grad_apply<T, true, true> : k_rms_grad_apply<T, true, false>) : (dr ? k_rms_grad_apply<T, false, true> : k_rms_grad_apply<T, false, false>);
         launch(apply, dim3((unsigned)sweeps, (unsigned)groups), 32 * kBandWarps, 0, st, a, mean, b.rows, b.bands);
         if (dgamma) launch(k_rms_gamma, (unsigned)((N + 31) / 32), 256, 0, st, a.gamma_part, dgamma, N, sweeps, accumulate);
