@@ -10,7 +10,8 @@
 // the backward pass, which is given that, sees the numbers that the statistics are of.
 //
 // Memory bounds it (16 bytes a value of fp32 forward with a residual, 16 backward).  A frame is needed whole before its first output.  Small calls take one launch: a
-// cluster of CTAs has the columns of 32 or 128 bytes of a row and goes over the rows twice, or once where they stay in registers.  Large ones go along the rows
+// cluster of CTAs has the columns of 32 or 128 bytes of a row and goes over the rows twice, or once where they stay in registers; 16 bytes of a row or less are taken
+// frame by frame by lanes that hold their rows.  Large calls go along the rows
 // in two passes, which move a quarter more (a residual's sum is written by the first and read by the second), at 5.9 to 6.9 TB/s.
 #include <algorithm>
 
@@ -345,6 +346,198 @@ __global__ void __launch_bounds__(256) k_rms_no_frames(float *dgamma, int N)
     grid_dependency();
     const int n = (int)blockIdx.x * 256 + threadIdx.x;
     if (n < N) dgamma[n] = 0.0f;
+}
+
+// ---- few frames: a lane has four neighbouring rows of one frame (a word of q), in up to kRounds rounds of a cluster's threads, and keeps them.  Nothing but the
+// latencies of one load, one exchange and one store counts, so a lane has numbers of its own only, and what a vector of 16 bytes would bring along is not touched.
+// The gradient of gamma needs no second launch, as a row's frames are neighbouring lanes.
+constexpr int kFewFrames = 8, kFewRounds = 4;
+
+template <int Q> struct FewExchange {
+    float warps[32][Q * kFewFrames], ctas[8][Q * kFewFrames];
+    uint64_t bar;
+    int gave_up;
+};
+
+template <int Q> __device__ __forceinline__ void few_meet(FewExchange<Q> &e, const Cluster &cl)
+{
+    if (cl.size == 1) return;
+    if (threadIdx.x == 0) {
+        e.gave_up = 0;
+        mbar_init(&e.bar, 1);
+        mbar_init_fence();
+    }
+    cluster_arrive();
+}
+
+// v of all rows of a lane's frame: of the warp's lanes, the CTA's warps and the cluster's CTAs, in a fixed order.  lanes: a power of two that the frames fit in.
+template <int Q, typename JOIN> __device__ __forceinline__ void few_join(float (&v)[Q], int lanes, FewExchange<Q> &e, const Cluster &cl, JOIN join)
+{
+    const int lane = threadIdx.x & 31, warp = (int)threadIdx.x >> 5, warps = (int)blockDim.x >> 5, f = lane & (lanes - 1);
+    for (int m = lanes; m < 32; m <<= 1)
+#pragma unroll
+        for (int q = 0; q < Q; ++q) v[q] = join(q, v[q], __shfl_xor_sync(0xffffffffu, v[q], m));
+    if (lane < lanes) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) e.warps[warp][q * kFewFrames + f] = v[q];
+    }
+    if (cl.size > 1) {
+        cluster_wait();                                                   // all CTAs have their barriers
+        if (threadIdx.x == 0) mbar_arrive_expect_tx(&e.bar, cl.size * Q * lanes * (uint32_t)sizeof(float));
+    }
+    __syncthreads();
+    for (int i = warp; i < Q * lanes; i += warps) {
+        const int q = i >= lanes, at = q * kFewFrames + (i & (lanes - 1));
+        float s = lane < warps ? e.warps[lane][at] : 0.0f;                // 0: for a sum and for a maximum of magnitudes
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) s = join(q, s, __shfl_xor_sync(0xffffffffu, s, m));
+        if (cl.size == 1) {
+            if (lane == 0) e.ctas[0][at] = s;
+        } else if (lane < (int)cl.size) {
+            peer_send(peer_addr(&e.ctas[cl.rank][at], (uint32_t)lane), s, peer_addr(&e.bar, (uint32_t)lane));
+        }
+    }
+    if (cl.size == 1) {
+        __syncthreads();
+    } else {
+        int spins = 0;
+        while (!mbar_try_wait(&e.bar, 0))
+            if (++spins == kWaitSpins) { *(volatile int *)&e.gave_up = 1; break; }
+        __syncwarp();
+        cluster_arrive();
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        v[q] = e.ctas[0][q * kFewFrames + f];
+        for (uint32_t r = 1; r < cl.size; ++r) v[q] = join(q, v[q], e.ctas[r][q * kFewFrames + f]);
+    }
+}
+
+template <int Q> __device__ __forceinline__ void few_leave(FewExchange<Q> &e, const Cluster &cl, int *fault)
+{
+    if (cl.size == 1) return;
+    if (*(volatile int *)&e.gave_up) atomicCAS(fault, 0, kFaultBarrierTimeout);
+    cluster_wait();
+}
+
+template <typename T, bool INT8, int ROUNDS>
+__global__ void __launch_bounds__(1024)
+k_rms_few(const RmsForward<T> a, int lanes)
+{
+    constexpr int kQ = INT8 ? 2 : 1;
+    __shared__ FewExchange<kQ> e;
+    const Cluster cl(&e.gave_up);
+    few_meet(e, cl);
+    grid_dependency();
+    const int f = (int)threadIdx.x & (lanes - 1), shift = __ffs(lanes) - 1;
+    auto row = [&](int k) { return ((k * (int)cl.size + (int)cl.rank) * (int)blockDim.x + (int)threadIdx.x >> shift) * 4; };
+    auto has = [&](int n) { return n < a.N && f < a.F; };
+    float s[ROUNDS][4], g[ROUNDS][4], v[kQ] = {};
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = row(k) + i;
+            s[k][i] = has(n) ? to_float(a.x[(long long)n * a.xs + f]) : 0.0f;
+            g[k][i] = a.gamma && n < a.N ? a.gamma[n] : 1.0f;
+        }
+    if (a.r) {
+        float r[ROUNDS][4];
+#pragma unroll
+        for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[k][i] = has(row(k) + i) ? to_float(a.r[(long long)(row(k) + i) * a.rs + f]) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const T sum = from_float<T>(s[k][i] + r[k][i]);
+                s[k][i] = to_float(sum);
+                if (has(row(k) + i)) a.s[(long long)(row(k) + i) * a.ss + f] = sum;
+            }
+    }
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[0] = fmaf(s[k][i], s[k][i], v[0]);
+            if constexpr (INT8) {
+                s[k][i] *= g[k][i];
+                v[1] = max_or_nan(v[1], fabsf(s[k][i]));
+            }
+        }
+    few_join(v, lanes, e, cl, [](int q, float p, float o) { return q == 0 ? p + o : max_or_nan(p, o); });
+    const float rstd = 1.0f / sqrtf(fmaf(v[0], 1.0f / (float)a.N, a.eps));
+    if constexpr (INT8) {
+        const float unit = quant_scale(__float_as_uint(v[1]) & 0x7fffffffu);
+        if (cl.rank == 0 && (int)threadIdx.x < a.F) {
+            a.scale[f] = unit * rstd;
+            if (a.rstd) a.rstd[f] = rstd;
+        }
+        const Quantizer quantizer(unit);
+        const int end = (a.N + 15) / 16 * 16;                             // zeros as far as the row's last 16 bytes
+#pragma unroll
+        for (int k = 0; k < ROUNDS; ++k)
+            if (row(k) < end && f < a.F) *reinterpret_cast<uint32_t *>(a.q + (long long)f * a.qs + row(k)) = quantizer(s[k][0], s[k][1], s[k][2], s[k][3]);
+    } else {
+        if (cl.rank == 0 && (int)threadIdx.x < a.F) a.rstd[f] = rstd;
+#pragma unroll
+        for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (has(row(k) + i)) a.y[(long long)(row(k) + i) * a.ys + f] = from_float<T>((s[k][i] * rstd) * g[k][i]);
+    }
+    few_leave(e, cl, a.fault);
+}
+
+template <typename T, int ROUNDS>
+__global__ void __launch_bounds__(1024)
+k_rms_grad_few(const RmsBackward<T> a, float *dgamma, int accumulate, int lanes)
+{
+    __shared__ FewExchange<1> e;
+    const Cluster cl(&e.gave_up);
+    few_meet(e, cl);
+    grid_dependency();
+    const int f = (int)threadIdx.x & (lanes - 1), shift = __ffs(lanes) - 1;
+    auto row = [&](int k) { return ((k * (int)cl.size + (int)cl.rank) * (int)blockDim.x + (int)threadIdx.x >> shift) * 4; };
+    auto has = [&](int n) { return n < a.N && f < a.F; };
+    const float rstd = f < a.F ? a.rstd[f] : 0.0f;
+    float xh[ROUNDS][4], d[ROUNDS][4], v[1] = {};
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = row(k) + i;
+            xh[k][i] = has(n) ? to_float(a.s[(long long)n * a.ss + f]) : 0.0f;
+            d[k][i] = has(n) ? to_float(a.dy[(long long)n * a.dys + f]) : 0.0f;
+        }
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = row(k) + i;
+            const float g = a.gamma && n < a.N ? a.gamma[n] : 1.0f;
+            xh[k][i] *= rstd;
+            float along = d[k][i] * xh[k][i];
+            v[0] = fmaf(g * d[k][i], xh[k][i], v[0]);
+            d[k][i] *= g;
+            if (dgamma) {
+                for (int m = 1; m < lanes; m <<= 1) along += __shfl_xor_sync(0xffffffffu, along, m);
+                if (f == 0 && n < a.N) dgamma[n] = accumulate ? dgamma[n] + along : along;
+            }
+        }
+    few_join(v, lanes, e, cl, [](int, float p, float o) { return p + o; });
+    const float c = v[0] / (float)a.N;
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+        float r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = a.dr && has(row(k) + i) ? to_float(a.dr[(long long)(row(k) + i) * a.drs + f]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (has(row(k) + i)) a.ds[(long long)(row(k) + i) * a.dss + f] = from_float<T>(fmaf(rstd, fmaf(-xh[k][i], c, d[k][i]), r[i]));
+    }
+    few_leave(e, cl, a.fault);
 }
 
 // ---- large layers in two passes along the rows: a CTA has 512 bytes of the rows of a band, a warp every eighth of them, and the bands are as many as the device
@@ -684,11 +877,34 @@ template <typename T> static RmsPlan plan_rms(int N, int F)
     return {lanes, cl, (N + round_rows * cl - 1) / (round_rows * cl), (unsigned)(tiles(lanes) * cl)};
 }
 
+// Lanes of a row, CTAs of the cluster (with 256 threads or more each), their threads and rounds; 0 rounds where this is not for the size.  (Device times in a graph, with
+// a residual, by vectors and by lanes, us: 8 bits of 4096 x 1 bf16 7.9 and 5.2, backward 7.7 and 6.8, 16384 x 1 19.4 and 10.1, 30000 x 3 fp32 27.3 and 18.2, 65536 x 1
+// 60.5 and 29.1; 4096 x 8 bf16 8.0 and 5.2, 7.5 and 7.0; beyond 16 bytes of a row vectors win, backward of 4096 x 12 fp32 6.6 and 9.7, 4096 x 16 bf16 7.1 and 9.6.)
+struct FewPlan { int lanes, cluster, threads, rounds; };
+template <typename T> static FewPlan plan_few(int N, int F)
+{
+    static_assert(kFramesPerVec<T> <= kFewFrames, "a frame a lane");
+    if (F > kFramesPerVec<T>) return {};
+    int lanes = 1, cl = 1, rounds = 1;
+    while (lanes < F) lanes *= 2;
+    const long long units = ((long long)N + 15) / 16 * 4 * lanes;         // of four rows
+    while (cl < 8 && cl * 256 < units) cl *= 2;
+    while (rounds <= kFewRounds && cl * 1024ll * rounds < units) rounds *= 2;
+    if (rounds > kFewRounds) return {};
+    return {lanes, cl, (int)((units + 32ll * cl * rounds - 1) / (32ll * cl * rounds)) * 32, rounds};
+}
+
 template <typename T, bool INT8> static int rms_forward(RmsForward<T> &a, bool aligned, cudaStream_t st)
 {
     // The cluster's second reading finds L2 as the first one left it where everything fits there, and costs a latency a round where columns are few and long.  (us, one
     // launch and two passes: 1024 x 16384 bf16 with a residual 21.1 / 26.4, fp32 55.9 / 49.7; 4096 x 1024 fp32 12.3 / 13.6; 5000 x 1000 bf16 20.4 / 16.4; 16384 x 100 fp32
     // 13.5 / 27.2.)
+    a.fault = fault_word();
+    BB200_REQUIRE(a.fault != nullptr, BBCU_ERR_NO_DEVICE);
+    if (const FewPlan few = plan_few<T>(a.N, a.F); few.rounds) {
+        auto kernel = few.rounds == 1 ? k_rms_few<T, INT8, 1> : few.rounds == 2 ? k_rms_few<T, INT8, 2> : k_rms_few<T, INT8, kFewRounds>;
+        return launch_cluster(kernel, (unsigned)few.cluster, (unsigned)few.cluster, (unsigned)few.threads, 0, st, a, few.lanes);
+    }
     const RmsPlan p = plan_rms<T>(a.N, a.F);
     const bool held = p.rounds <= kHeldRows / 4;
     const long long values = (long long)a.N * a.F, bytes = values * (long long)sizeof(T) * (a.r ? 3 : 1);
@@ -714,8 +930,6 @@ template <typename T, bool INT8> static int rms_forward(RmsForward<T> &a, bool a
         return launch_status();
     }
     a.rounds = p.rounds;
-    a.fault = fault_word();
-    BB200_REQUIRE(a.fault != nullptr, BBCU_ERR_NO_DEVICE);
 #define BB200_RMS(L) (aligned ? (held ? k_rms_forward<T, L, true, INT8, true> : k_rms_forward<T, L, true, INT8, false>)  \
                               : (held ? k_rms_forward<T, L, false, INT8, true> : k_rms_forward<T, L, false, INT8, false>))
     auto kernel = p.lanes == 2 ? BB200_RMS(2) : BB200_RMS(8);
@@ -759,6 +973,10 @@ static int rms_backward_checked(const T *s, const T *dy, const T *dr, T *ds, con
     RmsBackward<T> a{s, dy, dr, ds, gamma, rstd, nullptr, N, F, 0, ss, dys, drs, dss, fault_word()};
     BB200_REQUIRE(a.fault != nullptr, BBCU_ERR_NO_DEVICE);
     const bool aligned = frames_aligned<T>(s, ss) && frames_aligned<T>(dy, dys) && frames_aligned<T>(ds, dss) && (!dr || frames_aligned<T>(dr, drs));
+    if (const FewPlan few = plan_few<T>(N, F); few.rounds) {
+        auto kernel = few.rounds == 1 ? k_rms_grad_few<T, 1> : few.rounds == 2 ? k_rms_grad_few<T, 2> : k_rms_grad_few<T, kFewRounds>;
+        return launch_cluster(kernel, (unsigned)few.cluster, (unsigned)few.cluster, (unsigned)few.threads, 0, st, a, dgamma, accumulate, few.lanes);
+    }
     HeldScratch held_scratch;
     if ((long long)N * F > kRmsGradSmall) {
         const BandPlan b = plan_bands<T>(N, F);

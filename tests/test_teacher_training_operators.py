@@ -352,6 +352,33 @@ def test_rms_frames_that_are_not_numbers_and_frames_beyond_the_range():
     assert torch.isnan(scale[[3, 9]]).all() and not q[[3, 9]].any() and torch.isfinite(scale[others]).all() and scale[12] == 0
 
 
+# frames that are fewer than 16 bytes of a row, or as many: at the numbers of rows where a lane's rounds and the cluster end
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("layout", ["rows", "odd"])
+@pytest.mark.parametrize("N,F", [(4, 8), (17, 3), (1025, 2), (4095, 6), (4096, 4), (8193, 1), (16384, 8), (16385, 7), (20000, 5), (32768, 4), (32769, 3), (70003, 2), (131072, 1), (131089, 1)])
+def test_rms_norm_of_few_frames(N, F, layout, dtype):
+    test_rms_norm_forward(N, F, layout, dtype)
+    test_rms_norm_int8(N, F, layout, dtype)
+    test_rms_norm_backward(N, F, layout, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("N", [5, 300, 5000])
+def test_rms_few_frames_that_are_not_numbers(N, dtype):
+    from binarybrain_b200 import ops
+    x = normal(61, N, 4).to(dtype)
+    x[N - 1, 0], x[N // 2, 2] = float("nan"), float("inf")
+    xd = buffer(x, dtype)
+    y, _, rstd = ops.rms_norm_forward(xd, 4)
+    q, scale, _ = ops.rms_norm_int8(xd, 4)
+    y, alone = seen(y, 4), seen(ops.rms_norm_forward(buffer(x[:, 1:2], dtype), 1)[0], 1)
+    assert torch.isnan(y[:, 0]).all() and torch.isnan(y[N // 2, 2]) and (y[[n for n in range(N) if n != N // 2], 2] == 0).all() and rstd[2] == 0
+    assert torch.isfinite(y[:, [1, 3]]).all() and torch.isnan(scale[[0, 2]]).all() and not q[[0, 2]].any() and torch.isfinite(scale[[1, 3]]).all()
+    close(y[:, 1], alone[:, 0].double(), 64 * U * alone[:, 0].double().abs() + (2 * BF * alone[:, 0].double().abs() if dtype == BF16 else 0))
+
+
 @pytest.mark.gpu
 def test_rms_calls_without_frames():
     from binarybrain_b200 import ops
