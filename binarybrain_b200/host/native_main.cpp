@@ -394,6 +394,14 @@ struct Frames {
     PyObject *result() const { return given ? Py_NewRef(given) : THPVariable_Wrap(made); }
 };
 
+// an output that does not begin where one of the others does, whose elements are read or written in another order
+bool apart(const char *name, const Frames &out, std::initializer_list<const Frames *> others)
+{
+    for (const Frames *f : others)
+        if (out.t && f->t && f->t->numel() > 0 && f->t->const_data_ptr() == out.t->const_data_ptr()) return refuse(name, "expected memory of its own");
+    return true;
+}
+
 // fp32 numbers of nodes or frames: given, or for None absent (input) or new (output)
 struct Numbers {
     Place &place;
@@ -587,6 +595,7 @@ PyObject *rms_norm_forward_body(PyObject *const *o)
         (o[4] != Py_None && (!residual.take(o[4], "residual", frames, x.t, nodes) || !s.output(o[6], "s", frames, x.t->scalar_type(), *x.t, nodes))) ||
         !y.output(o[5], "y", frames, x.t->scalar_type(), *x.t, nodes) || !rstd.output(o[7], "rstd", frames, *x.t)) return nullptr;
     if (o[4] == Py_None && o[6] != Py_None) { refuse("s", "given without a residual"); return nullptr; }
+    if (!apart("y", y, {&s})) return nullptr;
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_RmsNormalization_Forward, bbcu_bf16_RmsNormalization_Forward, float, bbcu_bf16_t, x.in<const T *>(),
                            residual.t ? residual.in<const T *>() : nullptr, s.t ? s.out<T *>() : nullptr, y.out<T *>(), gamma.data, rstd.data, eps, nodes, frames, x.stride,
                            residual.stride, s.stride, y.stride, stream)) return nullptr;
@@ -677,7 +686,8 @@ PyObject *dense_forward_body(PyObject *const *o)
     const at::Tensor *W = parse(o[2], frames) && parse(o[4], act) && parse_flag(o[7], bf16) ? bf16_weights(o[1], place, w_stride) : nullptr;
     if (!W || !fits(W->size(0), nodes) || !fits(W->size(1), inputs) || !bf16_operand(x, o[0], "x", frames, inputs) || !bias.input(o[3], "bias", nodes) ||
         (o[6] != Py_None ? !y.take(o[6], "y", frames, nullptr, nodes) : !y.output(Py_None, "y", frames, bf16 ? at::kBFloat16 : at::kFloat, *x.t, nodes)) ||
-        (o[5] != Py_None && !residual.take(o[5], "residual", frames, y.t, nodes)) || !kept(z, o[8], frames, *x.t, nodes)) return nullptr;
+        (o[5] != Py_None && !residual.take(o[5], "residual", frames, y.t, nodes)) || !kept(z, o[8], frames, *x.t, nodes) || !apart("y", y, {&x}) ||
+        !apart("z", z, {&x, &y, &residual})) return nullptr;
     const auto *in = static_cast<const bbcu_bf16_t *>(x.t->const_data_ptr()), *w = static_cast<const bbcu_bf16_t *>(W->const_data_ptr());
     auto *zp = z.t ? z.out<bbcu_bf16_t *>() : nullptr;
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(y.fp32(), bbcu_bf16_fp32_DenseAffine_Forward, bbcu_bf16_DenseAffine_Forward, float, bbcu_bf16_t, in, w, bias.data,
@@ -712,7 +722,7 @@ PyObject *gated_dense_forward_body(PyObject *const *o)
     if (!W || !fits(W->size(0), rows) || !fits(W->size(1), inputs)) return nullptr;
     if (rows % 2) { refuse("W", "expected an even number of rows, the gate's and those that it multiplies"); return nullptr; }
     if (!bf16_operand(x, o[0], "x", frames, inputs) || !bias.input(o[3], "bias", rows) || !y.output(o[5], "y", frames, at::kBFloat16, *x.t, rows / 2) ||
-        !kept(z, o[6], frames, *x.t, rows)) return nullptr;
+        !kept(z, o[6], frames, *x.t, rows) || !apart("y", y, {&x}) || !apart("z", z, {&x, &y})) return nullptr;
     if (!place.stream(stream) || BB200_CALL(bbcu_bf16_GatedDense_Forward, x.in<const bbcu_bf16_t *>(), static_cast<const bbcu_bf16_t *>(W->const_data_ptr()), bias.data,
                            y.out<bbcu_bf16_t *>(), z.t ? z.out<bbcu_bf16_t *>() : nullptr, act, inputs, rows / 2, frames, w_stride, x.stride, y.stride, z.stride,
                            stream)) return nullptr;
@@ -731,7 +741,7 @@ PyObject *dense_backward_input_body(PyObject *const *o)
     if (!W || !fits(W->size(0), nodes) || !fits(W->size(1), inputs) || !bf16_operand(dy, o[0], "dy", frames, nodes)) return nullptr;
     if (gated && o[3] == Py_None) { refuse("z", "a gated block's gradient needs what its forward pass kept"); return nullptr; }
     const int64_t rows = gated ? 2 * (int64_t)inputs : inputs;
-    if ((o[3] != Py_None && !z.take(o[3], "z", frames, dy.t, rows)) || !dx.output(o[6], "dx", frames, at::kBFloat16, *dy.t, rows)) return nullptr;
+    if ((o[3] != Py_None && !z.take(o[3], "z", frames, dy.t, rows)) || !dx.output(o[6], "dx", frames, at::kBFloat16, *dy.t, rows) || !apart("dx", dx, {&dy})) return nullptr;
     if (!place.stream(stream) || BB200_CALL(bbcu_bf16_DenseAffine_BackwardInput, dy.in<const bbcu_bf16_t *>(), static_cast<const bbcu_bf16_t *>(W->const_data_ptr()),
                            z.t ? z.in<const bbcu_bf16_t *>() : nullptr, dx.out<bbcu_bf16_t *>(), act, gated, inputs, nodes, frames, w_stride, dy.stride, z.stride,
                            dx.stride, stream)) return nullptr;

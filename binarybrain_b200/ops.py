@@ -541,7 +541,7 @@ def dense_weights(W):
 
 def dense_forward(x, W, frames, bias=None, activation=None, residual=None, y=None, dtype=torch.bfloat16, keep=False):
     """y = activation(W x + bias) + residual as a frame buffer of `dtype` (bf16 or fp32).  x [in, frame_stride] and W [out, in] bf16 in rows on 16-byte
-    boundaries, bias [out] fp32, residual in y's type, activation none, relu, gelu or silu.  keep: True, or a bf16 buffer for it: z = W x + bias, which the
+    boundaries, bias [out] fp32, residual in y's type (y may be the residual itself), activation none, relu, gelu or silu.  keep: True, or a bf16 buffer for it: z = W x + bias, which the
     gradient of an activation needs, is returned as well."""
     if dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"dtype: expected float32 or bfloat16, got {dtype}")
@@ -555,7 +555,7 @@ def gated_dense_forward(x, W, frames, bias=None, activation="silu", y=None, keep
 
 
 def dense_backward_input(dy, W, frames, z=None, activation=None, gated=False, dx=None):
-    """dx = W^T dy, bf16.  Where the layer's input was activation(z): with z given, the gradient of z.  Where it was a gated block's output: with that block's z
+    """dx = W^T dy, bf16.  Where the layer's input was activation(z): with z given, the gradient of z (dx may be z itself).  Where it was a gated block's output: with that block's z
     and gated=True, the gradient of that z, [2 * in, frame_stride]."""
     return _n.dense_backward_input(dy, W, frames, z, _activation(activation), bool(gated), dx)
 

@@ -439,7 +439,7 @@ int bbcu_bf16_LossDistillation(const bbcu_bf16_t *dev_z_buf, bbcu_bf16_t *dev_dz
 /* ------------------------------------------------------------------ Additive: training and serving that teacher in bf16.
  * No counterparts in the reference.  The rules of the section above hold; each output is rounded once, from 32 bits.  The products' operands are read by
  * TMA: rows of W, x and dy start on 16-byte boundaries (strides in elements, multiples of 8; BBCU_ERR_BAD_STRIDE otherwise), what lies in their padding is
- * not used.  The other buffers may have any stride and alignment.  Extents up to 2^27, BBCU_ERR_TOO_LARGE beyond. */
+ * not used.  The other buffers may have any stride and alignment; y may be the residual itself, and dx the z that it is the gradient of.  Extents up to 2^27, BBCU_ERR_TOO_LARGE beyond. */
 #define BBCU_ACTIVATION_NONE 0
 #define BBCU_ACTIVATION_RELU 1
 #define BBCU_ACTIVATION_GELU 2          /* z * (1 + erf(z / sqrt 2)) / 2 */

@@ -219,6 +219,39 @@ def test_dense_calls_without_frames():
     assert (dW == 1).all() and (db == 1).all()
 
 
+# frames of odd rows, few frames, one CTA's tiles, tiles whose k is split, pairs; the values of a call with outputs of its own, bit by bit
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["rows", "odd"])
+@pytest.mark.parametrize("K,O,F", [(70, 33, 5), (520, 300, 1), (300, 130, 65), (1020, 250, 200), (4096, 100, 40), (640, 700, 3001), (512, 1100, 4100)])
+def test_dense_outputs_in_the_place_of_what_they_are_made_of(K, O, F, layout):
+    from binarybrain_b200 import ops
+    x, W, z = buffer(normal(90, K, F).to(BF16), BF16), ops.dense_weights(normal(91, O, K).cuda() / K ** 0.5), normal(92, 2 * K, F).to(BF16)
+    for dtype in (BF16, torch.float32):
+        r = normal(93, O, F).to(dtype)
+        want = ops.dense_forward(x, W, F, activation="silu", residual=buffer(r, dtype, layout), dtype=dtype, y=buffer(r, dtype, layout))
+        y = buffer(r, dtype, layout)
+        assert torch.equal(ops.dense_forward(x, W, F, activation="silu", residual=y, dtype=dtype, y=y)[:, :F], want[:, :F])
+    dy = buffer(normal(94, O, F).to(BF16), BF16)
+    for gated in (False, True):
+        zs = z if gated else z[:K]
+        want = ops.dense_backward_input(dy, W, F, z=buffer(zs, BF16, layout), activation="gelu", gated=gated, dx=buffer(zs, BF16, layout))
+        dz = buffer(zs, BF16, layout)
+        assert torch.equal(ops.dense_backward_input(dy, W, F, z=dz, activation="gelu", gated=gated, dx=dz)[:, :F], want[:, :F])
+
+
+@pytest.mark.gpu
+def test_outputs_in_the_place_of_what_is_still_read_are_refused():
+    from binarybrain_b200 import ops
+    x, W, W2 = torch.zeros((64, 48), dtype=BF16, device="cuda"), ops.dense_weights(torch.zeros(64, 64, device="cuda")), ops.dense_weights(torch.zeros(128, 64, device="cuda"))
+    other, z = torch.zeros_like(x), torch.zeros((128, 48), dtype=BF16, device="cuda")
+    calls = [lambda: ops.dense_forward(x, W, 48, y=x), lambda: ops.dense_forward(x, W, 48, keep=x), lambda: ops.dense_forward(x, W, 48, y=other, keep=other),
+             lambda: ops.dense_forward(x, W, 48, residual=other, keep=other), lambda: ops.gated_dense_forward(x, W2, 48, y=x), lambda: ops.gated_dense_forward(x, W2, 48, y=z[:64], keep=z),
+             lambda: ops.dense_backward_input(x, W, 48, dx=x), lambda: ops.rms_norm_forward(x, 48, residual=x, y=other, s=other)]
+    for call in calls:
+        with pytest.raises(ValueError, match="memory of its own"):
+            call()
+
+
 # ------------------------------------------------------------------------------------------------------------------------ RMS norm
 RMS_SIZES = [(1, 1), (1, 37), (2, 8), (3, 1), (7, 5), (31, 33), (64, 9), (70, 100), (129, 257), (420, 512), (1000, 31), (1024, 1), (1025, 130), (3000, 401), (4096, 1), (4097, 65),
              (5000, 1), (8192, 70), (9001, 16), (17000, 40), (40000, 3), (65536, 9), (70001, 33), (16, 20000), (100, 9001), (2500, 4800)]
