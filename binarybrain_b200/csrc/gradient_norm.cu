@@ -27,35 +27,62 @@ __device__ __forceinline__ double block_total(double v, double *smem)      // in
     return v;
 }
 
-// The tensors in pieces of kPieceSize elements (kSmallPiece where those would leave most CTAs without one), numbered through for 512 tensors at a time; the CTAs take
+// The tensors in pieces of kPieceSize elements (kSmallPiece where three quarters of the CTAs would have none), numbered through for 512 tensors at a time; the CTAs take
 // turns at them, from the first or, BACK, from the last one.  f(tensor, first element, count) is called by the whole CTA.  (Tensor by tensor, each over all
-// threads, 200 tensors of 1000 took 250 us, now 8.  Pieces of 4096: 6 x 65536 x 64 130 us, of 8192 126; four small tensors 7.8 and 9.5.)
+// threads, 200 tensors of 1000 took 250 us, now 8.  Pieces of 4096: 6 x 65536 x 64 130 us, of 8192 126; four small tensors then 7.8 and 9.5; numbered
+// by all warps, in one size after the other, and their sizes asked for behind the norm, those took 7.6, now 6.2.)
 constexpr int kPieceSize = 8192, kSmallPiece = 2048;
-template <bool BACK, typename F> __device__ __forceinline__ void for_pieces(int size, const int *__restrict__ size_table, F f)
+// start[t + 1] = the pieces of the tensors up to t.  Only the warps that have a tensor number theirs.
+__device__ __forceinline__ void number_pieces(int count, int size, int *start, int2 *warp_sum, int &piece)
 {
-    __shared__ int start[kNormThreads + 1], warp_sum[kNormThreads / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tables = (size + kNormThreads - 1) / kNormThreads;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int warps = (count + 31) / 32;
+    const bool both = count <= (int)gridDim.x / 4;                        // too few pieces are possible
+    int2 n;                                                               // by either size of pieces
+    __syncthreads();                                                      // the numbers before are done with
+    if (warp < warps) {
+        n = make_int2((int)((unsigned)(size + kPieceSize - 1) / kPieceSize), (int)((unsigned)(size + kSmallPiece - 1) / kSmallPiece));
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int2 before = make_int2(__shfl_up_sync(0xffffffffu, n.x, d), both ? __shfl_up_sync(0xffffffffu, n.y, d) : 0);
+            if (lane >= d) { n.x += before.x; n.y += before.y; }
+        }
+        if (lane == 31) warp_sum[warp] = n;
+    }
+    if (warps > 1) __syncthreads();
+    else __syncwarp();
+    if (warp < warps) {
+        int whole = 0;
+        for (int w = 0; w < (both ? warps : warp); ++w) {
+            const int2 s = warp_sum[w];
+            whole += s.x;
+            if (w < warp) { n.x += s.x; n.y += s.y; }
+        }
+        const bool small = both && whole <= (int)gridDim.x / 4;
+        start[threadIdx.x + 1] = small ? n.y : n.x;
+        if (threadIdx.x == 0) {
+            start[0] = 0;
+            piece = small ? kSmallPiece : kPieceSize;
+        }
+    }
+    __syncthreads();
+}
+
+template <bool BACK> __device__ __forceinline__ int first_size(int size, const int *__restrict__ size_table)
+{
+    const int t = (BACK ? (size - 1) / kNormThreads * kNormThreads : 0) + (int)threadIdx.x;
+    return t < size ? size_table[t] : 0;
+}
+template <bool BACK, typename F> __device__ __forceinline__ void for_pieces(int size, const int *__restrict__ size_table, int size_here, F f)
+{
+    __shared__ int start[kNormThreads + 1], piece_size;
+    __shared__ int2 warp_sum[kNormThreads / 32];
+    const int tables = (size + kNormThreads - 1) / kNormThreads;
     for (int k = 0; k < tables; ++k) {
         const int t0 = (BACK ? tables - 1 - k : k) * kNormThreads, count = min(kNormThreads, size - t0);
-        const long long size_here = (int)threadIdx.x < count ? size_table[t0 + threadIdx.x] : 0;
-        auto number = [&](int piece) {
-            int n = (int)((size_here + piece - 1) / piece);
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int before = __shfl_up_sync(0xffffffffu, n, d);
-                if (lane >= d) n += before;
-            }
-            __syncthreads();                                              // the numbers before are done with
-            if (lane == 31) warp_sum[warp] = n;
-            __syncthreads();
-            for (int w = 0; w < warp; ++w) n += warp_sum[w];
-            start[threadIdx.x + 1] = n;
-            if (threadIdx.x == 0) start[0] = 0;
-            __syncthreads();
-        };
-        int piece = kPieceSize;
-        number(piece);
-        if (start[count] * 4 <= (int)gridDim.x) number(piece = kSmallPiece);
+        if (k > 0) size_here = (int)threadIdx.x < count ? size_table[t0 + threadIdx.x] : 0;
+        number_pieces(count, size_here, start, warp_sum, piece_size);
+        const int piece = piece_size;
         const int total = start[count], step = (int)gridDim.x;
         int t = 0;
         for (int c = BACK ? (total - 1 - (int)blockIdx.x) / step * step + (int)blockIdx.x : (int)blockIdx.x; c >= (int)blockIdx.x && c < total; c += BACK ? -step : step) {
@@ -81,7 +108,7 @@ k_gradient_squares(int size, const int *__restrict__ size_table, float *const *_
     __shared__ double red[kNormThreads / 32];
     double sum = 0.0;
     auto add = [&](float g) { sum = fma((double)g, (double)g, sum); };
-    for_pieces<false>(size, size_table, [&](int t, int first, int count) {
+    for_pieces<false>(size, size_table, first_size<false>(size, size_table), [&](int t, int first, int count) {
         const float *g = grads[t] + first;
         const int quads = (reinterpret_cast<uintptr_t>(g) & 15) == 0 ? count / 4 : 0;
         float4 q[kPieceSize / 4 / kNormThreads];
@@ -121,11 +148,12 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtasPerSm)
 k_gradient_clip(int size, const int *__restrict__ size_table, float *const *__restrict__ grads, const double *part, int parts, float max_norm, float *norm_out)
 {
     grid_dependency();
+    const int size_here = first_size<true>(size, size_table);             // on its way beside the parts
     const double norm = norm_of(part, parts);
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const float factor = clip_factor(norm, max_norm);
     if (factor == 1.0f) return;                                           // nothing changes
-    for_pieces<true>(size, size_table, [&](int t, int first, int count) {
+    for_pieces<true>(size, size_table, size_here, [&](int t, int first, int count) {
         float *g = grads[t] + first;
         const int quads = (reinterpret_cast<uintptr_t>(g) & 15) == 0 ? count / 4 : 0;
 #pragma unroll 2
@@ -144,10 +172,11 @@ k_adam_clipped(int size, const int *__restrict__ size_table, float *const *__res
                float *const *__restrict__ v_tab, float lr_t, float beta1, float beta2, const double *part, int parts, float max_norm, float *norm_out)
 {
     grid_dependency();
+    const int size_here = first_size<true>(size, size_table);             // on its way beside the parts
     const double norm = norm_of(part, parts);
     if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
     const float factor = clip_factor(norm, max_norm);
-    for_pieces<true>(size, size_table, [&](int t, int first, int count) {
+    for_pieces<true>(size, size_table, size_here, [&](int t, int first, int count) {
         float *p = params[t] + first, *m = m_tab[t] + first, *v = v_tab[t] + first, *g = grads[t] + first;
         const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(g)) & 15) == 0;
         const int quads = vec ? count / 4 : 0;

@@ -497,6 +497,16 @@ def test_clipped_adam(sizes, max_norm, odd):
             assert torch.equal(g[i].double(), g0) if step < 2 else not g[i].any()
 
 
+# tensors as many as a warp, as a quarter of the CTAs and as a table of the kernels' has, and one more; empty ones among them, one larger than a piece
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [31, 32, 33, 74, 75, 511, 512, 513, 1300])
+def test_clipping_and_the_clipped_step_of_many_tensors(count):
+    sizes = [0 if i % 7 == 3 else 1 + 37 * i % 301 for i in range(count)]
+    sizes[count // 2] = 20011
+    test_gradient_norm_and_clipping(sizes, False)
+    test_clipped_adam(sizes, 0.5, False)
+
+
 @pytest.mark.gpu
 def test_a_limit_that_is_not_reached_leaves_the_plain_step():
     from binarybrain_b200 import ops
