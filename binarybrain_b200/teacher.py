@@ -75,15 +75,19 @@ class RmsNormalization:
 
 
 class DenseAffine:
-    """A dense layer in bf16: activation(W x + bias) + residual.  The weights that are trained are fp32; refresh() lays them out in bf16 as the product reads
-    them, after they have changed.  backward() returns the gradient of x and adds to dW and dbias; the residual's gradient is dy itself."""
+    """A dense layer in bf16: y = activation(z) + residual, z = W x + bias.  The weights that are trained are fp32; refresh() lays them out in bf16 as the product
+    reads them, after they have changed.  backward() returns the gradient of x and adds to dW and dbias.  Without an activation it takes the gradient of y, which is
+    the residual's as well.  With one it takes that of z, as the layer above returns it when this one is its `below`: what is made of y by anything else, a norm or a
+    loss, has no way back through an activation here, and neither has the residual beside one."""
+
+    gated = False                                        # a gated block's z has twice the rows of its y, which tells the gradients apart
 
     def __init__(self, W, bias=None, activation=None, dtype=torch.bfloat16):
         self.n_in, self.n_out, self.activation, self.dtype = W.shape[1], W.shape[0], activation, dtype
         self.W, self.bias = W.float().contiguous(), bias
         self.dW, self.dbias = torch.zeros_like(self.W), None if bias is None else torch.zeros_like(bias)
         self.W16 = ops.dense_weights(self.W)
-        self._saved = None
+        self._saved, self._z_given, self._beside = None, False, False
 
     def parameters(self):
         return [(self.W, self.dW)] + ([] if self.bias is None else [(self.bias, self.dbias)])
@@ -95,12 +99,14 @@ class DenseAffine:
         keep = train and self.activation not in (None, "none")
         y = ops.dense_forward(x, self.W16, frames, bias=self.bias, activation=self.activation, residual=residual, y=y, dtype=self.dtype, keep=keep)
         y, z = y if keep else (y, None)
-        self._saved = (x, z, frames) if train else None
+        self._saved, self._z_given, self._beside = (x, z, frames) if train else None, False, keep and residual is not None
         return y
 
-    def backward(self, dy, dx=None, below=None):
-        """dy: the gradient of y, or, for a layer with an activation, of z: what the layer above returns when this one is its `below`.  below: the layer whose
-        output x is; where that has an activation or is gated, the gradient of its z is returned."""
+    def backward(self, dy, dx=None, below=None, of_z=False):
+        """dy: the gradient of y, or, for a layer with an activation, of z: what the layer above returns when this one is its `below`, or, with of_z=True, the caller's
+        own.  below: the layer whose output x is; where that has an activation or is gated, the gradient of its z is returned."""
+        if self.activation not in (None, "none") and not (self.gated or self._z_given or of_z):
+            raise ValueError("dy: the gradient of y, where a layer with an activation takes that of z (give this layer to the one above as its `below`)")
         x, _, frames = self._saved
         ops.dense_backward_weights(x, dy, frames, dW=self.dW, dbias=self.dbias)
         z, activation, gated = below.kept() if below is not None else (None, None, False)
@@ -109,12 +115,18 @@ class DenseAffine:
         return dx
 
     def kept(self):
-        return self._saved[1], self.activation, False
+        """For the layer above, which returns the gradient of z."""
+        if self._beside:
+            raise ValueError("below: a layer with a residual beside its activation, whose gradient would be lost")
+        self._z_given = True
+        return self._saved[1], self.activation, self.gated
 
 
 class GatedDense(DenseAffine):
     """The gated block: activation(g) * u, g and u the upper and the lower half of W x + bias.  backward() takes the gradient of both, as the layer above
     returns it when this one is its `below`."""
+
+    gated = True
 
     def __init__(self, W, bias=None, activation="silu"):
         super().__init__(W, bias, activation)
@@ -125,9 +137,6 @@ class GatedDense(DenseAffine):
         y, z = y if train else (y, None)
         self._saved = (x, z, frames) if train else None
         return y
-
-    def kept(self):
-        return self._saved[1], self.activation, True
 
 
 class FeedForward:

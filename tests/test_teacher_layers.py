@@ -1,0 +1,114 @@
+"""Layers of the bf16 teacher as a network strings them together: which gradient a layer takes and returns, what it keeps, and what it refuses.
+
+The refusals come before any operator, so that they are tested without a GPU too, on operators that only give buffers of the right shape.
+"""
+import math
+import types
+
+import pytest
+import torch
+
+from test_teacher_operators import buffer, normal
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture
+def shapes_only(monkeypatch):
+    """The operators of `teacher` replaced by ones that return zeros of the shapes that the real ones return, and note their calls."""
+    from binarybrain_b200 import ops, teacher
+    calls = []
+
+    def frames(rows, x):
+        return torch.zeros((rows, x.shape[1]), dtype=BF16)
+
+    def dense_forward(x, W, n, activation=None, keep=False, **kw):
+        calls.append("dense_forward")
+        y = frames(W.shape[0], x)
+        return (y, frames(W.shape[0], x)) if keep else y
+
+    def gated_dense_forward(x, W, n, keep=False, **kw):
+        calls.append("gated_dense_forward")
+        y = frames(W.shape[0] // 2, x)
+        return (y, frames(W.shape[0], x)) if keep else y
+
+    def dense_backward_input(dy, W, n, z=None, activation=None, gated=False, dx=None):
+        calls.append(("dense_backward_input", None if z is None else tuple(z.shape), activation, gated))
+        return frames(W.shape[1] * (2 if gated else 1), dy)
+
+    def dense_backward_weights(x, dy, n, dW=None, dbias=None):
+        calls.append("dense_backward_weights")
+        return dW, dbias
+
+    def rms_norm_forward(x, n, gamma=None, eps=1e-5, residual=None, y=None, s=None, rstd=None):
+        return frames(x.shape[0], x), x if residual is None else frames(x.shape[0], x), torch.ones(n)
+
+    def rms_norm_backward(s, dy, rstd, n, gamma=None, dresidual=None, ds=None, dgamma=None):
+        return frames(s.shape[0], s), dgamma
+    plain = types.SimpleNamespace(dense_weights=ops.dense_weights, dense_forward=dense_forward, gated_dense_forward=gated_dense_forward, dense_backward_input=dense_backward_input,
+                                  dense_backward_weights=dense_backward_weights, rms_norm_forward=rms_norm_forward, rms_norm_backward=rms_norm_backward)
+    monkeypatch.setattr(teacher, "ops", plain)
+    return calls
+
+
+def test_a_gradient_of_y_is_refused_where_that_of_z_is_needed(shapes_only):
+    from binarybrain_b200.teacher import DenseAffine, GatedDense
+    x, dy = torch.zeros((8, 16), dtype=BF16), torch.zeros((12, 16), dtype=BF16)
+    for activation in ("relu", "gelu", "silu"):
+        lower, upper = DenseAffine(torch.zeros(12, 8), activation=activation), DenseAffine(torch.zeros(8, 12))
+        h = lower.forward(x, 16)
+        upper.forward(h, 16)
+        del shapes_only[:]
+        with pytest.raises(ValueError, match="gradient of y"):
+            lower.backward(dy)
+        g = upper.backward(x)                                             # without `below`: the gradient of y
+        with pytest.raises(ValueError, match="gradient of y"):
+            lower.backward(g)
+        assert "dense_backward_weights" in shapes_only and shapes_only.count("dense_backward_weights") == 1       # nothing was added to the refused layer's gradients
+        upper.forward(lower.forward(x, 16), 16)
+        assert lower.backward(upper.backward(x, below=lower)).shape == (8, 16)
+        assert ("dense_backward_input", (12, 16), activation, False) in shapes_only
+        lower.forward(x, 16)                                              # a new pass: the layer above has not been asked yet
+        with pytest.raises(ValueError, match="gradient of y"):
+            lower.backward(dy)
+        lower.backward(dy, of_z=True)
+    for plain in (DenseAffine(torch.zeros(12, 8)), DenseAffine(torch.zeros(12, 8), activation="none")):
+        plain.forward(x, 16, residual=dy)
+        plain.backward(dy)
+    gate = GatedDense(torch.zeros(24, 8))
+    gate.forward(x, 16)
+    gate.backward(torch.zeros((24, 16), dtype=BF16))
+
+
+def test_a_residual_beside_an_activation_is_for_serving(shapes_only):
+    from binarybrain_b200.teacher import DenseAffine
+    x, r = torch.zeros((8, 16), dtype=BF16), torch.zeros((12, 16), dtype=BF16)
+    lower, upper = DenseAffine(torch.zeros(12, 8), activation="relu"), DenseAffine(torch.zeros(8, 12))
+    upper.forward(lower.forward(x, 16, residual=r), 16)
+    with pytest.raises(ValueError, match="residual"):
+        upper.backward(x, below=lower)
+    upper.forward(lower.forward(x, 16), 16)
+    lower.backward(upper.backward(x, below=lower))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("K,H,O,F", [(64, 100, 40, 33), (300, 513, 260, 500)])
+def test_two_dense_layers_and_their_gradients(K, H, O, F, activation):
+    """activation(W1 x + b1), W2 of it + b2 + residual, against torch's gradients of the same in 64 bits.  Three stored intermediates (z, h and dz) lie between, each with a
+    relative error of 2^-8 / sqrt(3) in the 2-norm where errors are independent, and the output is rounded once more.  (A rounded z keeps its sign, so that relu's
+    slope is the same.)"""
+    from binarybrain_b200.teacher import DenseAffine
+    lower = DenseAffine((normal(1, H, K) / math.sqrt(K)).float().cuda(), bias=(0.5 * normal(2, H)).float().cuda(), activation=activation)
+    upper = DenseAffine((normal(3, O, H) / math.sqrt(H)).float().cuda(), bias=(0.5 * normal(4, O)).float().cuda())
+    x, r, dy = buffer(normal(5, K, F), BF16), buffer(normal(6, O, F), BF16), buffer(normal(7, O, F), BF16)
+    y = upper.forward(lower.forward(x, F), F, residual=r)
+    dx = lower.backward(upper.backward(dy, below=lower))
+    leaves = [t.double().requires_grad_() for t in (x[:, :F], lower.W16, lower.bias, upper.W16, upper.bias)]
+    z = leaves[1] @ leaves[0] + leaves[2][:, None]
+    h = {"relu": torch.relu, "silu": torch.nn.functional.silu, "gelu": lambda t: 0.5 * t * torch.special.erfc(-t * math.sqrt(0.5))}[activation](z)
+    y64 = leaves[3] @ h + leaves[4][:, None] + r[:, :F].double()
+    (y64 * dy[:, :F].double()).sum().backward()
+    bound = 4 * 2.0 ** -8 / math.sqrt(3)
+    for got, want in ((y[:, :F], y64), (dx[:, :F], leaves[0].grad), (lower.dW, leaves[1].grad), (lower.dbias, leaves[2].grad), (upper.dW, leaves[3].grad), (upper.dbias, leaves[4].grad)):
+        assert float((got.double() - want.detach()).norm() / want.detach().norm()) <= bound
