@@ -595,7 +595,7 @@ PyObject *rms_norm_forward_body(PyObject *const *o)
         (o[4] != Py_None && (!residual.take(o[4], "residual", frames, x.t, nodes) || !s.output(o[6], "s", frames, x.t->scalar_type(), *x.t, nodes))) ||
         !y.output(o[5], "y", frames, x.t->scalar_type(), *x.t, nodes) || !rstd.output(o[7], "rstd", frames, *x.t)) return nullptr;
     if (o[4] == Py_None && o[6] != Py_None) { refuse("s", "given without a residual"); return nullptr; }
-    if (!apart("y", y, {&s})) return nullptr;
+    if (!apart("y", y, {s.t ? &s : &x})) return nullptr;                  // without a residual x is what is returned as s
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_RmsNormalization_Forward, bbcu_bf16_RmsNormalization_Forward, float, bbcu_bf16_t, x.in<const T *>(),
                            residual.t ? residual.in<const T *>() : nullptr, s.t ? s.out<T *>() : nullptr, y.out<T *>(), gamma.data, rstd.data, eps, nodes, frames, x.stride,
                            residual.stride, s.stride, y.stride, stream)) return nullptr;

@@ -518,7 +518,7 @@ def _activation(name):
 
 def rms_norm_forward(x, frames, gamma=None, eps=1e-5, residual=None, y=None, s=None, rstd=None):
     """Root-mean-square norm over the nodes of every frame of s = x + residual, which is kept in x's type (without a residual s is x): returns (y, s, rstd),
-    y = s * rstd * gamma, rstd [frames] fp32.  A given s may be x or residual itself."""
+    y = s * rstd * gamma, rstd [frames] fp32.  A given s may be x or residual itself; y may not be s, nor, without a residual, x."""
     return _n.rms_norm_forward(x, frames, gamma, eps, residual, y, s, rstd)
 
 

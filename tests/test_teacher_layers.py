@@ -112,3 +112,18 @@ def test_two_dense_layers_and_their_gradients(K, H, O, F, activation):
     bound = 4 * 2.0 ** -8 / math.sqrt(3)
     for got, want in ((y[:, :F], y64), (dx[:, :F], leaves[0].grad), (lower.dW, leaves[1].grad), (lower.dbias, leaves[2].grad), (upper.dW, leaves[3].grad), (upper.dbias, leaves[4].grad)):
         assert float((got.double() - want.detach()).norm() / want.detach().norm()) <= bound
+
+
+@pytest.mark.gpu
+def test_the_norm_does_not_overwrite_what_it_returns_as_s():
+    """Without a residual s is x, which the backward pass reads: y in its place is refused, and x is left as it was."""
+    from binarybrain_b200 import ops
+    from binarybrain_b200.teacher import RmsNormalization
+    for N, F, dtype in ((70, 33, BF16), (300, 5, torch.float32)):
+        x = buffer(normal(20, N, F), dtype)
+        before = x.clone()
+        for call in (lambda: ops.rms_norm_forward(x, F, y=x), lambda: RmsNormalization(N).forward(x, F, y=x)):
+            with pytest.raises(ValueError, match="memory of its own"):
+                call()
+        assert torch.equal(x[:, :F], before[:, :F])
+        assert ops.rms_norm_forward(x, F, y=torch.empty_like(x))[1] is x
