@@ -354,12 +354,14 @@ struct Frames {
     at::Tensor made;
     const at::Tensor *t = nullptr;
     int stride = 0;
+    int64_t used = 0;                                    // columns that the call is about
 
     explicit Frames(Place &place) : place(place) {}
     bool check(PyObject *o, const char *name, int64_t frames, int64_t rows)
     {
         if (!THPVariable_Check(o)) { PyErr_Format(PyExc_TypeError, "%s: expected a tensor", name); return false; }
         given = o;
+        used = frames;
         t = &THPVariable_Unpack(o);
         if (!place.take(*t, name)) return false;
         if (t->dim() != 2 || t->size(1) < frames || (t->size(1) > 1 && t->stride(1) != 1) || (t->size(0) > 1 && t->stride(0) < frames))
@@ -394,11 +396,47 @@ struct Frames {
     PyObject *result() const { return given ? Py_NewRef(given) : THPVariable_Wrap(made); }
 };
 
-// an output that does not begin where one of the others does, whose elements are read or written in another order
-bool apart(const char *name, const Frames &out, std::initializer_list<const Frames *> others)
+// The memory that a call reads or writes of a matrix: `width` bytes of each row.
+struct Rows {
+    uintptr_t at = 0;
+    int64_t rows = 0, stride = 0, width = 0;
+
+    Rows() = default;
+    Rows(const Frames &f)
+    {
+        if (!f.given) return;                            // absent, or new
+        const int64_t size = (int64_t)f.t->element_size();
+        *this = Rows(*f.t, f.stride * size, f.used * size);
+    }
+    Rows(const at::Tensor &t, int64_t stride_bytes, int64_t width_bytes)
+        : at(reinterpret_cast<uintptr_t>(t.const_data_ptr())), rows(t.size(0)), stride(t.size(0) > 1 ? stride_bytes : 0), width(width_bytes) {}
+    bool empty() const { return rows <= 0 || width <= 0; }
+    uintptr_t end() const { return at + (uintptr_t)((rows - 1) * stride + width); }
+    bool same(const Rows &o) const { return at == o.at && rows == o.rows && stride == o.stride && width == o.width; }
+    // whether the two have memory in common; of rows at different distances, whether they reach into each other
+    bool meets(const Rows &o) const
+    {
+        if (empty() || o.empty() || end() <= o.at || o.end() <= at) return false;
+        const int64_t step = stride ? stride : o.stride;                  // a single row lies at any distance
+        if (step == 0 || (o.stride && o.stride != step)) return true;
+        const int64_t column = (((int64_t)(o.at - at)) % step + step) % step;
+        return column < width || column + o.width > step;                 // side by side in the same rows otherwise
+    }
+};
+
+// an output whose elements are none of the others', which are read or written in another order
+bool apart(const char *name, const Rows &out, std::initializer_list<Rows> others)
 {
-    for (const Frames *f : others)
-        if (out.t && f->t && f->t->numel() > 0 && f->t->const_data_ptr() == out.t->const_data_ptr()) return refuse(name, "expected memory of its own");
+    for (const Rows &o : others)
+        if (out.meets(o)) return refuse(name, "expected memory of its own");
+    return true;
+}
+
+// an output that is one of the others, element for element, or has nothing of it: each element is read before it is written, by the thread that writes it
+bool apart_or_same(const char *name, const Rows &out, std::initializer_list<Rows> others)
+{
+    for (const Rows &o : others)
+        if (out.meets(o) && !out.same(o)) return refuse(name, "expected memory of its own, or an input as a whole that it may take the place of");
     return true;
 }
 
@@ -595,7 +633,7 @@ PyObject *rms_norm_forward_body(PyObject *const *o)
         (o[4] != Py_None && (!residual.take(o[4], "residual", frames, x.t, nodes) || !s.output(o[6], "s", frames, x.t->scalar_type(), *x.t, nodes))) ||
         !y.output(o[5], "y", frames, x.t->scalar_type(), *x.t, nodes) || !rstd.output(o[7], "rstd", frames, *x.t)) return nullptr;
     if (o[4] == Py_None && o[6] != Py_None) { refuse("s", "given without a residual"); return nullptr; }
-    if (!apart("y", y, {s.t ? &s : &x})) return nullptr;                  // without a residual x is what is returned as s
+    if (!apart("y", y, {s.t ? s : x}) || !apart_or_same("y", y, {x, residual}) || !apart_or_same("s", s, {x, residual})) return nullptr;      // (no residual: x is s)
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_RmsNormalization_Forward, bbcu_bf16_RmsNormalization_Forward, float, bbcu_bf16_t, x.in<const T *>(),
                            residual.t ? residual.in<const T *>() : nullptr, s.t ? s.out<T *>() : nullptr, y.out<T *>(), gamma.data, rstd.data, eps, nodes, frames, x.stride,
                            residual.stride, s.stride, y.stride, stream)) return nullptr;
@@ -616,6 +654,7 @@ PyObject *rms_norm_int8_body(PyObject *const *o)
         (o[4] != Py_None && (!residual.take(o[4], "residual", frames, x.t, nodes) || !s.output(o[5], "s", frames, x.t->scalar_type(), *x.t, nodes))) ||
         !scale.output(Py_None, "scale", frames, *x.t)) return nullptr;
     if (o[4] == Py_None && o[5] != Py_None) { refuse("s", "given without a residual"); return nullptr; }
+    if (!apart_or_same("s", s, {x, residual})) return nullptr;
     const int row = (int)std::min<int64_t>(((int64_t)nodes + 15) / 16 * 16, INT_MAX / 16 * 16);
     at::Tensor q = at::empty({frames, row}, at::TensorOptions().dtype(at::kChar).device(x.t->device()));
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_RmsNormalization_QuantizeInt8, bbcu_bf16_RmsNormalization_QuantizeInt8, float, bbcu_bf16_t,
@@ -636,6 +675,7 @@ PyObject *rms_norm_backward_body(PyObject *const *o)
     if (!parse(o[3], frames) || !s.take(o[0], "s", frames, nullptr, -1) || !fits(s.t->size(0), nodes) || !dy.take(o[1], "dy", frames, s.t, nodes) ||
         !gamma.input(o[4], "gamma", nodes) || !rstd.check(o[2], "rstd", frames, false) || (o[5] != Py_None && !dresidual.take(o[5], "dresidual", frames, s.t, nodes)) ||
         !dgamma.output(o[7], "dgamma", nodes, *s.t) || !ds.output(o[6], "ds", frames, s.t->scalar_type(), *s.t, nodes)) return nullptr;
+    if (!apart_or_same("ds", ds, {s, dy, dresidual})) return nullptr;
     const int accumulate = o[7] != Py_None;
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(s.fp32(), bbcu_fp32_RmsNormalization_Backward, bbcu_bf16_RmsNormalization_Backward, float, bbcu_bf16_t, s.in<const T *>(),
                            dy.in<const T *>(), dresidual.t ? dresidual.in<const T *>() : nullptr, ds.out<T *>(), gamma.data, rstd.data, dgamma.data, accumulate, nodes,
@@ -659,6 +699,8 @@ const at::Tensor *bf16_weights(PyObject *o, Place &place, int &stride)
     if (row < t.size(1) || !on_16(t, row)) { refuse("W", "expected rows that start on 16-byte boundaries (a row stride that is a multiple of 8)"); return nullptr; }
     return fits(row, stride) ? &t : nullptr;
 }
+
+Rows rows_of_weights(const at::Tensor &W, int stride) { return Rows(W, 2 * (int64_t)stride, 2 * W.size(1)); }
 
 bool bf16_operand(Frames &f, PyObject *o, const char *name, int64_t frames, int64_t rows)
 {
@@ -686,8 +728,9 @@ PyObject *dense_forward_body(PyObject *const *o)
     const at::Tensor *W = parse(o[2], frames) && parse(o[4], act) && parse_flag(o[7], bf16) ? bf16_weights(o[1], place, w_stride) : nullptr;
     if (!W || !fits(W->size(0), nodes) || !fits(W->size(1), inputs) || !bf16_operand(x, o[0], "x", frames, inputs) || !bias.input(o[3], "bias", nodes) ||
         (o[6] != Py_None ? !y.take(o[6], "y", frames, nullptr, nodes) : !y.output(Py_None, "y", frames, bf16 ? at::kBFloat16 : at::kFloat, *x.t, nodes)) ||
-        (o[5] != Py_None && !residual.take(o[5], "residual", frames, y.t, nodes)) || !kept(z, o[8], frames, *x.t, nodes) || !apart("y", y, {&x}) ||
-        !apart("z", z, {&x, &y, &residual})) return nullptr;
+        (o[5] != Py_None && !residual.take(o[5], "residual", frames, y.t, nodes)) || !kept(z, o[8], frames, *x.t, nodes)) return nullptr;
+    const Rows of_w = rows_of_weights(*W, w_stride);
+    if (!apart("y", y, {x, of_w}) || !apart_or_same("y", y, {residual}) || !apart("z", z, {x, y, residual, of_w})) return nullptr;
     const auto *in = static_cast<const bbcu_bf16_t *>(x.t->const_data_ptr()), *w = static_cast<const bbcu_bf16_t *>(W->const_data_ptr());
     auto *zp = z.t ? z.out<bbcu_bf16_t *>() : nullptr;
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(y.fp32(), bbcu_bf16_fp32_DenseAffine_Forward, bbcu_bf16_DenseAffine_Forward, float, bbcu_bf16_t, in, w, bias.data,
@@ -722,7 +765,9 @@ PyObject *gated_dense_forward_body(PyObject *const *o)
     if (!W || !fits(W->size(0), rows) || !fits(W->size(1), inputs)) return nullptr;
     if (rows % 2) { refuse("W", "expected an even number of rows, the gate's and those that it multiplies"); return nullptr; }
     if (!bf16_operand(x, o[0], "x", frames, inputs) || !bias.input(o[3], "bias", rows) || !y.output(o[5], "y", frames, at::kBFloat16, *x.t, rows / 2) ||
-        !kept(z, o[6], frames, *x.t, rows) || !apart("y", y, {&x}) || !apart("z", z, {&x, &y})) return nullptr;
+        !kept(z, o[6], frames, *x.t, rows)) return nullptr;
+    const Rows of_w = rows_of_weights(*W, w_stride);
+    if (!apart("y", y, {x, of_w}) || !apart("z", z, {x, y, of_w})) return nullptr;
     if (!place.stream(stream) || BB200_CALL(bbcu_bf16_GatedDense_Forward, x.in<const bbcu_bf16_t *>(), static_cast<const bbcu_bf16_t *>(W->const_data_ptr()), bias.data,
                            y.out<bbcu_bf16_t *>(), z.t ? z.out<bbcu_bf16_t *>() : nullptr, act, inputs, rows / 2, frames, w_stride, x.stride, y.stride, z.stride,
                            stream)) return nullptr;
@@ -741,7 +786,8 @@ PyObject *dense_backward_input_body(PyObject *const *o)
     if (!W || !fits(W->size(0), nodes) || !fits(W->size(1), inputs) || !bf16_operand(dy, o[0], "dy", frames, nodes)) return nullptr;
     if (gated && o[3] == Py_None) { refuse("z", "a gated block's gradient needs what its forward pass kept"); return nullptr; }
     const int64_t rows = gated ? 2 * (int64_t)inputs : inputs;
-    if ((o[3] != Py_None && !z.take(o[3], "z", frames, dy.t, rows)) || !dx.output(o[6], "dx", frames, at::kBFloat16, *dy.t, rows) || !apart("dx", dx, {&dy})) return nullptr;
+    if ((o[3] != Py_None && !z.take(o[3], "z", frames, dy.t, rows)) || !dx.output(o[6], "dx", frames, at::kBFloat16, *dy.t, rows) ||
+        !apart("dx", dx, {dy, rows_of_weights(*W, w_stride)}) || !apart_or_same("dx", dx, {z})) return nullptr;
     if (!place.stream(stream) || BB200_CALL(bbcu_bf16_DenseAffine_BackwardInput, dy.in<const bbcu_bf16_t *>(), static_cast<const bbcu_bf16_t *>(W->const_data_ptr()),
                            z.t ? z.in<const bbcu_bf16_t *>() : nullptr, dx.out<bbcu_bf16_t *>(), act, gated, inputs, nodes, frames, w_stride, dy.stride, z.stride,
                            dx.stride, stream)) return nullptr;

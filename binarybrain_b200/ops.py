@@ -518,7 +518,8 @@ def _activation(name):
 
 def rms_norm_forward(x, frames, gamma=None, eps=1e-5, residual=None, y=None, s=None, rstd=None):
     """Root-mean-square norm over the nodes of every frame of s = x + residual, which is kept in x's type (without a residual s is x): returns (y, s, rstd),
-    y = s * rstd * gamma, rstd [frames] fp32.  A given s may be x or residual itself; y may not be s, nor, without a residual, x."""
+    y = s * rstd * gamma, rstd [frames] fp32.  A given s may be x or residual itself, and y either of them that s is not; y may
+    not be s, nor, without a residual, x."""
     return _n.rms_norm_forward(x, frames, gamma, eps, residual, y, s, rstd)
 
 
@@ -528,7 +529,8 @@ def rms_norm_int8(x, frames, gamma=None, eps=1e-5, residual=None, s=None):
 
 
 def rms_norm_backward(s, dy, rstd, frames, gamma=None, dresidual=None, ds=None, dgamma=None):
-    """Returns (ds, dgamma): ds the gradient of s through y, plus dresidual, the one that arrives by the other path.  A given dgamma is added to."""
+    """Returns (ds, dgamma): ds the gradient of s through y, plus dresidual, the one that arrives by the other path.  A given ds may be s, dy or
+    dresidual itself.  A given dgamma is added to."""
     return _n.rms_norm_backward(s, dy, rstd, frames, gamma, dresidual, ds, dgamma)
 
 

@@ -439,7 +439,8 @@ int bbcu_bf16_LossDistillation(const bbcu_bf16_t *dev_z_buf, bbcu_bf16_t *dev_dz
 /* ------------------------------------------------------------------ Additive: training and serving that teacher in bf16.
  * No counterparts in the reference.  The rules of the section above hold; each output is rounded once, from 32 bits.  The products' operands are read by
  * TMA: rows of W, x and dy start on 16-byte boundaries (strides in elements, multiples of 8; BBCU_ERR_BAD_STRIDE otherwise), what lies in their padding is
- * not used.  The other buffers may have any stride and alignment; y may be the residual itself, and dx the z that it is the gradient of.  Extents up to 2^27, BBCU_ERR_TOO_LARGE beyond. */
+ * not used.  The other buffers may have any stride and alignment; y may be the residual itself, and dx the z that it is the gradient of (the same rows at the same
+ * stride); other outputs have no element of an input or of one another.  Extents up to 2^27, BBCU_ERR_TOO_LARGE beyond. */
 #define BBCU_ACTIVATION_NONE 0
 #define BBCU_ACTIVATION_RELU 1
 #define BBCU_ACTIVATION_GELU 2          /* z * (1 + erf(z / sqrt 2)) / 2 */
@@ -471,7 +472,8 @@ int bbcu_bf16_DenseAffine_BackwardWeights(const bbcu_bf16_t *dev_x_buf, const bb
 
 /* Root-mean-square norm over the nodes of a frame with the residual's addition: s = x + residual, kept in the frames' type in dev_s_buf (dev_residual_buf NULL:
  * s = x, and dev_s_buf is not used); rstd [frame_size] = 1 / sqrt(mean s^2 + eps); y = s * rstd * gamma.  dev_gamma [node_size], NULL: 1.  dev_s_buf may be
- * dev_x_buf or dev_residual_buf itself.  Any stride and alignment; up to 2^20 nodes and 2^27 frames, BBCU_ERR_TOO_LARGE beyond. */
+ * dev_x_buf or dev_residual_buf itself, dev_y_buf either of them that dev_s_buf is not, or, without a residual, dev_x_buf.  Any stride and
+ * alignment; up to 2^20 nodes and 2^27 frames, BBCU_ERR_TOO_LARGE beyond. */
 int bbcu_fp32_RmsNormalization_Forward(const float *dev_x_buf, const float *dev_residual_buf, float *dev_s_buf, float *dev_y_buf, const float *dev_gamma,
                                        float *dev_rstd_buf, float eps, int node_size, int frame_size, int x_frame_stride, int residual_frame_stride,
                                        int s_frame_stride, int y_frame_stride, bbcu_stream_t stream);
@@ -487,7 +489,7 @@ int bbcu_bf16_RmsNormalization_QuantizeInt8(const bbcu_bf16_t *dev_x_buf, const 
                                             float *dev_scale_buf, const float *dev_gamma, float *dev_rstd_buf, float eps, int node_size, int frame_size,
                                             int x_frame_stride, int residual_frame_stride, int s_frame_stride, int q_node_stride, bbcu_stream_t stream);
 /* ds = the gradient of s through y, plus dev_dresidual_buf (may be NULL), the one that arrives by the other path; dgamma [node_size] (may be NULL)
- * overwritten, or with accumulate != 0 added to. */
+ * overwritten, or with accumulate != 0 added to.  dev_ds_buf may be dev_s_buf, dev_dy_buf or dev_dresidual_buf itself. */
 int bbcu_fp32_RmsNormalization_Backward(const float *dev_s_buf, const float *dev_dy_buf, const float *dev_dresidual_buf, float *dev_ds_buf, const float *dev_gamma,
                                         const float *dev_rstd_buf, float *dev_dgamma, int accumulate, int node_size, int frame_size, int s_frame_stride,
                                         int dy_frame_stride, int dresidual_frame_stride, int ds_frame_stride, bbcu_stream_t stream);

@@ -11,6 +11,7 @@ import torch
 from test_teacher_operators import buffer, normal
 
 BF16 = torch.bfloat16
+TYPES = [torch.float32, BF16]
 
 
 @pytest.fixture
@@ -127,3 +128,75 @@ def test_the_norm_does_not_overwrite_what_it_returns_as_s():
                 call()
         assert torch.equal(x[:, :F], before[:, :F])
         assert ops.rms_norm_forward(x, F, y=torch.empty_like(x))[1] is x
+
+
+@pytest.mark.gpu
+def test_outputs_that_reach_into_other_buffers_are_refused():
+    """Wherever they begin: a row further on, a column further on, or the same memory in rows of another length."""
+    from binarybrain_b200 import ops
+    flat = torch.zeros(4096 * 64, dtype=BF16, device="cuda")
+    rows = lambda first, n, stride=48, column=0: flat[first * 48 + column:].as_strided((n, 48 - column if stride == 48 else 48), (stride, 1))  # noqa: E731
+    W, W2 = ops.dense_weights(torch.zeros(64, 64, device="cuda")), ops.dense_weights(torch.zeros(128, 64, device="cuda"))
+    x, r, far, rstd = rows(0, 64), rows(100, 64), rows(500, 64), torch.ones(48, device="cuda")
+    f = 48
+    calls = [lambda: ops.dense_forward(x, W, f, y=rows(1, 64)), lambda: ops.dense_forward(x, W, f, y=rows(63, 64)), lambda: ops.dense_forward(x, W, 40, y=rows(0, 64, column=8)),
+             lambda: ops.dense_forward(x, W, f, residual=r, y=rows(101, 64)), lambda: ops.dense_forward(x, W, f, residual=r, y=rows(100, 64, stride=64)),
+             lambda: ops.dense_forward(x, W, f, residual=r, y=far, keep=rows(470, 64)), lambda: ops.dense_forward(x, W, f, y=far, keep=rows(37, 64)),
+             lambda: ops.dense_forward(x, flat[4800:].as_strided((64, 64), (64, 1)), f, y=rows(150, 64)),
+             lambda: ops.gated_dense_forward(x, W2, f, y=rows(564, 64), keep=rows(500, 128)), lambda: ops.gated_dense_forward(x, W2, f, y=far, keep=rows(20, 128)),
+             lambda: ops.dense_backward_input(x, W, f, dx=rows(2, 64)), lambda: ops.dense_backward_input(x, W, f, z=r, activation="relu", dx=rows(99, 64)),
+             lambda: ops.dense_backward_input(x, W, f, z=rows(100, 128), activation="relu", gated=True, dx=rows(164, 128)),
+             lambda: ops.dense_backward_input(x, W, f, z=r, activation="relu", dx=rows(100, 64, stride=64)),
+             lambda: ops.rms_norm_forward(x, f, y=rows(60, 64)), lambda: ops.rms_norm_forward(x, f, residual=r, s=rows(1, 64)), lambda: ops.rms_norm_forward(x, f, residual=r, y=rows(101, 64)),
+             lambda: ops.rms_norm_forward(x, f, residual=r, y=far, s=rows(501, 64)), lambda: ops.rms_norm_forward(x, f, residual=r, y=x, s=x),
+             lambda: ops.rms_norm_int8(x, f, residual=r, s=rows(120, 64)), lambda: ops.rms_norm_backward(x, r, rstd, f, ds=rows(1, 64)),
+             lambda: ops.rms_norm_backward(x, r, rstd, f, ds=rows(80, 64)), lambda: ops.rms_norm_backward(x, r, rstd, f, dresidual=far, ds=rows(500, 64, stride=64))]
+    for k, call in enumerate(calls):
+        with pytest.raises(ValueError, match="memory of its own"):
+            call()
+            pytest.fail(f"call {k}")
+
+
+@pytest.mark.gpu
+def test_buffers_side_by_side_in_the_same_rows_are_apart():
+    from binarybrain_b200 import ops
+    K, O, F = 96, 96, 40
+    wide = torch.full((K, 3 * 48), float("nan"), dtype=BF16, device="cuda")
+    x, y, z = wide[:, :48], wide[:, 48:96], wide[:, 96:]
+    x[:, :F] = normal(30, K, F).to(BF16).cuda()
+    W = ops.dense_weights((normal(31, O, K) / math.sqrt(K)).cuda())
+    want, kept = ops.dense_forward(x.clone(), W, F, activation="silu", keep=True)
+    ops.dense_forward(x, W, F, activation="silu", y=y, keep=z)
+    assert torch.equal(y[:, :F], want[:, :F]) and torch.equal(z[:, :F], kept[:, :F])
+    want = ops.rms_norm_forward(x.clone(), F)[0]
+    ops.rms_norm_forward(x, F, y=y)
+    assert torch.equal(y[:, :F], want[:, :F])
+
+
+# sizes: few frames by lanes, one launch held in registers and read twice, two passes along the rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=["fp32", "bf16"])
+@pytest.mark.parametrize("layout", ["rows", "odd"])
+@pytest.mark.parametrize("N,F", [(70, 3), (4096, 4), (70, 33), (1025, 130), (16000, 60), (70001, 33), (2500, 4800)])
+def test_norms_in_the_place_of_what_they_are_made_of(N, F, layout, dtype):
+    from binarybrain_b200 import _native, ops
+    x, r, dr = (normal(40 + i, N, F).to(dtype) for i in range(3))
+    gamma = (1 + 0.2 * normal(43, N)).float().cuda()
+    b = lambda t: buffer(t, dtype, layout)  # noqa: E731
+    y, s, rstd = ops.rms_norm_forward(b(x), F, gamma=gamma, residual=b(r), y=b(x), s=b(x))
+    for over_y, over_s in (("x", None), ("r", None), ("x", "r"), ("r", "x")):
+        xs, rs = b(x), b(r)
+        at = {"x": xs, "r": rs, None: b(x)}
+        got = ops.rms_norm_forward(xs, F, gamma=gamma, residual=rs, y=at[over_y], s=at[over_s])
+        assert got[0] is at[over_y] and got[1] is at[over_s]
+        assert torch.equal(got[0][:, :F], y[:, :F]) and torch.equal(got[1][:, :F], s[:, :F]) and torch.equal(got[2], rstd), (over_y, over_s)
+    want, _, alone = ops.rms_norm_forward(b(x), F, gamma=gamma, y=b(r))
+    xs, got = b(x), torch.empty_like(alone)                               # x as y, of which the operator itself keeps nothing
+    forward = _native.bbcu_fp32_RmsNormalization_Forward if dtype == torch.float32 else _native.bbcu_bf16_RmsNormalization_Forward
+    forward(xs.data_ptr(), None, None, xs.data_ptr(), gamma, got, 1e-5, N, F, xs.stride(0), 0, 0, xs.stride(0))
+    assert torch.equal(xs[:, :F], want[:, :F]) and torch.equal(got, alone)
+    ds, dgamma = ops.rms_norm_backward(b(x), b(r), rstd, F, gamma=gamma, dresidual=b(dr), ds=b(x))
+    for over in range(3):
+        given = [b(x), b(r), b(dr)]
+        got = ops.rms_norm_backward(given[0], given[1], rstd, F, gamma=gamma, dresidual=given[2], ds=given[over])
+        assert got[0] is given[over] and torch.equal(got[0][:, :F], ds[:, :F]) and torch.equal(got[1], dgamma), over
