@@ -235,6 +235,7 @@ k_dense_few(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__restrict
         const int rows = min(groups * 16, last - m0), per_group = (rows + groups - 1) / groups;
         const int r0 = group * per_group + g, here = min(per_group, rows - group * per_group);      // rows of the group that exist
         float acc[kParts][4] = {}, total[kParts][4] = {};
+        int done = 0;                                                     // blocks in acc, of whichever pieces of the inputs
         for (int k0 = 0; k0 < a.K; k0 += chunk) {
             const int inputs = min(chunk, a.K - k0), blocks = (inputs + kBlock - 1) / kBlock, begin = blocks * part / parts, end = blocks * (part + 1) / parts;
             const __nv_bfloat16 *const base = W + (long long)(m0 + r0) * ws + k0 + 8 * t;
@@ -265,7 +266,7 @@ k_dense_few(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__restrict
                 }
                 __syncthreads();
             }
-            for (int b = begin, done = 0; b < end; b += kBatch) {
+            for (int b = begin; b < end; b += kBatch) {
                 fetch(b + kBatch, next);
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {

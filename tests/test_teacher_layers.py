@@ -200,3 +200,26 @@ def test_norms_in_the_place_of_what_they_are_made_of(N, F, layout, dtype):
         given = [b(x), b(r), b(dr)]
         got = ops.rms_norm_backward(given[0], given[1], rstd, F, gamma=gamma, dresidual=given[2], ds=given[over])
         assert got[0] is given[over] and torch.equal(got[0][:, :F], ds[:, :F]) and torch.equal(got[1], dgamma), over
+
+
+# ------------------------------------------------------------------------------------------------------------------------ sums of 32 bits
+U = 2.0 ** -24
+
+
+def error_of_product(K, O, F):
+    """The error of the 2-norm of an fp32 product of K terms, and what that of a sum of 32 bits, term after term, is: the partial sums are sqrt(k / K) of the
+    last one, each addition rounds by up to U / 2 to U of one, 0.43 U with errors evenly spread, independently: 0.43 U sqrt(sum k / K) = 0.3 U sqrt(K).  (One more
+    rounding for the output.)"""
+    from binarybrain_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(K + F)
+    x = torch.randn((K, (F + 15) // 16 * 16), device="cuda", generator=g).to(BF16)
+    W = ops.dense_weights(torch.randn((O, K), device="cuda", generator=g))
+    got, want = ops.dense_forward(x, W, F, dtype=torch.float32)[:, :F].double(), W.double() @ x[:, :F].double()
+    return float((got - want).norm() / want.norm()), (0.3 * math.sqrt(K) + 1) * U
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,O,F", [(20000, 16, 8), (400000, 16, 8), (400000, 300, 4), (1 << 20, 150, 1)])
+def test_sums_of_few_frames_keep_their_digits(K, O, F):
+    error, in_order = error_of_product(K, O, F)
+    assert error <= in_order
