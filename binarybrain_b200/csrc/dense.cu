@@ -11,6 +11,7 @@
 // Frame buffers are read as they lie, frames next to each other: where the product sums over nodes, its operand is "across" (rows of shared memory along
 // the frames), which the tensor cores take from TMA's 128-byte swizzled boxes as well as rows along k; the gradients read W and x the other way round, and nothing is transposed.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include <cuda.h>
@@ -24,7 +25,6 @@ namespace bb200 {
 enum DenseKind { kForward, kGated, kInputGrad, kWeightGrad };
 
 constexpr int kTileM = 128, kTileK = 64;                 // output rows of a CTA; k of a stage (128 bytes)
-constexpr int kChunk = 12;                               // stages of k between two additions in registers, where sums are taken out on the way (see the tiles below)
 constexpr int kMostSplits = 8;
 constexpr int kTileGroup = 8;                            // tiles of output rows that are walked together, so that their operands stay in L2
 
@@ -34,7 +34,7 @@ struct DenseArgs {
     void *out, *z_out;
     int act, gated, accumulate, vec;                     // vec: the rows of extra, out and z_out start on 16-byte boundaries; 2: on 32-byte ones
     int M, N, K, half;                                   // half: rows of a gated block's output, the distance between its two products
-    int splits;
+    int splits, chunk;                                   // chunk: stages of k between two additions in registers, for fp32 outputs (see sums_chunk)
     long long extra_stride, out_stride, z_stride;
     int *fault;
 };
@@ -292,7 +292,7 @@ k_dense_few(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__restrict
                     }
                 }
                 done += kBatch;
-                if (sizeof(T) == 4 && done >= kChunk * kTileK / kBlock) {  // the tensor cores cut what does not fit their running sum, see kChunk
+                if (sizeof(T) == 4 && done >= a.chunk * (kTileK / kBlock)) {  // the tensor cores cut what does not fit their running sum
                     done = 0;
 #pragma unroll
                     for (int p = 0; p < kParts; ++p)
@@ -335,9 +335,7 @@ k_dense_few(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__restrict
 // that way, and 50 bytes a clock are what an SM gets.  A pair's tile is 128 rows x 256 columns of the output instead, 64 rows of either product in the 128
 // lanes of a CTA, and the warps of the lower lanes get the second product's sums from those of the upper ones through shared memory.
 //
-// fp32 outputs: the tensor cores cut the digits that do not fit their running sum, which over thousands of steps drifts towards zero; those sums are taken out
-// after every kChunk stages and added up in registers.  (Error of the 2-norm of dW, 4096 x 4096 x 8192, and of y: 4.8e-7 at 8 stages, 7.2e-7 at 12, 1.0e-6 at 16, 2.1e-6 at
-// 32; plain fp32 1e-6.  Taking them out stands in the products' way in TMEM: dW 246, 239, 236 us at 8, 12, 16.)
+// fp32 outputs: the sums are taken out every a.chunk stages and added up in registers, see sums_chunk().
 template <int KIND, typename T, int TN, bool PAIR> struct DenseShape {
     static constexpr bool kAAcross = KIND == kInputGrad, kBAcross = KIND != kWeightGrad, kPromote = sizeof(T) == 4;
     static constexpr bool kStacked = KIND == kGated && PAIR;
@@ -597,7 +595,7 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         bool ok = true;
         for (int tile = first; tile < tiles && ok; tile += step) {
             for (int c = k0; c < k1 && ok;) {
-                const int end = S::kPromote ? min(c + kChunk, k1) : k1, begin = c;
+                const int end = S::kPromote ? min(c + a.chunk, k1) : k1, begin = c;
                 ok = mbar_wait_one(&acc_empty[acc], acc_phase ^ 1, &gave_up);
                 if (!ok) break;
                 tcgen05_fence_after();
@@ -671,7 +669,7 @@ k_dense_tiles(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
             if constexpr (S::kPromote) {
 #pragma unroll
                 for (int i = 0; i < S::kWarpColumns; ++i) sums[i] = 0.0f;
-                for (int c = k0; c < k1; c += kChunk) {
+                for (int c = k0; c < k1; c += a.chunk) {
                     ok = mbar_wait_warp(&acc_full[acc], acc_phase, &gave_up);
                     if (!ok) break;
                     tcgen05_fence_after();
@@ -983,6 +981,14 @@ static int dense_tiles(const Operand &A, const Operand &B, const DenseArgs &a, c
     return launch_cluster(kernel, cluster, grid, S::kThreads, S::kSmem, st, map_a, map_b, a);
 }
 
+// The tensor cores cut the digits that do not fit their running sum, which drifts towards zero by 0.0154 half-units in the last place a term; fp32 outputs are taken
+// out of them after every so many stages of k and added up in registers.  A 32-bit sum term after term is off by 0.3 sqrt(K) of those, a library's product, which has
+// several sums, by 0.12 to 0.18 sqrt(K).  An output gets the second, 8 sqrt(K) terms at a time (0.12); a gradient, which is the time of a training step, the first,
+// 16 sqrt(K) terms (0.25), since taking sums out stands in the products' way in TMEM: by 8 sqrt(K), 16 sqrt(K) and 768 terms dW of 4096 x 4096 x 2048 88, 76, 76 us,
+// of 2000 x 5500 x 3001 84, 78, 78; y of 1024 x 4096 x 4096 64 us by 8 sqrt(K), 53 by 768 terms, its error 2.3e-7 and 6.4e-7, a library's in fp32 2.5e-7.
+// At most 12 stages (dW of 4096 x 4096 x 8192 246, 239, 236 us at 8, 12, 16).
+static int sums_chunk(int K, int terms_a_root) { return std::max(1, std::min(12, (int)std::lround(std::sqrt((double)K) * terms_a_root / kTileK))); }
+
 // Columns a tile (0: by a pair of CTAs) and CTAs that share the k of one, by what they take in nanoseconds, measured with one tile an SM: a stage of k 325 whatever the
 // columns (a CTA's 24 to 32 KB come at about 50 bytes a clock; both products of a gated block 505), by a pair 410; to start and to store 3700 and some for
 // each column, by a pair 7000; to join sums in a cluster 1500 and more for columns and CTAs.  A cluster has one tile, so that there are no more of them than
@@ -1019,6 +1025,7 @@ template <int KIND, typename T> static int dense_product(const Operand &A, const
     for (int i = 0; i < 4; ++i) clusters[i] = resident_clusters(reinterpret_cast<const void *>(kernel), 1 << i, S::kThreads, S::kSmem);
     const DenseTiles t = choose_dense_tiles(a.M, a.N, a.K, KIND == kGated ? 2 : 1, clusters);
     a.splits = t.splits;
+    a.chunk = sums_chunk(a.K, KIND == kWeightGrad ? 16 : 8);
     switch (t.columns) {
     case 32: return dense_tiles<KIND, T, 32, false>(A, B, a, st);
     case 64: return dense_tiles<KIND, T, 64, false>(A, B, a, st);
@@ -1033,6 +1040,7 @@ template <int KIND, typename T> static int dense_few(const __nv_bfloat16 *x, con
     int groups = 1;
     while (groups < kFewThreads / 32 && rows > 16 * groups) groups *= 2;
     const int chunk = std::min(few_chunk(a.N), (a.K + 31) / 32 * 32), smem = (a.N * (chunk + 8) + 8) * 2;
+    a.chunk = sums_chunk(a.K, 8);
     auto kernel = k_dense_few<KIND, T>;
     BB200_REQUIRE(allow_big_smem(kernel, (kFewInputs + 9 * 8) * 2), (int)cudaErrorInvalidValue);
     launch(kernel, (unsigned)ctas, kFewThreads, (size_t)smem, st, x, W, xs, ws, a, groups, chunk);

@@ -223,3 +223,17 @@ def error_of_product(K, O, F):
 def test_sums_of_few_frames_keep_their_digits(K, O, F):
     error, in_order = error_of_product(K, O, F)
     assert error <= in_order
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,O,F", [(64, 512, 512), (200, 300, 1000), (512, 512, 512), (700, 2048, 2000), (768, 2048, 2048), (768, 4000, 16), (1020, 1000, 200), (1500, 2500, 2500), (8192, 512, 2048)])
+def test_sums_of_frames_keep_their_digits(K, O, F):
+    from binarybrain_b200 import ops
+    error, in_order = error_of_product(K, O, F)
+    assert error <= in_order
+    frames = (K + 15) // 16 * 16                                          # the weights' gradient: a sum over K frames
+    g = torch.Generator(device="cuda").manual_seed(K)
+    dy, x = (torch.randn((rows, frames), device="cuda", generator=g).to(BF16) for rows in (O, F))
+    dW, _ = ops.dense_backward_weights(x, dy, K)
+    want = dy[:, :K].double() @ x[:, :K].double().t()
+    assert float((dW.double() - want).norm() / want.norm()) <= in_order
