@@ -440,7 +440,8 @@ int bbcu_bf16_LossDistillation(const bbcu_bf16_t *dev_z_buf, bbcu_bf16_t *dev_dz
  * No counterparts in the reference.  The rules of the section above hold; each output is rounded once, from 32 bits.  The products' operands are read by
  * TMA: rows of W, x and dy start on 16-byte boundaries (strides in elements, multiples of 8; BBCU_ERR_BAD_STRIDE otherwise), what lies in their padding is
  * not used.  The other buffers may have any stride and alignment; y may be the residual itself, and dx the z that it is the gradient of (the same rows at the same
- * stride); other outputs have no element of an input or of one another.  Extents up to 2^27, BBCU_ERR_TOO_LARGE beyond. */
+ * stride); other outputs have no element of an input or of one another.  Extents up to 2^27, sums for bf16 outputs (the inputs forward, the outputs backward) up to 2^20
+ * terms; BBCU_ERR_TOO_LARGE beyond. */
 #define BBCU_ACTIVATION_NONE 0
 #define BBCU_ACTIVATION_RELU 1
 #define BBCU_ACTIVATION_GELU 2          /* z * (1 + erf(z / sqrt 2)) / 2 */

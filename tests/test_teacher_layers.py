@@ -202,6 +202,29 @@ def test_norms_in_the_place_of_what_they_are_made_of(N, F, layout, dtype):
         assert got[0] is given[over] and torch.equal(got[0][:, :F], ds[:, :F]) and torch.equal(got[1], dgamma), over
 
 
+def test_sums_that_are_too_long_for_16_bits_are_refused():
+    """More than 2^20 terms of a bf16 output, before anything runs (the addresses are never read); fp32 outputs and gradients, whose sums are taken out, have no such limit."""
+    import os
+    from binarybrain_b200 import abi
+    if not os.path.exists(abi.LIB_PATH):
+        pytest.skip("library not built")
+    from binarybrain_b200 import _native as native
+    a, most = 1 << 20, 1 << 20
+    n = most + 8
+
+    def status(name, *args):
+        with pytest.raises(abi.BbcuError) as e:
+            getattr(native, name)(*args, 0)
+        return e.value.status
+    large, null = -6, -1
+    for k, want in ((most, null), (n, large)):                            # (without y: what is not too large goes as far as that)
+        assert status("bbcu_bf16_DenseAffine_Forward", a, a, None, None, None, None, 0, k, 8, 8, k, 8, 0, 8, 0) == want
+        assert status("bbcu_bf16_GatedDense_Forward", a, a, None, None, None, 3, k, 8, 8, k, 8, 8, 0) == want
+        assert status("bbcu_bf16_DenseAffine_BackwardInput", a, a, None, None, 0, 0, 8, k, 8, 8, 8, 0, 8) == want
+    assert status("bbcu_bf16_fp32_DenseAffine_Forward", a, a, None, None, None, None, 0, n, 8, 8, n, 8, 0, 8, 0) == null
+    assert status("bbcu_bf16_DenseAffine_BackwardWeights", None, None, a, a, 0, 8, 8, n, n, n, 8) == null
+
+
 # ------------------------------------------------------------------------------------------------------------------------ sums of 32 bits
 U = 2.0 ** -24
 
@@ -237,3 +260,16 @@ def test_sums_of_frames_keep_their_digits(K, O, F):
     dW, _ = ops.dense_backward_weights(x, dy, K)
     want = dy[:, :K].double() @ x[:, :K].double().t()
     assert float((dW.double() - want).norm() / want.norm()) <= in_order
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("F", [128, 8])
+def test_the_longest_sum_of_a_16_bit_output(F):
+    """2^20 terms that are all positive: what is cut is less than a tenth of the rounding to bf16, so that its error is that rounding, up to 2^-8 of the value, and a tenth."""
+    from binarybrain_b200 import ops
+    K, O = 1 << 20, 128
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x, W = (torch.rand(shape, device="cuda", generator=g).to(BF16) for shape in ((K, 128), (O, K)))
+    y = ops.dense_forward(x, W, F)[:, :F].double()
+    want = W.double() @ x[:, :F].double()
+    assert float(((y - want).abs() / want).max()) <= 1.1 * 2.0 ** -8
