@@ -8,6 +8,13 @@ import torch
 from . import ops
 
 
+def _kept(layer):
+    """What the last forward pass of a layer left for its backward pass."""
+    if layer._saved is None:
+        raise RuntimeError(f"{type(layer).__name__}: nothing is kept, the last pass was not one for training or has had its backward pass")
+    return layer._saved
+
+
 class LayerNormalization:
     """Layer norm over the nodes of a frame with a learned scale and offset a node; a batch that is sharded over frames needs no exchange but that of
     dgamma and dbeta, which backward() adds to."""
@@ -59,9 +66,9 @@ class RmsNormalization:
     def parameters(self):
         return [(self.gamma, self.dgamma)]
 
-    def forward(self, x, frames, total_frames=None, residual=None, y=None):
+    def forward(self, x, frames, total_frames=None, residual=None, y=None, train=True):
         y, s, rstd = ops.rms_norm_forward(x, frames, gamma=self.gamma, eps=self.eps, residual=residual, y=y)
-        self._saved = s, rstd, frames
+        self._saved = (s, rstd, frames) if train else None
         return y, s
 
     def forward_int8(self, x, frames, residual=None):
@@ -69,7 +76,7 @@ class RmsNormalization:
         return ops.rms_norm_int8(x, frames, gamma=self.gamma, eps=self.eps, residual=residual)
 
     def backward(self, dy, ds=None, out=None):
-        s, rstd, frames = self._saved
+        s, rstd, frames = _kept(self)
         self._saved = None
         return ops.rms_norm_backward(s, dy, rstd, frames, gamma=self.gamma, dresidual=ds, ds=out, dgamma=self.dgamma)[0]
 
@@ -105,11 +112,11 @@ class DenseAffine:
     def backward(self, dy, dx=None, below=None, of_z=False):
         """dy: the gradient of y, or, for a layer with an activation, of z: what the layer above returns when this one is its `below`, or, with of_z=True, the caller's
         own.  below: the layer whose output x is; where that has an activation or is gated, the gradient of its z is returned."""
+        x, _, frames = _kept(self)
         if self.activation not in (None, "none") and not (self.gated or self._z_given or of_z):
             raise ValueError("dy: the gradient of y, where a layer with an activation takes that of z (give this layer to the one above as its `below`)")
-        x, _, frames = self._saved
-        ops.dense_backward_weights(x, dy, frames, dW=self.dW, dbias=self.dbias)
         z, activation, gated = below.kept() if below is not None else (None, None, False)
+        ops.dense_backward_weights(x, dy, frames, dW=self.dW, dbias=self.dbias)
         dx = ops.dense_backward_input(dy, self.W16, frames, z=z, activation=activation, gated=gated, dx=dx)
         self._saved = None
         return dx
@@ -118,8 +125,9 @@ class DenseAffine:
         """For the layer above, which returns the gradient of z."""
         if self._beside:
             raise ValueError("below: a layer with a residual beside its activation, whose gradient would be lost")
+        z = _kept(self)[1]
         self._z_given = True
-        return self._saved[1], self.activation, self.gated
+        return z, self.activation, self.gated
 
 
 class GatedDense(DenseAffine):
@@ -158,7 +166,7 @@ class FeedForward:
         self.dense.refresh()
 
     def forward(self, x, frames, residual=None, train=True):
-        n, s = self.norm.forward(x, frames, residual=residual)
+        n, s = self.norm.forward(x, frames, residual=residual, train=train)
         return self.dense.forward(self.gated.forward(n, frames, train=train), frames, train=train), s
 
     def backward(self, dy, ds=None):

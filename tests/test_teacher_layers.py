@@ -92,6 +92,33 @@ def test_a_residual_beside_an_activation_is_for_serving(shapes_only):
     lower.backward(upper.backward(x, below=lower))
 
 
+def test_a_pass_that_is_not_for_training_keeps_nothing(shapes_only):
+    from binarybrain_b200.teacher import DenseAffine, FeedForward, GatedDense, RmsNormalization
+    x = torch.zeros((8, 16), dtype=BF16)
+    norm, block = RmsNormalization(8, device="cpu"), FeedForward(8, 12, device="cpu")
+    for layer, passes in ((norm, lambda train: norm.forward(x, 16, train=train)), (block, lambda train: block.forward(x, 16, residual=x, train=train))):
+        with pytest.raises(RuntimeError, match="nothing is kept"):
+            layer.backward(x)
+        passes(True)
+        assert layer.backward(x, x).shape == (8, 16)
+        with pytest.raises(RuntimeError, match="nothing is kept"):        # it has been used up
+            layer.backward(x)
+        passes(True)
+        passes(False)                                                     # an evaluation between a training pass and its backward pass
+        del shapes_only[:]
+        with pytest.raises(RuntimeError, match="nothing is kept"):
+            layer.backward(x)
+        assert not shapes_only
+    assert all(layer._saved is None for layer in (norm, block.norm, block.gated, block.dense))
+    lower, gate, upper = DenseAffine(torch.zeros(12, 8), activation="relu"), GatedDense(torch.zeros(24, 8)), DenseAffine(torch.zeros(8, 12))
+    for below in (lower, gate):
+        upper.forward(below.forward(x, 16, train=False), 16)
+        del shapes_only[:]
+        with pytest.raises(RuntimeError, match="nothing is kept"):
+            upper.backward(x, below=below)
+        assert not shapes_only                                            # no gradient has been added to
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("activation", ["relu", "gelu", "silu"])
 @pytest.mark.parametrize("K,H,O,F", [(64, 100, 40, 33), (300, 513, 260, 500)])
