@@ -32,6 +32,9 @@ __device__ __forceinline__ double block_total(double v, double *smem)      // in
 // threads, 200 tensors of 1000 took 250 us, now 8.  Pieces of 4096: 6 x 65536 x 64 130 us, of 8192 126; four small tensors then 7.8 and 9.5; numbered
 // by all warps, in one size after the other, and their sizes asked for behind the norm, those took 7.6, now 6.2.)
 constexpr int kPieceSize = 8192, kSmallPiece = 2048;
+__host__ __device__ constexpr int pieces_of(int size, int piece) { return size > 0 ? (size - 1) / piece + 1 : 0; }
+static_assert(pieces_of(0x7fffffff, kPieceSize) == 1 << 18 && pieces_of(0x7fffffff, kSmallPiece) == 1 << 20 && pieces_of(kPieceSize, kPieceSize) == 1 &&
+              pieces_of(kPieceSize + 1, kPieceSize) == 2 && pieces_of(0, kPieceSize) == 0, "pieces of the largest and the smallest tensors");
 // start[t + 1] = the pieces of the tensors up to t.  Only the warps that have a tensor number theirs.
 __device__ __forceinline__ void number_pieces(int count, int size, int *start, int2 *warp_sum, int &piece)
 {
@@ -41,7 +44,7 @@ __device__ __forceinline__ void number_pieces(int count, int size, int *start, i
     int2 n;                                                               // by either size of pieces
     __syncthreads();                                                      // the numbers before are done with
     if (warp < warps) {
-        n = make_int2((int)((unsigned)(size + kPieceSize - 1) / kPieceSize), (int)((unsigned)(size + kSmallPiece - 1) / kSmallPiece));
+        n = make_int2(pieces_of(size, kPieceSize), pieces_of(size, kSmallPiece));
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int2 before = make_int2(__shfl_up_sync(0xffffffffu, n.x, d), both ? __shfl_up_sync(0xffffffffu, n.y, d) : 0);

@@ -300,3 +300,30 @@ def test_the_longest_sum_of_a_16_bit_output(F):
     y = ops.dense_forward(x, W, F)[:, :F].double()
     want = W.double() @ x[:, :F].double()
     assert float(((y - want).abs() / want).max()) <= 1.1 * 2.0 ** -8
+
+
+# ------------------------------------------------------------------------------------------------------------------------ clipping
+def test_pieces_of_the_largest_tensors_are_counted_without_overflow():
+    """The count of a tensor's pieces is checked when the source is compiled, where an overflow is an error: for 2^31 - 1 elements, and by the kernels' own function."""
+    import re
+    from pathlib import Path
+    source = (Path(__file__).parent.parent / "binarybrain_b200" / "csrc" / "gradient_norm.cu").read_text()
+    assert re.search(r"static_assert\(pieces_of\(0x7fffffff, kPieceSize\)", source)
+    assert not re.search(r"size \+ k(PieceSize|SmallPiece)", source)
+
+
+@pytest.mark.gpu
+def test_clipping_of_the_largest_tensor():
+    """2^31 - 1 elements, 8 GB, in which ones lie in the first and the last pieces: the norm, the factor at both ends, and nothing else."""
+    from binarybrain_b200 import ops
+    n = (1 << 31) - 1
+    big, small = torch.zeros(n, device="cuda"), torch.full((5,), 2.0, device="cuda")
+    ones = [0, 8191, 8192, n - 8192, n - 8191, n - 2, n - 1]
+    big[torch.tensor(ones, device="cuda")] = 1.0
+    clip = ops.GradientNorm([small, big])
+    want = math.sqrt(len(ones) + 20)
+    assert abs(float(clip.norm()) - want) <= 2 * U * want
+    clip.clip_(1.0)
+    at = torch.nonzero(big).flatten().tolist()
+    assert at == ones and all(abs(float(big[i]) - 1 / want) <= 4 * U / want for i in ones) and float((small - 2 / want).abs().max()) <= 8 * U / want
+    assert abs(float(clip.norm()) - 1) <= 8 * U
