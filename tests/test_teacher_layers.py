@@ -302,6 +302,83 @@ def test_the_longest_sum_of_a_16_bit_output(F):
     assert float(((y - want).abs() / want).max()) <= 1.1 * 2.0 ** -8
 
 
+# ------------------------------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+@pytest.mark.gpu
+def test_norms_of_more_than_2_31_elements():
+    """The last rows and columns of every output against 64 bits, of numbers that depend on their place: s and dy have nothing to do with one another, so that rows read
+    from a wrong place show.  (Six buffers of 4.8 GB.)  Bounds: two roundings to bf16 of values of order 1, 2^-7 relative and absolute; dgamma a sum of 60000
+    products in 32 bits in some 500 partial sums, 300 half-units of their magnitudes."""
+    from binarybrain_b200 import ops
+    N, F, eps = 40000, 60000, 1e-5
+    g = torch.Generator(device="cuda").manual_seed(11)
+
+    def frames():
+        t = torch.empty((N, F), dtype=BF16, device="cuda")
+        for at in range(0, N, 4096):
+            t[at:at + 4096] = torch.randn((min(4096, N - at), F), device="cuda", generator=g)
+        return t
+    R, C = slice(-70, None), slice(-300, None)
+
+    def near(got, want):
+        assert float(((got.double() - want).abs() - 2.0 ** -7 * (1 + want.abs())).max()) <= 0
+    x, r, gamma = frames(), frames(), 1 + 0.2 * torch.randn(N, device="cuda", generator=g)
+    nowhere = lambda: torch.full((N, F), 77.0, dtype=BF16, device="cuda")  # noqa: E731
+    y, s, rstd = ops.rms_norm_forward(x, F, gamma=gamma, residual=r, y=nowhere())
+    s64 = (x[:, C] + r[:, C]).double()                                    # rounded once, as it is kept
+    assert torch.equal(s[:, C].double(), s64)
+    want = 1 / torch.sqrt((s64 * s64).mean(0) + eps)
+    assert float(((rstd[C].double() - want).abs() / want).max()) <= (N / 512 + 24) * U
+    near(y[R, C], s64[R] * want * gamma[R, None].double())
+    del y
+    q, scale, kept = ops.rms_norm_int8(x, F, gamma=gamma, residual=r)
+    t = s[:, C].float() * gamma[:, None]
+    unit = t.abs().amax(0) / torch.full((300,), 127.0, device="cuda")
+    assert torch.equal(kept[R, C], s[R, C]) and torch.equal(q[C, R], torch.round(t[R] / unit).clamp(-127, 127).to(torch.int8).t())
+    del q, kept, x, t
+    dy = frames()
+    ds, dgamma = ops.rms_norm_backward(s, dy, rstd, F, gamma=gamma, dresidual=r, ds=nowhere())
+    xh, gd = s64 * rstd[C].double(), dy[:, C].double() * gamma[:, None].double()
+    near(ds[R, C], (rstd[C].double() * (gd - xh * (gd * xh).mean(0)))[R] + r[R, C].double())
+    terms = dy[R].double() * s[R].double() * rstd.double()
+    assert float(((dgamma[R].double() - terms.sum(1)).abs() - 300 * U * terms.abs().sum(1)).max()) <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("F", [4, 7, 200])
+def test_rows_far_apart(F):
+    """Rows of one buffer of 2^31 elements and more, 480000 elements apart, side by side in it: the bits of the same calls on buffers of their own.  (What takes one launch, or a few
+    frames, has no such offsets otherwise.)"""
+    from binarybrain_b200 import ops
+    N, O, step, width = 4800, 4800, 480000, 208
+    wide = torch.empty((N, step), dtype=BF16, device="cuda")
+    column = iter(range(step - 12 * width, step, width))
+    far = lambda t=None: (lambda v: v if t is None else v.copy_(t))(wide[:, (c := next(column)):c + width])  # noqa: E731
+    x, r, dy, dr = (torch.zeros((N, width), dtype=BF16, device="cuda") for _ in range(4))
+    for i, t in enumerate((x, r, dy, dr)):
+        t[:, :F] = normal(60 + i, N, F).to(BF16).cuda()
+    gamma = (1 + 0.2 * normal(64, N)).float().cuda()
+    new = lambda: torch.empty((N, width), dtype=BF16, device="cuda")  # noqa: E731
+    y, s, rstd = ops.rms_norm_forward(x, F, gamma=gamma, residual=r, y=new(), s=new())
+    ds, dgamma = ops.rms_norm_backward(s, dy, rstd, F, gamma=gamma, dresidual=dr, ds=new())
+    xf, sf = far(x), far()
+    got = ops.rms_norm_forward(xf, F, gamma=gamma, residual=far(r), y=far(), s=sf)
+    assert torch.equal(got[0][:, :F], y[:, :F]) and torch.equal(got[1][:, :F], s[:, :F]) and torch.equal(got[2], rstd)
+    q, scale, _ = ops.rms_norm_int8(x, F, gamma=gamma, residual=r)
+    got = ops.rms_norm_int8(xf, F, gamma=gamma, residual=far(r))
+    assert torch.equal(got[0], q) and torch.equal(got[1], scale)
+    dyf = far(dy)
+    got = ops.rms_norm_backward(sf, dyf, rstd, F, gamma=gamma, dresidual=far(dr), ds=far())
+    assert torch.equal(got[0][:, :F], ds[:, :F]) and torch.equal(got[1], dgamma)
+    W = ops.dense_weights((normal(65, O, N) / math.sqrt(N)).cuda())
+    yd, z = ops.dense_forward(x, W, F, activation="gelu", residual=r, y=new(), keep=new())
+    got = ops.dense_forward(xf, W, F, activation="gelu", residual=far(r), y=far(), keep=far())
+    assert torch.equal(got[0][:, :F], yd[:, :F]) and torch.equal(got[1][:, :F], z[:, :F])
+    dx = ops.dense_backward_input(dy, W, F, z=r, activation="gelu", dx=new())
+    rf = far(r)
+    assert torch.equal(ops.dense_backward_input(dyf, W, F, z=rf, activation="gelu", dx=rf)[:, :F], dx[:, :F])
+    assert all(torch.equal(a, b) for a, b in zip(ops.dense_backward_weights(xf, dyf, F), ops.dense_backward_weights(x, dy, F)))
+
+
 # ------------------------------------------------------------------------------------------------------------------------ clipping
 def test_pieces_of_the_largest_tensors_are_counted_without_overflow():
     """The count of a tensor's pieces is checked when the source is compiled, where an overflow is an error: for 2^31 - 1 elements, and by the kernels' own function."""
