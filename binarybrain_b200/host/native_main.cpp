@@ -473,6 +473,14 @@ struct Numbers {
     PyObject *result() const { return given ? Py_NewRef(given) : THPVariable_Wrap(made); }
 };
 
+// the memory of numbers that were given
+Rows rows_of(const Numbers &numbers, int64_t size)
+{
+    Rows r;
+    if (numbers.given) { r.at = reinterpret_cast<uintptr_t>(numbers.data); r.rows = 1; r.width = 4 * size; }
+    return r;
+}
+
 // rows of 8-bit integers
 const at::Tensor *int8_rows(PyObject *o, const char *name, Place &place)
 {
@@ -634,6 +642,8 @@ PyObject *rms_norm_forward_body(PyObject *const *o)
         !y.output(o[5], "y", frames, x.t->scalar_type(), *x.t, nodes) || !rstd.output(o[7], "rstd", frames, *x.t)) return nullptr;
     if (o[4] == Py_None && o[6] != Py_None) { refuse("s", "given without a residual"); return nullptr; }
     if (!apart("y", y, {s.t ? s : x}) || !apart_or_same("y", y, {x, residual}) || !apart_or_same("s", s, {x, residual})) return nullptr;      // (no residual: x is s)
+    const Rows of_gamma = rows_of(gamma, nodes);
+    if (!apart("rstd", rows_of(rstd, frames), {x, residual, s, y, of_gamma}) || !apart("y", y, {of_gamma}) || !apart("s", s, {of_gamma})) return nullptr;
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_RmsNormalization_Forward, bbcu_bf16_RmsNormalization_Forward, float, bbcu_bf16_t, x.in<const T *>(),
                            residual.t ? residual.in<const T *>() : nullptr, s.t ? s.out<T *>() : nullptr, y.out<T *>(), gamma.data, rstd.data, eps, nodes, frames, x.stride,
                            residual.stride, s.stride, y.stride, stream)) return nullptr;
@@ -654,7 +664,7 @@ PyObject *rms_norm_int8_body(PyObject *const *o)
         (o[4] != Py_None && (!residual.take(o[4], "residual", frames, x.t, nodes) || !s.output(o[5], "s", frames, x.t->scalar_type(), *x.t, nodes))) ||
         !scale.output(Py_None, "scale", frames, *x.t)) return nullptr;
     if (o[4] == Py_None && o[5] != Py_None) { refuse("s", "given without a residual"); return nullptr; }
-    if (!apart_or_same("s", s, {x, residual})) return nullptr;
+    if (!apart_or_same("s", s, {x, residual}) || !apart("s", s, {rows_of(gamma, nodes)})) return nullptr;
     const int row = (int)std::min<int64_t>(((int64_t)nodes + 15) / 16 * 16, INT_MAX / 16 * 16);
     at::Tensor q = at::empty({frames, row}, at::TensorOptions().dtype(at::kChar).device(x.t->device()));
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(x.fp32(), bbcu_fp32_RmsNormalization_QuantizeInt8, bbcu_bf16_RmsNormalization_QuantizeInt8, float, bbcu_bf16_t,
@@ -675,7 +685,9 @@ PyObject *rms_norm_backward_body(PyObject *const *o)
     if (!parse(o[3], frames) || !s.take(o[0], "s", frames, nullptr, -1) || !fits(s.t->size(0), nodes) || !dy.take(o[1], "dy", frames, s.t, nodes) ||
         !gamma.input(o[4], "gamma", nodes) || !rstd.check(o[2], "rstd", frames, false) || (o[5] != Py_None && !dresidual.take(o[5], "dresidual", frames, s.t, nodes)) ||
         !dgamma.output(o[7], "dgamma", nodes, *s.t) || !ds.output(o[6], "ds", frames, s.t->scalar_type(), *s.t, nodes)) return nullptr;
-    if (!apart_or_same("ds", ds, {s, dy, dresidual})) return nullptr;
+    const Rows of_gamma = rows_of(gamma, nodes), of_rstd = rows_of(rstd, frames);
+    if (!apart_or_same("ds", ds, {s, dy, dresidual}) || !apart("ds", ds, {of_gamma, of_rstd}) || !apart("dgamma", rows_of(dgamma, nodes), {s, dy, dresidual, ds, of_gamma, of_rstd}))
+        return nullptr;
     const int accumulate = o[7] != Py_None;
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(s.fp32(), bbcu_fp32_RmsNormalization_Backward, bbcu_bf16_RmsNormalization_Backward, float, bbcu_bf16_t, s.in<const T *>(),
                            dy.in<const T *>(), dresidual.t ? dresidual.in<const T *>() : nullptr, ds.out<T *>(), gamma.data, rstd.data, dgamma.data, accumulate, nodes,
@@ -730,7 +742,8 @@ PyObject *dense_forward_body(PyObject *const *o)
         (o[6] != Py_None ? !y.take(o[6], "y", frames, nullptr, nodes) : !y.output(Py_None, "y", frames, bf16 ? at::kBFloat16 : at::kFloat, *x.t, nodes)) ||
         (o[5] != Py_None && !residual.take(o[5], "residual", frames, y.t, nodes)) || !kept(z, o[8], frames, *x.t, nodes)) return nullptr;
     const Rows of_w = rows_of_weights(*W, w_stride);
-    if (!apart("y", y, {x, of_w}) || !apart_or_same("y", y, {residual}) || !apart("z", z, {x, y, residual, of_w})) return nullptr;
+    const Rows of_bias = rows_of(bias, nodes);
+    if (!apart("y", y, {x, of_w, of_bias}) || !apart_or_same("y", y, {residual}) || !apart("z", z, {x, y, residual, of_w, of_bias})) return nullptr;
     const auto *in = static_cast<const bbcu_bf16_t *>(x.t->const_data_ptr()), *w = static_cast<const bbcu_bf16_t *>(W->const_data_ptr());
     auto *zp = z.t ? z.out<bbcu_bf16_t *>() : nullptr;
     if (!place.stream(stream) || BB200_CALL_OF_TYPE(y.fp32(), bbcu_bf16_fp32_DenseAffine_Forward, bbcu_bf16_DenseAffine_Forward, float, bbcu_bf16_t, in, w, bias.data,
@@ -767,7 +780,8 @@ PyObject *gated_dense_forward_body(PyObject *const *o)
     if (!bf16_operand(x, o[0], "x", frames, inputs) || !bias.input(o[3], "bias", rows) || !y.output(o[5], "y", frames, at::kBFloat16, *x.t, rows / 2) ||
         !kept(z, o[6], frames, *x.t, rows)) return nullptr;
     const Rows of_w = rows_of_weights(*W, w_stride);
-    if (!apart("y", y, {x, of_w}) || !apart("z", z, {x, y, of_w})) return nullptr;
+    const Rows of_bias = rows_of(bias, rows);
+    if (!apart("y", y, {x, of_w, of_bias}) || !apart("z", z, {x, y, of_w, of_bias})) return nullptr;
     if (!place.stream(stream) || BB200_CALL(bbcu_bf16_GatedDense_Forward, x.in<const bbcu_bf16_t *>(), static_cast<const bbcu_bf16_t *>(W->const_data_ptr()), bias.data,
                            y.out<bbcu_bf16_t *>(), z.t ? z.out<bbcu_bf16_t *>() : nullptr, act, inputs, rows / 2, frames, w_stride, x.stride, y.stride, z.stride,
                            stream)) return nullptr;
@@ -811,6 +825,8 @@ PyObject *dense_backward_weights_body(PyObject *const *o)
         if (!dW.check(o[3], "dW", (int64_t)nodes * inputs, true) || (o[4] != Py_None && !dbias.check(o[4], "dbias", nodes, true))) return nullptr;
         const at::Tensor &t = THPVariable_Unpack(o[3]);
         if (t.dim() != 2 || t.size(0) != nodes || t.size(1) != inputs) { refuse("dW", "expected [outputs, inputs]"); return nullptr; }
+        const Rows of_dw = rows_of(dW, (int64_t)nodes * inputs);
+        if (!apart("dW", of_dw, {x, dy}) || !apart("dbias", rows_of(dbias, nodes), {x, dy, of_dw})) return nullptr;
     } else {
         if (!place.here()) return nullptr;
         dW.made = at::empty({nodes, inputs}, at::TensorOptions().dtype(at::kFloat).device(x.t->device()));

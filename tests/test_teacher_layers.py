@@ -185,6 +185,33 @@ def test_outputs_that_reach_into_other_buffers_are_refused():
 
 
 @pytest.mark.gpu
+def test_sums_and_numbers_that_lie_in_other_buffers_are_refused():
+    from binarybrain_b200 import ops
+    flat = torch.zeros(8192, device="cuda")                               # 64 rows of 48 of bf16 are 1536 of these
+    x, y, dy, dr = (flat[1536 * i:1536 * (i + 1)].view(BF16).view(64, 48) for i in range(4))
+    numbers = lambda first, n=64: flat[first:first + n]  # noqa: E731
+    W, W2, rest, f = ops.dense_weights(torch.zeros(64, 64, device="cuda")), ops.dense_weights(torch.zeros(128, 64, device="cuda")), 1536 * 4, 48
+    weights = flat[:4096].view(64, 64)
+    far = torch.zeros((64, 48), dtype=BF16, device="cuda"), torch.zeros((64, 48), dtype=BF16, device="cuda")
+    calls = [lambda: ops.rms_norm_forward(x, f, y=y, rstd=numbers(1500)), lambda: ops.rms_norm_forward(x, f, y=y, rstd=numbers(1536)), lambda: ops.rms_norm_forward(x, f, y=y, gamma=numbers(3000)),
+             lambda: ops.rms_norm_forward(x, f, residual=y, s=dy, gamma=numbers(3100)), lambda: ops.rms_norm_forward(x, f, gamma=numbers(rest), rstd=numbers(rest + 63)),
+             lambda: ops.rms_norm_int8(x, f, residual=y, s=dy, gamma=numbers(3100)), lambda: ops.rms_norm_backward(x, dy, numbers(1536), f, ds=y),
+             lambda: ops.rms_norm_backward(x, dy, numbers(rest), f, gamma=numbers(1600), ds=y), lambda: ops.rms_norm_backward(x, dy, numbers(rest), f, dgamma=numbers(40)),
+             lambda: ops.rms_norm_backward(x, dy, numbers(rest), f, dresidual=dr, dgamma=numbers(5000)), lambda: ops.rms_norm_backward(x, dy, numbers(rest), f, dgamma=numbers(rest + 40)),
+             lambda: ops.rms_norm_backward(x, dy, numbers(rest), f, gamma=numbers(rest + 100), dgamma=numbers(rest + 100)),
+             lambda: ops.dense_forward(x, W, f, bias=numbers(1600), y=y), lambda: ops.dense_forward(x, W, f, bias=numbers(1600), y=dy, keep=y),
+             lambda: ops.gated_dense_forward(x, W2, f, bias=numbers(1600, 128), y=y), lambda: ops.dense_backward_weights(x, far[0], f, dW=weights),
+             lambda: ops.dense_backward_weights(far[0], dy, f, dW=weights), lambda: ops.dense_backward_weights(far[0], far[1], f, dW=weights, dbias=numbers(4095)),
+             lambda: ops.dense_backward_weights(dr, far[0], f, dW=weights[:, :0].new_zeros(64, 64), dbias=numbers(4608))]
+    for k, call in enumerate(calls):
+        with pytest.raises(ValueError, match="memory of its own"):
+            call()
+            pytest.fail(f"call {k}")
+    ops.dense_backward_weights(far[0], far[1], f, dW=weights, dbias=numbers(4096))
+    ops.rms_norm_backward(x, dy, numbers(rest), f, gamma=numbers(rest + 64), dgamma=numbers(rest + 128))
+
+
+@pytest.mark.gpu
 def test_buffers_side_by_side_in_the_same_rows_are_apart():
     from binarybrain_b200 import ops
     K, O, F = 96, 96, 40
