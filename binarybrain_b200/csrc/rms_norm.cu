@@ -12,7 +12,8 @@
 // Memory bounds it (16 bytes a value of fp32 forward with a residual, 16 backward).  A frame is needed whole before its first output.  Small calls take one launch: a
 // cluster of CTAs has the columns of 32 or 128 bytes of a row and goes over the rows twice, or once where they stay in registers; 16 bytes of a row or less are taken
 // frame by frame by lanes that hold their rows.  Large calls go along the rows
-// in two passes, which move a quarter more (a residual's sum is written by the first and read by the second), at 5.9 to 6.9 TB/s.
+// in two passes at 5.9 to 6.9 TB/s, which move a quarter more forward with a residual (its sum is written by the first and read by the second: five rows instead of
+// four), half more forward without one (three instead of two) and, with the second gradient, backward (six instead of four: s and dy are read twice).
 #include <algorithm>
 
 #include "frame_columns.cuh"

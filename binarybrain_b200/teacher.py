@@ -82,8 +82,8 @@ class RmsNormalization:
 
 
 class DenseAffine:
-    """A dense layer in bf16: y = activation(z) + residual, z = W x + bias.  The weights that are trained are fp32; refresh() lays them out in bf16 as the product
-    reads them, after they have changed.  backward() returns the gradient of x and adds to dW and dbias.  Without an activation it takes the gradient of y, which is
+    """A dense layer in bf16: y = activation(z) + residual, z = W x + bias.  The weights that are trained are fp32 (a contiguous fp32 W is taken as it is, and so is
+    the bias, not copied); refresh() lays them out in bf16 as the product reads them, after they have changed.  Gradients of frames are bf16, also where y is fp32.  backward() returns the gradient of x and adds to dW and dbias.  Without an activation it takes the gradient of y, which is
     the residual's as well.  With one it takes that of z, as the layer above returns it when this one is its `below`: what is made of y by anything else, a norm or a
     loss, has no way back through an activation here, and neither has the residual beside one."""
 
