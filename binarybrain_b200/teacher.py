@@ -83,9 +83,11 @@ class RmsNormalization:
 
 class DenseAffine:
     """A dense layer in bf16: y = activation(z) + residual, z = W x + bias.  The weights that are trained are fp32 (a contiguous fp32 W is taken as it is, and so is
-    the bias, not copied); refresh() lays them out in bf16 as the product reads them, after they have changed.  Gradients of frames are bf16, also where y is fp32.  backward() returns the gradient of x and adds to dW and dbias.  Without an activation it takes the gradient of y, which is
-    the residual's as well.  With one it takes that of z, as the layer above returns it when this one is its `below`: what is made of y by anything else, a norm or a
-    loss, has no way back through an activation here, and neither has the residual beside one."""
+    the bias, not copied); refresh() lays them out in bf16 as the product reads them, after they have changed.
+
+    backward() returns the gradient of x and adds to dW and dbias.  Without an activation it takes the gradient of y, which is the residual's as well.  With one it
+    takes that of z, as the layer above returns it when this one is its `below`: what is made of y by anything else, a norm or a loss, has no way back through an
+    activation here, and neither has the residual beside one.  Gradients of frames are bf16, also where y is fp32."""
 
     gated = False                                        # a gated block's z has twice the rows of its y, which tells the gradients apart
 
@@ -119,15 +121,15 @@ class DenseAffine:
         ops.dense_backward_weights(x, dy, frames, dW=self.dW, dbias=self.dbias)
         dx = ops.dense_backward_input(dy, self.W16, frames, z=z, activation=activation, gated=gated, dx=dx)
         self._saved = None
+        if below is not None:
+            below._z_given = True
         return dx
 
     def kept(self):
-        """For the layer above, which returns the gradient of z."""
+        """For the layer above, which makes the gradient of z."""
         if self._beside:
             raise ValueError("below: a layer with a residual beside its activation, whose gradient would be lost")
-        z = _kept(self)[1]
-        self._z_given = True
-        return z, self.activation, self.gated
+        return _kept(self)[1], self.activation, self.gated
 
 
 class GatedDense(DenseAffine):

@@ -81,6 +81,23 @@ def test_a_gradient_of_y_is_refused_where_that_of_z_is_needed(shapes_only):
     gate.backward(torch.zeros((24, 16), dtype=BF16))
 
 
+def test_a_refused_backward_pass_of_the_layer_above_gives_nothing(shapes_only, monkeypatch):
+    from binarybrain_b200 import teacher
+    lower, upper = teacher.DenseAffine(torch.zeros(12, 8), activation="relu"), teacher.DenseAffine(torch.zeros(8, 12))
+    x, dy = torch.zeros((8, 16), dtype=BF16), torch.zeros((12, 16), dtype=BF16)
+    upper.forward(lower.forward(x, 16), 16)
+
+    def refuses(*args, **kw):
+        raise ValueError("dx: expected another shape")
+    with monkeypatch.context() as m:
+        m.setattr(teacher.ops, "dense_backward_input", refuses)
+        with pytest.raises(ValueError, match="another shape"):
+            upper.backward(x, below=lower)
+    with pytest.raises(ValueError, match="gradient of y"):
+        lower.backward(dy)
+    lower.backward(upper.backward(x, below=lower))
+
+
 def test_a_residual_beside_an_activation_is_for_serving(shapes_only):
     from binarybrain_b200.teacher import DenseAffine
     x, r = torch.zeros((8, 16), dtype=BF16), torch.zeros((12, 16), dtype=BF16)
